@@ -51,7 +51,8 @@ typedef enum qkv_status {
   QKV_ERR_DEVICE = -5,      /* no usable gfx950 device / HIP runtime error             */
   QKV_ERR_LAUNCH = -6,      /* kernel launch failed                                    */
   QKV_ERR_WORKSPACE = -7,   /* workspace missing or smaller than the query says         */
-  QKV_ERR_TIMEOUT = -8      /* an in-kernel merge timed out; reset the workspace        */
+  QKV_ERR_TIMEOUT = -8,     /* an in-kernel merge timed out; reset the workspace        */
+  QKV_ERR_PAGES = -9        /* (device status of qkv_pages_reserve) no free page left   */
 } qkv_status;
 
 /* Library version (major*10000 + minor*100 + patch). */
@@ -493,6 +494,162 @@ int qkv_prefill_attn_tq3(const uint16_t* q, const qkv_block_tq3* k_cache,
                          const uint16_t* v_chunk, uint16_t* out, int num_q, int num_kv,
                          int head_dim, int start_pos, int n_tok, float scale, void* workspace,
                          size_t workspace_bytes, hipStream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * Rotary positions (RoPE).  No counterpart among the reference's compressed-KV
+ * launches: its attention path hands post-RoPE rows to the cache
+ * (model.cuh:2181-2306), and the inject of key planes applies RoPE between
+ * dequantization and append (model.cuh:3166-3233).
+ * Pair i of a head at position p turns by p * f_i, f_i = base^(-2i/rot_dim):
+ * (x, y) -> a (x cos - y sin, x sin + y cos).
+ * ------------------------------------------------------------------------- */
+
+/* Scaling of the frequencies for contexts `factor` times the trained one. */
+typedef enum qkv_rope_scaling {
+  QKV_ROPE_PLAIN = 0,
+  QKV_ROPE_LINEAR = 1, /* f / factor                                                     */
+  QKV_ROPE_NTK = 2,    /* base * factor^(rot_dim / (rot_dim - 2))                         */
+  QKV_ROPE_YARN = 3    /* by turns t = original_ctx * f / 2 pi: f for t >= beta_fast,
+                          f / factor for t <= beta_slow, linear in t between; amplitude
+                          a = 1 + 0.1 ln(factor)                                          */
+} qkv_rope_scaling;
+
+/* Fills the HOST array turns[rot_dim / 2] with the fraction of a full turn a
+ * position, 64-bit fixed point (position * turns mod 2^64 is the angle: exact at
+ * any distance), and *amplitude with a (1 but for YARN).  The caller copies
+ * turns to the device once.  rot_dim even (NTK: >= 4), base > 0, factor >= 1;
+ * factor, original_ctx and the betas are read where the scaling uses them. */
+int qkv_rope_table(int rot_dim, double base, int scaling, double factor, double original_ctx,
+                   double beta_fast, double beta_slow, uint64_t* turns, float* amplitude);
+
+/* Rotates n_tok tokens' query and key rows (fp16) in one launch.  Token t of q
+ * starts at q + t * q_stride (elements; heads head_dim apart), so views into a
+ * fused projection buffer work; k, and the outputs, likewise.  Out may be in
+ * (with its stride) or memory that does not overlap it.  num_q or num_k may be
+ * 0 (its pointers are not read).  positions: device int32 [n_tok], any sign.
+ * turns: device copy of qkv_rope_table's, rot_dim / 2 entries.  Elements from
+ * rot_dim on are copied.  layout 0: pairs (i, i + rot_dim / 2); 1: (2i, 2i + 1).
+ * inverse != 0 turns by the negative angle: it undoes the forward call up to
+ * amplitude^2, and is the gradient of the rows from that of the outputs.  fp32
+ * arithmetic, one rounding to fp16.  rot_dim even, <= head_dim <= 8192; at most
+ * 1024 heads each. */
+int qkv_rope(const uint16_t* q, long q_stride, uint16_t* q_out, long q_out_stride,
+             const uint16_t* k, long k_stride, uint16_t* k_out, long k_out_stride,
+             const int32_t* positions, const uint64_t* turns, float amplitude, int n_tok, int num_q,
+             int num_k, int head_dim, int rot_dim, int layout, int inverse, hipStream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * Paged 8-bit cache (F8).  No counterpart in the reference.
+ * A pool holds e4m3 codes [n_pages][block_tokens][num_kv][head_dim] (one byte
+ * an element, 16-byte aligned) and one exponent byte per page and kv head
+ * [n_pages][num_kv]: value = code * 2^(exp - 127).  block_tokens: a multiple of
+ * 16; head_dim 128 or 256.  Key p of slot s is row p % block_tokens of page
+ * block_tables[s * max_blocks + p / block_tokens].
+ * A batch is ragged: slot s owns rows starts[s] .. starts[s+1]-1 (device int32
+ * [n_slots + 1], not decreasing) of the row tensors, n_rows rows long, at
+ * positions positions[s], positions[s] + 1, .. (device int32 [n_slots]).  A slot
+ * may own none.  Rows past starts[n_slots] (a padded batch) are left alone; so
+ * are rows of a slot past its first max_tok, and slots with a negative position.
+ * ------------------------------------------------------------------------- */
+
+/* Appends the rows' K and V (fp16, element strides between tokens, heads
+ * head_dim apart, multiples of 8).  Per page and kv head the exponent is the
+ * smallest (>= 95) whose largest code, 448, holds the new rows' magnitudes, or
+ * the page's own if that is larger and the page has rows ahead of the new ones;
+ * those older rows are requantized when it rises (a power of two: only codes
+ * that become subnormal round).  Codes round to nearest even.  Magnitudes
+ * above 61440 are stored as 61440 and NaN as 0.  Rows whose table entry lies
+ * outside [0, n_pages) or past max_blocks are dropped.  No two slots of a call may
+ * write one page (qkv_pages_reserve makes pages a slot's own).
+ * With rot_dim > 0 (a multiple of 16) K is first rotated as by qkv_rope
+ * (rounded to fp16), and with num_q > 0 the query rows too, q -> q_out (in
+ * place or apart), all in the same launch; the result equals qkv_rope at those
+ * positions followed by this call without it. */
+int qkv_f8_append_kv_paged(const uint16_t* k, long k_stride, const uint16_t* v, long v_stride,
+                           uint8_t* k_pool, uint8_t* v_pool, uint8_t* k_exp, uint8_t* v_exp,
+                           int n_rows, int n_slots, int max_tok, int num_kv, int head_dim,
+                           const int32_t* block_tables, int max_blocks, int block_tokens,
+                           int n_pages, const int32_t* starts, const int32_t* positions,
+                           const uint16_t* q, long q_stride, uint16_t* q_out, long q_out_stride,
+                           int num_q, const uint64_t* turns, float amplitude, int rot_dim,
+                           int layout, hipStream_t stream);
+
+/* Attention of the rows' queries q [n_rows][num_q][head_dim] (fp16) over the
+ * pages: decode steps, verify blocks, prompt chunks and whole prompts, in any
+ * mix (max_tok the most rows of a slot).  The query at position p sees keys
+ * j <= p, j < max_ctx, of pages in [0, n_pages); with window_tok > 0 only those
+ * with j > p - window_tok or j < sink_tok.  So the pages of a slot that are out of
+ * its window may be given back (negative entries).  A query that sees no key gets
+ * a zero row.  out [n_rows][num_q][head_dim]; may be q.  num_q / num_kv 1..8.
+ * Values are read as fp16 (exact for exponents 95..135, which the append
+ * writes).  workspace: qkv_attn_f8_paged_workspace_bytes of the same numbers,
+ * 256-byte aligned, no initialisation; calls sharing one must be ordered. */
+size_t qkv_attn_f8_paged_workspace_bytes(int num_q, int num_kv, int head_dim, int n_slots,
+                                         int n_rows, int max_tok, int max_ctx);
+int qkv_attn_f8_paged(const uint16_t* q, const uint8_t* k_pool, const uint8_t* v_pool,
+                      const uint8_t* k_exp, const uint8_t* v_exp, uint16_t* out, int n_rows,
+                      int num_q, int num_kv, int head_dim, int n_slots, int max_tok, int max_ctx,
+                      const int32_t* block_tables, int max_blocks, int block_tokens, int n_pages,
+                      const int32_t* starts, const int32_t* positions, float scale, int window_tok,
+                      int sink_tok, void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * Pages of a cache, of any format.  No counterpart in the reference (its slots
+ * are contiguous).  The state is on the device, so that the calls can be captured
+ * into graphs: block_tables int32 [n_slots][max_blocks] (a negative entry: no
+ * page) and ref_counts int32 [n_pages], how many table entries name a page; a page
+ * is free at 0.  Page p of a plane is its bytes p * page_bytes ..; a plane is one
+ * pool of one layer (keys, values, exponents).  `planes` is a HOST array, read
+ * before the call returns, of at most 128; planes do not overlap.
+ * status (device int32 [n], may be NULL): per list entry QKV_OK,
+ * QKV_ERR_INVALID or QKV_ERR_PAGES; an entry that is not OK changes nothing.
+ * Lists are device int32; a slot may be named once a call.
+ * ------------------------------------------------------------------------- */
+typedef struct qkv_page_plane {
+  void* base;
+  size_t page_bytes;
+} qkv_page_plane;
+
+/* children[i] gets the pages of the first n_tokens[i] tokens of parents[i],
+ * shared.  A child has no pages beforehand, and is no parent of the call. */
+int qkv_pages_fork(int32_t* block_tables, int n_slots, int max_blocks, int block_tokens,
+                   int32_t* ref_counts, int n_pages, const int32_t* parents,
+                   const int32_t* children, const int32_t* n_tokens, int n, int32_t* status,
+                   hipStream_t stream);
+
+/* Gives back the pages of slots[i] past its first keep_tokens[i] tokens (0: all). */
+int qkv_pages_release(int32_t* block_tables, int n_slots, int max_blocks, int block_tokens,
+                      int32_t* ref_counts, int n_pages, const int32_t* slots,
+                      const int32_t* keep_tokens, int n, int32_t* status, hipStream_t stream);
+
+/* Readies slots[i] for writing tokens positions[i] .. + n_new[i]-1 (n_new <=
+ * max_new): missing pages are taken, and shared ones (count > 1 at the call)
+ * replaced by pages of its own; of those the first is copied, in every plane, if
+ * it holds rows ahead of positions[i].  Free pages are taken lowest index first,
+ * in list order; a slot that they do not suffice for, and those after it that
+ * want any, get QKV_ERR_PAGES.  n <= 1024.  scratch: device memory of
+ * qkv_pages_reserve_scratch_bytes; its first 2n int32 are afterwards the copied
+ * (from, to) pairs, -1 where none, for qkv_pages_copy of further planes. */
+size_t qkv_pages_reserve_scratch_bytes(int n, int max_new, int block_tokens);
+int qkv_pages_reserve(int32_t* block_tables, int n_slots, int max_blocks, int block_tokens,
+                      int32_t* ref_counts, int n_pages, const int32_t* slots,
+                      const int32_t* positions, const int32_t* n_new, int n, int max_new,
+                      int32_t* status, const qkv_page_plane* planes, int n_planes,
+                      int32_t* scratch, size_t scratch_bytes, hipStream_t stream);
+
+/* Copies page pairs[2i] to page pairs[2i+1] in every plane (device int32; a pair
+ * with an index outside [0, n_pages) is left out).  No page is the target of two
+ * pairs, or target and source. */
+int qkv_pages_copy(const qkv_page_plane* planes, int n_planes, int n_pages, const int32_t* pairs,
+                   int n, hipStream_t stream);
+
+/* Moves the pages in use to indices 0 .. *n_used - 1 (device int32): the i-th
+ * page in use at or past n_used goes to the i-th free one before it, in planes,
+ * tables and counts.  moved[p] (device int32 [n_pages]) is where page p is now, -1
+ * if it was free.  scratch: device, (n_pages + 2) * 4 bytes. */
+int qkv_pages_compact(int32_t* block_tables, int n_slots, int max_blocks, int32_t* ref_counts,
+                      int n_pages, int32_t* moved, int32_t* n_used, const qkv_page_plane* planes,
+                      int n_planes, int32_t* scratch, size_t scratch_bytes, hipStream_t stream);
 
 #ifdef __cplusplus
 }

@@ -21,7 +21,7 @@ QKV_OK = 0
 STATUS_NAMES = {
     0: "QKV_OK", -1: "QKV_ERR_INVALID", -2: "QKV_ERR_NULL", -3: "QKV_ERR_UNSUPPORTED",
     -4: "QKV_ERR_ALIGN", -5: "QKV_ERR_DEVICE", -6: "QKV_ERR_LAUNCH", -7: "QKV_ERR_WORKSPACE",
-    -8: "QKV_ERR_TIMEOUT",
+    -8: "QKV_ERR_TIMEOUT", -9: "QKV_ERR_PAGES",
 }
 
 
@@ -35,6 +35,8 @@ _P = ctypes.c_void_p
 _I = ctypes.c_int
 _F = ctypes.c_float
 _SZ = ctypes.c_size_t
+_L = ctypes.c_long
+_D = ctypes.c_double
 
 # name -> (restype, argtypes); must cover every function declared in include/qkv.h
 SIGNATURES = {
@@ -87,6 +89,19 @@ SIGNATURES = {
     "qkv_decode_noalloc_status_async": (_I, [_I, _P, _P]),
     "qkv_debug_set_merge_spin_limit": (_I, [_I]),
     "qkv_prefill_attn_tq3_workspace_bytes": (_SZ, [_I, _I, _I, _I]),
+    "qkv_rope_table": (_I, [_I, _D, _I, _D, _D, _D, _D, _P, _P]),
+    "qkv_rope": (_I, [_P, _L, _P, _L, _P, _L, _P, _L, _P, _P, _F, _I, _I, _I, _I, _I, _I, _I, _P]),
+    "qkv_f8_append_kv_paged": (_I, [_P, _L, _P, _L, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _I, _I, _I, _P,
+                                    _P, _P, _L, _P, _L, _I, _P, _F, _I, _I, _P]),
+    "qkv_attn_f8_paged_workspace_bytes": (_SZ, [_I, _I, _I, _I, _I, _I, _I]),
+    "qkv_attn_f8_paged": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _I, _I, _I, _P, _P, _F,
+                               _I, _I, _P, _SZ, _P]),
+    "qkv_pages_fork": (_I, [_P, _I, _I, _I, _P, _I, _P, _P, _P, _I, _P, _P]),
+    "qkv_pages_release": (_I, [_P, _I, _I, _I, _P, _I, _P, _P, _I, _P, _P]),
+    "qkv_pages_reserve_scratch_bytes": (_SZ, [_I, _I, _I]),
+    "qkv_pages_reserve": (_I, [_P, _I, _I, _I, _P, _I, _P, _P, _P, _I, _I, _P, _P, _I, _P, _SZ, _P]),
+    "qkv_pages_copy": (_I, [_P, _I, _I, _P, _I, _P]),
+    "qkv_pages_compact": (_I, [_P, _I, _I, _P, _I, _P, _P, _P, _I, _P, _SZ, _P]),
     "qkv_prefill_attn_tq3": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _F, _P, _SZ, _P]),
 }
 

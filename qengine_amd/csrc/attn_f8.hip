@@ -1,0 +1,875 @@
+// attn_f8.hip -- attention over the paged 8-bit cache (e4m3 codes, one power-of-two
+// exponent per page and KV head): ragged batches of one token to whole prompts a slot.
+//
+// Rows.  The rows of a (slot, KV head) are its (token, query head of the group) pairs,
+// row = token * gqa + head, so that a K/V tile read once serves the whole group.
+// Operands are swapped: S^T = K Q^T and O^T = V^T P^T, so that a lane's scores of a
+// row are exactly the key octet that it supplies as the second product's operand and
+// the softmax statistics of a row stay in its lanes.  Codes are converted to fp16 with
+// their exponent (exact: a stored value has 4 significant bits and lies in fp16's
+// range); both products run on the fp16 matrix cores with fp32 sums.
+//
+// Work.  The key tiles of all row tiles, heads and slots form one line that is cut
+// into equal parts, one per workgroup, so ragged lengths balance by themselves.  A
+// row tile that lies in one part is stored as output; one that is cut leaves records
+// (m, l, O) that the merge kernel joins.  A part has at most two cut ends, hence two
+// records a workgroup.
+#include <algorithm>
+
+#include "attn_common.h"
+#include "qkv_device.h"
+#include "qkv_launch.h"
+
+namespace qkv {
+
+namespace {
+
+typedef float f16x_t __attribute__((ext_vector_type(16)));
+typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
+
+// The weights are taken against a reference maximum that is raised only when a row's
+// maximum passes it by more than this (log2 units): they stay below 2^12, inside
+// fp16, and most tiles need no rescaling of the sums.
+constexpr float kSlack = 12.0f;
+
+__device__ __forceinline__ h2_t cvt2(uint32_t w, float scale, bool hi) {
+  return hi ? __builtin_bit_cast(h2_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, true))
+            : __builtin_bit_cast(h2_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, false));
+}
+__device__ __forceinline__ h8_t join8(h2_t a, h2_t b, h2_t c, h2_t d) {
+  return h8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+__device__ __forceinline__ float pow2f(uint32_t biased) { return __uint_as_float(biased << 23); }
+__device__ __forceinline__ float max32(float x) {   // with the lane 32 away
+  const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+}
+__device__ __forceinline__ float max16(float x) {   // with the lane 16 away
+  const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+}
+__device__ __forceinline__ float sum32(float x) {
+  const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(s[0]) + __uint_as_float(s[1]);
+}
+__device__ __forceinline__ float sum16(float x) {
+  const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(s[0]) + __uint_as_float(s[1]);
+}
+
+// A slot's tokens: rows t0 .. t0+n-1 of q at positions pos0 .. (n = 0: none)
+struct Slot {
+  int t0, n, pos0;
+};
+__device__ __forceinline__ Slot slot_of(const F8AttnArgs& p, int s) {
+  Slot x;
+  x.t0 = min(max(p.starts[s], 0), (int)p.rows);
+  x.n = min(min(max(p.starts[s + 1], x.t0), (int)p.rows) - x.t0, p.max_tok);
+  x.pos0 = p.positions[s];
+  if (x.pos0 < 0 || x.pos0 > (1 << 30)) x.n = 0;
+  return x;
+}
+
+// Row tile i of a slot, ROWS (token, head) rows each, over key tiles of KT keys: keys
+// lo .. end-1 and below the sinks.  Tile v of `tiles` is key tile v below n_sink, then w0 on.
+struct RowTile {
+  int tiles, n_sink, w0;
+  int end;              // keys that exist for the tile's last row
+  int pos_lo, pos_hi;   // positions of the first and last row's tokens
+  __device__ __forceinline__ int key0(int v, int kt) const { return (v < n_sink ? v : v - n_sink + w0) * kt; }
+};
+template <int ROWS, int KT>
+__device__ __forceinline__ RowTile row_tile(const F8AttnArgs& p, const Slot& x, int i, int gqa) {
+  RowTile r;
+  const int rows = x.n * gqa;
+  r.pos_lo = x.pos0 + i * ROWS / gqa;
+  r.pos_hi = x.pos0 + (min(rows, (i + 1) * ROWS) - 1) / gqa;
+  r.end = min(r.pos_hi + 1, p.max_ctx);
+  r.w0 = p.window > 0 ? max(0, r.pos_lo - p.window + 1) / KT : 0;
+  r.n_sink = p.window > 0 ? min((p.sink + KT - 1) / KT, r.w0) : 0;
+  r.tiles = max(1, r.n_sink + (r.end + KT - 1) / KT - r.w0);   // (a tile past every key is masked)
+  return r;
+}
+
+// Key units (PER tiles each) of entry x = slot * slot_tiles + row tile
+template <int ROWS, int KT, int PER>
+__device__ __forceinline__ int entry_units(const F8AttnArgs& p, int x, int gqa) {
+  const int s = x / p.slot_tiles, i = x - s * p.slot_tiles;
+  const Slot sl = slot_of(p, s);
+  if (i * ROWS >= sl.n * gqa) return 0;
+  return (row_tile<ROWS, KT>(p, sl, i, gqa).tiles + PER - 1) / PER;
+}
+
+// Where a workgroup's part begins: entry and unit in it, and the units of one head.
+struct Part {
+  int total;      // units of one head
+  int entry, at;  // first entry, units of it before the part
+};
+
+template <int THREADS>
+__device__ __forceinline__ int block_scan(int v, int* lds, int& sum) {   // inclusive
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int o = __shfl_up(v, d);
+    if (lane >= d) v += o;
+  }
+  __syncthreads();
+  if (lane == 63) lds[w] = v;
+  __syncthreads();
+  int before = 0;
+  sum = 0;
+#pragma unroll
+  for (int i = 0; i < THREADS / 64; i++) {
+    if (i < w) before += lds[i];
+    sum += lds[i];
+  }
+  return v + before;
+}
+
+// The unit line of one head; workgroup 0 leaves its prefix for the merge.
+template <int ROWS, int KT, int PER, int THREADS>
+__device__ __forceinline__ int line_units(const F8AttnArgs& p, int gqa, int* lds) {
+  const int entries = p.n_slots * p.slot_tiles;
+  const bool keep = blockIdx.x == 0;
+  int base = 0;
+  for (int c = 0; c < entries; c += THREADS) {
+    const int x = c + threadIdx.x;
+    int sum;
+    const int inc = block_scan<THREADS>(x < entries ? entry_units<ROWS, KT, PER>(p, x, gqa) : 0, lds, sum);
+    if (keep && x < entries) p.pre[x + 1] = base + inc;
+    base += sum;
+  }
+  if (keep && threadIdx.x == 0) p.pre[0] = 0;
+  return base;
+}
+// The entry that holds unit u of the line (u < its length)
+template <int ROWS, int KT, int PER, int THREADS>
+__device__ __forceinline__ Part line_find(const F8AttnArgs& p, int gqa, int total, int u, int* lds) {
+  const int entries = p.n_slots * p.slot_tiles;
+  __shared__ int found[2];
+  int base = 0;
+  for (int c = 0; c < entries; c += THREADS) {
+    const int x = c + threadIdx.x;
+    const int mine = x < entries ? entry_units<ROWS, KT, PER>(p, x, gqa) : 0;
+    int sum;
+    const int inc = base + block_scan<THREADS>(mine, lds, sum);
+    if (u >= inc - mine && u < inc) {
+      found[0] = x;
+      found[1] = u - (inc - mine);
+    }
+    base += sum;
+    if (base > u) break;
+  }
+  __syncthreads();
+  const Part r{total, __builtin_amdgcn_readfirstlane(found[0]), __builtin_amdgcn_readfirstlane(found[1])};
+  __syncthreads();
+  return r;
+}
+// Parts of the line: at most a workgroup's each, and none empty.
+__device__ __forceinline__ int part_count(long units, int groups) { return (int)min(units, (long)groups); }
+__device__ __forceinline__ long part_begin(long units, int g, int parts) { return units * g / parts; }
+
+__device__ __forceinline__ bool sees(int key, int pos, int end, int window, int sink) {
+  return key <= pos && key < end && (window <= 0 || key > pos - window || key < sink);
+}
+
+}  // namespace
+
+// ---------------------------------------------------------------------------
+// few rows: up to 64 (token, head) rows of a slot and KV head
+// ---------------------------------------------------------------------------
+// Four waves, each with key tiles of its own (32 keys, a fourth of the part), joined
+// through LDS at the end: nothing is shared on the way, so a wave waits only for its
+// own loads and K, V of the next tile are in flight while this one is computed
+// (16 KB a wave at head_dim 256).  K rows are the A operand as loaded: lane l%16 is
+// the key, and the group l/16 takes the same dims of K and Q.  V comes four keys
+// by a run of dims, and byte permutes pair the keys ahead of the conversion.
+template <int HD, int NR>
+__global__ __launch_bounds__(256, NR == 1 ? 2 : 1) void f8_few_kernel(F8AttnArgs p) {
+  constexpr int KT = 32, ROWS = 16 * NR, PER = 4, THREADS = 256;
+  constexpr int KW = HD / 64;        // 16-byte key loads of a lane and 16-key half
+  constexpr int VD = HD / 64;        // value dwords of a lane and key
+  constexpr int DB = HD / 16;        // 16-dim blocks of the output
+  constexpr int PITCH = HD + 4;
+  __shared__ float red[4 * 16 * PITCH];
+  __shared__ float ml[4][ROWS][2];
+  __shared__ int lds[THREADS / 64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int m = lane & 15, g = lane >> 4;
+  const int gqa = p.num_q / p.num_kv;
+
+  const int total = line_units<ROWS, KT, PER, THREADS>(p, gqa, lds);
+  const long all = (long)total * p.num_kv;
+  const int grp = blockIdx.x, parts = part_count(all, p.groups);
+  if (grp >= parts) return;
+  long u = part_begin(all, grp, parts);
+  const long u_end = part_begin(all, grp + 1, parts);
+  int h = (int)(u / total);
+  Part at = line_find<ROWS, KT, PER, THREADS>(p, gqa, total, (int)(u - (long)h * total), lds);
+  bool first_seg = true;
+  const long key_bytes = (long)p.num_kv * HD;
+
+  while (u < u_end) {
+    const int s = at.entry / p.slot_tiles;
+    const Slot sl = slot_of(p, s);
+    if (at.entry - s * p.slot_tiles != 0 || sl.n <= 0) {   // (one row tile a slot here)
+      at.entry = at.entry + 1 < p.n_slots * p.slot_tiles ? at.entry + 1 : 0;
+      if (at.entry == 0) h++;
+      continue;
+    }
+    const RowTile rt = row_tile<ROWS, KT>(p, sl, 0, gqa);
+    const int units = (rt.tiles + PER - 1) / PER;
+    const int n_u = (int)min((long)(units - at.at), u_end - u);
+    const int rows = sl.n * gqa;
+    const int v_end = min((at.at + n_u) * PER, rt.tiles);
+
+    // ---- queries: row 16 nr + m, dims 64 i + 16 g + 8 half ..
+    h8_t qf[NR][KW][2];
+    int pos_r[NR];
+#pragma unroll
+    for (int nr = 0; nr < NR; nr++) {
+      const int r = 16 * nr + m, rc = min(r, rows - 1);
+      const int t = rc / gqa;
+      pos_r[nr] = sl.pos0 + t;
+      const uint16_t* src = p.q + ((long)(sl.t0 + t) * p.num_q + h * gqa + (rc - t * gqa)) * HD + 16 * g;
+#pragma unroll
+      for (int i = 0; i < KW; i++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) qf[nr][i][e] = *reinterpret_cast<const h8_t*>(src + 64 * i + 8 * e);
+    }
+
+    f4_t acc[NR][DB];
+    float mx[NR], ls[NR];
+#pragma unroll
+    for (int nr = 0; nr < NR; nr++) {
+      mx[nr] = -INFINITY;
+      ls[nr] = 0.f;
+#pragma unroll
+      for (int d = 0; d < DB; d++) acc[nr][d] = f4_t{0.f, 0.f, 0.f, 0.f};
+    }
+
+    const int32_t* table = p.tables + (long)s * p.max_blocks;
+    auto page_of = [&](int key) {
+      const int b = key / p.block_tokens;
+      const int pg = key < rt.end && b < p.max_blocks ? table[b] : -1;
+      return pg >= 0 && pg < p.n_pages ? pg : -1;
+    };
+    // the two 16-key halves of a tile: pages (-1: none), rows inside the page, exponents
+    struct Tile {
+      int key0, pg[2];
+    };
+    u4_t kr[2][KW];
+    uint32_t vr[8][VD];
+    float ks[2], vs[2];
+    auto lookup = [&](int v) {
+      Tile t;
+      t.key0 = rt.key0(v, KT);
+      t.pg[0] = page_of(t.key0);
+      t.pg[1] = page_of(t.key0 + 16);
+      return t;
+    };
+    auto load_k = [&](const Tile& t) {
+#pragma unroll
+      for (int hf = 0; hf < 2; hf++) {
+        const int pg = max(t.pg[hf], 0), row = (t.key0 + 16 * hf) % p.block_tokens;
+        const uint8_t* base = p.k_pool + ((long)pg * p.block_tokens + row) * key_bytes + (long)h * HD;
+        ks[hf] = pow2f(p.k_exp[(long)pg * p.num_kv + h]);
+#pragma unroll
+        for (int i = 0; i < KW; i++)
+          kr[hf][i] = *reinterpret_cast<const u4_t*>(base + m * key_bytes + 64 * i + 16 * g);
+      }
+    };
+    auto load_v = [&](const Tile& t) {
+#pragma unroll
+      for (int hf = 0; hf < 2; hf++) {
+        const int pg = max(t.pg[hf], 0), row = (t.key0 + 16 * hf) % p.block_tokens;
+        const uint8_t* base = p.v_pool + ((long)pg * p.block_tokens + row) * key_bytes + (long)h * HD;
+        vs[hf] = pow2f(p.v_exp[(long)pg * p.num_kv + h]);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const uint8_t* src = base + (4 * g + i) * key_bytes + m * (4 * VD);
+          if constexpr (VD == 4) {
+            const u4_t w = *reinterpret_cast<const u4_t*>(src);
+#pragma unroll
+            for (int d = 0; d < 4; d++) vr[4 * hf + i][d] = w[d];
+          } else {
+            const u2_t w = *reinterpret_cast<const u2_t*>(src);
+#pragma unroll
+            for (int d = 0; d < 2; d++) vr[4 * hf + i][d] = w[d];
+          }
+        }
+      }
+    };
+
+    int v = at.at * PER + wave;
+    Tile cur{}, nxt{};
+    if (v < v_end) {
+      cur = lookup(v);
+      load_k(cur);
+      load_v(cur);
+      nxt = v + PER < v_end ? lookup(v + PER) : cur;
+    }
+    for (; v < v_end; v += PER) {
+      const bool more = v + PER < v_end;
+      // ---- scores: lane m's row, keys 16 hf + 4 g + i
+      f4_t sc[NR][2];
+#pragma unroll
+      for (int hf = 0; hf < 2; hf++) {
+        h8_t ka[KW][2];
+#pragma unroll
+        for (int i = 0; i < KW; i++)
+#pragma unroll
+          for (int e = 0; e < 2; e++)
+            ka[i][e] = join8(cvt2(kr[hf][i][2 * e], ks[hf], false), cvt2(kr[hf][i][2 * e], ks[hf], true),
+                             cvt2(kr[hf][i][2 * e + 1], ks[hf], false), cvt2(kr[hf][i][2 * e + 1], ks[hf], true));
+#pragma unroll
+        for (int nr = 0; nr < NR; nr++) {
+          f4_t a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int i = 0; i < KW; i++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) a = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[i][e], qf[nr][i][e], a, 0, 0, 0);
+          sc[nr][hf] = a * p.scale_log2;
+        }
+      }
+      const bool whole = cur.pg[0] >= 0 && cur.pg[1] >= 0 && cur.key0 + KT - 1 <= rt.pos_lo && cur.key0 + KT <= rt.end &&
+                         (p.window <= 0 || cur.key0 > rt.pos_hi - p.window || cur.key0 + KT <= p.sink);
+      if (more) load_k(nxt);
+      if (!whole) {
+#pragma unroll
+        for (int hf = 0; hf < 2; hf++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const int key = cur.key0 + 16 * hf + 4 * g + i;
+            const bool there = cur.pg[hf] >= 0 && key < rt.end;
+#pragma unroll
+            for (int nr = 0; nr < NR; nr++)
+              sc[nr][hf][i] = there && sees(key, pos_r[nr], rt.end, p.window, p.sink) ? sc[nr][hf][i] : -INFINITY;
+            // rows past the last key hold whatever the page held before
+#pragma unroll
+            for (int d = 0; d < VD; d++) vr[4 * hf + i][d] = there ? vr[4 * hf + i][d] : 0u;
+          }
+      }
+      h8_t pb[NR];
+#pragma unroll
+      for (int nr = 0; nr < NR; nr++) {
+        float t = sc[nr][0][0];
+#pragma unroll
+        for (int i = 1; i < 8; i++) t = fmaxf(t, sc[nr][i >> 2][i & 3]);
+        t = max32(max16(t));
+        if (__builtin_amdgcn_ballot_w64(t > mx[nr] + kSlack) != 0) {
+          const float mn = fmaxf(mx[nr], t);
+          const float f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mx[nr] - mn);
+          ls[nr] *= f;
+#pragma unroll
+          for (int d = 0; d < DB; d++) acc[nr][d] *= f;
+          mx[nr] = mn;
+        }
+        const float base = mx[nr] == -INFINITY ? 0.f : mx[nr];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          pb[nr][i] = (_Float16)__builtin_amdgcn_exp2f(sc[nr][i >> 2][i & 3] - base);
+          ls[nr] += (float)pb[nr][i];
+        }
+      }
+      // ---- O^T += V^T P^T: dims m * HD/16 + 4 d + j
+#pragma unroll
+      for (int d = 0; d < VD; d++) {
+        uint32_t w[4][2];   // key pairs x byte pairs
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          w[k][0] = __builtin_amdgcn_perm(vr[2 * k + 1][d], vr[2 * k][d], 0x05010400u);
+          w[k][1] = __builtin_amdgcn_perm(vr[2 * k + 1][d], vr[2 * k][d], 0x07030602u);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const h8_t a = join8(cvt2(w[0][j >> 1], vs[0], j & 1), cvt2(w[1][j >> 1], vs[0], j & 1),
+                               cvt2(w[2][j >> 1], vs[1], j & 1), cvt2(w[3][j >> 1], vs[1], j & 1));
+#pragma unroll
+          for (int nr = 0; nr < NR; nr++)
+            acc[nr][4 * d + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pb[nr], acc[nr][4 * d + j], 0, 0, 0);
+        }
+      }
+      if (more) {
+        load_v(nxt);
+        cur = nxt;
+        if (v + 2 * PER < v_end) nxt = lookup(v + 2 * PER);
+      }
+    }
+
+    // ---- join the waves; lane m, group g holds dims (4 g + i) * HD/16 + d of row m
+    const bool complete = n_u == units;
+    const int rec = 2 * grp + (first_seg ? 0 : 1);
+#pragma unroll
+    for (int nr = 0; nr < NR; nr++) {
+      ls[nr] = sum32(sum16(ls[nr]));
+      if (g == 0) {
+        ml[wave][16 * nr + m][0] = mx[nr];
+        ml[wave][16 * nr + m][1] = ls[nr];
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int nr = 0; nr < NR; nr++) {
+      if (16 * nr >= rows) break;
+      float M = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < 4; w++) M = fmaxf(M, ml[w][16 * nr + m][0]);
+      const float f = mx[nr] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx[nr] - M);
+      if (16 * nr + m < rows) {
+        float* dst = red + (wave * 16 + m) * PITCH;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+          for (int d = 0; d < DB; d += 4)
+            *reinterpret_cast<f4_t*>(dst + (4 * g + i) * DB + d) =
+                f4_t{acc[nr][d][i], acc[nr][d + 1][i], acc[nr][d + 2][i], acc[nr][d + 3][i]} * f;
+      }
+      __syncthreads();
+      const int here = min(16, rows - 16 * nr);
+      for (int x = tid * 4; x < here * HD; x += THREADS * 4) {
+        const int r = x / HD, d = x - r * HD, row = 16 * nr + r;
+        float Mr = -INFINITY, L = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; w++) Mr = fmaxf(Mr, ml[w][row][0]);
+#pragma unroll
+        for (int w = 0; w < 4; w++)
+          L += ml[w][row][0] == -INFINITY ? 0.f : ml[w][row][1] * __builtin_amdgcn_exp2f(ml[w][row][0] - Mr);
+        f4_t o = *reinterpret_cast<const f4_t*>(red + r * PITCH + d);
+#pragma unroll
+        for (int w = 1; w < 4; w++) o += *reinterpret_cast<const f4_t*>(red + (16 * w + r) * PITCH + d);
+        if (complete) {
+          const float inv = L > 0.f ? 1.f / L : 0.f;
+          o *= inv;
+          const int t = row / gqa;
+          *reinterpret_cast<u2_t*>(p.out + ((long)(sl.t0 + t) * p.num_q + h * gqa + (row - t * gqa)) * HD + d) =
+              u2_t{f2h(o[0]) | (f2h(o[1]) << 16), f2h(o[2]) | (f2h(o[3]) << 16)};
+        } else {
+          *reinterpret_cast<f4_t*>(p.rec_o + ((long)rec * p.rec_rows + row) * HD + d) = o;
+          if (d == 0) *reinterpret_cast<f2_t*>(p.rec_ml + ((long)rec * p.rec_rows + row) * 2) = f2_t{Mr, L};
+        }
+      }
+      __syncthreads();
+    }
+    first_seg = false;
+    u += n_u;
+    at.at = 0;
+    at.entry++;
+    if (at.entry == p.n_slots * p.slot_tiles) {
+      at.entry = 0;
+      h++;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// many rows: prompts and chunks
+// ---------------------------------------------------------------------------
+// Waves of 32 rows share fp16 K and V tiles in LDS, converted once by the workgroup
+// from the next tile's codes (in registers while the present tile is computed).
+// V is stored by dim, four keys to 8 bytes, in the order that the scores' lanes hold
+// them.  Pads and the key swizzle keep 16-byte reads of 16 lanes on distinct banks.
+template <int HD, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2))) void f8_many_kernel(F8AttnArgs p) {
+  constexpr int KT = 8192 / HD;              // 32 or 64 keys: 8 KB of codes
+  constexpr int ROWS = 32 * WAVES, THREADS = 64 * WAVES, PER = 1;
+  constexpr int NL = 512 / THREADS;          // loads of a thread for 8 KB
+  constexpr int VP = KT * 2;                 // bytes of a dim's values
+  constexpr int VPAD = KT == 32 ? 4 : 2;     // dims per 16-byte pad
+  constexpr int KB = KT * HD * 2, VB = HD * VP + HD / VPAD * 16;
+  __shared__ __align__(16) uint8_t tile_lds[2][KB + VB];
+  __shared__ int lds[WAVES];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c = lane & 31, hh = lane >> 5;
+  const int gqa = p.num_q / p.num_kv;
+
+  const int total = line_units<ROWS, KT, PER, THREADS>(p, gqa, lds);
+  const long all = (long)total * p.num_kv;
+  const int grp = blockIdx.x, parts = part_count(all, p.groups);
+  if (grp >= parts) return;
+  long u = part_begin(all, grp, parts);
+  const long u_end = part_begin(all, grp + 1, parts);
+  int h = (int)(u / total);
+  Part at = line_find<ROWS, KT, PER, THREADS>(p, gqa, total, (int)(u - (long)h * total), lds);
+  bool first_seg = true;
+  const long key_bytes = (long)p.num_kv * HD;
+  const int entries = p.n_slots * p.slot_tiles;
+
+  while (u < u_end) {
+    const int s = at.entry / p.slot_tiles, rti = at.entry - s * p.slot_tiles;
+    const Slot sl = slot_of(p, s);
+    if (rti * ROWS >= sl.n * gqa) {   // past this slot's rows
+      at.entry = (s + 1) * p.slot_tiles;
+      if (at.entry >= entries) {
+        at.entry = 0;
+        h++;
+      }
+      continue;
+    }
+    const RowTile rt = row_tile<ROWS, KT>(p, sl, rti, gqa);
+    const int n_u = (int)min((long)(rt.tiles - at.at), u_end - u);
+    const int v0 = at.at, v1 = at.at + n_u;
+    const int rows = sl.n * gqa;
+    const int row_w = rti * ROWS + wave * 32;      // this wave's first row
+    const int row = min(row_w + c, rows - 1), tok = row / gqa;
+    const int pos = sl.pos0 + tok;
+    const int pos_lo = sl.pos0 + min(row_w, rows - 1) / gqa, pos_hi = sl.pos0 + min(row_w + 31, rows - 1) / gqa;
+    const bool live = row_w < rows;
+
+    h8_t qf[HD / 16];
+    float sl2 = p.scale_log2;
+    {
+      const uint16_t* src = p.q + ((long)(sl.t0 + tok) * p.num_q + h * gqa + (row - tok * gqa)) * HD + 8 * hh;
+#pragma unroll
+      for (int i = 0; i < HD / 16; i++) qf[i] = *reinterpret_cast<const h8_t*>(src + 16 * i);
+      // (a negative scale is carried by the query, so that raw maxima serve)
+      if (sl2 < 0.f) {
+        sl2 = -sl2;
+#pragma unroll
+        for (int i = 0; i < HD / 16; i++) qf[i] = -qf[i];
+      }
+    }
+    f16x_t acc[HD / 32];
+#pragma unroll
+    for (int d = 0; d < HD / 32; d++) acc[d] = f16x_t{};
+    float mx = -INFINITY, ls = 0.f;
+
+    const int32_t* table = p.tables + (long)s * p.max_blocks;
+    auto page_of = [&](int key) {
+      const int b = key / p.block_tokens;
+      const int pg = key < rt.end && b < p.max_blocks ? table[b] : -1;
+      return pg >= 0 && pg < p.n_pages ? pg : -1;
+    };
+    // a thread's part of a tile: 16 bytes of a key row, and 4 dims of 4 keys
+    auto k_key = [&](int l) { return (tid + l * THREADS) / (HD / 16); };
+    const int vl = lane & (HD / 4 - 1);                                  // dims 4 vl ..
+    auto v_quad = [&](int l) { return (tid + l * THREADS) / (HD / 4); };   // keys 4 quad ..
+    int kpg[NL], vpg[NL];       // pages of the tile after next
+    u4_t kr[NL];
+    uint32_t vr[NL][4];
+    float ksc[NL], vsc[NL];
+    auto lookup = [&](int v) {
+      const int key0 = rt.key0(v, KT);
+#pragma unroll
+      for (int l = 0; l < NL; l++) {
+        kpg[l] = page_of(key0 + k_key(l));
+        vpg[l] = page_of(key0 + 4 * v_quad(l));
+      }
+    };
+    auto fetch = [&](int v) {
+      const int key0 = rt.key0(v, KT);
+#pragma unroll
+      for (int l = 0; l < NL; l++) {
+        const int key = key0 + k_key(l), slot = (tid + l * THREADS) % (HD / 16);
+        const int pk = max(kpg[l], 0);
+        kr[l] = *reinterpret_cast<const u4_t*>(p.k_pool + ((long)pk * p.block_tokens + key % p.block_tokens) * key_bytes +
+                                               (long)h * HD + 16 * slot);
+        ksc[l] = kpg[l] >= 0 ? pow2f(p.k_exp[(long)pk * p.num_kv + h]) : 0.f;
+        const int vk = key0 + 4 * v_quad(l), pv = max(vpg[l], 0);
+        const uint8_t* src = p.v_pool + ((long)pv * p.block_tokens + vk % p.block_tokens) * key_bytes + (long)h * HD + 4 * vl;
+        vsc[l] = vpg[l] >= 0 ? pow2f(p.v_exp[(long)pv * p.num_kv + h]) : 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const uint32_t w = *reinterpret_cast<const uint32_t*>(src + i * key_bytes);
+          vr[l][i] = vpg[l] >= 0 && vk + i < rt.end ? w : 0u;   // (rows past the last key: anything)
+        }
+        if (kpg[l] < 0) kr[l] = u4_t{0, 0, 0, 0};
+      }
+    };
+    auto stage = [&](int buf) {
+      uint8_t* kb = tile_lds[buf];
+      uint8_t* vb = kb + KB;
+#pragma unroll
+      for (int l = 0; l < NL; l++) {
+        const int key = k_key(l), slot = (tid + l * THREADS) % (HD / 16);
+        const float f = ksc[l];
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          const h8_t x = join8(cvt2(kr[l][2 * e], f, false), cvt2(kr[l][2 * e], f, true),
+                               cvt2(kr[l][2 * e + 1], f, false), cvt2(kr[l][2 * e + 1], f, true));
+          *reinterpret_cast<h8_t*>(kb + key * (HD * 2) + (((2 * slot + e) ^ (key & 15)) * 16)) = x;
+        }
+        const int q = v_quad(l);
+        // quad q of 16 keys (q & 3 = 2 a + half): 16-byte slot 2 (q / 4) + half, its part a
+        const int at8 = ((q >> 2) * 2 + (q & 1)) * 16 + ((q >> 1) & 1) * 8;
+        uint32_t w[2][2];
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+          w[k][0] = __builtin_amdgcn_perm(vr[l][2 * k + 1], vr[l][2 * k], 0x05010400u);
+          w[k][1] = __builtin_amdgcn_perm(vr[l][2 * k + 1], vr[l][2 * k], 0x07030602u);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const int dim = 4 * vl + j;
+          const u2_t x = {__builtin_bit_cast(uint32_t, cvt2(w[0][j >> 1], vsc[l], j & 1)),
+                          __builtin_bit_cast(uint32_t, cvt2(w[1][j >> 1], vsc[l], j & 1))};
+          *reinterpret_cast<u2_t*>(vb + dim * VP + dim / VPAD * 16 + at8) = x;
+        }
+      }
+    };
+
+    lookup(v0);
+    fetch(v0);
+    if (v0 + 1 < v1) lookup(v0 + 1);
+    __syncthreads();   // (the last segment's tiles are done with)
+    stage(0);
+    if (v0 + 1 < v1) fetch(v0 + 1);
+    if (v0 + 2 < v1) lookup(v0 + 2);
+    __syncthreads();
+    for (int v = v0; v < v1; v++) {
+      const int buf = (v - v0) & 1;
+      if (v + 1 < v1) stage(buf ^ 1);
+      if (v + 2 < v1) fetch(v + 2);
+      if (v + 3 < v1) lookup(v + 3);
+      const int key0 = rt.key0(v, KT);
+      // a wave none of whose rows sees the tile sits it out
+      const bool out = !live || key0 > pos_hi ||
+                       (p.window > 0 && key0 + KT - 1 <= pos_lo - p.window && key0 >= p.sink);
+      if (!out) {
+        const uint8_t* kb = tile_lds[buf];
+        const uint8_t* vb = kb + KB;
+#pragma unroll
+        for (int kh = 0; kh < KT / 32; kh++) {
+          const int k0 = key0 + 32 * kh;
+          f16x_t sd = f16x_t{};
+          {
+            const uint8_t* krow = kb + (32 * kh + c) * (HD * 2);
+#pragma unroll
+            for (int i = 0; i < HD / 16; i++) {
+              const h8_t a = *reinterpret_cast<const h8_t*>(krow + (((2 * i + hh) ^ (c & 15)) * 16));
+              sd = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qf[i], sd, 0, 0, 0);
+            }
+          }
+          // pages may be absent anywhere: which of the two 16-key halves exist
+          const int pa = page_of(k0), pb2 = page_of(k0 + 16);
+          const bool whole = pa >= 0 && pb2 >= 0 && k0 + 31 <= pos_lo && k0 + 32 <= rt.end &&
+                             (p.window <= 0 || k0 > pos_hi - p.window || k0 + 32 <= p.sink);
+          float t = -INFINITY, f = sl2;
+          if (whole) {
+#pragma unroll
+            for (int x = 0; x < 16; x++) t = fmaxf(t, sd[x]);
+            t = max32(t) * sl2;
+          } else {
+#pragma unroll
+            for (int x = 0; x < 16; x++) {
+              const int key = k0 + 8 * (x >> 2) + 4 * hh + (x & 3);
+              const bool there = x < 8 ? pa >= 0 : pb2 >= 0;
+              sd[x] = there && sees(key, pos, rt.end, p.window, p.sink) ? sd[x] * sl2 : -INFINITY;
+              t = fmaxf(t, sd[x]);
+            }
+            t = max32(t);
+            f = 1.f;
+          }
+          if (__builtin_amdgcn_ballot_w64(t > mx + kSlack) != 0) {
+            const float mn = fmaxf(mx, t);
+            const float r = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mx - mn);
+            ls *= r;
+#pragma unroll
+            for (int d = 0; d < HD / 32; d++) acc[d] *= r;
+            mx = mn;
+          }
+          const float base = mx == -INFINITY ? 0.f : mx;
+#pragma unroll
+          for (int sg = 0; sg < 2; sg++) {
+            h8_t w;
+#pragma unroll
+            for (int i = 0; i < 8; i++) w[i] = (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(sd[8 * sg + i], f, -base));
+#pragma unroll
+            for (int i = 0; i < 8; i++) ls += (float)w[i];
+#pragma unroll
+            for (int d = 0; d < HD / 32; d++) {
+              const int dim = 32 * d + c;
+              const h8_t a = *reinterpret_cast<const h8_t*>(vb + dim * VP + dim / VPAD * 16 + ((2 * kh + sg) * 2 + hh) * 16);
+              acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, w, acc[d], 0, 0, 0);
+            }
+          }
+        }
+      }
+      __syncthreads();
+    }
+
+    ls = sum32(ls);
+    const bool complete = n_u == rt.tiles;
+    if (row_w + c < rows) {
+      if (complete) {
+        const float inv = ls > 0.f ? 1.f / ls : 0.f;
+        uint16_t* o = p.out + ((long)(sl.t0 + tok) * p.num_q + h * gqa + (row - tok * gqa)) * HD + 4 * hh;
+#pragma unroll
+        for (int d = 0; d < HD / 32; d++)
+#pragma unroll
+          for (int a = 0; a < 4; a++)
+            *reinterpret_cast<u2_t*>(o + 32 * d + 8 * a) =
+                u2_t{f2h(acc[d][4 * a] * inv) | (f2h(acc[d][4 * a + 1] * inv) << 16),
+                     f2h(acc[d][4 * a + 2] * inv) | (f2h(acc[d][4 * a + 3] * inv) << 16)};
+      } else {
+        const long rec = (2 * grp + (first_seg ? 0 : 1)) * (long)p.rec_rows + wave * 32 + c;
+#pragma unroll
+        for (int d = 0; d < HD / 32; d++)
+#pragma unroll
+          for (int a = 0; a < 4; a++)
+            *reinterpret_cast<f4_t*>(p.rec_o + rec * HD + 32 * d + 8 * a + 4 * hh) =
+                f4_t{acc[d][4 * a], acc[d][4 * a + 1], acc[d][4 * a + 2], acc[d][4 * a + 3]};
+        if (hh == 0) *reinterpret_cast<f2_t*>(p.rec_ml + rec * 2) = f2_t{mx, ls};
+      }
+    }
+    first_seg = false;
+    u += n_u;
+    at.at = 0;
+    at.entry++;
+    if (at.entry >= entries) {
+      at.entry = 0;
+      h++;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// merge of the row tiles that were cut
+// ---------------------------------------------------------------------------
+// One wave per row at a time, WPR waves of a workgroup on the same row (each takes
+// every WPR-th record).
+template <int HD, int WPR>
+__global__ __launch_bounds__(256) void f8_merge_kernel(F8AttnArgs p, int rows_tile) {
+  constexpr int E = HD / 64;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int entries = p.n_slots * p.slot_tiles;
+  const int row_groups = (rows_tile * WPR + 3) / 4;
+  const int tile = blockIdx.x / row_groups, entry = tile % entries, h = tile / entries;
+  const int total = p.pre[entries], a = p.pre[entry], b = p.pre[entry + 1];
+  if (a == b) return;
+  const long all = (long)total * p.num_kv, x0 = (long)h * total + a, x1 = (long)h * total + b;
+  const int parts = part_count(all, p.groups);
+  // the parts that hold the tile's first and last unit
+  auto part_of = [&](long x) {
+    long g = ((x + 1) * parts - 1) / all;
+    while (g > 0 && part_begin(all, (int)g, parts) > x) g--;
+    while (part_begin(all, (int)g + 1, parts) <= x) g++;
+    return (int)g;
+  };
+  const int g0 = part_of(x0), g1 = part_of(x1 - 1);
+  if (g0 == g1) return;   // stored whole
+  const int r0 = 2 * g0 + (part_begin(all, g0, parts) == x0 ? 0 : 1);
+  const int n = g1 - g0 + 1;
+  auto rec_of = [&](int i) { return i == 0 ? r0 : 2 * (g0 + i); };
+  const int s = entry / p.slot_tiles, gqa = p.num_q / p.num_kv;
+  const Slot sl = slot_of(p, s);
+  const int base_row = (entry - s * p.slot_tiles) * rows_tile;
+  const int row = (blockIdx.x - tile * row_groups) * (4 / WPR) + wave / WPR;
+  const bool live = row < rows_tile && base_row + row < sl.n * gqa;
+
+  float M = -INFINITY, L = 0.f;
+  float o[E] = {};
+  if (live) {
+    for (int i0 = 0; i0 < n; i0 += 64) {
+      if (i0 + lane < n) {
+        const f2_t r = *reinterpret_cast<const f2_t*>(p.rec_ml + ((long)rec_of(i0 + lane) * p.rec_rows + row) * 2);
+        if (r[1] > 0.f) M = fmaxf(M, r[0]);
+      }
+    }
+    M = wave_max(M);
+    if (M == -INFINITY) M = 0.f;
+#pragma unroll 8
+    for (int i = wave % WPR; i < n; i += WPR) {
+      const long at = (long)rec_of(i) * p.rec_rows + row;
+      const f2_t r = *reinterpret_cast<const f2_t*>(p.rec_ml + at * 2);
+      const float w = r[1] > 0.f ? __builtin_amdgcn_exp2f(r[0] - M) : 0.f;
+      L += w * r[1];
+      const float* src = p.rec_o + at * HD + lane * E;
+      if constexpr (E == 4) {
+        const f4_t x = *reinterpret_cast<const f4_t*>(src);
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[e] = __builtin_fmaf(w, x[e], o[e]);
+      } else {
+        const f2_t x = *reinterpret_cast<const f2_t*>(src);
+#pragma unroll
+        for (int e = 0; e < 2; e++) o[e] = __builtin_fmaf(w, x[e], o[e]);
+      }
+    }
+  }
+  if constexpr (WPR > 1) {
+    __shared__ float part[4][64][E + 1];
+#pragma unroll
+    for (int e = 0; e < E; e++) part[wave][lane][e] = o[e];
+    part[wave][lane][E] = L;
+    __syncthreads();
+    if (wave % WPR != 0) return;
+#pragma unroll
+    for (int w = 1; w < WPR; w++) {
+#pragma unroll
+      for (int e = 0; e < E; e++) o[e] += part[wave + w][lane][e];
+      L += part[wave + w][lane][E];
+    }
+  }
+  if (!live) return;
+  const float inv = L > 0.f ? 1.f / L : 0.f;
+  const int r = base_row + row, t = r / gqa;
+  uint16_t* dst = p.out + ((long)(sl.t0 + t) * p.num_q + h * gqa + (r - t * gqa)) * HD + lane * E;
+  if constexpr (E == 4)
+    *reinterpret_cast<u2_t*>(dst) = u2_t{f2h(o[0] * inv) | (f2h(o[1] * inv) << 16), f2h(o[2] * inv) | (f2h(o[3] * inv) << 16)};
+  else
+    *reinterpret_cast<uint32_t*>(dst) = f2h(o[0] * inv) | (f2h(o[1] * inv) << 16);
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+constexpr int kManyWaves = 8;
+
+F8AttnPlan f8_attn_plan(int num_q, int num_kv, int head_dim, int n_slots, long q_rows, int max_tok, int max_ctx) {
+  F8AttnPlan x{};
+  const long rows = (long)max_tok * (num_q / num_kv);
+  x.many = rows > 64;
+  x.row_tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  long units;   // most units of all heads
+  if (x.many) {
+    const int tile_rows = 32 * kManyWaves, kt = 8192 / head_dim;
+    x.slot_tiles = (int)((rows + tile_rows - 1) / tile_rows);
+    x.rec_rows = tile_rows;
+    // (a slot has at most one row tile that is not full)
+    const long tiles = std::min<long>((long)n_slots * x.slot_tiles, q_rows * (num_q / num_kv) / tile_rows + n_slots);
+    units = tiles * num_kv * ((max_ctx + kt - 1) / kt);
+    x.groups = (int)std::min<long>(units, 256);
+    x.merges = true;
+  } else {
+    x.slot_tiles = 1;
+    x.rec_rows = (int)rows;
+    units = (long)n_slots * num_kv * ((max_ctx + 127) / 128);
+    x.groups = (int)std::min<long>(units, x.row_tiles == 1 ? 512 : 256);
+    x.merges = max_ctx > 128 || units > x.groups;
+  }
+  const size_t pre = (((size_t)n_slots * x.slot_tiles + 1) * 4 + 255) / 256 * 256;
+  const size_t recs = 2 * (size_t)x.groups * x.rec_rows;
+  x.ml_off = pre;
+  x.o_off = pre + (recs * 8 + 255) / 256 * 256;
+  x.total = x.o_off + recs * head_dim * 4;
+  return x;
+}
+
+template <int HD>
+static void launch_f8(const F8AttnArgs& a, const F8AttnPlan& x, hipStream_t stream) {
+  const dim3 grid((unsigned)x.groups);
+  if (x.many)
+    hipLaunchKernelGGL((f8_many_kernel<HD, kManyWaves>), grid, dim3(64 * kManyWaves), 0, stream, a);
+  else if (x.row_tiles == 1)
+    hipLaunchKernelGGL((f8_few_kernel<HD, 1>), grid, dim3(256), 0, stream, a);
+  else if (x.row_tiles == 2)
+    hipLaunchKernelGGL((f8_few_kernel<HD, 2>), grid, dim3(256), 0, stream, a);
+  else
+    hipLaunchKernelGGL((f8_few_kernel<HD, 4>), grid, dim3(256), 0, stream, a);
+  if (!x.merges) return;
+  const unsigned tiles = (unsigned)(a.n_slots * a.slot_tiles * a.num_kv);
+  if (x.many)
+    hipLaunchKernelGGL((f8_merge_kernel<HD, 1>), dim3(tiles * (unsigned)(x.rec_rows / 4)), dim3(256), 0, stream, a, x.rec_rows);
+  else
+    hipLaunchKernelGGL((f8_merge_kernel<HD, 4>), dim3(tiles * (unsigned)x.rec_rows), dim3(256), 0, stream, a, x.rec_rows);
+}
+
+hipError_t launch_f8_attn(const F8AttnArgs& a, const F8AttnPlan& plan, int head_dim, hipStream_t stream) {
+  if (head_dim == 256) launch_f8<256>(a, plan, stream);
+  else if (head_dim == 128) launch_f8<128>(a, plan, stream);
+  else return hipErrorInvalidValue;
+  return hipGetLastError();
+}
+
+}  // namespace qkv

@@ -44,6 +44,7 @@ const char* qkv_status_string(int s) {
     case QKV_ERR_LAUNCH: return "kernel launch failed";
     case QKV_ERR_WORKSPACE: return "workspace missing or too small";
     case QKV_ERR_TIMEOUT: return "in-kernel merge timed out; reset the workspace";
+    case QKV_ERR_PAGES: return "no free page";
     default: return "unknown status";
   }
 }

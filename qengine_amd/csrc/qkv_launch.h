@@ -119,4 +119,109 @@ void prefill_schedule(PrefillArgs& a, int max_split);
 hipError_t launch_prefill_tq3(const PrefillArgs& a, int max_split, int gqa, const uint16_t* q, const uint16_t* k,
                               const uint16_t* v, uint16_t* out, hipStream_t stream);
 
+// Rotary positions (rope.hip).  Strides in elements between tokens; heads of a
+// token are head_dim apart.
+struct RopeArgs {
+  const uint16_t* q;
+  uint16_t* q_out;
+  const uint16_t* k;
+  uint16_t* k_out;
+  const int32_t* positions;
+  const uint64_t* turns;     // [rot / 2] fractions of a turn a position, 64-bit fixed point
+  long q_stride, q_out_stride, k_stride, k_out_stride;
+  float amplitude;
+  int n_tok, num_q, num_k, head_dim, rot;
+  int layout;                // 0: pairs (i, i + rot / 2), 1: (2i, 2i + 1)
+  int inverse;
+  int units;                 // set by the launcher
+};
+// wide: 16-byte accesses (rot and head_dim multiples of 16, pointers and strides aligned)
+hipError_t launch_rope(RopeArgs a, bool wide, bool in_place, hipStream_t stream);
+
+// Append to the paged 8-bit cache (f8_codec.hip), K and with them the queries
+// rotated where rot > 0.  rows: tokens the input tensors hold.
+struct F8AppendArgs {
+  const uint16_t* k;
+  const uint16_t* v;
+  const uint16_t* q;         // nullptr: no queries
+  uint16_t* q_out;
+  uint8_t* k_pool;
+  uint8_t* v_pool;
+  uint8_t* k_exp;
+  uint8_t* v_exp;
+  const int32_t* tables;     // [n_slots][max_blocks]
+  const int32_t* starts;     // [n_slots + 1]
+  const int32_t* positions;  // [n_slots]
+  const uint64_t* turns;
+  long k_stride, v_stride, q_stride, q_out_stride, rows, kv_wgs;
+  float amplitude;
+  int n_slots, max_tok, max_blocks, block_tokens, n_pages, num_q, num_kv, head_dim, rot, layout;
+  int spans;                 // pages that a slot's new rows may touch (set by the launcher)
+};
+hipError_t launch_f8_append(F8AppendArgs a, hipStream_t stream);
+
+// Attention over the paged 8-bit cache (attn_f8.hip).
+struct F8AttnArgs {
+  const uint16_t* q;         // [rows][num_q][head_dim]
+  uint16_t* out;
+  const uint8_t* k_pool;     // [n_pages][block_tokens][num_kv][head_dim]
+  const uint8_t* v_pool;
+  const uint8_t* k_exp;      // [n_pages][num_kv]
+  const uint8_t* v_exp;
+  const int32_t* tables;
+  const int32_t* starts;
+  const int32_t* positions;
+  int* pre;                  // workspace: unit prefix of the row tiles, [tiles + 1]
+  float* rec_ml;             // workspace: {m (log2 units), l} of a partial row
+  float* rec_o;              // workspace: its unnormalised sums
+  long rows;
+  int num_q, num_kv, n_slots, max_tok, max_ctx, max_blocks, block_tokens, n_pages, window, sink;
+  int slot_tiles;            // row tiles of a slot with max_tok tokens
+  int rec_rows;              // rows of a record
+  int groups;                // workgroups
+  float scale_log2;
+};
+struct F8AttnPlan {
+  bool many;                 // the kernel for more than 64 (token, head) rows a slot
+  int row_tiles;             // 16-row tiles of the other one: 1, 2 or 4
+  int slot_tiles, rec_rows, groups;
+  bool merges;               // whether any row can be in several workgroups
+  size_t ml_off, o_off, total;
+};
+F8AttnPlan f8_attn_plan(int num_q, int num_kv, int head_dim, int n_slots, long rows, int max_tok, int max_ctx);
+hipError_t launch_f8_attn(const F8AttnArgs& a, const F8AttnPlan& plan, int head_dim, hipStream_t stream);
+
+// Pages of a cache (kv_pages.hip): tables [n_slots][max_blocks] with a negative
+// entry where there is no page, ref_counts [n_pages] (0: free).
+constexpr int kMaxPlanes = 128;
+struct PagePlanes {
+  uint8_t* base[kMaxPlanes];
+  uint64_t bytes[kMaxPlanes];   // of a page
+  int n;
+};
+struct PageTables {
+  int32_t* tables;
+  int32_t* refs;
+  int n_slots, max_blocks, block_tokens, n_pages;
+};
+struct PageStatus {
+  int ok, invalid, pages;
+};
+hipError_t launch_pages_fork(const PageTables& t, const int32_t* parents, const int32_t* children,
+                             const int32_t* tokens, int n, int32_t* status, const PageStatus& codes,
+                             hipStream_t stream);
+hipError_t launch_pages_release(const PageTables& t, const int32_t* slots, const int32_t* keep, int n,
+                                int32_t* status, const PageStatus& codes, hipStream_t stream);
+constexpr int kReserveMax = 1024;   // slots of one reserve call
+inline int reserve_blocks(int max_new, int block_tokens) { return (max_new + block_tokens - 2) / block_tokens + 1; }
+// scratch: reserve_scratch_ints(n, blocks) int32, the copied pairs [n][2] first
+inline size_t reserve_scratch_ints(int n, int blocks) { return 3 * (size_t)n + 2 * (size_t)n * blocks; }
+hipError_t launch_pages_reserve(const PageTables& t, const int32_t* slots, const int32_t* positions,
+                                const int32_t* n_new, int n, int max_new, int32_t* status, const PageStatus& codes,
+                                const PagePlanes& planes, int32_t* scratch, hipStream_t stream);
+hipError_t launch_pages_copy(const PagePlanes& planes, const int32_t* pairs, int n, int n_pages, hipStream_t stream);
+// scratch: n_pages + 2 int32
+hipError_t launch_pages_compact(const PageTables& t, int32_t* moved, int32_t* n_used, const PagePlanes& planes,
+                                int32_t* scratch, hipStream_t stream);
+
 }  // namespace qkv

@@ -10,6 +10,8 @@ torch.float16.  Calls are ordered on the current torch stream.
 """
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
 from ._lib import bench_lib, check, lib
@@ -534,3 +536,297 @@ def prefill_attn_tq3(q, k_cache, v_cache, k_chunk, v_chunk, out, workspace, *, n
         _dev_ptr(out, "out"), num_q, num_kv, head_dim, start_pos, n_tok, float(scale),
         _dev_ptr(workspace, "workspace"), workspace.numel() * workspace.element_size(),
         _stream(stream)), "qkv_prefill_attn_tq3")
+
+
+# ---------------------------------------------------------------------------
+# rotary positions
+# ---------------------------------------------------------------------------
+
+_ROPE_SCALING = {"linear": 1, "ntk": 2, "yarn": 3}
+_ROPE_LAYOUT = {"half": 0, "interleaved": 1}
+
+
+class RopeTable:
+    """Frequencies for `rope`: `turns`, an int64 device tensor [rot_dim / 2] of 64-bit
+    fractions of a turn a position, and the amplitude of the scaling."""
+
+    def __init__(self, turns, amplitude, rot_dim):
+        self.turns, self.amplitude, self.rot_dim = turns, amplitude, rot_dim
+
+
+def rope_table(rot_dim: int, *, base: float = 10000.0, scaling=None, device="cuda") -> RopeTable:
+    """Frequencies base^(-2i/rot_dim).  scaling: None, ("linear", factor), ("ntk", factor) or
+    ("yarn", factor, original_ctx[, beta_fast=32, beta_slow=1])."""
+    kind, args = 0, ()
+    if scaling is not None:
+        if scaling[0] not in _ROPE_SCALING:
+            raise ValueError(f"unknown rope scaling {scaling[0]!r}")
+        kind, args = _ROPE_SCALING[scaling[0]], tuple(float(x) for x in scaling[1:])
+        if not (len(args) == 1 if kind < 3 else 2 <= len(args) <= 4):
+            raise ValueError(f"rope scaling {scaling[0]!r} with {len(args)} numbers")
+    factor, ctx, fast, slow = (args + (1.0, 1.0, 32.0, 1.0)[len(args):])[:4]
+    turns = (ctypes.c_uint64 * max(1, rot_dim // 2))()
+    amp = ctypes.c_float()
+    check(lib().qkv_rope_table(rot_dim, float(base), kind, factor, ctx, fast, slow, ctypes.addressof(turns),
+                               ctypes.addressof(amp)), "qkv_rope_table")
+    host = torch.frombuffer(turns, dtype=torch.int64).clone()
+    return RopeTable(host.to(device), float(amp.value), rot_dim)
+
+
+def _on_device(stream, *tensors) -> None:
+    """Every tensor on the device that the call launches on: that of `stream`, or the current one."""
+    dev = torch.cuda.current_device() if stream is None else stream.device.index
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"every tensor must be on cuda:{dev}, where the call runs; got {t.device}")
+
+
+def _rows3(t, what, dtype=FP16):
+    """A tensor [tokens][heads][head_dim], a token's heads contiguous: pointer and token stride
+    (elements)."""
+    if t.dtype not in dtype:
+        raise ValueError(f"{what} must be {' or '.join(str(d) for d in dtype)}, got {t.dtype}")
+    if not t.is_cuda:
+        raise ValueError(f"{what} must be a device tensor")
+    st = t.stride()
+    if t.dim() != 3 or (st[2] != 1 and t.shape[2] > 1) or (st[1] != t.shape[2] and t.shape[1] > 1):
+        raise ValueError(f"{what} must be [tokens][heads][head_dim], the heads of a token contiguous")
+    return t.data_ptr(), st[0] if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+
+
+def _rope_layout(layout) -> int:
+    if layout not in _ROPE_LAYOUT:
+        raise ValueError(f"layout must be 'half' or 'interleaved', got {layout!r}")
+    return _ROPE_LAYOUT[layout]
+
+
+def rope(q, k, positions, table: RopeTable, *, layout="half", inverse=False, q_out=None, k_out=None,
+         stream=None) -> None:
+    """Rotates q and k (fp16 [tokens][heads][head_dim], views into a fused projection
+    buffer among them; either may be None) by int32 `positions` [tokens], into q_out / k_out,
+    or in place where these are None.  `inverse` turns back; it is also the gradient."""
+    one = q if q is not None else k
+    if one is None:
+        raise ValueError("q or k is required")
+    n_tok, hd = one.shape[0], one.shape[2]
+    ptrs, heads = [], []
+    for x, out, what in ((q, q_out, "q"), (k, k_out, "k")):
+        if x is None:
+            if out is not None:
+                raise ValueError(f"{what}_out without {what}")
+            ptrs += [0, 0, 0, 0]
+            heads.append(0)
+            continue
+        if out is None:
+            out = x
+        if x.shape[0] != n_tok or x.dim() != 3 or x.shape[2] != hd or out.shape != x.shape:
+            raise ValueError(f"{what} and {what}_out must be [{n_tok}][heads][{hd}]")
+        ptrs += [*_rows3(x, what), *_rows3(out, what + "_out")]
+        heads.append(x.shape[1])
+    _need(positions, n_tok * 4, "positions", torch.int32)
+    _on_device(stream, q, k, q_out, k_out, positions, table.turns)
+    check(lib().qkv_rope(*ptrs, _dev_ptr(positions, "positions"), table.turns.data_ptr(), table.amplitude, n_tok,
+                         heads[0], heads[1], hd, table.rot_dim, _rope_layout(layout), int(bool(inverse)),
+                         _stream(stream)), "qkv_rope")
+
+
+# ---------------------------------------------------------------------------
+# paged 8-bit cache: e4m3 codes, an exponent per page and kv head
+# ---------------------------------------------------------------------------
+
+def f8_pool(n_pages: int, block_tokens: int, num_kv: int, head_dim: int, device):
+    """Zeroed codes uint8 [n_pages][block_tokens][num_kv][head_dim] and exponents uint8
+    [n_pages][num_kv] of one tensor (keys or values) of a paged 8-bit cache."""
+    return (torch.zeros((n_pages, block_tokens, num_kv, head_dim), dtype=torch.uint8, device=device),
+            torch.zeros((n_pages, num_kv), dtype=torch.uint8, device=device))
+
+
+def _f8_shape(k_pool, v_pool, k_exp, v_exp, block_tables, starts, positions):
+    """(n_pages, block_tokens, num_kv, head_dim, n_slots, max_blocks) of a paged 8-bit batch."""
+    if k_pool.dim() != 4 or v_pool.shape != k_pool.shape:
+        raise ValueError("k_pool and v_pool must be [n_pages][block_tokens][num_kv][head_dim]")
+    n_pages, bt, kv, hd = k_pool.shape
+    if k_exp.shape != (n_pages, kv) or v_exp.shape != (n_pages, kv):
+        raise ValueError(f"k_exp and v_exp must be [{n_pages}][{kv}]")
+    for t, what in ((k_pool, "k_pool"), (v_pool, "v_pool"), (k_exp, "k_exp"), (v_exp, "v_exp")):
+        if t.dtype != torch.uint8:
+            raise ValueError(f"{what} must be torch.uint8, got {t.dtype}")
+    if block_tables.dim() != 2:
+        raise ValueError("block_tables must be [n_slots][max_blocks]")
+    n_slots = block_tables.shape[0]
+    if starts.numel() != n_slots + 1 or positions.numel() != n_slots:
+        raise ValueError(f"starts must hold {n_slots + 1} numbers and positions {n_slots}")
+    return n_pages, bt, kv, hd, n_slots, block_tables.shape[1]
+
+
+def f8_append_kv_paged(k, v, k_pool, v_pool, k_exp, v_exp, block_tables, starts, positions, *, max_tok, q=None,
+                       q_out=None, rope: RopeTable | None = None, layout="half", stream=None) -> None:
+    """Ragged append: rows starts[s] .. starts[s+1]-1 of k and v (fp16 [rows][num_kv][head_dim])
+    go to positions positions[s] .. of slot s.  With `rope` k is rotated first, and q (into
+    q_out, or in place), in the same launch."""
+    n_pages, bt, kv, hd, n_slots, mb = _f8_shape(k_pool, v_pool, k_exp, v_exp, block_tables, starts, positions)
+    rows = k.shape[0]
+    if k.shape != (rows, kv, hd) or v.shape != k.shape:
+        raise ValueError(f"k and v must be [rows][{kv}][{hd}]")
+    qp, nq = (0, 0, 0, 0), 0
+    if q is not None:
+        if rope is None:
+            raise ValueError("q without rope")
+        out = q if q_out is None else q_out
+        if q.dim() != 3 or q.shape[0] != rows or q.shape[2] != hd or out.shape != q.shape:
+            raise ValueError(f"q and q_out must be [{rows}][heads][{hd}]")
+        qp, nq = (*_rows3(q, "q"), *_rows3(out, "q_out")), q.shape[1]
+    elif q_out is not None:
+        raise ValueError("q_out without q")
+    _on_device(stream, k, v, k_pool, v_pool, k_exp, v_exp, block_tables, starts, positions, q, q_out,
+               None if rope is None else rope.turns)
+    check(lib().qkv_f8_append_kv_paged(
+        *_rows3(k, "k"), *_rows3(v, "v"), _dev_ptr(k_pool, "k_pool"), _dev_ptr(v_pool, "v_pool"),
+        _dev_ptr(k_exp, "k_exp"), _dev_ptr(v_exp, "v_exp"), rows, n_slots, max_tok, kv, hd,
+        _i32(block_tables, "block_tables"), mb, bt, n_pages, _i32(starts, "starts"), _i32(positions, "positions"),
+        *qp, nq, rope.turns.data_ptr() if rope is not None else 0, rope.amplitude if rope is not None else 1.0,
+        rope.rot_dim if rope is not None else 0, _rope_layout(layout), _stream(stream)), "qkv_f8_append_kv_paged")
+
+
+def attn_f8_paged_workspace(num_q, num_kv, n_slots, n_rows, max_tok, max_ctx, device, *, head_dim=256) -> torch.Tensor:
+    """Workspace of attn_f8_paged for these numbers (no initialisation needed)."""
+    n = int(lib().qkv_attn_f8_paged_workspace_bytes(num_q, num_kv, head_dim, n_slots, n_rows, max_tok, max_ctx))
+    return torch.empty(n, dtype=torch.uint8, device=device)
+
+
+def attn_f8_paged(q, k_pool, v_pool, k_exp, v_exp, out, workspace, block_tables, starts, positions, *, max_tok,
+                  max_ctx, scale, window=0, sink=0, stream=None) -> None:
+    """Causal attention of ragged query rows (fp16 [rows][num_q][head_dim]; slot s owns rows
+    starts[s] .. starts[s+1]-1 at positions positions[s] ..) over the paged 8-bit cache:
+    decode steps, verify blocks and prompts.  window > 0 limits a query to the last `window`
+    keys and the first `sink`.  Rows past starts[-1] are left alone; out may be q."""
+    n_pages, bt, kv, hd, n_slots, mb = _f8_shape(k_pool, v_pool, k_exp, v_exp, block_tables, starts, positions)
+    rows, nq = q.shape[0], q.shape[1]
+    if q.shape != (rows, nq, hd) or out.shape != q.shape:
+        raise ValueError(f"q and out must be [rows][num_q][{hd}]")
+    if q.dtype not in FP16 or out.dtype not in FP16:
+        raise ValueError(f"q and out must be fp16, got {q.dtype} and {out.dtype}")
+    _on_device(stream, q, k_pool, v_pool, k_exp, v_exp, out, workspace, block_tables, starts, positions)
+    check(lib().qkv_attn_f8_paged(
+        _dev_ptr(q, "q"), _dev_ptr(k_pool, "k_pool"), _dev_ptr(v_pool, "v_pool"), _dev_ptr(k_exp, "k_exp"),
+        _dev_ptr(v_exp, "v_exp"), _dev_ptr(out, "out"), rows, nq, kv, hd, n_slots, max_tok, max_ctx,
+        _i32(block_tables, "block_tables"), mb, bt, n_pages, _i32(starts, "starts"), _i32(positions, "positions"),
+        float(scale), window, sink, _dev_ptr(workspace, "workspace"), workspace.numel() * workspace.element_size(),
+        _stream(stream)), "qkv_attn_f8_paged")
+
+
+# ---------------------------------------------------------------------------
+# pages: sharing, reserving, giving back, compacting
+# ---------------------------------------------------------------------------
+
+class _Plane(ctypes.Structure):
+    _fields_ = [("base", ctypes.c_void_p), ("page_bytes", ctypes.c_size_t)]
+
+
+class PagePlanes:
+    """The pools that page calls copy: contiguous device tensors [n_pages, ...] of any type
+    (keys, values and exponents of every layer).  Kept with the tensors."""
+
+    def __init__(self, tensors):
+        self.tensors = list(tensors)
+        self.n = len(self.tensors)
+        self.n_pages = min((t.shape[0] for t in self.tensors), default=0)
+        self.array = (_Plane * max(1, self.n))()
+        for i, t in enumerate(self.tensors):
+            self.array[i] = _Plane(_dev_ptr(t, f"plane {i}"), t.numel() * t.element_size() // max(1, t.shape[0]))
+        self.ptr = ctypes.addressof(self.array)
+
+
+def page_planes(tensors) -> PagePlanes:
+    """The planes of pages_reserve, pages_compact and pages_copy."""
+    return PagePlanes(tensors)
+
+
+def _page_lists(block_tables, ref_counts, lists, status, stream):
+    """Checks of the page calls: pointers of the lists, their length, and the status pointer."""
+    _on_device(stream, block_tables, ref_counts, status, *(t for t, _ in lists))
+    if block_tables.dim() != 2:
+        raise ValueError("block_tables must be [n_slots][max_blocks]")
+    n = lists[0][0].numel()
+    for t, what in lists:
+        if t.numel() != n:
+            raise ValueError(f"{what} must hold {n} numbers")
+    if status is not None:
+        _need(status, n * 4, "status", torch.int32)
+    return [_i32(t, what) for t, what in lists], n, 0 if status is None else _dev_ptr(status, "status")
+
+
+def _planes_of(planes, n_pages):
+    if planes is None:
+        return 0, 0
+    if planes.n and planes.n_pages < n_pages:
+        raise ValueError(f"the planes hold {planes.n_pages} pages, ref_counts {n_pages}")
+    return planes.ptr, planes.n
+
+
+def _scratch(n_bytes, device, stream) -> torch.Tensor:
+    t = torch.empty(max(1, n_bytes // 4), dtype=torch.int32, device=device)
+    if stream is not None:
+        t.record_stream(stream)
+    return t
+
+
+def pages_fork(block_tables, ref_counts, parents, children, n_tokens, status=None, *, block_tokens,
+               stream=None) -> None:
+    """children[i] shares the pages of the first n_tokens[i] tokens of parents[i] (device int32
+    lists; block_tables int32 [n_slots][max_blocks], ref_counts int32 [n_pages])."""
+    p, n, st = _page_lists(block_tables, ref_counts,
+                           ((parents, "parents"), (children, "children"), (n_tokens, "n_tokens")), status, stream)
+    check(lib().qkv_pages_fork(_i32(block_tables, "block_tables"), *block_tables.shape, block_tokens,
+                               _i32(ref_counts, "ref_counts"), ref_counts.numel(), *p, n, st, _stream(stream)),
+          "qkv_pages_fork")
+
+
+def pages_release(block_tables, ref_counts, slots, keep_tokens, status=None, *, block_tokens, stream=None) -> None:
+    """Gives back the pages of slots[i] past its first keep_tokens[i] tokens."""
+    p, n, st = _page_lists(block_tables, ref_counts, ((slots, "slots"), (keep_tokens, "keep_tokens")), status, stream)
+    check(lib().qkv_pages_release(_i32(block_tables, "block_tables"), *block_tables.shape, block_tokens,
+                                  _i32(ref_counts, "ref_counts"), ref_counts.numel(), *p, n, st, _stream(stream)),
+          "qkv_pages_release")
+
+
+def pages_reserve(block_tables, ref_counts, slots, positions, n_new, status=None, planes=None, *, block_tokens,
+                  max_new, scratch=None, stream=None) -> None:
+    """Pages of its own for tokens positions[i] .. positions[i] + n_new[i] - 1 of slots[i]: missing ones are
+    taken, shared ones replaced (copied in `planes` where they hold earlier rows).  scratch: an int32
+    tensor (allocated here when None) whose first 2n numbers are afterwards the copied pairs."""
+    p, n, st = _page_lists(block_tables, ref_counts,
+                           ((slots, "slots"), (positions, "positions"), (n_new, "n_new")), status, stream)
+    if scratch is None:
+        scratch = _scratch(int(lib().qkv_pages_reserve_scratch_bytes(n, max_new, block_tokens)), block_tables.device,
+                           stream)
+    check(lib().qkv_pages_reserve(_i32(block_tables, "block_tables"), *block_tables.shape, block_tokens,
+                                  _i32(ref_counts, "ref_counts"), ref_counts.numel(), *p, n, max_new, st,
+                                  *_planes_of(planes, ref_counts.numel()), _i32(scratch, "scratch"),
+                                  scratch.numel() * 4, _stream(stream)), "qkv_pages_reserve")
+
+
+def pages_copy(planes: PagePlanes, pairs, *, stream=None) -> None:
+    """Page pairs[i][0] to page pairs[i][1] in every plane (device int32 [n][2])."""
+    if pairs.dim() != 2 or pairs.shape[1] != 2:
+        raise ValueError("pairs must be [n][2]")
+    _on_device(stream, pairs, *planes.tensors[:1])
+    check(lib().qkv_pages_copy(planes.ptr, planes.n, planes.n_pages, _i32(pairs, "pairs"), pairs.shape[0],
+                               _stream(stream)), "qkv_pages_copy")
+
+
+def pages_compact(block_tables, ref_counts, moved, n_used, planes=None, *, scratch=None, stream=None) -> None:
+    """Moves the pages in use to indices 0 .. n_used[0]-1, in planes, tables and counts; moved[p] (int32
+    [n_pages]) is where page p went, -1 if it was free."""
+    if block_tables.dim() != 2:
+        raise ValueError("block_tables must be [n_slots][max_blocks]")
+    n_pages = ref_counts.numel()
+    _need(moved, n_pages * 4, "moved", torch.int32)
+    _need(n_used, 4, "n_used", torch.int32)
+    _on_device(stream, block_tables, ref_counts, moved, n_used, scratch)
+    if scratch is None:
+        scratch = _scratch((n_pages + 2) * 4, block_tables.device, stream)
+    check(lib().qkv_pages_compact(_i32(block_tables, "block_tables"), *block_tables.shape,
+                                  _i32(ref_counts, "ref_counts"), n_pages, _dev_ptr(moved, "moved"),
+                                  _dev_ptr(n_used, "n_used"), *_planes_of(planes, n_pages), _i32(scratch, "scratch"),
+                                  scratch.numel() * 4, _stream(stream)), "qkv_pages_compact")
