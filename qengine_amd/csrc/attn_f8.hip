@@ -39,6 +39,13 @@ __device__ __forceinline__ h2_t cvt2(uint32_t w, float scale, bool hi) {
 __device__ __forceinline__ h8_t join8(h2_t a, h2_t b, h2_t c, h2_t d) {
   return h8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
+// l + the 8 rounded weights
+__device__ __forceinline__ float add8(h8_t w, float l) {
+  const h2_t one = {(_Float16)1.f, (_Float16)1.f};
+#pragma unroll
+  for (int i = 0; i < 4; i++) l = __builtin_amdgcn_fdot2(h2_t{w[2 * i], w[2 * i + 1]}, one, l, false);
+  return l;
+}
 __device__ __forceinline__ float pow2f(uint32_t biased) { return __uint_as_float(biased << 23); }
 __device__ __forceinline__ float max32(float x) {   // with the lane 32 away
   const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -55,6 +62,17 @@ __device__ __forceinline__ float sum32(float x) {
 __device__ __forceinline__ float sum16(float x) {
   const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return __uint_as_float(s[0]) + __uint_as_float(s[1]);
+}
+
+// Block of a key and the key's row in it (bt_magic = floor(2^32 / block_tokens): the product's
+// high half is the quotient or one less).
+struct BlockRow {
+  int b, row;
+};
+__device__ __forceinline__ BlockRow block_row(const F8AttnArgs& p, int key) {
+  const uint32_t q = __umulhi((uint32_t)key, p.bt_magic), r = (uint32_t)key - q * (uint32_t)p.block_tokens;
+  const bool more = r >= (uint32_t)p.block_tokens;
+  return {(int)(more ? q + 1 : q), (int)(more ? r - (uint32_t)p.block_tokens : r)};
 }
 
 // A slot's tokens: rows t0 .. t0+n-1 of q at positions pos0 .. (n = 0: none)
@@ -127,11 +145,11 @@ __device__ __forceinline__ int block_scan(int v, int* lds, int& sum) {   // incl
   return v + before;
 }
 
-// The unit line of one head; workgroup 0 leaves its prefix for the merge.
-template <int ROWS, int KT, int PER, int THREADS>
+// The units of one head's line; for KEEP workgroup 0 leaves its prefix for the merge.
+template <int ROWS, int KT, int PER, int THREADS, bool KEEP>
 __device__ __forceinline__ int line_units(const F8AttnArgs& p, int gqa, int* lds) {
   const int entries = p.n_slots * p.slot_tiles;
-  const bool keep = blockIdx.x == 0;
+  const bool keep = KEEP && blockIdx.x == 0;
   int base = 0;
   for (int c = 0; c < entries; c += THREADS) {
     const int x = c + threadIdx.x;
@@ -199,7 +217,7 @@ __global__ __launch_bounds__(256, NR == 1 ? 2 : 1) void f8_few_kernel(F8AttnArgs
   const int m = lane & 15, g = lane >> 4;
   const int gqa = p.num_q / p.num_kv;
 
-  const int total = line_units<ROWS, KT, PER, THREADS>(p, gqa, lds);
+  const int total = line_units<ROWS, KT, PER, THREADS, true>(p, gqa, lds);
   const long all = (long)total * p.num_kv;
   const int grp = blockIdx.x, parts = part_count(all, p.groups);
   if (grp >= parts) return;
@@ -370,8 +388,8 @@ __global__ __launch_bounds__(256, NR == 1 ? 2 : 1) void f8_few_kernel(F8AttnArgs
 #pragma unroll
         for (int i = 0; i < 8; i++) {
           pb[nr][i] = (_Float16)__builtin_amdgcn_exp2f(sc[nr][i >> 2][i & 3] - base);
-          ls[nr] += (float)pb[nr][i];
         }
+        ls[nr] = add8(pb[nr], ls[nr]);
       }
       // ---- O^T += V^T P^T: dims m * HD/16 + 4 d + j
 #pragma unroll
@@ -466,34 +484,47 @@ __global__ __launch_bounds__(256, NR == 1 ? 2 : 1) void f8_few_kernel(F8AttnArgs
 // ---------------------------------------------------------------------------
 // many rows: prompts and chunks
 // ---------------------------------------------------------------------------
-// Waves of 32 rows share fp16 K and V tiles in LDS, converted once by the workgroup
-// from the next tile's codes (in registers while the present tile is computed).
-// V is stored by dim, four keys to 8 bytes, in the order that the scores' lanes hold
-// them.  Pads and the key swizzle keep 16-byte reads of 16 lanes on distinct banks.
-template <int HD, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2))) void f8_many_kernel(F8AttnArgs p) {
+// Eight waves of 32 rows share fp16 K and V tiles in LDS.  The codes of the tile after
+// next go from memory straight to LDS (no registers: the sums and queries of a wave fill
+// three quarters of them); the workgroup converts the next tile's once for all rows, each
+// wave the rows that it loaded itself, so only its own loads are waited for.  V is stored
+// by dim, four keys to 8 bytes, in the order that the scores' lanes hold them.  Pads
+// keep 16-byte reads of 16 lanes on distinct banks, at constant offsets of one address.
+typedef __attribute__((address_space(3))) void lds_void;
+typedef __attribute__((address_space(1))) const void glb_void;
+typedef __attribute__((address_space(4))) const int32_t const_i32;
+
+template <int HD>
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void f8_many_kernel(F8AttnArgs p) {
+  constexpr int WAVES = 8, ROWS = 32 * WAVES, THREADS = 64 * WAVES, PER = 1;
   constexpr int KT = 8192 / HD;              // 32 or 64 keys: 8 KB of codes
-  constexpr int ROWS = 32 * WAVES, THREADS = 64 * WAVES, PER = 1;
-  constexpr int NL = 512 / THREADS;          // loads of a thread for 8 KB
+  constexpr int WK = KT / WAVES;             // keys that a wave loads and converts
+  constexpr int LPR = HD / 16;               // lanes of a key row's load
   constexpr int VP = KT * 2;                 // bytes of a dim's values
   constexpr int VPAD = KT == 32 ? 4 : 2;     // dims per 16-byte pad
-  constexpr int KB = KT * HD * 2, VB = HD * VP + HD / VPAD * 16;
+  constexpr int KP = HD * 2 + 16;            // bytes of a key's row
+  constexpr int KB = KT * KP, VB = HD * VP + HD / VPAD * 16;
   __shared__ __align__(16) uint8_t tile_lds[2][KB + VB];
+  __shared__ __align__(16) uint8_t raw_lds[2][8192];
+  __shared__ __align__(16) int gone_lds[2][WAVES];   // per tile and wave: its keys have no page
   __shared__ int lds[WAVES];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 31, hh = lane >> 5;
   const int gqa = p.num_q / p.num_kv;
 
-  const int total = line_units<ROWS, KT, PER, THREADS>(p, gqa, lds);
+  const int total = line_units<ROWS, KT, PER, THREADS, false>(p, gqa, lds);
   const long all = (long)total * p.num_kv;
-  const int grp = blockIdx.x, parts = part_count(all, p.groups);
+  if (blockIdx.x == 0 && tid == 0) *reinterpret_cast<long*>(p.cuts + 4 * p.groups) = all;
+  // neighbouring parts (the same head's keys) on one XCD, whose L2 holds their tiles
+  const int parts = part_count(all, p.groups);
+  const int grp = p.groups % 8 ? (int)blockIdx.x : (int)(blockIdx.x % 8) * (p.groups / 8) + (int)blockIdx.x / 8;
   if (grp >= parts) return;
   long u = part_begin(all, grp, parts);
   const long u_end = part_begin(all, grp + 1, parts);
   int h = (int)(u / total);
   Part at = line_find<ROWS, KT, PER, THREADS>(p, gqa, total, (int)(u - (long)h * total), lds);
   bool first_seg = true;
-  const long key_bytes = (long)p.num_kv * HD;
+  const uint32_t key_bytes = (uint32_t)p.num_kv * HD;
   const int entries = p.n_slots * p.slot_tiles;
 
   while (u < u_end) {
@@ -516,11 +547,12 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
     const int pos = sl.pos0 + tok;
     const int pos_lo = sl.pos0 + min(row_w, rows - 1) / gqa, pos_hi = sl.pos0 + min(row_w + 31, rows - 1) / gqa;
     const bool live = row_w < rows;
+    const long out_row = ((long)(sl.t0 + tok) * p.num_q + h * gqa + (row - tok * gqa)) * HD;
 
     h8_t qf[HD / 16];
     float sl2 = p.scale_log2;
     {
-      const uint16_t* src = p.q + ((long)(sl.t0 + tok) * p.num_q + h * gqa + (row - tok * gqa)) * HD + 8 * hh;
+      const uint16_t* src = p.q + out_row + 8 * hh;
 #pragma unroll
       for (int i = 0; i < HD / 16; i++) qf[i] = *reinterpret_cast<const h8_t*>(src + 16 * i);
       // (a negative scale is carried by the query, so that raw maxima serve)
@@ -535,93 +567,95 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
     for (int d = 0; d < HD / 32; d++) acc[d] = f16x_t{};
     float mx = -INFINITY, ls = 0.f;
 
-    const int32_t* table = p.tables + (long)s * p.max_blocks;
-    auto page_of = [&](int key) {
-      const int b = key / p.block_tokens;
+    const const_i32* table = (const const_i32*)(p.tables + (long)s * p.max_blocks);
+    auto page_of = [&](int key) {   // (key the same in the whole wave)
+      const int b = block_row(p, key).b;
       const int pg = key < rt.end && b < p.max_blocks ? table[b] : -1;
       return pg >= 0 && pg < p.n_pages ? pg : -1;
     };
-    // a thread's part of a tile: 16 bytes of a key row, and 4 dims of 4 keys
-    auto k_key = [&](int l) { return (tid + l * THREADS) / (HD / 16); };
-    const int vl = lane & (HD / 4 - 1);                                  // dims 4 vl ..
-    auto v_quad = [&](int l) { return (tid + l * THREADS) / (HD / 4); };   // keys 4 quad ..
-    int kpg[NL], vpg[NL];       // pages of the tile after next
-    u4_t kr[NL];
-    uint32_t vr[NL][4];
-    float ksc[NL], vsc[NL];
-    auto lookup = [&](int v) {
-      const int key0 = rt.key0(v, KT);
-#pragma unroll
-      for (int l = 0; l < NL; l++) {
-        kpg[l] = page_of(key0 + k_key(l));
-        vpg[l] = page_of(key0 + 4 * v_quad(l));
-      }
-    };
+    // this wave's WK keys of a tile lie in one page (pages are whole sixteens)
+    float ksc = 0.f, vsc = 0.f;      // their exponents' factors
+    int loaded = -1;                 // their page
+    int ahead = -1;                  // the page of the tile after that
+    auto lookup = [&](int v) { ahead = page_of(rt.key0(v, KT) + wave * WK); };
+    const uint32_t lane_off = (uint32_t)(lane / LPR) * key_bytes + (uint32_t)(lane % LPR) * 16;
     auto fetch = [&](int v) {
-      const int key0 = rt.key0(v, KT);
-#pragma unroll
-      for (int l = 0; l < NL; l++) {
-        const int key = key0 + k_key(l), slot = (tid + l * THREADS) % (HD / 16);
-        const int pk = max(kpg[l], 0);
-        kr[l] = *reinterpret_cast<const u4_t*>(p.k_pool + ((long)pk * p.block_tokens + key % p.block_tokens) * key_bytes +
-                                               (long)h * HD + 16 * slot);
-        ksc[l] = kpg[l] >= 0 ? pow2f(p.k_exp[(long)pk * p.num_kv + h]) : 0.f;
-        const int vk = key0 + 4 * v_quad(l), pv = max(vpg[l], 0);
-        const uint8_t* src = p.v_pool + ((long)pv * p.block_tokens + vk % p.block_tokens) * key_bytes + (long)h * HD + 4 * vl;
-        vsc[l] = vpg[l] >= 0 ? pow2f(p.v_exp[(long)pv * p.num_kv + h]) : 0.f;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const uint32_t w = *reinterpret_cast<const uint32_t*>(src + i * key_bytes);
-          vr[l][i] = vpg[l] >= 0 && vk + i < rt.end ? w : 0u;   // (rows past the last key: anything)
-        }
-        if (kpg[l] < 0) kr[l] = u4_t{0, 0, 0, 0};
-      }
+      loaded = ahead;
+      const int pg = max(ahead, 0), row0 = block_row(p, rt.key0(v, KT) + wave * WK).row;
+      const long base = ((long)pg * p.block_tokens + row0) * key_bytes + (long)h * HD;
+      __builtin_amdgcn_global_load_lds((glb_void*)(p.k_pool + base + lane_off), (lds_void*)(raw_lds[0] + wave * 1024), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((glb_void*)(p.v_pool + base + lane_off), (lds_void*)(raw_lds[1] + wave * 1024), 16, 0, 0);
+      ksc = pow2f(p.k_exp[(long)pg * p.num_kv + h]);
+      vsc = pow2f(p.v_exp[(long)pg * p.num_kv + h]);
     };
-    auto stage = [&](int buf) {
+    const int vl = lane % (HD / 4), vq = lane / (HD / 4);   // value dims 4 vl .., keys 4 vq .. of the wave's
+    auto stage = [&](int v, int buf) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the codes are in LDS
+      u4_t kr = *reinterpret_cast<const u4_t*>(raw_lds[0] + wave * 1024 + lane * 16);
+      uint32_t vr[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        vr[i] = *reinterpret_cast<const uint32_t*>(raw_lds[1] + wave * 1024 + (4 * vq + i) * HD + vl * 4);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // ... and out of it again: the next may land
+      const int key0 = rt.key0(v, KT) + wave * WK;
+      // keys that do not exist are zeros (a page past the last key holds anything)
+      if (loaded < 0 || key0 + WK > rt.end) {
+        if (loaded < 0 || key0 + lane / LPR >= rt.end) kr = u4_t{0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          if (loaded < 0 || key0 + 4 * vq + i >= rt.end) vr[i] = 0;
+      }
+      if (lane == 0) gone_lds[buf][wave] = loaded < 0;
       uint8_t* kb = tile_lds[buf];
       uint8_t* vb = kb + KB;
+      const int key = wave * WK + lane / LPR, slot = lane % LPR;
 #pragma unroll
-      for (int l = 0; l < NL; l++) {
-        const int key = k_key(l), slot = (tid + l * THREADS) % (HD / 16);
-        const float f = ksc[l];
+      for (int e = 0; e < 2; e++)
+        *reinterpret_cast<h8_t*>(kb + key * KP + slot * 32 + e * 16) =
+            join8(cvt2(kr[2 * e], ksc, false), cvt2(kr[2 * e], ksc, true), cvt2(kr[2 * e + 1], ksc, false),
+                  cvt2(kr[2 * e + 1], ksc, true));
+      const int q = wave * (WK / 4) + vq;
+      // quad q of 16 keys (q & 3 = 2 a + half): 16-byte slot 2 (q / 4) + half, its part a
+      const int at8 = ((q >> 2) * 2 + (q & 1)) * 16 + ((q >> 1) & 1) * 8;
+      uint32_t w[2][2];
 #pragma unroll
-        for (int e = 0; e < 2; e++) {
-          const h8_t x = join8(cvt2(kr[l][2 * e], f, false), cvt2(kr[l][2 * e], f, true),
-                               cvt2(kr[l][2 * e + 1], f, false), cvt2(kr[l][2 * e + 1], f, true));
-          *reinterpret_cast<h8_t*>(kb + key * (HD * 2) + (((2 * slot + e) ^ (key & 15)) * 16)) = x;
-        }
-        const int q = v_quad(l);
-        // quad q of 16 keys (q & 3 = 2 a + half): 16-byte slot 2 (q / 4) + half, its part a
-        const int at8 = ((q >> 2) * 2 + (q & 1)) * 16 + ((q >> 1) & 1) * 8;
-        uint32_t w[2][2];
+      for (int k = 0; k < 2; k++) {
+        w[k][0] = __builtin_amdgcn_perm(vr[2 * k + 1], vr[2 * k], 0x05010400u);
+        w[k][1] = __builtin_amdgcn_perm(vr[2 * k + 1], vr[2 * k], 0x07030602u);
+      }
 #pragma unroll
-        for (int k = 0; k < 2; k++) {
-          w[k][0] = __builtin_amdgcn_perm(vr[l][2 * k + 1], vr[l][2 * k], 0x05010400u);
-          w[k][1] = __builtin_amdgcn_perm(vr[l][2 * k + 1], vr[l][2 * k], 0x07030602u);
-        }
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-          const int dim = 4 * vl + j;
-          const u2_t x = {__builtin_bit_cast(uint32_t, cvt2(w[0][j >> 1], vsc[l], j & 1)),
-                          __builtin_bit_cast(uint32_t, cvt2(w[1][j >> 1], vsc[l], j & 1))};
-          *reinterpret_cast<u2_t*>(vb + dim * VP + dim / VPAD * 16 + at8) = x;
+      for (int j = 0; j < 4; j++) {
+        const int dim = 4 * vl + j;
+        *reinterpret_cast<u2_t*>(vb + dim * VP + dim / VPAD * 16 + at8) =
+            u2_t{__builtin_bit_cast(uint32_t, cvt2(w[0][j >> 1], vsc, j & 1)),
+                 __builtin_bit_cast(uint32_t, cvt2(w[1][j >> 1], vsc, j & 1))};
+      }
+    };
+    // the next tile into the other buffer, then the loads of the one after it
+    auto advance = [&](int v, int buf) {
+      if (v + 1 < v1) {
+        stage(v + 1, buf ^ 1);
+        if (v + 2 < v1) {
+          fetch(v + 2);
+          if (v + 3 < v1) lookup(v + 3);
         }
       }
     };
 
     lookup(v0);
+    __syncthreads();   // (the last segment's tiles are done with)
     fetch(v0);
     if (v0 + 1 < v1) lookup(v0 + 1);
-    __syncthreads();   // (the last segment's tiles are done with)
-    stage(0);
-    if (v0 + 1 < v1) fetch(v0 + 1);
-    if (v0 + 2 < v1) lookup(v0 + 2);
+    stage(v0, 0);
+    if (v0 + 1 < v1) {
+      fetch(v0 + 1);
+      if (v0 + 2 < v1) lookup(v0 + 2);
+    }
     __syncthreads();
     for (int v = v0; v < v1; v++) {
       const int buf = (v - v0) & 1;
-      if (v + 1 < v1) stage(buf ^ 1);
-      if (v + 2 < v1) fetch(v + 2);
-      if (v + 3 < v1) lookup(v + 3);
+      // one wave of each SIMD converts ahead of its products, the other after them
+      if (wave < 4) advance(v, buf);
       const int key0 = rt.key0(v, KT);
       // a wave none of whose rows sees the tile sits it out
       const bool out = !live || key0 > pos_hi ||
@@ -629,21 +663,33 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
       if (!out) {
         const uint8_t* kb = tile_lds[buf];
         const uint8_t* vb = kb + KB;
+        int gone = 0;
+#pragma unroll
+        for (int w = 0; w < WAVES; w++) gone |= gone_lds[buf][w];
+        const bool pages = __builtin_amdgcn_readfirstlane(gone) == 0;
 #pragma unroll
         for (int kh = 0; kh < KT / 32; kh++) {
           const int k0 = key0 + 32 * kh;
+          const uint8_t* krow = kb + 32 * kh * KP + c * KP + hh * 16;
+          auto k_operand = [&](int i) { return *reinterpret_cast<const h8_t*>(krow + i * 32); };
+          constexpr int NK = HD / 16;
           f16x_t sd = f16x_t{};
-          {
-            const uint8_t* krow = kb + (32 * kh + c) * (HD * 2);
+          h8_t ka[4];
 #pragma unroll
-            for (int i = 0; i < HD / 16; i++) {
-              const h8_t a = *reinterpret_cast<const h8_t*>(krow + (((2 * i + hh) ^ (c & 15)) * 16));
-              sd = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qf[i], sd, 0, 0, 0);
-            }
+          for (int i = 0; i < 4; i++) ka[i] = k_operand(i);
+#pragma unroll
+          for (int i = 0; i < NK; i++) {
+            sd = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka[i & 3], qf[i], sd, 0, 0, 0);
+            if (i + 4 < NK) ka[i & 3] = k_operand(i + 4);
           }
-          // pages may be absent anywhere: which of the two 16-key halves exist
-          const int pa = page_of(k0), pb2 = page_of(k0 + 16);
-          const bool whole = pa >= 0 && pb2 >= 0 && k0 + 31 <= pos_lo && k0 + 32 <= rt.end &&
+          __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);     // four reads ahead
+#pragma unroll
+          for (int i = 0; i < NK - 4; i++) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+          }
+          __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
+          const bool whole = pages && k0 + 31 <= pos_lo && k0 + 32 <= rt.end &&
                              (p.window <= 0 || k0 > pos_hi - p.window || k0 + 32 <= p.sink);
           float t = -INFINITY, f = sl2;
           if (whole) {
@@ -651,11 +697,11 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
             for (int x = 0; x < 16; x++) t = fmaxf(t, sd[x]);
             t = max32(t) * sl2;
           } else {
+            const bool pa = page_of(k0) >= 0, pb = page_of(k0 + 16) >= 0;
 #pragma unroll
             for (int x = 0; x < 16; x++) {
               const int key = k0 + 8 * (x >> 2) + 4 * hh + (x & 3);
-              const bool there = x < 8 ? pa >= 0 : pb2 >= 0;
-              sd[x] = there && sees(key, pos, rt.end, p.window, p.sink) ? sd[x] * sl2 : -INFINITY;
+              sd[x] = (x < 8 ? pa : pb) && sees(key, pos, rt.end, p.window, p.sink) ? sd[x] * sl2 : -INFINITY;
               t = fmaxf(t, sd[x]);
             }
             t = max32(t);
@@ -675,26 +721,29 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
             h8_t w;
 #pragma unroll
             for (int i = 0; i < 8; i++) w[i] = (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(sd[8 * sg + i], f, -base));
-#pragma unroll
-            for (int i = 0; i < 8; i++) ls += (float)w[i];
+            ls = add8(w, ls);
 #pragma unroll
             for (int d = 0; d < HD / 32; d++) {
-              const int dim = 32 * d + c;
-              const h8_t a = *reinterpret_cast<const h8_t*>(vb + dim * VP + dim / VPAD * 16 + ((2 * kh + sg) * 2 + hh) * 16);
+              const h8_t a = *reinterpret_cast<const h8_t*>(vb + c * VP + c / VPAD * 16 + hh * 16 +
+                                                            d * (32 * VP + 32 / VPAD * 16) + (2 * kh + sg) * 32);
               acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, w, acc[d], 0, 0, 0);
             }
           }
         }
       }
+      if (wave >= 4) advance(v, buf);
       __syncthreads();
     }
 
     ls = sum32(ls);
     const bool complete = n_u == rt.tiles;
+    // where the part begins, for the merge: row tile (-1: at its first unit), head, unit, units
+    if (first_seg && tid == 0)
+      *reinterpret_cast<int4*>(p.cuts + 4 * grp) = make_int4(v0 > 0 ? at.entry : -1, h, v0, rt.tiles);
     if (row_w + c < rows) {
       if (complete) {
         const float inv = ls > 0.f ? 1.f / ls : 0.f;
-        uint16_t* o = p.out + ((long)(sl.t0 + tok) * p.num_q + h * gqa + (row - tok * gqa)) * HD + 4 * hh;
+        uint16_t* o = p.out + out_row + 4 * hh;
 #pragma unroll
         for (int d = 0; d < HD / 32; d++)
 #pragma unroll
@@ -724,18 +773,65 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
   }
 }
 
+// The rows of the row tiles that parts cut: a wave per row, the workgroups of a part's cut only
+// if the tile begins in the part before (each tile once).
+template <int HD>
+__global__ __launch_bounds__(256) void f8_cut_merge_kernel(F8AttnArgs p) {
+  constexpr int E = HD / 64, ROWS = 256, RG = ROWS / 4;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int grp = blockIdx.x / RG + 1;
+  const long all = *reinterpret_cast<const long*>(p.cuts + 4 * p.groups);
+  const int parts = part_count(all, p.groups);
+  if (grp >= parts) return;
+  const int4 cut = *reinterpret_cast<const int4*>(p.cuts + 4 * grp);
+  const int entry = cut.x, h = cut.y, v0 = cut.z, tiles = cut.w;
+  if (entry < 0) return;
+  const long x0 = part_begin(all, grp, parts) - v0;
+  const long before = part_begin(all, grp - 1, parts);
+  if (before > x0) return;   // an earlier cut is in this tile
+  int n = 2;
+  while (part_begin(all, grp + n - 1, parts) < x0 + tiles) n++;
+  const int r0 = 2 * (grp - 1) + (before == x0 ? 0 : 1);
+  auto rec_of = [&](int i) { return i == 0 ? r0 : 2 * (grp - 1 + i); };
+  const int s = entry / p.slot_tiles, gqa = p.num_q / p.num_kv;
+  const Slot sl = slot_of(p, s);
+  const int row = (blockIdx.x % RG) * 4 + wave, r = (entry - s * p.slot_tiles) * ROWS + row;
+  if (r >= sl.n * gqa) return;
+  float M = -INFINITY;
+  for (int i = 0; i < n; i++) {
+    const f2_t ml = *reinterpret_cast<const f2_t*>(p.rec_ml + ((long)rec_of(i) * p.rec_rows + row) * 2);
+    if (ml[1] > 0.f) M = fmaxf(M, ml[0]);
+  }
+  if (M == -INFINITY) M = 0.f;
+  float L = 0.f, o[E] = {};
+#pragma unroll 4
+  for (int i = 0; i < n; i++) {
+    const long at = (long)rec_of(i) * p.rec_rows + row;
+    const f2_t ml = *reinterpret_cast<const f2_t*>(p.rec_ml + at * 2);
+    const float w = ml[1] > 0.f ? __builtin_amdgcn_exp2f(ml[0] - M) : 0.f;
+    L += w * ml[1];
+#pragma unroll
+    for (int e = 0; e < E; e++) o[e] = __builtin_fmaf(w, p.rec_o[at * HD + lane * E + e], o[e]);
+  }
+  const float inv = L > 0.f ? 1.f / L : 0.f;
+  const int t = r / gqa;
+  uint16_t* dst = p.out + ((long)(sl.t0 + t) * p.num_q + h * gqa + (r - t * gqa)) * HD + lane * E;
+#pragma unroll
+  for (int e = 0; e < E; e += 2)
+    *reinterpret_cast<uint32_t*>(dst + e) = f2h(o[e] * inv) | (f2h(o[e + 1] * inv) << 16);
+}
+
 // ---------------------------------------------------------------------------
 // merge of the row tiles that were cut
 // ---------------------------------------------------------------------------
-// One wave per row at a time, WPR waves of a workgroup on the same row (each takes
-// every WPR-th record).
-template <int HD, int WPR>
-__global__ __launch_bounds__(256) void f8_merge_kernel(F8AttnArgs p, int rows_tile) {
+// A workgroup per row, each wave every fourth record.
+template <int HD>
+__global__ __launch_bounds__(256) void f8_merge_kernel(F8AttnArgs p) {
   constexpr int E = HD / 64;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int entries = p.n_slots * p.slot_tiles;
-  const int row_groups = (rows_tile * WPR + 3) / 4;
-  const int tile = blockIdx.x / row_groups, entry = tile % entries, h = tile / entries;
+  const int tile = blockIdx.x / p.rec_rows, row = blockIdx.x - tile * p.rec_rows;
+  const int entry = tile % entries, h = tile / entries;
   const int total = p.pre[entries], a = p.pre[entry], b = p.pre[entry + 1];
   if (a == b) return;
   const long all = (long)total * p.num_kv, x0 = (long)h * total + a, x1 = (long)h * total + b;
@@ -754,57 +850,50 @@ __global__ __launch_bounds__(256) void f8_merge_kernel(F8AttnArgs p, int rows_ti
   auto rec_of = [&](int i) { return i == 0 ? r0 : 2 * (g0 + i); };
   const int s = entry / p.slot_tiles, gqa = p.num_q / p.num_kv;
   const Slot sl = slot_of(p, s);
-  const int base_row = (entry - s * p.slot_tiles) * rows_tile;
-  const int row = (blockIdx.x - tile * row_groups) * (4 / WPR) + wave / WPR;
-  const bool live = row < rows_tile && base_row + row < sl.n * gqa;
+  if (row >= sl.n * gqa) return;
 
   float M = -INFINITY, L = 0.f;
   float o[E] = {};
-  if (live) {
-    for (int i0 = 0; i0 < n; i0 += 64) {
-      if (i0 + lane < n) {
-        const f2_t r = *reinterpret_cast<const f2_t*>(p.rec_ml + ((long)rec_of(i0 + lane) * p.rec_rows + row) * 2);
-        if (r[1] > 0.f) M = fmaxf(M, r[0]);
-      }
+  for (int i0 = 0; i0 < n; i0 += 64) {
+    if (i0 + lane < n) {
+      const f2_t r = *reinterpret_cast<const f2_t*>(p.rec_ml + ((long)rec_of(i0 + lane) * p.rec_rows + row) * 2);
+      if (r[1] > 0.f) M = fmaxf(M, r[0]);
     }
-    M = wave_max(M);
-    if (M == -INFINITY) M = 0.f;
+  }
+  M = wave_max(M);
+  if (M == -INFINITY) M = 0.f;
 #pragma unroll 8
-    for (int i = wave % WPR; i < n; i += WPR) {
-      const long at = (long)rec_of(i) * p.rec_rows + row;
-      const f2_t r = *reinterpret_cast<const f2_t*>(p.rec_ml + at * 2);
-      const float w = r[1] > 0.f ? __builtin_amdgcn_exp2f(r[0] - M) : 0.f;
-      L += w * r[1];
-      const float* src = p.rec_o + at * HD + lane * E;
-      if constexpr (E == 4) {
-        const f4_t x = *reinterpret_cast<const f4_t*>(src);
+  for (int i = wave; i < n; i += 4) {
+    const long at = (long)rec_of(i) * p.rec_rows + row;
+    const f2_t r = *reinterpret_cast<const f2_t*>(p.rec_ml + at * 2);
+    const float w = r[1] > 0.f ? __builtin_amdgcn_exp2f(r[0] - M) : 0.f;
+    L += w * r[1];
+    const float* src = p.rec_o + at * HD + lane * E;
+    if constexpr (E == 4) {
+      const f4_t x = *reinterpret_cast<const f4_t*>(src);
 #pragma unroll
-        for (int e = 0; e < 4; e++) o[e] = __builtin_fmaf(w, x[e], o[e]);
-      } else {
-        const f2_t x = *reinterpret_cast<const f2_t*>(src);
+      for (int e = 0; e < 4; e++) o[e] = __builtin_fmaf(w, x[e], o[e]);
+    } else {
+      const f2_t x = *reinterpret_cast<const f2_t*>(src);
 #pragma unroll
-        for (int e = 0; e < 2; e++) o[e] = __builtin_fmaf(w, x[e], o[e]);
-      }
+      for (int e = 0; e < 2; e++) o[e] = __builtin_fmaf(w, x[e], o[e]);
     }
   }
-  if constexpr (WPR > 1) {
-    __shared__ float part[4][64][E + 1];
+  __shared__ float part[4][64][E + 1];
 #pragma unroll
-    for (int e = 0; e < E; e++) part[wave][lane][e] = o[e];
-    part[wave][lane][E] = L;
-    __syncthreads();
-    if (wave % WPR != 0) return;
+  for (int e = 0; e < E; e++) part[wave][lane][e] = o[e];
+  part[wave][lane][E] = L;
+  __syncthreads();
+  if (wave != 0) return;
 #pragma unroll
-    for (int w = 1; w < WPR; w++) {
+  for (int w = 1; w < 4; w++) {
 #pragma unroll
-      for (int e = 0; e < E; e++) o[e] += part[wave + w][lane][e];
-      L += part[wave + w][lane][E];
-    }
+    for (int e = 0; e < E; e++) o[e] += part[w][lane][e];
+    L += part[w][lane][E];
   }
-  if (!live) return;
   const float inv = L > 0.f ? 1.f / L : 0.f;
-  const int r = base_row + row, t = r / gqa;
-  uint16_t* dst = p.out + ((long)(sl.t0 + t) * p.num_q + h * gqa + (r - t * gqa)) * HD + lane * E;
+  const int t = row / gqa;
+  uint16_t* dst = p.out + ((long)(sl.t0 + t) * p.num_q + h * gqa + (row - t * gqa)) * HD + lane * E;
   if constexpr (E == 4)
     *reinterpret_cast<u2_t*>(dst) = u2_t{f2h(o[0] * inv) | (f2h(o[1] * inv) << 16), f2h(o[2] * inv) | (f2h(o[3] * inv) << 16)};
   else
@@ -814,8 +903,6 @@ __global__ __launch_bounds__(256) void f8_merge_kernel(F8AttnArgs p, int rows_ti
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
-constexpr int kManyWaves = 8;
-
 F8AttnPlan f8_attn_plan(int num_q, int num_kv, int head_dim, int n_slots, long q_rows, int max_tok, int max_ctx) {
   F8AttnPlan x{};
   const long rows = (long)max_tok * (num_q / num_kv);
@@ -823,7 +910,7 @@ F8AttnPlan f8_attn_plan(int num_q, int num_kv, int head_dim, int n_slots, long q
   x.row_tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
   long units;   // most units of all heads
   if (x.many) {
-    const int tile_rows = 32 * kManyWaves, kt = 8192 / head_dim;
+    const int tile_rows = 256, kt = 8192 / head_dim;
     x.slot_tiles = (int)((rows + tile_rows - 1) / tile_rows);
     x.rec_rows = tile_rows;
     // (a slot has at most one row tile that is not full)
@@ -838,7 +925,8 @@ F8AttnPlan f8_attn_plan(int num_q, int num_kv, int head_dim, int n_slots, long q
     x.groups = (int)std::min<long>(units, x.row_tiles == 1 ? 512 : 256);
     x.merges = max_ctx > 128 || units > x.groups;
   }
-  const size_t pre = (((size_t)n_slots * x.slot_tiles + 1) * 4 + 255) / 256 * 256;
+  const size_t ints = x.many ? 4 * (size_t)x.groups + 4 : (size_t)n_slots + 1;
+  const size_t pre = (ints * 4 + 255) / 256 * 256;
   const size_t recs = 2 * (size_t)x.groups * x.rec_rows;
   x.ml_off = pre;
   x.o_off = pre + (recs * 8 + 255) / 256 * 256;
@@ -850,7 +938,7 @@ template <int HD>
 static void launch_f8(const F8AttnArgs& a, const F8AttnPlan& x, hipStream_t stream) {
   const dim3 grid((unsigned)x.groups);
   if (x.many)
-    hipLaunchKernelGGL((f8_many_kernel<HD, kManyWaves>), grid, dim3(64 * kManyWaves), 0, stream, a);
+    hipLaunchKernelGGL((f8_many_kernel<HD>), grid, dim3(512), 0, stream, a);
   else if (x.row_tiles == 1)
     hipLaunchKernelGGL((f8_few_kernel<HD, 1>), grid, dim3(256), 0, stream, a);
   else if (x.row_tiles == 2)
@@ -858,11 +946,12 @@ static void launch_f8(const F8AttnArgs& a, const F8AttnPlan& x, hipStream_t stre
   else
     hipLaunchKernelGGL((f8_few_kernel<HD, 4>), grid, dim3(256), 0, stream, a);
   if (!x.merges) return;
-  const unsigned tiles = (unsigned)(a.n_slots * a.slot_tiles * a.num_kv);
-  if (x.many)
-    hipLaunchKernelGGL((f8_merge_kernel<HD, 1>), dim3(tiles * (unsigned)(x.rec_rows / 4)), dim3(256), 0, stream, a, x.rec_rows);
-  else
-    hipLaunchKernelGGL((f8_merge_kernel<HD, 4>), dim3(tiles * (unsigned)x.rec_rows), dim3(256), 0, stream, a, x.rec_rows);
+  if (x.many) {
+    if (x.groups > 1)
+      hipLaunchKernelGGL((f8_cut_merge_kernel<HD>), dim3((unsigned)(x.groups - 1) * 64), dim3(256), 0, stream, a);
+  } else {
+    hipLaunchKernelGGL((f8_merge_kernel<HD>), dim3((unsigned)(a.n_slots * a.num_kv * x.rec_rows)), dim3(256), 0, stream, a);
+  }
 }
 
 hipError_t launch_f8_attn(const F8AttnArgs& a, const F8AttnPlan& plan, int head_dim, hipStream_t stream) {

@@ -229,7 +229,7 @@ int qkv_attn_f8_paged(const uint16_t* q, const uint8_t* k_pool, const uint8_t* v
   a.tables = block_tables;
   a.starts = starts;
   a.positions = positions;
-  a.pre = reinterpret_cast<int*>(ws);
+  a.pre = a.cuts = reinterpret_cast<int*>(ws);
   a.rec_ml = reinterpret_cast<float*>(ws + x.ml_off);
   a.rec_o = reinterpret_cast<float*>(ws + x.o_off);
   a.rows = n_rows;
@@ -246,6 +246,7 @@ int qkv_attn_f8_paged(const uint16_t* q, const uint8_t* k_pool, const uint8_t* v
   a.slot_tiles = x.slot_tiles;
   a.rec_rows = x.rec_rows;
   a.groups = x.groups;
+  a.bt_magic = (uint32_t)((1ull << 32) / (uint64_t)block_tokens);
   a.scale_log2 = scale * 1.4426950408889634f;
   return launch_status(qkv::launch_f8_attn(a, x, head_dim, stream));
 }

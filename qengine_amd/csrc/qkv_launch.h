@@ -171,7 +171,9 @@ struct F8AttnArgs {
   const int32_t* tables;
   const int32_t* starts;
   const int32_t* positions;
-  int* pre;                  // workspace: unit prefix of the row tiles, [tiles + 1]
+  int* pre;                  // workspace: unit prefix of the slots, [n_slots + 1] (few rows)
+  int* cuts;                 // workspace, the same place: [groups][4] where each part begins, then
+                             // the units of all heads (many rows)
   float* rec_ml;             // workspace: {m (log2 units), l} of a partial row
   float* rec_o;              // workspace: its unnormalised sums
   long rows;
@@ -179,6 +181,7 @@ struct F8AttnArgs {
   int slot_tiles;            // row tiles of a slot with max_tok tokens
   int rec_rows;              // rows of a record
   int groups;                // workgroups
+  uint32_t bt_magic;         // floor(2^32 / block_tokens)
   float scale_log2;
 };
 struct F8AttnPlan {
