@@ -26,6 +26,9 @@ namespace {
 
 typedef float f16x_t __attribute__((ext_vector_type(16)));
 typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) void lds_void;
+typedef __attribute__((address_space(1))) const void glb_void;
+typedef __attribute__((address_space(4))) const int32_t const_i32;   // (read by scalar loads)
 
 // The weights are taken against a reference maximum that is raised only when a row's
 // maximum passes it by more than this (log2 units): they stay below 2^12, inside
@@ -145,20 +148,17 @@ __device__ __forceinline__ int block_scan(int v, int* lds, int& sum) {   // incl
   return v + before;
 }
 
-// The units of one head's line; for KEEP workgroup 0 leaves its prefix for the merge.
-template <int ROWS, int KT, int PER, int THREADS, bool KEEP>
+// The units of one head's line
+template <int ROWS, int KT, int PER, int THREADS>
 __device__ __forceinline__ int line_units(const F8AttnArgs& p, int gqa, int* lds) {
   const int entries = p.n_slots * p.slot_tiles;
-  const bool keep = KEEP && blockIdx.x == 0;
   int base = 0;
   for (int c = 0; c < entries; c += THREADS) {
     const int x = c + threadIdx.x;
     int sum;
-    const int inc = block_scan<THREADS>(x < entries ? entry_units<ROWS, KT, PER>(p, x, gqa) : 0, lds, sum);
-    if (keep && x < entries) p.pre[x + 1] = base + inc;
+    block_scan<THREADS>(x < entries ? entry_units<ROWS, KT, PER>(p, x, gqa) : 0, lds, sum);
     base += sum;
   }
-  if (keep && threadIdx.x == 0) p.pre[0] = 0;
   return base;
 }
 // The entry that holds unit u of the line (u < its length)
@@ -197,116 +197,150 @@ __device__ __forceinline__ bool sees(int key, int pos, int end, int window, int 
 // ---------------------------------------------------------------------------
 // few rows: up to 64 (token, head) rows of a slot and KV head
 // ---------------------------------------------------------------------------
+// One row tile a slot; the line of units is held 64 slots at a time in the lanes of each
+// wave (no LDS, no barrier ahead of the first loads of keys).
+template <int ROWS, int KT, int PER>
+struct SlotLine {
+  const F8AttnArgs& p;
+  int gqa, lane, base;   // lane l holds slot base + l
+  Slot mine;
+  int units, inc;
+
+  __device__ __forceinline__ SlotLine(const F8AttnArgs& args, int g) : p(args), gqa(g), lane(threadIdx.x & 63), base(-1) {}
+  __device__ __forceinline__ void load(int b) {
+    if (b == base) return;
+    base = b;
+    mine = b + lane < p.n_slots ? slot_of(p, b + lane) : Slot{0, 0, 0};
+    units = mine.n > 0 ? (row_tile<ROWS, KT>(p, mine, 0, gqa).tiles + PER - 1) / PER : 0;
+    inc = units;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int o = __shfl_up(inc, d);
+      if (lane >= d) inc += o;
+    }
+  }
+  // units of all slots; `keep`: their prefix, for the merge
+  __device__ __forceinline__ int total(bool keep) {
+    int t = 0;
+    for (int b = 0; b < p.n_slots; b += 64) {
+      load(b);
+      if (keep && b + lane < p.n_slots) p.pre[b + lane + 1] = t + inc;
+      t += __builtin_amdgcn_readlane(inc, 63);
+    }
+    if (keep && lane == 0) p.pre[0] = 0;
+    return t;
+  }
+  // the slot (lane of the loaded ones) that holds unit u of the line, and the unit in it
+  __device__ __forceinline__ int find(int u, int& at) {
+    for (int b = 0;; b += 64) {
+      load(b);
+      const int n = __builtin_amdgcn_readlane(inc, 63);
+      if (u < n) break;
+      u -= n;
+    }
+    const int e = __builtin_ctzll(__builtin_amdgcn_ballot_w64(inc > u));
+    at = u - (__builtin_amdgcn_readlane(inc, e) - __builtin_amdgcn_readlane(units, e));
+    return e;
+  }
+  // the next slot with units after lane e (from the first one on again: `wrapped`)
+  __device__ __forceinline__ int next(int e, bool& wrapped) {
+    wrapped = false;
+    uint64_t m = __builtin_amdgcn_ballot_w64(units > 0) & (e < 63 ? ~0ull << (e + 1) : 0ull);
+    while (m == 0) {
+      const int b = base + 64 < p.n_slots ? base + 64 : 0;
+      if (b == 0) wrapped = true;
+      load(b);
+      m = __builtin_amdgcn_ballot_w64(units > 0);
+    }
+    return __builtin_ctzll(m);
+  }
+  __device__ __forceinline__ Slot slot(int e) const {
+    return {__builtin_amdgcn_readlane(mine.t0, e), __builtin_amdgcn_readlane(mine.n, e),
+            __builtin_amdgcn_readlane(mine.pos0, e)};
+  }
+};
+
+// The two 16-key halves of a 32-key tile: first key, pages (-1: none) and first rows in them.
+struct Tile {
+  int key0, pg[2], row[2];
+};
+__device__ __forceinline__ Tile tile_at(const F8AttnArgs& p, const const_i32* table, int key0, int end) {
+  Tile t;
+  t.key0 = key0;
+#pragma unroll
+  for (int hf = 0; hf < 2; hf++) {
+    const int key = key0 + 16 * hf;
+    const BlockRow x = block_row(p, key);
+    const int pg = key < end && x.b < p.max_blocks ? table[x.b] : -1;
+    t.pg[hf] = pg >= 0 && pg < p.n_pages ? pg : -1;
+    t.row[hf] = x.row;
+  }
+  return t;
+}
+
 // Four waves, each with key tiles of its own (32 keys, a fourth of the part), joined
 // through LDS at the end: nothing is shared on the way, so a wave waits only for its
-// own loads and K, V of the next tile are in flight while this one is computed
+// own loads, and K, V of the next tile are in flight while this one is computed
 // (16 KB a wave at head_dim 256).  K rows are the A operand as loaded: lane l%16 is
 // the key, and the group l/16 takes the same dims of K and Q.  V comes four keys
 // by a run of dims, and byte permutes pair the keys ahead of the conversion.
-template <int HD, int NR>
-__global__ __launch_bounds__(256, NR == 1 ? 2 : 1) void f8_few_kernel(F8AttnArgs p) {
-  constexpr int KT = 32, ROWS = 16 * NR, PER = 4, THREADS = 256;
+template <int HD>
+__global__ __launch_bounds__(256, 2) void f8_few_kernel(F8AttnArgs p) {
+  constexpr int KT = 32, ROWS = 16, PER = 4, THREADS = 256;
   constexpr int KW = HD / 64;        // 16-byte key loads of a lane and 16-key half
   constexpr int VD = HD / 64;        // value dwords of a lane and key
   constexpr int DB = HD / 16;        // 16-dim blocks of the output
   constexpr int PITCH = HD + 4;
   __shared__ float red[4 * 16 * PITCH];
   __shared__ float ml[4][ROWS][2];
-  __shared__ int lds[THREADS / 64];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int m = lane & 15, g = lane >> 4;
   const int gqa = p.num_q / p.num_kv;
 
-  const int total = line_units<ROWS, KT, PER, THREADS, true>(p, gqa, lds);
+  SlotLine<ROWS, KT, PER> line(p, gqa);
+  const int total = line.total(blockIdx.x == 0 && wave == 0);
   const long all = (long)total * p.num_kv;
   const int grp = blockIdx.x, parts = part_count(all, p.groups);
   if (grp >= parts) return;
   long u = part_begin(all, grp, parts);
   const long u_end = part_begin(all, grp + 1, parts);
-  int h = (int)(u / total);
-  Part at = line_find<ROWS, KT, PER, THREADS>(p, gqa, total, (int)(u - (long)h * total), lds);
+  int h = __builtin_amdgcn_readfirstlane((int)(u / total)), at;
+  int e = line.find((int)(u - (long)h * total), at);
   bool first_seg = true;
-  const long key_bytes = (long)p.num_kv * HD;
+  const uint32_t key_bytes = (uint32_t)p.num_kv * HD;
+  const uint32_t k_off = m * key_bytes + 16 * g, v_off = 4 * g * key_bytes + m * (4 * VD);
 
-  while (u < u_end) {
-    const int s = at.entry / p.slot_tiles;
-    const Slot sl = slot_of(p, s);
-    if (at.entry - s * p.slot_tiles != 0 || sl.n <= 0) {   // (one row tile a slot here)
-      at.entry = at.entry + 1 < p.n_slots * p.slot_tiles ? at.entry + 1 : 0;
-      if (at.entry == 0) h++;
-      continue;
-    }
+  while (true) {
+    const Slot sl = line.slot(e);
     const RowTile rt = row_tile<ROWS, KT>(p, sl, 0, gqa);
     const int units = (rt.tiles + PER - 1) / PER;
-    const int n_u = (int)min((long)(units - at.at), u_end - u);
+    const int n_u = (int)min((long)(units - at), u_end - u);
     const int rows = sl.n * gqa;
-    const int v_end = min((at.at + n_u) * PER, rt.tiles);
+    const int v_end = min((at + n_u) * PER, rt.tiles);
+    const const_i32* table = (const const_i32*)(p.tables + (long)(line.base + e) * p.max_blocks);
 
-    // ---- queries: row 16 nr + m, dims 64 i + 16 g + 8 half ..
-    h8_t qf[NR][KW][2];
-    int pos_r[NR];
-#pragma unroll
-    for (int nr = 0; nr < NR; nr++) {
-      const int r = 16 * nr + m, rc = min(r, rows - 1);
-      const int t = rc / gqa;
-      pos_r[nr] = sl.pos0 + t;
-      const uint16_t* src = p.q + ((long)(sl.t0 + t) * p.num_q + h * gqa + (rc - t * gqa)) * HD + 16 * g;
-#pragma unroll
-      for (int i = 0; i < KW; i++)
-#pragma unroll
-        for (int e = 0; e < 2; e++) qf[nr][i][e] = *reinterpret_cast<const h8_t*>(src + 64 * i + 8 * e);
-    }
-
-    f4_t acc[NR][DB];
-    float mx[NR], ls[NR];
-#pragma unroll
-    for (int nr = 0; nr < NR; nr++) {
-      mx[nr] = -INFINITY;
-      ls[nr] = 0.f;
-#pragma unroll
-      for (int d = 0; d < DB; d++) acc[nr][d] = f4_t{0.f, 0.f, 0.f, 0.f};
-    }
-
-    const int32_t* table = p.tables + (long)s * p.max_blocks;
-    auto page_of = [&](int key) {
-      const int b = key / p.block_tokens;
-      const int pg = key < rt.end && b < p.max_blocks ? table[b] : -1;
-      return pg >= 0 && pg < p.n_pages ? pg : -1;
-    };
-    // the two 16-key halves of a tile: pages (-1: none), rows inside the page, exponents
-    struct Tile {
-      int key0, pg[2];
-    };
     u4_t kr[2][KW];
     uint32_t vr[8][VD];
-    float ks[2], vs[2];
-    auto lookup = [&](int v) {
-      Tile t;
-      t.key0 = rt.key0(v, KT);
-      t.pg[0] = page_of(t.key0);
-      t.pg[1] = page_of(t.key0 + 16);
-      return t;
-    };
+    uint32_t ke[2], ve[2];
     auto load_k = [&](const Tile& t) {
 #pragma unroll
       for (int hf = 0; hf < 2; hf++) {
-        const int pg = max(t.pg[hf], 0), row = (t.key0 + 16 * hf) % p.block_tokens;
-        const uint8_t* base = p.k_pool + ((long)pg * p.block_tokens + row) * key_bytes + (long)h * HD;
-        ks[hf] = pow2f(p.k_exp[(long)pg * p.num_kv + h]);
+        const long pg = max(t.pg[hf], 0);
+        const uint8_t* base = p.k_pool + (pg * p.block_tokens + t.row[hf]) * key_bytes + (long)h * HD;
+        ke[hf] = p.k_exp[pg * p.num_kv + h];
 #pragma unroll
-        for (int i = 0; i < KW; i++)
-          kr[hf][i] = *reinterpret_cast<const u4_t*>(base + m * key_bytes + 64 * i + 16 * g);
+        for (int i = 0; i < KW; i++) kr[hf][i] = *reinterpret_cast<const u4_t*>(base + k_off + 64 * i);
       }
     };
     auto load_v = [&](const Tile& t) {
 #pragma unroll
       for (int hf = 0; hf < 2; hf++) {
-        const int pg = max(t.pg[hf], 0), row = (t.key0 + 16 * hf) % p.block_tokens;
-        const uint8_t* base = p.v_pool + ((long)pg * p.block_tokens + row) * key_bytes + (long)h * HD;
-        vs[hf] = pow2f(p.v_exp[(long)pg * p.num_kv + h]);
+        const long pg = max(t.pg[hf], 0);
+        const uint8_t* base = p.v_pool + (pg * p.block_tokens + t.row[hf]) * key_bytes + (long)h * HD;
+        ve[hf] = p.v_exp[pg * p.num_kv + h];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-          const uint8_t* src = base + (4 * g + i) * key_bytes + m * (4 * VD);
+          const uint8_t* src = base + (long)i * key_bytes + v_off;
           if constexpr (VD == 4) {
             const u4_t w = *reinterpret_cast<const u4_t*>(src);
 #pragma unroll
@@ -320,36 +354,49 @@ __global__ __launch_bounds__(256, NR == 1 ? 2 : 1) void f8_few_kernel(F8AttnArgs
       }
     };
 
-    int v = at.at * PER + wave;
+    int v = at * PER + wave;
     Tile cur{}, nxt{};
     if (v < v_end) {
-      cur = lookup(v);
+      cur = tile_at(p, table, rt.key0(v, KT), rt.end);
       load_k(cur);
       load_v(cur);
-      nxt = v + PER < v_end ? lookup(v + PER) : cur;
     }
+
+    // ---- queries: row m, dims 64 i + 16 g + 8 half ..
+    h8_t qf[KW][2];
+    const int rc = min(m, rows - 1), tok = rc / gqa;
+    const int pos_r = sl.pos0 + tok;
+    {
+      const uint16_t* src = p.q + ((long)(sl.t0 + tok) * p.num_q + h * gqa + (rc - tok * gqa)) * HD + 16 * g;
+#pragma unroll
+      for (int i = 0; i < KW; i++)
+#pragma unroll
+        for (int x = 0; x < 2; x++) qf[i][x] = *reinterpret_cast<const h8_t*>(src + 64 * i + 8 * x);
+    }
+    if (v + PER < v_end) nxt = tile_at(p, table, rt.key0(v + PER, KT), rt.end);
+
+    f4_t acc[DB];
+    float mx = -INFINITY, ls = 0.f;
+#pragma unroll
+    for (int d = 0; d < DB; d++) acc[d] = f4_t{0.f, 0.f, 0.f, 0.f};
+
     for (; v < v_end; v += PER) {
       const bool more = v + PER < v_end;
       // ---- scores: lane m's row, keys 16 hf + 4 g + i
-      f4_t sc[NR][2];
+      f4_t sc[2];
 #pragma unroll
       for (int hf = 0; hf < 2; hf++) {
-        h8_t ka[KW][2];
+        const float f = pow2f(ke[hf]);
+        f4_t a = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < KW; i++)
 #pragma unroll
-          for (int e = 0; e < 2; e++)
-            ka[i][e] = join8(cvt2(kr[hf][i][2 * e], ks[hf], false), cvt2(kr[hf][i][2 * e], ks[hf], true),
-                             cvt2(kr[hf][i][2 * e + 1], ks[hf], false), cvt2(kr[hf][i][2 * e + 1], ks[hf], true));
-#pragma unroll
-        for (int nr = 0; nr < NR; nr++) {
-          f4_t a = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int i = 0; i < KW; i++)
-#pragma unroll
-            for (int e = 0; e < 2; e++) a = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[i][e], qf[nr][i][e], a, 0, 0, 0);
-          sc[nr][hf] = a * p.scale_log2;
-        }
+          for (int x = 0; x < 2; x++)
+            a = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                join8(cvt2(kr[hf][i][2 * x], f, false), cvt2(kr[hf][i][2 * x], f, true),
+                      cvt2(kr[hf][i][2 * x + 1], f, false), cvt2(kr[hf][i][2 * x + 1], f, true)),
+                qf[i][x], a, 0, 0, 0);
+        sc[hf] = a * p.scale_log2;
       }
       const bool whole = cur.pg[0] >= 0 && cur.pg[1] >= 0 && cur.key0 + KT - 1 <= rt.pos_lo && cur.key0 + KT <= rt.end &&
                          (p.window <= 0 || cur.key0 > rt.pos_hi - p.window || cur.key0 + KT <= p.sink);
@@ -361,37 +408,31 @@ __global__ __launch_bounds__(256, NR == 1 ? 2 : 1) void f8_few_kernel(F8AttnArgs
           for (int i = 0; i < 4; i++) {
             const int key = cur.key0 + 16 * hf + 4 * g + i;
             const bool there = cur.pg[hf] >= 0 && key < rt.end;
-#pragma unroll
-            for (int nr = 0; nr < NR; nr++)
-              sc[nr][hf][i] = there && sees(key, pos_r[nr], rt.end, p.window, p.sink) ? sc[nr][hf][i] : -INFINITY;
+            sc[hf][i] = there && sees(key, pos_r, rt.end, p.window, p.sink) ? sc[hf][i] : -INFINITY;
             // rows past the last key hold whatever the page held before
 #pragma unroll
             for (int d = 0; d < VD; d++) vr[4 * hf + i][d] = there ? vr[4 * hf + i][d] : 0u;
           }
       }
-      h8_t pb[NR];
+      float t = sc[0][0];
 #pragma unroll
-      for (int nr = 0; nr < NR; nr++) {
-        float t = sc[nr][0][0];
+      for (int i = 1; i < 8; i++) t = fmaxf(t, sc[i >> 2][i & 3]);
+      t = max32(max16(t));
+      if (__builtin_amdgcn_ballot_w64(t > mx + kSlack) != 0) {
+        const float mn = fmaxf(mx, t);
+        const float f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mx - mn);
+        ls *= f;
 #pragma unroll
-        for (int i = 1; i < 8; i++) t = fmaxf(t, sc[nr][i >> 2][i & 3]);
-        t = max32(max16(t));
-        if (__builtin_amdgcn_ballot_w64(t > mx[nr] + kSlack) != 0) {
-          const float mn = fmaxf(mx[nr], t);
-          const float f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mx[nr] - mn);
-          ls[nr] *= f;
-#pragma unroll
-          for (int d = 0; d < DB; d++) acc[nr][d] *= f;
-          mx[nr] = mn;
-        }
-        const float base = mx[nr] == -INFINITY ? 0.f : mx[nr];
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-          pb[nr][i] = (_Float16)__builtin_amdgcn_exp2f(sc[nr][i >> 2][i & 3] - base);
-        }
-        ls[nr] = add8(pb[nr], ls[nr]);
+        for (int d = 0; d < DB; d++) acc[d] *= f;
+        mx = mn;
       }
+      const float base = mx == -INFINITY ? 0.f : mx;
+      h8_t pb;
+#pragma unroll
+      for (int i = 0; i < 8; i++) pb[i] = (_Float16)__builtin_amdgcn_exp2f(sc[i >> 2][i & 3] - base);
+      ls = add8(pb, ls);
       // ---- O^T += V^T P^T: dims m * HD/16 + 4 d + j
+      const float v0 = pow2f(ve[0]), v1 = pow2f(ve[1]);
 #pragma unroll
       for (int d = 0; d < VD; d++) {
         uint32_t w[4][2];   // key pairs x byte pairs
@@ -401,83 +442,291 @@ __global__ __launch_bounds__(256, NR == 1 ? 2 : 1) void f8_few_kernel(F8AttnArgs
           w[k][1] = __builtin_amdgcn_perm(vr[2 * k + 1][d], vr[2 * k][d], 0x07030602u);
         }
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-          const h8_t a = join8(cvt2(w[0][j >> 1], vs[0], j & 1), cvt2(w[1][j >> 1], vs[0], j & 1),
-                               cvt2(w[2][j >> 1], vs[1], j & 1), cvt2(w[3][j >> 1], vs[1], j & 1));
-#pragma unroll
-          for (int nr = 0; nr < NR; nr++)
-            acc[nr][4 * d + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pb[nr], acc[nr][4 * d + j], 0, 0, 0);
-        }
+        for (int j = 0; j < 4; j++)
+          acc[4 * d + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+              join8(cvt2(w[0][j >> 1], v0, j & 1), cvt2(w[1][j >> 1], v0, j & 1), cvt2(w[2][j >> 1], v1, j & 1),
+                    cvt2(w[3][j >> 1], v1, j & 1)),
+              pb, acc[4 * d + j], 0, 0, 0);
       }
       if (more) {
         load_v(nxt);
         cur = nxt;
-        if (v + 2 * PER < v_end) nxt = lookup(v + 2 * PER);
+        if (v + 2 * PER < v_end) nxt = tile_at(p, table, rt.key0(v + 2 * PER, KT), rt.end);
       }
     }
 
     // ---- join the waves; lane m, group g holds dims (4 g + i) * HD/16 + d of row m
     const bool complete = n_u == units;
     const int rec = 2 * grp + (first_seg ? 0 : 1);
+    ls = sum32(sum16(ls));
+    if (g == 0) {
+      ml[wave][m][0] = mx;
+      ml[wave][m][1] = ls;
+    }
+    if (m < rows) {
+      float* dst = red + (wave * 16 + m) * PITCH;
 #pragma unroll
-    for (int nr = 0; nr < NR; nr++) {
-      ls[nr] = sum32(sum16(ls[nr]));
-      if (g == 0) {
-        ml[wave][16 * nr + m][0] = mx[nr];
-        ml[wave][16 * nr + m][1] = ls[nr];
-      }
+      for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int d = 0; d < DB; d += 4)
+          *reinterpret_cast<f4_t*>(dst + (4 * g + i) * DB + d) =
+              f4_t{acc[d][i], acc[d + 1][i], acc[d + 2][i], acc[d + 3][i]};
     }
     __syncthreads();
+    for (int x = tid * 4; x < rows * HD; x += THREADS * 4) {
+      const int r = x / HD, d = x - r * HD;
+      float M = -INFINITY, L = 0.f;
 #pragma unroll
-    for (int nr = 0; nr < NR; nr++) {
-      if (16 * nr >= rows) break;
-      float M = -INFINITY;
+      for (int w = 0; w < 4; w++) M = fmaxf(M, ml[w][r][0]);
+      f4_t o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int w = 0; w < 4; w++) M = fmaxf(M, ml[w][16 * nr + m][0]);
-      const float f = mx[nr] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx[nr] - M);
-      if (16 * nr + m < rows) {
-        float* dst = red + (wave * 16 + m) * PITCH;
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-#pragma unroll
-          for (int d = 0; d < DB; d += 4)
-            *reinterpret_cast<f4_t*>(dst + (4 * g + i) * DB + d) =
-                f4_t{acc[nr][d][i], acc[nr][d + 1][i], acc[nr][d + 2][i], acc[nr][d + 3][i]} * f;
+      for (int w = 0; w < 4; w++) {
+        const float f = ml[w][r][0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[w][r][0] - M);
+        L += ml[w][r][1] * f;
+        o += f * *reinterpret_cast<const f4_t*>(red + (16 * w + r) * PITCH + d);
       }
-      __syncthreads();
-      const int here = min(16, rows - 16 * nr);
-      for (int x = tid * 4; x < here * HD; x += THREADS * 4) {
-        const int r = x / HD, d = x - r * HD, row = 16 * nr + r;
-        float Mr = -INFINITY, L = 0.f;
+      if (complete) {
+        o *= L > 0.f ? 1.f / L : 0.f;
+        const int t = r / gqa;
+        *reinterpret_cast<u2_t*>(p.out + ((long)(sl.t0 + t) * p.num_q + h * gqa + (r - t * gqa)) * HD + d) =
+            u2_t{f2h(o[0]) | (f2h(o[1]) << 16), f2h(o[2]) | (f2h(o[3]) << 16)};
+      } else {
+        *reinterpret_cast<f4_t*>(p.rec_o + ((long)rec * p.rec_rows + r) * HD + d) = o;
+        if (d == 0) *reinterpret_cast<f2_t*>(p.rec_ml + ((long)rec * p.rec_rows + r) * 2) = f2_t{M, L};
+      }
+    }
+    u += n_u;
+    if (u >= u_end) break;
+    __syncthreads();   // (the next segment's waves write the same LDS)
+    first_seg = false;
+    at = 0;
+    bool wrapped;
+    e = line.next(e, wrapped);
+    if (wrapped) h++;
+  }
+}
+
+// 17 to 64 rows: waves of 32 rows on the 32x32 matrix instruction, RG of them side by
+// side on the same keys (the second's loads meet the first's lines in the caches), 4 / RG
+// key streams.  Otherwise as above: lane l%32 is the key of K's operand and takes 16 of
+// every 32 dims; V comes by runs of HD/32 dims, and output block d has dims HD/32 * m + d.
+template <int HD, int RG>
+__global__ __launch_bounds__(256, 1) void f8_mid_kernel(F8AttnArgs p) {
+  constexpr int KT = 32, ROWS = 32 * RG, KG = 4 / RG, PER = KG, THREADS = 256;
+  constexpr int KW = HD / 32;        // 16-byte key loads of a lane
+  constexpr int DB = HD / 32;        // 32-dim blocks of the output, value bytes of a lane and key
+  constexpr int VD = DB / 4;         // value dwords of a lane and key
+  constexpr int PITCH = HD + 4;
+  __shared__ float red[4 * 32 * PITCH];
+  __shared__ float ml[KG][ROWS][2];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c = lane & 31, hh = lane >> 5, rg = wave % RG, kg = wave / RG;
+  const int gqa = p.num_q / p.num_kv;
+
+  SlotLine<ROWS, KT, PER> line(p, gqa);
+  const int total = line.total(blockIdx.x == 0 && wave == 0);
+  const long all = (long)total * p.num_kv;
+  const int grp = blockIdx.x, parts = part_count(all, p.groups);
+  if (grp >= parts) return;
+  long u = part_begin(all, grp, parts);
+  const long u_end = part_begin(all, grp + 1, parts);
+  int h = __builtin_amdgcn_readfirstlane((int)(u / total)), at;
+  int e = line.find((int)(u - (long)h * total), at);
+  bool first_seg = true;
+  const uint32_t key_bytes = (uint32_t)p.num_kv * HD;
+  const uint32_t k_off = (c & 15) * key_bytes + 16 * hh, v_off = 4 * hh * key_bytes + c * DB;
+
+  while (true) {
+    const Slot sl = line.slot(e);
+    const RowTile rt = row_tile<ROWS, KT>(p, sl, 0, gqa);
+    const int units = (rt.tiles + PER - 1) / PER;
+    const int n_u = (int)min((long)(units - at), u_end - u);
+    const int rows = sl.n * gqa;
+    // a wave without rows loads nothing (the others wait for nobody)
+    const int v_end = 32 * rg < rows ? min((at + n_u) * PER, rt.tiles) : 0;
+    const const_i32* table = (const const_i32*)(p.tables + (long)(line.base + e) * p.max_blocks);
+
+    u4_t kr[KW];
+    uint32_t vr[16][VD];
+    uint32_t ke[2], ve[2];
+    auto load_k = [&](const Tile& t) {
+      // the lane's key is in the first or the second half
+      const uint8_t* base[2];
 #pragma unroll
-        for (int w = 0; w < 4; w++) Mr = fmaxf(Mr, ml[w][row][0]);
+      for (int hf = 0; hf < 2; hf++) {
+        const long pg = max(t.pg[hf], 0);
+        base[hf] = p.k_pool + (pg * p.block_tokens + t.row[hf]) * key_bytes + (long)h * HD;
+        ke[hf] = p.k_exp[pg * p.num_kv + h];
+      }
+      const uint8_t* src = (c < 16 ? base[0] : base[1]) + k_off;
 #pragma unroll
-        for (int w = 0; w < 4; w++)
-          L += ml[w][row][0] == -INFINITY ? 0.f : ml[w][row][1] * __builtin_amdgcn_exp2f(ml[w][row][0] - Mr);
-        f4_t o = *reinterpret_cast<const f4_t*>(red + r * PITCH + d);
+      for (int i = 0; i < KW; i++) kr[i] = *reinterpret_cast<const u4_t*>(src + 32 * i);
+    };
+    auto load_v = [&](const Tile& t) {
+      // keys 16 hf + 8 a + 4 hh + i
 #pragma unroll
-        for (int w = 1; w < 4; w++) o += *reinterpret_cast<const f4_t*>(red + (16 * w + r) * PITCH + d);
-        if (complete) {
-          const float inv = L > 0.f ? 1.f / L : 0.f;
-          o *= inv;
-          const int t = row / gqa;
-          *reinterpret_cast<u2_t*>(p.out + ((long)(sl.t0 + t) * p.num_q + h * gqa + (row - t * gqa)) * HD + d) =
-              u2_t{f2h(o[0]) | (f2h(o[1]) << 16), f2h(o[2]) | (f2h(o[3]) << 16)};
-        } else {
-          *reinterpret_cast<f4_t*>(p.rec_o + ((long)rec * p.rec_rows + row) * HD + d) = o;
-          if (d == 0) *reinterpret_cast<f2_t*>(p.rec_ml + ((long)rec * p.rec_rows + row) * 2) = f2_t{Mr, L};
+      for (int hf = 0; hf < 2; hf++) {
+        const long pg = max(t.pg[hf], 0);
+        const uint8_t* base = p.v_pool + (pg * p.block_tokens + t.row[hf]) * key_bytes + (long)h * HD;
+        ve[hf] = p.v_exp[pg * p.num_kv + h];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          const uint8_t* src = base + (long)(8 * (i >> 2) + (i & 3)) * key_bytes + v_off;
+          if constexpr (VD == 2) {
+            const u2_t w = *reinterpret_cast<const u2_t*>(src);
+            vr[8 * hf + i][0] = w[0];
+            vr[8 * hf + i][1] = w[1];
+          } else {
+            vr[8 * hf + i][0] = *reinterpret_cast<const uint32_t*>(src);
+          }
         }
       }
-      __syncthreads();
+    };
+
+    int v = at * PER + kg;
+    Tile cur{}, nxt{};
+    if (v < v_end) {
+      cur = tile_at(p, table, rt.key0(v, KT), rt.end);
+      load_k(cur);
+      load_v(cur);
     }
-    first_seg = false;
+    // ---- queries: row c of the wave, dims 32 i + 16 hh + 8 x ..
+    h8_t qf[KW][2];
+    const int rc = min(32 * rg + c, rows - 1), tok = rc / gqa;
+    const int pos_r = sl.pos0 + tok;
+    {
+      const uint16_t* src = p.q + ((long)(sl.t0 + tok) * p.num_q + h * gqa + (rc - tok * gqa)) * HD + 16 * hh;
+#pragma unroll
+      for (int i = 0; i < KW; i++)
+#pragma unroll
+        for (int x = 0; x < 2; x++) qf[i][x] = *reinterpret_cast<const h8_t*>(src + 32 * i + 8 * x);
+    }
+    if (v + PER < v_end) nxt = tile_at(p, table, rt.key0(v + PER, KT), rt.end);
+
+    f16x_t acc[DB];
+    float mx = -INFINITY, ls = 0.f;
+#pragma unroll
+    for (int d = 0; d < DB; d++) acc[d] = f16x_t{};
+
+    for (; v < v_end; v += PER) {
+      const bool more = v + PER < v_end;
+      // ---- scores: lane c's row, keys 8 (x / 4) + 4 hh + x % 4
+      f16x_t sc = f16x_t{};
+      const float f = pow2f(c < 16 ? ke[0] : ke[1]);
+#pragma unroll
+      for (int i = 0; i < KW; i++)
+#pragma unroll
+        for (int x = 0; x < 2; x++)
+          sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(
+              join8(cvt2(kr[i][2 * x], f, false), cvt2(kr[i][2 * x], f, true), cvt2(kr[i][2 * x + 1], f, false),
+                    cvt2(kr[i][2 * x + 1], f, true)),
+              qf[i][x], sc, 0, 0, 0);
+      sc *= p.scale_log2;
+      const bool whole = cur.pg[0] >= 0 && cur.pg[1] >= 0 && cur.key0 + KT - 1 <= rt.pos_lo && cur.key0 + KT <= rt.end &&
+                         (p.window <= 0 || cur.key0 > rt.pos_hi - p.window || cur.key0 + KT <= p.sink);
+      if (more) load_k(nxt);
+      if (!whole) {
+#pragma unroll
+        for (int x = 0; x < 16; x++) {
+          const int key = cur.key0 + 8 * (x >> 2) + 4 * hh + (x & 3);
+          const bool there = cur.pg[x >> 3] >= 0 && key < rt.end;
+          sc[x] = there && sees(key, pos_r, rt.end, p.window, p.sink) ? sc[x] : -INFINITY;
+          // rows past the last key hold whatever the page held before
+#pragma unroll
+          for (int d = 0; d < VD; d++) vr[x][d] = there ? vr[x][d] : 0u;
+        }
+      }
+      float t = sc[0];
+#pragma unroll
+      for (int x = 1; x < 16; x++) t = fmaxf(t, sc[x]);
+      t = max32(t);
+      if (__builtin_amdgcn_ballot_w64(t > mx + kSlack) != 0) {
+        const float mn = fmaxf(mx, t);
+        const float r = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mx - mn);
+        ls *= r;
+#pragma unroll
+        for (int d = 0; d < DB; d++) acc[d] *= r;
+        mx = mn;
+      }
+      const float base = mx == -INFINITY ? 0.f : mx;
+#pragma unroll
+      for (int hf = 0; hf < 2; hf++) {
+        h8_t pb;
+#pragma unroll
+        for (int i = 0; i < 8; i++) pb[i] = (_Float16)__builtin_amdgcn_exp2f(sc[8 * hf + i] - base);
+        ls = add8(pb, ls);
+        const float vf = pow2f(ve[hf]);
+#pragma unroll
+        for (int d = 0; d < VD; d++) {
+          uint32_t w[4][2];   // key pairs x byte pairs
+#pragma unroll
+          for (int k = 0; k < 4; k++) {
+            w[k][0] = __builtin_amdgcn_perm(vr[8 * hf + 2 * k + 1][d], vr[8 * hf + 2 * k][d], 0x05010400u);
+            w[k][1] = __builtin_amdgcn_perm(vr[8 * hf + 2 * k + 1][d], vr[8 * hf + 2 * k][d], 0x07030602u);
+          }
+#pragma unroll
+          for (int j = 0; j < 4; j++)
+            acc[4 * d + j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
+                join8(cvt2(w[0][j >> 1], vf, j & 1), cvt2(w[1][j >> 1], vf, j & 1), cvt2(w[2][j >> 1], vf, j & 1),
+                      cvt2(w[3][j >> 1], vf, j & 1)),
+                pb, acc[4 * d + j], 0, 0, 0);
+        }
+      }
+      if (more) {
+        load_v(nxt);
+        cur = nxt;
+        if (v + 2 * PER < v_end) nxt = tile_at(p, table, rt.key0(v + 2 * PER, KT), rt.end);
+      }
+    }
+
+    // ---- join the streams; lane c holds dims DB * (8 (x / 4) + 4 hh + x % 4) + d of row c
+    const bool complete = n_u == units;
+    const int rec = 2 * grp + (first_seg ? 0 : 1);
+    ls = sum32(ls);
+    if (hh == 0) {
+      ml[kg][32 * rg + c][0] = mx;
+      ml[kg][32 * rg + c][1] = ls;
+    }
+    if (32 * rg + c < rows) {
+      float* dst = red + (kg * ROWS + 32 * rg + c) * PITCH;
+#pragma unroll
+      for (int x = 0; x < 16; x++)
+#pragma unroll
+        for (int d = 0; d < DB; d += 4)
+          *reinterpret_cast<f4_t*>(dst + DB * (8 * (x >> 2) + 4 * hh + (x & 3)) + d) =
+              f4_t{acc[d][x], acc[d + 1][x], acc[d + 2][x], acc[d + 3][x]};
+    }
+    __syncthreads();
+    for (int x = tid * 4; x < rows * HD; x += THREADS * 4) {
+      const int r = x / HD, d = x - r * HD;
+      float M = -INFINITY, L = 0.f;
+#pragma unroll
+      for (int w = 0; w < KG; w++) M = fmaxf(M, ml[w][r][0]);
+      f4_t o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < KG; w++) {
+        const float fw = ml[w][r][0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[w][r][0] - M);
+        L += ml[w][r][1] * fw;
+        o += fw * *reinterpret_cast<const f4_t*>(red + (w * ROWS + r) * PITCH + d);
+      }
+      if (complete) {
+        o *= L > 0.f ? 1.f / L : 0.f;
+        const int t = r / gqa;
+        *reinterpret_cast<u2_t*>(p.out + ((long)(sl.t0 + t) * p.num_q + h * gqa + (r - t * gqa)) * HD + d) =
+            u2_t{f2h(o[0]) | (f2h(o[1]) << 16), f2h(o[2]) | (f2h(o[3]) << 16)};
+      } else {
+        *reinterpret_cast<f4_t*>(p.rec_o + ((long)rec * p.rec_rows + r) * HD + d) = o;
+        if (d == 0) *reinterpret_cast<f2_t*>(p.rec_ml + ((long)rec * p.rec_rows + r) * 2) = f2_t{M, L};
+      }
+    }
     u += n_u;
-    at.at = 0;
-    at.entry++;
-    if (at.entry == p.n_slots * p.slot_tiles) {
-      at.entry = 0;
-      h++;
-    }
+    if (u >= u_end) break;
+    __syncthreads();   // (the next segment's waves write the same LDS)
+    first_seg = false;
+    at = 0;
+    bool wrapped;
+    e = line.next(e, wrapped);
+    if (wrapped) h++;
   }
 }
 
@@ -490,9 +739,6 @@ __global__ __launch_bounds__(256, NR == 1 ? 2 : 1) void f8_few_kernel(F8AttnArgs
 // wave the rows that it loaded itself, so only its own loads are waited for.  V is stored
 // by dim, four keys to 8 bytes, in the order that the scores' lanes hold them.  Pads
 // keep 16-byte reads of 16 lanes on distinct banks, at constant offsets of one address.
-typedef __attribute__((address_space(3))) void lds_void;
-typedef __attribute__((address_space(1))) const void glb_void;
-typedef __attribute__((address_space(4))) const int32_t const_i32;
 
 template <int HD>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void f8_many_kernel(F8AttnArgs p) {
@@ -512,7 +758,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const int c = lane & 31, hh = lane >> 5;
   const int gqa = p.num_q / p.num_kv;
 
-  const int total = line_units<ROWS, KT, PER, THREADS, false>(p, gqa, lds);
+  const int total = line_units<ROWS, KT, PER, THREADS>(p, gqa, lds);
   const long all = (long)total * p.num_kv;
   if (blockIdx.x == 0 && tid == 0) *reinterpret_cast<long*>(p.cuts + 4 * p.groups) = all;
   // neighbouring parts (the same head's keys) on one XCD, whose L2 holds their tiles
@@ -824,11 +1070,11 @@ __global__ __launch_bounds__(256) void f8_cut_merge_kernel(F8AttnArgs p) {
 // ---------------------------------------------------------------------------
 // merge of the row tiles that were cut
 // ---------------------------------------------------------------------------
-// A workgroup per row, each wave every fourth record.
+// A workgroup per row.
 template <int HD>
 __global__ __launch_bounds__(256) void f8_merge_kernel(F8AttnArgs p) {
   constexpr int E = HD / 64;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int entries = p.n_slots * p.slot_tiles;
   const int tile = blockIdx.x / p.rec_rows, row = blockIdx.x - tile * p.rec_rows;
   const int entry = tile % entries, h = tile / entries;
@@ -852,45 +1098,51 @@ __global__ __launch_bounds__(256) void f8_merge_kernel(F8AttnArgs p) {
   const Slot sl = slot_of(p, s);
   if (row >= sl.n * gqa) return;
 
+  // 64 records a round: lane i holds record i's {m, l}, the wave reads 16 records' sums (all
+  // of a round's loads are under way before the first is used), weights by lane reads
   float M = -INFINITY, L = 0.f;
   float o[E] = {};
   for (int i0 = 0; i0 < n; i0 += 64) {
-    if (i0 + lane < n) {
-      const f2_t r = *reinterpret_cast<const f2_t*>(p.rec_ml + ((long)rec_of(i0 + lane) * p.rec_rows + row) * 2);
-      if (r[1] > 0.f) M = fmaxf(M, r[0]);
+    float x[16][E];
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+      const float* src = p.rec_o + ((long)rec_of(min(i0 + 16 * wave + i, n - 1)) * p.rec_rows + row) * HD + lane * E;
+      if constexpr (E == 4) {
+        const f4_t v = *reinterpret_cast<const f4_t*>(src);
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[i][e] = v[e];
+      } else {
+        const f2_t v = *reinterpret_cast<const f2_t*>(src);
+        x[i][0] = v[0];
+        x[i][1] = v[1];
+      }
+    }
+    f2_t r = {-INFINITY, 0.f};
+    if (i0 + lane < n) r = *reinterpret_cast<const f2_t*>(p.rec_ml + ((long)rec_of(i0 + lane) * p.rec_rows + row) * 2);
+    const bool any = r[1] > 0.f;
+    const float mn = fmaxf(M, wave_max(any ? r[0] : -INFINITY));
+    if (mn == -INFINITY) continue;   // no key so far
+    const float f = __builtin_amdgcn_exp2f(M - mn), w = any ? __builtin_amdgcn_exp2f(r[0] - mn) : 0.f;
+    M = mn;
+    L = L * f + wave_sum(w * r[1]);
+#pragma unroll
+    for (int e = 0; e < E; e++) o[e] *= f;
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+      const float wi = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), 16 * wave + i));
+#pragma unroll
+      for (int e = 0; e < E; e++) o[e] = __builtin_fmaf(wi, x[i][e], o[e]);
     }
   }
-  M = wave_max(M);
-  if (M == -INFINITY) M = 0.f;
-#pragma unroll 8
-  for (int i = wave; i < n; i += 4) {
-    const long at = (long)rec_of(i) * p.rec_rows + row;
-    const f2_t r = *reinterpret_cast<const f2_t*>(p.rec_ml + at * 2);
-    const float w = r[1] > 0.f ? __builtin_amdgcn_exp2f(r[0] - M) : 0.f;
-    L += w * r[1];
-    const float* src = p.rec_o + at * HD + lane * E;
-    if constexpr (E == 4) {
-      const f4_t x = *reinterpret_cast<const f4_t*>(src);
-#pragma unroll
-      for (int e = 0; e < 4; e++) o[e] = __builtin_fmaf(w, x[e], o[e]);
-    } else {
-      const f2_t x = *reinterpret_cast<const f2_t*>(src);
-#pragma unroll
-      for (int e = 0; e < 2; e++) o[e] = __builtin_fmaf(w, x[e], o[e]);
-    }
-  }
-  __shared__ float part[4][64][E + 1];
+  __shared__ float part[4][64][E];
 #pragma unroll
   for (int e = 0; e < E; e++) part[wave][lane][e] = o[e];
-  part[wave][lane][E] = L;
   __syncthreads();
   if (wave != 0) return;
 #pragma unroll
-  for (int w = 1; w < 4; w++) {
+  for (int w = 1; w < 4; w++)
 #pragma unroll
     for (int e = 0; e < E; e++) o[e] += part[w][lane][e];
-    L += part[w][lane][E];
-  }
   const float inv = L > 0.f ? 1.f / L : 0.f;
   const int t = row / gqa;
   uint16_t* dst = p.out + ((long)(sl.t0 + t) * p.num_q + h * gqa + (row - t * gqa)) * HD + lane * E;
@@ -921,9 +1173,10 @@ F8AttnPlan f8_attn_plan(int num_q, int num_kv, int head_dim, int n_slots, long q
   } else {
     x.slot_tiles = 1;
     x.rec_rows = (int)rows;
-    units = (long)n_slots * num_kv * ((max_ctx + 127) / 128);
+    const int unit_keys = x.row_tiles == 4 ? 64 : 128;
+    units = (long)n_slots * num_kv * ((max_ctx + unit_keys - 1) / unit_keys);
     x.groups = (int)std::min<long>(units, x.row_tiles == 1 ? 512 : 256);
-    x.merges = max_ctx > 128 || units > x.groups;
+    x.merges = max_ctx > unit_keys || units > x.groups;
   }
   const size_t ints = x.many ? 4 * (size_t)x.groups + 4 : (size_t)n_slots + 1;
   const size_t pre = (ints * 4 + 255) / 256 * 256;
@@ -940,11 +1193,11 @@ static void launch_f8(const F8AttnArgs& a, const F8AttnPlan& x, hipStream_t stre
   if (x.many)
     hipLaunchKernelGGL((f8_many_kernel<HD>), grid, dim3(512), 0, stream, a);
   else if (x.row_tiles == 1)
-    hipLaunchKernelGGL((f8_few_kernel<HD, 1>), grid, dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((f8_few_kernel<HD>), grid, dim3(256), 0, stream, a);
   else if (x.row_tiles == 2)
-    hipLaunchKernelGGL((f8_few_kernel<HD, 2>), grid, dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((f8_mid_kernel<HD, 1>), grid, dim3(256), 0, stream, a);
   else
-    hipLaunchKernelGGL((f8_few_kernel<HD, 4>), grid, dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((f8_mid_kernel<HD, 2>), grid, dim3(256), 0, stream, a);
   if (!x.merges) return;
   if (x.many) {
     if (x.groups > 1)
