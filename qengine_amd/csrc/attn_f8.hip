@@ -184,9 +184,21 @@ __device__ __forceinline__ Part line_find(const F8AttnArgs& p, int gqa, int tota
   __syncthreads();
   return r;
 }
-// Parts of the line: at most a workgroup's each, and none empty.
-__device__ __forceinline__ int part_count(long units, int groups) { return (int)min(units, (long)groups); }
-__device__ __forceinline__ long part_begin(long units, int g, int parts) { return units * g / parts; }
+// Parts of the line: at most a workgroup's each and none empty, the first `more` of them one
+// unit longer (the units of all heads stay below 2^31: the host sees to it).
+struct Parts {
+  int n, q, more;
+  __device__ __forceinline__ Parts(int units, int groups) {
+    n = min(units, groups);
+    q = n > 0 ? units / n : 0;
+    more = units - q * n;
+  }
+  __device__ __forceinline__ int begin(int g) const { return g * q + min(g, more); }
+  __device__ __forceinline__ int of(int x) const {   // the part that holds unit x
+    const int lo = more * (q + 1);
+    return x < lo ? x / (q + 1) : more + (x - lo) / q;
+  }
+};
 
 __device__ __forceinline__ bool sees(int key, int pos, int end, int window, int sink) {
   return key <= pos && key < end && (window <= 0 || key > pos - window || key < sink);
@@ -278,34 +290,34 @@ __device__ __forceinline__ Tile tile_at(const F8AttnArgs& p, const const_i32* ta
   return t;
 }
 
-// Four waves, each with key tiles of its own (32 keys, a fourth of the part), joined
-// through LDS at the end: nothing is shared on the way, so a wave waits only for its
+// W waves, each with key tiles of its own (every W-th of the part's 32-key tiles), joined
+// through LDS at the end; a unit is PER tiles.  Nothing is shared on the way, so a wave waits only for its
 // own loads, and K, V of the next tile are in flight while this one is computed
 // (16 KB a wave at head_dim 256).  K rows are the A operand as loaded: lane l%16 is
 // the key, and the group l/16 takes the same dims of K and Q.  V comes four keys
 // by a run of dims, and byte permutes pair the keys ahead of the conversion.
-template <int HD>
-__global__ __launch_bounds__(256, 2) void f8_few_kernel(F8AttnArgs p) {
-  constexpr int KT = 32, ROWS = 16, PER = 4, THREADS = 256;
+template <int HD, int W, int PER>
+__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) void f8_few_kernel(F8AttnArgs p) {
+  constexpr int KT = 32, ROWS = 16, THREADS = 64 * W;
   constexpr int KW = HD / 64;        // 16-byte key loads of a lane and 16-key half
   constexpr int VD = HD / 64;        // value dwords of a lane and key
   constexpr int DB = HD / 16;        // 16-dim blocks of the output
   constexpr int PITCH = HD + 4;
-  __shared__ float red[4 * 16 * PITCH];
-  __shared__ float ml[4][ROWS][2];
+  __shared__ float red[W * 16 * PITCH];
+  __shared__ float ml[W][ROWS][2];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int m = lane & 15, g = lane >> 4;
   const int gqa = p.num_q / p.num_kv;
 
   SlotLine<ROWS, KT, PER> line(p, gqa);
   const int total = line.total(blockIdx.x == 0 && wave == 0);
-  const long all = (long)total * p.num_kv;
-  const int grp = blockIdx.x, parts = part_count(all, p.groups);
-  if (grp >= parts) return;
-  long u = part_begin(all, grp, parts);
-  const long u_end = part_begin(all, grp + 1, parts);
-  int h = __builtin_amdgcn_readfirstlane((int)(u / total)), at;
-  int e = line.find((int)(u - (long)h * total), at);
+  const Parts parts(total * p.num_kv, p.groups);
+  const int grp = blockIdx.x;
+  if (grp >= parts.n) return;
+  int u = parts.begin(grp);
+  const int u_end = parts.begin(grp + 1);
+  int h = __builtin_amdgcn_readfirstlane(u / total), at;
+  int e = line.find(u - h * total, at);
   bool first_seg = true;
   const uint32_t key_bytes = (uint32_t)p.num_kv * HD;
   const uint32_t k_off = m * key_bytes + 16 * g, v_off = 4 * g * key_bytes + m * (4 * VD);
@@ -314,7 +326,7 @@ __global__ __launch_bounds__(256, 2) void f8_few_kernel(F8AttnArgs p) {
     const Slot sl = line.slot(e);
     const RowTile rt = row_tile<ROWS, KT>(p, sl, 0, gqa);
     const int units = (rt.tiles + PER - 1) / PER;
-    const int n_u = (int)min((long)(units - at), u_end - u);
+    const int n_u = min(units - at, u_end - u);
     const int rows = sl.n * gqa;
     const int v_end = min((at + n_u) * PER, rt.tiles);
     const const_i32* table = (const const_i32*)(p.tables + (long)(line.base + e) * p.max_blocks);
@@ -373,15 +385,15 @@ __global__ __launch_bounds__(256, 2) void f8_few_kernel(F8AttnArgs p) {
 #pragma unroll
         for (int x = 0; x < 2; x++) qf[i][x] = *reinterpret_cast<const h8_t*>(src + 64 * i + 8 * x);
     }
-    if (v + PER < v_end) nxt = tile_at(p, table, rt.key0(v + PER, KT), rt.end);
+    if (v + W < v_end) nxt = tile_at(p, table, rt.key0(v + W, KT), rt.end);
 
     f4_t acc[DB];
     float mx = -INFINITY, ls = 0.f;
 #pragma unroll
     for (int d = 0; d < DB; d++) acc[d] = f4_t{0.f, 0.f, 0.f, 0.f};
 
-    for (; v < v_end; v += PER) {
-      const bool more = v + PER < v_end;
+    for (; v < v_end; v += W) {
+      const bool more = v + W < v_end;
       // ---- scores: lane m's row, keys 16 hf + 4 g + i
       f4_t sc[2];
 #pragma unroll
@@ -451,7 +463,7 @@ __global__ __launch_bounds__(256, 2) void f8_few_kernel(F8AttnArgs p) {
       if (more) {
         load_v(nxt);
         cur = nxt;
-        if (v + 2 * PER < v_end) nxt = tile_at(p, table, rt.key0(v + 2 * PER, KT), rt.end);
+        if (v + 2 * W < v_end) nxt = tile_at(p, table, rt.key0(v + 2 * W, KT), rt.end);
       }
     }
 
@@ -477,10 +489,10 @@ __global__ __launch_bounds__(256, 2) void f8_few_kernel(F8AttnArgs p) {
       const int r = x / HD, d = x - r * HD;
       float M = -INFINITY, L = 0.f;
 #pragma unroll
-      for (int w = 0; w < 4; w++) M = fmaxf(M, ml[w][r][0]);
+      for (int w = 0; w < W; w++) M = fmaxf(M, ml[w][r][0]);
       f4_t o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int w = 0; w < 4; w++) {
+      for (int w = 0; w < W; w++) {
         const float f = ml[w][r][0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[w][r][0] - M);
         L += ml[w][r][1] * f;
         o += f * *reinterpret_cast<const f4_t*>(red + (16 * w + r) * PITCH + d);
@@ -525,13 +537,13 @@ __global__ __launch_bounds__(256, 1) void f8_mid_kernel(F8AttnArgs p) {
 
   SlotLine<ROWS, KT, PER> line(p, gqa);
   const int total = line.total(blockIdx.x == 0 && wave == 0);
-  const long all = (long)total * p.num_kv;
-  const int grp = blockIdx.x, parts = part_count(all, p.groups);
-  if (grp >= parts) return;
-  long u = part_begin(all, grp, parts);
-  const long u_end = part_begin(all, grp + 1, parts);
-  int h = __builtin_amdgcn_readfirstlane((int)(u / total)), at;
-  int e = line.find((int)(u - (long)h * total), at);
+  const Parts parts(total * p.num_kv, p.groups);
+  const int grp = blockIdx.x;
+  if (grp >= parts.n) return;
+  int u = parts.begin(grp);
+  const int u_end = parts.begin(grp + 1);
+  int h = __builtin_amdgcn_readfirstlane(u / total), at;
+  int e = line.find(u - h * total, at);
   bool first_seg = true;
   const uint32_t key_bytes = (uint32_t)p.num_kv * HD;
   const uint32_t k_off = (c & 15) * key_bytes + 16 * hh, v_off = 4 * hh * key_bytes + c * DB;
@@ -540,7 +552,7 @@ __global__ __launch_bounds__(256, 1) void f8_mid_kernel(F8AttnArgs p) {
     const Slot sl = line.slot(e);
     const RowTile rt = row_tile<ROWS, KT>(p, sl, 0, gqa);
     const int units = (rt.tiles + PER - 1) / PER;
-    const int n_u = (int)min((long)(units - at), u_end - u);
+    const int n_u = min(units - at, u_end - u);
     const int rows = sl.n * gqa;
     // a wave without rows loads nothing (the others wait for nobody)
     const int v_end = 32 * rg < rows ? min((at + n_u) * PER, rt.tiles) : 0;
@@ -744,6 +756,7 @@ template <int HD>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void f8_many_kernel(F8AttnArgs p) {
   constexpr int WAVES = 8, ROWS = 32 * WAVES, THREADS = 64 * WAVES, PER = 1;
   constexpr int KT = 8192 / HD;              // 32 or 64 keys: 8 KB of codes
+  constexpr int KH = KT / 32;                // 32-key halves
   constexpr int WK = KT / WAVES;             // keys that a wave loads and converts
   constexpr int LPR = HD / 16;               // lanes of a key row's load
   constexpr int VP = KT * 2;                 // bytes of a dim's values
@@ -752,25 +765,25 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   constexpr int KB = KT * KP, VB = HD * VP + HD / VPAD * 16;
   __shared__ __align__(16) uint8_t tile_lds[2][KB + VB];
   __shared__ __align__(16) uint8_t raw_lds[2][8192];
-  __shared__ __align__(16) int gone_lds[2][WAVES];   // per tile and wave: its keys have no page
   __shared__ int lds[WAVES];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 31, hh = lane >> 5;
   const int gqa = p.num_q / p.num_kv;
 
   const int total = line_units<ROWS, KT, PER, THREADS>(p, gqa, lds);
-  const long all = (long)total * p.num_kv;
-  if (blockIdx.x == 0 && tid == 0) *reinterpret_cast<long*>(p.cuts + 4 * p.groups) = all;
+  if (blockIdx.x == 0 && tid == 0) p.cuts[4 * p.groups] = total * p.num_kv;
   // neighbouring parts (the same head's keys) on one XCD, whose L2 holds their tiles
-  const int parts = part_count(all, p.groups);
+  const Parts parts(total * p.num_kv, p.groups);
   const int grp = p.groups % 8 ? (int)blockIdx.x : (int)(blockIdx.x % 8) * (p.groups / 8) + (int)blockIdx.x / 8;
-  if (grp >= parts) return;
-  long u = part_begin(all, grp, parts);
-  const long u_end = part_begin(all, grp + 1, parts);
-  int h = (int)(u / total);
-  Part at = line_find<ROWS, KT, PER, THREADS>(p, gqa, total, (int)(u - (long)h * total), lds);
+  if (grp >= parts.n) return;
+  int u = parts.begin(grp);
+  const int u_end = parts.begin(grp + 1);
+  int h = u / total;
+  Part at = line_find<ROWS, KT, PER, THREADS>(p, gqa, total, u - h * total, lds);
   bool first_seg = true;
   const uint32_t key_bytes = (uint32_t)p.num_kv * HD;
+  const uint32_t page_bytes = (uint32_t)p.block_tokens * key_bytes;
+  const int kt_div = KT / p.block_tokens, kt_mod = KT % p.block_tokens;
   const int entries = p.n_slots * p.slot_tiles;
 
   while (u < u_end) {
@@ -785,7 +798,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       continue;
     }
     const RowTile rt = row_tile<ROWS, KT>(p, sl, rti, gqa);
-    const int n_u = (int)min((long)(rt.tiles - at.at), u_end - u);
+    const int n_u = min(rt.tiles - at.at, u_end - u);
     const int v0 = at.at, v1 = at.at + n_u;
     const int rows = sl.n * gqa;
     const int row_w = rti * ROWS + wave * 32;      // this wave's first row
@@ -795,44 +808,64 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     const bool live = row_w < rows;
     const long out_row = ((long)(sl.t0 + tok) * p.num_q + h * gqa + (row - tok * gqa)) * HD;
 
-    h8_t qf[HD / 16];
-    float sl2 = p.scale_log2;
-    {
-      const uint16_t* src = p.q + out_row + 8 * hh;
-#pragma unroll
-      for (int i = 0; i < HD / 16; i++) qf[i] = *reinterpret_cast<const h8_t*>(src + 16 * i);
-      // (a negative scale is carried by the query, so that raw maxima serve)
-      if (sl2 < 0.f) {
-        sl2 = -sl2;
-#pragma unroll
-        for (int i = 0; i < HD / 16; i++) qf[i] = -qf[i];
-      }
-    }
-    f16x_t acc[HD / 32];
-#pragma unroll
-    for (int d = 0; d < HD / 32; d++) acc[d] = f16x_t{};
-    float mx = -INFINITY, ls = 0.f;
-
     const const_i32* table = (const const_i32*)(p.tables + (long)s * p.max_blocks);
     auto page_of = [&](int key) {   // (key the same in the whole wave)
       const int b = block_row(p, key).b;
       const int pg = key < rt.end && b < p.max_blocks ? table[b] : -1;
       return pg >= 0 && pg < p.n_pages ? pg : -1;
     };
-    // this wave's WK keys of a tile lie in one page (pages are whole sixteens)
-    float ksc = 0.f, vsc = 0.f;      // their exponents' factors
-    int loaded = -1;                 // their page
-    int ahead = -1;                  // the page of the tile after that
-    auto lookup = [&](int v) { ahead = page_of(rt.key0(v, KT) + wave * WK); };
+    // Where this wave's rows see tiles whole, in halves y of 32 keys (key 32 (y + y_off) past the
+    // sinks): y < y_sink or y_lo <= y < y_hi.  Tiles that none of them sees: v >= v_hi, and
+    // v_sink <= v < v_lo.
+    const int off = rt.w0 - rt.n_sink, y_off = off * KH;
+    const int seen = min(pos_lo + 1, rt.end) / 32;
+    const int y_hi = seen - y_off;
+    int y_lo = rt.n_sink * KH, y_sink = 0;
+    int v_hi = live ? pos_hi / KT + 1 - off : 0, v_lo = 0, v_sink = 0;
+    if (p.window > 0) {
+      if (pos_hi >= p.window) y_lo = max(y_lo, (pos_hi - p.window) / 32 + 1 - y_off);
+      y_sink = min(min(p.sink / 32, seen), rt.n_sink * KH);
+      v_sink = max(rt.n_sink, (p.sink + KT - 1) / KT - off);
+      v_lo = pos_lo >= p.window ? (pos_lo - p.window + 1) / KT - off : 0;
+      if (!live) v_hi = 0;
+    }
+    // This wave's WK keys of a tile lie in one page (pages are whole sixteens).  The next tile to
+    // fetch is at row w_row of block w_base + w_at; lane i holds the page of block w_base + i.
+    int w_base, w_at, w_row, pages;
+    auto load_pages = [&](int b) {
+      w_base = b;
+      w_at = 0;
+      const int pg = b + lane < p.max_blocks ? table[b + lane] : -1;
+      pages = pg < p.n_pages ? pg : -1;
+    };
+    auto seek = [&](int v) {
+      const BlockRow x = block_row(p, rt.key0(v, KT) + wave * WK);
+      load_pages(x.b);
+      w_row = x.row;
+    };
+    float ksc = 0.f, vsc = 0.f;      // the fetched tile's exponents as factors
+    int loaded = -1;                 // and its page
     const uint32_t lane_off = (uint32_t)(lane / LPR) * key_bytes + (uint32_t)(lane % LPR) * 16;
+    const uint8_t* k_head = p.k_pool + (long)h * HD;
+    const uint8_t* v_head = p.v_pool + (long)h * HD;
     auto fetch = [&](int v) {
-      loaded = ahead;
-      const int pg = max(ahead, 0), row0 = block_row(p, rt.key0(v, KT) + wave * WK).row;
-      const long base = ((long)pg * p.block_tokens + row0) * key_bytes + (long)h * HD;
-      __builtin_amdgcn_global_load_lds((glb_void*)(p.k_pool + base + lane_off), (lds_void*)(raw_lds[0] + wave * 1024), 16, 0, 0);
-      __builtin_amdgcn_global_load_lds((glb_void*)(p.v_pool + base + lane_off), (lds_void*)(raw_lds[1] + wave * 1024), 16, 0, 0);
-      ksc = pow2f(p.k_exp[(long)pg * p.num_kv + h]);
-      vsc = pow2f(p.v_exp[(long)pg * p.num_kv + h]);
+      loaded = __builtin_amdgcn_readlane(pages, w_at);
+      const uint32_t pg = max(loaded, 0);
+      const uint64_t from = (uint64_t)pg * page_bytes + (uint32_t)w_row * key_bytes;
+      __builtin_amdgcn_global_load_lds((glb_void*)(k_head + from + lane_off), (lds_void*)(raw_lds[0] + wave * 1024), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((glb_void*)(v_head + from + lane_off), (lds_void*)(raw_lds[1] + wave * 1024), 16, 0, 0);
+      const uint32_t ex = pg * (uint32_t)p.num_kv + h;
+      ksc = pow2f(p.k_exp[ex]);
+      vsc = pow2f(p.v_exp[ex]);
+      // on to the next tile
+      w_row += kt_mod;
+      w_at += kt_div;
+      if (w_row >= p.block_tokens) {
+        w_row -= p.block_tokens;
+        w_at++;
+      }
+      if (v + 1 == rt.n_sink) seek(v + 1);
+      else if (w_at >= 64) load_pages(w_base + w_at);
     };
     const int vl = lane % (HD / 4), vq = lane / (HD / 4);   // value dims 4 vl .., keys 4 vq .. of the wave's
     auto stage = [&](int v, int buf) {
@@ -851,7 +884,6 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         for (int i = 0; i < 4; i++)
           if (loaded < 0 || key0 + 4 * vq + i >= rt.end) vr[i] = 0;
       }
-      if (lane == 0) gone_lds[buf][wave] = loaded < 0;
       uint8_t* kb = tile_lds[buf];
       uint8_t* vb = kb + KB;
       const int key = wave * WK + lane / LPR, slot = lane % LPR;
@@ -881,41 +913,51 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     auto advance = [&](int v, int buf) {
       if (v + 1 < v1) {
         stage(v + 1, buf ^ 1);
-        if (v + 2 < v1) {
-          fetch(v + 2);
-          if (v + 3 < v1) lookup(v + 3);
-        }
+        if (v + 2 < v1) fetch(v + 2);
       }
     };
 
-    lookup(v0);
-    __syncthreads();   // (the last segment's tiles are done with)
+    seek(v0);
     fetch(v0);
-    if (v0 + 1 < v1) lookup(v0 + 1);
-    stage(v0, 0);
-    if (v0 + 1 < v1) {
-      fetch(v0 + 1);
-      if (v0 + 2 < v1) lookup(v0 + 2);
+    // (the queries and the page check arrive beside the first codes)
+    h8_t qf[HD / 16];
+    {
+      const uint16_t* src = p.q + out_row + 8 * hh;
+#pragma unroll
+      for (int i = 0; i < HD / 16; i++) qf[i] = *reinterpret_cast<const h8_t*>(src + 16 * i);
     }
+    // whether every key from the part's first tile to its last has a page (else: looked up by tile)
+    bool paged = true;
+    for (int b = block_row(p, rt.key0(v0, KT)).b + lane, e = block_row(p, min(rt.key0(v1 - 1, KT) + KT, rt.end) - 1).b; b <= e; b += 64) {
+      const int pg = b < p.max_blocks ? table[b] : -1;
+      paged = paged && pg >= 0 && pg < p.n_pages;
+    }
+    paged = __builtin_amdgcn_ballot_w64(!paged) == 0;
+    f16x_t acc[HD / 32];
+#pragma unroll
+    for (int d = 0; d < HD / 32; d++) acc[d] = f16x_t{};
+    float mx = -INFINITY, ls = 0.f;
+    // a negative scale is carried by the query, so that raw maxima serve; masked scores are -inf
+    // ahead of the scale
+    const float sl2 = fmaxf(fabsf(p.scale_log2), 1e-30f);
+    if (p.scale_log2 < 0.f) {
+#pragma unroll
+      for (int i = 0; i < HD / 16; i++) qf[i] = -qf[i];
+    }
+    __syncthreads();   // (the last segment's tiles are done with)
+    stage(v0, 0);
+    if (v0 + 1 < v1) fetch(v0 + 1);
     __syncthreads();
     for (int v = v0; v < v1; v++) {
       const int buf = (v - v0) & 1;
       // one wave of each SIMD converts ahead of its products, the other after them
       if (wave < 4) advance(v, buf);
-      const int key0 = rt.key0(v, KT);
-      // a wave none of whose rows sees the tile sits it out
-      const bool out = !live || key0 > pos_hi ||
-                       (p.window > 0 && key0 + KT - 1 <= pos_lo - p.window && key0 >= p.sink);
-      if (!out) {
+      if (v < v_hi && !(v >= v_sink && v < v_lo)) {   // (a wave none of whose rows sees the tile sits it out)
+        __builtin_amdgcn_s_setprio(1);
         const uint8_t* kb = tile_lds[buf];
         const uint8_t* vb = kb + KB;
-        int gone = 0;
-#pragma unroll
-        for (int w = 0; w < WAVES; w++) gone |= gone_lds[buf][w];
-        const bool pages = __builtin_amdgcn_readfirstlane(gone) == 0;
 #pragma unroll
         for (int kh = 0; kh < KT / 32; kh++) {
-          const int k0 = key0 + 32 * kh;
           const uint8_t* krow = kb + 32 * kh * KP + c * KP + hh * 16;
           auto k_operand = [&](int i) { return *reinterpret_cast<const h8_t*>(krow + i * 32); };
           constexpr int NK = HD / 16;
@@ -935,24 +977,28 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
             __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
           }
           __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
-          const bool whole = pages && k0 + 31 <= pos_lo && k0 + 32 <= rt.end &&
-                             (p.window <= 0 || k0 > pos_hi - p.window || k0 + 32 <= p.sink);
-          float t = -INFINITY, f = sl2;
-          if (whole) {
+          // the first values' reads go ahead of the weights
+          const uint8_t* vat = vb + c * VP + c / VPAD * 16 + hh * 16 + kh * 64;
+          constexpr int NV = HD / 16;   // of 16 keys, then of the other 16
+          auto v_operand = [&](int i) {
+            return *reinterpret_cast<const h8_t*>(vat + (i % (NV / 2)) * (32 * VP + 32 / VPAD * 16) + i / (NV / 2) * 32);
+          };
+          h8_t va[4];
 #pragma unroll
-            for (int x = 0; x < 16; x++) t = fmaxf(t, sd[x]);
-            t = max32(t) * sl2;
-          } else {
+          for (int i = 0; i < 4; i++) va[i] = v_operand(i);
+          const int y = v * KH + kh, k0 = (y < rt.n_sink * KH ? y : y + y_off) * 32;
+          if (!((y >= y_lo && y < y_hi) || y < y_sink) || !paged) {
             const bool pa = page_of(k0) >= 0, pb = page_of(k0 + 16) >= 0;
 #pragma unroll
             for (int x = 0; x < 16; x++) {
               const int key = k0 + 8 * (x >> 2) + 4 * hh + (x & 3);
-              sd[x] = (x < 8 ? pa : pb) && sees(key, pos, rt.end, p.window, p.sink) ? sd[x] * sl2 : -INFINITY;
-              t = fmaxf(t, sd[x]);
+              sd[x] = (x < 8 ? pa : pb) && sees(key, pos, rt.end, p.window, p.sink) ? sd[x] : -INFINITY;
             }
-            t = max32(t);
-            f = 1.f;
           }
+          float t = sd[0];
+#pragma unroll
+          for (int x = 1; x < 16; x++) t = fmaxf(t, sd[x]);
+          t = max32(t) * sl2;
           if (__builtin_amdgcn_ballot_w64(t > mx + kSlack) != 0) {
             const float mn = fmaxf(mx, t);
             const float r = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mx - mn);
@@ -962,21 +1008,32 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
             mx = mn;
           }
           const float base = mx == -INFINITY ? 0.f : mx;
-#pragma unroll
-          for (int sg = 0; sg < 2; sg++) {
+          auto weights = [&](int sg) {
             h8_t w;
 #pragma unroll
-            for (int i = 0; i < 8; i++) w[i] = (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(sd[8 * sg + i], f, -base));
+            for (int i = 0; i < 8; i++) w[i] = (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(sd[8 * sg + i], sl2, -base));
             ls = add8(w, ls);
+            return w;
+          };
+          const h8_t w0 = weights(0);
+          __builtin_amdgcn_sched_barrier(0);
+          // the second weights are formed under the first products
+          const h8_t w1 = weights(1);
 #pragma unroll
-            for (int d = 0; d < HD / 32; d++) {
-              const h8_t a = *reinterpret_cast<const h8_t*>(vb + c * VP + c / VPAD * 16 + hh * 16 +
-                                                            d * (32 * VP + 32 / VPAD * 16) + (2 * kh + sg) * 32);
-              acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, w, acc[d], 0, 0, 0);
-            }
+          for (int i = 0; i < NV; i++) {
+            acc[i % (NV / 2)] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va[i & 3], i < NV / 2 ? w0 : w1, acc[i % (NV / 2)], 0, 0, 0);
+            if (i + 4 < NV) va[i & 3] = v_operand(i + 4);
           }
+#pragma unroll
+          for (int i = 0; i < NV - 4; i++) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            if (i < NV / 2 - 1) __builtin_amdgcn_sched_group_barrier(0x002, HD == 256 ? 5 : 10, 0);
+          }
+          __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
         }
       }
+      __builtin_amdgcn_s_setprio(0);
       if (wave >= 4) advance(v, buf);
       __syncthreads();
     }
@@ -998,14 +1055,15 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                 u2_t{f2h(acc[d][4 * a] * inv) | (f2h(acc[d][4 * a + 1] * inv) << 16),
                      f2h(acc[d][4 * a + 2] * inv) | (f2h(acc[d][4 * a + 3] * inv) << 16)};
       } else {
-        const long rec = (2 * grp + (first_seg ? 0 : 1)) * (long)p.rec_rows + wave * 32 + c;
+        // (in the registers' order: 1 KB a store; the merge reads them so)
+        const long rec = 2 * grp + (first_seg ? 0 : 1);
+        f4_t* ro = reinterpret_cast<f4_t*>(p.rec_o + (rec * ROWS + 32 * wave) * HD) + lane;
 #pragma unroll
         for (int d = 0; d < HD / 32; d++)
 #pragma unroll
           for (int a = 0; a < 4; a++)
-            *reinterpret_cast<f4_t*>(p.rec_o + rec * HD + 32 * d + 8 * a + 4 * hh) =
-                f4_t{acc[d][4 * a], acc[d][4 * a + 1], acc[d][4 * a + 2], acc[d][4 * a + 3]};
-        if (hh == 0) *reinterpret_cast<f2_t*>(p.rec_ml + rec * 2) = f2_t{mx, ls};
+            ro[(4 * d + a) * 64] = f4_t{acc[d][4 * a], acc[d][4 * a + 1], acc[d][4 * a + 2], acc[d][4 * a + 3]};
+        if (hh == 0) *reinterpret_cast<f2_t*>(p.rec_ml + (rec * ROWS + 32 * wave + c) * 2) = f2_t{mx, ls};
       }
     }
     first_seg = false;
@@ -1019,52 +1077,56 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   }
 }
 
-// The rows of the row tiles that parts cut: a wave per row, the workgroups of a part's cut only
-// if the tile begins in the part before (each tile once).
+// The row tiles that parts cut: a wave per 32 rows and 32 dims, in the registers' order of the
+// kernel above; the workgroups of a part's cut only if the tile begins in the part before
+// (each tile once).
 template <int HD>
 __global__ __launch_bounds__(256) void f8_cut_merge_kernel(F8AttnArgs p) {
-  constexpr int E = HD / 64, ROWS = 256, RG = ROWS / 4;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int grp = blockIdx.x / RG + 1;
-  const long all = *reinterpret_cast<const long*>(p.cuts + 4 * p.groups);
-  const int parts = part_count(all, p.groups);
-  if (grp >= parts) return;
+  constexpr int ROWS = 256, DB = HD / 32, WGS = 8 * DB / 4;
+  const int lane = threadIdx.x & 63, c = lane & 31, hh = lane >> 5;
+  const int cut_at = blockIdx.x / WGS, grp = cut_at + 1;
+  const int unit = (blockIdx.x - cut_at * WGS) * 4 + (threadIdx.x >> 6), rw = unit / DB, d = unit - rw * DB;
   const int4 cut = *reinterpret_cast<const int4*>(p.cuts + 4 * grp);
+  const Parts parts(p.cuts[4 * p.groups], p.groups);
+  if (grp >= parts.n) return;
   const int entry = cut.x, h = cut.y, v0 = cut.z, tiles = cut.w;
   if (entry < 0) return;
-  const long x0 = part_begin(all, grp, parts) - v0;
-  const long before = part_begin(all, grp - 1, parts);
+  const int x0 = parts.begin(grp) - v0, before = parts.begin(grp - 1);
   if (before > x0) return;   // an earlier cut is in this tile
-  int n = 2;
-  while (part_begin(all, grp + n - 1, parts) < x0 + tiles) n++;
-  const int r0 = 2 * (grp - 1) + (before == x0 ? 0 : 1);
-  auto rec_of = [&](int i) { return i == 0 ? r0 : 2 * (grp - 1 + i); };
+  const int n = parts.of(x0 + tiles - 1) - grp + 2;
+  const long r0 = 2 * (grp - 1) + (before == x0 ? 0 : 1);
+  auto rec_of = [&](int i) { return i == 0 ? r0 : 2l * (grp - 1 + i); };
   const int s = entry / p.slot_tiles, gqa = p.num_q / p.num_kv;
   const Slot sl = slot_of(p, s);
-  const int row = (blockIdx.x % RG) * 4 + wave, r = (entry - s * p.slot_tiles) * ROWS + row;
+  const int r = (entry - s * p.slot_tiles) * ROWS + 32 * rw + c;
   if (r >= sl.n * gqa) return;
-  float M = -INFINITY;
+  float M = -INFINITY, L = 0.f;
+  f4_t o[4] = {};
+#pragma unroll 2
   for (int i = 0; i < n; i++) {
-    const f2_t ml = *reinterpret_cast<const f2_t*>(p.rec_ml + ((long)rec_of(i) * p.rec_rows + row) * 2);
-    if (ml[1] > 0.f) M = fmaxf(M, ml[0]);
-  }
-  if (M == -INFINITY) M = 0.f;
-  float L = 0.f, o[E] = {};
-#pragma unroll 4
-  for (int i = 0; i < n; i++) {
-    const long at = (long)rec_of(i) * p.rec_rows + row;
-    const f2_t ml = *reinterpret_cast<const f2_t*>(p.rec_ml + at * 2);
-    const float w = ml[1] > 0.f ? __builtin_amdgcn_exp2f(ml[0] - M) : 0.f;
-    L += w * ml[1];
+    const long rec = rec_of(i);
+    const f2_t ml = *reinterpret_cast<const f2_t*>(p.rec_ml + (rec * ROWS + 32 * rw + c) * 2);
+    const f4_t* src = reinterpret_cast<const f4_t*>(p.rec_o + (rec * ROWS + 32 * rw) * HD) + 4 * d * 64 + lane;
+    f4_t x[4];
 #pragma unroll
-    for (int e = 0; e < E; e++) o[e] = __builtin_fmaf(w, p.rec_o[at * HD + lane * E + e], o[e]);
+    for (int a = 0; a < 4; a++) x[a] = src[a * 64];
+    const bool any = ml[1] > 0.f;
+    const float mn = fmaxf(M, any ? ml[0] : -INFINITY);
+    const float f = mn == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - mn);
+    const float w = any ? __builtin_amdgcn_exp2f(ml[0] - mn) : 0.f;
+    M = mn;
+    L = L * f + w * ml[1];
+#pragma unroll
+    for (int a = 0; a < 4; a++) o[a] = o[a] * f + x[a] * w;
   }
   const float inv = L > 0.f ? 1.f / L : 0.f;
   const int t = r / gqa;
-  uint16_t* dst = p.out + ((long)(sl.t0 + t) * p.num_q + h * gqa + (r - t * gqa)) * HD + lane * E;
+  uint16_t* dst = p.out + ((long)(sl.t0 + t) * p.num_q + h * gqa + (r - t * gqa)) * HD + 32 * d + 4 * hh;
 #pragma unroll
-  for (int e = 0; e < E; e += 2)
-    *reinterpret_cast<uint32_t*>(dst + e) = f2h(o[e] * inv) | (f2h(o[e + 1] * inv) << 16);
+  for (int a = 0; a < 4; a++) {
+    const f4_t y = o[a] * inv;
+    *reinterpret_cast<u2_t*>(dst + 8 * a) = u2_t{f2h(y[0]) | (f2h(y[1]) << 16), f2h(y[2]) | (f2h(y[3]) << 16)};
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -1080,18 +1142,12 @@ __global__ __launch_bounds__(256) void f8_merge_kernel(F8AttnArgs p) {
   const int entry = tile % entries, h = tile / entries;
   const int total = p.pre[entries], a = p.pre[entry], b = p.pre[entry + 1];
   if (a == b) return;
-  const long all = (long)total * p.num_kv, x0 = (long)h * total + a, x1 = (long)h * total + b;
-  const int parts = part_count(all, p.groups);
+  const int x0 = h * total + a, x1 = h * total + b;
+  const Parts parts(total * p.num_kv, p.groups);
   // the parts that hold the tile's first and last unit
-  auto part_of = [&](long x) {
-    long g = ((x + 1) * parts - 1) / all;
-    while (g > 0 && part_begin(all, (int)g, parts) > x) g--;
-    while (part_begin(all, (int)g + 1, parts) <= x) g++;
-    return (int)g;
-  };
-  const int g0 = part_of(x0), g1 = part_of(x1 - 1);
+  const int g0 = parts.of(x0), g1 = parts.of(x1 - 1);
   if (g0 == g1) return;   // stored whole
-  const int r0 = 2 * g0 + (part_begin(all, g0, parts) == x0 ? 0 : 1);
+  const int r0 = 2 * g0 + (parts.begin(g0) == x0 ? 0 : 1);
   const int n = g1 - g0 + 1;
   auto rec_of = [&](int i) { return i == 0 ? r0 : 2 * (g0 + i); };
   const int s = entry / p.slot_tiles, gqa = p.num_q / p.num_kv;
@@ -1155,6 +1211,8 @@ __global__ __launch_bounds__(256) void f8_merge_kernel(F8AttnArgs p) {
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
+constexpr int kWholeKeys = 1024;
+
 F8AttnPlan f8_attn_plan(int num_q, int num_kv, int head_dim, int n_slots, long q_rows, int max_tok, int max_ctx) {
   F8AttnPlan x{};
   const long rows = (long)max_tok * (num_q / num_kv);
@@ -1173,14 +1231,16 @@ F8AttnPlan f8_attn_plan(int num_q, int num_kv, int head_dim, int n_slots, long q
   } else {
     x.slot_tiles = 1;
     x.rec_rows = (int)rows;
-    const int unit_keys = x.row_tiles == 4 ? 64 : 128;
+    // A slot of at most 1,024 keys is one workgroup's: eight waves, four tiles each at most.
+    x.whole = x.row_tiles == 1 && max_ctx <= kWholeKeys;
+    const int unit_keys = x.whole ? kWholeKeys : x.row_tiles == 4 ? 64 : 128;
     units = (long)n_slots * num_kv * ((max_ctx + unit_keys - 1) / unit_keys);
-    x.groups = (int)std::min<long>(units, x.row_tiles == 1 ? 512 : 256);
-    x.merges = max_ctx > unit_keys || units > x.groups;
+    x.groups = (int)std::min<long>(units, x.whole ? 4096 : x.row_tiles == 1 ? 512 : 256);
+    x.merges = max_ctx > unit_keys;   // (parts are whole units)
   }
   const size_t ints = x.many ? 4 * (size_t)x.groups + 4 : (size_t)n_slots + 1;
   const size_t pre = (ints * 4 + 255) / 256 * 256;
-  const size_t recs = 2 * (size_t)x.groups * x.rec_rows;
+  const size_t recs = x.merges ? 2 * (size_t)x.groups * x.rec_rows : 0;
   x.ml_off = pre;
   x.o_off = pre + (recs * 8 + 255) / 256 * 256;
   x.total = x.o_off + recs * head_dim * 4;
@@ -1192,8 +1252,10 @@ static void launch_f8(const F8AttnArgs& a, const F8AttnPlan& x, hipStream_t stre
   const dim3 grid((unsigned)x.groups);
   if (x.many)
     hipLaunchKernelGGL((f8_many_kernel<HD>), grid, dim3(512), 0, stream, a);
+  else if (x.whole)
+    hipLaunchKernelGGL((f8_few_kernel<HD, 8, kWholeKeys / 32>), grid, dim3(512), 0, stream, a);
   else if (x.row_tiles == 1)
-    hipLaunchKernelGGL((f8_few_kernel<HD>), grid, dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((f8_few_kernel<HD, 4, 4>), grid, dim3(256), 0, stream, a);
   else if (x.row_tiles == 2)
     hipLaunchKernelGGL((f8_mid_kernel<HD, 1>), grid, dim3(256), 0, stream, a);
   else
@@ -1201,7 +1263,7 @@ static void launch_f8(const F8AttnArgs& a, const F8AttnPlan& x, hipStream_t stre
   if (!x.merges) return;
   if (x.many) {
     if (x.groups > 1)
-      hipLaunchKernelGGL((f8_cut_merge_kernel<HD>), dim3((unsigned)(x.groups - 1) * 64), dim3(256), 0, stream, a);
+      hipLaunchKernelGGL((f8_cut_merge_kernel<HD>), dim3((unsigned)(x.groups - 1) * (HD / 16)), dim3(256), 0, stream, a);
   } else {
     hipLaunchKernelGGL((f8_merge_kernel<HD>), dim3((unsigned)(a.n_slots * a.num_kv * x.rec_rows)), dim3(256), 0, stream, a);
   }

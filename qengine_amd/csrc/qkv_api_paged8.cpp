@@ -188,8 +188,10 @@ static int check_f8_attn(int num_q, int num_kv, int head_dim, int n_slots, int n
   if (num_kv <= 0 || num_q <= 0 || num_q % num_kv != 0 || n_slots <= 0 || n_rows <= 0 || max_tok <= 0 || max_ctx <= 0)
     return QKV_ERR_INVALID;
   if (num_q / num_kv > 8 || num_q > 1024 || max_ctx > (1 << 30)) return QKV_ERR_UNSUPPORTED;
-  // row tiles of the call, and the workgroups of their merge
-  if ((double)n_slots * ((double)max_tok * (num_q / num_kv) / 256 + 1) * num_kv > (double)(1 << 22)) return QKV_ERR_UNSUPPORTED;
+  // row tiles of the call, and the key tiles of them all (counted in 32 bits)
+  const double gqa = num_q / num_kv, full = (double)n_slots * ((double)max_tok * gqa / 256 + 1);
+  const double tiles = full < n_rows * gqa / 256 + n_slots ? full : n_rows * gqa / 256 + n_slots;
+  if (full * num_kv > (double)(1 << 22) || tiles * num_kv * (max_ctx / 32.0 + 1) > 2147483647.0) return QKV_ERR_UNSUPPORTED;
   return QKV_OK;
 }
 

@@ -188,6 +188,7 @@ struct F8AttnPlan {
   bool many;                 // the kernel for more than 64 (token, head) rows a slot
   int row_tiles;             // 16-row tiles of the other one: 1, 2 or 4
   int slot_tiles, rec_rows, groups;
+  bool whole;                // every slot one workgroup's
   bool merges;               // whether any row can be in several workgroups
   size_t ml_off, o_off, total;
 };

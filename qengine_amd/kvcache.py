@@ -573,25 +573,51 @@ def rope_table(rot_dim: int, *, base: float = 10000.0, scaling=None, device="cud
     return RopeTable(host.to(device), float(amp.value), rot_dim)
 
 
-def _on_device(stream, *tensors) -> None:
-    """Every tensor on the device that the call launches on: that of `stream`, or the current one."""
-    dev = torch.cuda.current_device() if stream is None else stream.device.index
+def _run_device(stream, t) -> int:
+    """The device that the call launches on, that of `stream` or the current one: tensor t's."""
+    dev = t.get_device()
+    if dev < 0:
+        raise ValueError("every tensor must be a device tensor")
+    if dev != (torch._C._cuda_getDevice() if stream is None else stream.device.index):
+        raise ValueError(f"the tensors are on {t.device}, the call runs on another device")
+    return dev
+
+
+def _on_device(dev, *tensors) -> None:
+    """Every tensor contiguous and on device `dev`."""
     for t in tensors:
-        if t is not None and t.get_device() != dev:
+        if t.get_device() != dev:
             raise ValueError(f"every tensor must be on cuda:{dev}, where the call runs; got {t.device}")
+        if not t.is_contiguous():
+            raise ValueError("every tensor but q, k and v must be contiguous")
 
 
-def _rows3(t, what, dtype=FP16):
-    """A tensor [tokens][heads][head_dim], a token's heads contiguous: pointer and token stride
-    (elements)."""
-    if t.dtype not in dtype:
-        raise ValueError(f"{what} must be {' or '.join(str(d) for d in dtype)}, got {t.dtype}")
-    if not t.is_cuda:
-        raise ValueError(f"{what} must be a device tensor")
-    st = t.stride()
-    if t.dim() != 3 or (st[2] != 1 and t.shape[2] > 1) or (st[1] != t.shape[2] and t.shape[1] > 1):
-        raise ValueError(f"{what} must be [tokens][heads][head_dim], the heads of a token contiguous")
-    return t.data_ptr(), st[0] if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+def _raw_stream(stream, dev) -> int:
+    return torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream.cuda_stream
+
+
+_INT32, _UINT8 = torch.int32, torch.uint8
+
+
+def _need_i32(n, what, t) -> None:
+    if t.dtype is not _INT32 or t.numel() < n:
+        raise ValueError(f"{what} must hold {n} numbers of torch.int32")
+
+
+def _rows3(t, what, dev, shape):
+    """Pointer and token stride (elements) of a tensor [tokens][heads][head_dim], a token's heads
+    contiguous."""
+    if t.shape != shape:
+        raise ValueError(f"{what} must be {list(shape)}, got {list(t.shape)}")
+    if t.dtype not in FP16:
+        raise ValueError(f"{what} must be {' or '.join(str(d) for d in FP16)}, got {t.dtype}")
+    if t.get_device() != dev:
+        raise ValueError(f"{what} must be on cuda:{dev}, where the call runs; got {t.device}")
+    n, heads, hd = shape
+    s0, s1, s2 = t.stride()
+    if (s2 != 1 and hd > 1) or (s1 != hd and heads > 1):
+        raise ValueError(f"{what}: the heads of a token must be contiguous")
+    return t.data_ptr(), s0 if n > 1 else heads * hd
 
 
 def _rope_layout(layout) -> int:
@@ -608,26 +634,30 @@ def rope(q, k, positions, table: RopeTable, *, layout="half", inverse=False, q_o
     one = q if q is not None else k
     if one is None:
         raise ValueError("q or k is required")
-    n_tok, hd = one.shape[0], one.shape[2]
-    ptrs, heads = [], []
-    for x, out, what in ((q, q_out, "q"), (k, k_out, "k")):
-        if x is None:
-            if out is not None:
-                raise ValueError(f"{what}_out without {what}")
-            ptrs += [0, 0, 0, 0]
-            heads.append(0)
-            continue
-        if out is None:
-            out = x
-        if x.shape[0] != n_tok or x.dim() != 3 or x.shape[2] != hd or out.shape != x.shape:
-            raise ValueError(f"{what} and {what}_out must be [{n_tok}][heads][{hd}]")
-        ptrs += [*_rows3(x, what), *_rows3(out, what + "_out")]
-        heads.append(x.shape[1])
-    _need(positions, n_tok * 4, "positions", torch.int32)
-    _on_device(stream, q, k, q_out, k_out, positions, table.turns)
-    check(lib().qkv_rope(*ptrs, _dev_ptr(positions, "positions"), table.turns.data_ptr(), table.amplitude, n_tok,
-                         heads[0], heads[1], hd, table.rot_dim, _rope_layout(layout), int(bool(inverse)),
-                         _stream(stream)), "qkv_rope")
+    if (q is None and q_out is not None) or (k is None and k_out is not None):
+        raise ValueError("an output without its input")
+    n_tok, nq, hd = one.shape
+    nk, dev = 0, _run_device(stream, one)
+    qp = kp = (0, 0, 0, 0)
+    if q is not None:
+        shape = q.shape
+        qp = _rows3(q, "q", dev, shape)
+        qp += _rows3(q_out, "q_out", dev, shape) if q_out is not None else qp
+    else:
+        nq = 0
+    if k is not None:
+        shape = k.shape
+        if shape[0] != n_tok or shape[2] != hd:
+            raise ValueError(f"k must be [{n_tok}][heads][{hd}]")
+        nk = shape[1]
+        kp = _rows3(k, "k", dev, shape)
+        kp += _rows3(k_out, "k_out", dev, shape) if k_out is not None else kp
+    _need_i32(n_tok, "positions", positions)
+    turns = table.turns
+    _on_device(dev, positions, turns)
+    check(lib().qkv_rope(*qp, *kp, positions.data_ptr(), turns.data_ptr(), table.amplitude, n_tok, nq, nk, hd,
+                         table.rot_dim, _rope_layout(layout), 1 if inverse else 0, _raw_stream(stream, dev)),
+          "qkv_rope")
 
 
 # ---------------------------------------------------------------------------
@@ -641,22 +671,23 @@ def f8_pool(n_pages: int, block_tokens: int, num_kv: int, head_dim: int, device)
             torch.zeros((n_pages, num_kv), dtype=torch.uint8, device=device))
 
 
-def _f8_shape(k_pool, v_pool, k_exp, v_exp, block_tables, starts, positions):
-    """(n_pages, block_tokens, num_kv, head_dim, n_slots, max_blocks) of a paged 8-bit batch."""
-    if k_pool.dim() != 4 or v_pool.shape != k_pool.shape:
+def _f8_batch(dev, k_pool, v_pool, k_exp, v_exp, block_tables, starts, positions):
+    """Checks of a paged 8-bit batch.  Returns (n_pages, block_tokens, num_kv, head_dim, n_slots,
+    max_blocks)."""
+    n_pages, bt, kv, hd = shape = k_pool.shape
+    if v_pool.shape != shape:
         raise ValueError("k_pool and v_pool must be [n_pages][block_tokens][num_kv][head_dim]")
-    n_pages, bt, kv, hd = k_pool.shape
     if k_exp.shape != (n_pages, kv) or v_exp.shape != (n_pages, kv):
         raise ValueError(f"k_exp and v_exp must be [{n_pages}][{kv}]")
-    for t, what in ((k_pool, "k_pool"), (v_pool, "v_pool"), (k_exp, "k_exp"), (v_exp, "v_exp")):
-        if t.dtype != torch.uint8:
-            raise ValueError(f"{what} must be torch.uint8, got {t.dtype}")
-    if block_tables.dim() != 2:
-        raise ValueError("block_tables must be [n_slots][max_blocks]")
-    n_slots = block_tables.shape[0]
+    if not (k_pool.dtype is v_pool.dtype is k_exp.dtype is v_exp.dtype is _UINT8):
+        raise ValueError("the pools and their exponents must be torch.uint8")
+    if not (block_tables.dtype is starts.dtype is positions.dtype is _INT32):
+        raise ValueError("block_tables, starts and positions must be torch.int32")
+    n_slots, mb = block_tables.shape
     if starts.numel() != n_slots + 1 or positions.numel() != n_slots:
         raise ValueError(f"starts must hold {n_slots + 1} numbers and positions {n_slots}")
-    return n_pages, bt, kv, hd, n_slots, block_tables.shape[1]
+    _on_device(dev, k_pool, v_pool, k_exp, v_exp, block_tables, starts, positions)
+    return n_pages, bt, kv, hd, n_slots, mb
 
 
 def f8_append_kv_paged(k, v, k_pool, v_pool, k_exp, v_exp, block_tables, starts, positions, *, max_tok, q=None,
@@ -664,28 +695,28 @@ def f8_append_kv_paged(k, v, k_pool, v_pool, k_exp, v_exp, block_tables, starts,
     """Ragged append: rows starts[s] .. starts[s+1]-1 of k and v (fp16 [rows][num_kv][head_dim])
     go to positions positions[s] .. of slot s.  With `rope` k is rotated first, and q (into
     q_out, or in place), in the same launch."""
-    n_pages, bt, kv, hd, n_slots, mb = _f8_shape(k_pool, v_pool, k_exp, v_exp, block_tables, starts, positions)
+    dev = _run_device(stream, k_pool)
+    n_pages, bt, kv, hd, n_slots, mb = _f8_batch(dev, k_pool, v_pool, k_exp, v_exp, block_tables, starts, positions)
     rows = k.shape[0]
-    if k.shape != (rows, kv, hd) or v.shape != k.shape:
-        raise ValueError(f"k and v must be [rows][{kv}][{hd}]")
-    qp, nq = (0, 0, 0, 0), 0
+    shape = (rows, kv, hd)
+    qp, nq, tp, amp, rot = (0, 0, 0, 0), 0, 0, 1.0, 0
+    if rope is not None:
+        _on_device(dev, rope.turns)
+        tp, amp, rot = rope.turns.data_ptr(), rope.amplitude, rope.rot_dim
     if q is not None:
         if rope is None:
             raise ValueError("q without rope")
-        out = q if q_out is None else q_out
-        if q.dim() != 3 or q.shape[0] != rows or q.shape[2] != hd or out.shape != q.shape:
-            raise ValueError(f"q and q_out must be [{rows}][heads][{hd}]")
-        qp, nq = (*_rows3(q, "q"), *_rows3(out, "q_out")), q.shape[1]
+        nq = q.shape[1]
+        qs = (rows, nq, hd)
+        qp = _rows3(q, "q", dev, qs)
+        qp += _rows3(q_out, "q_out", dev, qs) if q_out is not None else qp
     elif q_out is not None:
         raise ValueError("q_out without q")
-    _on_device(stream, k, v, k_pool, v_pool, k_exp, v_exp, block_tables, starts, positions, q, q_out,
-               None if rope is None else rope.turns)
     check(lib().qkv_f8_append_kv_paged(
-        *_rows3(k, "k"), *_rows3(v, "v"), _dev_ptr(k_pool, "k_pool"), _dev_ptr(v_pool, "v_pool"),
-        _dev_ptr(k_exp, "k_exp"), _dev_ptr(v_exp, "v_exp"), rows, n_slots, max_tok, kv, hd,
-        _i32(block_tables, "block_tables"), mb, bt, n_pages, _i32(starts, "starts"), _i32(positions, "positions"),
-        *qp, nq, rope.turns.data_ptr() if rope is not None else 0, rope.amplitude if rope is not None else 1.0,
-        rope.rot_dim if rope is not None else 0, _rope_layout(layout), _stream(stream)), "qkv_f8_append_kv_paged")
+        *_rows3(k, "k", dev, shape), *_rows3(v, "v", dev, shape), k_pool.data_ptr(), v_pool.data_ptr(),
+        k_exp.data_ptr(), v_exp.data_ptr(), rows, n_slots, max_tok, kv, hd, block_tables.data_ptr(), mb, bt, n_pages,
+        starts.data_ptr(), positions.data_ptr(), *qp, nq, tp, amp, rot, _rope_layout(layout),
+        _raw_stream(stream, dev)), "qkv_f8_append_kv_paged")
 
 
 def attn_f8_paged_workspace(num_q, num_kv, n_slots, n_rows, max_tok, max_ctx, device, *, head_dim=256) -> torch.Tensor:
@@ -700,19 +731,19 @@ def attn_f8_paged(q, k_pool, v_pool, k_exp, v_exp, out, workspace, block_tables,
     starts[s] .. starts[s+1]-1 at positions positions[s] ..) over the paged 8-bit cache:
     decode steps, verify blocks and prompts.  window > 0 limits a query to the last `window`
     keys and the first `sink`.  Rows past starts[-1] are left alone; out may be q."""
-    n_pages, bt, kv, hd, n_slots, mb = _f8_shape(k_pool, v_pool, k_exp, v_exp, block_tables, starts, positions)
-    rows, nq = q.shape[0], q.shape[1]
-    if q.shape != (rows, nq, hd) or out.shape != q.shape:
+    dev = _run_device(stream, k_pool)
+    n_pages, bt, kv, hd, n_slots, mb = _f8_batch(dev, k_pool, v_pool, k_exp, v_exp, block_tables, starts, positions)
+    rows, nq, qd = shape = q.shape
+    if qd != hd or out.shape != shape:
         raise ValueError(f"q and out must be [rows][num_q][{hd}]")
     if q.dtype not in FP16 or out.dtype not in FP16:
         raise ValueError(f"q and out must be fp16, got {q.dtype} and {out.dtype}")
-    _on_device(stream, q, k_pool, v_pool, k_exp, v_exp, out, workspace, block_tables, starts, positions)
+    _on_device(dev, q, out, workspace)
     check(lib().qkv_attn_f8_paged(
-        _dev_ptr(q, "q"), _dev_ptr(k_pool, "k_pool"), _dev_ptr(v_pool, "v_pool"), _dev_ptr(k_exp, "k_exp"),
-        _dev_ptr(v_exp, "v_exp"), _dev_ptr(out, "out"), rows, nq, kv, hd, n_slots, max_tok, max_ctx,
-        _i32(block_tables, "block_tables"), mb, bt, n_pages, _i32(starts, "starts"), _i32(positions, "positions"),
-        float(scale), window, sink, _dev_ptr(workspace, "workspace"), workspace.numel() * workspace.element_size(),
-        _stream(stream)), "qkv_attn_f8_paged")
+        q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr(), out.data_ptr(), rows,
+        nq, kv, hd, n_slots, max_tok, max_ctx, block_tables.data_ptr(), mb, bt, n_pages, starts.data_ptr(),
+        positions.data_ptr(), float(scale), window, sink, workspace.data_ptr(), workspace.nbytes,
+        _raw_stream(stream, dev)), "qkv_attn_f8_paged")
 
 
 # ---------------------------------------------------------------------------
@@ -731,8 +762,11 @@ class PagePlanes:
         self.tensors = list(tensors)
         self.n = len(self.tensors)
         self.n_pages = min((t.shape[0] for t in self.tensors), default=0)
+        self.device = self.tensors[0].get_device() if self.tensors else -1
         self.array = (_Plane * max(1, self.n))()
         for i, t in enumerate(self.tensors):
+            if t.get_device() != self.device:
+                raise ValueError("the planes must be on one device")
             self.array[i] = _Plane(_dev_ptr(t, f"plane {i}"), t.numel() * t.element_size() // max(1, t.shape[0]))
         self.ptr = ctypes.addressof(self.array)
 
@@ -742,25 +776,37 @@ def page_planes(tensors) -> PagePlanes:
     return PagePlanes(tensors)
 
 
-def _page_lists(block_tables, ref_counts, lists, status, stream):
-    """Checks of the page calls: pointers of the lists, their length, and the status pointer."""
-    _on_device(stream, block_tables, ref_counts, status, *(t for t, _ in lists))
-    if block_tables.dim() != 2:
-        raise ValueError("block_tables must be [n_slots][max_blocks]")
-    n = lists[0][0].numel()
-    for t, what in lists:
-        if t.numel() != n:
-            raise ValueError(f"{what} must hold {n} numbers")
-    if status is not None:
-        _need(status, n * 4, "status", torch.int32)
-    return [_i32(t, what) for t, what in lists], n, 0 if status is None else _dev_ptr(status, "status")
+def _page_state(dev, block_tables, ref_counts):
+    """Checks of the tables and counts; returns the leading arguments of the page calls."""
+    if not (block_tables.dtype is ref_counts.dtype is _INT32):
+        raise ValueError("block_tables and ref_counts must be torch.int32")
+    n_slots, mb = block_tables.shape
+    _on_device(dev, block_tables, ref_counts)
+    return block_tables.data_ptr(), n_slots, mb, ref_counts.data_ptr(), ref_counts.numel()
 
 
-def _planes_of(planes, n_pages):
+def _page_lists(dev, status, *lists):
+    """Checks of the int32 lists of a page call; returns their length and the status pointer."""
+    n = lists[0].numel()
+    for t in lists:
+        if t.dtype is not _INT32 or t.numel() != n:
+            raise ValueError(f"the lists must be torch.int32 of one length, {n}")
+    _on_device(dev, *lists)
+    if status is None:
+        return n, 0
+    _need_i32(n, "status", status)
+    _on_device(dev, status)
+    return n, status.data_ptr()
+
+
+def _planes_of(planes, n_pages, dev):
     if planes is None:
         return 0, 0
-    if planes.n and planes.n_pages < n_pages:
-        raise ValueError(f"the planes hold {planes.n_pages} pages, ref_counts {n_pages}")
+    if planes.n:
+        if planes.n_pages < n_pages:
+            raise ValueError(f"the planes hold {planes.n_pages} pages, ref_counts {n_pages}")
+        if planes.device != dev:
+            raise ValueError(f"the planes must be on cuda:{dev}, where the call runs")
     return planes.ptr, planes.n
 
 
@@ -775,19 +821,20 @@ def pages_fork(block_tables, ref_counts, parents, children, n_tokens, status=Non
                stream=None) -> None:
     """children[i] shares the pages of the first n_tokens[i] tokens of parents[i] (device int32
     lists; block_tables int32 [n_slots][max_blocks], ref_counts int32 [n_pages])."""
-    p, n, st = _page_lists(block_tables, ref_counts,
-                           ((parents, "parents"), (children, "children"), (n_tokens, "n_tokens")), status, stream)
-    check(lib().qkv_pages_fork(_i32(block_tables, "block_tables"), *block_tables.shape, block_tokens,
-                               _i32(ref_counts, "ref_counts"), ref_counts.numel(), *p, n, st, _stream(stream)),
-          "qkv_pages_fork")
+    dev = _run_device(stream, block_tables)
+    t, n_slots, mb, r, n_pages = _page_state(dev, block_tables, ref_counts)
+    n, st = _page_lists(dev, status, parents, children, n_tokens)
+    check(lib().qkv_pages_fork(t, n_slots, mb, block_tokens, r, n_pages, parents.data_ptr(), children.data_ptr(),
+                               n_tokens.data_ptr(), n, st, _raw_stream(stream, dev)), "qkv_pages_fork")
 
 
 def pages_release(block_tables, ref_counts, slots, keep_tokens, status=None, *, block_tokens, stream=None) -> None:
     """Gives back the pages of slots[i] past its first keep_tokens[i] tokens."""
-    p, n, st = _page_lists(block_tables, ref_counts, ((slots, "slots"), (keep_tokens, "keep_tokens")), status, stream)
-    check(lib().qkv_pages_release(_i32(block_tables, "block_tables"), *block_tables.shape, block_tokens,
-                                  _i32(ref_counts, "ref_counts"), ref_counts.numel(), *p, n, st, _stream(stream)),
-          "qkv_pages_release")
+    dev = _run_device(stream, block_tables)
+    t, n_slots, mb, r, n_pages = _page_state(dev, block_tables, ref_counts)
+    n, st = _page_lists(dev, status, slots, keep_tokens)
+    check(lib().qkv_pages_release(t, n_slots, mb, block_tokens, r, n_pages, slots.data_ptr(), keep_tokens.data_ptr(),
+                                  n, st, _raw_stream(stream, dev)), "qkv_pages_release")
 
 
 def pages_reserve(block_tables, ref_counts, slots, positions, n_new, status=None, planes=None, *, block_tokens,
@@ -795,38 +842,41 @@ def pages_reserve(block_tables, ref_counts, slots, positions, n_new, status=None
     """Pages of its own for tokens positions[i] .. positions[i] + n_new[i] - 1 of slots[i]: missing ones are
     taken, shared ones replaced (copied in `planes` where they hold earlier rows).  scratch: an int32
     tensor (allocated here when None) whose first 2n numbers are afterwards the copied pairs."""
-    p, n, st = _page_lists(block_tables, ref_counts,
-                           ((slots, "slots"), (positions, "positions"), (n_new, "n_new")), status, stream)
+    dev = _run_device(stream, block_tables)
+    t, n_slots, mb, r, n_pages = _page_state(dev, block_tables, ref_counts)
+    n, st = _page_lists(dev, status, slots, positions, n_new)
+    L = lib()
     if scratch is None:
-        scratch = _scratch(int(lib().qkv_pages_reserve_scratch_bytes(n, max_new, block_tokens)), block_tables.device,
+        scratch = _scratch(int(L.qkv_pages_reserve_scratch_bytes(n, max_new, block_tokens)), block_tables.device,
                            stream)
-    check(lib().qkv_pages_reserve(_i32(block_tables, "block_tables"), *block_tables.shape, block_tokens,
-                                  _i32(ref_counts, "ref_counts"), ref_counts.numel(), *p, n, max_new, st,
-                                  *_planes_of(planes, ref_counts.numel()), _i32(scratch, "scratch"),
-                                  scratch.numel() * 4, _stream(stream)), "qkv_pages_reserve")
+    _need_i32(0, "scratch", scratch)
+    _on_device(dev, scratch)
+    check(L.qkv_pages_reserve(t, n_slots, mb, block_tokens, r, n_pages, slots.data_ptr(), positions.data_ptr(),
+                              n_new.data_ptr(), n, max_new, st, *_planes_of(planes, n_pages, dev), scratch.data_ptr(),
+                              scratch.nbytes, _raw_stream(stream, dev)), "qkv_pages_reserve")
 
 
 def pages_copy(planes: PagePlanes, pairs, *, stream=None) -> None:
     """Page pairs[i][0] to page pairs[i][1] in every plane (device int32 [n][2])."""
-    if pairs.dim() != 2 or pairs.shape[1] != 2:
-        raise ValueError("pairs must be [n][2]")
-    _on_device(stream, pairs, *planes.tensors[:1])
-    check(lib().qkv_pages_copy(planes.ptr, planes.n, planes.n_pages, _i32(pairs, "pairs"), pairs.shape[0],
-                               _stream(stream)), "qkv_pages_copy")
+    dev = _run_device(stream, pairs)
+    if pairs.dim() != 2 or pairs.shape[1] != 2 or pairs.dtype is not _INT32:
+        raise ValueError("pairs must be torch.int32 [n][2]")
+    _on_device(dev, pairs)
+    check(lib().qkv_pages_copy(*_planes_of(planes, 0, dev), planes.n_pages, pairs.data_ptr(), pairs.shape[0],
+                               _raw_stream(stream, dev)), "qkv_pages_copy")
 
 
 def pages_compact(block_tables, ref_counts, moved, n_used, planes=None, *, scratch=None, stream=None) -> None:
     """Moves the pages in use to indices 0 .. n_used[0]-1, in planes, tables and counts; moved[p] (int32
     [n_pages]) is where page p went, -1 if it was free."""
-    if block_tables.dim() != 2:
-        raise ValueError("block_tables must be [n_slots][max_blocks]")
-    n_pages = ref_counts.numel()
-    _need(moved, n_pages * 4, "moved", torch.int32)
-    _need(n_used, 4, "n_used", torch.int32)
-    _on_device(stream, block_tables, ref_counts, moved, n_used, scratch)
+    dev = _run_device(stream, block_tables)
+    t, n_slots, mb, r, n_pages = _page_state(dev, block_tables, ref_counts)
+    _need_i32(n_pages, "moved", moved)
+    _need_i32(1, "n_used", n_used)
     if scratch is None:
         scratch = _scratch((n_pages + 2) * 4, block_tables.device, stream)
-    check(lib().qkv_pages_compact(_i32(block_tables, "block_tables"), *block_tables.shape,
-                                  _i32(ref_counts, "ref_counts"), n_pages, _dev_ptr(moved, "moved"),
-                                  _dev_ptr(n_used, "n_used"), *_planes_of(planes, n_pages), _i32(scratch, "scratch"),
-                                  scratch.numel() * 4, _stream(stream)), "qkv_pages_compact")
+    _need_i32(0, "scratch", scratch)
+    _on_device(dev, moved, n_used, scratch)
+    check(lib().qkv_pages_compact(t, n_slots, mb, r, n_pages, moved.data_ptr(), n_used.data_ptr(),
+                                  *_planes_of(planes, n_pages, dev), scratch.data_ptr(), scratch.nbytes,
+                                  _raw_stream(stream, dev)), "qkv_pages_compact")
