@@ -266,6 +266,10 @@ struct SlotLine {
     }
     return __builtin_ctzll(m);
   }
+  // units of the line ahead of lane e's slot (one load of lanes: at most 64 slots)
+  __device__ __forceinline__ int before(int e) const {
+    return __builtin_amdgcn_readlane(inc, e) - __builtin_amdgcn_readlane(units, e);
+  }
   __device__ __forceinline__ Slot slot(int e) const {
     return {__builtin_amdgcn_readlane(mine.t0, e), __builtin_amdgcn_readlane(mine.n, e),
             __builtin_amdgcn_readlane(mine.pos0, e)};
@@ -290,15 +294,18 @@ __device__ __forceinline__ Tile tile_at(const F8AttnArgs& p, const const_i32* ta
   return t;
 }
 
-// W waves, each with key tiles of its own (every W-th of the part's 32-key tiles), joined
-// through LDS at the end; a unit is PER tiles.  Nothing is shared on the way, so a wave waits only for its
+// Four waves, each with key tiles of its own (every fourth of the part's 32-key tiles), joined
+// through LDS at the end: nothing is shared on the way, so a wave waits only for its
 // own loads, and K, V of the next tile are in flight while this one is computed
 // (16 KB a wave at head_dim 256).  K rows are the A operand as loaded: lane l%16 is
 // the key, and the group l/16 takes the same dims of K and Q.  V comes four keys
 // by a run of dims, and byte permutes pair the keys ahead of the conversion.
-template <int HD, int W, int PER>
-__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) void f8_few_kernel(F8AttnArgs p) {
-  constexpr int KT = 32, ROWS = 16, THREADS = 64 * W;
+// JOIN: contexts of up to kJoinKeys keys, whose records the last workgroup of a tile
+// joins in this launch.
+constexpr int kJoinKeys = 1024, kJoinMost = kJoinKeys / 128;
+template <int HD, bool JOIN>
+__global__ __launch_bounds__(256, 2) void f8_few_kernel(F8AttnArgs p) {
+  constexpr int KT = 32, ROWS = 16, W = 4, PER = 4, THREADS = 64 * W;
   constexpr int KW = HD / 64;        // 16-byte key loads of a lane and 16-key half
   constexpr int VD = HD / 64;        // value dwords of a lane and key
   constexpr int DB = HD / 16;        // 16-dim blocks of the output
@@ -503,8 +510,66 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) 
         *reinterpret_cast<u2_t*>(p.out + ((long)(sl.t0 + t) * p.num_q + h * gqa + (r - t * gqa)) * HD + d) =
             u2_t{f2h(o[0]) | (f2h(o[1]) << 16), f2h(o[2]) | (f2h(o[3]) << 16)};
       } else {
-        *reinterpret_cast<f4_t*>(p.rec_o + ((long)rec * p.rec_rows + r) * HD + d) = o;
-        if (d == 0) *reinterpret_cast<f2_t*>(p.rec_ml + ((long)rec * p.rec_rows + r) * 2) = f2_t{M, L};
+        float* ro = p.rec_o + ((long)rec * p.rec_rows + r) * HD + d;
+        float* rm = p.rec_ml + ((long)rec * p.rec_rows + r) * 2;
+        if constexpr (JOIN) {   // (to where every XCD sees it)
+#pragma unroll
+          for (int i = 0; i < 4; i++) __hip_atomic_store(ro + i, o[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+          if (d == 0) {
+            __hip_atomic_store(rm, M, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            __hip_atomic_store(rm + 1, L, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+          }
+        } else {
+          *reinterpret_cast<f4_t*>(ro) = o;
+          if (d == 0) *reinterpret_cast<f2_t*>(rm) = f2_t{M, L};
+        }
+      }
+    }
+    // ---- the last of a row tile's workgroups joins their records (the stores above have
+    // completed when it is counted; a count goes back to zero with its last)
+    if constexpr (JOIN) {
+      if (!complete) {
+        __shared__ int order;
+        const int x0 = h * total + line.before(e), g0 = parts.of(x0), n = parts.of(x0 + units - 1) - g0 + 1;
+        int* count = p.counts + (line.base + e) * p.num_kv + h;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (tid == 0) order = __hip_atomic_fetch_add(count, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __syncthreads();
+        if (order == n - 1) {
+          const int r0 = 2 * g0 + (parts.begin(g0) == x0 ? 0 : 1);
+          for (int x = tid * 4; x < rows * HD; x += THREADS * 4) {
+            const int r = x / HD, d = x - r * HD;
+            float mr[kJoinMost], lr[kJoinMost];
+            f4_t ov[kJoinMost];
+#pragma unroll
+            for (int i = 0; i < kJoinMost; i++) {
+              const long at_r = (long)(i == 0 ? r0 : 2 * (g0 + min(i, n - 1))) * p.rec_rows + r;
+              mr[i] = __hip_atomic_load(p.rec_ml + at_r * 2, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+              lr[i] = __hip_atomic_load(p.rec_ml + at_r * 2 + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+              for (int k = 0; k < 4; k++)
+                ov[i][k] = __hip_atomic_load(p.rec_o + at_r * HD + d + k, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+            float M = -INFINITY, L = 0.f;
+#pragma unroll
+            for (int i = 0; i < kJoinMost; i++)
+              if (i < n && lr[i] > 0.f) M = fmaxf(M, mr[i]);
+            f4_t o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < kJoinMost; i++)
+              if (i < n && lr[i] > 0.f) {
+                const float w = __builtin_amdgcn_exp2f(mr[i] - M);
+                L += w * lr[i];
+                o += w * ov[i];
+              }
+            o *= L > 0.f ? 1.f / L : 0.f;
+            const int t = r / gqa;
+            *reinterpret_cast<u2_t*>(p.out + ((long)(sl.t0 + t) * p.num_q + h * gqa + (r - t * gqa)) * HD + d) =
+                u2_t{f2h(o[0]) | (f2h(o[1]) << 16), f2h(o[2]) | (f2h(o[3]) << 16)};
+          }
+          if (tid == 0) __hip_atomic_store(count, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
       }
     }
     u += n_u;
@@ -1211,8 +1276,6 @@ __global__ __launch_bounds__(256) void f8_merge_kernel(F8AttnArgs p) {
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
-constexpr int kWholeKeys = 1024;
-
 F8AttnPlan f8_attn_plan(int num_q, int num_kv, int head_dim, int n_slots, long q_rows, int max_tok, int max_ctx) {
   F8AttnPlan x{};
   const long rows = (long)max_tok * (num_q / num_kv);
@@ -1231,15 +1294,16 @@ F8AttnPlan f8_attn_plan(int num_q, int num_kv, int head_dim, int n_slots, long q
   } else {
     x.slot_tiles = 1;
     x.rec_rows = (int)rows;
-    // A slot of at most 1,024 keys is one workgroup's: eight waves, four tiles each at most.
-    x.whole = x.row_tiles == 1 && max_ctx <= kWholeKeys;
-    const int unit_keys = x.whole ? kWholeKeys : x.row_tiles == 4 ? 64 : 128;
+    // Short contexts: few records, joined in the launch (a second one costs as much as the
+    // attention); many records are merged by one, whose workgroups share them.
+    x.join = x.row_tiles == 1 && max_ctx <= kJoinKeys && n_slots <= 64 && n_slots * num_kv <= kJoinCounts;
+    const int unit_keys = x.row_tiles == 4 ? 64 : 128;
     units = (long)n_slots * num_kv * ((max_ctx + unit_keys - 1) / unit_keys);
-    x.groups = (int)std::min<long>(units, x.whole ? 4096 : x.row_tiles == 1 ? 512 : 256);
-    x.merges = max_ctx > unit_keys;   // (parts are whole units)
+    x.groups = (int)std::min<long>(units, x.row_tiles == 1 ? 512 : 256);
+    x.merges = max_ctx > unit_keys;   // (else no slot has two units)
   }
   const size_t ints = x.many ? 4 * (size_t)x.groups + 4 : (size_t)n_slots + 1;
-  const size_t pre = (ints * 4 + 255) / 256 * 256;
+  const size_t pre = kJoinCounts * 4 + (ints * 4 + 255) / 256 * 256;
   const size_t recs = x.merges ? 2 * (size_t)x.groups * x.rec_rows : 0;
   x.ml_off = pre;
   x.o_off = pre + (recs * 8 + 255) / 256 * 256;
@@ -1252,15 +1316,15 @@ static void launch_f8(const F8AttnArgs& a, const F8AttnPlan& x, hipStream_t stre
   const dim3 grid((unsigned)x.groups);
   if (x.many)
     hipLaunchKernelGGL((f8_many_kernel<HD>), grid, dim3(512), 0, stream, a);
-  else if (x.whole)
-    hipLaunchKernelGGL((f8_few_kernel<HD, 8, kWholeKeys / 32>), grid, dim3(512), 0, stream, a);
+  else if (x.join)
+    hipLaunchKernelGGL((f8_few_kernel<HD, true>), grid, dim3(256), 0, stream, a);
   else if (x.row_tiles == 1)
-    hipLaunchKernelGGL((f8_few_kernel<HD, 4, 4>), grid, dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((f8_few_kernel<HD, false>), grid, dim3(256), 0, stream, a);
   else if (x.row_tiles == 2)
     hipLaunchKernelGGL((f8_mid_kernel<HD, 1>), grid, dim3(256), 0, stream, a);
   else
     hipLaunchKernelGGL((f8_mid_kernel<HD, 2>), grid, dim3(256), 0, stream, a);
-  if (!x.merges) return;
+  if (!x.merges || x.join) return;
   if (x.many) {
     if (x.groups > 1)
       hipLaunchKernelGGL((f8_cut_merge_kernel<HD>), dim3((unsigned)(x.groups - 1) * (HD / 16)), dim3(256), 0, stream, a);

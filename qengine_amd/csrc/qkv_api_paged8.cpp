@@ -231,7 +231,8 @@ int qkv_attn_f8_paged(const uint16_t* q, const uint8_t* k_pool, const uint8_t* v
   a.tables = block_tables;
   a.starts = starts;
   a.positions = positions;
-  a.pre = a.cuts = reinterpret_cast<int*>(ws);
+  a.counts = reinterpret_cast<int*>(ws);
+  a.pre = a.cuts = a.counts + qkv::kJoinCounts;
   a.rec_ml = reinterpret_cast<float*>(ws + x.ml_off);
   a.rec_o = reinterpret_cast<float*>(ws + x.o_off);
   a.rows = n_rows;

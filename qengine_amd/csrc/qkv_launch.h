@@ -171,6 +171,7 @@ struct F8AttnArgs {
   const int32_t* tables;
   const int32_t* starts;
   const int32_t* positions;
+  int* counts;               // workspace, its first kJoinCounts ints: zero between calls
   int* pre;                  // workspace: unit prefix of the slots, [n_slots + 1] (few rows)
   int* cuts;                 // workspace, the same place: [groups][4] where each part begins, then
                              // the units of all heads (many rows)
@@ -184,11 +185,14 @@ struct F8AttnArgs {
   uint32_t bt_magic;         // floor(2^32 / block_tokens)
   float scale_log2;
 };
+// Workspaces begin with these counts, whatever the call's numbers, so that calls of different
+// shapes can share one.
+constexpr int kJoinCounts = 1024;
 struct F8AttnPlan {
   bool many;                 // the kernel for more than 64 (token, head) rows a slot
   int row_tiles;             // 16-row tiles of the other one: 1, 2 or 4
   int slot_tiles, rec_rows, groups;
-  bool whole;                // every slot one workgroup's
+  bool join;                 // records joined in the launch
   bool merges;               // whether any row can be in several workgroups
   size_t ml_off, o_off, total;
 };

@@ -720,9 +720,9 @@ def f8_append_kv_paged(k, v, k_pool, v_pool, k_exp, v_exp, block_tables, starts,
 
 
 def attn_f8_paged_workspace(num_q, num_kv, n_slots, n_rows, max_tok, max_ctx, device, *, head_dim=256) -> torch.Tensor:
-    """Workspace of attn_f8_paged for these numbers (no initialisation needed)."""
+    """Zero-filled workspace of attn_f8_paged for these numbers (calls leave it ready for the next)."""
     n = int(lib().qkv_attn_f8_paged_workspace_bytes(num_q, num_kv, head_dim, n_slots, n_rows, max_tok, max_ctx))
-    return torch.empty(n, dtype=torch.uint8, device=device)
+    return torch.zeros(n, dtype=torch.uint8, device=device)
 
 
 def attn_f8_paged(q, k_pool, v_pool, k_exp, v_exp, out, workspace, block_tables, starts, positions, *, max_tok,

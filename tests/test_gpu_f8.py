@@ -124,9 +124,11 @@ def _attend(q, kp, vp, ke, ve, tables, starts, pos, scale, window=0, sink=0, max
     qd = dev(q)
     out = qd if alias else torch.full_like(qd, 9.0)
     ws = kvcache.attn_f8_paged_workspace(nq, kv, len(pos), q.shape[0], mt, mc, DEV, head_dim=hd)
-    ws.fill_(0xff)   # (nothing in it is trusted)
+    assert not ws.any()
+    ws[4096:] = 0xff   # (past the counts nothing in it is trusted)
     kvcache.attn_f8_paged(qd, dev(kp), dev(vp), dev(ke), dev(ve), out, ws, dev(tables), dev(starts), dev(pos), max_tok=mt,
                           max_ctx=mc, scale=scale, window=window, sink=sink)
+    assert not ws[:4096].any()   # ready for the next call
     return out.cpu().numpy()
 
 
@@ -256,6 +258,23 @@ def test_same_result_every_time_and_on_another_stream():
     assert np.array_equal(a, b)
     case = _attn_case(8, [300, 0], [90, 300], 64, 2, 4, 256)
     assert np.array_equal(_attend(*case, 0.06), _attend(*case, 0.06))
+
+
+def test_one_workspace_for_calls_of_every_shape():
+    """Short and long contexts, single tokens and prompts in turn on one workspace, without a reset."""
+    cases = [(_attn_case(11, [300, 900, 5], [1, 1, 1], 16, 2, 4, 128), 0.09), (_attn_case(12, [3000], [1], 64, 2, 4, 128), 0.09),
+             (_attn_case(13, [20, 0], [70, 130], 16, 2, 4, 128), 0.09), (_attn_case(14, [700] * 9, [1] * 9, 16, 2, 4, 128), 0.09),
+             (_attn_case(15, [64, 300], [9, 16], 16, 2, 4, 128), 0.09)]
+    want = [_attend(*c, f) for c, f in cases]
+    ws = kvcache.attn_f8_paged_workspace(8, 2, 9, 1000, 200, 4000, DEV, head_dim=128)
+    for turn in range(3):
+        for (c, f), w in zip(cases, want):
+            q, kp, vp, ke, ve, tables, starts, pos = map(dev, c)
+            n = np.diff(c[6])
+            out = torch.full_like(q, 9.0)
+            kvcache.attn_f8_paged(q, kp, vp, ke, ve, out, ws, tables, starts, pos, max_tok=int(n.max()),
+                                  max_ctx=int((c[7] + n).max()), scale=f)
+            assert np.array_equal(out.cpu().numpy(), w), turn
 
 
 def test_offsets_past_four_gigabytes():
