@@ -112,13 +112,14 @@ __device__ __forceinline__ RowTile row_tile(const F8AttnArgs& p, const Slot& x, 
   return r;
 }
 
-// Key units (PER tiles each) of entry x = slot * slot_tiles + row tile
-template <int ROWS, int KT, int PER>
+// Units of entry x = slot * slot_tiles + row tile: its key tiles, and LEAD for what a row tile
+// costs beside them (its queries, first loads and output)
+template <int ROWS, int KT, int LEAD>
 __device__ __forceinline__ int entry_units(const F8AttnArgs& p, int x, int gqa) {
   const int s = x / p.slot_tiles, i = x - s * p.slot_tiles;
   const Slot sl = slot_of(p, s);
   if (i * ROWS >= sl.n * gqa) return 0;
-  return (row_tile<ROWS, KT>(p, sl, i, gqa).tiles + PER - 1) / PER;
+  return LEAD + row_tile<ROWS, KT>(p, sl, i, gqa).tiles;
 }
 
 // Where a workgroup's part begins: entry and unit in it, and the units of one head.
@@ -149,27 +150,27 @@ __device__ __forceinline__ int block_scan(int v, int* lds, int& sum) {   // incl
 }
 
 // The units of one head's line
-template <int ROWS, int KT, int PER, int THREADS>
+template <int ROWS, int KT, int LEAD, int THREADS>
 __device__ __forceinline__ int line_units(const F8AttnArgs& p, int gqa, int* lds) {
   const int entries = p.n_slots * p.slot_tiles;
   int base = 0;
   for (int c = 0; c < entries; c += THREADS) {
     const int x = c + threadIdx.x;
     int sum;
-    block_scan<THREADS>(x < entries ? entry_units<ROWS, KT, PER>(p, x, gqa) : 0, lds, sum);
+    block_scan<THREADS>(x < entries ? entry_units<ROWS, KT, LEAD>(p, x, gqa) : 0, lds, sum);
     base += sum;
   }
   return base;
 }
 // The entry that holds unit u of the line (u < its length)
-template <int ROWS, int KT, int PER, int THREADS>
+template <int ROWS, int KT, int LEAD, int THREADS>
 __device__ __forceinline__ Part line_find(const F8AttnArgs& p, int gqa, int total, int u, int* lds) {
   const int entries = p.n_slots * p.slot_tiles;
   __shared__ int found[2];
   int base = 0;
   for (int c = 0; c < entries; c += THREADS) {
     const int x = c + threadIdx.x;
-    const int mine = x < entries ? entry_units<ROWS, KT, PER>(p, x, gqa) : 0;
+    const int mine = x < entries ? entry_units<ROWS, KT, LEAD>(p, x, gqa) : 0;
     int sum;
     const int inc = base + block_scan<THREADS>(mine, lds, sum);
     if (u >= inc - mine && u < inc) {
@@ -817,9 +818,12 @@ __global__ __launch_bounds__(256, 1) void f8_mid_kernel(F8AttnArgs p) {
 // by dim, four keys to 8 bytes, in the order that the scores' lanes hold them.  Pads
 // keep 16-byte reads of 16 lanes on distinct banks, at constant offsets of one address.
 
+// A row tile's cost beside its key tiles, in tiles (11 against 2.1 us)
+constexpr int kLead = 4;
+
 template <int HD>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void f8_many_kernel(F8AttnArgs p) {
-  constexpr int WAVES = 8, ROWS = 32 * WAVES, THREADS = 64 * WAVES, PER = 1;
+  constexpr int WAVES = 8, ROWS = 32 * WAVES, THREADS = 64 * WAVES, LEAD = kLead;
   constexpr int KT = 8192 / HD;              // 32 or 64 keys: 8 KB of codes
   constexpr int KH = KT / 32;                // 32-key halves
   constexpr int WK = KT / WAVES;             // keys that a wave loads and converts
@@ -835,7 +839,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const int c = lane & 31, hh = lane >> 5;
   const int gqa = p.num_q / p.num_kv;
 
-  const int total = line_units<ROWS, KT, PER, THREADS>(p, gqa, lds);
+  const int total = line_units<ROWS, KT, LEAD, THREADS>(p, gqa, lds);
   if (blockIdx.x == 0 && tid == 0) p.cuts[4 * p.groups] = total * p.num_kv;
   // neighbouring parts (the same head's keys) on one XCD, whose L2 holds their tiles
   const Parts parts(total * p.num_kv, p.groups);
@@ -844,7 +848,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   int u = parts.begin(grp);
   const int u_end = parts.begin(grp + 1);
   int h = u / total;
-  Part at = line_find<ROWS, KT, PER, THREADS>(p, gqa, total, u - h * total, lds);
+  Part at = line_find<ROWS, KT, LEAD, THREADS>(p, gqa, total, u - h * total, lds);
   bool first_seg = true;
   const uint32_t key_bytes = (uint32_t)p.num_kv * HD;
   const uint32_t page_bytes = (uint32_t)p.block_tokens * key_bytes;
@@ -863,8 +867,14 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       continue;
     }
     const RowTile rt = row_tile<ROWS, KT>(p, sl, rti, gqa);
-    const int n_u = min(rt.tiles - at.at, u_end - u);
-    const int v0 = at.at, v1 = at.at + n_u;
+    const int n_u = min(LEAD + rt.tiles - at.at, u_end - u);
+    const int v0 = max(at.at - LEAD, 0), v1 = at.at + n_u - LEAD;   // (v1 <= v0: the next part's)
+    // where the part begins, for the merge: row tile (-1: not past its first key tile), head, tile,
+    // tiles
+    if (first_seg && tid == 0)
+      *reinterpret_cast<int4*>(p.cuts + 4 * grp) = make_int4(v0 > 0 ? at.entry : -1, h, v0, rt.tiles);
+    const bool complete = v0 == 0 && v1 == rt.tiles;
+    if (v1 > v0) {
     const int rows = sl.n * gqa;
     const int row_w = rti * ROWS + wave * 32;      // this wave's first row
     const int row = min(row_w + c, rows - 1), tok = row / gqa;
@@ -1104,10 +1114,6 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     }
 
     ls = sum32(ls);
-    const bool complete = n_u == rt.tiles;
-    // where the part begins, for the merge: row tile (-1: at its first unit), head, unit, units
-    if (first_seg && tid == 0)
-      *reinterpret_cast<int4*>(p.cuts + 4 * grp) = make_int4(v0 > 0 ? at.entry : -1, h, v0, rt.tiles);
     if (row_w + c < rows) {
       if (complete) {
         const float inv = ls > 0.f ? 1.f / ls : 0.f;
@@ -1130,6 +1136,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
             ro[(4 * d + a) * 64] = f4_t{acc[d][4 * a], acc[d][4 * a + 1], acc[d][4 * a + 2], acc[d][4 * a + 3]};
         if (hh == 0) *reinterpret_cast<f2_t*>(p.rec_ml + (rec * ROWS + 32 * wave + c) * 2) = f2_t{mx, ls};
       }
+    }
     }
     first_seg = false;
     u += n_u;
@@ -1156,10 +1163,11 @@ __global__ __launch_bounds__(256) void f8_cut_merge_kernel(F8AttnArgs p) {
   if (grp >= parts.n) return;
   const int entry = cut.x, h = cut.y, v0 = cut.z, tiles = cut.w;
   if (entry < 0) return;
-  const int x0 = parts.begin(grp) - v0, before = parts.begin(grp - 1);
-  if (before > x0) return;   // an earlier cut is in this tile
-  const int n = parts.of(x0 + tiles - 1) - grp + 2;
-  const long r0 = 2 * (grp - 1) + (before == x0 ? 0 : 1);
+  // units of the row tile's first key tile, and of its lead
+  const int x1 = parts.begin(grp) - v0, x0 = x1 - kLead, before = parts.begin(grp - 1);
+  if (before > x1) return;   // an earlier cut is in this tile
+  const int n = parts.of(x1 + tiles - 1) - grp + 2;
+  const long r0 = 2 * (grp - 1) + (before >= x0 ? 0 : 1);
   auto rec_of = [&](int i) { return i == 0 ? r0 : 2l * (grp - 1 + i); };
   const int s = entry / p.slot_tiles, gqa = p.num_q / p.num_kv;
   const Slot sl = slot_of(p, s);
@@ -1288,7 +1296,7 @@ F8AttnPlan f8_attn_plan(int num_q, int num_kv, int head_dim, int n_slots, long q
     x.rec_rows = tile_rows;
     // (a slot has at most one row tile that is not full)
     const long tiles = std::min<long>((long)n_slots * x.slot_tiles, q_rows * (num_q / num_kv) / tile_rows + n_slots);
-    units = tiles * num_kv * ((max_ctx + kt - 1) / kt);
+    units = tiles * num_kv * ((max_ctx + kt - 1) / kt);   // (key tiles: a part for less would be all lead)
     x.groups = (int)std::min<long>(units, 256);
     x.merges = true;
   } else {
