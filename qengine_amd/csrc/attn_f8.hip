@@ -232,15 +232,13 @@ struct SlotLine {
       if (lane >= d) inc += o;
     }
   }
-  // units of all slots; `keep`: their prefix, for the merge
-  __device__ __forceinline__ int total(bool keep) {
+  // units of all slots
+  __device__ __forceinline__ int total() {
     int t = 0;
     for (int b = 0; b < p.n_slots; b += 64) {
       load(b);
-      if (keep && b + lane < p.n_slots) p.pre[b + lane + 1] = t + inc;
       t += __builtin_amdgcn_readlane(inc, 63);
     }
-    if (keep && lane == 0) p.pre[0] = 0;
     return t;
   }
   // the slot (lane of the loaded ones) that holds unit u of the line, and the unit in it
@@ -318,7 +316,7 @@ __global__ __launch_bounds__(256, 2) void f8_few_kernel(F8AttnArgs p) {
   const int gqa = p.num_q / p.num_kv;
 
   SlotLine<ROWS, KT, PER> line(p, gqa);
-  const int total = line.total(blockIdx.x == 0 && wave == 0);
+  const int total = line.total();
   const Parts parts(total * p.num_kv, p.groups);
   const int grp = blockIdx.x;
   if (grp >= parts.n) return;
@@ -338,6 +336,11 @@ __global__ __launch_bounds__(256, 2) void f8_few_kernel(F8AttnArgs p) {
     const int rows = sl.n * gqa;
     const int v_end = min((at + n_u) * PER, rt.tiles);
     const const_i32* table = (const const_i32*)(p.tables + (long)(line.base + e) * p.max_blocks);
+    // for the merge: the parts that hold the tile, and its first record
+    if (!JOIN && at == 0 && tid == 0) {
+      const int n = parts.of(u + units - 1) - grp + 1;
+      p.desc[(line.base + e) * p.num_kv + h] = make_int2(n, 2 * grp + (first_seg ? 0 : 1));
+    }
 
     u4_t kr[2][KW];
     uint32_t vr[8][VD];
@@ -602,7 +605,7 @@ __global__ __launch_bounds__(256, 1) void f8_mid_kernel(F8AttnArgs p) {
   const int gqa = p.num_q / p.num_kv;
 
   SlotLine<ROWS, KT, PER> line(p, gqa);
-  const int total = line.total(blockIdx.x == 0 && wave == 0);
+  const int total = line.total();
   const Parts parts(total * p.num_kv, p.groups);
   const int grp = blockIdx.x;
   if (grp >= parts.n) return;
@@ -623,6 +626,11 @@ __global__ __launch_bounds__(256, 1) void f8_mid_kernel(F8AttnArgs p) {
     // a wave without rows loads nothing (the others wait for nobody)
     const int v_end = 32 * rg < rows ? min((at + n_u) * PER, rt.tiles) : 0;
     const const_i32* table = (const const_i32*)(p.tables + (long)(line.base + e) * p.max_blocks);
+    // for the merge: the parts that hold the tile, and its first record
+    if (at == 0 && tid == 0) {
+      const int n = parts.of(u + units - 1) - grp + 1;
+      p.desc[(line.base + e) * p.num_kv + h] = make_int2(n, 2 * grp + (first_seg ? 0 : 1));
+    }
 
     u4_t kr[KW];
     uint32_t vr[16][VD];
@@ -818,8 +826,8 @@ __global__ __launch_bounds__(256, 1) void f8_mid_kernel(F8AttnArgs p) {
 // by dim, four keys to 8 bytes, in the order that the scores' lanes hold them.  Pads
 // keep 16-byte reads of 16 lanes on distinct banks, at constant offsets of one address.
 
-// A row tile's cost beside its key tiles, in tiles (11 against 2.1 us)
-constexpr int kLead = 4;
+// A row tile's cost beside its key tiles, in tiles (11 us against 2.1; six ragged prompts: 187 us at 2, 156 at 4 and 6, 165 at 9)
+constexpr int kLead = 6;
 
 template <int HD>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void f8_many_kernel(F8AttnArgs p) {
@@ -1210,22 +1218,13 @@ template <int HD>
 __global__ __launch_bounds__(256) void f8_merge_kernel(F8AttnArgs p) {
   constexpr int E = HD / 64;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int entries = p.n_slots * p.slot_tiles;
   const int tile = blockIdx.x / p.rec_rows, row = blockIdx.x - tile * p.rec_rows;
-  const int entry = tile % entries, h = tile / entries;
-  const int total = p.pre[entries], a = p.pre[entry], b = p.pre[entry + 1];
-  if (a == b) return;
-  const int x0 = h * total + a, x1 = h * total + b;
-  const Parts parts(total * p.num_kv, p.groups);
-  // the parts that hold the tile's first and last unit
-  const int g0 = parts.of(x0), g1 = parts.of(x1 - 1);
-  if (g0 == g1) return;   // stored whole
-  const int r0 = 2 * g0 + (parts.begin(g0) == x0 ? 0 : 1);
-  const int n = g1 - g0 + 1;
-  auto rec_of = [&](int i) { return i == 0 ? r0 : 2 * (g0 + i); };
-  const int s = entry / p.slot_tiles, gqa = p.num_q / p.num_kv;
+  const int s = tile / p.num_kv, h = tile - s * p.num_kv, gqa = p.num_q / p.num_kv;
+  const int2 desc = p.desc[tile];
   const Slot sl = slot_of(p, s);
-  if (row >= sl.n * gqa) return;
+  const int n = desc.x, r0 = desc.y;
+  if (row >= sl.n * gqa || n < 2) return;   // (one part: stored whole)
+  auto rec_of = [&](int i) { return i == 0 ? r0 : 2 * (r0 / 2 + i); };
 
   // 64 records a round: lane i holds record i's {m, l}, the wave reads 16 records' sums (all
   // of a round's loads are under way before the first is used), weights by lane reads
@@ -1310,7 +1309,7 @@ F8AttnPlan f8_attn_plan(int num_q, int num_kv, int head_dim, int n_slots, long q
     x.groups = (int)std::min<long>(units, x.row_tiles == 1 ? 512 : 256);
     x.merges = max_ctx > unit_keys;   // (else no slot has two units)
   }
-  const size_t ints = x.many ? 4 * (size_t)x.groups + 4 : (size_t)n_slots + 1;
+  const size_t ints = x.many ? 4 * (size_t)x.groups + 4 : 2 * (size_t)n_slots * num_kv;
   const size_t pre = kJoinCounts * 4 + (ints * 4 + 255) / 256 * 256;
   const size_t recs = x.merges ? 2 * (size_t)x.groups * x.rec_rows : 0;
   x.ml_off = pre;

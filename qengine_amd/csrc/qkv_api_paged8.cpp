@@ -232,7 +232,8 @@ int qkv_attn_f8_paged(const uint16_t* q, const uint8_t* k_pool, const uint8_t* v
   a.starts = starts;
   a.positions = positions;
   a.counts = reinterpret_cast<int*>(ws);
-  a.pre = a.cuts = a.counts + qkv::kJoinCounts;
+  a.cuts = a.counts + qkv::kJoinCounts;
+  a.desc = reinterpret_cast<int2*>(a.cuts);
   a.rec_ml = reinterpret_cast<float*>(ws + x.ml_off);
   a.rec_o = reinterpret_cast<float*>(ws + x.o_off);
   a.rows = n_rows;

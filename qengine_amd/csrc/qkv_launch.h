@@ -172,7 +172,7 @@ struct F8AttnArgs {
   const int32_t* starts;
   const int32_t* positions;
   int* counts;               // workspace, its first kJoinCounts ints: zero between calls
-  int* pre;                  // workspace: unit prefix of the slots, [n_slots + 1] (few rows)
+  int2* desc;                // workspace: [n_slots][num_kv] {parts, first record} of a row tile (few rows)
   int* cuts;                 // workspace, the same place: [groups][4] where each part begins, then
                              // the units of all heads (many rows)
   float* rec_ml;             // workspace: {m (log2 units), l} of a partial row
