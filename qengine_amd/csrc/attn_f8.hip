@@ -15,6 +15,7 @@
 // (m, l, O) that the merge kernel joins.  A part has at most two cut ends, hence two
 // records a workgroup.
 #include <algorithm>
+#include <type_traits>
 
 #include "attn_common.h"
 #include "qkv_device.h"
@@ -591,6 +592,9 @@ __global__ __launch_bounds__(256, 2) void f8_few_kernel(F8AttnArgs p) {
 // side on the same keys (the second's loads meet the first's lines in the caches), 4 / RG
 // key streams.  Otherwise as above: lane l%32 is the key of K's operand and takes 16 of
 // every 32 dims; V comes by runs of HD/32 dims, and output block d has dims HD/32 * m + d.
+// One wave a SIMD holds the sums, so the codes of two tiles ahead wait in LDS, loaded there
+// past the registers (32 KB a wave at head_dim 256).  K's 16-byte chunks are permuted within
+// a row by the row's number, which keeps its reads on distinct banks.
 template <int HD, int RG>
 __global__ __launch_bounds__(256, 1) void f8_mid_kernel(F8AttnArgs p) {
   constexpr int KT = 32, ROWS = 32 * RG, KG = 4 / RG, PER = KG, THREADS = 256;
@@ -598,7 +602,13 @@ __global__ __launch_bounds__(256, 1) void f8_mid_kernel(F8AttnArgs p) {
   constexpr int DB = HD / 32;        // 32-dim blocks of the output, value bytes of a lane and key
   constexpr int VD = DB / 4;         // value dwords of a lane and key
   constexpr int PITCH = HD + 4;
-  __shared__ float red[4 * 32 * PITCH];
+  constexpr int TB = KT * HD;        // bytes of a tile's K or V codes
+  constexpr int RL = 1024 / HD;      // rows of a 1 KB load
+  __shared__ __align__(16) union {
+    uint8_t ring[4][2][2][TB];       // wave, tile parity, K / V
+    float red[4 * 32 * PITCH];       // (after the last tile)
+  } sm;
+  float* red = sm.red;
   __shared__ float ml[KG][ROWS][2];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 31, hh = lane >> 5, rg = wave % RG, kg = wave / RG;
@@ -615,7 +625,9 @@ __global__ __launch_bounds__(256, 1) void f8_mid_kernel(F8AttnArgs p) {
   int e = line.find(u - h * total, at);
   bool first_seg = true;
   const uint32_t key_bytes = (uint32_t)p.num_kv * HD;
-  const uint32_t k_off = (c & 15) * key_bytes + 16 * hh, v_off = 4 * hh * key_bytes + c * DB;
+  // a load's lane: row lane / (HD/16), its chunk permuted by the row (K) or in place (V)
+  const int ld_row = lane / (HD / 16), ld_chunk = lane % (HD / 16);
+  const uint32_t v_off = ld_row * key_bytes + ld_chunk * 16;
 
   while (true) {
     const Slot sl = line.slot(e);
@@ -632,49 +644,41 @@ __global__ __launch_bounds__(256, 1) void f8_mid_kernel(F8AttnArgs p) {
       p.desc[(line.base + e) * p.num_kv + h] = make_int2(n, 2 * grp + (first_seg ? 0 : 1));
     }
 
-    u4_t kr[KW];
-    uint32_t vr[16][VD];
-    uint32_t ke[2], ve[2];
-    auto load_k = [&](const Tile& t) {
-      // the lane's key is in the first or the second half
-      const uint8_t* base[2];
+    uint8_t* ring = sm.ring[wave][0][0];
+    auto load = [&](const Tile& t, int to_par) {   // (to_par: byte offset of the parity's codes)
 #pragma unroll
       for (int hf = 0; hf < 2; hf++) {
-        const long pg = max(t.pg[hf], 0);
-        base[hf] = p.k_pool + (pg * p.block_tokens + t.row[hf]) * key_bytes + (long)h * HD;
-        ke[hf] = p.k_exp[pg * p.num_kv + h];
-      }
-      const uint8_t* src = (c < 16 ? base[0] : base[1]) + k_off;
+        const long pg = max(t.pg[hf], 0), from = (pg * p.block_tokens + t.row[hf]) * key_bytes + (long)h * HD;
 #pragma unroll
-      for (int i = 0; i < KW; i++) kr[i] = *reinterpret_cast<const u4_t*>(src + 32 * i);
-    };
-    auto load_v = [&](const Tile& t) {
-      // keys 16 hf + 8 a + 4 hh + i
-#pragma unroll
-      for (int hf = 0; hf < 2; hf++) {
-        const long pg = max(t.pg[hf], 0);
-        const uint8_t* base = p.v_pool + (pg * p.block_tokens + t.row[hf]) * key_bytes + (long)h * HD;
-        ve[hf] = p.v_exp[pg * p.num_kv + h];
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-          const uint8_t* src = base + (long)(8 * (i >> 2) + (i & 3)) * key_bytes + v_off;
-          if constexpr (VD == 2) {
-            const u2_t w = *reinterpret_cast<const u2_t*>(src);
-            vr[8 * hf + i][0] = w[0];
-            vr[8 * hf + i][1] = w[1];
-          } else {
-            vr[8 * hf + i][0] = *reinterpret_cast<const uint32_t*>(src);
-          }
+        for (int l = 0; l < 16 / RL; l++) {
+          const int r0 = l * RL;     // first row of the load, in the half
+          const uint32_t k_off = ld_row * key_bytes + ((ld_chunk ^ ((r0 + ld_row) & (HD / 16 - 1))) * 16);
+          const int to = (16 * hf + r0) * HD;
+          __builtin_amdgcn_global_load_lds((glb_void*)(p.k_pool + from + (long)r0 * key_bytes + k_off), (lds_void*)(ring + to_par + to), 16, 0, 0);
+          __builtin_amdgcn_global_load_lds((glb_void*)(p.v_pool + from + (long)r0 * key_bytes + v_off), (lds_void*)(ring + to_par + TB + to), 16, 0, 0);
         }
+      }
+    };
+    uint32_t ke[2], ve[2];           // a tile's exponents by half, loaded a tile ahead
+    auto load_exp = [&](const Tile& t) {
+#pragma unroll
+      for (int hf = 0; hf < 2; hf++) {
+        const long pg = max(t.pg[hf], 0);
+        ke[hf] = p.k_exp[pg * p.num_kv + h];
+        ve[hf] = p.v_exp[pg * p.num_kv + h];
       }
     };
 
     int v = at * PER + kg;
-    Tile cur{}, nxt{};
+    Tile cur{}, nxt{}, far{};        // tiles v, v + PER (both loaded) and v + 2 PER
     if (v < v_end) {
       cur = tile_at(p, table, rt.key0(v, KT), rt.end);
-      load_k(cur);
-      load_v(cur);
+      load(cur, 0);
+      load_exp(cur);
+    }
+    if (v + PER < v_end) {
+      nxt = tile_at(p, table, rt.key0(v + PER, KT), rt.end);
+      load(nxt, 2 * TB);
     }
     // ---- queries: row c of the wave, dims 32 i + 16 hh + 8 x ..
     h8_t qf[KW][2];
@@ -687,39 +691,44 @@ __global__ __launch_bounds__(256, 1) void f8_mid_kernel(F8AttnArgs p) {
 #pragma unroll
         for (int x = 0; x < 2; x++) qf[i][x] = *reinterpret_cast<const h8_t*>(src + 32 * i + 8 * x);
     }
-    if (v + PER < v_end) nxt = tile_at(p, table, rt.key0(v + PER, KT), rt.end);
+    if (v + 2 * PER < v_end) far = tile_at(p, table, rt.key0(v + 2 * PER, KT), rt.end);
 
     f16x_t acc[DB];
     float mx = -INFINITY, ls = 0.f;
 #pragma unroll
     for (int d = 0; d < DB; d++) acc[d] = f16x_t{};
 
-    for (; v < v_end; v += PER) {
+    for (int par = 0; v < v_end; v += PER, par ^= 2 * TB) {
       const bool more = v + PER < v_end;
+      // this tile's codes have landed; the next one's (all newer) may be under way
+      if (more) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(64 / RL) : "memory");
+      else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      const float k0 = pow2f(ke[0]), k1 = pow2f(ke[1]), vf[2] = {pow2f(ve[0]), pow2f(ve[1])};
+      if (more) load_exp(nxt);
+      const uint8_t* kt = ring + par + c * HD;
+      const uint8_t* vt = ring + par + TB + 4 * hh * HD + c * DB;
       // ---- scores: lane c's row, keys 8 (x / 4) + 4 hh + x % 4
       f16x_t sc = f16x_t{};
-      const float f = pow2f(c < 16 ? ke[0] : ke[1]);
+      const float f = c < 16 ? k0 : k1;
 #pragma unroll
-      for (int i = 0; i < KW; i++)
+      for (int i = 0; i < KW; i++) {
+        const u4_t kr = *reinterpret_cast<const u4_t*>(kt + (((2 * i + hh) ^ (c & (HD / 16 - 1))) * 16));
 #pragma unroll
         for (int x = 0; x < 2; x++)
           sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(
-              join8(cvt2(kr[i][2 * x], f, false), cvt2(kr[i][2 * x], f, true), cvt2(kr[i][2 * x + 1], f, false),
-                    cvt2(kr[i][2 * x + 1], f, true)),
+              join8(cvt2(kr[2 * x], f, false), cvt2(kr[2 * x], f, true), cvt2(kr[2 * x + 1], f, false),
+                    cvt2(kr[2 * x + 1], f, true)),
               qf[i][x], sc, 0, 0, 0);
+      }
       sc *= p.scale_log2;
       const bool whole = cur.pg[0] >= 0 && cur.pg[1] >= 0 && cur.key0 + KT - 1 <= rt.pos_lo && cur.key0 + KT <= rt.end &&
                          (p.window <= 0 || cur.key0 > rt.pos_hi - p.window || cur.key0 + KT <= p.sink);
-      if (more) load_k(nxt);
       if (!whole) {
 #pragma unroll
         for (int x = 0; x < 16; x++) {
           const int key = cur.key0 + 8 * (x >> 2) + 4 * hh + (x & 3);
-          const bool there = cur.pg[x >> 3] >= 0 && key < rt.end;
+          const bool there = cur.pg[x >> 3] >= 0;
           sc[x] = there && sees(key, pos_r, rt.end, p.window, p.sink) ? sc[x] : -INFINITY;
-          // rows past the last key hold whatever the page held before
-#pragma unroll
-          for (int d = 0; d < VD; d++) vr[x][d] = there ? vr[x][d] : 0u;
         }
       }
       float t = sc[0];
@@ -741,34 +750,55 @@ __global__ __launch_bounds__(256, 1) void f8_mid_kernel(F8AttnArgs p) {
 #pragma unroll
         for (int i = 0; i < 8; i++) pb[i] = (_Float16)__builtin_amdgcn_exp2f(sc[8 * hf + i] - base);
         ls = add8(pb, ls);
-        const float vf = pow2f(ve[hf]);
+        uint32_t vr[8][VD];          // keys 16 hf + 8 a + 4 hh + i
+#pragma unroll
+        for (int x = 0; x < 8; x++) {
+          const uint8_t* src = vt + (16 * hf + 8 * (x >> 2) + (x & 3)) * HD;
+          if constexpr (VD == 2) {
+            const u2_t w = *reinterpret_cast<const u2_t*>(src);
+            vr[x][0] = w[0];
+            vr[x][1] = w[1];
+          } else {
+            vr[x][0] = *reinterpret_cast<const uint32_t*>(src);
+          }
+        }
+        if (!whole) {   // rows past the last key hold whatever the page held before
+#pragma unroll
+          for (int x = 0; x < 8; x++) {
+            const int key = cur.key0 + 16 * hf + 8 * (x >> 2) + 4 * hh + (x & 3);
+#pragma unroll
+            for (int d = 0; d < VD; d++) vr[x][d] = cur.pg[hf] >= 0 && key < rt.end ? vr[x][d] : 0u;
+          }
+        }
 #pragma unroll
         for (int d = 0; d < VD; d++) {
           uint32_t w[4][2];   // key pairs x byte pairs
 #pragma unroll
           for (int k = 0; k < 4; k++) {
-            w[k][0] = __builtin_amdgcn_perm(vr[8 * hf + 2 * k + 1][d], vr[8 * hf + 2 * k][d], 0x05010400u);
-            w[k][1] = __builtin_amdgcn_perm(vr[8 * hf + 2 * k + 1][d], vr[8 * hf + 2 * k][d], 0x07030602u);
+            w[k][0] = __builtin_amdgcn_perm(vr[2 * k + 1][d], vr[2 * k][d], 0x05010400u);
+            w[k][1] = __builtin_amdgcn_perm(vr[2 * k + 1][d], vr[2 * k][d], 0x07030602u);
           }
 #pragma unroll
           for (int j = 0; j < 4; j++)
             acc[4 * d + j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
-                join8(cvt2(w[0][j >> 1], vf, j & 1), cvt2(w[1][j >> 1], vf, j & 1), cvt2(w[2][j >> 1], vf, j & 1),
-                      cvt2(w[3][j >> 1], vf, j & 1)),
+                join8(cvt2(w[0][j >> 1], vf[hf], j & 1), cvt2(w[1][j >> 1], vf[hf], j & 1), cvt2(w[2][j >> 1], vf[hf], j & 1),
+                      cvt2(w[3][j >> 1], vf[hf], j & 1)),
                 pb, acc[4 * d + j], 0, 0, 0);
         }
       }
-      if (more) {
-        load_v(nxt);
-        cur = nxt;
-        if (v + 2 * PER < v_end) nxt = tile_at(p, table, rt.key0(v + 2 * PER, KT), rt.end);
-      }
+      // (every read of this tile's codes is done: its registers have been used)
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      if (v + 2 * PER < v_end) load(far, par);
+      cur = nxt;
+      nxt = far;
+      if (v + 3 * PER < v_end) far = tile_at(p, table, rt.key0(v + 3 * PER, KT), rt.end);
     }
 
     // ---- join the streams; lane c holds dims DB * (8 (x / 4) + 4 hh + x % 4) + d of row c
     const bool complete = n_u == units;
     const int rec = 2 * grp + (first_seg ? 0 : 1);
     ls = sum32(ls);
+    __syncthreads();   // (the ring is done with)
     if (hh == 0) {
       ml[kg][32 * rg + c][0] = mx;
       ml[kg][32 * rg + c][1] = ls;

@@ -105,16 +105,19 @@ __device__ __forceinline__ uint32_t rescale4(uint32_t codes, float f) {
 // One workgroup per (slot, touched page, KV head, K or V); the workgroups past those
 // rotate query rows.  The rows of a page stay in registers between the maximum and
 // the store where KEEP 8-element runs a thread hold them (a 64-row page of 256).
-template <int THREADS>
-__global__ __launch_bounds__(THREADS) void f8_append_kernel(F8AppendArgs p) {
+template <int THREADS, bool ROPE>
+__global__ __launch_bounds__(THREADS, ROPE || THREADS == 1024 ? 4 : 8) void f8_append_kernel(F8AppendArgs p) {
   constexpr int KEEP = 8;
   const int tid = threadIdx.x;
-  const int hd = p.head_dim, cpr = hd / 8;
+  const int hd = p.head_dim, cpr = hd / 8, cpr_log = hd == 256 ? 5 : 4;   // (head_dim is 128 or 256)
   const RowRope rope{p.turns, p.amplitude, p.rot, p.layout};
   long wg = blockIdx.x;
-  if (wg >= p.kv_wgs) {   // query rows: 16 elements a thread, both sides of its pairs (they may be in place)
+  if (ROPE && wg >= p.kv_wgs) {
+    // query rows: 16 elements of QH heads a thread, both sides of their pairs (they may be in place),
+    // whose cosines are formed once
+    constexpr int QH = 4;
     const long u = (wg - p.kv_wgs) * THREADS + tid;
-    const int per_tok = p.num_q * (hd / 16);
+    const int per_head = hd / 16, per_tok = (p.num_q + QH - 1) / QH * per_head;
     const long tok = u / per_tok;
     if (tok >= p.rows) return;
     // the slot of the token: the last whose start is not past it
@@ -126,21 +129,36 @@ __global__ __launch_bounds__(THREADS) void f8_append_kernel(F8AppendArgs p) {
     const int s0 = p.starts[lo];
     // (not behind the last slot, nor past what the call covers of this one)
     if (tok < s0 || tok >= p.starts[lo + 1] || tok - s0 >= p.max_tok || p.positions[lo] < 0) return;
-    const int r = (int)(u - tok * per_tok), h = r / (hd / 16), c = r - h * (hd / 16);
-    const uint16_t* in = p.q + tok * p.q_stride + (long)h * hd;
-    uint16_t* out = p.q_out + tok * p.q_out_stride + (long)h * hd;
+    const int r = (int)(u - tok * per_tok), c = r % per_head, h0 = r / per_head * QH;
     const RopeRuns run = rope_runs(c, rope.rot, rope.layout);
-    u4_t x = *reinterpret_cast<const u4_t*>(in + run.a0), y = *reinterpret_cast<const u4_t*>(in + run.a1);
+    const uint16_t* in = p.q + tok * p.q_stride;
+    uint16_t* out = p.q_out + tok * p.q_out_stride;
+    if (!run.turned && in == out) return;
+    u4_t x[QH], y[QH];
+#pragma unroll
+    for (int i = 0; i < QH; i++) {
+      const uint16_t* at = in + (long)min(h0 + i, p.num_q - 1) * hd;
+      x[i] = *reinterpret_cast<const u4_t*>(at + run.a0);
+      y[i] = *reinterpret_cast<const u4_t*>(at + run.a1);
+    }
     if (run.turned) {
       const int pos = p.positions[lo] + (int)(tok - s0);
       float cs[8], sn[8];
 #pragma unroll
       for (int i = 0; i < 8; i++) rope_cos_sin(pos, rope.turns[8 * c + i], rope.amp, cs[i], sn[i]);
-      if (rope.layout == 0) turn8(x, y, cs, sn, x, y);
-      else turn8_pairs(x, y, cs, sn, x, y);
+#pragma unroll
+      for (int i = 0; i < QH; i++) {
+        if (rope.layout == 0) turn8(x[i], y[i], cs, sn, x[i], y[i]);
+        else turn8_pairs(x[i], y[i], cs, sn, x[i], y[i]);
+      }
     }
-    *reinterpret_cast<u4_t*>(out + run.a0) = x;
-    *reinterpret_cast<u4_t*>(out + run.a1) = y;
+#pragma unroll
+    for (int i = 0; i < QH; i++) {
+      if (h0 + i >= p.num_q) break;
+      uint16_t* at = out + (long)(h0 + i) * hd;
+      *reinterpret_cast<u4_t*>(at + run.a0) = x[i];
+      *reinterpret_cast<u4_t*>(at + run.a1) = y[i];
+    }
     return;
   }
   const bool is_v = wg & 1;
@@ -166,10 +184,10 @@ __global__ __launch_bounds__(THREADS) void f8_append_kernel(F8AppendArgs p) {
   uint8_t* exp_at = (is_v ? p.v_exp : p.k_exp) + (long)page * p.num_kv + h;
   const int was = off > 0 ? min((int)*exp_at, 254) : 0;
 
-  const bool turn = !is_v && p.rot > 0;
+  const bool turn = ROPE && !is_v;
   const int units = rows * cpr;
   auto load = [&](int u) {
-    const int r = u / cpr, c = u - r * cpr;
+    const int r = u >> cpr_log, c = u & (cpr - 1);
     const uint16_t* row = in + r * stride;
     return limit8(turn ? load_turned(row, c, (int)(first + r), rope) : *reinterpret_cast<const u4_t*>(row + 8 * c));
   };
@@ -194,7 +212,7 @@ __global__ __launch_bounds__(THREADS) void f8_append_kernel(F8AppendArgs p) {
   const int e = max(f8_exponent(top), was);
   const float inv = pow2_bits(254 - e);
   auto store = [&](int u, u4_t v) {
-    const int r = u / cpr, c = u - r * cpr;
+    const int r = u >> cpr_log, c = u & (cpr - 1);
     *reinterpret_cast<u2_t*>(pool + (long)(off + r) * row_bytes + 8 * c) = encode8(v, inv);
   };
 #pragma unroll
@@ -204,7 +222,7 @@ __global__ __launch_bounds__(THREADS) void f8_append_kernel(F8AppendArgs p) {
   if (off > 0 && e > was) {   // the older rows, at the raised exponent
     const float f = pow2_bits(127 - min(e - was, 126));
     for (int u = tid; u < off * cpr; u += THREADS) {
-      const int r = u / cpr, c = u - r * cpr;
+      const int r = u >> cpr_log, c = u & (cpr - 1);
       u2_t* at = reinterpret_cast<u2_t*>(pool + (long)r * row_bytes + 8 * c);
       const u2_t v = *at;
       *at = u2_t{rescale4(v[0], f), rescale4(v[1], f)};
@@ -216,16 +234,19 @@ __global__ __launch_bounds__(THREADS) void f8_append_kernel(F8AppendArgs p) {
 hipError_t launch_f8_append(F8AppendArgs a, hipStream_t stream) {
   a.spans = (a.max_tok + a.block_tokens - 2) / a.block_tokens + 1;
   const long kv = (long)a.n_slots * a.spans * a.num_kv * 2;
-  const long q_units = a.q ? a.rows * a.num_q * (a.head_dim / 16) : 0;
-  // a wave where a page's new rows are few (a decode step), else four
-  const int threads = (long)std::min(a.max_tok, a.block_tokens) * a.head_dim <= 64 * 8 * 4 ? 64 : 256;
+  const long q_units = a.q ? a.rows * ((a.num_q + 3) / 4) * (a.head_dim / 16) : 0;
+  // As many threads as hold a page's new rows in their registers: a wave in a decode step, 256 for
+  // 64 rows of 256, 1,024 for longer pages (256-row pages, 8,192 tokens: 29.7 us with 256).
+  const long elems = (long)std::min(a.max_tok, a.block_tokens) * a.head_dim;
+  const int threads = elems <= 64 * 8 * 4 ? 64 : elems <= 256 * 8 * 8 ? 256 : 1024;
   const long wgs = kv + (q_units + threads - 1) / threads;
   if (wgs > 0x7fffffffL) return hipErrorInvalidValue;
   a.kv_wgs = kv;
-  if (threads == 64)
-    hipLaunchKernelGGL(f8_append_kernel<64>, dim3((unsigned)wgs), dim3(64), 0, stream, a);
-  else
-    hipLaunchKernelGGL(f8_append_kernel<256>, dim3((unsigned)wgs), dim3(256), 0, stream, a);
+  const dim3 grid((unsigned)wgs), block((unsigned)threads);
+  auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, stream, a); };
+  if (threads == 64) a.rot ? launch(f8_append_kernel<64, true>) : launch(f8_append_kernel<64, false>);
+  else if (threads == 256) a.rot ? launch(f8_append_kernel<256, true>) : launch(f8_append_kernel<256, false>);
+  else a.rot ? launch(f8_append_kernel<1024, true>) : launch(f8_append_kernel<1024, false>);
   return hipGetLastError();
 }
 

@@ -52,7 +52,9 @@ __device__ __forceinline__ bool any_of(bool v, int* lds) {   // over 256 threads
 
 __device__ __forceinline__ int blocks_of(int tokens, int bt) { return (int)(((long)tokens + bt - 1) / bt); }
 
-// One 16 KB chunk of page src to page dst of a plane.
+// One 16 KB chunk of page src to page dst of a plane.  STREAM: past the caches, for bulk moves
+// (compacting 370 MB: 89 -> 82 us); a reserve's few pages are read again at once (8 against 10 us).
+template <bool STREAM>
 __device__ __forceinline__ void copy_chunk(uint8_t* base, uint64_t bytes, int src, int dst, uint64_t at) {
   const uint8_t* from = base + (uint64_t)src * bytes + at;
   uint8_t* to = base + (uint64_t)dst * bytes + at;
@@ -64,10 +66,17 @@ __device__ __forceinline__ void copy_chunk(uint8_t* base, uint64_t bytes, int sr
     u4_t v[4];
 #pragma unroll
     for (int i = 0; i < 4; i++)
-      if (tid + 256 * i < q) v[i] = reinterpret_cast<const u4_t*>(from)[tid + 256 * i];
+      if (tid + 256 * i < q) {
+        const u4_t* at = reinterpret_cast<const u4_t*>(from) + tid + 256 * i;
+        v[i] = STREAM ? __builtin_nontemporal_load(at) : *at;
+      }
 #pragma unroll
     for (int i = 0; i < 4; i++)
-      if (tid + 256 * i < q) reinterpret_cast<u4_t*>(to)[tid + 256 * i] = v[i];
+      if (tid + 256 * i < q) {
+        u4_t* at = reinterpret_cast<u4_t*>(to) + tid + 256 * i;
+        if (STREAM) __builtin_nontemporal_store(v[i], at);
+        else *at = v[i];
+      }
   } else if ((align & 3) == 0) {
     for (int i = tid; i < n / 4; i += 256) reinterpret_cast<uint32_t*>(to)[i] = reinterpret_cast<const uint32_t*>(from)[i];
   } else {
@@ -77,6 +86,7 @@ __device__ __forceinline__ void copy_chunk(uint8_t* base, uint64_t bytes, int sr
 
 // Pairs (from, to) over every plane, the work spread over `wgs` workgroups; a pair out of
 // range, or of a page with itself, is left out.
+template <bool STREAM>
 __device__ __forceinline__ void copy_pairs(const PagePlanes& pl, const int32_t* pairs, int n, int n_pages, int chunks,
                                            long wg, long wgs) {
   const long per = (long)pl.n * chunks;
@@ -85,7 +95,7 @@ __device__ __forceinline__ void copy_pairs(const PagePlanes& pl, const int32_t* 
     const uint64_t at = (uint64_t)(r - k * chunks) * kChunk;
     const int src = pairs[2 * i], dst = pairs[2 * i + 1];
     if (at >= pl.bytes[k] || src < 0 || dst < 0 || src >= n_pages || dst >= n_pages || src == dst) continue;
-    copy_chunk(pl.base[k], pl.bytes[k], src, dst, at);
+    copy_chunk<STREAM>(pl.base[k], pl.bytes[k], src, dst, at);
   }
 }
 
@@ -267,7 +277,7 @@ __global__ __launch_bounds__(256) void pages_apply_kernel(PageTables t, const in
                                                           int32_t* scratch) {
   const ReserveScratch r = reserve_scratch(scratch, n, blocks);
   if (blockIdx.x >= (unsigned)n) {
-    copy_pairs(planes, r.pairs, n, t.n_pages, chunks, (long)blockIdx.x - n, (long)gridDim.x - n);
+    copy_pairs<false>(planes, r.pairs, n, t.n_pages, chunks, (long)blockIdx.x - n, (long)gridDim.x - n);
     return;
   }
   const int i = blockIdx.x, lane = threadIdx.x;
@@ -303,7 +313,7 @@ hipError_t launch_pages_reserve(const PageTables& t, const int32_t* slots, const
 // ---- copy ------------------------------------------------------------------
 __global__ __launch_bounds__(256) void pages_copy_kernel(PagePlanes planes, const int32_t* pairs, int n, int n_pages,
                                                          int chunks) {
-  copy_pairs(planes, pairs, n, n_pages, chunks, blockIdx.x, gridDim.x);
+  copy_pairs<true>(planes, pairs, n, n_pages, chunks, blockIdx.x, gridDim.x);
 }
 
 hipError_t launch_pages_copy(const PagePlanes& planes, const int32_t* pairs, int n, int n_pages, hipStream_t stream) {
@@ -355,7 +365,7 @@ __global__ __launch_bounds__(1024) void pages_compact_plan_kernel(PageTables t, 
 __global__ __launch_bounds__(256) void pages_compact_kernel(PageTables t, const int32_t* moved, PagePlanes planes,
                                                             int chunks, const int32_t* scratch, int table_wgs) {
   if (blockIdx.x >= (unsigned)table_wgs) {
-    copy_pairs(planes, scratch + 2, scratch[0], t.n_pages, chunks, (long)blockIdx.x - table_wgs,
+    copy_pairs<true>(planes, scratch + 2, scratch[0], t.n_pages, chunks, (long)blockIdx.x - table_wgs,
                (long)gridDim.x - table_wgs);
     return;
   }
