@@ -644,8 +644,9 @@ __global__ __launch_bounds__(256, 1) void f8_mid_kernel(F8AttnArgs p) {
       p.desc[(line.base + e) * p.num_kv + h] = make_int2(n, 2 * grp + (first_seg ? 0 : 1));
     }
 
-    uint8_t* ring = sm.ring[wave][0][0];
-    auto load = [&](const Tile& t, int to_par) {   // (to_par: byte offset of the parity's codes)
+    uint8_t (*ring)[2][TB] = sm.ring[wave];
+    uint32_t ke[2][2], ve[2][2];     // exponents, by parity and half
+    auto load = [&](const Tile& t, int par) {
 #pragma unroll
       for (int hf = 0; hf < 2; hf++) {
         const long pg = max(t.pg[hf], 0), from = (pg * p.block_tokens + t.row[hf]) * key_bytes + (long)h * HD;
@@ -654,18 +655,11 @@ __global__ __launch_bounds__(256, 1) void f8_mid_kernel(F8AttnArgs p) {
           const int r0 = l * RL;     // first row of the load, in the half
           const uint32_t k_off = ld_row * key_bytes + ((ld_chunk ^ ((r0 + ld_row) & (HD / 16 - 1))) * 16);
           const int to = (16 * hf + r0) * HD;
-          __builtin_amdgcn_global_load_lds((glb_void*)(p.k_pool + from + (long)r0 * key_bytes + k_off), (lds_void*)(ring + to_par + to), 16, 0, 0);
-          __builtin_amdgcn_global_load_lds((glb_void*)(p.v_pool + from + (long)r0 * key_bytes + v_off), (lds_void*)(ring + to_par + TB + to), 16, 0, 0);
+          __builtin_amdgcn_global_load_lds((glb_void*)(p.k_pool + from + (long)r0 * key_bytes + k_off), (lds_void*)(ring[par][0] + to), 16, 0, 0);
+          __builtin_amdgcn_global_load_lds((glb_void*)(p.v_pool + from + (long)r0 * key_bytes + v_off), (lds_void*)(ring[par][1] + to), 16, 0, 0);
         }
-      }
-    };
-    uint32_t ke[2], ve[2];           // a tile's exponents by half, loaded a tile ahead
-    auto load_exp = [&](const Tile& t) {
-#pragma unroll
-      for (int hf = 0; hf < 2; hf++) {
-        const long pg = max(t.pg[hf], 0);
-        ke[hf] = p.k_exp[pg * p.num_kv + h];
-        ve[hf] = p.v_exp[pg * p.num_kv + h];
+        ke[par][hf] = p.k_exp[pg * p.num_kv + h];
+        ve[par][hf] = p.v_exp[pg * p.num_kv + h];
       }
     };
 
@@ -674,11 +668,10 @@ __global__ __launch_bounds__(256, 1) void f8_mid_kernel(F8AttnArgs p) {
     if (v < v_end) {
       cur = tile_at(p, table, rt.key0(v, KT), rt.end);
       load(cur, 0);
-      load_exp(cur);
     }
     if (v + PER < v_end) {
       nxt = tile_at(p, table, rt.key0(v + PER, KT), rt.end);
-      load(nxt, 2 * TB);
+      load(nxt, 1);
     }
     // ---- queries: row c of the wave, dims 32 i + 16 hh + 8 x ..
     h8_t qf[KW][2];
@@ -698,18 +691,17 @@ __global__ __launch_bounds__(256, 1) void f8_mid_kernel(F8AttnArgs p) {
 #pragma unroll
     for (int d = 0; d < DB; d++) acc[d] = f16x_t{};
 
-    for (int par = 0; v < v_end; v += PER, par ^= 2 * TB) {
+    auto step = [&](auto parity) {
+      constexpr int P = decltype(parity)::value;
       const bool more = v + PER < v_end;
       // this tile's codes have landed; the next one's (all newer) may be under way
-      if (more) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(64 / RL) : "memory");
+      if (more) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * 32 / RL + 4) : "memory");
       else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      const float k0 = pow2f(ke[0]), k1 = pow2f(ke[1]), vf[2] = {pow2f(ve[0]), pow2f(ve[1])};
-      if (more) load_exp(nxt);
-      const uint8_t* kt = ring + par + c * HD;
-      const uint8_t* vt = ring + par + TB + 4 * hh * HD + c * DB;
+      const uint8_t* kt = ring[P][0] + c * HD;
+      const uint8_t* vt = ring[P][1] + 4 * hh * HD + c * DB;
       // ---- scores: lane c's row, keys 8 (x / 4) + 4 hh + x % 4
       f16x_t sc = f16x_t{};
-      const float f = c < 16 ? k0 : k1;
+      const float f = pow2f(c < 16 ? ke[P][0] : ke[P][1]);
 #pragma unroll
       for (int i = 0; i < KW; i++) {
         const u4_t kr = *reinterpret_cast<const u4_t*>(kt + (((2 * i + hh) ^ (c & (HD / 16 - 1))) * 16));
@@ -720,6 +712,18 @@ __global__ __launch_bounds__(256, 1) void f8_mid_kernel(F8AttnArgs p) {
                     cvt2(kr[2 * x + 1], f, true)),
               qf[i][x], sc, 0, 0, 0);
       }
+      uint32_t vr[16][VD];           // keys 16 hf + 8 a + 4 hh + i
+#pragma unroll
+      for (int x = 0; x < 16; x++) {
+        const uint8_t* src = vt + (8 * (x >> 2) + (x & 3)) * HD;
+        if constexpr (VD == 2) {
+          const u2_t w = *reinterpret_cast<const u2_t*>(src);
+          vr[x][0] = w[0];
+          vr[x][1] = w[1];
+        } else {
+          vr[x][0] = *reinterpret_cast<const uint32_t*>(src);
+        }
+      }
       sc *= p.scale_log2;
       const bool whole = cur.pg[0] >= 0 && cur.pg[1] >= 0 && cur.key0 + KT - 1 <= rt.pos_lo && cur.key0 + KT <= rt.end &&
                          (p.window <= 0 || cur.key0 > rt.pos_hi - p.window || cur.key0 + KT <= p.sink);
@@ -727,8 +731,11 @@ __global__ __launch_bounds__(256, 1) void f8_mid_kernel(F8AttnArgs p) {
 #pragma unroll
         for (int x = 0; x < 16; x++) {
           const int key = cur.key0 + 8 * (x >> 2) + 4 * hh + (x & 3);
-          const bool there = cur.pg[x >> 3] >= 0;
+          const bool there = cur.pg[x >> 3] >= 0 && key < rt.end;
           sc[x] = there && sees(key, pos_r, rt.end, p.window, p.sink) ? sc[x] : -INFINITY;
+          // rows past the last key hold whatever the page held before
+#pragma unroll
+          for (int d = 0; d < VD; d++) vr[x][d] = there ? vr[x][d] : 0u;
         }
       }
       float t = sc[0];
@@ -750,48 +757,34 @@ __global__ __launch_bounds__(256, 1) void f8_mid_kernel(F8AttnArgs p) {
 #pragma unroll
         for (int i = 0; i < 8; i++) pb[i] = (_Float16)__builtin_amdgcn_exp2f(sc[8 * hf + i] - base);
         ls = add8(pb, ls);
-        uint32_t vr[8][VD];          // keys 16 hf + 8 a + 4 hh + i
-#pragma unroll
-        for (int x = 0; x < 8; x++) {
-          const uint8_t* src = vt + (16 * hf + 8 * (x >> 2) + (x & 3)) * HD;
-          if constexpr (VD == 2) {
-            const u2_t w = *reinterpret_cast<const u2_t*>(src);
-            vr[x][0] = w[0];
-            vr[x][1] = w[1];
-          } else {
-            vr[x][0] = *reinterpret_cast<const uint32_t*>(src);
-          }
-        }
-        if (!whole) {   // rows past the last key hold whatever the page held before
-#pragma unroll
-          for (int x = 0; x < 8; x++) {
-            const int key = cur.key0 + 16 * hf + 8 * (x >> 2) + 4 * hh + (x & 3);
-#pragma unroll
-            for (int d = 0; d < VD; d++) vr[x][d] = cur.pg[hf] >= 0 && key < rt.end ? vr[x][d] : 0u;
-          }
-        }
+        const float vf = pow2f(ve[P][hf]);
 #pragma unroll
         for (int d = 0; d < VD; d++) {
           uint32_t w[4][2];   // key pairs x byte pairs
 #pragma unroll
           for (int k = 0; k < 4; k++) {
-            w[k][0] = __builtin_amdgcn_perm(vr[2 * k + 1][d], vr[2 * k][d], 0x05010400u);
-            w[k][1] = __builtin_amdgcn_perm(vr[2 * k + 1][d], vr[2 * k][d], 0x07030602u);
+            w[k][0] = __builtin_amdgcn_perm(vr[8 * hf + 2 * k + 1][d], vr[8 * hf + 2 * k][d], 0x05010400u);
+            w[k][1] = __builtin_amdgcn_perm(vr[8 * hf + 2 * k + 1][d], vr[8 * hf + 2 * k][d], 0x07030602u);
           }
 #pragma unroll
           for (int j = 0; j < 4; j++)
             acc[4 * d + j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
-                join8(cvt2(w[0][j >> 1], vf[hf], j & 1), cvt2(w[1][j >> 1], vf[hf], j & 1), cvt2(w[2][j >> 1], vf[hf], j & 1),
-                      cvt2(w[3][j >> 1], vf[hf], j & 1)),
+                join8(cvt2(w[0][j >> 1], vf, j & 1), cvt2(w[1][j >> 1], vf, j & 1), cvt2(w[2][j >> 1], vf, j & 1),
+                      cvt2(w[3][j >> 1], vf, j & 1)),
                 pb, acc[4 * d + j], 0, 0, 0);
         }
       }
       // (every read of this tile's codes is done: its registers have been used)
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      if (v + 2 * PER < v_end) load(far, par);
+      if (v + 2 * PER < v_end) load(far, P);
       cur = nxt;
       nxt = far;
       if (v + 3 * PER < v_end) far = tile_at(p, table, rt.key0(v + 3 * PER, KT), rt.end);
+      v += PER;
+    };
+    while (v < v_end) {
+      step(std::integral_constant<int, 0>{});
+      if (v < v_end) step(std::integral_constant<int, 1>{});
     }
 
     // ---- join the streams; lane c holds dims DB * (8 (x / 4) + 4 hh + x % 4) + d of row c
