@@ -1068,30 +1068,30 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
           auto k_operand = [&](int i) { return *reinterpret_cast<const h8_t*>(krow + i * 32); };
           constexpr int NK = HD / 16;
           f16x_t sd = f16x_t{};
-          h8_t ka[4];
+          h8_t ka[3];
 #pragma unroll
-          for (int i = 0; i < 4; i++) ka[i] = k_operand(i);
+          for (int i = 0; i < 3; i++) ka[i] = k_operand(i);
 #pragma unroll
           for (int i = 0; i < NK; i++) {
-            sd = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka[i & 3], qf[i], sd, 0, 0, 0);
-            if (i + 4 < NK) ka[i & 3] = k_operand(i + 4);
+            sd = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka[i % 3], qf[i], sd, 0, 0, 0);
+            if (i + 3 < NK) ka[i % 3] = k_operand(i + 3);
           }
-          __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);     // four reads ahead
+          __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
 #pragma unroll
-          for (int i = 0; i < NK - 4; i++) {
+          for (int i = 0; i < NK - 3; i++) {
             __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
             __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
           }
-          __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
+          __builtin_amdgcn_sched_group_barrier(0x008, 3, 0);
           // the first values' reads go ahead of the weights
           const uint8_t* vat = vb + c * VP + c / VPAD * 16 + hh * 16 + kh * 64;
           constexpr int NV = HD / 16;   // of 16 keys, then of the other 16
           auto v_operand = [&](int i) {
             return *reinterpret_cast<const h8_t*>(vat + (i % (NV / 2)) * (32 * VP + 32 / VPAD * 16) + i / (NV / 2) * 32);
           };
-          h8_t va[4];
+          h8_t va[3];
 #pragma unroll
-          for (int i = 0; i < 4; i++) va[i] = v_operand(i);
+          for (int i = 0; i < 3; i++) va[i] = v_operand(i);
           const int y = v * KH + kh, k0 = (y < rt.n_sink * KH ? y : y + y_off) * 32;
           if (!((y >= y_lo && y < y_hi) || y < y_sink) || !paged) {
             const bool pa = page_of(k0) >= 0, pb = page_of(k0 + 16) >= 0;
@@ -1127,16 +1127,16 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
           const h8_t w1 = weights(1);
 #pragma unroll
           for (int i = 0; i < NV; i++) {
-            acc[i % (NV / 2)] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va[i & 3], i < NV / 2 ? w0 : w1, acc[i % (NV / 2)], 0, 0, 0);
-            if (i + 4 < NV) va[i & 3] = v_operand(i + 4);
+            acc[i % (NV / 2)] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va[i % 3], i < NV / 2 ? w0 : w1, acc[i % (NV / 2)], 0, 0, 0);
+            if (i + 3 < NV) va[i % 3] = v_operand(i + 3);
           }
 #pragma unroll
-          for (int i = 0; i < NV - 4; i++) {
+          for (int i = 0; i < NV - 3; i++) {
             __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
             __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
             if (i < NV / 2 - 1) __builtin_amdgcn_sched_group_barrier(0x002, HD == 256 ? 5 : 10, 0);
           }
-          __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
+          __builtin_amdgcn_sched_group_barrier(0x008, 3, 0);
         }
       }
       __builtin_amdgcn_s_setprio(0);
