@@ -302,7 +302,7 @@ __device__ __forceinline__ Tile tile_at(const F8AttnArgs& p, const const_i32* ta
 // by a run of dims, and byte permutes pair the keys ahead of the conversion.
 // JOIN: contexts of up to kJoinKeys keys, whose records the last workgroup of a tile
 // joins in this launch.
-constexpr int kJoinKeys = 1024, kJoinMost = kJoinKeys / 128;
+constexpr int kJoinKeys = 1024, kJoinStep = 8;
 template <int HD, bool JOIN>
 __global__ __launch_bounds__(256, 2) void f8_few_kernel(F8AttnArgs p) {
   constexpr int KT = 32, ROWS = 16, W = 4, PER = 4, THREADS = 64 * W;
@@ -364,13 +364,14 @@ __global__ __launch_bounds__(256, 2) void f8_few_kernel(F8AttnArgs p) {
         ve[hf] = p.v_exp[pg * p.num_kv + h];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
+          // (each byte is used once: past the caches; K's rows come in four pieces of a line)
           const uint8_t* src = base + (long)i * key_bytes + v_off;
           if constexpr (VD == 4) {
-            const u4_t w = *reinterpret_cast<const u4_t*>(src);
+            const u4_t w = __builtin_nontemporal_load(reinterpret_cast<const u4_t*>(src));
 #pragma unroll
             for (int d = 0; d < 4; d++) vr[4 * hf + i][d] = w[d];
           } else {
-            const u2_t w = *reinterpret_cast<const u2_t*>(src);
+            const u2_t w = __builtin_nontemporal_load(reinterpret_cast<const u2_t*>(src));
 #pragma unroll
             for (int d = 0; d < 2; d++) vr[4 * hf + i][d] = w[d];
           }
@@ -545,29 +546,39 @@ __global__ __launch_bounds__(256, 2) void f8_few_kernel(F8AttnArgs p) {
           const int r0 = 2 * g0 + (parts.begin(g0) == x0 ? 0 : 1);
           for (int x = tid * 4; x < rows * HD; x += THREADS * 4) {
             const int r = x / HD, d = x - r * HD;
-            float mr[kJoinMost], lr[kJoinMost];
-            f4_t ov[kJoinMost];
-#pragma unroll
-            for (int i = 0; i < kJoinMost; i++) {
-              const long at_r = (long)(i == 0 ? r0 : 2 * (g0 + min(i, n - 1))) * p.rec_rows + r;
-              mr[i] = __hip_atomic_load(p.rec_ml + at_r * 2, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-              lr[i] = __hip_atomic_load(p.rec_ml + at_r * 2 + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-#pragma unroll
-              for (int k = 0; k < 4; k++)
-                ov[i][k] = __hip_atomic_load(p.rec_o + at_r * HD + d + k, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            }
             float M = -INFINITY, L = 0.f;
-#pragma unroll
-            for (int i = 0; i < kJoinMost; i++)
-              if (i < n && lr[i] > 0.f) M = fmaxf(M, mr[i]);
             f4_t o = {0.f, 0.f, 0.f, 0.f};
+            for (int i0 = 0; i0 < n; i0 += kJoinStep) {   // (a step's loads are all under way at once)
+              float mr[kJoinStep], lr[kJoinStep];
+              f4_t ov[kJoinStep];
 #pragma unroll
-            for (int i = 0; i < kJoinMost; i++)
-              if (i < n && lr[i] > 0.f) {
-                const float w = __builtin_amdgcn_exp2f(mr[i] - M);
-                L += w * lr[i];
-                o += w * ov[i];
+              for (int i = 0; i < kJoinStep; i++) {
+                const int k = min(i0 + i, n - 1);
+                const long at_r = (long)(k == 0 ? r0 : 2 * (g0 + k)) * p.rec_rows + r;
+                mr[i] = __hip_atomic_load(p.rec_ml + at_r * 2, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                lr[i] = __hip_atomic_load(p.rec_ml + at_r * 2 + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                if (i0 + i >= n) lr[i] = 0.f;
+#pragma unroll
+                for (int q = 0; q < 4; q++)
+                  ov[i][q] = __hip_atomic_load(p.rec_o + at_r * HD + d + q, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
               }
+              float mn = M;
+#pragma unroll
+              for (int i = 0; i < kJoinStep; i++)
+                if (lr[i] > 0.f) mn = fmaxf(mn, mr[i]);
+              if (mn == -INFINITY) continue;   // no key so far
+              const float f = __builtin_amdgcn_exp2f(M - mn);
+              M = mn;
+              L *= f;
+              o *= f;
+#pragma unroll
+              for (int i = 0; i < kJoinStep; i++)
+                if (lr[i] > 0.f) {
+                  const float w = __builtin_amdgcn_exp2f(mr[i] - M);
+                  L += w * lr[i];
+                  o += w * ov[i];
+                }
+            }
             o *= L > 0.f ? 1.f / L : 0.f;
             const int t = r / gqa;
             *reinterpret_cast<u2_t*>(p.out + ((long)(sl.t0 + t) * p.num_q + h * gqa + (r - t * gqa)) * HD + d) =
@@ -655,8 +666,8 @@ __global__ __launch_bounds__(256, 1) void f8_mid_kernel(F8AttnArgs p) {
           const int r0 = l * RL;     // first row of the load, in the half
           const uint32_t k_off = ld_row * key_bytes + ((ld_chunk ^ ((r0 + ld_row) & (HD / 16 - 1))) * 16);
           const int to = (16 * hf + r0) * HD;
-          __builtin_amdgcn_global_load_lds((glb_void*)(p.k_pool + from + (long)r0 * key_bytes + k_off), (lds_void*)(ring[par][0] + to), 16, 0, 0);
-          __builtin_amdgcn_global_load_lds((glb_void*)(p.v_pool + from + (long)r0 * key_bytes + v_off), (lds_void*)(ring[par][1] + to), 16, 0, 0);
+          __builtin_amdgcn_global_load_lds((glb_void*)(p.k_pool + from + (long)r0 * key_bytes + k_off), (lds_void*)(ring[par][0] + to), 16, 0, 2);
+          __builtin_amdgcn_global_load_lds((glb_void*)(p.v_pool + from + (long)r0 * key_bytes + v_off), (lds_void*)(ring[par][1] + to), 16, 0, 2);
         }
         ke[par][hf] = p.k_exp[pg * p.num_kv + h];
         ve[par][hf] = p.v_exp[pg * p.num_kv + h];

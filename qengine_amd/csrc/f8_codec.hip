@@ -189,7 +189,8 @@ __global__ __launch_bounds__(THREADS, ROPE || THREADS == 1024 ? 4 : 8) void f8_a
   auto load = [&](int u) {
     const int r = u >> cpr_log, c = u & (cpr - 1);
     const uint16_t* row = in + r * stride;
-    return limit8(turn ? load_turned(row, c, (int)(first + r), rope) : *reinterpret_cast<const u4_t*>(row + 8 * c));
+    return limit8(turn ? load_turned(row, c, (int)(first + r), rope)
+                       : __builtin_nontemporal_load(reinterpret_cast<const u4_t*>(row + 8 * c)));
   };
   u4_t kept[KEEP];
   uint32_t top = 0;

@@ -162,7 +162,7 @@ def _check_attn(case, scale, window=0, sink=0, rows_left=True, **kw):
 @pytest.mark.parametrize("hd", [128, 256])
 @pytest.mark.parametrize("bt,lens,gqa,kv", [
     (64, [0], 4, 2), (16, [1, 14, 15, 16], 1, 1), (16, [700], 8, 2), (64, [31, 32, 33, 127, 128, 129], 6, 1),
-    (256, [3000, 5, 0, 260], 4, 2), (48, [1000, 47], 3, 3), (16, [0] * 20 + [2000], 5, 1)])
+    (256, [3000, 5, 0, 260], 4, 2), (64, [2047, 1500, 100], 4, 2), (16, [1023], 8, 1), (48, [1000, 47], 3, 3), (16, [0] * 20 + [2000], 5, 1)])
 def test_decode(hd, bt, lens, gqa, kv):
     """One query a slot, from no earlier key to several parts of a workgroup's line."""
     _check_attn(_attn_case(hd + bt + len(lens), lens, [1] * len(lens), bt, kv, gqa, hd), hd ** -0.5)
