@@ -19,6 +19,8 @@ int check_f8_pool(int num_kv, int head_dim, int max_blocks, int block_tokens, in
   if (head_dim != 128 && head_dim != 256) return QKV_ERR_UNSUPPORTED;
   if (num_kv <= 0 || max_blocks <= 0 || block_tokens <= 0 || n_pages <= 0) return QKV_ERR_INVALID;
   if (block_tokens % 16) return QKV_ERR_UNSUPPORTED;
+  // (the kernels address inside a page in 32 bits)
+  if ((double)block_tokens * num_kv * head_dim > 2147483647.0) return QKV_ERR_UNSUPPORTED;
   return QKV_OK;
 }
 

@@ -91,6 +91,7 @@ def test_append_refusals(L, p):
     assert f(rows=0) == f(slots=0) == f(mt=0) == 0
     assert f(rows=-1) == f(slots=-1) == f(mt=-1) == f(kv=0) == f(mb=0) == f(bl=0) == f(np=0) == -1
     assert f(hd=64) == f(bl=24) == f(rot=40) == -3
+    assert f(bl=1 << 22) == f(kv=1 << 20) == f(bl=0x7ffffff0, kv=0x7fffffff) == -3   # pages of 2 GiB and more
     assert f(rot=-16) == f(rot=256) == f(lay=3) == f(nq=4) == -1    # (queries without a rotation)
     assert f(k=None) == f(v=None) == f(kp=None) == f(ve=None) == f(bt=None) == f(st=None) == f(pos=None) == -2
     assert f(rot=64) == -2 and f(rot=64, t=p, nq=4) == -2           # no table; no queries
@@ -112,6 +113,7 @@ def test_attention_refusals(L, p):
     assert f(rows=0) == f(slots=0) == f(mt=0) == 0
     assert f(rows=-1) == f(slots=-1) == f(mt=-1) == f(mc=0) == f(nq=7) == f(kv=0) == f(np=0) == -1
     assert f(nq=18) == f(hd=192) == f(bl=8) == f(mc=(1 << 30) + 1) == -3
+    assert f(bl=1 << 23) == f(bl=0x7ffffff0) == -3      # pages of 2 GiB and more
     assert f(w=-1) == f(s=-1) == -1
     assert f(q=None) == f(ke=None) == f(out=None) == f(bt=None) == f(st=None) == -2
     assert f(q=p + 8) == f(vp=p + 4) == f(pos=p + 1) == f(ws=p + 16) == -4
