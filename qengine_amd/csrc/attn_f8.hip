@@ -123,11 +123,15 @@ __device__ __forceinline__ int entry_units(const F8AttnArgs& p, int x, int gqa) 
   return LEAD + row_tile<ROWS, KT>(p, sl, i, gqa).tiles;
 }
 
-// Where a workgroup's part begins: entry and unit in it, and the units of one head.
+// Where a workgroup's part begins: entry, and units of it before the part
 struct Part {
-  int total;      // units of one head
-  int entry, at;  // first entry, units of it before the part
+  int entry, at;
 };
+
+// Sums stop at kLineMax: starts that are not in order can name the same rows many times, and the
+// line of them all may pass 32 bits.
+constexpr int kLineMax = (1 << 30) - 1;
+__device__ __forceinline__ int add_units(int a, int b) { return min(a + b, kLineMax); }
 
 template <int THREADS>
 __device__ __forceinline__ int block_scan(int v, int* lds, int& sum) {   // inclusive
@@ -135,7 +139,7 @@ __device__ __forceinline__ int block_scan(int v, int* lds, int& sum) {   // incl
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
     const int o = __shfl_up(v, d);
-    if (lane >= d) v += o;
+    if (lane >= d) v = add_units(v, o);
   }
   __syncthreads();
   if (lane == 63) lds[w] = v;
@@ -144,13 +148,13 @@ __device__ __forceinline__ int block_scan(int v, int* lds, int& sum) {   // incl
   sum = 0;
 #pragma unroll
   for (int i = 0; i < THREADS / 64; i++) {
-    if (i < w) before += lds[i];
-    sum += lds[i];
+    if (i < w) before = add_units(before, lds[i]);
+    sum = add_units(sum, lds[i]);
   }
-  return v + before;
+  return add_units(v, before);
 }
 
-// The units of one head's line
+// The units of one head's line (0: too long, which starts in order cannot make it)
 template <int ROWS, int KT, int LEAD, int THREADS>
 __device__ __forceinline__ int line_units(const F8AttnArgs& p, int gqa, int* lds) {
   const int entries = p.n_slots * p.slot_tiles;
@@ -159,13 +163,13 @@ __device__ __forceinline__ int line_units(const F8AttnArgs& p, int gqa, int* lds
     const int x = c + threadIdx.x;
     int sum;
     block_scan<THREADS>(x < entries ? entry_units<ROWS, KT, LEAD>(p, x, gqa) : 0, lds, sum);
-    base += sum;
+    base = add_units(base, sum);
   }
-  return base;
+  return base < kLineMax && (long)base * p.num_kv < (1l << 31) ? base : 0;
 }
 // The entry that holds unit u of the line (u < its length)
 template <int ROWS, int KT, int LEAD, int THREADS>
-__device__ __forceinline__ Part line_find(const F8AttnArgs& p, int gqa, int total, int u, int* lds) {
+__device__ __forceinline__ Part line_find(const F8AttnArgs& p, int gqa, int u, int* lds) {
   const int entries = p.n_slots * p.slot_tiles;
   __shared__ int found[2];
   int base = 0;
@@ -182,7 +186,7 @@ __device__ __forceinline__ Part line_find(const F8AttnArgs& p, int gqa, int tota
     if (base > u) break;
   }
   __syncthreads();
-  const Part r{total, __builtin_amdgcn_readfirstlane(found[0]), __builtin_amdgcn_readfirstlane(found[1])};
+  const Part r{__builtin_amdgcn_readfirstlane(found[0]), __builtin_amdgcn_readfirstlane(found[1])};
   __syncthreads();
   return r;
 }
@@ -898,7 +902,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   int u = parts.begin(grp);
   const int u_end = parts.begin(grp + 1);
   int h = u / total;
-  Part at = line_find<ROWS, KT, LEAD, THREADS>(p, gqa, total, u - h * total, lds);
+  Part at = line_find<ROWS, KT, LEAD, THREADS>(p, gqa, u - h * total, lds);
   bool first_seg = true;
   const uint32_t key_bytes = (uint32_t)p.num_kv * HD;
   const uint32_t page_bytes = (uint32_t)p.block_tokens * key_bytes;

@@ -2,6 +2,7 @@
 // calls (declared in include/qkv.h): argument checks, then launches on the caller's stream.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 
 #include "../../include/qkv.h"
@@ -190,10 +191,13 @@ static int check_f8_attn(int num_q, int num_kv, int head_dim, int n_slots, int n
   if (num_kv <= 0 || num_q <= 0 || num_q % num_kv != 0 || n_slots <= 0 || n_rows <= 0 || max_tok <= 0 || max_ctx <= 0)
     return QKV_ERR_INVALID;
   if (num_q / num_kv > 8 || num_q > 1024 || max_ctx > (1 << 30)) return QKV_ERR_UNSUPPORTED;
-  // row tiles of the call, and the key tiles of them all (counted in 32 bits)
+  if (max_tok > n_rows) max_tok = n_rows;
+  // row tiles of the call, and the key tiles of them all with their leads (counted in 32 bits,
+  // a head's in 30)
   const double gqa = num_q / num_kv, full = (double)n_slots * ((double)max_tok * gqa / 256 + 1);
   const double tiles = full < n_rows * gqa / 256 + n_slots ? full : n_rows * gqa / 256 + n_slots;
-  if (full * num_kv > (double)(1 << 22) || tiles * num_kv * (max_ctx / 32.0 + 1) > 2147483647.0) return QKV_ERR_UNSUPPORTED;
+  if (full * num_kv > (double)(1 << 22) || tiles * std::max(num_kv, 2) * (max_ctx / 32.0 + 8) > 2147483000.0)
+    return QKV_ERR_UNSUPPORTED;
   return QKV_OK;
 }
 

@@ -249,6 +249,22 @@ def test_context_limit():
     _check_attn(case, 0.09, max_ctx=200)
 
 
+def test_starts_out_of_order():
+    """Starts that decrease name the same rows again and again: 2^32 key tiles of a head here, which is no call
+    that can be carried out (nothing is), and a few, which is."""
+    rows, slots, ctx = 16384, 64, 1 << 24
+    q = torch.zeros((rows, 4, 128), dtype=torch.float16, device=DEV)
+    pool, exp = torch.zeros((2, 16384, 1, 128), dtype=torch.uint8, device=DEV), torch.full((2, 1), 120, dtype=torch.uint8, device=DEV)
+    tables = torch.full((slots, ctx // 16384), -1, dtype=torch.int32, device=DEV)
+    starts = torch.tensor([0, rows] * (slots // 2) + [0], dtype=torch.int32, device=DEV)
+    ws = kvcache.attn_f8_paged_workspace(4, 1, slots, rows, rows, ctx, DEV, head_dim=128)
+    for pos, want in ((ctx - rows, 5.0), (0, 0.0)):
+        out = torch.full_like(q, 5.0)
+        at = torch.full((slots,), pos, dtype=torch.int32, device=DEV)
+        kvcache.attn_f8_paged(q, pool, pool, exp, exp, out, ws, tables, starts, at, max_tok=rows, max_ctx=ctx, scale=0.1)
+        assert (out == want).all()
+
+
 def test_same_result_every_time_and_on_another_stream():
     case = _attn_case(8, [3000, 10, 700], [1, 1, 1], 64, 2, 4, 256)
     a = _attend(*case, 0.06)
