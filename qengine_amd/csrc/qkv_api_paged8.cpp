@@ -252,7 +252,7 @@ int qkv_attn_f8_paged(const uint16_t* q, const uint8_t* k_pool, const uint8_t* v
   a.block_tokens = block_tokens;
   a.n_pages = n_pages;
   a.window = window_tok;
-  a.sink = sink_tok;
+  a.sink = sink_tok < max_ctx ? sink_tok : max_ctx;   // (rounded up to tiles in 32 bits)
   a.slot_tiles = x.slot_tiles;
   a.rec_rows = x.rec_rows;
   a.groups = x.groups;

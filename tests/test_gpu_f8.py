@@ -186,7 +186,7 @@ def test_prompts(hd, bt, lens, new, gqa):
 
 
 @pytest.mark.parametrize("new", [[1, 1, 1], [6, 1, 9], [70, 3, 100]])
-@pytest.mark.parametrize("window,sink", [(1, 0), (20, 0), (64, 4), (100, 33), (5000, 1)])
+@pytest.mark.parametrize("window,sink", [(1, 0), (20, 0), (64, 4), (100, 33), (5000, 1), (7, 2**31 - 1), (2**31 - 1, 2**31 - 1)])
 def test_window_and_sinks(new, window, sink):
     """Exact to the key; pages out of every query's window are given back first."""
     case = _attn_case(window + sum(new), [400, 30, 999], new, 16, 2, 4, 128)
