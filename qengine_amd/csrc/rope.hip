@@ -31,7 +31,7 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs p) {
   }
   if (run.turned) {
     float cs[8], sn[8];
-    const int pos = p.inverse ? -p.positions[tok] : p.positions[tok];
+    const int64_t pos = p.inverse ? -(int64_t)p.positions[tok] : p.positions[tok];
 #pragma unroll
     for (int i = 0; i < 8; i++) rope_cos_sin(pos, p.turns[8 * c + i], p.amplitude, cs[i], sn[i]);
 #pragma unroll
@@ -76,7 +76,7 @@ __global__ __launch_bounds__(256) void rope_any_kernel(RopeArgs p) {
   const int a0 = p.layout == 0 ? i : 2 * i, a1 = p.layout == 0 ? i + half : 2 * i + 1;
   const float x = h2f(in[a0]), y = h2f(in[a1]);
   float c, s;
-  const int pos = p.inverse ? -p.positions[tok] : p.positions[tok];
+  const int64_t pos = p.inverse ? -(int64_t)p.positions[tok] : p.positions[tok];
   rope_cos_sin(pos, p.turns[i], p.amplitude, c, s);
   out[a0] = __builtin_bit_cast(uint16_t, round16(__builtin_fmaf(x, c, -y * s)));
   out[a1] = __builtin_bit_cast(uint16_t, round16(__builtin_fmaf(x, s, y * c)));

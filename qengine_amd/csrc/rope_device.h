@@ -18,8 +18,8 @@ namespace qkv {
 // x^10 (first term left out 1.1e-10) and sin to x^9 (1.8e-9), are fp32-exact to
 // a rounding or two; v_sin_f32's error (about 2^-20) would show in the last
 // bit of one fp16 product in a few hundred.
-__device__ __forceinline__ void rope_cos_sin(int pos, uint64_t R, float amp, float& c, float& s) {
-  const uint32_t ph = (uint32_t)(((uint64_t)(int64_t)pos * R) >> 32);
+__device__ __forceinline__ void rope_cos_sin(int64_t pos, uint64_t R, float amp, float& c, float& s) {
+  const uint32_t ph = (uint32_t)(((uint64_t)pos * R) >> 32);
   const uint32_t quarter = (ph + 0x20000000u) >> 30;
   const int rem = (int)(ph - (quarter << 30));
   const float x = (float)rem * (6.283185307179586f / 4294967296.0f), z = x * x;

@@ -50,6 +50,18 @@ def test_far_and_negative_positions(scaling):
     assert (np.abs(got - ref) <= R.rope_tolerance(x, ref, 128, "half", amp) + extra).all()
 
 
+def test_the_lowest_position():
+    """-2^31 has no int32 negative: its inverse turns as 2^31 does, one position past 2^31 - 1."""
+    rng = np.random.default_rng(8)
+    for hd in (128, 66):   # (each kernel)
+        x = rng.standard_normal((1, 2, hd)).astype(np.float16)
+        t = kvcache.rope_table(hd, base=500000.0, device=DEV)
+        got = _run(torch.from_numpy(x).to(DEV), torch.tensor([-2**31], dtype=torch.int32, device=DEV), t, inverse=True)
+        ref = R.rotate(x, np.array([2**31]), hd, "half", base=500000.0)
+        extra = 2.0 ** 31 * 2.0 ** -51 * np.abs(x).max() * 2
+        assert (np.abs(got.cpu().numpy().astype(np.float64) - ref) <= R.rope_tolerance(x, ref, hd, "half") + extra).all()
+
+
 @pytest.mark.parametrize("hd,rot", [(256, 64), (128, 128), (48, 30)])
 def test_strided_views_in_place_and_q_with_k(hd, rot):
     """q and k as views of one projection buffer, in place and apart: the same bits, and v untouched."""
