@@ -97,6 +97,7 @@ int qkv_rope(const uint16_t* q, long q_stride, uint16_t* q_out, long q_out_strid
     return QKV_ERR_INVALID;
   if ((num_q && q == q_out && q_stride != q_out_stride) || (num_k && k == k_out && k_stride != k_out_stride))
     return QKV_ERR_INVALID;
+  if (num_q && num_k && q_out == k_out) return QKV_ERR_INVALID;
   if ((num_q && (!aligned(q, 2) || !aligned(q_out, 2))) || (num_k && (!aligned(k, 2) || !aligned(k_out, 2))) ||
       !aligned(positions, 4) || !aligned(turns, 8))
     return QKV_ERR_ALIGN;

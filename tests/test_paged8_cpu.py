@@ -65,7 +65,7 @@ def test_rope_table_refusals(L):
 
 def test_rope_refusals(L, p):
     def f(**kw):
-        a = dict(q=p, qs=512, qo=p, qos=512, k=p, ks=256, ko=p, kos=256, pos=p, t=p, n=4, nq=4, nk=2, hd=128, rot=64,
+        a = dict(q=p, qs=512, qo=p, qos=512, k=p + 64, ks=256, ko=p + 64, kos=256, pos=p, t=p, n=4, nq=4, nk=2, hd=128, rot=64,
                  lay=0)
         a.update(kw)
         return L.qkv_rope(a["q"], a["qs"], a["qo"], a["qos"], a["k"], a["ks"], a["ko"], a["kos"], a["pos"], a["t"], 1.0,
@@ -74,6 +74,7 @@ def test_rope_refusals(L, p):
     assert f(n=-1) == f(nq=0, nk=0) == f(nq=-1) == f(rot=0) == f(rot=63) == f(rot=130) == f(lay=2) == f(hd=0) == -1
     assert f(qs=500) == f(ks=100) == -1            # strides shorter than a token's heads
     assert f(qos=1024) == -1                       # in place with another stride
+    assert f(k=p, ko=p) == f(ko=p) == -1           # one memory for both outputs
     assert f(q=None) == f(qo=None) == f(k=None) == f(pos=None) == f(t=None) == -2
     assert f(q=p + 1, qo=p + 1) == f(pos=p + 2) == f(t=p + 4) == -4
     assert f(nq=2000) == -1
