@@ -468,7 +468,8 @@ __global__ __launch_bounds__(256, 2) void f8_few_kernel(F8AttnArgs p) {
         pl[i] = (_Float16)(w - (float)pb[i]);
       }
       // ---- O^T += V^T P^T: dims m * HD/16 + 4 d + j
-      const float v0 = pow2f(ve[0]), v1 = pow2f(ve[1]);
+      // (an absent page's exponent is not one: zeros times it may be no number)
+      const float v0 = pow2f(cur.pg[0] < 0 ? 127 : ve[0]), v1 = pow2f(cur.pg[1] < 0 ? 127 : ve[1]);
 #pragma unroll
       for (int d = 0; d < VD; d++) {
         uint32_t w[4][2];   // key pairs x byte pairs
@@ -780,7 +781,7 @@ __global__ __launch_bounds__(256, 1) void f8_mid_kernel(F8AttnArgs p) {
 #pragma unroll
         for (int i = 0; i < 8; i++) pb[i] = (_Float16)__builtin_amdgcn_exp2f(sc[8 * hf + i] - base);
         ls = add8(pb, ls);
-        const float vf = pow2f(ve[P][hf]);
+        const float vf = pow2f(cur.pg[hf] < 0 ? 127 : ve[P][hf]);
 #pragma unroll
         for (int d = 0; d < VD; d++) {
           uint32_t w[4][2];   // key pairs x byte pairs
@@ -1012,6 +1013,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
         for (int i = 0; i < 4; i++)
           if (loaded < 0 || key0 + 4 * vq + i >= rt.end) vr[i] = 0;
+        if (loaded < 0) vsc = 1.f;   // (an absent page's exponent is not one)
       }
       uint8_t* kb = tile_lds[buf];
       uint8_t* vb = kb + KB;

@@ -212,6 +212,20 @@ def test_absent_pages(new, hd):
     assert (got[n0:int(case[6][2])] == 0).all()
 
 
+@pytest.mark.parametrize("new", [[1, 1], [5, 12], [90, 2]])
+@pytest.mark.parametrize("hd", [128, 256])
+def test_pages_that_were_never_written(new, hd):
+    """Pages in no table hold anything, exponents too: absent pages do not bring in those of another."""
+    q, kp, vp, ke, ve, tables, starts, pos = _attn_case(8 + hd, [200, 40], new, 16, 2, 4, hd)
+    tables[0, 3], tables[0, 5], tables[1, 1] = -1, len(kp) + 1, -2
+    if 0 in tables:   # page 0 is in no table: its own content goes to a new last page
+        kp, vp, ke, ve = (np.concatenate([x, x[:1]]) for x in (kp, vp, ke, ve))
+        tables[tables == 0] = len(kp) - 1
+    for free in sorted(set(range(len(kp))) - set(tables.ravel().tolist())):
+        kp[free], vp[free], ke[free], ve[free] = 0x7f, 0xff, 255, 255
+    _check_attn((q, kp, vp, ke, ve, tables, starts, pos), 0.1)
+
+
 @pytest.mark.parametrize("new", [[1, 1, 1], [4, 9, 2], [80, 1, 40]])
 def test_extreme_scores(new):
     """Peaked rows (one weight is all), a negative scale, and a scale of zero (the mean)."""
