@@ -206,6 +206,10 @@ struct Parts {
   }
 };
 
+// The maximum that a record carries (l = 0: no key).  A sum that is no number, from a query that is
+// not finite, is joined above every other and so reaches the output.
+__device__ __forceinline__ float rec_max(float m, float l) { return l != l ? INFINITY : m; }
+
 __device__ __forceinline__ bool sees(int key, int pos, int end, int window, int sink) {
   return key <= pos && key < end && (window <= 0 || key > pos - window || key < sink);
 }
@@ -535,12 +539,12 @@ __global__ __launch_bounds__(256, 2) void f8_few_kernel(F8AttnArgs p) {
 #pragma unroll
           for (int i = 0; i < 4; i++) __hip_atomic_store(ro + i, o[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
           if (d == 0) {
-            __hip_atomic_store(rm, M, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            __hip_atomic_store(rm, rec_max(M, L), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             __hip_atomic_store(rm + 1, L, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
           }
         } else {
           *reinterpret_cast<f4_t*>(ro) = o;
-          if (d == 0) *reinterpret_cast<f2_t*>(rm) = f2_t{M, L};
+          if (d == 0) *reinterpret_cast<f2_t*>(rm) = f2_t{rec_max(M, L), L};
         }
       }
     }
@@ -578,7 +582,7 @@ __global__ __launch_bounds__(256, 2) void f8_few_kernel(F8AttnArgs p) {
               float mn = M;
 #pragma unroll
               for (int i = 0; i < kJoinStep; i++)
-                if (lr[i] > 0.f) mn = fmaxf(mn, mr[i]);
+                if (lr[i] != 0.f) mn = fmaxf(mn, mr[i]);
               if (mn == -INFINITY) continue;   // no key so far
               const float f = __builtin_amdgcn_exp2f(M - mn);
               M = mn;
@@ -586,7 +590,7 @@ __global__ __launch_bounds__(256, 2) void f8_few_kernel(F8AttnArgs p) {
               o *= f;
 #pragma unroll
               for (int i = 0; i < kJoinStep; i++)
-                if (lr[i] > 0.f) {
+                if (lr[i] != 0.f) {
                   const float w = __builtin_amdgcn_exp2f(mr[i] - M);
                   L += w * lr[i];
                   o += w * ov[i];
@@ -849,7 +853,7 @@ __global__ __launch_bounds__(256, 1) void f8_mid_kernel(F8AttnArgs p) {
             u2_t{f2h(o[0]) | (f2h(o[1]) << 16), f2h(o[2]) | (f2h(o[3]) << 16)};
       } else {
         *reinterpret_cast<f4_t*>(p.rec_o + ((long)rec * p.rec_rows + r) * HD + d) = o;
-        if (d == 0) *reinterpret_cast<f2_t*>(p.rec_ml + ((long)rec * p.rec_rows + r) * 2) = f2_t{M, L};
+        if (d == 0) *reinterpret_cast<f2_t*>(p.rec_ml + ((long)rec * p.rec_rows + r) * 2) = f2_t{rec_max(M, L), L};
       }
     }
     u += n_u;
@@ -1190,7 +1194,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
           for (int a = 0; a < 4; a++)
             ro[(4 * d + a) * 64] = f4_t{acc[d][4 * a], acc[d][4 * a + 1], acc[d][4 * a + 2], acc[d][4 * a + 3]};
-        if (hh == 0) *reinterpret_cast<f2_t*>(p.rec_ml + (rec * ROWS + 32 * wave + c) * 2) = f2_t{mx, ls};
+        if (hh == 0) *reinterpret_cast<f2_t*>(p.rec_ml + (rec * ROWS + 32 * wave + c) * 2) = f2_t{rec_max(mx, ls), ls};
       }
     }
     }
@@ -1239,7 +1243,7 @@ __global__ __launch_bounds__(256) void f8_cut_merge_kernel(F8AttnArgs p) {
     f4_t x[4];
 #pragma unroll
     for (int a = 0; a < 4; a++) x[a] = src[a * 64];
-    const bool any = ml[1] > 0.f;
+    const bool any = ml[1] != 0.f;
     const float mn = fmaxf(M, any ? ml[0] : -INFINITY);
     const float f = mn == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - mn);
     const float w = any ? __builtin_amdgcn_exp2f(ml[0] - mn) : 0.f;
@@ -1295,7 +1299,7 @@ __global__ __launch_bounds__(256) void f8_merge_kernel(F8AttnArgs p) {
     }
     f2_t r = {-INFINITY, 0.f};
     if (i0 + lane < n) r = *reinterpret_cast<const f2_t*>(p.rec_ml + ((long)rec_of(i0 + lane) * p.rec_rows + row) * 2);
-    const bool any = r[1] > 0.f;
+    const bool any = r[1] != 0.f;
     const float mn = fmaxf(M, wave_max(any ? r[0] : -INFINITY));
     if (mn == -INFINITY) continue;   // no key so far
     const float f = __builtin_amdgcn_exp2f(M - mn), w = any ? __builtin_amdgcn_exp2f(r[0] - mn) : 0.f;

@@ -257,6 +257,18 @@ def test_output_in_place_of_the_queries():
         _check_attn(case, 0.09, alias=True)
 
 
+@pytest.mark.parametrize("lens,new", [([20], [1]), ([900, 5], [1, 1]), ([9000], [1]), ([2000], [12]), ([3000, 4], [90, 7])])
+def test_queries_that_are_not_finite(lens, new):
+    """A NaN in a query row makes that row NaN, whole or joined from parts, and no other."""
+    q, *rest = _attn_case(17, lens, new, 16, 2, 4, 128, spare_rows=0)
+    want = _attend(q, *rest, 0.09)
+    q[0, 5, 77] = np.nan
+    got = _attend(q, *rest, 0.09)
+    assert np.isnan(got[0, 5]).all()
+    got[0, 5] = want[0, 5]
+    assert np.array_equal(got, want)
+
+
 def test_context_limit():
     """Keys at or past max_ctx are not seen, and a larger table is not read."""
     case = _attn_case(6, [300, 100], [1, 1], 16, 1, 4, 128)
