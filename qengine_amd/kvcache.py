@@ -551,6 +551,8 @@ class RopeTable:
     fractions of a turn a position, and the amplitude of the scaling."""
 
     def __init__(self, turns, amplitude, rot_dim):
+        if turns.dtype is not torch.int64 or 2 * turns.numel() != rot_dim:
+            raise ValueError(f"turns must hold {rot_dim // 2} numbers of torch.int64")
         self.turns, self.amplitude, self.rot_dim = turns, amplitude, rot_dim
 
 

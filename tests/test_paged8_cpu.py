@@ -59,6 +59,10 @@ def test_rope_table_refusals(L):
     for bad in (("cubic", 2.0), ("linear",), ("yarn", 2.0), ("linear", 2.0, 3.0)):
         with pytest.raises(ValueError):
             kvcache.rope_table(64, scaling=bad, device="cpu")
+    t = kvcache.rope_table(64, device="cpu")
+    for turns in (t.turns[:31], t.turns.double()):   # (the kernels read rot_dim / 2 of them)
+        with pytest.raises(ValueError):
+            kvcache.RopeTable(turns, 1.0, 64)
 
 
 # ---- the C entry points -----------------------------------------------------
