@@ -92,6 +92,18 @@ __device__ __forceinline__ Slot slot_of(const F8AttnArgs& p, int s) {
   return x;
 }
 
+// The same for a slot that the whole wave asks for: by scalar loads, so that what follows from it
+// stays out of the vector registers
+__device__ __forceinline__ Slot slot_at(const F8AttnArgs& p, int s) {
+  const const_i32 *starts = (const const_i32*)p.starts + s, *positions = (const const_i32*)p.positions + s;
+  Slot x;
+  x.t0 = min(max(starts[0], 0), (int)p.rows);
+  x.n = min(min(max(starts[1], x.t0), (int)p.rows) - x.t0, p.max_tok);
+  x.pos0 = positions[0];
+  if (x.pos0 < 0 || x.pos0 > (1 << 30)) x.n = 0;
+  return x;
+}
+
 // Row tile i of a slot, ROWS (token, head) rows each, over key tiles of KT keys: keys
 // lo .. end-1 and below the sinks.  Tile v of `tiles` is key tile v below n_sink, then w0 on.
 struct RowTile {
@@ -898,10 +910,12 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const int c = lane & 31, hh = lane >> 5;
   const int gqa = p.num_q / p.num_kv;
 
-  const int total = line_units<ROWS, KT, LEAD, THREADS>(p, gqa, lds);
-  if (blockIdx.x == 0 && tid == 0) p.cuts[4 * p.groups] = total * p.num_kv;
+  // (the same in every lane: said to the compiler, what follows stays out of the vector registers)
+  const int total = __builtin_amdgcn_readfirstlane(line_units<ROWS, KT, LEAD, THREADS>(p, gqa, lds));
+  const int all = __builtin_amdgcn_readfirstlane(total * p.num_kv);
+  if (blockIdx.x == 0 && tid == 0) p.cuts[4 * p.groups] = all;
   // neighbouring parts (the same head's keys) on one XCD, whose L2 holds their tiles
-  const Parts parts(total * p.num_kv, p.groups);
+  const Parts parts(all, p.groups);
   const int grp = p.groups % 8 ? (int)blockIdx.x : (int)(blockIdx.x % 8) * (p.groups / 8) + (int)blockIdx.x / 8;
   if (grp >= parts.n) return;
   int u = parts.begin(grp);
@@ -916,7 +930,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 
   while (u < u_end) {
     const int s = at.entry / p.slot_tiles, rti = at.entry - s * p.slot_tiles;
-    const Slot sl = slot_of(p, s);
+    const Slot sl = slot_at(p, s);
     if (rti * ROWS >= sl.n * gqa) {   // past this slot's rows
       at.entry = (s + 1) * p.slot_tiles;
       if (at.entry >= entries) {
