@@ -79,7 +79,7 @@ __device__ __forceinline__ BlockRow block_row(const F8AttnArgs& p, int key) {
   return {(int)(more ? q + 1 : q), (int)(more ? r - (uint32_t)p.block_tokens : r)};
 }
 
-// A slot's tokens: rows t0 .. t0+n-1 of q at positions pos0 .. (n = 0: none)
+// A slot's tokens: rows t0 .. t0+n-1 of q at positions pos0 .. (n = 0: none, or not of this launch)
 struct Slot {
   int t0, n, pos0;
 };
@@ -88,7 +88,7 @@ __device__ __forceinline__ Slot slot_of(const F8AttnArgs& p, int s) {
   x.t0 = min(max(p.starts[s], 0), (int)p.rows);
   x.n = min(min(max(p.starts[s + 1], x.t0), (int)p.rows) - x.t0, p.max_tok);
   x.pos0 = p.positions[s];
-  if (x.pos0 < 0 || x.pos0 > (1 << 30)) x.n = 0;
+  if (x.pos0 < 0 || x.pos0 > (1 << 30) || x.n < p.from_tok || x.n > p.to_tok) x.n = 0;
   return x;
 }
 
@@ -100,7 +100,7 @@ __device__ __forceinline__ Slot slot_at(const F8AttnArgs& p, int s) {
   x.t0 = min(max(starts[0], 0), (int)p.rows);
   x.n = min(min(max(starts[1], x.t0), (int)p.rows) - x.t0, p.max_tok);
   x.pos0 = positions[0];
-  if (x.pos0 < 0 || x.pos0 > (1 << 30)) x.n = 0;
+  if (x.pos0 < 0 || x.pos0 > (1 << 30) || x.n < p.from_tok || x.n > p.to_tok) x.n = 0;
   return x;
 }
 
@@ -1382,6 +1382,18 @@ F8AttnPlan f8_attn_plan(int num_q, int num_kv, int head_dim, int n_slots, long q
   x.o_off = pre + (recs * 8 + 255) / 256 * 256;
   x.total = x.o_off + recs * head_dim * 4;
   return x;
+}
+
+// A call may hold prompts and single tokens.  A one-token slot costs the kernel for many rows the
+// conversion of whole tiles for a 64th of their rows (32 slots at 4,000 keys and a prompt of 2,048
+// tokens: 221 us in one launch, 134 as two); a launch for nothing costs 7 us.  The numbers do not
+// say how the rows spread: the fewest slots that can hold them all are taken to be prompts, and the
+// others to have up to 16 rows, with whole contexts.
+int f8_attn_apart(int num_q, int num_kv, int head_dim, int n_slots, long rows, int max_tok, int max_ctx) {
+  const int gqa = num_q / num_kv;
+  if ((long)max_tok * gqa <= 64) return 0;
+  const double small = n_slots - (rows + max_tok - 1) / max_tok;
+  return small * num_kv * max_ctx * head_dim >= (double)(1 << 25) ? 16 / gqa : 0;
 }
 
 template <int HD>

@@ -202,10 +202,34 @@ static int check_f8_attn(int num_q, int num_kv, int head_dim, int n_slots, int n
   return QKV_OK;
 }
 
+}  // extern "C"
+
+namespace {
+
+// The launches of a call, one after the other in the same workspace: the slots of up to `apart`
+// tokens (if any), then the others.
+struct F8AttnPlans {
+  int apart;
+  qkv::F8AttnPlan few, rest;
+  size_t total() const { return apart ? std::max(few.total, rest.total) : rest.total; }
+};
+F8AttnPlans f8_attn_plans(int num_q, int num_kv, int head_dim, int n_slots, int n_rows, int max_tok, int max_ctx) {
+  if (max_tok > n_rows) max_tok = n_rows;
+  F8AttnPlans x{};
+  x.apart = qkv::f8_attn_apart(num_q, num_kv, head_dim, n_slots, n_rows, max_tok, max_ctx);
+  if (x.apart) x.few = qkv::f8_attn_plan(num_q, num_kv, head_dim, n_slots, n_rows, x.apart, max_ctx);
+  x.rest = qkv::f8_attn_plan(num_q, num_kv, head_dim, n_slots, n_rows, max_tok, max_ctx);
+  return x;
+}
+
+}  // namespace
+
+extern "C" {
+
 size_t qkv_attn_f8_paged_workspace_bytes(int num_q, int num_kv, int head_dim, int n_slots, int n_rows, int max_tok,
                                          int max_ctx) {
   if (check_f8_attn(num_q, num_kv, head_dim, n_slots, n_rows, max_tok, max_ctx) != QKV_OK) return 0;
-  return qkv::f8_attn_plan(num_q, num_kv, head_dim, n_slots, n_rows, max_tok < n_rows ? max_tok : n_rows, max_ctx).total;
+  return f8_attn_plans(num_q, num_kv, head_dim, n_slots, n_rows, max_tok, max_ctx).total();
 }
 
 int qkv_attn_f8_paged(const uint16_t* q, const uint8_t* k_pool, const uint8_t* v_pool, const uint8_t* k_exp,
@@ -224,8 +248,8 @@ int qkv_attn_f8_paged(const uint16_t* q, const uint8_t* k_pool, const uint8_t* v
       !aligned(block_tables, 4) || !aligned(starts, 4) || !aligned(positions, 4))
     return QKV_ERR_ALIGN;
   if (max_tok > n_rows) max_tok = n_rows;
-  const qkv::F8AttnPlan x = qkv::f8_attn_plan(num_q, num_kv, head_dim, n_slots, n_rows, max_tok, max_ctx);
-  if (!workspace || workspace_bytes < x.total) return QKV_ERR_WORKSPACE;
+  const F8AttnPlans plans = f8_attn_plans(num_q, num_kv, head_dim, n_slots, n_rows, max_tok, max_ctx);
+  if (!workspace || workspace_bytes < plans.total()) return QKV_ERR_WORKSPACE;
   if (!aligned(workspace, 256)) return QKV_ERR_ALIGN;
   qkv::F8AttnArgs a{};
   uint8_t* ws = static_cast<uint8_t*>(workspace);
@@ -241,8 +265,6 @@ int qkv_attn_f8_paged(const uint16_t* q, const uint8_t* k_pool, const uint8_t* v
   a.counts = reinterpret_cast<int*>(ws);
   a.cuts = a.counts + qkv::kJoinCounts;
   a.desc = reinterpret_cast<int2*>(a.cuts);
-  a.rec_ml = reinterpret_cast<float*>(ws + x.ml_off);
-  a.rec_o = reinterpret_cast<float*>(ws + x.o_off);
   a.rows = n_rows;
   a.num_q = num_q;
   a.num_kv = num_kv;
@@ -254,12 +276,23 @@ int qkv_attn_f8_paged(const uint16_t* q, const uint8_t* k_pool, const uint8_t* v
   a.n_pages = n_pages;
   a.window = window_tok;
   a.sink = sink_tok < max_ctx ? sink_tok : max_ctx;   // (rounded up to tiles in 32 bits)
-  a.slot_tiles = x.slot_tiles;
-  a.rec_rows = x.rec_rows;
-  a.groups = x.groups;
   a.bt_magic = (uint32_t)((1ull << 32) / (uint64_t)block_tokens);
   a.scale_log2 = scale * 1.4426950408889634f;
-  return launch_status(qkv::launch_f8_attn(a, x, head_dim, stream));
+  auto launch = [&](const qkv::F8AttnPlan& x, int from, int to) {
+    a.rec_ml = reinterpret_cast<float*>(ws + x.ml_off);
+    a.rec_o = reinterpret_cast<float*>(ws + x.o_off);
+    a.slot_tiles = x.slot_tiles;
+    a.rec_rows = x.rec_rows;
+    a.groups = x.groups;
+    a.from_tok = from;
+    a.to_tok = to;
+    return launch_status(qkv::launch_f8_attn(a, x, head_dim, stream));
+  };
+  if (plans.apart) {
+    const int st1 = launch(plans.few, 1, plans.apart);
+    if (st1 != QKV_OK) return st1;
+  }
+  return launch(plans.rest, plans.apart + 1, 0x7fffffff);
 }
 
 int qkv_pages_fork(int32_t* block_tables, int n_slots, int max_blocks, int block_tokens, int32_t* ref_counts,

@@ -179,6 +179,7 @@ struct F8AttnArgs {
   float* rec_o;              // workspace: its unnormalised sums
   long rows;
   int num_q, num_kv, n_slots, max_tok, max_ctx, max_blocks, block_tokens, n_pages, window, sink;
+  int from_tok, to_tok;      // the slots of this launch: those that own so many rows
   int slot_tiles;            // row tiles of a slot with max_tok tokens
   int rec_rows;              // rows of a record
   int groups;                // workgroups
@@ -197,6 +198,9 @@ struct F8AttnPlan {
   size_t ml_off, o_off, total;
 };
 F8AttnPlan f8_attn_plan(int num_q, int num_kv, int head_dim, int n_slots, long rows, int max_tok, int max_ctx);
+// Tokens of a slot up to which it goes to a launch of its own kind beside the one for many rows
+// (0: one launch for all).
+int f8_attn_apart(int num_q, int num_kv, int head_dim, int n_slots, long rows, int max_tok, int max_ctx);
 hipError_t launch_f8_attn(const F8AttnArgs& a, const F8AttnPlan& plan, int head_dim, hipStream_t stream);
 
 // Pages of a cache (kv_pages.hip): tables [n_slots][max_blocks] with a negative
@@ -221,7 +225,9 @@ hipError_t launch_pages_fork(const PageTables& t, const int32_t* parents, const 
 hipError_t launch_pages_release(const PageTables& t, const int32_t* slots, const int32_t* keep, int n,
                                 int32_t* status, const PageStatus& codes, hipStream_t stream);
 constexpr int kReserveMax = 1024;   // slots of one reserve call
-inline int reserve_blocks(int max_new, int block_tokens) { return (max_new + block_tokens - 2) / block_tokens + 1; }
+inline int reserve_blocks(int max_new, int block_tokens) {
+  return (int)(((long)max_new + block_tokens - 2) / block_tokens + 1);
+}
 // scratch: reserve_scratch_ints(n, blocks) int32, the copied pairs [n][2] first
 inline size_t reserve_scratch_ints(int n, int blocks) { return 3 * (size_t)n + 2 * (size_t)n * blocks; }
 hipError_t launch_pages_reserve(const PageTables& t, const int32_t* slots, const int32_t* positions,

@@ -185,6 +185,16 @@ def test_prompts(hd, bt, lens, new, gqa):
     _check_attn(_attn_case(hd + bt + gqa, lens, new, bt, 2, gqa, hd), hd ** -0.5)
 
 
+@pytest.mark.parametrize("hd,gqa", [(128, 4), (256, 4), (128, 1), (256, 6), (128, 8)])
+@pytest.mark.parametrize("lens,new", [
+    ([500, 3, 0, 300, 64, 1000], [1, 200, 1, 2, 0, 1]),       # single tokens beside a prompt
+    ([500, 3, 90, 300, 64, 10], [5, 400, 17, 2, 3, 9]),       # on both sides of the bound
+    ([10, 20, 30], [80, 90, 100]), ([0], [130])])             # none to take apart
+def test_prompts_with_single_tokens(lens, new, hd, gqa):
+    """Slots of few tokens go to a launch of their own where contexts may be long; two of them share the workspace."""
+    _check_attn(_attn_case(hd + gqa, lens, new, 16, 2, gqa, hd), hd ** -0.5, max_ctx=1 << 20)
+
+
 @pytest.mark.parametrize("new", [[1, 1, 1], [6, 1, 9], [70, 3, 100]])
 @pytest.mark.parametrize("window,sink", [(1, 0), (20, 0), (64, 4), (100, 33), (5000, 1), (7, 2**31 - 1), (2**31 - 1, 2**31 - 1)])
 def test_window_and_sinks(new, window, sink):
