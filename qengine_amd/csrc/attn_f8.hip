@@ -125,16 +125,6 @@ __device__ __forceinline__ RowTile row_tile(const F8AttnArgs& p, const Slot& x, 
   return r;
 }
 
-// Units of entry x = slot * slot_tiles + row tile: its key tiles, and LEAD for what a row tile
-// costs beside them (its queries, first loads and output)
-template <int ROWS, int KT, int LEAD>
-__device__ __forceinline__ int entry_units(const F8AttnArgs& p, int x, int gqa) {
-  const int s = x / p.slot_tiles, i = x - s * p.slot_tiles;
-  const Slot sl = slot_of(p, s);
-  if (i * ROWS >= sl.n * gqa) return 0;
-  return LEAD + row_tile<ROWS, KT>(p, sl, i, gqa).tiles;
-}
-
 // Where a workgroup's part begins: entry, and units of it before the part
 struct Part {
   int entry, at;
@@ -166,42 +156,76 @@ __device__ __forceinline__ int block_scan(int v, int* lds, int& sum) {   // incl
   return add_units(v, before);
 }
 
-// The units of one head's line (0: too long, which starts in order cannot make it)
+// The line of one head: the row tiles of the slots in order, ROWS rows and key tiles of KT keys,
+// each LEAD units for what it costs beside its key tiles (queries, first loads, output) and one
+// for each of those.  Walked THREADS slots at a time: their row tiles are counted, then taken up by as
+// many threads as there are (most slots of a batch may hold none here).
 template <int ROWS, int KT, int LEAD, int THREADS>
-__device__ __forceinline__ int line_units(const F8AttnArgs& p, int gqa, int* lds) {
-  const int entries = p.n_slots * p.slot_tiles;
-  int base = 0;
-  for (int c = 0; c < entries; c += THREADS) {
-    const int x = c + threadIdx.x;
-    int sum;
-    block_scan<THREADS>(x < entries ? entry_units<ROWS, KT, LEAD>(p, x, gqa) : 0, lds, sum);
-    base = add_units(base, sum);
-  }
-  return base < kLineMax && (long)base * p.num_kv < (1l << 31) ? base : 0;
-}
-// The entry that holds unit u of the line (u < its length)
-template <int ROWS, int KT, int LEAD, int THREADS>
-__device__ __forceinline__ Part line_find(const F8AttnArgs& p, int gqa, int u, int* lds) {
-  const int entries = p.n_slots * p.slot_tiles;
-  __shared__ int found[2];
-  int base = 0;
-  for (int c = 0; c < entries; c += THREADS) {
-    const int x = c + threadIdx.x;
-    const int mine = x < entries ? entry_units<ROWS, KT, LEAD>(p, x, gqa) : 0;
-    int sum;
-    const int inc = base + block_scan<THREADS>(mine, lds, sum);
-    if (u >= inc - mine && u < inc) {
-      found[0] = x;
-      found[1] = u - (inc - mine);
+struct RowLine {
+  const F8AttnArgs& p;
+  int gqa;
+  int *lds, *upto;             // THREADS / 64 and THREADS ints of LDS
+  int entry, mine, inc;        // this thread's row tile of the last step (slot * slot_tiles + tile), its
+                               // units and the line's up to its end
+  bool one = true;             // the line is one step: what the registers hold
+
+  template <class F>
+  __device__ __forceinline__ void walk(F&& done) {   // done(units so far): whether to stop
+    int base = 0;
+    for (int s0 = 0; s0 < p.n_slots; s0 += THREADS) {
+      const int s = s0 + (int)threadIdx.x;
+      int n;
+      const int tiles = s < p.n_slots ? (slot_of(p, s).n * gqa + ROWS - 1) / ROWS : 0;
+      upto[threadIdx.x] = block_scan<THREADS>(tiles, lds, n);
+      __syncthreads();
+      n = __builtin_amdgcn_readfirstlane(n);
+      for (int x0 = 0; x0 < n; x0 += THREADS) {
+        const int x = x0 + (int)threadIdx.x;
+        mine = 0;
+        if (x < n) {
+          int lo = 0, hi = THREADS - 1;   // the first slot whose tiles end past x
+#pragma unroll
+          for (int w = THREADS / 2; w; w >>= 1) {
+            const int mid = (lo + hi) / 2;
+            if (upto[mid] > x) hi = mid; else lo = mid + 1;
+          }
+          const int i = x - (lo ? upto[lo - 1] : 0);
+          entry = (s0 + lo) * p.slot_tiles + i;
+          mine = LEAD + row_tile<ROWS, KT>(p, slot_of(p, s0 + lo), i, gqa).tiles;
+        }
+        int sum;
+        inc = add_units(base, block_scan<THREADS>(mine, lds, sum));
+        base = __builtin_amdgcn_readfirstlane(add_units(base, sum));
+        if (done(base)) return;
+      }
+      __syncthreads();   // (upto is written again)
     }
-    base += sum;
-    if (base > u) break;
   }
-  __syncthreads();
-  const Part r{__builtin_amdgcn_readfirstlane(found[0]), __builtin_amdgcn_readfirstlane(found[1])};
-  __syncthreads();
-  return r;
-}
+  // units of the line (0: too many, which starts in order cannot make)
+  __device__ __forceinline__ int units() {
+    int total = 0, steps = 0;
+    walk([&](int so_far) {
+      total = so_far;
+      steps++;
+      return false;
+    });
+    one = steps <= 1;
+    return total < kLineMax && (long)total * p.num_kv < (1l << 31) ? total : 0;
+  }
+  // the row tile that holds unit u of the line (u < its length)
+  __device__ __forceinline__ Part find(int u, int* found) {
+    auto look = [&](int so_far) {
+      if (u >= inc - mine && u < inc) {
+        found[0] = entry;
+        found[1] = u - (inc - mine);
+      }
+      return so_far > u;
+    };
+    if (one) look(0); else walk(look);
+    __syncthreads();
+    return {__builtin_amdgcn_readfirstlane(found[0]), __builtin_amdgcn_readfirstlane(found[1])};
+  }
+};
 // Parts of the line: at most a workgroup's each and none empty, the first `more` of them one
 // unit longer (the units of all heads stay below 2^31: the host sees to it).
 struct Parts {
@@ -905,13 +929,14 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   constexpr int KB = KT * KP, VB = HD * VP + HD / VPAD * 16;
   __shared__ __align__(16) uint8_t tile_lds[2][KB + VB];
   __shared__ __align__(16) uint8_t raw_lds[2][8192];
-  __shared__ int lds[WAVES];
+  __shared__ int lds[WAVES], upto[THREADS], found[2];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 31, hh = lane >> 5;
   const int gqa = p.num_q / p.num_kv;
 
   // (the same in every lane: said to the compiler, what follows stays out of the vector registers)
-  const int total = __builtin_amdgcn_readfirstlane(line_units<ROWS, KT, LEAD, THREADS>(p, gqa, lds));
+  RowLine<ROWS, KT, LEAD, THREADS> line{p, gqa, lds, upto};
+  const int total = __builtin_amdgcn_readfirstlane(line.units());
   const int all = __builtin_amdgcn_readfirstlane(total * p.num_kv);
   if (blockIdx.x == 0 && tid == 0) p.cuts[4 * p.groups] = all;
   // neighbouring parts (the same head's keys) on one XCD, whose L2 holds their tiles
@@ -921,7 +946,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   int u = parts.begin(grp);
   const int u_end = parts.begin(grp + 1);
   int h = u / total;
-  Part at = line_find<ROWS, KT, LEAD, THREADS>(p, gqa, u - h * total, lds);
+  Part at = line.find(u - h * total, found);
   bool first_seg = true;
   const uint32_t key_bytes = (uint32_t)p.num_kv * HD;
   const uint32_t page_bytes = (uint32_t)p.block_tokens * key_bytes;
@@ -931,12 +956,19 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   while (u < u_end) {
     const int s = at.entry / p.slot_tiles, rti = at.entry - s * p.slot_tiles;
     const Slot sl = slot_at(p, s);
-    if (rti * ROWS >= sl.n * gqa) {   // past this slot's rows
-      at.entry = (s + 1) * p.slot_tiles;
-      if (at.entry >= entries) {
-        at.entry = 0;
-        h++;
+    if (rti * ROWS >= sl.n * gqa) {   // past this slot's rows: on to the next slot with any, 64 at a time
+      uint64_t any = 0;
+      int t = s + 1;
+      while (true) {
+        if (t >= p.n_slots) {
+          t = 0;
+          h++;
+        }
+        any = __builtin_amdgcn_ballot_w64(t + lane < p.n_slots && slot_of(p, min(t + lane, p.n_slots - 1)).n > 0);
+        if (any) break;
+        t += 64;
       }
+      at.entry = (t + __builtin_ctzll(any)) * p.slot_tiles;
       continue;
     }
     const RowTile rt = row_tile<ROWS, KT>(p, sl, rti, gqa);
