@@ -913,12 +913,16 @@ __global__ __launch_bounds__(256, 1) void f8_mid_kernel(F8AttnArgs p) {
 // by dim, four keys to 8 bytes, in the order that the scores' lanes hold them.  Pads
 // keep 16-byte reads of 16 lanes on distinct banks, at constant offsets of one address.
 
-// A row tile's cost beside its key tiles, in tiles (11 us against 2.1; six ragged prompts: 187 us at 2, 156 at 4 and 6, 165 at 9)
-constexpr int kLead = 6;
+// A row tile's cost beside its key tiles, in tiles (measured to its first product and from its last:
+// 11 us against 2.1 a tile at head_dim 256, 8 against 2.6 at 128; and a part that begins inside a row
+// tile pays it too).  Geometric mean over 44 batches of prompts of 300 to 8,000 tokens: 98.7 us at
+// 4, 95.5 at 6, 93.9 at 8, 92.6 at 10 and 5, 93.3 at 14 and 5.
+template <int HD>
+constexpr int kLead = HD == 256 ? 10 : 5;
 
 template <int HD>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void f8_many_kernel(F8AttnArgs p) {
-  constexpr int WAVES = 8, ROWS = 32 * WAVES, THREADS = 64 * WAVES, LEAD = kLead;
+  constexpr int WAVES = 8, ROWS = 32 * WAVES, THREADS = 64 * WAVES, LEAD = kLead<HD>;
   constexpr int KT = 8192 / HD;              // 32 or 64 keys: 8 KB of codes
   constexpr int KH = KT / 32;                // 32-key halves
   constexpr int WK = KT / WAVES;             // keys that a wave loads and converts
@@ -1270,7 +1274,7 @@ __global__ __launch_bounds__(256) void f8_cut_merge_kernel(F8AttnArgs p) {
   const int entry = cut.x, h = cut.y, v0 = cut.z, tiles = cut.w;
   if (entry < 0) return;
   // units of the row tile's first key tile, and of its lead
-  const int x1 = parts.begin(grp) - v0, x0 = x1 - kLead, before = parts.begin(grp - 1);
+  const int x1 = parts.begin(grp) - v0, x0 = x1 - kLead<HD>, before = parts.begin(grp - 1);
   if (before > x1) return;   // an earlier cut is in this tile
   const int n = parts.of(x1 + tiles - 1) - grp + 2;
   const long r0 = 2 * (grp - 1) + (before >= x0 ? 0 : 1);

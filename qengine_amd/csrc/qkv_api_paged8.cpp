@@ -197,7 +197,7 @@ static int check_f8_attn(int num_q, int num_kv, int head_dim, int n_slots, int n
   // a head's in 30)
   const double gqa = num_q / num_kv, full = (double)n_slots * ((double)max_tok * gqa / 256 + 1);
   const double tiles = full < n_rows * gqa / 256 + n_slots ? full : n_rows * gqa / 256 + n_slots;
-  if (full * num_kv > (double)(1 << 22) || tiles * std::max(num_kv, 2) * (max_ctx / 32.0 + 8) > 2147483000.0)
+  if (full * num_kv > (double)(1 << 22) || tiles * std::max(num_kv, 2) * (max_ctx / 32.0 + 16) > 2147483000.0)
     return QKV_ERR_UNSUPPORTED;
   return QKV_OK;
 }
