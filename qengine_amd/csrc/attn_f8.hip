@@ -915,8 +915,9 @@ __global__ __launch_bounds__(256, 1) void f8_mid_kernel(F8AttnArgs p) {
 
 // A row tile's cost beside its key tiles, in tiles (measured to its first product and from its last:
 // 11 us against 2.1 a tile at head_dim 256, 8 against 2.6 at 128; and a part that begins inside a row
-// tile pays it too).  Geometric mean over 44 batches of prompts of 300 to 8,000 tokens: 98.7 us at
-// 4, 95.5 at 6, 93.9 at 8, 92.6 at 10 and 5, 93.3 at 14 and 5.
+// tile pays it too).  Geometric mean over 44 batches of prompts of 300 to 8,000 tokens, the loop as
+// it then was: 98.7 us at 4, 95.5 at 6, 93.9 at 8, 92.6 at 10 and 5; now 90.3 to 91.1 anywhere
+// between 8 and 4 and 12 and 6.
 template <int HD>
 constexpr int kLead = HD == 256 ? 10 : 5;
 
@@ -1027,7 +1028,9 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       load_pages(x.b);
       w_row = x.row;
     };
-    float ksc = 0.f, vsc = 0.f;      // the fetched tile's exponents as factors
+    // the fetched tile's exponents: the aligned words around them, by scalar loads (a vector load's
+    // first use would wait for the codes under way too), and the bits at which they lie
+    uint32_t kx = 0, vx = 0, k_bit = 0, v_bit = 0;
     int loaded = -1;                 // and its page
     const uint32_t lane_off = (uint32_t)(lane / LPR) * key_bytes + (uint32_t)(lane % LPR) * 16;
     const uint8_t* k_head = p.k_pool + (long)h * HD;
@@ -1036,11 +1039,16 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       loaded = __builtin_amdgcn_readlane(pages, w_at);
       const uint32_t pg = max(loaded, 0);
       const uint64_t from = (uint64_t)pg * page_bytes + (uint32_t)w_row * key_bytes;
-      __builtin_amdgcn_global_load_lds((glb_void*)(k_head + from + lane_off), (lds_void*)(raw_lds[0] + wave * 1024), 16, 0, 0);
-      __builtin_amdgcn_global_load_lds((glb_void*)(v_head + from + lane_off), (lds_void*)(raw_lds[1] + wave * 1024), 16, 0, 0);
+      uint32_t lo = lane_off;
+      asm volatile("" : "+v"(lo));   // (else both sums with the bases are kept in registers)
+      __builtin_amdgcn_global_load_lds((glb_void*)(k_head + from + lo), (lds_void*)(raw_lds[0] + wave * 1024), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((glb_void*)(v_head + from + lo), (lds_void*)(raw_lds[1] + wave * 1024), 16, 0, 0);
       const uint32_t ex = pg * (uint32_t)p.num_kv + h;
-      ksc = pow2f(p.k_exp[ex]);
-      vsc = pow2f(p.v_exp[ex]);
+      const uint64_t ka = (uint64_t)p.k_exp + ex, va = (uint64_t)p.v_exp + ex;
+      kx = *(const const_i32*)(ka & ~3ull);
+      vx = *(const const_i32*)(va & ~3ull);
+      k_bit = 8 * (uint32_t)(ka & 3);
+      v_bit = 8 * (uint32_t)(va & 3);
       // on to the next tile
       w_row += kt_mod;
       w_at += kt_div;
@@ -1067,8 +1075,9 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
         for (int i = 0; i < 4; i++)
           if (loaded < 0 || key0 + 4 * vq + i >= rt.end) vr[i] = 0;
-        if (loaded < 0) vsc = 1.f;   // (an absent page's exponent is not one)
       }
+      // (an absent page's exponent is not one)
+      const float ksc = pow2f((kx >> k_bit) & 255u), vsc = pow2f(loaded < 0 ? 127 : (vx >> v_bit) & 255u);
       uint8_t* kb = tile_lds[buf];
       uint8_t* vb = kb + KB;
       const int key = wave * WK + lane / LPR, slot = lane % LPR;
@@ -1124,7 +1133,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     float mx = -INFINITY, ls = 0.f;
     // a negative scale is carried by the query, so that raw maxima serve; masked scores are -inf
     // ahead of the scale
-    const float sl2 = fmaxf(fabsf(p.scale_log2), 1e-30f);
+    const float sl2 = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(fmaxf(fabsf(p.scale_log2), 1e-30f))));
     if (p.scale_log2 < 0.f) {
 #pragma unroll
       for (int i = 0; i < HD / 16; i++) qf[i] = -qf[i];
@@ -1135,91 +1144,91 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     __syncthreads();
     for (int v = v0; v < v1; v++) {
       const int buf = (v - v0) & 1;
-      // one wave of each SIMD converts ahead of its products, the other after them
-      if (wave < 4) advance(v, buf);
+      advance(v, buf);
       if (v < v_hi && !(v >= v_sink && v < v_lo)) {   // (a wave none of whose rows sees the tile sits it out)
-        __builtin_amdgcn_s_setprio(1);
         const uint8_t* kb = tile_lds[buf];
         const uint8_t* vb = kb + KB;
+        // scores of the tile's halves in turn (two chains of products at head_dim 128)
+        const uint8_t* krow = kb + c * KP + hh * 16;
+        auto k_operand = [&](int i) { return *reinterpret_cast<const h8_t*>(krow + i % KH * (32 * KP) + i / KH * 32); };
+        constexpr int NK = KH * HD / 16;
+        f16x_t sd[KH] = {};
+        h8_t ka[4];
 #pragma unroll
-        for (int kh = 0; kh < KT / 32; kh++) {
-          const uint8_t* krow = kb + 32 * kh * KP + c * KP + hh * 16;
-          auto k_operand = [&](int i) { return *reinterpret_cast<const h8_t*>(krow + i * 32); };
-          constexpr int NK = HD / 16;
-          f16x_t sd = f16x_t{};
-          h8_t ka[3];
+        for (int i = 0; i < 4; i++) ka[i] = k_operand(i);
 #pragma unroll
-          for (int i = 0; i < 3; i++) ka[i] = k_operand(i);
+        for (int i = 0; i < NK; i++) {
+          sd[i % KH] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka[i % 4], qf[i / KH], sd[i % KH], 0, 0, 0);
+          if (i + 4 < NK) ka[i % 4] = k_operand(i + 4);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
 #pragma unroll
-          for (int i = 0; i < NK; i++) {
-            sd = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka[i % 3], qf[i], sd, 0, 0, 0);
-            if (i + 3 < NK) ka[i % 3] = k_operand(i + 3);
-          }
-          __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
+        for (int i = 0; i < NK - 4; i++) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
+        const uint8_t* vat = vb + c * VP + c / VPAD * 16 + hh * 16;
+        constexpr int ND = HD / 32, NV = 2 * KH * ND;   // 32-dim blocks; of each 16 keys in turn
+        auto v_operand = [&](int i) {
+          return *reinterpret_cast<const h8_t*>(vat + i % ND * (32 * VP + 32 / VPAD * 16) + i / ND * 32);
+        };
 #pragma unroll
-          for (int i = 0; i < NK - 3; i++) {
-            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-          }
-          __builtin_amdgcn_sched_group_barrier(0x008, 3, 0);
-          // the first values' reads go ahead of the weights
-          const uint8_t* vat = vb + c * VP + c / VPAD * 16 + hh * 16 + kh * 64;
-          constexpr int NV = HD / 16;   // of 16 keys, then of the other 16
-          auto v_operand = [&](int i) {
-            return *reinterpret_cast<const h8_t*>(vat + (i % (NV / 2)) * (32 * VP + 32 / VPAD * 16) + i / (NV / 2) * 32);
-          };
-          h8_t va[3];
-#pragma unroll
-          for (int i = 0; i < 3; i++) va[i] = v_operand(i);
+        for (int kh = 0; kh < KH; kh++) {
           const int y = v * KH + kh, k0 = (y < rt.n_sink * KH ? y : y + y_off) * 32;
           if (!((y >= y_lo && y < y_hi) || y < y_sink) || !paged) {
             const bool pa = page_of(k0) >= 0, pb = page_of(k0 + 16) >= 0;
 #pragma unroll
             for (int x = 0; x < 16; x++) {
               const int key = k0 + 8 * (x >> 2) + 4 * hh + (x & 3);
-              sd[x] = (x < 8 ? pa : pb) && sees(key, pos, rt.end, p.window, p.sink) ? sd[x] : -INFINITY;
+              sd[kh][x] = (x < 8 ? pa : pb) && sees(key, pos, rt.end, p.window, p.sink) ? sd[kh][x] : -INFINITY;
             }
           }
-          float t = sd[0];
-#pragma unroll
-          for (int x = 1; x < 16; x++) t = fmaxf(t, sd[x]);
-          t = max32(t) * sl2;
-          if (__builtin_amdgcn_ballot_w64(t > mx + kSlack) != 0) {
-            const float mn = fmaxf(mx, t);
-            const float r = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mx - mn);
-            ls *= r;
-#pragma unroll
-            for (int d = 0; d < HD / 32; d++) acc[d] *= r;
-            mx = mn;
-          }
-          const float base = mx == -INFINITY ? 0.f : mx;
-          auto weights = [&](int sg) {
-            h8_t w;
-#pragma unroll
-            for (int i = 0; i < 8; i++) w[i] = (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(sd[8 * sg + i], sl2, -base));
-            ls = add8(w, ls);
-            return w;
-          };
-          const h8_t w0 = weights(0);
-          __builtin_amdgcn_sched_barrier(0);
-          // the second weights are formed under the first products
-          const h8_t w1 = weights(1);
-#pragma unroll
-          for (int i = 0; i < NV; i++) {
-            acc[i % (NV / 2)] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va[i % 3], i < NV / 2 ? w0 : w1, acc[i % (NV / 2)], 0, 0, 0);
-            if (i + 3 < NV) va[i % 3] = v_operand(i + 3);
-          }
-#pragma unroll
-          for (int i = 0; i < NV - 3; i++) {
-            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-            if (i < NV / 2 - 1) __builtin_amdgcn_sched_group_barrier(0x002, HD == 256 ? 5 : 10, 0);
-          }
-          __builtin_amdgcn_sched_group_barrier(0x008, 3, 0);
         }
+        // the first values' reads go ahead of the weights (and behind the masks, which need the registers)
+        h8_t va[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) va[i] = v_operand(i);
+        float t = sd[0][0];
+#pragma unroll
+        for (int x = 1; x < 16 * KH; x++) t = fmaxf(t, sd[x / 16][x % 16]);
+        t = max32(t) * sl2;
+        if (__builtin_amdgcn_ballot_w64(t > mx + kSlack) != 0) {
+          const float mn = fmaxf(mx, t);
+          const float r = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mx - mn);
+          ls *= r;
+#pragma unroll
+          for (int d = 0; d < HD / 32; d++) acc[d] *= r;
+          mx = mn;
+        }
+        const float base = mx == -INFINITY ? 0.f : mx;
+        auto weights = [&](int sg) {
+          h8_t w;
+#pragma unroll
+          for (int i = 0; i < 8; i++)
+            w[i] = (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(sd[sg / 2][8 * (sg % 2) + i], sl2, -base));
+          ls = add8(w, ls);
+          return w;
+        };
+        h8_t w[2 * KH];
+        w[0] = weights(0);
+        __builtin_amdgcn_sched_barrier(0);
+        // the other weights are formed under the products of those before them
+#pragma unroll
+        for (int g = 1; g < 2 * KH; g++) w[g] = weights(g);
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+          acc[i % ND] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va[i % 4], w[i / ND], acc[i % ND], 0, 0, 0);
+          if (i + 4 < NV) va[i % 4] = v_operand(i + 4);
+        }
+#pragma unroll
+        for (int i = 0; i < NV - 4; i++) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+          if (i < NV - ND - 1) __builtin_amdgcn_sched_group_barrier(0x002, HD == 256 ? 4 : 6, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
       }
-      __builtin_amdgcn_s_setprio(0);
-      if (wave >= 4) advance(v, buf);
       __syncthreads();
     }
 
