@@ -1,6 +1,13 @@
 // attn_f8.hip -- attention over the paged 8-bit cache (e4m3 codes, one power-of-two
 // exponent per page and KV head): ragged batches of one token to whole prompts a slot.
 //
+//   o_t = sum_j w_j v_j / sum_j w_j,  w_j = 2^(scale log2(e) q_t . k_j - m)
+//
+// over the keys j that query t sees, in one pass: m is the reference maximum of the keys so
+// far, and raising it rescales both sums.  Single tokens and verify blocks read 2 * head_dim
+// bytes a key and KV head and are bound by HBM; prompts do 4 * head_dim operations a (head,
+// visible pair) and are bound by the matrix cores.
+//
 // Rows.  The rows of a (slot, KV head) are its (token, query head of the group) pairs,
 // row = token * gqa + head, so that a K/V tile read once serves the whole group.
 // Operands are swapped: S^T = K Q^T and O^T = V^T P^T, so that a lane's scores of a
@@ -253,7 +260,7 @@ __device__ __forceinline__ bool sees(int key, int pos, int end, int window, int 
 }  // namespace
 
 // ---------------------------------------------------------------------------
-// few rows: up to 64 (token, head) rows of a slot and KV head
+// few rows: up to 16 (token, head) rows of a slot and KV head
 // ---------------------------------------------------------------------------
 // One row tile a slot; the line of units is held 64 slots at a time in the lanes of each
 // wave (no LDS, no barrier ahead of the first loads of keys).
@@ -341,11 +348,17 @@ __device__ __forceinline__ Tile tile_at(const F8AttnArgs& p, const const_i32* ta
 // Four waves, each with key tiles of its own (every fourth of the part's 32-key tiles), joined
 // through LDS at the end: nothing is shared on the way, so a wave waits only for its
 // own loads, and K, V of the next tile are in flight while this one is computed
-// (16 KB a wave at head_dim 256).  K rows are the A operand as loaded: lane l%16 is
-// the key, and the group l/16 takes the same dims of K and Q.  V comes four keys
-// by a run of dims, and byte permutes pair the keys ahead of the conversion.
-// JOIN: contexts of up to kJoinKeys keys, whose records the last workgroup of a tile
-// joins in this launch.
+// (16 KB a wave at head_dim 256; 128 KB a CU at two workgroups).  K rows are the A operand as
+// loaded: lane l%16 is the key, and the group l/16 takes the same dims of K and Q.  V comes
+// four keys by a run of dims, and byte permutes pair the keys ahead of the conversion.
+// Bound by HBM: one slot at 131,072 keys, GQA 4, 4 KV heads of 256, 268 MB in 48.5 us (5.5 TB/s; a
+// kernel that only reads reaches 6.4), 5 us of merge after it; 32 slots of 500 to 32,768 keys in
+// 16-row pages of 128, 358 MB in 65 us.  Parts for 256, 768 or 1,024 workgroups were slower than
+// for 512 (two a CU).
+// JOIN: contexts of up to kJoinKeys keys, whose records the last workgroup of a tile joins in this
+// launch: there latency is all (700 keys: 10.6 us; with the merge's launch 12.9; by one workgroup
+// of eight waves a KV head 13.4).  Longer contexts have too many records for it (16 slots at 2,000
+// keys 19.4 against 15.5 us).
 constexpr int kJoinKeys = 1024, kJoinStep = 8;
 template <int HD, bool JOIN>
 __global__ __launch_bounds__(256, 2) void f8_few_kernel(F8AttnArgs p) {
@@ -656,11 +669,16 @@ __global__ __launch_bounds__(256, 2) void f8_few_kernel(F8AttnArgs p) {
 // side on the same keys (the second's loads meet the first's lines in the caches), 4 / RG
 // key streams.  Otherwise as above: lane l%32 is the key of K's operand and takes 16 of
 // every 32 dims; V comes by runs of HD/32 dims, and output block d has dims HD/32 * m + d.
-// One wave a SIMD holds the sums, so the codes of two tiles ahead wait in LDS, loaded there
-// past the registers (32 KB a wave at head_dim 256).  K's 16-byte chunks are permuted within
-// a row by the row's number, which keeps its reads on distinct banks.
+// At head_dim 256 one wave a SIMD holds the sums, so the codes of two tiles ahead wait in LDS,
+// loaded there past the registers (32 KB a wave; with one tile ahead in registers 93 against 83 us)
+// and past the caches (RG = 1: every byte is used once).  At 128 two workgroups fit a CU (9 tokens, GQA
+// 4, at 131,072 keys: 49 against 60 us with one).  K's 16-byte chunks are permuted within a row by
+// the row's number, which keeps its reads on distinct banks.  Up to 32 rows bound by HBM: four slots of
+// 5 to 8 tokens, GQA 4, at 32K to 64K keys, 403 MB in 80 us (5.0 TB/s).  Beyond, by one wave's chain
+// of scores, softmax and values: 16 tokens at 131,072 keys, 268 MB, 95 us (8 tokens 65; one wave with
+// both row groups needs more registers than there are).
 template <int HD, int RG>
-__global__ __launch_bounds__(256, 1) void f8_mid_kernel(F8AttnArgs p) {
+__global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void f8_mid_kernel(F8AttnArgs p) {
   constexpr int KT = 32, ROWS = 32 * RG, KG = 4 / RG, PER = KG, THREADS = 256;
   constexpr int KW = HD / 32;        // 16-byte key loads of a lane
   constexpr int DB = HD / 32;        // 32-dim blocks of the output, value bytes of a lane and key
@@ -719,8 +737,8 @@ __global__ __launch_bounds__(256, 1) void f8_mid_kernel(F8AttnArgs p) {
           const int r0 = l * RL;     // first row of the load, in the half
           const uint32_t k_off = ld_row * key_bytes + ((ld_chunk ^ ((r0 + ld_row) & (HD / 16 - 1))) * 16);
           const int to = (16 * hf + r0) * HD;
-          __builtin_amdgcn_global_load_lds((glb_void*)(p.k_pool + from + (long)r0 * key_bytes + k_off), (lds_void*)(ring[par][0] + to), 16, 0, 2);
-          __builtin_amdgcn_global_load_lds((glb_void*)(p.v_pool + from + (long)r0 * key_bytes + v_off), (lds_void*)(ring[par][1] + to), 16, 0, 2);
+          __builtin_amdgcn_global_load_lds((glb_void*)(p.k_pool + from + (long)r0 * key_bytes + k_off), (lds_void*)(ring[par][0] + to), 16, 0, RG == 1 ? 2 : 0);
+          __builtin_amdgcn_global_load_lds((glb_void*)(p.v_pool + from + (long)r0 * key_bytes + v_off), (lds_void*)(ring[par][1] + to), 16, 0, RG == 1 ? 2 : 0);
         }
         ke[par][hf] = p.k_exp[pg * p.num_kv + h];
         ve[par][hf] = p.v_exp[pg * p.num_kv + h];
@@ -912,6 +930,14 @@ __global__ __launch_bounds__(256, 1) void f8_mid_kernel(F8AttnArgs p) {
 // wave the rows that it loaded itself, so only its own loads are waited for.  V is stored
 // by dim, four keys to 8 bytes, in the order that the scores' lanes hold them.  Pads
 // keep 16-byte reads of 16 lanes on distinct banks, at constant offsets of one address.
+// At head_dim 128 a tile is two halves of 32 keys, both scored before the weights, which are
+// formed under the products of those before them.  All waves convert ahead of their products: one of
+// each SIMD behind them was slower (1,112 against 1,070 us below), and so were two workgroups of
+// four waves a CU.
+// Bound by the matrix cores at 2,048 tokens over 32,000 keys, GQA 4, 4 KV heads of 256: 1,108 GFLOP in
+// 1,075 us, 1.03 PFLOP/s (a library product of fp16 matrices: 1.19; the conversion of tiles takes
+// about a quarter).  Short prompts pay 8 to 11 us a row tile before its first product and after its
+// last: six of 150 to 4,000 tokens, GQA 8, 128, window 1,500: 88 GFLOP in 157 us.
 
 // A row tile's cost beside its key tiles, in tiles (measured to its first product and from its last:
 // 11 us against 2.1 a tile at head_dim 256, 8 against 2.6 at 128; and a part that begins inside a row
@@ -1270,7 +1296,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 
 // The row tiles that parts cut: a wave per 32 rows and 32 dims, in the registers' order of the
 // kernel above; the workgroups of a part's cut only if the tile begins in the part before
-// (each tile once).
+// (each tile once).  Bound by HBM: the records of 256 parts of 256 rows of 256, 134 MB, in 25 us.
 template <int HD>
 __global__ __launch_bounds__(256) void f8_cut_merge_kernel(F8AttnArgs p) {
   constexpr int ROWS = 256, DB = HD / 32, WGS = 8 * DB / 4;
@@ -1324,7 +1350,8 @@ __global__ __launch_bounds__(256) void f8_cut_merge_kernel(F8AttnArgs p) {
 // ---------------------------------------------------------------------------
 // merge of the row tiles that were cut
 // ---------------------------------------------------------------------------
-// A workgroup per row.
+// A workgroup per row, whose waves share its records; bound by latency (5 us: the row's place, then
+// its records at once).
 template <int HD>
 __global__ __launch_bounds__(256) void f8_merge_kernel(F8AttnArgs p) {
   constexpr int E = HD / 64;
@@ -1417,7 +1444,7 @@ F8AttnPlan f8_attn_plan(int num_q, int num_kv, int head_dim, int n_slots, long q
     x.join = x.row_tiles == 1 && max_ctx <= kJoinKeys && n_slots <= 64 && n_slots * num_kv <= kJoinCounts;
     const int unit_keys = x.row_tiles == 4 ? 64 : 128;
     units = (long)n_slots * num_kv * ((max_ctx + unit_keys - 1) / unit_keys);
-    x.groups = (int)std::min<long>(units, x.row_tiles == 1 ? 512 : 256);
+    x.groups = (int)std::min<long>(units, x.row_tiles == 1 || head_dim == 128 ? 512 : 256);   // (what the CUs hold at once)
     x.merges = max_ctx > unit_keys;   // (else no slot has two units)
   }
   const size_t ints = x.many ? 4 * (size_t)x.groups + 4 : 2 * (size_t)n_slots * num_kv;
