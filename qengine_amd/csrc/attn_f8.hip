@@ -351,13 +351,13 @@ __device__ __forceinline__ Tile tile_at(const F8AttnArgs& p, const const_i32* ta
 // (16 KB a wave at head_dim 256; 128 KB a CU at two workgroups).  K rows are the A operand as
 // loaded: lane l%16 is the key, and the group l/16 takes the same dims of K and Q.  V comes
 // four keys by a run of dims, and byte permutes pair the keys ahead of the conversion.
-// Bound by HBM: one slot at 131,072 keys, GQA 4, 4 KV heads of 256, 268 MB in 48.5 us (5.5 TB/s; a
+// Bound by HBM: one slot at 131,072 keys, GQA 4, 4 KV heads of 256, 268 MB in 48 to 50 us (5.5 TB/s; a
 // kernel that only reads reaches 6.4), 5 us of merge after it; 32 slots of 500 to 32,768 keys in
-// 16-row pages of 128, 358 MB in 65 us.  Parts for 256, 768 or 1,024 workgroups were slower than
+// 16-row pages of 128, 358 MB in 64 to 67 us.  Parts for 256, 768 or 1,024 workgroups were slower than
 // for 512 (two a CU).
 // JOIN: contexts of up to kJoinKeys keys, whose records the last workgroup of a tile joins in this
-// launch: there latency is all (700 keys: 10.6 us; with the merge's launch 12.9; by one workgroup
-// of eight waves a KV head 13.4).  Longer contexts have too many records for it (16 slots at 2,000
+// launch: there latency is all (a call at 700 keys 10.9 us, with the merge's launch 12.6; by one
+// workgroup of eight waves a KV head 13.4).  Longer contexts have too many records for it (16 slots at 2,000
 // keys 19.4 against 15.5 us).
 constexpr int kJoinKeys = 1024, kJoinStep = 8;
 template <int HD, bool JOIN>

@@ -4,6 +4,8 @@
 // elements of every head, the rest copied; the inverse turns by -t, which is also
 // the gradient (the rotation is orthogonal).  One pass: each element is read and
 // written once, so large calls are bound by HBM and small ones by the launch.
+// 32,768 tokens of 28 heads of 128, all turned: 470 MB in 97 to 103 us (4.6 to 4.8 TB/s, the rate
+// of a large copy); a decode step of eight tokens 3.9 us.  Stores past the caches were slower (146 us).
 #include "qkv_device.h"
 #include "qkv_launch.h"
 #include "rope_device.h"
@@ -11,7 +13,9 @@
 namespace qkv {
 
 // A thread takes 16 elements (8 pairs, or 16 copied ones) of one token in HPT
-// heads, so that their cosines are formed once.
+// heads, so that their cosines are formed once: four, or one where that leaves few threads (eight
+// tokens of 20 heads: 3.9 us with one, 4.7 with four; 8,192 tokens of 20 turned heads of 128: 19.7 and
+// 17.8 us; the same from 2,000 to 4,000 tokens).
 template <int HPT>
 __global__ __launch_bounds__(256) void rope_kernel(RopeArgs p) {
   const long u = (long)blockIdx.x * 256 + threadIdx.x;
@@ -88,7 +92,7 @@ hipError_t launch_rope(RopeArgs a, bool wide, bool in_place, hipStream_t stream)
     a.units = (in_place ? a.rot : a.head_dim) / 16;
     const long threads = (long)a.n_tok * a.units;
     const unsigned gx = (unsigned)((threads + 255) / 256);
-    if (threads * heads <= 256 * 1024)   // few elements: a thread a head
+    if (threads * heads <= 256 * 1024)
       hipLaunchKernelGGL(rope_kernel<1>, dim3(gx, (unsigned)heads), dim3(256), 0, stream, a);
     else
       hipLaunchKernelGGL(rope_kernel<4>, dim3(gx, (unsigned)((heads + 3) / 4)), dim3(256), 0, stream, a);
