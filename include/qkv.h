@@ -549,7 +549,8 @@ int qkv_rope(const uint16_t* q, long q_stride, uint16_t* q_out, long q_out_strid
  * [n_slots + 1], not decreasing) of the row tensors, n_rows rows long, at
  * positions positions[s], positions[s] + 1, .. (device int32 [n_slots]).  A slot
  * may own none.  Rows past starts[n_slots] (a padded batch) are left alone; so
- * are rows of a slot past its first max_tok, and slots with a negative position.
+ * are rows of a slot past its first max_tok, and slots whose position lies outside
+ * [0, 2^30].
  * ------------------------------------------------------------------------- */
 
 /* Appends the rows' K and V (fp16, element strides between tokens, heads

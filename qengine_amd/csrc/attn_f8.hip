@@ -95,7 +95,7 @@ __device__ __forceinline__ Slot slot_of(const F8AttnArgs& p, int s) {
   x.t0 = min(max(p.starts[s], 0), (int)p.rows);
   x.n = min(min(max(p.starts[s + 1], x.t0), (int)p.rows) - x.t0, p.max_tok);
   x.pos0 = p.positions[s];
-  if (x.pos0 < 0 || x.pos0 > (1 << 30) || x.n < p.from_tok || x.n > p.to_tok) x.n = 0;
+  if (x.pos0 < 0 || x.pos0 > kMaxPosition || x.n < p.from_tok || x.n > p.to_tok) x.n = 0;
   return x;
 }
 
@@ -107,7 +107,7 @@ __device__ __forceinline__ Slot slot_at(const F8AttnArgs& p, int s) {
   x.t0 = min(max(starts[0], 0), (int)p.rows);
   x.n = min(min(max(starts[1], x.t0), (int)p.rows) - x.t0, p.max_tok);
   x.pos0 = positions[0];
-  if (x.pos0 < 0 || x.pos0 > (1 << 30) || x.n < p.from_tok || x.n > p.to_tok) x.n = 0;
+  if (x.pos0 < 0 || x.pos0 > kMaxPosition || x.n < p.from_tok || x.n > p.to_tok) x.n = 0;
   return x;
 }
 

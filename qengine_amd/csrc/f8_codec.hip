@@ -134,7 +134,9 @@ __global__ __launch_bounds__(THREADS, ROPE || THREADS == 1024 ? 4 : 8) void f8_a
     }
     const int s0 = p.starts[lo];
     // (not behind the last slot, nor past what the call covers of this one)
-    if (tok < s0 || tok >= p.starts[lo + 1] || tok - s0 >= p.max_tok || p.positions[lo] < 0) return;
+    if (tok < s0 || tok >= p.starts[lo + 1] || tok - s0 >= p.max_tok || p.positions[lo] < 0 ||
+        p.positions[lo] > kMaxPosition)
+      return;
     const int r = (int)(u - tok * per_tok), c = r % per_head, h0 = r / per_head * QH;
     const RopeRuns run = rope_runs(c, rope.rot, rope.layout);
     const uint16_t* in = p.q + tok * p.q_stride;
@@ -175,7 +177,7 @@ __global__ __launch_bounds__(THREADS, ROPE || THREADS == 1024 ? 4 : 8) void f8_a
   const int t0 = min(max(p.starts[s], 0), (int)p.rows);
   const int n = min(min(max(p.starts[s + 1], t0), (int)p.rows) - t0, p.max_tok);
   const int pos0 = p.positions[s];
-  if (pos0 < 0 || n <= 0) return;
+  if (pos0 < 0 || pos0 > kMaxPosition || n <= 0) return;
   const long b = (long)pos0 / p.block_tokens + j;
   const long first = max((long)pos0, b * p.block_tokens), end = min((long)pos0 + n, (b + 1) * p.block_tokens);
   if (first >= end || b >= p.max_blocks) return;

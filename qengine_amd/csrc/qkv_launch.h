@@ -161,6 +161,7 @@ struct F8AppendArgs {
 hipError_t launch_f8_append(F8AppendArgs a, hipStream_t stream);
 
 // Attention over the paged 8-bit cache (attn_f8.hip).
+constexpr int kMaxPosition = 1 << 30;   // of a paged 8-bit slot's first row
 struct F8AttnArgs {
   const uint16_t* q;         // [rows][num_q][head_dim]
   uint16_t* out;

@@ -84,6 +84,27 @@ def test_append_bad_pages_and_short_max_tok():
     _check_append(_append_case(rng, [3, 4], [30, 20], 16, 2, 128), max_tok=7)
 
 
+def test_slots_out_of_range():
+    """A slot whose position is negative or past 2^30 is left alone: cache, rotated queries and outputs."""
+    rng = np.random.default_rng(3)
+    tables, starts, pos, kp, ke, vp, ve, k, v = _append_case(rng, [3, 4, 5], [2, 3, 4], 16, 2, 128)
+    pos[0], pos[2] = -1, (1 << 30) + 1
+    g = [dev(x) for x in (kp, vp, ke, ve)]
+    q = torch.full((len(k), 8, 128), 1.0, dtype=torch.float16, device=DEV)
+    got = torch.full_like(q, 5.0)
+    kvcache.f8_append_kv_paged(dev(k), dev(v), *g, dev(tables), dev(starts), dev(pos), max_tok=4, q=q, q_out=got,
+                               rope=kvcache.rope_table(128, device=DEV))
+    assert (got[:2] == 5).all() and (got[5:] == 5).all() and (got[2:5] != 5).all()
+    own = set(tables[1].tolist())
+    for x, y in zip(g, (kp, vp, ke, ve)):
+        x = x.cpu().numpy()
+        assert all(np.array_equal(x[i], y[i]) for i in range(len(y)) if i not in own)
+    out = torch.full_like(q, 5.0)
+    ws = kvcache.attn_f8_paged_workspace(8, 2, 3, len(k), 4, 64, DEV, head_dim=128)
+    kvcache.attn_f8_paged(q, g[0], g[1], g[2], g[3], out, ws, dev(tables), dev(starts), dev(pos), max_tok=4, max_ctx=64, scale=0.1)
+    assert (out[:2] == 5).all() and (out[5:] == 5).all() and (out[2:5] != 5).any()
+
+
 @pytest.mark.parametrize("layout,rot", [("half", 64), ("interleaved", 256), ("half", 256), ("interleaved", 16)])
 @pytest.mark.parametrize("new", [[1, 1, 1, 1], [70, 0, 3, 20]])
 def test_rope_in_the_append(layout, rot, new):
