@@ -930,14 +930,13 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void f8_mid_kernel(F8AttnAr
 // wave the rows that it loaded itself, so only its own loads are waited for.  V is stored
 // by dim, four keys to 8 bytes, in the order that the scores' lanes hold them.  Pads
 // keep 16-byte reads of 16 lanes on distinct banks, at constant offsets of one address.
-// At head_dim 128 a tile is two halves of 32 keys, both scored before the weights, which are
-// formed under the products of those before them.  All waves convert ahead of their products: one of
-// each SIMD behind them was slower (1,112 against 1,070 us below), and so were two workgroups of
-// four waves a CU.
+// At head_dim 128 a tile is two halves of 32 keys, both scored before the weights.  All waves convert
+// ahead of a tile's scores: one of each SIMD behind its values was slower (1,112 against 1,070 us
+// below), and so were two workgroups of four waves a CU.
 // Bound by the matrix cores at 2,048 tokens over 32,000 keys, GQA 4, 4 KV heads of 256: 1,108 GFLOP in
-// 1,075 us, 1.03 PFLOP/s (a library product of fp16 matrices: 1.19; the conversion of tiles takes
+// 1,017 to 1,110 us (boxes differ), 1.0 to 1.09 PFLOP/s (a library product of fp16 matrices: 1.19; the conversion of tiles takes
 // about a quarter).  Short prompts pay 8 to 11 us a row tile before its first product and after its
-// last: six of 150 to 4,000 tokens, GQA 8, 128, window 1,500: 88 GFLOP in 157 us.
+// last: six of 150 to 4,000 tokens, GQA 8, 128, window 1,500: 88 GFLOP in 150 to 157 us.
 
 // A row tile's cost beside its key tiles, in tiles (measured to its first product and from its last:
 // 11 us against 2.1 a tile at head_dim 256, 8 against 2.6 at 128; and a part that begins inside a row
@@ -958,7 +957,10 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   constexpr int VPAD = KT == 32 ? 4 : 2;     // dims per 16-byte pad
   constexpr int KP = HD * 2 + 16;            // bytes of a key's row
   constexpr int KB = KT * KP, VB = HD * VP + HD / VPAD * 16;
-  __shared__ __align__(16) uint8_t tile_lds[2][KB + VB];
+  // (see `late` below)
+  constexpr bool SHIFT = HD == 128;
+  constexpr int VBUFS = SHIFT ? 3 : 2;
+  __shared__ __align__(16) uint8_t k_lds[2][KB], v_lds[VBUFS][VB];
   __shared__ __align__(16) uint8_t raw_lds[2][8192];
   __shared__ int lds[WAVES], upto[THREADS], found[2];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -1086,7 +1088,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       else if (w_at >= 64) load_pages(w_base + w_at);
     };
     const int vl = lane % (HD / 4), vq = lane / (HD / 4);   // value dims 4 vl .., keys 4 vq .. of the wave's
-    auto stage = [&](int v, int buf) {
+    auto stage = [&](int v, int k_buf, int v_buf) {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the codes are in LDS
       u4_t kr = *reinterpret_cast<const u4_t*>(raw_lds[0] + wave * 1024 + lane * 16);
       uint32_t vr[4];
@@ -1104,8 +1106,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       }
       // (an absent page's exponent is not one)
       const float ksc = pow2f((kx >> k_bit) & 255u), vsc = pow2f(loaded < 0 ? 127 : (vx >> v_bit) & 255u);
-      uint8_t* kb = tile_lds[buf];
-      uint8_t* vb = kb + KB;
+      uint8_t* kb = k_lds[k_buf];
+      uint8_t* vb = v_lds[v_buf];
       const int key = wave * WK + lane / LPR, slot = lane % LPR;
 #pragma unroll
       for (int e = 0; e < 2; e++)
@@ -1129,14 +1131,6 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                  __builtin_bit_cast(uint32_t, cvt2(w[1][j >> 1], vsc, j & 1))};
       }
     };
-    // the next tile into the other buffer, then the loads of the one after it
-    auto advance = [&](int v, int buf) {
-      if (v + 1 < v1) {
-        stage(v + 1, buf ^ 1);
-        if (v + 2 < v1) fetch(v + 2);
-      }
-    };
-
     seek(v0);
     fetch(v0);
     // (the queries and the page check arrive beside the first codes)
@@ -1165,16 +1159,54 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       for (int i = 0; i < HD / 16; i++) qf[i] = -qf[i];
     }
     __syncthreads();   // (the last segment's tiles are done with)
-    stage(v0, 0);
+    stage(v0, 0, 0);
     if (v0 + 1 < v1) fetch(v0 + 1);
     __syncthreads();
-    for (int v = v0; v < v1; v++) {
-      const int buf = (v - v0) & 1;
-      advance(v, buf);
-      if (v < v_hi && !(v >= v_sink && v < v_lo)) {   // (a wave none of whose rows sees the tile sits it out)
-        const uint8_t* kb = tile_lds[buf];
-        const uint8_t* vb = kb + KB;
+    // At head_dim 128, with twice the weights for the same products, one wave of each SIMD takes a tile's
+    // values in its turn and the other with the next tile, ahead of converting: one's products run
+    // beside the other's conversions and weights (a prompt of 8,000 tokens, GQA 8, 585 -> 570 us; at 256
+    // slower, 1,120 against 1,068 us for 2,048 tokens over 32,000 keys).
+    const bool late = SHIFT && wave >= 4;
+    bool held = false;
+    h8_t w[2 * KH];
+    constexpr int ND = HD / 32, NV = 2 * KH * ND;   // 32-dim blocks; of each 16 keys in turn
+    auto products = [&](int v_buf) {
+      const uint8_t* vat = v_lds[v_buf] + c * VP + c / VPAD * 16 + hh * 16;
+      auto v_operand = [&](int i) {
+        return *reinterpret_cast<const h8_t*>(vat + i % ND * (32 * VP + 32 / VPAD * 16) + i / ND * 32);
+      };
+      if (SHIFT) __builtin_amdgcn_s_setprio(1);
+      h8_t va[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) va[i] = v_operand(i);
+#pragma unroll
+      for (int i = 0; i < NV; i++) {
+        acc[i % ND] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va[i % 4], w[i / ND], acc[i % ND], 0, 0, 0);
+        if (i + 4 < NV) va[i % 4] = v_operand(i + 4);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+      for (int i = 0; i < NV - 4; i++) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
+      if (SHIFT) __builtin_amdgcn_s_setprio(0);
+    };
+    int v_buf = 0;
+    for (int v = v0;; v++) {
+      const int k_buf = (v - v0) & 1, v_next = v_buf == VBUFS - 1 ? 0 : v_buf + 1;
+      if (late && held) products(v_buf == 0 ? VBUFS - 1 : v_buf - 1);
+      if (v == v1) break;
+      if (v + 1 < v1) {
+        stage(v + 1, k_buf ^ 1, v_next);
+        if (v + 2 < v1) fetch(v + 2);
+      }
+      held = v < v_hi && !(v >= v_sink && v < v_lo);   // (a wave none of whose rows sees the tile sits it out)
+      if (held) {
+        const uint8_t* kb = k_lds[k_buf];
         // scores of the tile's halves in turn (two chains of products at head_dim 128)
+        if (SHIFT) __builtin_amdgcn_s_setprio(1);
         const uint8_t* krow = kb + c * KP + hh * 16;
         auto k_operand = [&](int i) { return *reinterpret_cast<const h8_t*>(krow + i % KH * (32 * KP) + i / KH * 32); };
         constexpr int NK = KH * HD / 16;
@@ -1194,11 +1226,6 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
           __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
         }
         __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
-        const uint8_t* vat = vb + c * VP + c / VPAD * 16 + hh * 16;
-        constexpr int ND = HD / 32, NV = 2 * KH * ND;   // 32-dim blocks; of each 16 keys in turn
-        auto v_operand = [&](int i) {
-          return *reinterpret_cast<const h8_t*>(vat + i % ND * (32 * VP + 32 / VPAD * 16) + i / ND * 32);
-        };
 #pragma unroll
         for (int kh = 0; kh < KH; kh++) {
           const int y = v * KH + kh, k0 = (y < rt.n_sink * KH ? y : y + y_off) * 32;
@@ -1211,10 +1238,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
             }
           }
         }
-        // the first values' reads go ahead of the weights (and behind the masks, which need the registers)
-        h8_t va[4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) va[i] = v_operand(i);
+        if (SHIFT) __builtin_amdgcn_s_setprio(0);
         float t = sd[0][0];
 #pragma unroll
         for (int x = 1; x < 16 * KH; x++) t = fmaxf(t, sd[x / 16][x % 16]);
@@ -1236,25 +1260,11 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
           ls = add8(w, ls);
           return w;
         };
-        h8_t w[2 * KH];
-        w[0] = weights(0);
-        __builtin_amdgcn_sched_barrier(0);
-        // the other weights are formed under the products of those before them
 #pragma unroll
-        for (int g = 1; g < 2 * KH; g++) w[g] = weights(g);
-#pragma unroll
-        for (int i = 0; i < NV; i++) {
-          acc[i % ND] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va[i % 4], w[i / ND], acc[i % ND], 0, 0, 0);
-          if (i + 4 < NV) va[i % 4] = v_operand(i + 4);
-        }
-#pragma unroll
-        for (int i = 0; i < NV - 4; i++) {
-          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-          if (i < NV - ND - 1) __builtin_amdgcn_sched_group_barrier(0x002, HD == 256 ? 4 : 6, 0);
-        }
-        __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
+        for (int g = 0; g < 2 * KH; g++) w[g] = weights(g);
+        if (!late) products(v_buf);
       }
+      v_buf = v_next;
       __syncthreads();
     }
 
