@@ -298,10 +298,10 @@ struct SlotLine {
     for (int b = 0;; b += 64) {
       load(b);
       const int n = __builtin_amdgcn_readlane(inc, 63);
-      if (u < n) break;
+      if (u < n || b + 64 >= p.n_slots) break;
       u -= n;
     }
-    const int e = __builtin_ctzll(__builtin_amdgcn_ballot_w64(inc > u));
+    const int e = min(63, (int)__builtin_ctzll(__builtin_amdgcn_ballot_w64(inc > u) | 1ull << 63));
     at = u - (__builtin_amdgcn_readlane(inc, e) - __builtin_amdgcn_readlane(units, e));
     return e;
   }
@@ -311,7 +311,10 @@ struct SlotLine {
     uint64_t m = __builtin_amdgcn_ballot_w64(units > 0) & (e < 63 ? ~0ull << (e + 1) : 0ull);
     while (m == 0) {
       const int b = base + 64 < p.n_slots ? base + 64 : 0;
-      if (b == 0) wrapped = true;
+      if (b == 0) {
+        if (wrapped) return 0;   // (none: see `rows` below)
+        wrapped = true;
+      }
       load(b);
       m = __builtin_amdgcn_ballot_w64(units > 0);
     }
@@ -392,6 +395,7 @@ __global__ __launch_bounds__(256, 2) void f8_few_kernel(F8AttnArgs p) {
     const int units = (rt.tiles + PER - 1) / PER;
     const int n_u = min(units - at, u_end - u);
     const int rows = sl.n * gqa;
+    if (rows <= 0 || n_u <= 0) return;   // (starts or positions that change under the call: no loop without end)
     const int v_end = min((at + n_u) * PER, rt.tiles);
     const const_i32* table = (const const_i32*)(p.tables + (long)(line.base + e) * p.max_blocks);
     // for the merge: the parts that hold the tile, and its first record
@@ -717,6 +721,7 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void f8_mid_kernel(F8AttnAr
     const int units = (rt.tiles + PER - 1) / PER;
     const int n_u = min(units - at, u_end - u);
     const int rows = sl.n * gqa;
+    if (rows <= 0 || n_u <= 0) return;   // (starts or positions that change under the call: no loop without end)
     // a wave without rows loads nothing (the others wait for nobody)
     const int v_end = 32 * rg < rows ? min((at + n_u) * PER, rt.tiles) : 0;
     const const_i32* table = (const const_i32*)(p.tables + (long)(line.base + e) * p.max_blocks);
@@ -995,7 +1000,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       while (true) {
         if (t >= p.n_slots) {
           t = 0;
-          h++;
+          if (++h >= p.num_kv) return;   // (starts or positions that change under the call)
         }
         any = __builtin_amdgcn_ballot_w64(t + lane < p.n_slots && slot_of(p, min(t + lane, p.n_slots - 1)).n > 0);
         if (any) break;
@@ -1006,6 +1011,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     }
     const RowTile rt = row_tile<ROWS, KT>(p, sl, rti, gqa);
     const int n_u = min(LEAD + rt.tiles - at.at, u_end - u);
+    if (n_u <= 0) return;
     const int v0 = max(at.at - LEAD, 0), v1 = at.at + n_u - LEAD;   // (v1 <= v0: the next part's)
     // where the part begins, for the merge: row tile (-1: not past its first key tile), head, tile,
     // tiles
