@@ -545,6 +545,8 @@ int qkv_rope(const uint16_t* q, long q_stride, uint16_t* q_out, long q_out_strid
  * [n_pages][num_kv]: value = code * 2^(exp - 127).  block_tokens: a multiple of
  * 16, and a page below 2 GiB; head_dim 128 or 256.  Key p of slot s is row
  * p % block_tokens of page block_tables[s * max_blocks + p / block_tokens].
+ * Exponents are read by whole aligned 4-byte words: up to 3 bytes before and past
+ * the array's own, which must be there to read (any allocation's are).
  * A batch is ragged: slot s owns rows starts[s] .. starts[s+1]-1 (device int32
  * [n_slots + 1], not decreasing) of the row tensors, n_rows rows long, at
  * positions positions[s], positions[s] + 1, .. (device int32 [n_slots]).  A slot
