@@ -991,6 +991,16 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const int kt_div = KT / p.block_tokens, kt_mod = KT % p.block_tokens;
   const int entries = p.n_slots * p.slot_tiles;
 
+  auto next = [&](int n_u) {
+    first_seg = false;
+    u += n_u;
+    at.at = 0;
+    at.entry++;
+    if (at.entry >= entries) {
+      at.entry = 0;
+      h++;
+    }
+  };
   while (u < u_end) {
     const int s = at.entry / p.slot_tiles, rti = at.entry - s * p.slot_tiles;
     const Slot sl = slot_at(p, s);
@@ -1018,7 +1028,10 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     if (first_seg && tid == 0)
       *reinterpret_cast<int4*>(p.cuts + 4 * grp) = make_int4(v0 > 0 ? at.entry : -1, h, v0, rt.tiles);
     const bool complete = v0 == 0 && v1 == rt.tiles;
-    if (v1 > v0) {
+    if (v1 <= v0) {
+      next(n_u);
+      continue;
+    }
     const int rows = sl.n * gqa;
     const int row_w = rti * ROWS + wave * 32;      // this wave's first row
     const int row = min(row_w + c, rows - 1), tok = row / gqa;
@@ -1298,15 +1311,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         if (hh == 0) *reinterpret_cast<f2_t*>(p.rec_ml + (rec * ROWS + 32 * wave + c) * 2) = f2_t{rec_max(mx, ls), ls};
       }
     }
-    }
-    first_seg = false;
-    u += n_u;
-    at.at = 0;
-    at.entry++;
-    if (at.entry >= entries) {
-      at.entry = 0;
-      h++;
-    }
+    next(n_u);
   }
 }
 
