@@ -512,3 +512,48 @@ def test_captured_steps():
         b.step()
         for p, q in ((a.out, b.out), (a.kp, b.kp), (a.ve, b.ve), (a.tables, b.tables), (a.refs, b.refs), (a.pos, b.pos)):
             assert torch.equal(p, q), step
+
+
+def test_captured_prompts_and_two_streams():
+    """A captured batch of prompts and single tokens (two launches and both merges), replayed with new queries and
+    eager calls on the same workspace between; and the same batches on two streams at once."""
+    cases = [_attn_case(41, [3000, 0, 900, 700], [1, 300, 1, 2], 16, 2, 4, 128), _attn_case(42, [0, 2500], [500, 1], 64, 2, 4, 256)]
+    calls = []
+    for case in cases:
+        q, kp, vp, ke, ve, tables, starts, pos = map(dev, case)
+        mt, rows = int(np.diff(case[6]).max()), q.shape[0]
+        ws = [kvcache.attn_f8_paged_workspace(8, 2, len(pos), rows, mt, 1 << 17, DEV, head_dim=q.shape[2]) for _ in range(2)]
+
+        def call(out, w, q=q, rest=(kp, vp, ke, ve), idx=(tables, starts, pos), mt=mt):
+            kvcache.attn_f8_paged(q, *rest, out, w, *idx, max_tok=mt, max_ctx=1 << 17, scale=0.09)
+        calls.append((q, ws, call))
+    for q, ws, call in calls:
+        out, want = torch.full_like(q, 9.0), torch.full_like(q, 9.0)
+        call(out, ws[0])
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            call(out, ws[0])
+        for step in range(5):
+            q.copy_(torch.randn(q.shape, device=DEV).half())
+            out.fill_(9.0)
+            g.replay()
+            call(want, ws[0] if step % 2 else ws[1])
+            assert torch.equal(out, want), step
+    # at once: each stream with its own workspace
+    want = []
+    for q, ws, call in calls:
+        want.append(torch.full_like(q, 9.0))
+        call(want[-1], ws[0])
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[torch.full_like(q, 9.0) for q, _, _ in calls] for _ in streams]
+    torch.cuda.synchronize()
+    for i, s in enumerate(streams):
+        with torch.cuda.stream(s):
+            for _ in range(4):
+                for out, (q, ws, call) in zip(got[i], calls):
+                    call(out, ws[i])
+    torch.cuda.synchronize()
+    for outs in got:
+        for out, w in zip(outs, want):
+            assert torch.equal(out, w)
