@@ -86,6 +86,24 @@ __device__ __forceinline__ BlockRow block_row(const F8AttnArgs& p, int key) {
   return {(int)(more ? q + 1 : q), (int)(more ? r - (uint32_t)p.block_tokens : r)};
 }
 
+// Token of a (token, head) row x >= 0 (the same way; the compiler's division is five times as long)
+__device__ __forceinline__ int token_of(const F8AttnArgs& p, int x) {
+  const uint32_t q = __umulhi((uint32_t)x, p.gqa_magic), r = (uint32_t)x - q * (uint32_t)p.gqa;
+  return (int)(r >= (uint32_t)p.gqa ? q + 1 : q);
+}
+
+// Inclusive sums over the lanes, none above `top`
+__device__ __forceinline__ int scan64(int v, int top) {
+  auto add = [&](int o) { v = min(v + o, top); };
+  add(__builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false));   // within rows of 16, from 1, 2, 4, 8 lanes below
+  add(__builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false));
+  add(__builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false));
+  add(__builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false));
+  add(__builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false));   // the row before, the half before
+  add(__builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false));
+  return v;
+}
+
 // A slot's tokens: rows t0 .. t0+n-1 of q at positions pos0 .. (n = 0: none, or not of this launch)
 struct Slot {
   int t0, n, pos0;
@@ -123,8 +141,8 @@ template <int ROWS, int KT>
 __device__ __forceinline__ RowTile row_tile(const F8AttnArgs& p, const Slot& x, int i, int gqa) {
   RowTile r;
   const int rows = x.n * gqa;
-  r.pos_lo = x.pos0 + i * ROWS / gqa;
-  r.pos_hi = x.pos0 + (min(rows, (i + 1) * ROWS) - 1) / gqa;
+  r.pos_lo = x.pos0 + token_of(p, i * ROWS);
+  r.pos_hi = x.pos0 + token_of(p, min(rows, (i + 1) * ROWS) - 1);
   r.end = min(r.pos_hi + 1, p.max_ctx);
   r.w0 = p.window > 0 ? max(0, r.pos_lo - p.window + 1) / KT : 0;
   r.n_sink = p.window > 0 ? min((p.sink + KT - 1) / KT, r.w0) : 0;
@@ -145,11 +163,7 @@ __device__ __forceinline__ int add_units(int a, int b) { return min(a + b, kLine
 template <int THREADS>
 __device__ __forceinline__ int block_scan(int v, int* lds, int& sum) {   // inclusive
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int o = __shfl_up(v, d);
-    if (lane >= d) v = add_units(v, o);
-  }
+  v = scan64(v, kLineMax);
   __syncthreads();
   if (lane == 63) lds[w] = v;
   __syncthreads();
@@ -277,12 +291,7 @@ struct SlotLine {
     base = b;
     mine = b + lane < p.n_slots ? slot_of(p, b + lane) : Slot{0, 0, 0};
     units = mine.n > 0 ? (row_tile<ROWS, KT>(p, mine, 0, gqa).tiles + PER - 1) / PER : 0;
-    inc = units;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int o = __shfl_up(inc, d);
-      if (lane >= d) inc += o;
-    }
+    inc = scan64(units, 0x7fffffff);
   }
   // units of all slots
   __device__ __forceinline__ int total() {
@@ -374,7 +383,7 @@ __global__ __launch_bounds__(256, 2) void f8_few_kernel(F8AttnArgs p) {
   __shared__ float ml[W][ROWS][2];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int m = lane & 15, g = lane >> 4;
-  const int gqa = p.num_q / p.num_kv;
+  const int gqa = p.gqa;
 
   SlotLine<ROWS, KT, PER> line(p, gqa);
   const int total = line.total();
@@ -450,7 +459,7 @@ __global__ __launch_bounds__(256, 2) void f8_few_kernel(F8AttnArgs p) {
 
     // ---- queries: row m, dims 64 i + 16 g + 8 half ..
     h8_t qf[KW][2];
-    const int rc = min(m, rows - 1), tok = rc / gqa;
+    const int rc = min(m, rows - 1), tok = token_of(p, rc);
     const int pos_r = sl.pos0 + tok;
     {
       const uint16_t* src = p.q + ((long)(sl.t0 + tok) * p.num_q + h * gqa + (rc - tok * gqa)) * HD + 16 * g;
@@ -582,7 +591,7 @@ __global__ __launch_bounds__(256, 2) void f8_few_kernel(F8AttnArgs p) {
       }
       if (complete) {
         o *= L > 0.f ? 1.f / L : 0.f;
-        const int t = r / gqa;
+        const int t = token_of(p, r);
         *reinterpret_cast<u2_t*>(p.out + ((long)(sl.t0 + t) * p.num_q + h * gqa + (r - t * gqa)) * HD + d) =
             u2_t{f2h(o[0]) | (f2h(o[1]) << 16), f2h(o[2]) | (f2h(o[3]) << 16)};
       } else {
@@ -650,7 +659,7 @@ __global__ __launch_bounds__(256, 2) void f8_few_kernel(F8AttnArgs p) {
                 }
             }
             o *= L > 0.f ? 1.f / L : 0.f;
-            const int t = r / gqa;
+            const int t = token_of(p, r);
             *reinterpret_cast<u2_t*>(p.out + ((long)(sl.t0 + t) * p.num_q + h * gqa + (r - t * gqa)) * HD + d) =
                 u2_t{f2h(o[0]) | (f2h(o[1]) << 16), f2h(o[2]) | (f2h(o[3]) << 16)};
           }
@@ -698,7 +707,7 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void f8_mid_kernel(F8AttnAr
   __shared__ float ml[KG][ROWS][2];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 31, hh = lane >> 5, rg = wave % RG, kg = wave / RG;
-  const int gqa = p.num_q / p.num_kv;
+  const int gqa = p.gqa;
 
   SlotLine<ROWS, KT, PER> line(p, gqa);
   const int total = line.total();
@@ -762,7 +771,7 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void f8_mid_kernel(F8AttnAr
     }
     // ---- queries: row c of the wave, dims 32 i + 16 hh + 8 x ..
     h8_t qf[KW][2];
-    const int rc = min(32 * rg + c, rows - 1), tok = rc / gqa;
+    const int rc = min(32 * rg + c, rows - 1), tok = token_of(p, rc);
     const int pos_r = sl.pos0 + tok;
     {
       const uint16_t* src = p.q + ((long)(sl.t0 + tok) * p.num_q + h * gqa + (rc - tok * gqa)) * HD + 16 * hh;
@@ -907,7 +916,7 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void f8_mid_kernel(F8AttnAr
       }
       if (complete) {
         o *= L > 0.f ? 1.f / L : 0.f;
-        const int t = r / gqa;
+        const int t = token_of(p, r);
         *reinterpret_cast<u2_t*>(p.out + ((long)(sl.t0 + t) * p.num_q + h * gqa + (r - t * gqa)) * HD + d) =
             u2_t{f2h(o[0]) | (f2h(o[1]) << 16), f2h(o[2]) | (f2h(o[3]) << 16)};
       } else {
@@ -970,7 +979,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   __shared__ int lds[WAVES], upto[THREADS], found[2];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 31, hh = lane >> 5;
-  const int gqa = p.num_q / p.num_kv;
+  const int gqa = p.gqa;
 
   // (the same in every lane: said to the compiler, what follows stays out of the vector registers)
   RowLine<ROWS, KT, LEAD, THREADS> line{p, gqa, lds, upto};
@@ -1034,9 +1043,9 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     }
     const int rows = sl.n * gqa;
     const int row_w = rti * ROWS + wave * 32;      // this wave's first row
-    const int row = min(row_w + c, rows - 1), tok = row / gqa;
+    const int row = min(row_w + c, rows - 1), tok = token_of(p, row);
     const int pos = sl.pos0 + tok;
-    const int pos_lo = sl.pos0 + min(row_w, rows - 1) / gqa, pos_hi = sl.pos0 + min(row_w + 31, rows - 1) / gqa;
+    const int pos_lo = sl.pos0 + token_of(p, min(row_w, rows - 1)), pos_hi = sl.pos0 + token_of(p, min(row_w + 31, rows - 1));
     const bool live = row_w < rows;
     const long out_row = ((long)(sl.t0 + tok) * p.num_q + h * gqa + (row - tok * gqa)) * HD;
 
@@ -1335,7 +1344,7 @@ __global__ __launch_bounds__(256) void f8_cut_merge_kernel(F8AttnArgs p) {
   const int n = parts.of(x1 + tiles - 1) - grp + 2;
   const long r0 = 2 * (grp - 1) + (before >= x0 ? 0 : 1);
   auto rec_of = [&](int i) { return i == 0 ? r0 : 2l * (grp - 1 + i); };
-  const int s = entry / p.slot_tiles, gqa = p.num_q / p.num_kv;
+  const int s = entry / p.slot_tiles, gqa = p.gqa;
   const Slot sl = slot_of(p, s);
   const int r = (entry - s * p.slot_tiles) * ROWS + 32 * rw + c;
   if (r >= sl.n * gqa) return;
@@ -1359,7 +1368,7 @@ __global__ __launch_bounds__(256) void f8_cut_merge_kernel(F8AttnArgs p) {
     for (int a = 0; a < 4; a++) o[a] = o[a] * f + x[a] * w;
   }
   const float inv = L > 0.f ? 1.f / L : 0.f;
-  const int t = r / gqa;
+  const int t = token_of(p, r);
   uint16_t* dst = p.out + ((long)(sl.t0 + t) * p.num_q + h * gqa + (r - t * gqa)) * HD + 32 * d + 4 * hh;
 #pragma unroll
   for (int a = 0; a < 4; a++) {
@@ -1378,7 +1387,7 @@ __global__ __launch_bounds__(256) void f8_merge_kernel(F8AttnArgs p) {
   constexpr int E = HD / 64;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int tile = blockIdx.x / p.rec_rows, row = blockIdx.x - tile * p.rec_rows;
-  const int s = tile / p.num_kv, h = tile - s * p.num_kv, gqa = p.num_q / p.num_kv;
+  const int s = tile / p.num_kv, h = tile - s * p.num_kv, gqa = p.gqa;
   const int2 desc = p.desc[tile];
   const Slot sl = slot_of(p, s);
   const int n = desc.x, r0 = desc.y;
@@ -1431,7 +1440,7 @@ __global__ __launch_bounds__(256) void f8_merge_kernel(F8AttnArgs p) {
 #pragma unroll
     for (int e = 0; e < E; e++) o[e] += part[w][lane][e];
   const float inv = L > 0.f ? 1.f / L : 0.f;
-  const int t = row / gqa;
+  const int t = token_of(p, row);
   uint16_t* dst = p.out + ((long)(sl.t0 + t) * p.num_q + h * gqa + (row - t * gqa)) * HD + lane * E;
   if constexpr (E == 4)
     *reinterpret_cast<u2_t*>(dst) = u2_t{f2h(o[0] * inv) | (f2h(o[1] * inv) << 16), f2h(o[2] * inv) | (f2h(o[3] * inv) << 16)};

@@ -276,7 +276,9 @@ int qkv_attn_f8_paged(const uint16_t* q, const uint8_t* k_pool, const uint8_t* v
   a.n_pages = n_pages;
   a.window = window_tok;
   a.sink = sink_tok < max_ctx ? sink_tok : max_ctx;   // (rounded up to tiles in 32 bits)
+  a.gqa = num_q / num_kv;
   a.bt_magic = (uint32_t)((1ull << 32) / (uint64_t)block_tokens);
+  a.gqa_magic = (uint32_t)std::min<uint64_t>((1ull << 32) / (uint64_t)a.gqa, 0xffffffffull);
   a.scale_log2 = scale * 1.4426950408889634f;
   auto launch = [&](const qkv::F8AttnPlan& x, int from, int to) {
     a.rec_ml = reinterpret_cast<float*>(ws + x.ml_off);

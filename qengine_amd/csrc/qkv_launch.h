@@ -184,7 +184,9 @@ struct F8AttnArgs {
   int slot_tiles;            // row tiles of a slot with max_tok tokens
   int rec_rows;              // rows of a record
   int groups;                // workgroups
+  int gqa;                   // num_q / num_kv
   uint32_t bt_magic;         // floor(2^32 / block_tokens)
+  uint32_t gqa_magic;        // the same of gqa, below 2^32
   float scale_log2;
 };
 // Workspaces begin with these counts, whatever the call's numbers, so that calls of different
