@@ -367,11 +367,11 @@ __device__ __forceinline__ Tile tile_at(const F8AttnArgs& p, const const_i32* ta
 // kernel that only reads reaches 6.4), 5 us of merge after it; 32 slots of 500 to 32,768 keys in
 // 16-row pages of 128, 358 MB in 64 to 67 us.  Parts for 256, 768 or 1,024 workgroups were slower than
 // for 512 (two a CU).
-// JOIN: contexts of up to kJoinKeys keys, whose records the last workgroup of a tile joins in this
-// launch: there latency is all (a call at 700 keys 10.9 us, with the merge's launch 12.6; by one
-// workgroup of eight waves a KV head 13.4).  Longer contexts have too many records for it (16 slots at 2,000
-// keys 19.4 against 15.5 us).
+// JOIN: short contexts, whose records the last workgroup of a tile joins in this launch: there latency
+// is all (a call at 700 keys 9.7 us, with the merge's launch 12.9; by one workgroup of eight waves a
+// KV head 13.4).
 constexpr int kJoinKeys = 1024, kJoinStep = 8;
+constexpr int kCoherent = 1 | 16;   // sc0 | sc1: where every XCD sees it, as device-wide atomics go
 template <int HD, bool JOIN>
 __global__ __launch_bounds__(256, 2) void f8_few_kernel(F8AttnArgs p) {
   constexpr int KT = 32, ROWS = 16, W = 4, PER = 4, THREADS = 64 * W;
@@ -384,6 +384,10 @@ __global__ __launch_bounds__(256, 2) void f8_few_kernel(F8AttnArgs p) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int m = lane & 15, g = lane >> 4;
   const int gqa = p.gqa;
+
+  const int recs = JOIN ? 2 * p.groups * p.rec_rows : 0;
+  const __amdgpu_buffer_rsrc_t rec_ml = __builtin_amdgcn_make_buffer_rsrc(p.rec_ml, 0, recs * 8, kBufferRsrcWord3);
+  const __amdgpu_buffer_rsrc_t rec_o = __builtin_amdgcn_make_buffer_rsrc(p.rec_o, 0, recs * HD * 4, kBufferRsrcWord3);
 
   SlotLine<ROWS, KT, PER> line(p, gqa);
   const int total = line.total();
@@ -595,18 +599,13 @@ __global__ __launch_bounds__(256, 2) void f8_few_kernel(F8AttnArgs p) {
         *reinterpret_cast<u2_t*>(p.out + ((long)(sl.t0 + t) * p.num_q + h * gqa + (r - t * gqa)) * HD + d) =
             u2_t{f2h(o[0]) | (f2h(o[1]) << 16), f2h(o[2]) | (f2h(o[3]) << 16)};
       } else {
-        float* ro = p.rec_o + ((long)rec * p.rec_rows + r) * HD + d;
-        float* rm = p.rec_ml + ((long)rec * p.rec_rows + r) * 2;
+        const int at_r = rec * p.rec_rows + r;   // (at most 2 x 512 records of 16 rows)
         if constexpr (JOIN) {   // (to where every XCD sees it)
-#pragma unroll
-          for (int i = 0; i < 4; i++) __hip_atomic_store(ro + i, o[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-          if (d == 0) {
-            __hip_atomic_store(rm, rec_max(M, L), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            __hip_atomic_store(rm + 1, L, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-          }
+          __builtin_amdgcn_raw_buffer_store_b128(o, rec_o, (uint32_t)(at_r * HD + d) * 4, 0, kCoherent);
+          if (d == 0) __builtin_amdgcn_raw_buffer_store_b64(f2_t{rec_max(M, L), L}, rec_ml, (uint32_t)at_r * 8, 0, kCoherent);
         } else {
-          *reinterpret_cast<f4_t*>(ro) = o;
-          if (d == 0) *reinterpret_cast<f2_t*>(rm) = f2_t{rec_max(M, L), L};
+          *reinterpret_cast<f4_t*>(p.rec_o + (long)at_r * HD + d) = o;
+          if (d == 0) *reinterpret_cast<f2_t*>(p.rec_ml + (long)at_r * 2) = f2_t{rec_max(M, L), L};
         }
       }
     }
@@ -623,46 +622,66 @@ __global__ __launch_bounds__(256, 2) void f8_few_kernel(F8AttnArgs p) {
         __syncthreads();
         if (order == n - 1) {
           const int r0 = 2 * g0 + (parts.begin(g0) == x0 ? 0 : 1);
-          for (int x = tid * 4; x < rows * HD; x += THREADS * 4) {
-            const int r = x / HD, d = x - r * HD;
-            float M = -INFINITY, L = 0.f;
-            f4_t o = {0.f, 0.f, 0.f, 0.f};
-            for (int i0 = 0; i0 < n; i0 += kJoinStep) {   // (a step's loads are all under way at once)
-              float mr[kJoinStep], lr[kJoinStep];
-              f4_t ov[kJoinStep];
+          // (a step's loads of all records and elements are under way at once: one element a thread in
+          // a decode step, else two)
+          auto join = [&](auto wide) {
+            constexpr int kJoinWide = decltype(wide)::value;
+            for (int x0 = tid * 4; x0 < rows * HD; x0 += kJoinWide * THREADS * 4) {
+              float M[kJoinWide], L[kJoinWide];
+              f4_t o[kJoinWide];
 #pragma unroll
-              for (int i = 0; i < kJoinStep; i++) {
-                const int k = min(i0 + i, n - 1);
-                const long at_r = (long)(k == 0 ? r0 : 2 * (g0 + k)) * p.rec_rows + r;
-                mr[i] = __hip_atomic_load(p.rec_ml + at_r * 2, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                lr[i] = __hip_atomic_load(p.rec_ml + at_r * 2 + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                if (i0 + i >= n) lr[i] = 0.f;
-#pragma unroll
-                for (int q = 0; q < 4; q++)
-                  ov[i][q] = __hip_atomic_load(p.rec_o + at_r * HD + d + q, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+              for (int b = 0; b < kJoinWide; b++) {
+                M[b] = -INFINITY;
+                L[b] = 0.f;
+                o[b] = f4_t{0.f, 0.f, 0.f, 0.f};
               }
-              float mn = M;
+              for (int i0 = 0; i0 < n; i0 += kJoinStep) {
+                f2_t ml_r[kJoinWide][kJoinStep];
+                f4_t ov[kJoinWide][kJoinStep];
 #pragma unroll
-              for (int i = 0; i < kJoinStep; i++)
-                if (lr[i] != 0.f) mn = fmaxf(mn, mr[i]);
-              if (mn == -INFINITY) continue;   // no key so far
-              const float f = __builtin_amdgcn_exp2f(M - mn);
-              M = mn;
-              L *= f;
-              o *= f;
+                for (int b = 0; b < kJoinWide; b++)
 #pragma unroll
-              for (int i = 0; i < kJoinStep; i++)
-                if (lr[i] != 0.f) {
-                  const float w = __builtin_amdgcn_exp2f(mr[i] - M);
-                  L += w * lr[i];
-                  o += w * ov[i];
+                  for (int i = 0; i < kJoinStep; i++) {
+                    const int x = min(x0 + b * THREADS * 4, rows * HD - 4), k = min(i0 + i, n - 1);
+                    const int at_r = (k == 0 ? r0 : 2 * (g0 + k)) * p.rec_rows + x / HD;
+                    ml_r[b][i] = __builtin_amdgcn_raw_buffer_load_b64(rec_ml, (uint32_t)at_r * 8, 0, kCoherent);
+                    ov[b][i] = __builtin_amdgcn_raw_buffer_load_b128(rec_o, (uint32_t)(at_r * HD + x % HD) * 4, 0, kCoherent);
+                  }
+#pragma unroll
+                for (int b = 0; b < kJoinWide; b++) {
+                  float mn = M[b];
+#pragma unroll
+                  for (int i = 0; i < kJoinStep; i++) {
+                    if (i0 + i >= n) ml_r[b][i][1] = 0.f;
+                    if (ml_r[b][i][1] != 0.f) mn = fmaxf(mn, ml_r[b][i][0]);
+                  }
+                  if (mn == -INFINITY) continue;   // no key so far
+                  const float f = __builtin_amdgcn_exp2f(M[b] - mn);
+                  M[b] = mn;
+                  L[b] *= f;
+                  o[b] *= f;
+#pragma unroll
+                  for (int i = 0; i < kJoinStep; i++)
+                    if (ml_r[b][i][1] != 0.f) {
+                      const float w = __builtin_amdgcn_exp2f(ml_r[b][i][0] - mn);
+                      L[b] += w * ml_r[b][i][1];
+                      o[b] += w * ov[b][i];
+                    }
                 }
+              }
+#pragma unroll
+              for (int b = 0; b < kJoinWide; b++) {
+                const int x = x0 + b * THREADS * 4;
+                if (x >= rows * HD) break;
+                const int r = x / HD, d = x - r * HD, t = token_of(p, r);
+                const f4_t y = o[b] * (L[b] > 0.f ? 1.f / L[b] : 0.f);
+                *reinterpret_cast<u2_t*>(p.out + ((long)(sl.t0 + t) * p.num_q + h * gqa + (r - t * gqa)) * HD + d) =
+                    u2_t{f2h(y[0]) | (f2h(y[1]) << 16), f2h(y[2]) | (f2h(y[3]) << 16)};
+              }
             }
-            o *= L > 0.f ? 1.f / L : 0.f;
-            const int t = token_of(p, r);
-            *reinterpret_cast<u2_t*>(p.out + ((long)(sl.t0 + t) * p.num_q + h * gqa + (r - t * gqa)) * HD + d) =
-                u2_t{f2h(o[0]) | (f2h(o[1]) << 16), f2h(o[2]) | (f2h(o[3]) << 16)};
-          }
+          };
+          if (rows * HD <= THREADS * 4) join(std::integral_constant<int, 1>{});
+          else join(std::integral_constant<int, 2>{});
           if (tid == 0) __hip_atomic_store(count, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
       }
@@ -1469,9 +1488,13 @@ F8AttnPlan f8_attn_plan(int num_q, int num_kv, int head_dim, int n_slots, long q
   } else {
     x.slot_tiles = 1;
     x.rec_rows = (int)rows;
-    // Short contexts: few records, joined in the launch (a second one costs as much as the
-    // attention); many records are merged by one, whose workgroups share them.
-    x.join = x.row_tiles == 1 && max_ctx <= kJoinKeys && n_slots <= 64 && n_slots * num_kv <= kJoinCounts;
+    // Short contexts: few records, joined in the launch where one workgroup takes no longer for them than
+    // a second launch: up to 1,024 keys (16 slots of 16 rows of 256: 20.3 against 20.1 us, 16 rows
+    // of 128 14.4 and 17.4), for rows of up to 2,048 elements up to 2,048 keys (one token of 2,000 keys
+    // 13.1 and 16.3 us, two in eight slots 17.5 and 18.7, but 16 rows of 256 24.2 and 19.8; four slots
+    // of 4,000 keys 19.3 and 17.4).
+    const long row_elems = rows * head_dim;
+    x.join = x.row_tiles == 1 && max_ctx <= (row_elems <= 2048 ? 2 : 1) * kJoinKeys && n_slots <= 64 && n_slots * num_kv <= kJoinCounts;
     const int unit_keys = x.row_tiles == 4 ? 64 : 128;
     units = (long)n_slots * num_kv * ((max_ctx + unit_keys - 1) / unit_keys);
     x.groups = (int)std::min<long>(units, x.row_tiles == 1 || head_dim == 128 ? 512 : 256);   // (what the CUs hold at once)
