@@ -969,7 +969,7 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void f8_mid_kernel(F8AttnAr
 // Bound by the matrix cores at 2,048 tokens over 32,000 keys, GQA 4, 4 KV heads of 256: 1,108 GFLOP in
 // 1,017 to 1,110 us (boxes differ), 1.0 to 1.09 PFLOP/s (a library product of fp16 matrices: 1.19; the conversion of tiles takes
 // about a quarter).  Short prompts pay 8 to 11 us a row tile before its first product and after its
-// last: six of 150 to 4,000 tokens, GQA 8, 128, window 1,500: 88 GFLOP in 150 to 157 us.
+// last: six of 150 to 4,000 tokens, GQA 8, 128, window 1,500: 88 GFLOP in 147 to 157 us.
 
 // A row tile's cost beside its key tiles, in tiles (measured to its first product and from its last:
 // 11 us against 2.1 a tile at head_dim 256, 8 against 2.6 at 128; and a part that begins inside a row
