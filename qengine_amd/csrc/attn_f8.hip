@@ -1151,8 +1151,9 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         for (int i = 0; i < 4; i++)
           if (loaded < 0 || key0 + 4 * vq + i >= rt.end) vr[i] = 0;
       }
-      // (an absent page's exponent is not one)
-      const float ksc = pow2f((kx >> k_bit) & 255u), vsc = pow2f(loaded < 0 ? 127 : (vx >> v_bit) & 255u);
+      // (the exponent of an absent page is not one, nor that of a page that begins past the last key)
+      const bool none = loaded < 0 || key0 >= rt.end;
+      const float ksc = pow2f((kx >> k_bit) & 255u), vsc = pow2f(none ? 127 : (vx >> v_bit) & 255u);
       uint8_t* kb = k_lds[k_buf];
       uint8_t* vb = v_lds[v_buf];
       const int key = wave * WK + lane / LPR, slot = lane % LPR;

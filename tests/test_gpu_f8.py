@@ -257,6 +257,26 @@ def test_pages_that_were_never_written(new, hd):
     _check_attn((q, kp, vp, ke, ve, tables, starts, pos), 0.1)
 
 
+@pytest.mark.parametrize("new", [[1, 1, 1], [5, 12, 2], [90, 1, 33], [70, 100, 8]])
+@pytest.mark.parametrize("bt", [16, 32, 48])
+@pytest.mark.parametrize("hd", [128, 256])
+def test_pages_reserved_ahead(new, bt, hd):
+    """Pages of a slot's table past its last key were never written and hold anything, exponents too: a tile that
+    reaches into one is not touched by it."""
+    rng = np.random.default_rng(bt + hd + sum(new))
+    lens = [200, 40, 7]
+    blocks = -(-max(a + b for a, b in zip(lens, new)) // bt) + 6
+    tables, starts, pos, n_pages = R.layout(rng, lens, new, bt, 2, hd, spare=blocks, max_blocks=blocks)
+    (kp, ke), (vp, ve) = R.random_pool(rng, n_pages, bt, 2, hd), R.random_pool(rng, n_pages, bt, 2, hd)
+    free = sorted(set(range(n_pages)) - set(tables.ravel().tolist()))
+    kp[free], vp[free], ke[free], ve[free] = 0x7f, 0xff, 255, 255
+    for s in range(3):
+        ahead = np.flatnonzero(tables[s] < 0)
+        tables[s, ahead] = free[:len(ahead)]
+    q = rng.standard_normal((int(starts[-1]) + 2, 8, hd)).astype(np.float16)
+    _check_attn((q, kp, vp, ke, ve, tables, starts, pos), 0.1)
+
+
 @pytest.mark.parametrize("new", [[1, 1, 1], [4, 9, 2], [80, 1, 40]])
 def test_extreme_scores(new):
     """Peaked rows (one weight is all), a negative scale, and a scale of zero (the mean)."""
