@@ -146,7 +146,8 @@ __device__ __forceinline__ RowTile row_tile(const F8AttnArgs& p, const Slot& x, 
   r.end = min(r.pos_hi + 1, p.max_ctx);
   r.w0 = p.window > 0 ? max(0, r.pos_lo - p.window + 1) / KT : 0;
   r.n_sink = p.window > 0 ? min((p.sink + KT - 1) / KT, r.w0) : 0;
-  r.tiles = max(1, r.n_sink + (r.end + KT - 1) / KT - r.w0);   // (a tile past every key is masked)
+  // (the window may lie past max_ctx: then the sinks alone; a tile past every key is masked)
+  r.tiles = max(1, r.n_sink + max(0, (r.end + KT - 1) / KT - r.w0));
   return r;
 }
 

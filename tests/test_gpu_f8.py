@@ -326,6 +326,15 @@ def test_context_limit():
     _check_attn(case, 0.09, max_ctx=200)
 
 
+@pytest.mark.parametrize("new", [[1, 1, 1], [5, 9, 2], [16, 1, 12], [70, 300, 5]])
+@pytest.mark.parametrize("hd", [128, 256])
+@pytest.mark.parametrize("max_ctx,window,sink", [(200, 50, 40), (200, 1, 200), (333, 64, 100), (33, 20, 1)])
+def test_sinks_past_the_context_limit(new, hd, max_ctx, window, sink):
+    """Queries whose window lies past max_ctx see the sinks, all of them, and nothing else."""
+    got = _check_attn(_attn_case(hd + sum(new) + sink, [400, 30, 1000], new, 16, 2, 4, hd), 0.09, window, sink, max_ctx=max_ctx)
+    assert np.abs(got[0]).max() > 0   # (the first slot's queries are past the limit by more than the window)
+
+
 def test_starts_out_of_order():
     """Starts that decrease name the same rows again and again: 2^32 key tiles of a head here, which is no call
     that can be carried out (nothing is), and a few, which is."""
