@@ -633,7 +633,8 @@ int qkv_pages_release(int32_t* block_tables, int n_slots, int max_blocks, int bl
  * it holds rows ahead of positions[i].  Free pages are taken lowest index first,
  * in list order; a slot that they do not suffice for, and those after it that
  * want any, get QKV_ERR_PAGES.  n <= 1024.  scratch: device memory of
- * qkv_pages_reserve_scratch_bytes; its first 2n int32 are afterwards the copied
+ * qkv_pages_reserve_scratch_bytes, in use until the call's work is done (it carries
+ * the plan from one kernel to the next); its first 2n int32 are afterwards the copied
  * (from, to) pairs, -1 where none, for qkv_pages_copy of further planes. */
 size_t qkv_pages_reserve_scratch_bytes(int n, int max_new, int block_tokens);
 int qkv_pages_reserve(int32_t* block_tables, int n_slots, int max_blocks, int block_tokens,
@@ -651,7 +652,8 @@ int qkv_pages_copy(const qkv_page_plane* planes, int n_planes, int n_pages, cons
 /* Moves the pages in use to indices 0 .. *n_used - 1 (device int32): the i-th
  * page in use at or past n_used goes to the i-th free one before it, in planes,
  * tables and counts.  moved[p] (device int32 [n_pages]) is where page p is now, -1
- * if it was free.  scratch: device, (n_pages + 2) * 4 bytes. */
+ * if it was free.  scratch: device, (n_pages + 2) * 4 bytes, in use until the call's
+ * work is done. */
 int qkv_pages_compact(int32_t* block_tables, int n_slots, int max_blocks, int32_t* ref_counts,
                       int n_pages, int32_t* moved, int32_t* n_used, const qkv_page_plane* planes,
                       int n_planes, int32_t* scratch, size_t scratch_bytes, hipStream_t stream);

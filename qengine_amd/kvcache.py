@@ -813,10 +813,13 @@ def _planes_of(planes, n_pages, dev):
 
 
 def _scratch(n_bytes, device, stream) -> torch.Tensor:
-    t = torch.empty(max(1, n_bytes // 4), dtype=torch.int32, device=device)
-    if stream is not None:
-        t.record_stream(stream)
-    return t
+    """Scratch of a call on `stream` (the current one when None), out of that stream's memory: a block of
+    another stream's may still be written by work under way there."""
+    n = max(1, n_bytes // 4)
+    if stream is None:
+        return torch.empty(n, dtype=torch.int32, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(n, dtype=torch.int32, device=device)
 
 
 def pages_fork(block_tables, ref_counts, parents, children, n_tokens, status=None, *, block_tokens,

@@ -206,3 +206,39 @@ def test_offsets_past_four_gigabytes():
     big[4195] = 77
     kvcache.pages_copy(kvcache.page_planes([big]), i32([(4195, 4199)]))
     assert (big[4199] == 77).all() and (big[4194] == 0).all() and (big[3] == 0).all()
+
+
+def test_scratch_on_a_given_stream():
+    """With stream= and no scratch the plan lies in that stream's memory, not in a block that the current stream
+    gave back and may still write; the calls' results are the same."""
+    s = torch.cuda.Stream()
+    lent = torch.empty(10000, dtype=torch.int32, device=DEV)   # a block for the current stream to have at hand
+    del lent
+    t = kvcache._scratch(40000, torch.device(DEV), s)
+    owner = [x["stream"] for x in torch.cuda.memory_snapshot() if x["address"] <= t.data_ptr() < x["address"] + x["total_size"]]
+    assert owner == [s.cuda_stream]
+
+    p = Pool(6, 20, 200, 16, plane_bytes=(4096, 20), seed=11)
+    p.fill([100, 37, 5, 0, 0, 0])
+    p.put()
+    st = i32([9] * 3)
+    calls = [i32(x) for x in ([0, 1, 0], [3, 4, 5], [100, 37, 90])], [i32(x) for x in ([0, 3, 4], [100, 100, 37], [1, 40, 3])]
+    back, keep, moved, used = i32([0, 5]), i32([0, 33]), i32([0] * 200), i32([0])
+    R.fork(p.tables, p.refs, [0, 1, 0], [3, 4, 5], [100, 37, 90], 16)
+    s.wait_stream(torch.cuda.current_stream())
+    kvcache.pages_fork(p.t, p.r, *calls[0], block_tokens=16, stream=s)
+    kvcache.pages_reserve(p.t, p.r, *calls[1], st, p.planes, block_tokens=16, max_new=40, stream=s)
+    want, pairs = R.reserve(p.tables, p.refs, [0, 3, 4], [100, 100, 37], [1, 40, 3], 40, 16)
+    p.copied(pairs)
+    kvcache.pages_release(p.t, p.r, back, keep, block_tokens=16, stream=s)
+    R.release(p.tables, p.refs, [0, 5], [0, 33], 16)
+    kvcache.pages_compact(p.t, p.r, moved, used, p.planes, stream=s)
+    to, n = R.compact(p.tables, p.refs)
+    src = [x.copy() for x in p.data]
+    for a, b in enumerate(to):
+        if b >= 0 and a != b:
+            for x, y in zip(p.data, src):
+                x[b] = y[a]
+    s.synchronize()
+    assert st.tolist() == want == [0] * 3 and used.item() == n and np.array_equal(moved.cpu().numpy(), to)
+    p.check()

@@ -257,3 +257,30 @@ def test_wrappers_refuse_before_the_launch():
     for f in bad:
         with pytest.raises(ValueError):
             f()
+
+
+def test_scratch_is_of_the_stream_of_the_call(monkeypatch):
+    """Scratch that a page call allocates for another stream is allocated with that stream current: memory of
+    the current one may still be in use by its work, and the plan in it is trusted."""
+    inside, seen = [None], []
+
+    class Within:
+        def __init__(self, stream):
+            self.stream = stream
+
+        def __enter__(self):
+            inside.append(self.stream)
+
+        def __exit__(self, *_):
+            inside.pop()
+
+    empty = torch.empty
+    monkeypatch.setattr(torch.cuda, "stream", Within)
+    monkeypatch.setattr(torch, "empty", lambda *a, **k: (seen.append(inside[-1]), empty(*a, **k))[1])
+
+    class Stream:
+        pass
+
+    s = Stream()
+    assert kvcache._scratch(64, "cpu", s).numel() == 16 and seen == [s]
+    assert kvcache._scratch(0, "cpu", None).numel() == 1 and seen == [s, None]
