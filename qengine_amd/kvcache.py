@@ -57,6 +57,16 @@ def _dev_ptr(t: torch.Tensor, what: str) -> int:
     return t.data_ptr()
 
 
+def _scratch(n_bytes, device, stream) -> torch.Tensor:
+    """Scratch of a call on `stream` (the current one when None), out of that stream's memory: a block of
+    another stream's may still be written by work under way there."""
+    n = max(1, n_bytes // 4)
+    if stream is None:
+        return torch.empty(n, dtype=torch.int32, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(n, dtype=torch.int32, device=device)
+
+
 def tq3_blocks(n_blocks: int, device) -> torch.Tensor:
     """Zero-initialised TQ3 block storage [n_blocks, 52] (model.cuh:1914-1920)."""
     return torch.zeros((n_blocks, TQ3_BLOCK_BYTES), dtype=torch.uint8, device=device)
@@ -285,7 +295,7 @@ def block_index_ms(q, k_pool, k_pool_max, block_index, *, num_q, num_kv, sub_n, 
     through `workspace` (allocated here when None)."""
     if workspace is None:
         n = int(lib().qkv_block_index_ms_workspace_bytes(num_kv, sub_n, n_blocks))
-        workspace = torch.empty(max(n, 256), dtype=torch.uint8, device=block_index.device)
+        workspace = _scratch(max(n, 256), block_index.device, stream)
     check(lib().qkv_block_index_ms(
         _dev_ptr(q, "q"), _dev_ptr(k_pool, "k_pool"), _dev_ptr(k_pool_max, "k_pool_max"),
         _i32(block_index, "block_index"), num_q, num_kv, head_dim, sub_n, block_index.shape[1],
@@ -810,16 +820,6 @@ def _planes_of(planes, n_pages, dev):
         if planes.device != dev:
             raise ValueError(f"the planes must be on cuda:{dev}, where the call runs")
     return planes.ptr, planes.n
-
-
-def _scratch(n_bytes, device, stream) -> torch.Tensor:
-    """Scratch of a call on `stream` (the current one when None), out of that stream's memory: a block of
-    another stream's may still be written by work under way there."""
-    n = max(1, n_bytes // 4)
-    if stream is None:
-        return torch.empty(n, dtype=torch.int32, device=device)
-    with torch.cuda.stream(stream):
-        return torch.empty(n, dtype=torch.int32, device=device)
 
 
 def pages_fork(block_tables, ref_counts, parents, children, n_tokens, status=None, *, block_tokens,

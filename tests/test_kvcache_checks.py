@@ -94,3 +94,24 @@ def test_row_copies_reject_short_flat_buffers(fn):
         fn(pool_k, pool_v, _u8(rows * kr), _u8(rows * vr), table[:1], **kw)
     with pytest.raises(ValueError, match="block_table must be"):
         fn(pool_k, pool_v, _u8(rows * kr), _u8(rows * vr), table.to(torch.int64), **kw)
+
+
+def test_block_index_workspace_is_of_the_stream_of_the_call(monkeypatch):
+    """The workspace that block_index_ms allocates is taken from the memory of the stream that uses it: it is
+    given back when the call returns, while the kernels may still be under way there."""
+    class Stop(Exception):
+        pass
+
+    asked = []
+
+    def scratch(n_bytes, device, stream):
+        asked.append((n_bytes, device, stream))
+        raise Stop
+
+    monkeypatch.setattr(K, "_scratch", scratch)
+    side = object()
+    index = torch.zeros((NKV, 16, 8), dtype=torch.int32)
+    with pytest.raises(Stop):
+        K.block_index_ms(_f16(16 * NQ * HD), _f16(1), _f16(1), index, num_q=NQ, num_kv=NKV, sub_n=16, start_pos=0,
+                         top_k=8, n_blocks=70, stream=side)
+    assert asked == [(NKV * 16 * 70 * 4, index.device, side)]
