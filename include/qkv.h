@@ -585,9 +585,10 @@ int qkv_f8_append_kv_paged(const uint16_t* k, long k_stride, const uint16_t* v, 
  * its window may be given back (negative entries).  A query that sees no key gets
  * a zero row.  out [n_rows][num_q][head_dim]; may be q.  num_q / num_kv 1..8.
  * Values are read as fp16 (exact for exponents 95..135, which the append
- * writes).  workspace: qkv_attn_f8_paged_workspace_bytes of the same numbers,
- * 256-byte aligned, ZERO-FILLED before its first use; calls leave it ready for the
- * next one, of any numbers it is large enough for.  Calls sharing one must be
+ * writes).  workspace: qkv_attn_f8_paged_workspace_bytes of these numbers or larger
+ * ones (the most that any call with up to its n_slots, n_rows, max_tok and max_ctx
+ * needs), 256-byte aligned, ZERO-FILLED before its first use; calls leave it ready for
+ * the next one, of any numbers it is large enough for.  Calls sharing one must be
  * ordered. */
 size_t qkv_attn_f8_paged_workspace_bytes(int num_q, int num_kv, int head_dim, int n_slots,
                                          int n_rows, int max_tok, int max_ctx);

@@ -229,7 +229,15 @@ extern "C" {
 size_t qkv_attn_f8_paged_workspace_bytes(int num_q, int num_kv, int head_dim, int n_slots, int n_rows, int max_tok,
                                          int max_ctx) {
   if (check_f8_attn(num_q, num_kv, head_dim, n_slots, n_rows, max_tok, max_ctx) != QKV_OK) return 0;
-  return f8_attn_plans(num_q, num_kv, head_dim, n_slots, n_rows, max_tok, max_ctx).total();
+  // The largest of any call with up to these numbers.  A kernel's workspace grows with each of them, but
+  // the kernel for more rows may need less than that for fewer, so each is asked for the most rows it takes.
+  if (max_tok > n_rows) max_tok = n_rows;
+  size_t most = qkv::f8_attn_plan(num_q, num_kv, head_dim, n_slots, n_rows, max_tok, max_ctx).total;
+  const int gqa = num_q / num_kv;
+  for (int rows : {16, 32, 64})
+    if (rows / gqa < max_tok)
+      most = std::max(most, qkv::f8_attn_plan(num_q, num_kv, head_dim, n_slots, n_rows, rows / gqa, max_ctx).total);
+  return most;
 }
 
 int qkv_attn_f8_paged(const uint16_t* q, const uint8_t* k_pool, const uint8_t* v_pool, const uint8_t* k_exp,

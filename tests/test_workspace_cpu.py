@@ -25,3 +25,25 @@ def test_tq3_workspace_of_many_queries(num_q, num_kv, sub_n):
     # which whole queries fill at least half of the 64 columns
     records = max(rows, 256 * 64 + rows)
     assert last <= 2 * 1040 * records + 512, (last, records)
+
+
+@pytest.mark.parametrize("head_dim", [128, 256])
+@pytest.mark.parametrize("num_q,num_kv", [(8, 8), (16, 8), (9, 3), (16, 4), (20, 4), (24, 4), (14, 2), (32, 4), (8, 1)])
+def test_paged8_workspace_serves_smaller_calls(num_q, num_kv, head_dim):
+    """A workspace for the largest batch serves every smaller one: the size never falls as any of its numbers grows."""
+    size = lib().qkv_attn_f8_paged_workspace_bytes
+    grid = [(1, 2, 4, 33, 64, 65, 300), (1, 4, 17, 64, 300, 5000), (1, 2, 3, 4, 5, 7, 8, 9, 16, 17, 32, 33, 64, 65, 257, 3000),
+            (1, 64, 65, 1024, 1025, 2048, 2049, 65536, 1 << 20)]
+    need = {}
+    for slots in grid[0]:
+        for rows in grid[1]:
+            for tok in grid[2]:
+                for ctx in grid[3]:
+                    need[slots, rows, tok, ctx] = size(num_q, num_kv, head_dim, slots, rows, tok, ctx)
+    assert min(need.values()) > 0
+    for at, n in need.items():
+        for i in range(4):
+            up = grid[i].index(at[i]) + 1
+            if up < len(grid[i]):
+                more = at[:i] + (grid[i][up],) + at[i + 1:]
+                assert need[more] >= n, (at, more)
