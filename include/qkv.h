@@ -567,7 +567,9 @@ int qkv_rope(const uint16_t* q, long q_stride, uint16_t* q_out, long q_out_strid
  * With rot_dim > 0 (a multiple of 16) K is first rotated as by qkv_rope
  * (rounded to fp16), and with num_q > 0 the query rows too, q -> q_out (in
  * place or apart), all in the same launch; the result equals qkv_rope at those
- * positions followed by this call without it. */
+ * positions followed by this call without it.  QKV_ERR_UNSUPPORTED past 2^31
+ * workgroups: n_slots * (max_tok / block_tokens + 2) * num_kv * 2 for the cache and
+ * n_rows * num_q * head_dim / 512 for the queries. */
 int qkv_f8_append_kv_paged(const uint16_t* k, long k_stride, const uint16_t* v, long v_stride,
                            uint8_t* k_pool, uint8_t* v_pool, uint8_t* k_exp, uint8_t* v_exp,
                            int n_rows, int n_slots, int max_tok, int num_kv, int head_dim,

@@ -117,8 +117,9 @@ __global__ __launch_bounds__(THREADS, ROPE || THREADS == 1024 ? 4 : 8) void f8_a
   const int tid = threadIdx.x;
   const int hd = p.head_dim, cpr = hd / 8, cpr_log = hd == 256 ? 5 : 4;   // (head_dim is 128 or 256)
   const RowRope rope{p.turns, p.amplitude, p.rot, p.layout};
-  long wg = blockIdx.x;
-  if (ROPE && wg >= p.kv_wgs) {
+  long wg = (long)blockIdx.y * gridDim.x + blockIdx.x;
+  if (wg >= p.kv_wgs) {
+    if (!ROPE || p.q == nullptr) return;
     // query rows: 16 elements of QH heads a thread, both sides of their pairs (they may be in place),
     // whose cosines are formed once
     constexpr int QH = 4;
@@ -253,7 +254,7 @@ hipError_t launch_f8_append(F8AppendArgs a, hipStream_t stream) {
   const long wgs = kv + (q_units + threads - 1) / threads;
   if (wgs > 0x7fffffffL) return hipErrorInvalidValue;
   a.kv_wgs = kv;
-  const dim3 grid((unsigned)wgs), block((unsigned)threads);
+  const dim3 grid = grid_xy(wgs), block((unsigned)threads);
   auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, stream, a); };
   if (threads == 64) a.rot ? launch(f8_append_kernel<64, true>) : launch(f8_append_kernel<64, false>);
   else if (threads == 256) a.rot ? launch(f8_append_kernel<256, true>) : launch(f8_append_kernel<256, false>);

@@ -6,6 +6,15 @@
 
 namespace qkv {
 
+// `wgs` workgroups over x and y: a dimension of a launch holds fewer than 2^32 threads (what is
+// past them is dropped without an error).  A workgroup's number is y * gridDim.x + x; those
+// from `wgs` on have nothing to do.
+inline dim3 grid_xy(long wgs) {
+  constexpr long kMaxX = 1l << 21;   // (of up to 1,024 threads)
+  const long x = wgs < kMaxX ? wgs : kMaxX;
+  return dim3((unsigned)x, (unsigned)((wgs + x - 1) / x));
+}
+
 // Row mapping of a paged append: input block i (token i / blocks_per_row,
 // slot token / n_tok, position positions[slot] + token % n_tok) goes to
 // pool row block_tables[slot * max_blocks + pos / block_tokens] *

@@ -134,6 +134,35 @@ def test_rope_in_the_append(layout, rot, new):
     assert torch.equal(buf[:n, :6], qo[:n]) and torch.equal(buf[n:], keep)
 
 
+def test_append_of_a_long_prompt_beside_many_slots():
+    """255 single tokens beside a prompt of 65,536 in 16-row pages: more than 2^32 threads. The same bits as the two apart."""
+    slots, prompt, bt, kv, hd, nq = 256, 65536, 16, 8, 256, 8
+    g = torch.Generator(device=DEV).manual_seed(5)
+    n, blocks = prompt + slots - 1, prompt // bt
+    q, k, v = (torch.randn(n, heads, hd, device=DEV, generator=g, dtype=torch.float16) for heads in (nq, kv, kv))
+    tables = torch.full((slots, blocks), -1, dtype=torch.int32, device=DEV)
+    tables[slots // 2] = torch.arange(blocks, device=DEV)
+    own = torch.cat([torch.arange(slots // 2), torch.arange(slots // 2 + 1, slots)])
+    tables[own, 0] = blocks + torch.arange(slots - 1, dtype=torch.int32, device=DEV)
+    new = [1] * slots
+    new[slots // 2] = prompt
+    starts = torch.tensor(np.cumsum([0] + new), dtype=torch.int32, device=DEV)
+    pos = torch.zeros(slots, dtype=torch.int32, device=DEV)
+    t = kvcache.rope_table(64, device=DEV)
+    a = [*kvcache.f8_pool(blocks + slots - 1, bt, kv, hd, DEV), *kvcache.f8_pool(blocks + slots - 1, bt, kv, hd, DEV)]
+    b = [x.clone() for x in a]
+    got, want = torch.zeros_like(q), torch.zeros_like(q)
+
+    def call(c, out, lo, hi, most):
+        kvcache.f8_append_kv_paged(k, v, c[0], c[2], c[1], c[3], tables[lo:hi], starts[lo:hi + 1], pos[lo:hi], max_tok=most,
+                                   q=q, q_out=out, rope=t)
+    call(a, got, 0, slots, prompt)
+    for lo, hi, most in ((0, slots // 2, 1), (slots // 2, slots // 2 + 1, prompt), (slots // 2 + 1, slots, 1)):
+        call(b, want, lo, hi, most)
+    assert all(torch.equal(x, y) for x, y in zip(a, b)) and torch.equal(got, want)
+    assert (a[1] > 0).all() and (a[3] > 0).all()   # (every page was written)
+
+
 # ---------------------------------------------------------------------------
 # attention
 # ---------------------------------------------------------------------------
