@@ -1407,8 +1407,10 @@ template <int HD>
 __global__ __launch_bounds__(256) void f8_merge_kernel(F8AttnArgs p) {
   constexpr int E = HD / 64;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int tile = blockIdx.x / p.rec_rows, row = blockIdx.x - tile * p.rec_rows;
-  const int s = tile / p.num_kv, h = tile - s * p.num_kv, gqa = p.gqa;
+  const uint32_t at = blockIdx.y * gridDim.x + blockIdx.x, tile = at / p.rec_rows;
+  const int row = (int)(at - tile * p.rec_rows);
+  if (tile >= (uint32_t)(p.n_slots * p.num_kv)) return;
+  const int s = (int)tile / p.num_kv, h = (int)tile - s * p.num_kv, gqa = p.gqa;
   const int2 desc = p.desc[tile];
   const Slot sl = slot_of(p, s);
   const int n = desc.x, r0 = desc.y;
@@ -1541,7 +1543,8 @@ static void launch_f8(const F8AttnArgs& a, const F8AttnPlan& x, hipStream_t stre
     if (x.groups > 1)
       hipLaunchKernelGGL((f8_cut_merge_kernel<HD>), dim3((unsigned)(x.groups - 1) * (HD / 16)), dim3(256), 0, stream, a);
   } else {
-    hipLaunchKernelGGL((f8_merge_kernel<HD>), dim3((unsigned)(a.n_slots * a.num_kv * x.rec_rows)), dim3(256), 0, stream, a);
+    // (at most 2^22 row tiles of 64 rows)
+    hipLaunchKernelGGL((f8_merge_kernel<HD>), grid_xy((long)a.n_slots * a.num_kv * x.rec_rows), dim3(256), 0, stream, a);
   }
 }
 

@@ -380,6 +380,26 @@ def test_starts_out_of_order():
         assert (out == want).all()
 
 
+def test_more_than_four_billion_merge_threads():
+    """32,771 slots of 64 rows of eight heads, some of them cut between parts: each slot's rows as the one slot's
+    of the reference."""
+    slots, kv, gqa, tok, bt, hd = 32771, 8, 8, 8, 16, 128
+    one = _attn_case(77, [140], [tok], bt, kv, gqa, hd, spare_rows=0)
+    q, kp, vp, ke, ve, tables, _, _ = one
+    ref, tol = R.attention(*one[:6], [0, tok], [140], 0.09)
+    qd = dev(q).repeat(slots, 1, 1)
+    out = torch.zeros_like(qd)
+    starts = torch.arange(0, slots * tok + 1, tok, dtype=torch.int32, device=DEV)
+    pos = torch.full((slots,), 140, dtype=torch.int32, device=DEV)
+    ws = kvcache.attn_f8_paged_workspace(kv * gqa, kv, slots, slots * tok, tok, 148, DEV, head_dim=hd)
+    kvcache.attn_f8_paged(qd, dev(kp), dev(vp), dev(ke), dev(ve), out, ws, dev(tables).repeat(slots, 1), starts, pos,
+                          max_tok=tok, max_ctx=148, scale=0.09)
+    del qd
+    rd, td = dev(ref), dev(tol)
+    for part in out.view(slots, tok, kv * gqa, hd).split(1024):
+        assert ((part.double() - rd).abs() <= td).all()
+
+
 def test_same_result_every_time_and_on_another_stream():
     case = _attn_case(8, [3000, 10, 700], [1, 1, 1], 64, 2, 4, 256)
     a = _attend(*case, 0.06)
