@@ -532,7 +532,7 @@ int qkv_rope_table(int rot_dim, double base, int scaling, double factor, double 
  * inverse != 0 turns by the negative angle: it undoes the forward call up to
  * amplitude^2, and is the gradient of the rows from that of the outputs.  fp32
  * arithmetic, one rounding to fp16.  rot_dim even, <= head_dim <= 8192; at most
- * 1024 heads each. */
+ * 1024 heads each, and below 2^39 elements in all (QKV_ERR_UNSUPPORTED). */
 int qkv_rope(const uint16_t* q, long q_stride, uint16_t* q_out, long q_out_stride,
              const uint16_t* k, long k_stride, uint16_t* k_out, long k_out_stride,
              const int32_t* positions, const uint64_t* turns, float amplitude, int n_tok, int num_q,

@@ -18,7 +18,7 @@ namespace qkv {
 // 17.8 us; the same from 2,000 to 4,000 tokens).
 template <int HPT>
 __global__ __launch_bounds__(256) void rope_kernel(RopeArgs p) {
-  const long u = (long)blockIdx.x * 256 + threadIdx.x;
+  const long u = ((long)blockIdx.z * gridDim.x + blockIdx.x) * 256 + threadIdx.x;
   if (u >= (long)p.n_tok * p.units) return;
   const int tok = (int)(u / p.units), c = (int)(u - (long)tok * p.units);
   const int h0 = blockIdx.y * HPT;
@@ -62,7 +62,7 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs p) {
 // Any even rot, head size, stride and alignment: a thread per pair or copied element.
 __global__ __launch_bounds__(256) void rope_any_kernel(RopeArgs p) {
   const int per = p.units;   // rot / 2 pairs, then the copied elements (none in place)
-  const long u = (long)blockIdx.x * 256 + threadIdx.x;
+  const long u = ((long)blockIdx.y * gridDim.x + blockIdx.x) * 256 + threadIdx.x;
   if (u >= (long)p.n_tok * (p.num_q + p.num_k) * per) return;
   const long row = u / per;
   const int i = (int)(u - row * per);
@@ -91,15 +91,15 @@ hipError_t launch_rope(RopeArgs a, bool wide, bool in_place, hipStream_t stream)
   if (wide) {
     a.units = (in_place ? a.rot : a.head_dim) / 16;
     const long threads = (long)a.n_tok * a.units;
-    const unsigned gx = (unsigned)((threads + 255) / 256);
+    const dim3 g = grid_xy((threads + 255) / 256);
     if (threads * heads <= 256 * 1024)
-      hipLaunchKernelGGL(rope_kernel<1>, dim3(gx, (unsigned)heads), dim3(256), 0, stream, a);
+      hipLaunchKernelGGL(rope_kernel<1>, dim3(g.x, (unsigned)heads, g.y), dim3(256), 0, stream, a);
     else
-      hipLaunchKernelGGL(rope_kernel<4>, dim3(gx, (unsigned)((heads + 3) / 4)), dim3(256), 0, stream, a);
+      hipLaunchKernelGGL(rope_kernel<4>, dim3(g.x, (unsigned)((heads + 3) / 4), g.y), dim3(256), 0, stream, a);
   } else {
     a.units = in_place ? a.rot / 2 : a.head_dim - a.rot / 2;
     const long n = (long)a.n_tok * heads * a.units;
-    hipLaunchKernelGGL(rope_any_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL(rope_any_kernel, grid_xy((n + 255) / 256), dim3(256), 0, stream, a);
   }
   return hipGetLastError();
 }

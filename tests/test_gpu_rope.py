@@ -132,3 +132,16 @@ def test_undoes_itself_and_moves_cached_keys():
     lim = 2 * 2.0 ** -11 * 1.5 * x.abs().max().item() + 1e-5
     assert (back.float() - x.float()).abs().max().item() <= lim
     assert (_run(y, d, t).float() - _run(x, pos + d, t).float()).abs().max().item() <= lim
+
+
+def test_more_than_four_billion_threads():
+    """A call of 2^32 elements and more (9 GB, rows that the wide kernel does not take): first, middle and last
+    tokens as in calls of their own."""
+    n, heads, hd = 70000, 64, 1001
+    x = torch.randn(64, heads, hd, device=DEV).half().repeat(n // 64 + 1, 1, 1)[:n]
+    out = torch.zeros_like(x)
+    pos = torch.arange(n, dtype=torch.int32, device=DEV)
+    t = kvcache.rope_table(2, device=DEV)
+    kvcache.rope(x, None, pos, t, q_out=out)
+    for a in (0, n // 2, n - 4000, n - 64):
+        assert torch.equal(out[a:a + 64], _run(x[a:a + 64], pos[a:a + 64], t))
