@@ -611,7 +611,8 @@ int qkv_attn_f8_paged(const uint16_t* q, const uint8_t* k_pool, const uint8_t* v
  * before the call returns, of at most 128; planes do not overlap.
  * status (device int32 [n], may be NULL): per list entry QKV_OK,
  * QKV_ERR_INVALID or QKV_ERR_PAGES; an entry that is not OK changes nothing.
- * Lists are device int32; a slot may be named once a call.
+ * Lists are device int32, below 2^24 entries (reserve: 1024); a slot may be named
+ * once a call.
  * ------------------------------------------------------------------------- */
 typedef struct qkv_page_plane {
   void* base;

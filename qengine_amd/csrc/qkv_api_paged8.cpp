@@ -13,6 +13,9 @@ namespace {
 inline bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 inline int launch_status(hipError_t e) { return e == hipSuccess ? QKV_OK : QKV_ERR_LAUNCH; }
 
+// entries of a fork or release: a launch of 256 threads each drops what is past 2^32 threads
+constexpr int kMaxList = 1 << 24;
+
 constexpr qkv::PageStatus kPageStatus{QKV_OK, QKV_ERR_INVALID, QKV_ERR_PAGES};
 
 // the shape of a paged 8-bit cache
@@ -312,6 +315,7 @@ int qkv_pages_fork(int32_t* block_tables, int n_slots, int max_blocks, int block
   const int st = check_tables(t);
   if (st != QKV_OK) return st;
   if (n < 0 || n > n_slots) return QKV_ERR_INVALID;
+  if (n >= kMaxList) return QKV_ERR_UNSUPPORTED;
   if (n == 0) return QKV_OK;
   if (!parents || !children || !n_tokens) return QKV_ERR_NULL;
   if (!aligned(parents, 4) || !aligned(children, 4) || !aligned(n_tokens, 4) || !aligned(status, 4)) return QKV_ERR_ALIGN;
@@ -325,6 +329,7 @@ int qkv_pages_release(int32_t* block_tables, int n_slots, int max_blocks, int bl
   const int st = check_tables(t);
   if (st != QKV_OK) return st;
   if (n < 0 || n > n_slots) return QKV_ERR_INVALID;
+  if (n >= kMaxList) return QKV_ERR_UNSUPPORTED;
   if (n == 0) return QKV_OK;
   if (!slots || !keep_tokens) return QKV_ERR_NULL;
   if (!aligned(slots, 4) || !aligned(keep_tokens, 4) || !aligned(status, 4)) return QKV_ERR_ALIGN;

@@ -284,3 +284,10 @@ def test_scratch_is_of_the_stream_of_the_call(monkeypatch):
     s = Stream()
     assert kvcache._scratch(64, "cpu", s).numel() == 16 and seen == [s]
     assert kvcache._scratch(0, "cpu", None).numel() == 1 and seen == [s, None]
+
+
+def test_lists_that_one_launch_does_not_hold(L, p):
+    """Forks and releases of 2^24 entries and more, 2^32 threads, of which a launch would drop the last."""
+    for n in (1 << 24, (1 << 24) + 5, 2**31 - 1):
+        assert L.qkv_pages_fork(p, 2**31 - 1, 1, 16, p, 8, p, p, p, n, p, None) == -3
+        assert L.qkv_pages_release(p, 2**31 - 1, 1, 16, p, 8, p, p, n, p, None) == -3
