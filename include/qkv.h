@@ -585,7 +585,12 @@ int qkv_f8_append_kv_paged(const uint16_t* k, long k_stride, const uint16_t* v, 
  * j <= p, j < max_ctx, of pages in [0, n_pages); with window_tok > 0 only those
  * with j > p - window_tok or j < sink_tok.  So the pages of a slot that are out of
  * its window may be given back (negative entries).  A query that sees no key gets
- * a zero row.  out [n_rows][num_q][head_dim]; may be q.  num_q / num_kv 1..8.
+ * a zero row.  out [n_rows][num_q][head_dim]; may be q.  num_q / num_kv 1..8, num_q
+ * <= 1024, max_ctx <= 2^30; with R = max_tok * num_q / num_kv / 256 + 1 row tiles a
+ * slot, n_slots * R * num_kv <= 2^22 and, for the tiles of all slots (at most n_slots
+ * * R and n_rows * num_q / num_kv / 256 + n_slots), tiles * max(num_kv, 2) *
+ * (max_ctx / 32 + 16) < 2147483000: QKV_ERR_UNSUPPORTED past these, and 0 from the
+ * workspace query.
  * Values are read as fp16 (exact for exponents 95..135, which the append
  * writes).  workspace: qkv_attn_f8_paged_workspace_bytes of these numbers or larger
  * ones (the most that any call with up to its n_slots, n_rows, max_tok and max_ctx

@@ -734,6 +734,9 @@ def f8_append_kv_paged(k, v, k_pool, v_pool, k_exp, v_exp, block_tables, starts,
 def attn_f8_paged_workspace(num_q, num_kv, n_slots, n_rows, max_tok, max_ctx, device, *, head_dim=256) -> torch.Tensor:
     """Zero-filled workspace of attn_f8_paged for these numbers (calls leave it ready for the next)."""
     n = int(lib().qkv_attn_f8_paged_workspace_bytes(num_q, num_kv, head_dim, n_slots, n_rows, max_tok, max_ctx))
+    if n == 0 and min(n_slots, n_rows, max_tok) > 0:   # (a batch without rows needs none)
+        raise ValueError(f"no call of these numbers: num_q {num_q}, num_kv {num_kv}, head_dim {head_dim}, n_slots {n_slots}, "
+                         f"n_rows {n_rows}, max_tok {max_tok}, max_ctx {max_ctx}")
     return torch.zeros(n, dtype=torch.uint8, device=device)
 
 

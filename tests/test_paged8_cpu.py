@@ -291,3 +291,24 @@ def test_lists_that_one_launch_does_not_hold(L, p):
     for n in (1 << 24, (1 << 24) + 5, 2**31 - 1):
         assert L.qkv_pages_fork(p, 2**31 - 1, 1, 16, p, 8, p, p, p, n, p, None) == -3
         assert L.qkv_pages_release(p, 2**31 - 1, 1, 16, p, 8, p, p, n, p, None) == -3
+
+
+def test_workspace_of_calls_that_are_refused():
+    """The wrapper refuses numbers that the call refuses, at the stated limits, instead of handing out nothing; a
+    batch without rows needs none."""
+    def w(nq=16, kv=4, slots=4, rows=64, tok=4, ctx=4096, hd=256):
+        return kvcache.attn_f8_paged_workspace(nq, kv, slots, rows, tok, ctx, "cpu", head_dim=hd)
+    assert w().numel() > 0
+    assert w(slots=0).numel() == w(rows=0).numel() == w(tok=0).numel() == 0
+    for bad in (dict(nq=18), dict(nq=36), dict(hd=64), dict(kv=0), dict(ctx=0), dict(ctx=(1 << 30) + 1), dict(nq=2048, kv=1024)):
+        with pytest.raises(ValueError, match="no call of these numbers"):
+            w(**bad)
+    size = kvcache.lib().qkv_attn_f8_paged_workspace_bytes
+    # n_slots * (max_tok * gqa / 256 + 1) * num_kv up to 2^22: 2^20 / (1 + 1/64) slots of one token
+    for hd in (128, 256):
+        last = int((1 << 20) / (1 + 4 / 256))
+        assert size(16, 4, hd, last, 1 << 20, 1, 100) > 0 and size(16, 4, hd, last + 1, 1 << 20, 1, 100) == 0
+        # tiles * max(num_kv, 2) * (max_ctx / 32 + 16): one prompt of 2^20 rows at GQA 4
+        tiles = (1 << 20) * 4 / 256 + 1
+        ctx = int((2147483000 / (tiles * 8) - 16) * 32)
+        assert size(32, 8, hd, 1, 1 << 20, 1 << 20, ctx - 32) > 0 == size(32, 8, hd, 1, 1 << 20, 1 << 20, ctx + 32)
