@@ -511,14 +511,17 @@ typedef enum qkv_rope_scaling {
   QKV_ROPE_NTK = 2,    /* base * factor^(rot_dim / (rot_dim - 2))                         */
   QKV_ROPE_YARN = 3    /* by turns t = original_ctx * f / 2 pi: f for t >= beta_fast,
                           f / factor for t <= beta_slow, linear in t between; amplitude
-                          a = 1 + 0.1 ln(factor)                                          */
+                          a = 1 + 0.1 ln(factor).  Not the form whose ramp is linear in
+                          the pair's index i, which many models were trained with        */
 } qkv_rope_scaling;
 
 /* Fills the HOST array turns[rot_dim / 2] with the fraction of a full turn a
  * position, 64-bit fixed point (position * turns mod 2^64 is the angle: exact at
  * any distance), and *amplitude with a (1 but for YARN).  The caller copies
  * turns to the device once.  rot_dim even (NTK: >= 4), base > 0, factor >= 1;
- * factor, original_ctx and the betas are read where the scaling uses them. */
+ * factor, original_ctx and the betas are read where the scaling uses them.  A model
+ * with other frequencies f_i fills turns itself, with f_i / 2 pi * 2^64 (rounded,
+ * modulo 2^64), and passes its own amplitude to the calls. */
 int qkv_rope_table(int rot_dim, double base, int scaling, double factor, double original_ctx,
                    double beta_fast, double beta_slow, uint64_t* turns, float* amplitude);
 

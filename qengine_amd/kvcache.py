@@ -558,7 +558,8 @@ _ROPE_LAYOUT = {"half": 0, "interleaved": 1}
 
 class RopeTable:
     """Frequencies for `rope`: `turns`, an int64 device tensor [rot_dim / 2] of 64-bit
-    fractions of a turn a position, and the amplitude of the scaling."""
+    fractions of a turn a position (f / 2 pi * 2^64), and the amplitude of the scaling.  Made by
+    `rope_table`, or by hand for frequencies or an amplitude that it does not offer."""
 
     def __init__(self, turns, amplitude, rot_dim):
         if turns.dtype is not torch.int64 or 2 * turns.numel() != rot_dim:
@@ -568,7 +569,8 @@ class RopeTable:
 
 def rope_table(rot_dim: int, *, base: float = 10000.0, scaling=None, device="cuda") -> RopeTable:
     """Frequencies base^(-2i/rot_dim).  scaling: None, ("linear", factor), ("ntk", factor) or
-    ("yarn", factor, original_ctx[, beta_fast=32, beta_slow=1])."""
+    ("yarn", factor, original_ctx[, beta_fast=32, beta_slow=1]), whose ramp between the betas is
+    linear in a pair's turns over the original context, not in its index."""
     kind, args = 0, ()
     if scaling is not None:
         if scaling[0] not in _ROPE_SCALING:

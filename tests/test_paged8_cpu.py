@@ -47,6 +47,18 @@ def test_rope_table_is_the_formula(L, rot, scaling):
     assert abs(t.amplitude - amp) <= 2.0 ** -23 * amp and t.rot_dim == rot
 
 
+def test_a_table_from_a_models_own_frequencies():
+    """Made by hand from 64-bit frequencies, the table is rope_table's to the rounding of those: f by 4 of 2^-53
+    (the power, the division and the two products), and half a unit."""
+    f, amp = R.frequencies(128, 1e6)
+    t = kvcache.RopeTable(torch.tensor([round(x / (2 * np.pi) * 2.0 ** 64) for x in f]), 1.25, 128)
+    want = kvcache.rope_table(128, base=1e6, device="cpu")
+    err = np.abs(np.array([int(a) - int(b) for a, b in zip(t.turns, want.turns)], np.float64)) / 2.0 ** 64
+    # (the exponent of the power is rounded too: 2^-53 of ln f, at most 14)
+    assert (err <= f / (2 * np.pi) * (4 + 14) * 2.0 ** -53 + 2.0 ** -64).all()
+    assert t.amplitude == 1.25 and t.rot_dim == 128 and t.turns.dtype is torch.int64
+
+
 def test_rope_table_refusals(L):
     assert _table(L, 64)[0] == 0
     assert _table(L, 0)[0] == _table(L, 7)[0] == _table(L, -2)[0] == -1
