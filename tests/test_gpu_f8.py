@@ -452,6 +452,106 @@ def test_offsets_past_four_gigabytes():
     assert (R.CODES[kb[page, 900 % 64].cpu().numpy()] * 2.0 ** (e - 127)[:, None] == 1).all()
 
 
+def _check_many_slots(case, order, scale, max_ctx=None):
+    """A batch whose slot i is slot order[i] of `case`: every row as the reference's of that slot."""
+    q, kp, vp, ke, ve, tables, starts, pos = case
+    ref, tol = R.attention(q, kp, vp, ke, ve, tables, starts.tolist(), pos.tolist(), scale)
+    n = np.diff(starts)
+    rows = np.concatenate([np.arange(starts[s], starts[s + 1]) for s in order])
+    first = np.cumsum([0] + [n[s] for s in order]).astype(np.int32)
+    big = np.concatenate([q[rows], q[:3]])   # (and rows behind the last slot)
+    got = _attend(big, kp, vp, ke, ve, tables[order], first, pos[order], scale, max_ctx=max_ctx)
+    assert (got[len(rows):] == 9.0).all()
+    err = np.abs(got[:len(rows)].astype(np.float64) - ref[rows])
+    bad = np.flatnonzero((err > tol[rows]).any((1, 2)))
+    assert not len(bad), (len(bad), bad[:5], err.max())
+
+
+@pytest.mark.parametrize("hd", [128, 256])
+@pytest.mark.parametrize("max_ctx", [None, 1 << 17])   # (by the contexts; prompts and the others in launches of their own)
+@pytest.mark.parametrize("slots", [64, 65, 130, 600])
+@pytest.mark.parametrize("new,gqa", [
+    ([1, 1, 0, 1, 1], 4), ([5, 9, 0, 2, 1], 4), ([5, 8, 0, 2, 3], 8), ([40, 33, 0, 65, 1], 8)])
+def test_many_slots(new, gqa, slots, max_ctx, hd):
+    """More slots than a wave or a workgroup takes up at a time, runs of slots without rows among them, and more row
+    tiles than slots at a time."""
+    rng = np.random.default_rng(slots + hd + gqa)
+    order = rng.integers(0, 5, slots)
+    order[20:min(160, slots - 10)] = np.where(rng.random(min(160, slots - 10) - 20) < 0.02, 1, 2)
+    if slots > 300:
+        order[200:420] = 2
+    if max(new) > 64:   # (few of the longest)
+        order = np.where((order == 3) & (rng.random(slots) < 0.8), 0, order)
+    _check_many_slots(_attn_case(slots, [40, 300, 10, 5, 700], new, 16, 2, gqa, hd), order, hd ** -0.5, max_ctx)
+
+
+@pytest.mark.parametrize("hd", [128, 256])
+def test_prompts_beside_many_slots(hd):
+    """A few prompts among 600 single tokens, in one launch and in two."""
+    rng = np.random.default_rng(hd)
+    order = rng.integers(0, 3, 600)
+    order[[0, 77, 511, 512, 599]] = 3
+    for max_ctx in (None, 1 << 17):
+        _check_many_slots(_attn_case(hd, [90, 3, 10, 50], [1, 1, 0, 300], 32, 1, 4, hd), order, hd ** -0.5, max_ctx)
+
+
+@pytest.mark.parametrize("new", [[1, 1], [5, 12], [16, 3], [90, 300]])
+@pytest.mark.parametrize("hd", [128, 256])
+def test_context_limit_of_every_kernel(new, hd):
+    """As test_context_limit, for up to 16 rows, up to 64 and more, with the limit inside a slot's new rows and ahead
+    of them."""
+    for max_ctx in (100, 310, 200):
+        _check_attn(_attn_case(hd + max_ctx, [300, 30], new, 16, 2, 4, hd), 0.09, max_ctx=max_ctx)
+
+
+@pytest.mark.parametrize("hd", [128, 256])
+@pytest.mark.parametrize("lens,new,gqa", [([20000], [1], 4), ([9000, 12000], [1, 1], 1), ([20000], [12], 2), ([17000, 3], [10, 9], 6)])
+def test_merges_of_many_records(lens, new, gqa, hd):
+    """Row tiles in more than 64 parts, the records that the merge takes up at a time."""
+    _check_attn(_attn_case(hd + gqa, lens, new, 64, 1, gqa, hd), hd ** -0.5)
+
+
+@pytest.mark.parametrize("new", [[1, 1, 1], [6, 1, 9], [16, 3, 12], [70, 3, 100]])
+@pytest.mark.parametrize("window,sink", [(1, 0), (20, 0), (64, 4), (100, 33), (300, 70), (5000, 1), (7, 2**31 - 1)])
+def test_window_and_sinks_of_wide_heads(new, window, sink):
+    """As test_window_and_sinks, at head_dim 256, with every page that no query sees given back."""
+    case = _attn_case(window + sum(new), [400, 30, 999], new, 16, 2, 4, 256)
+    tables, pos = case[5], case[7]
+    for s in range(3):
+        for b in range(tables.shape[1]):
+            if b * 16 >= sink and b * 16 + 15 <= pos[s] - window:
+                tables[s, b] = -1
+    _check_attn(case, 256 ** -0.5, window, sink)
+
+
+def test_calls_on_a_given_stream():
+    """Rotation, append and attention with stream=: what they give on the current stream."""
+    rng = np.random.default_rng(12)
+    s = torch.cuda.Stream()
+    tables, starts, pos, n_pages = R.layout(rng, [30, 100, 0], [1, 20, 90], 16, 2, 128)
+    rows = int(starts[-1])
+    q, k, v = (dev(rng.standard_normal((rows, h, 128)).astype(np.float16)) for h in (8, 2, 2))
+    at = dev(np.concatenate([pos[i] + np.arange(starts[i + 1] - starts[i]) for i in range(3)]).astype(np.int32))
+    idx = [dev(x) for x in (tables, starts, pos)]
+    t = kvcache.rope_table(64, device=DEV)
+    pools = [dev(x) for x in (*R.random_pool(rng, n_pages, 16, 2, 128), *R.random_pool(rng, n_pages, 16, 2, 128))]
+    ws = [kvcache.attn_f8_paged_workspace(8, 2, 3, rows, 90, 128, DEV, head_dim=128) for _ in range(2)]
+
+    def run(stream, w):
+        kp, ke, vp, ve = [x.clone() for x in pools]
+        qr, qa, out = torch.zeros_like(q), torch.zeros_like(q), torch.zeros_like(q)
+        if stream is not None:
+            stream.wait_stream(torch.cuda.current_stream())
+        kvcache.rope(q, None, at, t, q_out=qr, stream=stream)
+        kvcache.f8_append_kv_paged(k, v, kp, vp, ke, ve, *idx, max_tok=90, q=q, q_out=qa, rope=t, stream=stream)
+        kvcache.attn_f8_paged(qr, kp, vp, ke, ve, out, w, *idx, max_tok=90, max_ctx=128, scale=0.09, stream=stream)
+        if stream is not None:
+            stream.synchronize()
+        return qr, qa, kp, vp, ke, ve, out
+    for x, y in zip(run(None, ws[0]), run(s, ws[1])):
+        assert torch.equal(x, y)
+
+
 # ---------------------------------------------------------------------------
 # together
 # ---------------------------------------------------------------------------

@@ -145,3 +145,16 @@ def test_more_than_four_billion_threads():
     kvcache.rope(x, None, pos, t, q_out=out)
     for a in (0, n // 2, n - 4000, n - 64):
         assert torch.equal(out[a:a + 64], _run(x[a:a + 64], pos[a:a + 64], t))
+
+
+@pytest.mark.parametrize("hd,rot", [(256, 64), (128, 128), (48, 30)])
+def test_a_rotation_apart_leaves_its_input(hd, rot):
+    """q, k and v of one projection buffer are as they were after q and k are rotated into buffers of their own."""
+    rng = np.random.default_rng(hd + rot)
+    buf = torch.from_numpy(rng.standard_normal((37, 6 + 2 + 2, hd)).astype(np.float16)).to(DEV)
+    before = buf.clone()
+    qo, ko = torch.empty(37, 6, hd, dtype=torch.float16, device=DEV), torch.empty(37, 2, hd, dtype=torch.float16, device=DEV)
+    kvcache.rope(buf[:, :6], buf[:, 6:8], torch.arange(37, dtype=torch.int32, device=DEV) * 11,
+                 kvcache.rope_table(rot, device=DEV), q_out=qo, k_out=ko)
+    assert torch.equal(buf, before)
+    assert not torch.equal(qo, before[:, :6]) and torch.equal(ko[..., rot:], before[:, 6:8, rot:])
