@@ -1091,12 +1091,14 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       if (!live) v_hi = 0;
     }
     // This wave's WK keys of a tile lie in one page (pages are whole sixteens).  The next tile to
-    // fetch is at row w_row of block w_base + w_at; lane i holds the page of block w_base + i.
+    // fetch is at row w_row of block w_base + w_at; lane i holds the page of block w_base + i (-1 past the
+    // last key's: a page that was never written holds anything, its exponent too).
     int w_base, w_at, w_row, pages;
     auto load_pages = [&](int b) {
       w_base = b;
       w_at = 0;
-      const int pg = b + lane < p.max_blocks ? table[b + lane] : -1;
+      const bool any = b + lane < p.max_blocks && (uint32_t)(b + lane) * (uint32_t)p.block_tokens < (uint32_t)rt.end;
+      const int pg = any ? table[b + lane] : -1;
       pages = pg < p.n_pages ? pg : -1;
     };
     auto seek = [&](int v) {
@@ -1152,9 +1154,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         for (int i = 0; i < 4; i++)
           if (loaded < 0 || key0 + 4 * vq + i >= rt.end) vr[i] = 0;
       }
-      // (the exponent of an absent page is not one, nor that of a page that begins past the last key)
-      const bool none = loaded < 0 || key0 >= rt.end;
-      const float ksc = pow2f((kx >> k_bit) & 255u), vsc = pow2f(none ? 127 : (vx >> v_bit) & 255u);
+      // (an absent page's exponent is not one)
+      const float ksc = pow2f((kx >> k_bit) & 255u), vsc = pow2f(loaded < 0 ? 127 : (vx >> v_bit) & 255u);
       uint8_t* kb = k_lds[k_buf];
       uint8_t* vb = v_lds[v_buf];
       const int key = wave * WK + lane / LPR, slot = lane % LPR;
@@ -1407,7 +1408,7 @@ template <int HD>
 __global__ __launch_bounds__(256) void f8_merge_kernel(F8AttnArgs p) {
   constexpr int E = HD / 64;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const uint32_t at = blockIdx.y * gridDim.x + blockIdx.x, tile = at / p.rec_rows;
+  const uint32_t at = blockIdx.y * kGridX + blockIdx.x, tile = at / p.rec_rows;
   const int row = (int)(at - tile * p.rec_rows);
   if (tile >= (uint32_t)(p.n_slots * p.num_kv)) return;
   const int s = (int)tile / p.num_kv, h = (int)tile - s * p.num_kv, gqa = p.gqa;

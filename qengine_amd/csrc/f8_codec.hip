@@ -117,7 +117,7 @@ __global__ __launch_bounds__(THREADS, ROPE || THREADS == 1024 ? 4 : 8) void f8_a
   const int tid = threadIdx.x;
   const int hd = p.head_dim, cpr = hd / 8, cpr_log = hd == 256 ? 5 : 4;   // (head_dim is 128 or 256)
   const RowRope rope{p.turns, p.amplitude, p.rot, p.layout};
-  long wg = (long)blockIdx.y * gridDim.x + blockIdx.x;
+  long wg = blockIdx.y * kGridX + blockIdx.x;   // (in 32 bits: so are the divisions below)
   if (wg >= p.kv_wgs) {
     if (!ROPE || p.q == nullptr) return;
     // query rows: 16 elements of QH heads a thread, both sides of their pairs (they may be in place),

@@ -7,12 +7,11 @@
 namespace qkv {
 
 // `wgs` workgroups over x and y: a dimension of a launch holds fewer than 2^32 threads (what is
-// past them is dropped without an error).  A workgroup's number is y * gridDim.x + x; those
-// from `wgs` on have nothing to do.
+// past them is dropped without an error).  A workgroup's number (below 2^32) is
+// y * kGridX + x; those from `wgs` on have nothing to do.
+constexpr uint32_t kGridX = 1u << 21;   // (of up to 1,024 threads)
 inline dim3 grid_xy(long wgs) {
-  constexpr long kMaxX = 1l << 21;   // (of up to 1,024 threads)
-  const long x = wgs < kMaxX ? wgs : kMaxX;
-  return dim3((unsigned)x, (unsigned)((wgs + x - 1) / x));
+  return wgs <= kGridX ? dim3((unsigned)wgs) : dim3(kGridX, (unsigned)((wgs + kGridX - 1) / kGridX));
 }
 
 // Row mapping of a paged append: input block i (token i / blocks_per_row,

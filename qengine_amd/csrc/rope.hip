@@ -18,7 +18,7 @@ namespace qkv {
 // 17.8 us; the same from 2,000 to 4,000 tokens).
 template <int HPT>
 __global__ __launch_bounds__(256) void rope_kernel(RopeArgs p) {
-  const long u = ((long)blockIdx.z * gridDim.x + blockIdx.x) * 256 + threadIdx.x;
+  const long u = (long)(blockIdx.z * kGridX + blockIdx.x) * 256 + threadIdx.x;
   if (u >= (long)p.n_tok * p.units) return;
   const int tok = (int)(u / p.units), c = (int)(u - (long)tok * p.units);
   const int h0 = blockIdx.y * HPT;
@@ -62,7 +62,7 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs p) {
 // Any even rot, head size, stride and alignment: a thread per pair or copied element.
 __global__ __launch_bounds__(256) void rope_any_kernel(RopeArgs p) {
   const int per = p.units;   // rot / 2 pairs, then the copied elements (none in place)
-  const long u = ((long)blockIdx.y * gridDim.x + blockIdx.x) * 256 + threadIdx.x;
+  const long u = (long)(blockIdx.y * kGridX + blockIdx.x) * 256 + threadIdx.x;
   if (u >= (long)p.n_tok * (p.num_q + p.num_k) * per) return;
   const long row = u / per;
   const int i = (int)(u - row * per);
