@@ -242,3 +242,52 @@ def test_scratch_on_a_given_stream():
     s.synchronize()
     assert st.tolist() == want == [0] * 3 and used.item() == n and np.array_equal(moved.cpu().numpy(), to)
     p.check()
+
+
+def test_captured_without_scratch():
+    """Release, reserve and compact in one graph, their scratch out of the graph's own memory: every replay, with
+    eager calls and other allocations between, as the bookkeeping."""
+    p = Pool(5, 30, 120, 16, plane_bytes=(4096, 20), seed=12)
+    p.fill([100, 37, 5, 0, 60])
+    p.put()
+    slots, pos, new = list(range(5)), np.array([100, 37, 5, 0, 60]), [3, 17, 1, 2, 0]
+    back, keep = i32([4]), i32([9])
+    sl, at, nw, moved, used, st = i32(slots), i32(pos), i32(new), i32([0] * 120), i32([0]), i32([9] * 5)
+
+    def step():
+        kvcache.pages_release(p.t, p.r, back, keep, block_tokens=16)
+        kvcache.pages_reserve(p.t, p.r, sl, at, nw, st, p.planes, block_tokens=16, max_new=20)
+        kvcache.pages_compact(p.t, p.r, moved, used, p.planes)
+
+    def plain():
+        R.release(p.tables, p.refs, [4], [9], 16)
+        want, pairs = R.reserve(p.tables, p.refs, slots, [int(x) for x in pos], new, 20, 16)
+        p.copied(pairs)
+        to, n = R.compact(p.tables, p.refs)
+        src = [x.copy() for x in p.data]
+        for a, b in enumerate(to):
+            if b >= 0 and a != b:
+                for x, y in zip(p.data, src):
+                    x[b] = y[a]
+        return want, n
+    R.fork(p.tables, p.refs, [0], [3], [100], 16)
+    kvcache.pages_fork(p.t, p.r, i32([0]), i32([3]), i32([100]), block_tokens=16)
+    pos[3] = 100
+    at.copy_(i32(pos))
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        step()
+    p.check()   # (capturing runs nothing)
+    for turn in range(9):
+        junk = [torch.full((n,), -7, dtype=torch.int32, device=DEV) for n in (16, 34, 122, 500)]
+        if turn % 3 == 1:
+            step()
+        else:
+            g.replay()
+        want, n = plain()
+        assert st.tolist() == want and used.item() == n, turn
+        p.check()
+        del junk
+        pos[:4] += new[:4]
+        pos[4] = 9
+        at.copy_(i32(pos))
