@@ -527,8 +527,8 @@ int qkv_rope_table(int rot_dim, double base, int scaling, double factor, double 
 
 /* Rotates n_tok tokens' query and key rows (fp16) in one launch.  Token t of q
  * starts at q + t * q_stride (elements; heads head_dim apart), so views into a
- * fused projection buffer work; k, and the outputs, likewise.  Out may be in
- * (with its stride) or memory that does not overlap it.  num_q or num_k may be
+ * fused projection buffer work; k, and the outputs, likewise.  Out may be its in
+ * (with its stride) or memory that overlaps neither q nor k.  num_q or num_k may be
  * 0 (its pointers are not read).  positions: device int32 [n_tok], any sign.
  * turns: device copy of qkv_rope_table's, rot_dim / 2 entries.  Elements from
  * rot_dim on are copied.  layout 0: pairs (i, i + rot_dim / 2); 1: (2i, 2i + 1).

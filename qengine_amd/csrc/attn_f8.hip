@@ -369,8 +369,8 @@ __device__ __forceinline__ Tile tile_at(const F8AttnArgs& p, const const_i32* ta
 // 16-row pages of 128, 358 MB in 64 to 67 us.  Parts for 256, 768 or 1,024 workgroups were slower than
 // for 512 (two a CU).
 // JOIN: short contexts, whose records the last workgroup of a tile joins in this launch: there latency
-// is all (a call at 700 keys 9.7 us, with the merge's launch 12.9; by one workgroup of eight waves a
-// KV head 13.4).
+// is all (a call at 700 keys 8.8 us, with the merge's launch 11.1 to 13.1; by one workgroup of eight
+// waves a KV head 13.4).
 constexpr int kJoinKeys = 1024, kJoinStep = 8;
 constexpr int kCoherent = 1 | 16;   // sc0 | sc1: where every XCD sees it, as device-wide atomics go
 template <int HD, bool JOIN>
@@ -967,10 +967,14 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void f8_mid_kernel(F8AttnAr
 // At head_dim 128 a tile is two halves of 32 keys, both scored before the weights.  All waves convert
 // ahead of a tile's scores: one of each SIMD behind its values was slower (1,112 against 1,070 us
 // below), and so were two workgroups of four waves a CU.
+// Weights are rounded once to fp16 (2^-11 of a weight; their sum is that of the rounded ones), which
+// puts the output's error against 64 bits at 2.5e-4 to 2.9e-4, beside 2.1e-4 of its own rounding: two
+// parts, as the kernel for few rows has, take 1,347 against 1,023 us below and 191 against 147.
 // Bound by the matrix cores at 2,048 tokens over 32,000 keys, GQA 4, 4 KV heads of 256: 1,108 GFLOP in
-// 1,017 to 1,110 us (boxes differ), 1.0 to 1.09 PFLOP/s (a library product of fp16 matrices: 1.19; the conversion of tiles takes
-// about a quarter).  Short prompts pay 8 to 11 us a row tile before its first product and after its
-// last: six of 150 to 4,000 tokens, GQA 8, 128, window 1,500: 88 GFLOP in 147 to 157 us.
+// 1,008 to 1,110 us (boxes differ), 1.0 to 1.10 PFLOP/s (a library product of fp16 matrices: 1.19; the
+// conversion of tiles takes about a quarter).  Short prompts pay 8 to 11 us a row tile before its first
+// product and after its last: six of 150 to 4,000 tokens, GQA 8, 128, window 1,500: 88 GFLOP in 145 to
+// 157 us.
 
 // A row tile's cost beside its key tiles, in tiles (measured to its first product and from its last:
 // 11 us against 2.1 a tile at head_dim 256, 8 against 2.6 at 128; and a part that begins inside a row
@@ -1494,10 +1498,10 @@ F8AttnPlan f8_attn_plan(int num_q, int num_kv, int head_dim, int n_slots, long q
     x.slot_tiles = 1;
     x.rec_rows = (int)rows;
     // Short contexts: few records, joined in the launch where one workgroup takes no longer for them than
-    // a second launch: up to 1,024 keys (16 slots of 16 rows of 256: 20.3 against 20.1 us, 16 rows
-    // of 128 14.4 and 17.4), for rows of up to 2,048 elements up to 2,048 keys (one token of 2,000 keys
-    // 13.1 and 16.3 us, two in eight slots 17.5 and 18.7, but 16 rows of 256 24.2 and 19.8; four slots
-    // of 4,000 keys 19.3 and 17.4).
+    // a second launch: up to 1,024 keys (16 slots of 16 rows of 256: 19.8 against 18.8 to 19.6 us, 16 rows
+    // of 128 12.9 and 14.0 to 15.4), for rows of up to 2,048 elements up to 2,048 keys (one token of 2,000
+    // keys 10.5 and 11.1 to 13.3 us, though two in eight slots 17.3 and 14.9 to 16.1; not 16 rows of 256,
+    // 24.2 and 19.8, nor four slots of 4,000 keys, 19.3 and 17.4).
     const long row_elems = rows * head_dim;
     x.join = x.row_tiles == 1 && max_ctx <= (row_elems <= 2048 ? 2 : 1) * kJoinKeys && n_slots <= 64 && n_slots * num_kv <= kJoinCounts;
     const int unit_keys = x.row_tiles == 4 ? 64 : 128;
@@ -1516,7 +1520,7 @@ F8AttnPlan f8_attn_plan(int num_q, int num_kv, int head_dim, int n_slots, long q
 
 // A call may hold prompts and single tokens.  A one-token slot costs the kernel for many rows the
 // conversion of whole tiles for a 64th of their rows (32 slots at 4,000 keys and a prompt of 2,048
-// tokens: 221 us in one launch, 134 as two); a launch for nothing costs 7 us.  The numbers do not
+// tokens: 184 to 190 us in one launch, 132 to 140 as two); a launch for nothing costs 7 us.  The numbers do not
 // say how the rows spread: the fewest slots that can hold them all are taken to be prompts, and the
 // others to have up to 16 rows, with whole contexts.
 int f8_attn_apart(int num_q, int num_kv, int head_dim, int n_slots, long rows, int max_tok, int max_ctx) {

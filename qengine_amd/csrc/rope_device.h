@@ -2,9 +2,9 @@
 //
 // Pair i of a head at position p turns by p * f_i radians.  The frequency is
 // held as R_i, the fraction f_i / 2 pi of a full turn in 64-bit fixed point, so
-// that p * R_i mod 2^64 is the angle modulo one turn, exactly: 32 bits of angle
-// would be off by p * 2^-33 turns (0.1 mrad at p = 2^20 from fp32 products, whose
-// angle itself is rounded to 0.06 rad there).  The top 32 bits of the product give
+// that p * R_i mod 2^64 is the angle modulo one turn, exactly: 32 bits of fraction
+// would be off by p * 2^-33 turns (2^-13 turns, 0.77 mrad, at p = 2^20), and an angle
+// of 2^20 radians in fp32 by up to 0.06 rad.  The top 32 bits of the product give
 // the nearest quarter turn and a remainder of at most an eighth (error 2^-32 turns).
 #pragma once
 #include <hip/hip_runtime.h>
