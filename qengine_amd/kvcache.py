@@ -67,6 +67,17 @@ def _scratch(n_bytes, device, stream) -> torch.Tensor:
         return torch.empty(n, dtype=torch.int32, device=device)
 
 
+def _result(n, device, stream) -> torch.Tensor:
+    """n fp16 numbers that a call on `stream` writes and its caller uses on the current stream: out of the
+    memory of the former, and kept until the latter is done with them."""
+    if stream is None:
+        return torch.empty(n, dtype=torch.float16, device=device)
+    with torch.cuda.stream(stream):
+        t = torch.empty(n, dtype=torch.float16, device=device)
+    t.record_stream(torch.cuda.current_stream(device))
+    return t
+
+
 def tq3_blocks(n_blocks: int, device) -> torch.Tensor:
     """Zero-initialised TQ3 block storage [n_blocks, 52] (model.cuh:1914-1920)."""
     return torch.zeros((n_blocks, TQ3_BLOCK_BYTES), dtype=torch.uint8, device=device)
@@ -102,7 +113,7 @@ def tq3_dequant(blocks: torch.Tensor, out: torch.Tensor | None = None, stream=No
     """turboquant.cuh:169-200.  Returns fp16 [n_blocks*128]."""
     n = blocks.numel() // TQ3_BLOCK_BYTES
     if out is None:
-        out = torch.empty(n * 128, dtype=torch.float16, device=blocks.device)
+        out = _result(n * 128, blocks.device, stream)
     check(lib().qkv_tq3_dequant(_dev_ptr(blocks, "blocks"), _dev_ptr(out, "out"), n,
                                 _stream(stream)), "qkv_tq3_dequant")
     return out
@@ -134,7 +145,7 @@ def q8_dequant(blocks: torch.Tensor, out: torch.Tensor | None = None, stream=Non
     """attention.cuh:2614-2626."""
     n = blocks.numel() // Q8_BLOCK_BYTES
     if out is None:
-        out = torch.empty(n * 32, dtype=torch.float16, device=blocks.device)
+        out = _result(n * 32, blocks.device, stream)
     check(lib().qkv_q8_dequant(_dev_ptr(blocks, "blocks"), _dev_ptr(out, "out"), n,
                                _stream(stream)), "qkv_q8_dequant")
     return out

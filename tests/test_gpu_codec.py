@@ -216,3 +216,25 @@ def test_q8_dequant_bitexact(dev):
     got = kvcache.q8_dequant(_to_dev(blocks.view(np.uint8).reshape(-1, 36), dev))
     torch.cuda.synchronize()
     assert np.array_equal(got.cpu().numpy().view(np.uint16), O.q8_decode(blocks))
+
+
+def test_dequant_on_a_given_stream(dev):
+    """With stream= and no out, the output lies in that stream's memory and holds what the current stream's would."""
+    import torch
+    from qengine_amd import kvcache
+    x = torch.randn(64 * 128, device=dev, generator=torch.Generator(device=dev).manual_seed(2)).half()
+    s = torch.cuda.Stream()
+    for make, append, dequant, n in ((kvcache.tq3_blocks, kvcache.tq3_append, kvcache.tq3_dequant, 64),
+                                     (kvcache.q8_blocks, kvcache.q8_append, kvcache.q8_dequant, 256)):
+        blocks = make(n, dev)
+        append(x, blocks)
+        want = dequant(blocks)
+        lent = torch.empty_like(want)   # a block for the current stream to have at hand
+        del lent
+        s.wait_stream(torch.cuda.current_stream())
+        got = dequant(blocks, stream=s)
+        owner = [y["stream"] for y in torch.cuda.memory_snapshot()
+                 if y["address"] <= got.data_ptr() < y["address"] + y["total_size"]]
+        assert owner == [s.cuda_stream]
+        torch.cuda.current_stream().wait_stream(s)
+        assert torch.equal(got, want)

@@ -115,3 +115,23 @@ def test_block_index_workspace_is_of_the_stream_of_the_call(monkeypatch):
         K.block_index_ms(_f16(16 * NQ * HD), _f16(1), _f16(1), index, num_q=NQ, num_kv=NKV, sub_n=16, start_pos=0,
                          top_k=8, n_blocks=70, stream=side)
     assert asked == [(NKV * 16 * 70 * 4, index.device, side)]
+
+
+@pytest.mark.parametrize("call,block,per", [(K.tq3_dequant, K.TQ3_BLOCK_BYTES, 128), (K.q8_dequant, K.Q8_BLOCK_BYTES, 32)])
+def test_dequant_output_is_of_the_stream_of_the_call(monkeypatch, call, block, per):
+    """The output that a dequant on a given stream allocates is asked for that stream: a block of the current
+    stream's may still be in use by work under way there."""
+    class Stop(Exception):
+        pass
+
+    asked = []
+
+    def result(n, device, stream):
+        asked.append((n, device, stream))
+        raise Stop
+
+    monkeypatch.setattr(K, "_result", result)
+    side = object()
+    with pytest.raises(Stop):
+        call(_u8(3 * block), stream=side)
+    assert asked == [(3 * per, torch.device("cpu"), side)]
