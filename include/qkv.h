@@ -97,7 +97,8 @@ int qkv_tq3_dequant(const qkv_block_tq3* in, uint16_t* out_f16, int n_blocks,
 
 /* Replaces quantize_kv_q8_0_kern<<<n_blocks, 32, 0, stream>>>(in, out, n_blocks)
  * (attention.cuh:2587-2609; launched at model.cuh:2316-2317).  `pad` is not
- * written.  in: n_blocks*32 fp16 (16-byte aligned). */
+ * written.  in: n_blocks*32 fp16 (16-byte aligned).  The Q8_0 calls take up to
+ * 2^30 - 64 blocks (QKV_ERR_UNSUPPORTED past them). */
 int qkv_q8_append(const uint16_t* in_f16, qkv_block_q8* out, int n_blocks,
                   hipStream_t stream);
 
@@ -118,7 +119,7 @@ int qkv_q8_dequant(const qkv_block_q8* in, uint16_t* out_f16, int n_blocks,
  * kv_dim) (model.cuh:149-159; launched at model.cuh:3189-3192):
  * out[i] = half(float(q[i]) * float(scales[i / 128])), the scales of a row of
  * kv_dim elements being scales[row * kv_dim / 128 ...].  kv_dim a multiple of
- * 128, n a multiple of 8; q 8-byte and out 16-byte aligned. */
+ * 128, n a multiple of 8 below 2^35; q 8-byte and out 16-byte aligned. */
 int qkv_dfk2_dequant(const int8_t* q, const uint16_t* scales, uint16_t* out_f16, long long n,
                      int kv_dim, hipStream_t stream);
 
@@ -230,7 +231,8 @@ int qkv_attn_split_q8(const uint16_t* q, const qkv_block_q8* k, const qkv_block_
  * ceil(total_kv / block_size_n) - 1 of each kv head: the fp16 mean and the
  * sign-preserving max-abs over the block's dequantized keys, into
  * k_pool / k_pool_max [num_kv][n_blocks_stride][256] fp16.  Bit-identical to
- * the reference.  block_size_n <= 64. */
+ * the reference.  block_size_n <= 64; fewer than 2^24 (head, block) pairs a call
+ * (QKV_ERR_UNSUPPORTED). */
 int qkv_tq3_kpool_update(const qkv_block_tq3* k_cache, uint16_t* k_pool, uint16_t* k_pool_max,
                          int num_kv, int head_dim, int total_kv, int blk_lo, int n_blocks_stride,
                          int block_size_n, hipStream_t stream);

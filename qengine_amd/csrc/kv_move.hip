@@ -67,7 +67,7 @@ __global__ __launch_bounds__(256) void kv_page_copy_kernel(PageCopyArgs a) {
   typedef typename std::conditional<UNIT == 16, uint4, uint32_t>::type unit_t;
   const int t = blockIdx.y;
   const uint32_t row_units = a.row_bytes[t] / UNIT;
-  const long g = (long)blockIdx.x * 256 + threadIdx.x;
+  const long g = (long)(blockIdx.z * kGridX + blockIdx.x) * 256 + threadIdx.x;
   if (g >= (long)a.n_rows * row_units) return;
   const long r = g / row_units;
   const uint32_t c = (uint32_t)(g - r * row_units);
@@ -95,7 +95,7 @@ hipError_t launch_kv_page_copy(const PageCopyArgs& a, bool scatter, hipStream_t 
   uint32_t max_units = a.row_bytes[0] / unit;
   if (a.n_tensors == 2) max_units = std::max(max_units, a.row_bytes[1] / unit);
   const long total = (long)a.n_rows * max_units;
-  const dim3 grid((unsigned)((total + 255) / 256), a.n_tensors);
+  const dim3 xy = grid_xy((total + 255) / 256), grid(xy.x, a.n_tensors, xy.y);
   if (wide && scatter)
     hipLaunchKernelGGL((kv_page_copy_kernel<16, true>), grid, dim3(256), 0, stream, a);
   else if (wide)

@@ -6,6 +6,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <atomic>
 #include <cstring>
 #include <mutex>
@@ -22,6 +23,9 @@ inline bool aligned(const void* p, size_t a) {
 }
 
 inline int launch_status(hipError_t e) { return e == hipSuccess ? QKV_OK : QKV_ERR_LAUNCH; }
+
+// a launch holds fewer than 2^32 threads (what is past them is dropped without an error): four a block
+constexpr int kMaxQ8Blocks = (1 << 30) - 64;
 
 std::mutex g_init_mu;
 bool g_init_ok[64];
@@ -126,6 +130,7 @@ int qkv_tq3_dequant(const qkv_block_tq3* in, uint16_t* out_f16, int n_blocks, hi
 
 int qkv_q8_append(const uint16_t* in_f16, qkv_block_q8* out, int n_blocks, hipStream_t stream) {
   if (n_blocks < 0) return QKV_ERR_INVALID;
+  if (n_blocks > kMaxQ8Blocks) return QKV_ERR_UNSUPPORTED;
   if (n_blocks == 0) return QKV_OK;
   if (!in_f16 || !out) return QKV_ERR_NULL;
   if (!aligned(in_f16, 16) || !aligned(out, 4)) return QKV_ERR_ALIGN;
@@ -135,6 +140,7 @@ int qkv_q8_append(const uint16_t* in_f16, qkv_block_q8* out, int n_blocks, hipSt
 int qkv_q8_append_kv(const uint16_t* k_f16, const uint16_t* v_f16, qkv_block_q8* k_out,
                      qkv_block_q8* v_out, int n_blocks, hipStream_t stream) {
   if (n_blocks < 0) return QKV_ERR_INVALID;
+  if (n_blocks > kMaxQ8Blocks) return QKV_ERR_UNSUPPORTED;
   if (n_blocks == 0) return QKV_OK;
   if (!k_f16 || !v_f16 || !k_out || !v_out) return QKV_ERR_NULL;
   if (!aligned(k_f16, 16) || !aligned(v_f16, 16) || !aligned(k_out, 4) || !aligned(v_out, 4))
@@ -144,7 +150,7 @@ int qkv_q8_append_kv(const uint16_t* k_f16, const uint16_t* v_f16, qkv_block_q8*
 int qkv_dfk2_dequant(const int8_t* q, const uint16_t* scales, uint16_t* out_f16, long long n,
                      int kv_dim, hipStream_t stream) {
   if (n < 0 || kv_dim <= 0) return QKV_ERR_INVALID;
-  if (kv_dim % 128 != 0 || n % 8 != 0) return QKV_ERR_UNSUPPORTED;
+  if (kv_dim % 128 != 0 || n % 8 != 0 || n / 8 > (1ll << 32) - 256) return QKV_ERR_UNSUPPORTED;   // (a thread each)
   if (n == 0) return QKV_OK;
   if (!q || !scales || !out_f16) return QKV_ERR_NULL;
   if (!aligned(q, 8) || !aligned(scales, 2) || !aligned(out_f16, 16)) return QKV_ERR_ALIGN;
@@ -164,6 +170,7 @@ int qkv_tq3_append_dfk2(const int8_t* q, const uint16_t* scales, qkv_block_tq3* 
 int qkv_q8_append_dfk2(const int8_t* q, const uint16_t* scales, qkv_block_q8* out, int n_blocks,
                        hipStream_t stream) {
   if (n_blocks < 0) return QKV_ERR_INVALID;
+  if (n_blocks > kMaxQ8Blocks) return QKV_ERR_UNSUPPORTED;
   if (n_blocks % 4 != 0) return QKV_ERR_UNSUPPORTED;
   if (n_blocks == 0) return QKV_OK;
   if (!q || !scales || !out) return QKV_ERR_NULL;
@@ -219,6 +226,8 @@ static int kv_page_copy(void* k_pool, void* v_pool, void* k_flat, void* v_flat,
   if (n_tensors == 2 && (v_row_bytes == 0 || v_row_bytes % 4 || v_row_bytes > 0x7fffffffULL))
     return QKV_ERR_INVALID;
   if ((long)(n_rows - 1) / block_tokens >= max_blocks) return QKV_ERR_INVALID;
+  if ((double)n_rows * std::max(k_row_bytes, n_tensors == 2 ? v_row_bytes : 0) >= (double)(1l << 40))
+    return QKV_ERR_UNSUPPORTED;
   if (!aligned(k_pool, 4) || !aligned(k_flat, 4) || !aligned(block_table, 4) ||
       (n_tensors == 2 && (!aligned(v_pool, 4) || !aligned(v_flat, 4))))
     return QKV_ERR_ALIGN;
@@ -260,6 +269,7 @@ int qkv_kv_scatter_rows(void* k_pool, void* v_pool, const void* k_flat, const vo
 
 int qkv_q8_dequant(const qkv_block_q8* in, uint16_t* out_f16, int n_blocks, hipStream_t stream) {
   if (n_blocks < 0) return QKV_ERR_INVALID;
+  if (n_blocks > kMaxQ8Blocks) return QKV_ERR_UNSUPPORTED;
   if (n_blocks == 0) return QKV_OK;
   if (!in || !out_f16) return QKV_ERR_NULL;
   if (!aligned(in, 4) || !aligned(out_f16, 16)) return QKV_ERR_ALIGN;
@@ -394,7 +404,7 @@ int qkv_tq3_kpool_update(const qkv_block_tq3* k_cache, uint16_t* k_pool, uint16_
   const int cur_blocks = (int)(((long)total_kv + block_size_n - 1) / block_size_n);
   if (cur_blocks > n_blocks_stride) return QKV_ERR_INVALID;
   if (blk_lo >= cur_blocks) return QKV_OK;
-  if ((long)num_kv * (cur_blocks - blk_lo) > 0x7fffffffL) return QKV_ERR_UNSUPPORTED;
+  if ((long)num_kv * (cur_blocks - blk_lo) >= 1l << 24) return QKV_ERR_UNSUPPORTED;   // (of 256 threads each)
   if (!k_cache || !k_pool || !k_pool_max) return QKV_ERR_NULL;
   if (!aligned(k_cache, 4) || !aligned(k_pool, 2) || !aligned(k_pool_max, 2)) return QKV_ERR_ALIGN;
   qkv::KpoolArgs a{};

@@ -364,7 +364,9 @@ hipError_t launch_tq3_kpool(const KpoolArgs& a, hipStream_t stream) {
 hipError_t launch_block_index(const BlockIndexArgs& a, float* scores, hipStream_t stream) {
   const bool two = a.sub_n > 8;   // queries per thread
   const long n_wg = (long)a.num_kv * ((a.n_blocks + kScBlocks - 1) / kScBlocks) * ((a.sub_n + (two ? 15 : 7)) / (two ? 16 : 8));
-  if (n_wg <= 0) return hipErrorInvalidValue;
+  // (a launch of 2^32 threads and more drops the last without an error)
+  if (n_wg <= 0 || n_wg * kSpThreads >= 1l << 32 || (long)a.num_kv * a.sub_n * kTkThreads >= 1l << 32)
+    return hipErrorInvalidValue;
   if (two)
     hipLaunchKernelGGL((block_score_kernel<2>), dim3((unsigned)n_wg), dim3(kSpThreads), 0, stream, a, scores);
   else

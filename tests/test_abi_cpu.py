@@ -286,3 +286,17 @@ def test_header_compiles_as_c_and_cxx(lang, compiler, std):
         cmd.insert(2, "-pedantic")
     r = subprocess.run(cmd, capture_output=True, text=True)
     assert r.returncode == 0, r.stderr
+
+
+def test_calls_of_more_threads_than_a_launch_holds():
+    """2^32 threads and more, of which a launch drops the last, are refused before anything is launched."""
+    L = _lib.lib()
+    p = 1 << 20   # (an aligned address that is not read)
+    for n in ((1 << 30) - 63, 1 << 30, 2**31 - 4):
+        assert L.qkv_q8_append(p, p, n, None) == L.qkv_q8_dequant(p, p, n, None) == -3
+        assert L.qkv_q8_append_kv(p, p, p, p, n, None) == L.qkv_q8_append_dfk2(p, p, p, n, None) == -3
+    assert L.qkv_dfk2_dequant(p, p, p, 1 << 35, 1024, None) == -3
+    # (num_kv * blocks) of 2^24
+    assert L.qkv_tq3_kpool_update(p, p, p, 8, 256, (1 << 21) * 64, 0, 1 << 21, 64, None) == -3
+    for f in (L.qkv_kv_gather_rows, L.qkv_kv_scatter_rows):
+        assert f(p, None, p, None, 1 << 12, 0, 1 << 30, p, 1 << 28, 16, 1 << 28, None) == -3   # 2^40 bytes

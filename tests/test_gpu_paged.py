@@ -326,3 +326,26 @@ def test_pool_beyond_4gib(dev):
                       np.ascontiguousarray(vb).view(O.BLOCK_TQ3).reshape(-1), bt_small, ctx,
                       num_q=num_q, num_kv=num_kv, block_tokens=bt_tok)
     assert_tq3_attn(out["small"].astype(np.float64), ref.view(np.float16).astype(np.float64), ex)
+
+
+def test_gather_and_scatter_of_more_than_four_billion_threads(dev):
+    """Rows of 20 bytes, 17 GB of them, in 4-byte units: the first and the last rows through the table, unmapped ones
+    zeros, and back."""
+    import torch
+    from qengine_amd import kvcache
+    bt, row = 1 << 20, 20
+    n = 860_000_000
+    blocks = -(-n // bt)
+    table = torch.full((blocks,), -1, dtype=torch.int32, device=dev)
+    table[0], table[blocks - 1], table[blocks // 2] = 1, 0, 2
+    pool = torch.randint(0, 256, (3 * bt, row), dtype=torch.uint8, device=dev)
+    flat = torch.full((n, row), 7, dtype=torch.uint8, device=dev)
+    kvcache.kv_gather_rows(pool, None, flat, None, table, n_rows=n, block_tokens=bt, k_row_bytes=row)
+    last = (blocks - 1) * bt
+    mid = blocks // 2 * bt
+    assert torch.equal(flat[:bt], pool[bt:2 * bt]) and torch.equal(flat[last:], pool[:n - last])
+    assert torch.equal(flat[mid:mid + bt], pool[2 * bt:])
+    assert not flat[bt:mid].any() and not flat[mid + bt:last].any()
+    back = torch.zeros_like(pool)
+    kvcache.kv_scatter_rows(back, None, flat, None, table, n_rows=n, block_tokens=bt, k_row_bytes=row)
+    assert torch.equal(back[bt:], pool[bt:]) and torch.equal(back[:n - last], pool[:n - last])
