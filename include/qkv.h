@@ -543,6 +543,32 @@ int qkv_rope(const uint16_t* q, long q_stride, uint16_t* q_out, long q_out_strid
              const int32_t* positions, const uint64_t* turns, float amplitude, int n_tok, int num_q,
              int num_k, int head_dim, int rot_dim, int layout, int inverse, hipStream_t stream);
 
+/* Norms of query and key heads with the rotation in the same pass, for models that norm them ahead of it:
+ * u = x w / sqrt(mean(x^2) + eps) over a head's elements, then u turned as by qkv_rope (no rounding
+ * between).  q_weight, k_weight: device fp32 [head_dim], NULL for ones (a model whose weights stand for
+ * 1 + w passes 1 + w).  rot_dim 0: no rotation (positions and turns are not read, amplitude does not
+ * count).  Rows, strides, positions and places as for qkv_rope.  eps > 0; head_dim <= 1024
+ * (QKV_ERR_UNSUPPORTED); any head_dim, alignment to 2 bytes; fast with head_dim 64, 128, 256, 512 or 1024,
+ * rot_dim a multiple of 16, rows and weights aligned to 16 bytes. */
+int qkv_norm_rope(const uint16_t* q, long q_stride, uint16_t* q_out, long q_out_stride, const float* q_weight,
+                  const uint16_t* k, long k_stride, uint16_t* k_out, long k_out_stride, const float* k_weight,
+                  float eps, const int32_t* positions, const uint64_t* turns, float amplitude, int n_tok, int num_q,
+                  int num_k, int head_dim, int rot_dim, int layout, hipStream_t stream);
+
+/* Its gradient.  q, k: the rows that were its inputs; q_dy, k_dy: the gradients of its outputs; q_dx, k_dx
+ * gets those of its inputs (fp16, one rounding; may be the rows, or q_dy / k_dy, with their stride); q_dw,
+ * k_dw (device fp32 [head_dim], NULL: not wanted) the gradients of the weights, summed over tokens and heads
+ * in fp32, in an order that does not change from call to call.  With num_q or num_k 0 that side's
+ * pointers are neither read nor written.  workspace: qkv_norm_rope_grad_workspace_bytes of these numbers or
+ * larger ones where a weight's gradient is wanted (no initialisation needed). */
+size_t qkv_norm_rope_grad_workspace_bytes(int n_tok, int num_q, int num_k, int head_dim);
+int qkv_norm_rope_grad(const uint16_t* q, long q_stride, const uint16_t* q_dy, long q_dy_stride, uint16_t* q_dx,
+                       long q_dx_stride, const float* q_weight, float* q_dw, const uint16_t* k, long k_stride,
+                       const uint16_t* k_dy, long k_dy_stride, uint16_t* k_dx, long k_dx_stride, const float* k_weight,
+                       float* k_dw, float eps, const int32_t* positions, const uint64_t* turns, float amplitude,
+                       int n_tok, int num_q, int num_k, int head_dim, int rot_dim, int layout, void* workspace,
+                       size_t workspace_bytes, hipStream_t stream);
+
 /* ---------------------------------------------------------------------------
  * Paged 8-bit cache (F8).  No counterpart in the reference.
  * A pool holds e4m3 codes [n_pages][block_tokens][num_kv][head_dim] (one byte

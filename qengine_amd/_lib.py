@@ -91,6 +91,10 @@ SIGNATURES = {
     "qkv_prefill_attn_tq3_workspace_bytes": (_SZ, [_I, _I, _I, _I]),
     "qkv_rope_table": (_I, [_I, _D, _I, _D, _D, _D, _D, _P, _P]),
     "qkv_rope": (_I, [_P, _L, _P, _L, _P, _L, _P, _L, _P, _P, _F, _I, _I, _I, _I, _I, _I, _I, _P]),
+    "qkv_norm_rope": (_I, [_P, _L, _P, _L, _P, _P, _L, _P, _L, _P, _F, _P, _P, _F, _I, _I, _I, _I, _I, _I, _P]),
+    "qkv_norm_rope_grad_workspace_bytes": (_SZ, [_I, _I, _I, _I]),
+    "qkv_norm_rope_grad": (_I, [_P, _L, _P, _L, _P, _L, _P, _P, _P, _L, _P, _L, _P, _L, _P, _P, _F, _P, _P, _F, _I,
+                                _I, _I, _I, _I, _I, _P, _SZ, _P]),
     "qkv_f8_append_kv_paged": (_I, [_P, _L, _P, _L, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _I, _I, _I, _P,
                                     _P, _P, _L, _P, _L, _I, _P, _F, _I, _I, _P]),
     "qkv_attn_f8_paged_workspace_bytes": (_SZ, [_I, _I, _I, _I, _I, _I, _I]),

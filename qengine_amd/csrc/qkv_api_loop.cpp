@@ -1,0 +1,162 @@
+// qkv_api_loop.cpp -- the C ABI of the operators around the paged 8-bit cache in a decoding loop: norms
+// of heads with the rotation, weighing and evicting keys, beam selection and the reordering of
+// slots (declared in include/qkv.h): argument checks, then launches on the caller's stream.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "qkv_api_checks.h"
+
+namespace {
+
+// Rows of a call: n_tok tokens of `heads` heads, `stride` elements apart
+bool stride_ok(int n_tok, int heads, int head_dim, long stride) { return n_tok <= 1 || stride >= (long)heads * head_dim; }
+
+int check_norm(int n_tok, int num_q, int num_k, int head_dim, int rot_dim, int layout, float eps) {
+  if (n_tok < 0 || num_q < 0 || num_k < 0 || num_q + num_k == 0 || num_q > 1024 || num_k > 1024 || head_dim <= 0 ||
+      rot_dim < 0 || rot_dim % 2 || rot_dim > head_dim || layout < 0 || layout > 1 || !(eps > 0.f) || !std::isfinite(eps))
+    return QKV_ERR_INVALID;
+  if (head_dim > qkv::kNormMaxHead) return QKV_ERR_UNSUPPORTED;
+  return QKV_OK;
+}
+
+// 16-byte accesses of every row
+bool norm_wide(int head_dim, int rot_dim) {
+  const int lanes = head_dim / 16;
+  return head_dim % 16 == 0 && rot_dim % 16 == 0 && lanes >= 4 && (lanes & (lanes - 1)) == 0;
+}
+bool wide_rows(const void* p, long stride) { return aligned(p, 16) && stride % 8 == 0; }
+
+// Workgroups of a gradient, the queries' and the keys' (at least one of each)
+int norm_grad_groups(int n_tok, int num_q, int num_k) {
+  const double rows = (double)n_tok * (num_q + num_k);
+  return (int)std::min((double)qkv::kNormGradGroups, std::max(2.0, rows / 16));
+}
+
+}  // namespace
+
+extern "C" {
+
+int qkv_norm_rope(const uint16_t* q, long q_stride, uint16_t* q_out, long q_out_stride, const float* q_weight,
+                  const uint16_t* k, long k_stride, uint16_t* k_out, long k_out_stride, const float* k_weight,
+                  float eps, const int32_t* positions, const uint64_t* turns, float amplitude, int n_tok, int num_q,
+                  int num_k, int head_dim, int rot_dim, int layout, hipStream_t stream) {
+  const int st = check_norm(n_tok, num_q, num_k, head_dim, rot_dim, layout, eps);
+  if (st != QKV_OK) return st;
+  if (n_tok == 0) return QKV_OK;
+  if ((num_q && (!q || !q_out)) || (num_k && (!k || !k_out)) || (rot_dim && (!positions || !turns))) return QKV_ERR_NULL;
+  if ((num_q && (!stride_ok(n_tok, num_q, head_dim, q_stride) || !stride_ok(n_tok, num_q, head_dim, q_out_stride))) ||
+      (num_k && (!stride_ok(n_tok, num_k, head_dim, k_stride) || !stride_ok(n_tok, num_k, head_dim, k_out_stride))))
+    return QKV_ERR_INVALID;
+  if ((num_q && q == q_out && q_stride != q_out_stride) || (num_k && k == k_out && k_stride != k_out_stride))
+    return QKV_ERR_INVALID;
+  if (num_q && num_k && q_out == k_out) return QKV_ERR_INVALID;
+  if ((num_q && (!aligned(q, 2) || !aligned(q_out, 2) || !aligned(q_weight, 4))) ||
+      (num_k && (!aligned(k, 2) || !aligned(k_out, 2) || !aligned(k_weight, 4))) ||
+      (rot_dim && (!aligned(positions, 4) || !aligned(turns, 8))))
+    return QKV_ERR_ALIGN;
+  if ((double)n_tok * (num_q + num_k) * head_dim / 256 > 2147483647.0) return QKV_ERR_UNSUPPORTED;
+  qkv::NormRopeArgs a{};
+  a.q = num_q ? q : nullptr;
+  a.q_out = q_out;
+  a.k = num_k ? k : nullptr;
+  a.k_out = k_out;
+  a.q_weight = q_weight;
+  a.k_weight = k_weight;
+  a.positions = positions;
+  a.turns = turns;
+  a.q_stride = q_stride;
+  a.q_out_stride = q_out_stride;
+  a.k_stride = k_stride;
+  a.k_out_stride = k_out_stride;
+  a.amplitude = amplitude;
+  a.eps = eps;
+  a.n_tok = n_tok;
+  a.num_q = num_q;
+  a.num_k = num_k;
+  a.head_dim = head_dim;
+  a.rot = rot_dim;
+  a.layout = layout;
+  bool wide = norm_wide(head_dim, rot_dim);
+  if (num_q) wide = wide && wide_rows(q, q_stride) && wide_rows(q_out, q_out_stride) && aligned(q_weight, 16);
+  if (num_k) wide = wide && wide_rows(k, k_stride) && wide_rows(k_out, k_out_stride) && aligned(k_weight, 16);
+  return launch_status(qkv::launch_norm_rope(a, wide, stream));
+}
+
+size_t qkv_norm_rope_grad_workspace_bytes(int n_tok, int num_q, int num_k, int head_dim) {
+  if (check_norm(n_tok, num_q, num_k, head_dim, 0, 0, 1.f) != QKV_OK) return 0;
+  return (size_t)norm_grad_groups(n_tok, num_q, num_k) * head_dim * 4;
+}
+
+int qkv_norm_rope_grad(const uint16_t* q, long q_stride, const uint16_t* q_dy, long q_dy_stride, uint16_t* q_dx,
+                       long q_dx_stride, const float* q_weight, float* q_dw, const uint16_t* k, long k_stride,
+                       const uint16_t* k_dy, long k_dy_stride, uint16_t* k_dx, long k_dx_stride, const float* k_weight,
+                       float* k_dw, float eps, const int32_t* positions, const uint64_t* turns, float amplitude,
+                       int n_tok, int num_q, int num_k, int head_dim, int rot_dim, int layout, void* workspace,
+                       size_t workspace_bytes, hipStream_t stream) {
+  const int st = check_norm(n_tok, num_q, num_k, head_dim, rot_dim, layout, eps);
+  if (st != QKV_OK) return st;
+  if (!num_q) q_dw = nullptr;
+  if (!num_k) k_dw = nullptr;
+  const bool sums = q_dw || k_dw;
+  if (n_tok == 0 && !sums) return QKV_OK;
+  if (n_tok && ((num_q && (!q || !q_dy || !q_dx)) || (num_k && (!k || !k_dy || !k_dx)) ||
+                (rot_dim && (!positions || !turns))))
+    return QKV_ERR_NULL;
+  auto strides = [&](int heads, long s) { return !heads || stride_ok(n_tok, heads, head_dim, s); };
+  if (!strides(num_q, q_stride) || !strides(num_q, q_dy_stride) || !strides(num_q, q_dx_stride) ||
+      !strides(num_k, k_stride) || !strides(num_k, k_dy_stride) || !strides(num_k, k_dx_stride))
+    return QKV_ERR_INVALID;
+  // in place of the rows or of their outputs' gradients, with the same stride
+  auto places = [](const uint16_t* in, long s, const uint16_t* out, long so) { return in != out || s == so; };
+  if (n_tok && ((num_q && (!places(q, q_stride, q_dx, q_dx_stride) || !places(q_dy, q_dy_stride, q_dx, q_dx_stride))) ||
+                (num_k && (!places(k, k_stride, k_dx, k_dx_stride) || !places(k_dy, k_dy_stride, k_dx, k_dx_stride))) ||
+                (num_q && num_k && q_dx == k_dx)))
+    return QKV_ERR_INVALID;
+  if ((q_dw && q_dw == k_dw)) return QKV_ERR_INVALID;
+  if ((num_q && (!aligned(q, 2) || !aligned(q_dy, 2) || !aligned(q_dx, 2) || !aligned(q_weight, 4) || !aligned(q_dw, 4))) ||
+      (num_k && (!aligned(k, 2) || !aligned(k_dy, 2) || !aligned(k_dx, 2) || !aligned(k_weight, 4) || !aligned(k_dw, 4))) ||
+      (rot_dim && (!aligned(positions, 4) || !aligned(turns, 8))))
+    return QKV_ERR_ALIGN;
+  if ((double)n_tok * (num_q + num_k) * head_dim / 256 > 2147483647.0) return QKV_ERR_UNSUPPORTED;
+  if (sums && (!workspace || workspace_bytes < qkv_norm_rope_grad_workspace_bytes(n_tok, num_q, num_k, head_dim)))
+    return QKV_ERR_WORKSPACE;
+  if (sums && !aligned(workspace, 4)) return QKV_ERR_ALIGN;
+  qkv::NormRopeArgs a{};
+  a.q = num_q ? q : nullptr;
+  a.dq = q_dy;
+  a.q_out = q_dx;
+  a.k = num_k ? k : nullptr;
+  a.dk = k_dy;
+  a.k_out = k_dx;
+  a.q_weight = q_weight;
+  a.k_weight = k_weight;
+  a.q_dw = q_dw;
+  a.k_dw = k_dw;
+  a.partial = sums ? static_cast<float*>(workspace) : nullptr;
+  a.positions = positions;
+  a.turns = turns;
+  a.q_stride = q_stride;
+  a.dq_stride = q_dy_stride;
+  a.q_out_stride = q_dx_stride;
+  a.k_stride = k_stride;
+  a.dk_stride = k_dy_stride;
+  a.k_out_stride = k_dx_stride;
+  a.amplitude = amplitude;
+  a.eps = eps;
+  a.n_tok = n_tok;
+  a.num_q = num_q;
+  a.num_k = num_k;
+  a.head_dim = head_dim;
+  a.rot = rot_dim;
+  a.layout = layout;
+  bool wide = norm_wide(head_dim, rot_dim);
+  if (num_q)
+    wide = wide && wide_rows(q, q_stride) && wide_rows(q_dy, q_dy_stride) && wide_rows(q_dx, q_dx_stride) && aligned(q_weight, 16);
+  if (num_k)
+    wide = wide && wide_rows(k, k_stride) && wide_rows(k_dy, k_dy_stride) && wide_rows(k_dx, k_dx_stride) && aligned(k_weight, 16);
+  return launch_status(qkv::launch_norm_rope_grad(a, wide, norm_grad_groups(n_tok, num_q, num_k), stream));
+}
+
+}  // extern "C"

@@ -146,6 +146,33 @@ struct RopeArgs {
 // wide: 16-byte accesses (rot and head_dim multiples of 16, pointers and strides aligned)
 hipError_t launch_rope(RopeArgs a, bool wide, bool in_place, hipStream_t stream);
 
+// Norms of heads with the rotation, and the gradient (norm_rope.hip).  dq, dk and their strides, the
+// sums of the weights' gradients (q_dw, k_dw) and the partial sums are the gradient's alone.
+constexpr int kNormMaxHead = 1024;
+constexpr int kNormGradGroups = 1024;   // workgroups of a gradient: 4 on each CU
+struct NormRopeArgs {
+  const uint16_t* q;
+  const uint16_t* dq;
+  uint16_t* q_out;
+  const uint16_t* k;
+  const uint16_t* dk;
+  uint16_t* k_out;
+  const float* q_weight;     // [head_dim], nullptr: ones
+  const float* k_weight;
+  float* q_dw;               // [head_dim], nullptr: not wanted
+  float* k_dw;
+  float* partial;            // [groups][head_dim], nullptr: neither wanted
+  const int32_t* positions;
+  const uint64_t* turns;
+  long q_stride, dq_stride, q_out_stride, k_stride, dk_stride, k_out_stride;
+  float amplitude, eps;
+  int n_tok, num_q, num_k, head_dim, rot, layout;
+  int q_groups;              // workgroups of the queries' rows (set by the launcher)
+};
+// wide: 16-byte accesses, head_dim 16 times a power of two from 4 to 64, rot a multiple of 16
+hipError_t launch_norm_rope(const NormRopeArgs& a, bool wide, hipStream_t stream);
+hipError_t launch_norm_rope_grad(NormRopeArgs a, bool wide, int groups, hipStream_t stream);
+
 // Append to the paged 8-bit cache (f8_codec.hip), K and with them the queries
 // rotated where rot > 0.  rows: tokens the input tensors hold.
 struct F8AppendArgs {

@@ -686,6 +686,111 @@ def rope(q, k, positions, table: RopeTable, *, layout="half", inverse=False, q_o
 
 
 # ---------------------------------------------------------------------------
+# norms of heads with the rotation
+# ---------------------------------------------------------------------------
+
+_FP32 = torch.float32
+
+
+def _head_weight(w, hd, what, dev) -> int:
+    """Pointer of a weight (or of its gradient) of a head's elements; None: 0."""
+    if w is None:
+        return 0
+    if w.dtype is not _FP32 or w.numel() != hd:
+        raise ValueError(f"{what} must hold {hd} numbers of torch.float32")
+    _on_device(dev, w)
+    return w.data_ptr()
+
+
+def _turning(table, positions, n_tok, dev):
+    """Pointers of positions and turns, the amplitude and the turned elements (table None: no rotation)."""
+    if table is None:
+        return 0, 0, 1.0, 0
+    if positions is None:
+        raise ValueError("positions are required with a table")
+    _need_i32(n_tok, "positions", positions)
+    _on_device(dev, positions, table.turns)
+    return positions.data_ptr(), table.turns.data_ptr(), table.amplitude, table.rot_dim
+
+
+def _sides(q, k):
+    """Tokens and head size of the rows of a call, either of which may be None."""
+    one = q if q is not None else k
+    if one is None:
+        raise ValueError("q or k is required")
+    if one.dim() != 3 or (k is not None and k.dim() != 3):
+        raise ValueError("q and k must be [tokens][heads][head_dim]")
+    n_tok, _, hd = one.shape
+    if k is not None and (k.shape[0] != n_tok or k.shape[2] != hd):
+        raise ValueError(f"k must be [{n_tok}][heads][{hd}]")
+    return one, n_tok, hd
+
+
+def norm_rope(q, k, q_weight, k_weight, positions, table: RopeTable | None, *, eps=1e-6, layout="half", q_out=None,
+              k_out=None, stream=None) -> None:
+    """Norms of the heads of q and k (fp16 [tokens][heads][head_dim], views into a fused projection buffer among
+    them; either may be None), x * weight / sqrt(mean(x^2) + eps) with fp32 weights [head_dim] (None: ones), then
+    the rotation by `positions` (table None: none), into q_out / k_out, or in place where these are None."""
+    if (q is None and q_out is not None) or (k is None and k_out is not None):
+        raise ValueError("an output without its input")
+    one, n_tok, hd = _sides(q, k)
+    dev = _run_device(stream, one)
+    sides, heads = [], []
+    for x, out, w, what in ((q, q_out, q_weight, "q"), (k, k_out, k_weight, "k")):
+        if x is None:
+            sides += [0, 0, 0, 0, 0]
+            heads.append(0)
+            continue
+        at = _rows3(x, what, dev, x.shape)
+        sides += [*at, *(_rows3(out, what + "_out", dev, x.shape) if out is not None else at),
+                  _head_weight(w, hd, what + "_weight", dev)]
+        heads.append(x.shape[1])
+    pos, turns, amp, rot = _turning(table, positions, n_tok, dev)
+    check(lib().qkv_norm_rope(*sides, float(eps), pos, turns, amp, n_tok, *heads, hd, rot, _rope_layout(layout),
+                              _raw_stream(stream, dev)), "qkv_norm_rope")
+
+
+def norm_rope_grad_workspace(n_tok, num_q, num_k, head_dim, device) -> torch.Tensor:
+    """Workspace of norm_rope_grad for up to these numbers."""
+    n = int(lib().qkv_norm_rope_grad_workspace_bytes(n_tok, num_q, num_k, head_dim))
+    if n == 0:
+        raise ValueError(f"no call of these numbers: n_tok {n_tok}, num_q {num_q}, num_k {num_k}, head_dim {head_dim}")
+    return torch.empty(n, dtype=torch.uint8, device=device)
+
+
+def norm_rope_grad(q, k, dq, dk, q_weight, k_weight, positions, table: RopeTable | None, q_weight_grad=None,
+                   k_weight_grad=None, *, eps=1e-6, layout="half", q_grad=None, k_grad=None, workspace=None,
+                   stream=None) -> None:
+    """The gradient of norm_rope at its inputs q and k: dq and dk, the gradients of its outputs, become those of
+    its inputs, in q_grad / k_grad or in place, and q_weight_grad / k_weight_grad (fp32 [head_dim], None: not
+    wanted) those of the weights.  workspace: norm_rope_grad_workspace's (allocated here when None)."""
+    one, n_tok, hd = _sides(q, k)
+    dev = _run_device(stream, one)
+    sides, heads = [], []
+    for x, dy, dx, w, dw, what in ((q, dq, q_grad, q_weight, q_weight_grad, "q"), (k, dk, k_grad, k_weight, k_weight_grad, "k")):
+        if x is None:
+            if dy is not None or dx is not None or dw is not None:
+                raise ValueError(f"a gradient of {what} without {what}")
+            sides += [0] * 8
+            heads.append(0)
+            continue
+        if dy is None:
+            raise ValueError(f"d{what} is required")
+        at = _rows3(dy, "d" + what, dev, x.shape)
+        sides += [*_rows3(x, what, dev, x.shape), *at,
+                  *(_rows3(dx, what + "_grad", dev, x.shape) if dx is not None else at),
+                  _head_weight(w, hd, what + "_weight", dev), _head_weight(dw, hd, what + "_weight_grad", dev)]
+        heads.append(x.shape[1])
+    pos, turns, amp, rot = _turning(table, positions, n_tok, dev)
+    L = lib()
+    if workspace is None:
+        workspace = _scratch(int(L.qkv_norm_rope_grad_workspace_bytes(n_tok, *heads, hd)), one.device, stream)
+    _on_device(dev, workspace)
+    check(L.qkv_norm_rope_grad(*sides, float(eps), pos, turns, amp, n_tok, *heads, hd, rot, _rope_layout(layout),
+                               workspace.data_ptr(), workspace.nbytes, _raw_stream(stream, dev)), "qkv_norm_rope_grad")
+
+
+# ---------------------------------------------------------------------------
 # paged 8-bit cache: e4m3 codes, an exponent per page and kv head
 # ---------------------------------------------------------------------------
 
