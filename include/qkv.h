@@ -683,6 +683,17 @@ int qkv_pages_reserve(int32_t* block_tables, int n_slots, int max_blocks, int bl
                       int32_t* status, const qkv_page_plane* planes, int n_planes,
                       int32_t* scratch, size_t scratch_bytes, hipStream_t stream);
 
+/* slots[i] gets what parents[i] held at the call: the pages of its first n_tokens[i] tokens, shared (those that it
+ * had are given back), and its row of every state plane (`states`: a HOST array like planes, page_bytes the bytes
+ * of a slot's row, rows [n_slots]: token histories, recurrent states; may be NULL with n_states 0).  As after a
+ * beam search step: parents may be slots of the call, in any permutation, the same one many times, or
+ * the slot itself.  n <= 1024.  A table entry past the pool is carried over and not counted.  A parent outside
+ * [0, n_slots), as that of a candidate that is none, is QKV_ERR_INVALID.  Writing a page that is shared
+ * afterwards takes qkv_pages_reserve first. */
+int qkv_pages_reorder(int32_t* block_tables, int n_slots, int max_blocks, int block_tokens, int32_t* ref_counts,
+                      int n_pages, const int32_t* slots, const int32_t* parents, const int32_t* n_tokens, int n,
+                      int32_t* status, const qkv_page_plane* states, int n_states, hipStream_t stream);
+
 /* Copies page pairs[2i] to page pairs[2i+1] in every plane (device int32; a pair
  * with an index outside [0, n_pages) is left out).  No page is the target of two
  * pairs, or target and source. */
@@ -697,6 +708,28 @@ int qkv_pages_copy(const qkv_page_plane* planes, int n_planes, int n_pages, cons
 int qkv_pages_compact(int32_t* block_tables, int n_slots, int max_blocks, int32_t* ref_counts,
                       int n_pages, int32_t* moved, int32_t* n_used, const qkv_page_plane* planes,
                       int n_planes, int32_t* scratch, size_t scratch_bytes, hipStream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * Beam search.  No counterpart in the reference.
+ * ------------------------------------------------------------------------- */
+typedef enum qkv_logits_type { QKV_LOGITS_F16 = 0, QKV_LOGITS_F32 = 1, QKV_LOGITS_BF16 = 2 } qkv_logits_type;
+
+/* The `take` best continuations of each of n requests over its `beams` beams and the vocabulary:
+ *   S(b, v) = scores[b] + logits[b][v] - log(sum_u exp(logits[b][u])),
+ * largest first, ties to the lowest beam, then token.  logits: [n * beams][vocab] with `stride` elements between
+ * rows, of any alignment (read by whole 16-byte words: up to 15 bytes before and past a row must be there to
+ * read, as any allocation's are).  A logit of NaN or +infinity counts as -infinity, which is no candidate.
+ * scores: device fp32 [n * beams]; a beam of -infinity or NaN offers nothing (before the first step all beams of
+ * a request but one).  done (device int32 [n * beams], NULL: none): a beam with a nonzero entry has ended, its
+ * logits are not read, and it offers end_token at its own score.  parents, tokens, top_scores [n][take]: the
+ * logits row of the beam (request * beams + b), the token and S as fp32; -1, -1 and -infinity where there are
+ * fewer candidates.  S is compared in 64 bits.  beams, take <= 64, beams * vocab < 2^31, n * beams <= 2^24
+ * (QKV_ERR_UNSUPPORTED).  workspace: qkv_beam_select_workspace_bytes of these numbers or larger ones, aligned to 8
+ * bytes (no initialisation needed). */
+size_t qkv_beam_select_workspace_bytes(int n, int beams, int vocab, int take);
+int qkv_beam_select(const void* logits, int logits_type, long stride, const float* scores, const int32_t* done,
+                    int end_token, int n, int beams, int vocab, int take, int32_t* parents, int32_t* tokens,
+                    float* top_scores, void* workspace, size_t workspace_bytes, hipStream_t stream);
 
 #ifdef __cplusplus
 }

@@ -104,6 +104,9 @@ SIGNATURES = {
     "qkv_pages_release": (_I, [_P, _I, _I, _I, _P, _I, _P, _P, _I, _P, _P]),
     "qkv_pages_reserve_scratch_bytes": (_SZ, [_I, _I, _I]),
     "qkv_pages_reserve": (_I, [_P, _I, _I, _I, _P, _I, _P, _P, _P, _I, _I, _P, _P, _I, _P, _SZ, _P]),
+    "qkv_pages_reorder": (_I, [_P, _I, _I, _I, _P, _I, _P, _P, _P, _I, _P, _P, _I, _P]),
+    "qkv_beam_select_workspace_bytes": (_SZ, [_I, _I, _I, _I]),
+    "qkv_beam_select": (_I, [_P, _I, _L, _P, _P, _I, _I, _I, _I, _I, _P, _P, _P, _P, _SZ, _P]),
     "qkv_pages_copy": (_I, [_P, _I, _I, _P, _I, _P]),
     "qkv_pages_compact": (_I, [_P, _I, _I, _P, _I, _P, _P, _P, _I, _P, _SZ, _P]),
     "qkv_prefill_attn_tq3": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _F, _P, _SZ, _P]),

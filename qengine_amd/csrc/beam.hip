@@ -1,0 +1,456 @@
+// beam.hip -- beam search's selection over beams and vocabulary.
+//
+//   S(b, v) = s_b + x_bv - log(sum_u exp(x_bu)),  the `take` largest of a request, ties to the lowest (b, v)
+//
+// The logits are read once: a workgroup takes a segment of one row, holds it in registers, sums its
+// exponentials and keeps its `take` largest logits; a second launch joins a request's segments.  Inside a
+// row the order of S is that of x, so segments compare the logits themselves, without a rounding.
+//
+// The exponentials are taken in base 2 of the distance to the segment's maximum (exact for 16-bit logits),
+// times log2(e) as two floats: their error stays near their own rounding, where a product of the logit and one
+// float would be off by a common factor of x 2^-24.  Sums of segments are joined, and scores formed, in 64
+// bits, so that beams compare to about 2^-24.
+#include <algorithm>
+#include <type_traits>
+
+#include "qkv_device.h"
+#include "qkv_launch.h"
+
+namespace qkv {
+
+namespace {
+
+constexpr float kLog2eHi = 1.44269502162933349609375f;   // log2(e) to 24 bits, and what is left of it
+constexpr float kLog2eLo = 1.925963033500011e-8f;
+constexpr int kCap = 512;                                // candidates of a workgroup in LDS
+
+// v of the lane that steps 1, 2, 7, 15 (mirrored in its quad, half row and row), 16 and 32 pair this one with
+template <int STEP>
+__device__ __forceinline__ float pair_of(float v) {
+  if constexpr (STEP < 16) {
+    constexpr int ctrl = STEP == 1 ? 0xb1 : STEP == 2 ? 0x4e : STEP == 7 ? 0x141 : 0x140;
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), ctrl, 0xf, 0xf, true));
+  } else {
+    const uint32_t b = __float_as_uint(v);
+    const auto s = STEP == 16 ? __builtin_amdgcn_permlane16_swap(b, b, false, false)
+                              : __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    return __uint_as_float(((threadIdx.x & STEP) != 0) ? s[0] : s[1]);
+  }
+}
+template <int STEP>
+__device__ __forceinline__ double pair_of(double v) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint64_t lo = __float_as_uint(pair_of<STEP>(__uint_as_float((uint32_t)b)));
+  const uint64_t hi = __float_as_uint(pair_of<STEP>(__uint_as_float((uint32_t)(b >> 32))));
+  return __builtin_bit_cast(double, hi << 32 | lo);
+}
+template <class V>
+__device__ __forceinline__ V larger(V a, V b) { return b > a ? b : a; }
+template <class V>
+__device__ __forceinline__ V wave_max(V v) {   // (no NaN)
+  v = larger(v, pair_of<1>(v));
+  v = larger(v, pair_of<2>(v));
+  v = larger(v, pair_of<7>(v));
+  v = larger(v, pair_of<15>(v));
+  v = larger(v, pair_of<16>(v));
+  return larger(v, pair_of<32>(v));
+}
+__device__ __forceinline__ float wave_sum(float v) {
+  v += pair_of<1>(v);
+  v += pair_of<2>(v);
+  v += pair_of<7>(v);
+  v += pair_of<15>(v);
+  v += pair_of<16>(v);
+  return v + pair_of<32>(v);
+}
+
+template <class V>
+struct Found {   // candidates of a workgroup: values and what they stand for
+  V v[kCap];
+  int at[kCap];
+  V low[4];
+  int n;
+};
+
+template <class V>
+__device__ __forceinline__ bool better(V a, int ia, V b, int ib) { return a > b || (a == b && ia < ib); }
+
+// The k <= 64 largest of what the 256 threads hold, ties to the lowest index, as put(rank, value, index) by
+// any thread; returns how many there are (at most k).  `top` is this thread's largest, each(f, low) calls
+// f(value, index) for at least those of its values that are >= low; -infinity is no value.
+//
+// At least k threads hold a value >= the smallest, over the four waves, of the (k + 3) / 4-th largest of the
+// lanes' maxima (and >= the k-th largest of any one wave's, which counts where another wave has too few).  What
+// is at or above that goes to LDS, usually a few times k, and is ranked there by counting.  Where more values
+// tie than LDS holds, they are found one after the other.
+template <class V, class Each, class Put>
+__device__ __forceinline__ int top_of_group(Found<V>& found, int k, V top, Each&& each, Put&& put) {
+  const V none = -INFINITY;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  V mine = top, low = none;
+  auto next = [&](int from, int to) {   // the to-th largest, after `from` of them
+    for (int i = from; i < to; i++) {
+      low = wave_max(mine);
+      const uint64_t m = __builtin_amdgcn_ballot_w64(mine == low);
+      if (m && lane == (int)__builtin_ctzll(m)) mine = none;
+    }
+    if (lane == 0) found.low[wave] = low;
+  };
+  next(0, (k + 3) / 4);
+  if (tid == 0) found.n = 0;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 4; w++) low = found.low[w] < low ? found.low[w] : low;
+  if (low == none) {   // (the same in every wave)
+    __syncthreads();
+    next((k + 3) / 4, k);
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 4; w++) low = found.low[w] > low ? found.low[w] : low;
+  }
+  if (top >= low)
+    each([&](V v, int at) __attribute__((always_inline)) {
+      if (v >= low && v > none) {
+        const int i = atomicAdd(&found.n, 1);
+        if (i < kCap) {
+          found.v[i] = v;
+          found.at[i] = at;
+        }
+      }
+    }, low);
+  __syncthreads();
+  const int n = found.n;
+  if (n <= kCap) {
+    for (int i = tid; i < n; i += 256) {
+      const V v = found.v[i];
+      const int at = found.at[i];
+      int rank = 0;
+      for (int j = 0; j < n; j++) rank += better(found.v[j], found.at[j], v, at);
+      if (rank < k) put(rank, v, at);
+    }
+    return min(n, k);
+  }
+  V last = INFINITY;
+  int last_at = -1;
+  for (int r = 0; r < k; r++) {
+    V best = none;
+    int best_at = 0x7fffffff;
+    each([&](V v, int at) __attribute__((always_inline)) {
+      if (better(last, last_at, v, at) && better(v, at, best, best_at)) {
+        best = v;
+        best_at = at;
+      }
+    }, none);
+#pragma unroll
+    for (int d = 32; d; d >>= 1) {
+      const V v = __shfl_xor(best, d);
+      const int at = __shfl_xor(best_at, d);
+      if (better(v, at, best, best_at)) {
+        best = v;
+        best_at = at;
+      }
+    }
+    __syncthreads();   // (the entries are read by the step before)
+    if (lane == 0) {
+      found.v[wave] = best;
+      found.at[wave] = best_at;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 4; w++)
+      if (better(found.v[w], found.at[w], best, best_at)) {
+        best = found.v[w];
+        best_at = found.at[w];
+      }
+    if (best == none) return r;
+    if (tid == 0) put(r, best, best_at);
+    last = best;
+    last_at = best_at;
+  }
+  return k;
+}
+
+// Logits of one 16-byte word
+template <int TYPE>
+struct Word;
+template <>
+struct Word<0> {   // fp16
+  static constexpr int N = 8;
+  static constexpr uint32_t kNone = 0xfc00u;
+  __device__ static __forceinline__ float at(u4_t w, int i) { return h2f(i & 1 ? w[i >> 1] >> 16 : w[i >> 1] & 0xffffu); }
+};
+template <>
+struct Word<1> {   // fp32
+  static constexpr int N = 4;
+  static constexpr uint32_t kNone = 0xff800000u;
+  __device__ static __forceinline__ float at(u4_t w, int i) { return __uint_as_float(w[i]); }
+};
+template <>
+struct Word<2> {   // bf16
+  static constexpr int N = 8;
+  static constexpr uint32_t kNone = 0xff80u;
+  __device__ static __forceinline__ float at(u4_t w, int i) {
+    return __uint_as_float(i & 1 ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16);
+  }
+};
+// NaN and +infinity to -infinity
+template <int TYPE>
+__device__ __forceinline__ void leave_out(u4_t& w) {
+  using W = Word<TYPE>;
+#pragma unroll
+  for (int i = 0; i < W::N; i++) {
+    if (W::at(w, i) < INFINITY) continue;
+    if constexpr (W::N == 8) w[i >> 1] = (w[i >> 1] & (i & 1 ? 0xffffu : 0xffff0000u)) | (i & 1 ? W::kNone << 16 : W::kNone);
+    else w[i] = W::kNone;
+  }
+}
+
+__device__ __forceinline__ bool searched(const BeamArgs& p, long row) {   // a beam whose logits count
+  return p.scores[row] > -INFINITY && !(p.done && p.done[row]);
+}
+
+}  // namespace
+
+// A workgroup takes NV words a thread of a row.  Rows need not be aligned: words are, and what they hold
+// outside the row is left out.
+template <int TYPE, int NV>
+__global__ __launch_bounds__(256, 4) void beam_rows_kernel(BeamArgs p) {
+  using W = Word<TYPE>;
+  constexpr int SIZE = 16 / W::N;
+  __shared__ Found<float> found;
+  __shared__ float part[4], sums[4];
+  const long wg = (long)blockIdx.y * kGridX + blockIdx.x;
+  if (wg >= (long)p.rows * p.segments) return;
+  const long row = wg / p.segments;
+  const int seg = (int)(wg - row * p.segments), tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  if (!searched(p, row)) return;
+  const uintptr_t addr = reinterpret_cast<uintptr_t>(p.logits) + (uintptr_t)(row * p.stride) * SIZE;
+  const u4_t* words = reinterpret_cast<const u4_t*>(addr & ~(uintptr_t)15);
+  const int skip = (int)(addr & 15) / SIZE;   // elements of the first word ahead of the row
+  const long w0 = (long)seg * (256 * NV), end = (long)p.vocab + skip;
+  u4_t raw[NV];
+#pragma unroll
+  for (int j = 0; j < NV; j++) {
+    const long e = (w0 + 256 * j + tid) * W::N;
+    if (e < end) {
+      raw[j] = __builtin_nontemporal_load(words + w0 + 256 * j + tid);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; i++) raw[j][i] = SIZE == 2 ? W::kNone * 0x10001u : W::kNone;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < NV; j++) {
+    const long e = (w0 + 256 * j + tid) * W::N;
+    if (e < skip || (e < end && e + W::N > end)) {
+#pragma unroll
+      for (int i = 0; i < W::N; i++)
+        if (e + i < skip || e + i >= end) {
+          if constexpr (SIZE == 2) {
+            const uint32_t keep = i & 1 ? 0xffffu : 0xffff0000u;
+            raw[j][i >> 1] = (raw[j][i >> 1] & keep) | (i & 1 ? W::kNone << 16 : W::kNone);
+          } else {
+            raw[j][i] = W::kNone;
+          }
+        }
+    }
+  }
+  // Logits that are left out show in the maximum (+infinity) or in the sum (NaN): only then are all looked at.
+  float tops[NV], top;
+  auto look = [&]() __attribute__((always_inline)) {
+    top = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+      tops[j] = -INFINITY;   // (fmaxf leaves a NaN out)
+#pragma unroll
+      for (int i = 0; i < W::N; i += 2) tops[j] = fmaxf(fmaxf(tops[j], W::at(raw[j], i)), W::at(raw[j], i + 1));
+      top = fmaxf(top, tops[j]);
+    }
+    return wave_max(top);
+  };
+  auto clean = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < NV; j++) leave_out<TYPE>(raw[j]);
+    return look();
+  };
+  float wmax = look();
+  if (wmax == INFINITY) wmax = clean();
+  if (lane == 0) part[wave] = wmax;
+  __syncthreads();
+  const float m = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])), ref = m == -INFINITY ? 0.f : m;
+  auto add = [&]() __attribute__((always_inline)) {
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+      asm("" : "+v"(raw[j]));   // (converted again, not held as floats)
+#pragma unroll
+      for (int i = 0; i < W::N; i++) {
+        const float t = W::at(raw[j], i) - ref;
+        sum[i & 3] += __builtin_amdgcn_exp2f(__builtin_fmaf(t, kLog2eLo, t * kLog2eHi));
+      }
+    }
+    return wave_sum((sum[0] + sum[1]) + (sum[2] + sum[3]));
+  };
+  float l = add();
+  if (l != l) {
+    clean();
+    l = add();
+  }
+  if (lane == 0) sums[wave] = l;
+  const long rec = wg * p.take;
+  const int token0 = (int)(w0 * W::N - skip);
+  const int n = top_of_group<float>(found, p.take, top, [&](auto&& f, float low) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < NV; j++)
+      if (tops[j] >= low) {
+        u4_t w = raw[j];
+        int at = token0 + (256 * j + tid) * W::N;
+        asm volatile("" : "+v"(w), "+v"(at));   // (formed here: ahead of a loop they would fill the registers)
+#pragma unroll
+        for (int i = 0; i < W::N; i++) f(W::at(w, i), at + i);
+      }
+  }, [&](int rank, float v, int at) {
+    p.rec_x[rec + rank] = v;
+    p.rec_at[rec + rank] = at;
+  });
+  for (int i = n + tid; i < p.take; i += 256) p.rec_x[rec + i] = -INFINITY;
+  if (tid == 0) {   // (the sums were written ahead of a barrier in the selection)
+    p.rec_sum[2 * wg] = m;
+    p.rec_sum[2 * wg + 1] = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+  }
+}
+
+// A request's segments: every beam's logarithm of its sum, then the largest scores of what is left, RPT
+// records a thread at a time together with the best of those before.
+template <int RPT>
+__global__ __launch_bounds__(256) void beam_join_kernel(BeamArgs p) {
+  __shared__ Found<double> found;
+  __shared__ double most[kMaxBeams], log_sum[kMaxBeams], best[kMaxTake];
+  __shared__ int best_at[kMaxTake];
+  __shared__ float score[kMaxBeams];
+  __shared__ int state[kMaxBeams];   // 0: not alive, 1: searched, 2: done
+  const long req = blockIdx.x, row0 = req * p.beams;
+  const int tid = threadIdx.x, S = p.segments, k = p.take;
+  const int per = S * k, total = p.beams * per;
+  const float* rec_x = p.rec_x + row0 * per;
+  const int32_t* rec_at = p.rec_at + row0 * per;
+  float x[RPT];
+  int at[RPT];
+  // Of 256 records each wave takes 16 from every quarter: the wave's best, which bound what is looked at, are
+  // then not those of one beam.
+  const int mine = (tid & 3) * 64 + (tid >> 2);
+  auto load = [&](int x0) {   // (records of beams that are not searched hold anything)
+#pragma unroll
+    for (int i = 0; i < RPT; i++) {
+      const int r = min(x0 + 256 * i + mine, total - 1);
+      x[i] = rec_x[r];
+      at[i] = rec_at[r];
+    }
+  };
+  load(0);
+  // 4 lanes a beam or more
+  const int lanes = p.beams <= 4 ? 64 : p.beams <= 8 ? 32 : p.beams <= 16 ? 16 : p.beams <= 32 ? 8 : 4;
+  const int b = tid / lanes, part = tid % lanes;
+  if (b < p.beams) {
+    const long row = row0 + b;
+    const float2* rec = reinterpret_cast<const float2*>(p.rec_sum) + row * S;
+    const float2 one = rec[min(part, S - 1)];
+    const float s = p.scores[row];
+    const int over = p.done ? p.done[row] : 0;
+    const bool alive = s > -INFINITY;
+    float m = part < S ? one.x : -INFINITY;
+    for (int i = part + lanes; i < S; i += lanes) m = fmaxf(m, rec[i].x);
+    for (int d = lanes / 2; d; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
+    double l = 0.0;
+    for (int i = part; i < S; i += lanes) {
+      const float2 r = i == part ? one : rec[i];
+      l += r.x == m ? (double)r.y : (double)r.y * exp((double)r.x - (double)m);
+    }
+    for (int d = lanes / 2; d; d >>= 1) l += __shfl_xor(l, d);
+    if (part == 0) {
+      score[b] = s;
+      state[b] = !alive ? 0 : over ? 2 : 1;
+      most[b] = (double)m;
+      log_sum[b] = log(l);   // (no logit: no record's value is one)
+    }
+  }
+  __syncthreads();
+  int n = 0;
+  for (int x0 = 0; x0 < total; x0 += 256 * RPT) {
+    if (x0 > 0) load(x0);
+    // scores (-infinity: none) and, in one whole number, beam and token
+    double v[RPT + 1], top = -INFINITY;
+    int id[RPT + 1];
+    v[RPT] = tid < n ? best[tid] : -INFINITY;
+    id[RPT] = tid < n ? best_at[tid] : 0;
+#pragma unroll
+    for (int i = 0; i < RPT; i++) {
+      const int r = x0 + 256 * i + mine, bi = min(r, total - 1) / per;
+      const int st = r < total ? state[bi] : 0;
+      v[i] = -INFINITY;
+      id[i] = 0;
+      if (st == 1 && x[i] > -INFINITY) {
+        v[i] = (double)score[bi] + (((double)x[i] - most[bi]) - log_sum[bi]);
+        id[i] = bi * p.vocab + at[i];
+      }
+      if (st == 2 && r == bi * per) {
+        v[i] = (double)score[bi];
+        id[i] = bi * p.vocab + p.end_token;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i <= RPT; i++) top = larger(top, v[i]);
+    auto each = [&](auto&& f, double) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i <= RPT; i++) f(v[i], id[i]);
+    };
+    n = top_of_group<double>(found, k, top, each, [&](int rank, double value, int what) {
+      best[rank] = value;
+      best_at[rank] = what;
+    });
+    __syncthreads();
+  }
+  for (int i = tid; i < k; i += 256) {
+    const int bi = i < n ? best_at[i] / p.vocab : -1;
+    p.parents[req * k + i] = i < n ? (int)(row0 + bi) : -1;
+    p.tokens[req * k + i] = i < n ? best_at[i] - bi * p.vocab : -1;
+    p.top[req * k + i] = i < n ? (float)best[i] : -INFINITY;
+  }
+}
+
+// 16-byte words of a thread: few where few rows leave workgroups idle, unless a request's records then
+// outgrow what its join holds at a time.
+BeamPlan beam_plan(long rows, int beams, int vocab, int take, int type, bool whole) {
+  const int n = type == 1 ? 4 : 8;
+  BeamPlan x{8, 0};
+  for (int nv : {1, 4, 8}) {
+    x.words = nv;
+    // (a row that does not begin with a word holds up to n - 1 elements of another)
+    x.segments = (int)(((long)vocab + (whole ? 0 : n - 1) + 256L * nv * n - 1) / (256L * nv * n));
+    if (rows * x.segments <= kBeamGroups && (long)beams * x.segments * take <= kBeamRecords) break;
+  }
+  return x;
+}
+
+hipError_t launch_beam(BeamArgs a, const BeamPlan& plan, int type, hipStream_t stream) {
+  a.segments = plan.segments;
+  const dim3 grid = grid_xy((long)a.rows * a.segments), block(256), requests((unsigned)(a.rows / a.beams));
+  auto launch = [&](auto t) {
+    constexpr int T = decltype(t)::value;
+    switch (plan.words) {
+      case 1: hipLaunchKernelGGL((beam_rows_kernel<T, 1>), grid, block, 0, stream, a); break;
+      case 4: hipLaunchKernelGGL((beam_rows_kernel<T, 4>), grid, block, 0, stream, a); break;
+      default: hipLaunchKernelGGL((beam_rows_kernel<T, 8>), grid, block, 0, stream, a); break;
+    }
+  };
+  if (type == 0) launch(std::integral_constant<int, 0>{});
+  else if (type == 1) launch(std::integral_constant<int, 1>{});
+  else launch(std::integral_constant<int, 2>{});
+  if ((long)a.beams * a.segments * a.take <= 1024)
+    hipLaunchKernelGGL(beam_join_kernel<4>, requests, block, 0, stream, a);
+  else
+    hipLaunchKernelGGL(beam_join_kernel<16>, requests, block, 0, stream, a);
+  return hipGetLastError();
+}
+
+}  // namespace qkv

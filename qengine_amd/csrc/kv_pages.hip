@@ -312,6 +312,152 @@ hipError_t launch_pages_reserve(const PageTables& t, const int32_t* slots, const
   return hipGetLastError();
 }
 
+// ---- reorder ---------------------------------------------------------------
+// Slots take over what their parents held, any of which may be slots of the call: a permutation with copies,
+// in place.  A workgroup takes a band of columns (entries of the tables, or 16, 4 or 1 bytes of a state
+// plane) of all n rows, holds it in registers and writes it when all of it has been read, so no second
+// copy of a row is needed and no workgroup waits for another.
+constexpr int kBandUnits = 8;   // of a thread
+
+// W = 2^w_log columns a band, n * W <= 1024 * kBandUnits.
+template <class T>
+__device__ __forceinline__ void move_band(uint8_t* base, uint64_t row_bytes, long col0, long cols, int w_log, int n,
+                                          const int* slot, const int* parent) {
+  T v[kBandUnits];
+  // row (-1: nothing to do) and column of a thread's unit u
+  auto place = [&](int u, bool to, int& row) {
+    const int x = (int)threadIdx.x + 1024 * u, i = min(x >> w_log, n - 1);
+    const long col = col0 + (x & ((1 << w_log) - 1));
+    const int s = slot[i], p = parent[i];
+    const bool moves = (x >> w_log < n) & (col < cols) & (s >= 0) & (s != p);
+    row = moves ? (to ? s : p) : -1;
+    return reinterpret_cast<T*>(base + (uint64_t)max(row, 0) * row_bytes) + (moves ? col : 0);
+  };
+#pragma unroll
+  for (int u = 0; u < kBandUnits; u++) {   // (one that has nothing to do reads row 0: no branch)
+    int row;
+    v[u] = *place(u, false, row);
+  }
+  // (every thread's reads have returned before any thread writes)
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < kBandUnits; u++) {
+    int row;
+    T* to = place(u, true, row);
+    if (row >= 0) *to = v[u];
+  }
+}
+
+__global__ __launch_bounds__(1024) void pages_reorder_kernel(PageTables t, const int32_t* slots, const int32_t* parents,
+                                                             const int32_t* tokens, int n, int32_t* status,
+                                                             PageStatus c, PagePlanes states, int w_log,
+                                                             int table_bands, long bands) {
+  __shared__ __align__(16) int slot_s[kReorderMax];
+  __shared__ int parent_s[kReorderMax], blocks_s[kReorderMax], owner[2 * kReorderMax];
+  const int tid = threadIdx.x;
+  slot_s[tid] = tid < n ? slots[tid] : -1;
+  owner[tid] = owner[tid + kReorderMax] = kReorderMax;
+  __syncthreads();
+  // the first in the list of the slots of one remainder: only an entry behind it may name a slot again
+  const int hash = slot_s[tid] & (2 * kReorderMax - 1);
+  if (tid < n) atomicMin(&owner[hash], tid);
+  __syncthreads();
+  bool bad = tid >= n;
+  if (tid < n) {
+    const int slot = slot_s[tid], parent = parents[tid], tok = tokens[tid];
+    const int nb = tok >= 0 ? blocks_of(tok, t.block_tokens) : 0;
+    bad = slot < 0 || slot >= t.n_slots || parent < 0 || parent >= t.n_slots || tok < 0 || nb > t.max_blocks;
+    for (int j = 0; owner[hash] < tid && j < tid; j += 4) {   // named before in the list
+      const int4 s = *reinterpret_cast<const int4*>(slot_s + j);
+      bad |= s.x == slot || (j + 1 < tid && s.y == slot) || (j + 2 < tid && s.z == slot) || (j + 3 < tid && s.w == slot);
+    }
+    parent_s[tid] = parent;
+    blocks_s[tid] = nb;
+    if (blockIdx.x == 0 && blockIdx.y == 0 && status) status[tid] = bad ? c.invalid : c.ok;
+  }
+  __syncthreads();
+  if (bad) slot_s[tid] = -1;
+  __syncthreads();
+  // Neighbouring bands on one XCD: rows lie at one stride, often a power of two, and every eighth band alone
+  // would meet in a few channels of that XCD's cache (512 rows of 262,144 bytes: 2,970 us).
+  long band = (long)blockIdx.y * kGridX + blockIdx.x;
+  const long eighth = bands / 8;
+  if (band < 8 * eighth) band = band % 8 * eighth + band / 8;
+  if (band < table_bands) {
+    const long col0 = band << w_log;
+    int now[kBandUnits], was[kBandUnits];
+    auto place = [&](int u, int& i, long& col) {
+      const int x = tid + 1024 * u;
+      i = min(x >> w_log, n - 1);
+      col = col0 + (x & ((1 << w_log) - 1));
+      const bool mine = (x >> w_log < n) & (col < t.max_blocks) & (slot_s[i] >= 0);
+      if (!mine) col = -1;
+      return mine;
+    };
+#pragma unroll
+    for (int u = 0; u < kBandUnits; u++) {
+      int i;
+      long col;
+      const bool mine = place(u, i, col), has = mine & (col < blocks_s[i]);
+      was[u] = t.tables[mine ? (long)slot_s[i] * t.max_blocks + col : 0];
+      now[u] = t.tables[has ? (long)parent_s[i] * t.max_blocks + col : 0];
+      now[u] = has ? max(now[u], -1) : -1;
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < kBandUnits; u++) {
+      int i;
+      long col;
+      if (place(u, i, col) && now[u] != was[u]) {
+        t.tables[(long)slot_s[i] * t.max_blocks + col] = now[u];
+        if (now[u] >= 0 && now[u] < t.n_pages) atomicAdd(t.refs + now[u], 1);
+        if (was[u] >= 0 && was[u] < t.n_pages) atomicSub(t.refs + was[u], 1);
+      }
+    }
+    return;
+  }
+  band -= table_bands;
+  uint8_t* base = nullptr;
+  uint64_t bytes = 0;
+  int unit = 0;
+  long cols = 0;
+  for (int k = 0; k < states.n; k++) {
+    const uint64_t align = reinterpret_cast<uintptr_t>(states.base[k]) | states.bytes[k];
+    base = states.base[k];
+    bytes = states.bytes[k];
+    unit = (align & 15) == 0 ? 16 : (align & 3) == 0 ? 4 : 1;
+    cols = (long)(bytes / unit);
+    const long here = (cols + (1 << w_log) - 1) >> w_log;
+    if (band < here) break;
+    band -= here;
+    unit = 0;
+  }
+  const long col0 = band << w_log;
+  if (unit == 16) move_band<u4_t>(base, bytes, col0, cols, w_log, n, slot_s, parent_s);
+  else if (unit == 4) move_band<uint32_t>(base, bytes, col0, cols, w_log, n, slot_s, parent_s);
+  else if (unit == 1) move_band<uint8_t>(base, bytes, col0, cols, w_log, n, slot_s, parent_s);
+}
+
+hipError_t launch_pages_reorder(const PageTables& t, const int32_t* slots, const int32_t* parents,
+                                const int32_t* tokens, int n, int32_t* status, const PageStatus& codes,
+                                const PagePlanes& states, hipStream_t stream) {
+  int w_log = 0;
+  while (w_log < 8 && n << (w_log + 1) <= 1024 * kBandUnits) w_log++;
+  const long w = 1 << w_log;
+  const int table_bands = (int)((t.max_blocks + w - 1) / w);
+  long bands = table_bands;
+  for (int k = 0; k < states.n; k++) {
+    const uint64_t align = reinterpret_cast<uintptr_t>(states.base[k]) | states.bytes[k];
+    const long cols = (long)(states.bytes[k] / ((align & 15) == 0 ? 16 : (align & 3) == 0 ? 4 : 1));
+    bands += (cols + w - 1) / w;
+  }
+  hipLaunchKernelGGL(pages_reorder_kernel, grid_xy(bands), dim3(1024), 0, stream, t, slots, parents, tokens, n,
+                     status, codes, states, w_log, table_bands, bands);
+  return hipGetLastError();
+}
+
 // ---- copy ------------------------------------------------------------------
 __global__ __launch_bounds__(256) void pages_copy_kernel(PagePlanes planes, const int32_t* pairs, int n, int n_pages,
                                                          int chunks) {

@@ -189,7 +189,7 @@ __global__ __launch_bounds__(256) void norm_rope_any_kernel(NormRopeArgs p) {
 // group in turn HPT heads of a token.  A lane's elements are the same in all of its rows, so its part of
 // dw stays in 16 registers; a workgroup's is summed through LDS and stored once.
 template <int LPR, int HPT>
-__global__ __launch_bounds__(256) void norm_rope_grad_kernel(NormRopeArgs p) {
+__global__ __launch_bounds__(256, 3) void norm_rope_grad_kernel(NormRopeArgs p) {
   constexpr int GROUPS = 256 / LPR, HD = 16 * LPR;
   __shared__ float part[GROUPS * HD];   // 16 KB
   const int tid = threadIdx.x, c = tid % LPR, grp = tid / LPR;
@@ -321,22 +321,36 @@ __global__ __launch_bounds__(256) void norm_rope_grad_any_kernel(NormRopeArgs p)
     p.partial[(long)blockIdx.x * hd + e] = part[0][e] + part[1][e] + part[2][e] + part[3][e];
 }
 
-// dw from the workgroups' sums: 16 columns a workgroup, every 16th partial sum a thread of each.
-__global__ __launch_bounds__(256) void norm_rope_dw_kernel(NormRopeArgs p, int groups) {
-  __shared__ float part[16][17];
+// dw from the workgroups' sums: 16 columns a workgroup, every 64th partial sum a thread of each.
+__global__ __launch_bounds__(1024) void norm_rope_dw_kernel(NormRopeArgs p, int groups) {
+  constexpr int R = 64;
+  __shared__ float part[R][17];
   const bool isq = blockIdx.y == 0;
   float* out = isq ? p.q_dw : p.k_dw;
-  const int c = threadIdx.x & 15, r = threadIdx.x >> 4, e = blockIdx.x * 16 + c;
+  if (!out) return;
+  const int c = threadIdx.x & 15, r = threadIdx.x >> 4, e = min((int)blockIdx.x * 16 + c, p.head_dim - 1);
   const int from = isq ? 0 : p.q_groups, to = isq ? p.q_groups : groups;
   float s = 0.f;
-  if (e < p.head_dim)
-    for (int i = from + r; i < to; i += 16) s += p.partial[(long)i * p.head_dim + e];
+  for (int i0 = from + r; i0 < to; i0 += 8 * R) {
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = p.partial[(long)min(i0 + i * R, to - 1) * p.head_dim + e];
+#pragma unroll
+    for (int i = 0; i < 8; i++) s += i0 + i * R < to ? v[i] : 0.f;
+  }
   part[r][c] = s;
   __syncthreads();
-  if (r == 0 && e < p.head_dim && out) {
+  if (r < 8) {
     s = 0.f;
 #pragma unroll
-    for (int i = 0; i < 16; i++) s += part[i][c];
+    for (int i = 0; i < R / 8; i++) s += part[r + 8 * i][c];
+    part[r][c] = s;
+  }
+  __syncthreads();
+  if (r == 0 && (int)blockIdx.x * 16 + c < p.head_dim) {
+    s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; i++) s += part[i][c];
     out[e] = s;
   }
 }
@@ -382,7 +396,7 @@ hipError_t launch_norm_rope_grad(NormRopeArgs a, bool wide, int groups, hipStrea
     }
   }
   if (a.partial)
-    hipLaunchKernelGGL(norm_rope_dw_kernel, dim3((unsigned)((a.head_dim + 15) / 16), 2), block, 0, stream, a, groups);
+    hipLaunchKernelGGL(norm_rope_dw_kernel, dim3((unsigned)((a.head_dim + 15) / 16), 2), dim3(1024), 0, stream, a, groups);
   return hipGetLastError();
 }
 

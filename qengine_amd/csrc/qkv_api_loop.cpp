@@ -159,4 +159,74 @@ int qkv_norm_rope_grad(const uint16_t* q, long q_stride, const uint16_t* q_dy, l
   return launch_status(qkv::launch_norm_rope_grad(a, wide, norm_grad_groups(n_tok, num_q, num_k), stream));
 }
 
+static int check_beam(int n, int beams, int vocab, int take) {
+  if (n < 0 || beams <= 0 || vocab <= 0 || take <= 0) return QKV_ERR_INVALID;
+  // (beam and token of a request are one whole number of 31 bits; rows are workgroups of a launch)
+  if (beams > qkv::kMaxBeams || take > qkv::kMaxTake || (double)beams * vocab > 2147483647.0 ||
+      (double)n * beams > (double)(1 << 24))
+    return QKV_ERR_UNSUPPORTED;
+  return QKV_OK;
+}
+
+size_t qkv_beam_select_workspace_bytes(int n, int beams, int vocab, int take) {
+  if (n <= 0 || check_beam(n, beams, vocab, take) != QKV_OK) return 0;
+  // rows are cut finer only up to kBeamGroups segments in all: the coarsest cut's, or those
+  const double coarse = (double)n * beams * ((vocab + 3.0) / (256 * 8 * 4) + 1);
+  return (size_t)(std::max(coarse, (double)qkv::kBeamGroups) + 1) * 8 * (take + 1);
+}
+
+int qkv_beam_select(const void* logits, int logits_type, long stride, const float* scores, const int32_t* done,
+                    int end_token, int n, int beams, int vocab, int take, int32_t* parents, int32_t* tokens,
+                    float* top_scores, void* workspace, size_t workspace_bytes, hipStream_t stream) {
+  const int st = check_beam(n, beams, vocab, take);
+  if (st != QKV_OK) return st;
+  if (logits_type < QKV_LOGITS_F16 || logits_type > QKV_LOGITS_BF16) return QKV_ERR_INVALID;
+  if (done && (end_token < 0 || end_token >= vocab)) return QKV_ERR_INVALID;
+  if (n == 0) return QKV_OK;
+  if ((double)n * beams > 1 && stride < vocab) return QKV_ERR_INVALID;
+  if (!logits || !scores || !parents || !tokens || !top_scores) return QKV_ERR_NULL;
+  if (!aligned(logits, logits_type == QKV_LOGITS_F32 ? 4 : 2) || !aligned(scores, 4) || !aligned(done, 4) ||
+      !aligned(parents, 4) || !aligned(tokens, 4) || !aligned(top_scores, 4))
+    return QKV_ERR_ALIGN;
+  if (!workspace || workspace_bytes < qkv_beam_select_workspace_bytes(n, beams, vocab, take)) return QKV_ERR_WORKSPACE;
+  if (!aligned(workspace, 8)) return QKV_ERR_ALIGN;
+  qkv::BeamArgs a{};
+  a.logits = logits;
+  a.scores = scores;
+  a.done = done;
+  a.parents = parents;
+  a.tokens = tokens;
+  a.top = top_scores;
+  a.stride = stride;
+  a.rows = (long)n * beams;
+  a.beams = beams;
+  a.vocab = vocab;
+  a.take = take;
+  a.end_token = end_token;
+  const bool whole = aligned(logits, 16) && (a.rows == 1 || stride * (logits_type == QKV_LOGITS_F32 ? 4 : 2) % 16 == 0);
+  const qkv::BeamPlan plan = qkv::beam_plan(a.rows, beams, vocab, take, logits_type, whole);
+  const size_t segments = (size_t)a.rows * plan.segments;
+  a.rec_sum = static_cast<float*>(workspace);
+  a.rec_x = a.rec_sum + 2 * segments;
+  a.rec_at = reinterpret_cast<int32_t*>(a.rec_x + segments * take);
+  return launch_status(qkv::launch_beam(a, plan, logits_type, stream));
+}
+
+int qkv_pages_reorder(int32_t* block_tables, int n_slots, int max_blocks, int block_tokens, int32_t* ref_counts,
+                      int n_pages, const int32_t* slots, const int32_t* parents, const int32_t* n_tokens, int n,
+                      int32_t* status, const qkv_page_plane* states, int n_states, hipStream_t stream) {
+  const qkv::PageTables t{block_tables, ref_counts, n_slots, max_blocks, block_tokens, n_pages};
+  int st = check_tables(t);
+  if (st != QKV_OK) return st;
+  qkv::PagePlanes pl{};
+  st = take_planes(states, n_states, pl);
+  if (st != QKV_OK) return st;
+  if (n < 0 || n > n_slots) return QKV_ERR_INVALID;
+  if (n > qkv::kReorderMax) return QKV_ERR_UNSUPPORTED;
+  if (n == 0) return QKV_OK;
+  if (!slots || !parents || !n_tokens) return QKV_ERR_NULL;
+  if (!aligned(slots, 4) || !aligned(parents, 4) || !aligned(n_tokens, 4) || !aligned(status, 4)) return QKV_ERR_ALIGN;
+  return launch_status(qkv::launch_pages_reorder(t, slots, parents, n_tokens, n, status, kPageStatus, pl, stream));
+}
+
 }  // extern "C"

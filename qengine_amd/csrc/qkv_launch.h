@@ -149,7 +149,7 @@ hipError_t launch_rope(RopeArgs a, bool wide, bool in_place, hipStream_t stream)
 // Norms of heads with the rotation, and the gradient (norm_rope.hip).  dq, dk and their strides, the
 // sums of the weights' gradients (q_dw, k_dw) and the partial sums are the gradient's alone.
 constexpr int kNormMaxHead = 1024;
-constexpr int kNormGradGroups = 1024;   // workgroups of a gradient: 4 on each CU
+constexpr int kNormGradGroups = 768;   // workgroups of a gradient: the 3 that fit each CU
 struct NormRopeArgs {
   const uint16_t* q;
   const uint16_t* dq;
@@ -241,6 +241,32 @@ F8AttnPlan f8_attn_plan(int num_q, int num_kv, int head_dim, int n_slots, long r
 int f8_attn_apart(int num_q, int num_kv, int head_dim, int n_slots, long rows, int max_tok, int max_ctx);
 hipError_t launch_f8_attn(const F8AttnArgs& a, const F8AttnPlan& plan, int head_dim, hipStream_t stream);
 
+// Beam search's selection (beam.hip): rows = requests * beams.
+constexpr int kMaxBeams = 64, kMaxTake = 64;
+constexpr int kBeamGroups = 2048;   // workgroups of a call, and records of a request, below which a row
+constexpr int kBeamRecords = 4096;  // is cut finer
+struct BeamArgs {
+  const void* logits;        // [rows][vocab], `stride` elements between rows
+  const float* scores;       // [rows], -infinity: no beam
+  const int32_t* done;       // [rows], nullptr: none
+  int32_t* parents;          // [requests][take]
+  int32_t* tokens;
+  float* top;
+  float* rec_x;              // workspace: [rows][segments][take] the largest logits of a segment
+  int32_t* rec_at;           // and their tokens
+  float* rec_sum;            // workspace: [rows][segments] {largest logit m, sum of e^(x - m)}
+  long stride, rows;
+  int beams, vocab, take, end_token;
+  int segments;              // set by the launcher
+};
+struct BeamPlan {
+  int words;                 // 16-byte words a thread holds
+  int segments;              // workgroups of a row
+};
+// type 0: fp16, 1: fp32, 2: bf16; whole: every row begins with a 16-byte word
+BeamPlan beam_plan(long rows, int beams, int vocab, int take, int type, bool whole);
+hipError_t launch_beam(BeamArgs a, const BeamPlan& plan, int type, hipStream_t stream);
+
 // Pages of a cache (kv_pages.hip): tables [n_slots][max_blocks] with a negative
 // entry where there is no page, ref_counts [n_pages] (0: free).
 constexpr int kMaxPlanes = 128;
@@ -272,6 +298,11 @@ hipError_t launch_pages_reserve(const PageTables& t, const int32_t* slots, const
                                 const int32_t* n_new, int n, int max_new, int32_t* status, const PageStatus& codes,
                                 const PagePlanes& planes, int32_t* scratch, hipStream_t stream);
 hipError_t launch_pages_copy(const PagePlanes& planes, const int32_t* pairs, int n, int n_pages, hipStream_t stream);
+// Slots take over their parents' pages and rows of `states` (bytes: of a slot); n <= kReorderMax.
+constexpr int kReorderMax = 1024;
+hipError_t launch_pages_reorder(const PageTables& t, const int32_t* slots, const int32_t* parents,
+                                const int32_t* tokens, int n, int32_t* status, const PageStatus& codes,
+                                const PagePlanes& states, hipStream_t stream);
 // scratch: n_pages + 2 int32
 hipError_t launch_pages_compact(const PageTables& t, int32_t* moved, int32_t* n_used, const PagePlanes& planes,
                                 int32_t* scratch, hipStream_t stream);

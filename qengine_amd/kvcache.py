@@ -982,6 +982,25 @@ def pages_reserve(block_tables, ref_counts, slots, positions, n_new, status=None
                               scratch.nbytes, _raw_stream(stream, dev)), "qkv_pages_reserve")
 
 
+def pages_reorder(block_tables, ref_counts, slots, parents, n_tokens, status=None, states: PagePlanes | None = None, *,
+                  block_tokens, stream=None) -> None:
+    """slots[i] takes over what parents[i] held at the call (device int32 lists): the pages of its first n_tokens[i]
+    tokens, and its row of every tensor of `states` (page_planes of tensors [n_slots, ...]).  Any permutation, with
+    one parent for many slots: a beam search step's."""
+    dev = _run_device(stream, block_tables)
+    t, n_slots, mb, r, n_pages = _page_state(dev, block_tables, ref_counts)
+    n, st = _page_lists(dev, status, slots, parents, n_tokens)
+    sp, ns = 0, 0
+    if states is not None and states.n:
+        if states.n_pages < n_slots:
+            raise ValueError(f"the states hold {states.n_pages} rows, block_tables {n_slots}")
+        if states.device != dev:
+            raise ValueError(f"the states must be on cuda:{dev}, where the call runs")
+        sp, ns = states.ptr, states.n
+    check(lib().qkv_pages_reorder(t, n_slots, mb, block_tokens, r, n_pages, slots.data_ptr(), parents.data_ptr(),
+                                  n_tokens.data_ptr(), n, st, sp, ns, _raw_stream(stream, dev)), "qkv_pages_reorder")
+
+
 def pages_copy(planes: PagePlanes, pairs, *, stream=None) -> None:
     """Page pairs[i][0] to page pairs[i][1] in every plane (device int32 [n][2])."""
     dev = _run_device(stream, pairs)
@@ -1006,3 +1025,50 @@ def pages_compact(block_tables, ref_counts, moved, n_used, planes=None, *, scrat
     check(lib().qkv_pages_compact(t, n_slots, mb, r, n_pages, moved.data_ptr(), n_used.data_ptr(),
                                   *_planes_of(planes, n_pages, dev), scratch.data_ptr(), scratch.nbytes,
                                   _raw_stream(stream, dev)), "qkv_pages_compact")
+
+
+# ---------------------------------------------------------------------------
+# beam search
+# ---------------------------------------------------------------------------
+
+_LOGITS = {torch.float16: 0, torch.float32: 1, torch.bfloat16: 2}
+
+
+def beam_select_workspace(n, beams, vocab, take, device) -> torch.Tensor:
+    """Workspace of beam_select for up to these numbers."""
+    b = int(lib().qkv_beam_select_workspace_bytes(n, beams, vocab, take))
+    if b == 0 and n > 0:
+        raise ValueError(f"no call of these numbers: n {n}, beams {beams}, vocab {vocab}, take {take}")
+    return torch.empty(b, dtype=torch.uint8, device=device)
+
+
+def beam_select(logits, scores, parents, tokens, top_scores, workspace, *, done=None, end_token=0, stream=None) -> None:
+    """The best continuations of every request: logits fp16, bf16 or fp32 [n * beams][vocab] (rows may be apart),
+    scores fp32 [n][beams] (-inf: no beam), done int32 [n][beams] or None (ended beams offer end_token at their own
+    score); into parents int32, tokens int32 and top_scores fp32 [n][take]: logits row, token, score + log
+    probability, best first, -1, -1 and -inf where there are none."""
+    dev = _run_device(stream, logits)
+    if logits.dim() != 2 or logits.dtype not in _LOGITS:
+        raise ValueError("logits must be torch.float16, torch.bfloat16 or torch.float32 [n * beams][vocab]")
+    rows, vocab = logits.shape
+    if vocab > 1 and logits.stride(1) != 1:
+        raise ValueError("logits: a row must be contiguous")
+    if scores.dim() != 2 or scores.dtype is not _FP32 or scores.numel() != rows:
+        raise ValueError(f"scores must be torch.float32 [n][beams], {rows} in all")
+    n, beams = scores.shape
+    if parents.dim() != 2 or parents.shape[0] != n or tokens.shape != parents.shape or top_scores.shape != parents.shape:
+        raise ValueError(f"parents, tokens and top_scores must be [{n}][take]")
+    take = parents.shape[1]
+    if not (parents.dtype is tokens.dtype is _INT32) or top_scores.dtype is not _FP32:
+        raise ValueError("parents and tokens must be torch.int32, top_scores torch.float32")
+    dp = 0
+    if done is not None:
+        if done.dtype is not _INT32 or done.numel() != rows:
+            raise ValueError(f"done must hold {rows} numbers of torch.int32")
+        _on_device(dev, done)
+        dp = done.data_ptr()
+    _on_device(dev, scores, parents, tokens, top_scores, workspace)
+    check(lib().qkv_beam_select(
+        logits.data_ptr(), _LOGITS[logits.dtype], logits.stride(0) if rows > 1 else vocab, scores.data_ptr(), dp, end_token,
+        n, beams, vocab, take, parents.data_ptr(), tokens.data_ptr(), top_scores.data_ptr(), workspace.data_ptr(),
+        workspace.nbytes, _raw_stream(stream, dev)), "qkv_beam_select")

@@ -66,3 +66,92 @@ def norm_rope_grad(x, dy, w, positions, rot, layout, eps=1e-6, base=10000.0, sca
     # sums of rows numbers in any order: rows additions
     tw = (np.abs(xr) * eg).sum((0, 1)) + np.abs(g * xr).sum((0, 1)) * (er + (rows + 4) * 2.0 ** -24)
     return dx, tol, dw, tw
+
+
+# ---- beam search -------------------------------------------------------------
+
+def beam_scores(logits, scores, done=None, end_token=0):
+    """S [n][beams * vocab] in 64 bits (-inf: no candidate) and the tolerance of the searched beams' scores.
+
+    Ahead of the rounding to fp32 (2^-24 of S): the distances t to a segment's maximum (rounded once), their product
+    with log2(e) (two roundings) and the exponential (2^-23), weighted by their share of the sum; the sum's additions
+    in a thread (32), a wave (6) and a workgroup (2)."""
+    n, beams = scores.shape
+    x = logits.astype(np.float64)
+    x[~(x < np.inf)] = -np.inf
+    x = x.reshape(n, beams, -1)
+    out = np.full(x.shape, -np.inf)
+    tol = np.zeros((n, beams))
+    for r in range(n):
+        for b in range(beams):
+            s = float(scores[r, b])
+            if not s > -np.inf:
+                continue
+            if done is not None and done[r, b]:
+                out[r, b, end_token] = s
+                continue
+            m = x[r, b].max()
+            if m == -np.inf:
+                continue
+            t = x[r, b] - m
+            p = np.exp(t)
+            out[r, b] = s + (t - np.log(p.sum()))
+            far = np.where(p > 0, -t, 0)
+            tol[r, b] = ((p * far).sum() / p.sum() * 5 + 2 + 40) * 2.0 ** -24
+    return out.reshape(n, -1), tol
+
+
+def beam_check(logits, scores, take, parents, tokens, top, done=None, end_token=0):
+    """Asserts that parents, tokens and top (numpy) are the selection, and returns how many candidates there were."""
+    n, beams = scores.shape
+    S, tol = beam_scores(logits, scores, done, end_token)
+    vocab = S.shape[1] // beams
+    total = 0
+    for r in range(n):
+        order = np.lexsort((np.arange(S.shape[1]), -S[r]))[:take + 1]
+        order = order[S[r][order] > -np.inf]
+        want = order[:take]
+        k = len(want)
+        total += k
+        assert (parents[r, k:] == -1).all() and (tokens[r, k:] == -1).all() and (top[r, k:] == -np.inf).all()
+        got = (parents[r, :k] - r * beams) * vocab + tokens[r, :k]
+        assert (parents[r, :k] // beams == r).all() and ((tokens[r, :k] >= 0) & (tokens[r, :k] < vocab)).all()
+        s = S[r][want]
+        lim = np.abs(s) * 2.0 ** -24 + tol[r].max()
+        assert (np.abs(top[r, :k] - s) <= lim).all()
+        assert len(set(got.tolist())) == k and (np.abs(S[r][got] - s) <= 2 * lim).all()
+        # the same entries, but where two beams' candidates are nearer than the scores' errors
+        for i in range(k):
+            near = [j for j in (i - 1, i + 1) if 0 <= j < len(order) and order[j] // vocab != order[i] // vocab and
+                    abs(S[r][order[j]] - s[i]) <= 4 * lim[i]]
+            assert got[i] == want[i] or near, (r, i, got, want)
+    return total
+
+
+# ---- pages -------------------------------------------------------------------
+
+def reorder(tables, refs, slots, parents, n_tokens, bt, states=()):
+    """In place; the statuses."""
+    n_slots, mb = tables.shape
+    before, rows = tables.copy(), [s.copy() for s in states]
+    st = []
+    for i, (s, p, k) in enumerate(zip(slots, parents, n_tokens)):
+        nb = -(-k // bt)
+        bad = not (0 <= s < n_slots and 0 <= p < n_slots and k >= 0) or nb > mb or s in slots[:i]
+        st.append(R.INVALID if bad else R.OK)
+        if bad:
+            continue
+        new = np.full(mb, -1, np.int32)
+        new[:nb] = before[p, :nb]
+        new[new < 0] = -1
+        for g in new:
+            if 0 <= g < len(refs):
+                refs[g] += 1
+        for g in before[s]:
+            if 0 <= g < len(refs):
+                refs[g] -= 1
+        # (an entry below zero that stays one is not written)
+        tables[s] = np.where((new < 0) & (before[s] < 0) & (np.arange(mb) >= nb) & (before[s] == -1), before[s], new)
+        for a, b in zip(states, rows):
+            a[s] = b[p]
+    return st
