@@ -637,6 +637,29 @@ int qkv_attn_f8_paged(const uint16_t* q, const uint8_t* k_pool, const uint8_t* v
                       const int32_t* starts, const int32_t* positions, float scale, int window_tok,
                       int sink_tok, void* workspace, size_t workspace_bytes, hipStream_t stream);
 
+/* Eviction by accumulated attention weight.  weights: device fp32 [n_pages][num_kv][block_tokens], one for each key
+ * of a page and KV head (a plane of the page calls; qkv_weigh_f8_paged accumulates them).  Of the lens[s] rows of
+ * slot s (device int32 [n_slots]), keep[s] stay in each KV head, each head choosing its own: the last recent_tok,
+ * then the first sink_tok (as many of them as keep[s] allows), then those of the largest weights, ties to the lowest
+ * row (a NaN is below every other weight).  They move to rows 0 .. keep[s] - 1 of the slot, in order, in both pools
+ * and in weights; the slot's new length is min(lens[s], keep[s]) (the caller's to note; qkv_pages_release gives back
+ * the pages past it).  A page's exponent becomes the largest of those its rows had; codes of other exponents are
+ * requantized (a power of two: only codes that become subnormal round).  Rows past the new length hold anything.
+ * kept (device int32 [n_slots][num_kv][max_keep]): the former row of each, ascending, -1 past the last.
+ * A slot is left alone, its kept all -1, where lens[s] lies outside [0, max_ctx], keep[s] is negative,
+ * min(lens[s], keep[s]) passes max_keep, or one of its rows has no page; where keep[s] >= lens[s] nothing moves.
+ * No page that is written (those from the first row on that moves or that a raised exponent reaches) may
+ * belong to two slots, nor twice to one.  After an eviction a row's number is not its position: new rows are turned at
+ * their positions by qkv_rope or qkv_norm_rope and appended without a rotation, and windows count rows.
+ * max_ctx, max_keep <= 2^30, n_slots * num_kv < 2^22 and n_slots * num_kv * (max_keep / 64 + 1) < 2^24
+ * (QKV_ERR_UNSUPPORTED).  workspace: qkv_evict_f8_paged_workspace_bytes of these numbers or larger ones (no
+ * initialisation needed).  Calls sharing one must be ordered. */
+size_t qkv_evict_f8_paged_workspace_bytes(int n_slots, int num_kv, int block_tokens, int max_ctx, int max_keep);
+int qkv_evict_f8_paged(uint8_t* k_pool, uint8_t* v_pool, uint8_t* k_exp, uint8_t* v_exp, float* weights, int n_slots,
+                       int num_kv, int head_dim, int max_ctx, int max_keep, const int32_t* block_tables, int max_blocks,
+                       int block_tokens, int n_pages, const int32_t* lens, const int32_t* keep, int sink_tok,
+                       int recent_tok, int32_t* kept, void* workspace, size_t workspace_bytes, hipStream_t stream);
+
 /* ---------------------------------------------------------------------------
  * Pages of a cache, of any format.  No counterpart in the reference (its slots
  * are contiguous).  The state is on the device, so that the calls can be captured

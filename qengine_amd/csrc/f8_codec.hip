@@ -15,6 +15,7 @@
 // step of 32 slots with its rotation 5.3 us, which is latency.
 #include <algorithm>
 
+#include "f8_device.h"
 #include "qkv_device.h"
 #include "qkv_launch.h"
 #include "rope_device.h"
@@ -36,8 +37,6 @@ __device__ __forceinline__ int f8_exponent(uint32_t bits) {
   const uint32_t f = __float_as_uint(h2f(bits));
   return max(95, (int)(f >> 23) - 8 + ((f & 0x7fffffu) > 0x600000u ? 1 : 0));   // (zero: 95)
 }
-
-__device__ __forceinline__ float pow2_bits(int biased) { return __uint_as_float((uint32_t)biased << 23); }
 
 }  // namespace
 
@@ -101,11 +100,6 @@ __device__ __forceinline__ u2_t encode8(u4_t v, float inv) {
     o[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32((float)x[4 * i + 2] * inv, (float)x[4 * i + 3] * inv, w, true);
   }
   return o;
-}
-__device__ __forceinline__ uint32_t rescale4(uint32_t codes, float f) {
-  const f2_t lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, true);
-  const int w = __builtin_amdgcn_cvt_pk_fp8_f32(lo[0] * f, lo[1] * f, 0, false);
-  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(hi[0] * f, hi[1] * f, w, true);
 }
 
 // One workgroup per (slot, touched page, KV head, K or V); the workgroups past those

@@ -159,6 +159,65 @@ int qkv_norm_rope_grad(const uint16_t* q, long q_stride, const uint16_t* q_dy, l
   return launch_status(qkv::launch_norm_rope_grad(a, wide, norm_grad_groups(n_tok, num_q, num_k), stream));
 }
 
+static int check_evict(int n_slots, int num_kv, int block_tokens, int max_ctx, int max_keep) {
+  if (n_slots < 0 || num_kv <= 0 || block_tokens <= 0 || max_ctx < 0 || max_keep < 0) return QKV_ERR_INVALID;
+  // chunks of all slots and heads are workgroups of 256 threads of one launch, slots and heads of 1,024
+  if (max_ctx > (1 << 30) || max_keep > (1 << 30) || (double)n_slots * num_kv >= (double)(1 << 22) ||
+      (double)n_slots * num_kv * (max_keep / 64 + 1.0) >= (double)(1 << 24))
+    return QKV_ERR_UNSUPPORTED;
+  return QKV_OK;
+}
+
+size_t qkv_evict_f8_paged_workspace_bytes(int n_slots, int num_kv, int block_tokens, int max_ctx, int max_keep) {
+  if (n_slots == 0 || check_evict(n_slots, num_kv, block_tokens, max_ctx, max_keep) != QKV_OK) return 0;
+  return 256 + 4 * ((size_t)n_slots * num_kv * (max_keep / 64 + 2));
+}
+
+int qkv_evict_f8_paged(uint8_t* k_pool, uint8_t* v_pool, uint8_t* k_exp, uint8_t* v_exp, float* weights, int n_slots,
+                       int num_kv, int head_dim, int max_ctx, int max_keep, const int32_t* block_tables, int max_blocks,
+                       int block_tokens, int n_pages, const int32_t* lens, const int32_t* keep, int sink_tok,
+                       int recent_tok, int32_t* kept, void* workspace, size_t workspace_bytes, hipStream_t stream) {
+  int st = check_f8_pool(num_kv, head_dim, max_blocks, block_tokens, n_pages);
+  if (st != QKV_OK) return st;
+  st = check_evict(n_slots, num_kv, block_tokens, max_ctx, max_keep);
+  if (st != QKV_OK) return st;
+  if (sink_tok < 0 || recent_tok < 0) return QKV_ERR_INVALID;
+  if (n_slots == 0 || max_keep == 0) return QKV_OK;
+  if (!k_pool || !v_pool || !k_exp || !v_exp || !weights || !block_tables || !lens || !keep || !kept) return QKV_ERR_NULL;
+  if (!aligned(k_pool, 16) || !aligned(v_pool, 16) || !aligned(weights, 4) || !aligned(block_tables, 4) ||
+      !aligned(lens, 4) || !aligned(keep, 4) || !aligned(kept, 4))
+    return QKV_ERR_ALIGN;
+  if (!workspace || workspace_bytes < qkv_evict_f8_paged_workspace_bytes(n_slots, num_kv, block_tokens, max_ctx, max_keep))
+    return QKV_ERR_WORKSPACE;
+  if (!aligned(workspace, 4)) return QKV_ERR_ALIGN;
+  qkv::EvictArgs a{};
+  a.k_pool = k_pool;
+  a.v_pool = v_pool;
+  a.k_exp = k_exp;
+  a.v_exp = v_exp;
+  a.weights = weights;
+  a.tables = block_tables;
+  a.lens = lens;
+  a.keep = keep;
+  a.kept = kept;
+  a.ticket = static_cast<int*>(workspace);
+  a.moves = a.ticket + 64;
+  a.flags = a.moves + (size_t)n_slots * num_kv;
+  a.n_slots = n_slots;
+  a.num_kv = num_kv;
+  a.max_ctx = max_ctx;
+  a.max_keep = max_keep;
+  a.max_blocks = max_blocks;
+  a.block_tokens = block_tokens;
+  a.n_pages = n_pages;
+  a.sink = sink_tok;
+  a.recent = recent_tok;
+  const int rows = qkv::kEvictBytes / head_dim;
+  a.chunks = (max_keep + rows - 1) / rows;
+  a.bt_magic = (uint32_t)((1ull << 32) / (uint64_t)block_tokens);
+  return launch_status(qkv::launch_evict(a, head_dim, stream));
+}
+
 static int check_beam(int n, int beams, int vocab, int take) {
   if (n < 0 || beams <= 0 || vocab <= 0 || take <= 0) return QKV_ERR_INVALID;
   // (beam and token of a request are one whole number of 31 bits; rows are workgroups of a launch)

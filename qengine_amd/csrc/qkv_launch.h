@@ -241,6 +241,27 @@ F8AttnPlan f8_attn_plan(int num_q, int num_kv, int head_dim, int n_slots, long r
 int f8_attn_apart(int num_q, int num_kv, int head_dim, int n_slots, long rows, int max_tok, int max_ctx);
 hipError_t launch_f8_attn(const F8AttnArgs& a, const F8AttnPlan& plan, int head_dim, hipStream_t stream);
 
+// Eviction from the paged 8-bit cache (evict_f8.hip).
+constexpr int kEvictBytes = 16384;   // codes of a chunk of rows, of each pool
+struct EvictArgs {
+  uint8_t* k_pool;
+  uint8_t* v_pool;
+  uint8_t* k_exp;
+  uint8_t* v_exp;
+  float* weights;            // [n_pages][num_kv][block_tokens]
+  const int32_t* tables;
+  const int32_t* lens;       // [n_slots] rows of a slot
+  const int32_t* keep;       // [n_slots] rows that stay
+  int32_t* kept;             // [n_slots][num_kv][max_keep]
+  int* ticket;               // workspace: chunks taken; set to 0 by the first launch
+  int* moves;                // workspace: [n_slots * num_kv] rows to write (0: none)
+  int* flags;                // workspace: [n_slots * num_kv][chunks] 1: read, 2: all before too
+  int n_slots, num_kv, max_ctx, max_keep, max_blocks, block_tokens, n_pages, sink, recent;
+  int chunks;                // of max_keep rows
+  uint32_t bt_magic;         // floor(2^32 / block_tokens)
+};
+hipError_t launch_evict(EvictArgs a, int head_dim, hipStream_t stream);
+
 // Beam search's selection (beam.hip): rows = requests * beams.
 constexpr int kMaxBeams = 64, kMaxTake = 64;
 constexpr int kBeamGroups = 2048;   // workgroups of a call, and records of a request, below which a row

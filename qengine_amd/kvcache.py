@@ -880,6 +880,60 @@ def attn_f8_paged(q, k_pool, v_pool, k_exp, v_exp, out, workspace, block_tables,
 
 
 # ---------------------------------------------------------------------------
+# eviction from the paged 8-bit cache by accumulated attention weight
+# ---------------------------------------------------------------------------
+
+def f8_weights(n_pages: int, block_tokens: int, num_kv: int, device) -> torch.Tensor:
+    """Zeroed weights fp32 [n_pages][num_kv][block_tokens] of the keys of a paged 8-bit cache (a plane of the page
+    calls beside its pools)."""
+    return torch.zeros((n_pages, num_kv, block_tokens), dtype=torch.float32, device=device)
+
+
+def _need_weights(weights, k_pool) -> None:
+    n_pages, bt, kv, _ = k_pool.shape
+    if weights.dtype is not _FP32 or weights.shape != (n_pages, kv, bt):
+        raise ValueError(f"weights must be torch.float32 [{n_pages}][{kv}][{bt}]")
+
+
+def evict_f8_paged_workspace(n_slots, num_kv, block_tokens, max_ctx, max_keep, device) -> torch.Tensor:
+    """Workspace of evict_f8_paged for up to these numbers."""
+    n = int(lib().qkv_evict_f8_paged_workspace_bytes(n_slots, num_kv, block_tokens, max_ctx, max_keep))
+    if n == 0 and n_slots > 0:
+        raise ValueError(f"no call of these numbers: n_slots {n_slots}, num_kv {num_kv}, block_tokens {block_tokens}, "
+                         f"max_ctx {max_ctx}, max_keep {max_keep}")
+    return torch.empty(n, dtype=torch.uint8, device=device)
+
+
+def evict_f8_paged(k_pool, v_pool, k_exp, v_exp, weights, block_tables, lens, keep, kept, workspace, *, max_ctx, sink=0,
+                   recent=0, stream=None) -> None:
+    """Of the lens[s] rows of each slot keep[s] stay in every KV head: the last `recent`, the first `sink` and those of
+    the largest weights (fp32 [n_pages][num_kv][block_tokens]), moved in order to the slot's first rows, in the pools
+    and in weights.  kept: int32 [n_slots][num_kv][max_keep], their former rows (-1 past the last).  The slot's length
+    is then min(lens[s], keep[s]); rows are no longer positions."""
+    dev = _run_device(stream, k_pool)
+    n_pages, bt, kv, hd = shape = k_pool.shape
+    if v_pool.shape != shape:
+        raise ValueError("k_pool and v_pool must be [n_pages][block_tokens][num_kv][head_dim]")
+    if k_exp.shape != (n_pages, kv) or v_exp.shape != (n_pages, kv):
+        raise ValueError(f"k_exp and v_exp must be [{n_pages}][{kv}]")
+    if not (k_pool.dtype is v_pool.dtype is k_exp.dtype is v_exp.dtype is _UINT8):
+        raise ValueError("the pools and their exponents must be torch.uint8")
+    _need_weights(weights, k_pool)
+    if not (block_tables.dtype is lens.dtype is keep.dtype is kept.dtype is _INT32):
+        raise ValueError("block_tables, lens, keep and kept must be torch.int32")
+    n_slots, mb = block_tables.shape
+    if lens.numel() != n_slots or keep.numel() != n_slots:
+        raise ValueError(f"lens and keep must hold {n_slots} numbers")
+    if kept.dim() != 3 or kept.shape[:2] != (n_slots, kv):
+        raise ValueError(f"kept must be [{n_slots}][{kv}][max_keep]")
+    _on_device(dev, k_pool, v_pool, k_exp, v_exp, weights, block_tables, lens, keep, kept, workspace)
+    check(lib().qkv_evict_f8_paged(
+        k_pool.data_ptr(), v_pool.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr(), weights.data_ptr(), n_slots, kv, hd,
+        max_ctx, kept.shape[2], block_tables.data_ptr(), mb, bt, n_pages, lens.data_ptr(), keep.data_ptr(), sink, recent,
+        kept.data_ptr(), workspace.data_ptr(), workspace.nbytes, _raw_stream(stream, dev)), "qkv_evict_f8_paged")
+
+
+# ---------------------------------------------------------------------------
 # pages: sharing, reserving, giving back, compacting
 # ---------------------------------------------------------------------------
 

@@ -155,3 +155,46 @@ def reorder(tables, refs, slots, parents, n_tokens, bt, states=()):
         for a, b in zip(states, rows):
             a[s] = b[p]
     return st
+
+
+# ---- eviction ------------------------------------------------------------------
+
+def evict(pools, exps, weights, tables, lens, keep, max_ctx, max_keep, sink=0, recent=0):
+    """In place on [k, v] pools, exponents and weights [pages][kv][bt]; returns kept."""
+    n_pages, bt, kv, _ = pools[0].shape
+    n_slots, mb = tables.shape
+    kept = np.full((n_slots, kv, max_keep), -1, np.int32)
+    for s in range(n_slots):
+        n, k = int(lens[s]), int(keep[s])
+        if n < 0 or n > max_ctx or k < 0 or min(n, k) > max_keep or -(-n // bt) > mb:
+            continue
+        pages = tables[s, :-(-n // bt)]
+        if ((pages < 0) | (pages >= n_pages)).any():
+            continue
+        j = np.arange(n)
+        page, row = pages[j // bt], j % bt
+        for h in range(kv):
+            if k >= n:
+                kept[s, h, :n] = j
+                continue
+            last = min(k, recent)
+            first = min(k - last, sink)
+            w = weights[page, h, row].astype(np.float64)
+            mid = np.arange(first, n - last)
+            v = np.where(np.isnan(w[mid]), -np.inf, w[mid])
+            # (a NaN is below -infinity too)
+            order = np.lexsort((mid, -v, np.isnan(w[mid])))
+            rows = np.sort(np.concatenate([np.arange(first), mid[order[:k - first - last]], np.arange(n - last, n)]).astype(int))
+            kept[s, h, :k] = rows
+            if k == 0:
+                continue
+            weights[page[:k], h, row[:k]] = weights[page[rows], h, row[rows]]
+            for pool, exp in zip(pools, exps):
+                codes, e = pool[page[rows], row[rows], h], exp[page[rows], h].astype(int)
+                for a in range(0, k, bt):
+                    b = min(k, a + bt)
+                    top = e[a:b].max()
+                    x = R.e4m3_encode(R.CODES[codes[a:b]] * 2.0 ** (e[a:b] - top)[:, None])
+                    pool[page[a], :b - a, h] = np.where((e[a:b] == top)[:, None], codes[a:b], x)
+                    exp[page[a], h] = top
+    return kept
