@@ -637,6 +637,29 @@ int qkv_attn_f8_paged(const uint16_t* q, const uint8_t* k_pool, const uint8_t* v
                       const int32_t* starts, const int32_t* positions, float scale, int window_tok,
                       int sink_tok, void* workspace, size_t workspace_bytes, hipStream_t stream);
 
+/* Attention weight of each key, accumulated.  q, starts, positions, max_tok, max_ctx, the window and the pages are as
+ * for qkv_attn_f8_paged (the rows may be all of a call's, or others: a prompt's last few, to choose by them what an
+ * eviction keeps).  For slot s with n rows, and its keys j < min(positions[s] + n, max_ctx):
+ *   weights[j] = (j < weighed[s] ? decay * weights[j] : 0) + sum over the rows and the query heads of j's KV head of
+ *                the softmax weights that qkv_attn_f8_paged gives key j (0 where a row does not see it),
+ * in fp32, in an order that does not change from call to call.  weights: device fp32 [n_pages][num_kv][block_tokens],
+ * an entry for each key of a page and KV head.  weighed (device int32 [n_slots], NULL: positions): how many of
+ * the slot's first keys have a weight that stands; others hold anything before.  decay finite; with 0 nothing that
+ * stood is read.  Slots without rows, keys past the last and keys without a page are left alone, and of two slots
+ * that share a page only one may be named with rows in a call (the other's weights would take its place).  A row
+ * that sees no key adds nothing; one whose query is not finite makes weights that are not.  Limits as for
+ * qkv_attn_f8_paged, and n_slots * num_kv * (max_tok * num_q / num_kv / 256 + 1) * (max_ctx / 128 + 1) < 2^31 suffices
+ * (QKV_ERR_UNSUPPORTED past what the launches count, and 0 from the workspace query).  workspace:
+ * qkv_weigh_f8_paged_workspace_bytes of these numbers or larger ones (n_slots, n_rows, max_tok, max_ctx), 256-byte
+ * aligned (no initialisation needed).  Calls sharing one must be ordered. */
+size_t qkv_weigh_f8_paged_workspace_bytes(int num_q, int num_kv, int head_dim, int n_slots, int n_rows, int max_tok,
+                                          int max_ctx);
+int qkv_weigh_f8_paged(const uint16_t* q, const uint8_t* k_pool, const uint8_t* k_exp, float* weights, int n_rows,
+                       int num_q, int num_kv, int head_dim, int n_slots, int max_tok, int max_ctx,
+                       const int32_t* block_tables, int max_blocks, int block_tokens, int n_pages, const int32_t* starts,
+                       const int32_t* positions, const int32_t* weighed, float decay, float scale, int window_tok,
+                       int sink_tok, void* workspace, size_t workspace_bytes, hipStream_t stream);
+
 /* Eviction by accumulated attention weight.  weights: device fp32 [n_pages][num_kv][block_tokens], one for each key
  * of a page and KV head (a plane of the page calls; qkv_weigh_f8_paged accumulates them).  Of the lens[s] rows of
  * slot s (device int32 [n_slots]), keep[s] stay in each KV head, each head choosing its own: the last recent_tok,

@@ -100,6 +100,9 @@ SIGNATURES = {
     "qkv_attn_f8_paged_workspace_bytes": (_SZ, [_I, _I, _I, _I, _I, _I, _I]),
     "qkv_attn_f8_paged": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _I, _I, _I, _P, _P, _F,
                                _I, _I, _P, _SZ, _P]),
+    "qkv_weigh_f8_paged_workspace_bytes": (_SZ, [_I, _I, _I, _I, _I, _I, _I]),
+    "qkv_weigh_f8_paged": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _I, _I, _I, _P, _P, _P, _F, _F, _I, _I,
+                                _P, _SZ, _P]),
     "qkv_evict_f8_paged_workspace_bytes": (_SZ, [_I, _I, _I, _I, _I]),
     "qkv_evict_f8_paged": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _I, _I, _I, _P, _P, _I, _I, _P, _P, _SZ,
                                 _P]),

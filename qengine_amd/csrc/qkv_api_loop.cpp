@@ -159,6 +159,91 @@ int qkv_norm_rope_grad(const uint16_t* q, long q_stride, const uint16_t* q_dy, l
   return launch_status(qkv::launch_norm_rope_grad(a, wide, norm_grad_groups(n_tok, num_q, num_k), stream));
 }
 
+static int check_weigh(int num_q, int num_kv, int head_dim, int n_slots, int n_rows, int max_tok, int max_ctx) {
+  if (head_dim != 128 && head_dim != 256) return QKV_ERR_UNSUPPORTED;
+  if (num_kv <= 0 || num_q <= 0 || num_q % num_kv != 0 || n_slots <= 0 || n_rows <= 0 || max_tok <= 0 || max_ctx <= 0)
+    return QKV_ERR_INVALID;
+  if (num_q / num_kv > 8 || num_q > 1024 || max_ctx > (1 << 30)) return QKV_ERR_UNSUPPORTED;
+  // workgroups of a launch, and rows of a slot and KV head, counted in 31 bits
+  const double heads = (double)n_slots * num_kv, rows = (double)std::min(max_tok, n_rows) * (num_q / num_kv);
+  const double wgs = heads * std::max({(rows / qkv::kWeighRows + 1) * (max_ctx / (double)qkv::kWeighChunk + 1),
+                                       (rows / qkv::kWeighSpan + 1) * (max_ctx / (double)qkv::kWeighKeys + 1), rows / 16 + 1,
+                                       max_ctx / 128.0 + 1});
+  if (wgs > 2147483000.0 || rows > (double)(1 << 30)) return QKV_ERR_UNSUPPORTED;
+  return QKV_OK;
+}
+
+static size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
+static size_t weigh_total(const qkv::WeighPlan& x) { return round256(x.stat_bytes) + round256(x.rec_bytes) + round256(x.sum_bytes); }
+
+size_t qkv_weigh_f8_paged_workspace_bytes(int num_q, int num_kv, int head_dim, int n_slots, int n_rows, int max_tok,
+                                          int max_ctx) {
+  if (check_weigh(num_q, num_kv, head_dim, n_slots, n_rows, max_tok, max_ctx) != QKV_OK) return 0;
+  if (max_tok > n_rows) max_tok = n_rows;
+  const qkv::WeighPlan x = qkv::weigh_plan(num_q, num_kv, n_slots, n_rows, max_tok, max_ctx);
+  // Calls with smaller numbers: their scores need at most kWeighScores bytes and at most those of up to 64 rows a
+  // slot at this context, their records a 64th of it (8 bytes for 128 scores or more) and their rows' statistics
+  // one of 32 bytes; the other sizes grow with each number.
+  const double pitch = (max_ctx + 31.0) / 32 * 32, tokens = std::min(64 / (num_q / num_kv), max_tok);
+  const size_t most = (size_t)std::min((double)qkv::kWeighScores, (double)n_slots * tokens * num_q * pitch * 4);
+  const size_t few_rows = (size_t)((double)n_slots * tokens * num_q);
+  return round256(std::max(x.stat_bytes, 8 * few_rows)) + round256(std::max(x.rec_bytes, most / 64 + 8 * few_rows)) +
+         round256(std::max(x.sum_bytes, most)) + 1024;
+}
+
+int qkv_weigh_f8_paged(const uint16_t* q, const uint8_t* k_pool, const uint8_t* k_exp, float* weights, int n_rows,
+                       int num_q, int num_kv, int head_dim, int n_slots, int max_tok, int max_ctx,
+                       const int32_t* block_tables, int max_blocks, int block_tokens, int n_pages, const int32_t* starts,
+                       const int32_t* positions, const int32_t* weighed, float decay, float scale, int window_tok,
+                       int sink_tok, void* workspace, size_t workspace_bytes, hipStream_t stream) {
+  int st = check_f8_pool(num_kv, head_dim, max_blocks, block_tokens, n_pages);
+  if (st != QKV_OK) return st;
+  if (n_rows == 0 || n_slots == 0 || max_tok == 0) return QKV_OK;
+  st = check_weigh(num_q, num_kv, head_dim, n_slots, n_rows, max_tok, max_ctx);
+  if (st != QKV_OK) return st;
+  if (window_tok < 0 || sink_tok < 0 || !std::isfinite(decay)) return QKV_ERR_INVALID;
+  if (!q || !k_pool || !k_exp || !weights || !block_tables || !starts || !positions) return QKV_ERR_NULL;
+  if (!aligned(q, 16) || !aligned(k_pool, 16) || !aligned(weights, 4) || !aligned(block_tables, 4) || !aligned(starts, 4) ||
+      !aligned(positions, 4) || !aligned(weighed, 4))
+    return QKV_ERR_ALIGN;
+  if (max_tok > n_rows) max_tok = n_rows;
+  const qkv::WeighPlan x = qkv::weigh_plan(num_q, num_kv, n_slots, n_rows, max_tok, max_ctx);
+  if (!workspace || workspace_bytes < weigh_total(x)) return QKV_ERR_WORKSPACE;
+  if (!aligned(workspace, 256)) return QKV_ERR_ALIGN;
+  qkv::WeighArgs a{};
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  a.q = q;
+  a.k_pool = k_pool;
+  a.k_exp = k_exp;
+  a.weights = weights;
+  a.tables = block_tables;
+  a.starts = starts;
+  a.positions = positions;
+  a.weighed = weighed;
+  a.stat = reinterpret_cast<float*>(ws);
+  a.rec = reinterpret_cast<float*>(ws + round256(x.stat_bytes));
+  a.scores = reinterpret_cast<float*>(ws + round256(x.stat_bytes) + round256(x.rec_bytes));
+  a.partial = a.scores;   // (the one kind's launches are done before the other's)
+  a.rows = n_rows;
+  a.score_pitch = x.pitch;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.decay = decay;
+  a.num_q = num_q;
+  a.num_kv = num_kv;
+  a.n_slots = n_slots;
+  a.max_tok = max_tok;
+  a.max_ctx = max_ctx;
+  a.max_blocks = max_blocks;
+  a.block_tokens = block_tokens;
+  a.n_pages = n_pages;
+  a.window = window_tok;
+  a.sink = sink_tok < max_ctx ? sink_tok : max_ctx;
+  a.gqa = num_q / num_kv;
+  a.bt_magic = (uint32_t)((1ull << 32) / (uint64_t)block_tokens);
+  a.gqa_magic = (uint32_t)std::min<uint64_t>((1ull << 32) / (uint64_t)a.gqa, 0xffffffffull);
+  return launch_status(qkv::launch_weigh(a, x, head_dim, stream));
+}
+
 static int check_evict(int n_slots, int num_kv, int block_tokens, int max_ctx, int max_keep) {
   if (n_slots < 0 || num_kv <= 0 || block_tokens <= 0 || max_ctx < 0 || max_keep < 0) return QKV_ERR_INVALID;
   // chunks of all slots and heads are workgroups of 256 threads of one launch, slots and heads of 1,024

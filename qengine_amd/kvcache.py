@@ -895,6 +895,48 @@ def _need_weights(weights, k_pool) -> None:
         raise ValueError(f"weights must be torch.float32 [{n_pages}][{kv}][{bt}]")
 
 
+def weigh_f8_paged_workspace(num_q, num_kv, n_slots, n_rows, max_tok, max_ctx, device, *, head_dim=256) -> torch.Tensor:
+    """Workspace of weigh_f8_paged for up to these numbers."""
+    n = int(lib().qkv_weigh_f8_paged_workspace_bytes(num_q, num_kv, head_dim, n_slots, n_rows, max_tok, max_ctx))
+    if n == 0 and min(n_slots, n_rows, max_tok) > 0:
+        raise ValueError(f"no call of these numbers: num_q {num_q}, num_kv {num_kv}, head_dim {head_dim}, n_slots {n_slots}, "
+                         f"n_rows {n_rows}, max_tok {max_tok}, max_ctx {max_ctx}")
+    return torch.empty(n, dtype=torch.uint8, device=device)
+
+
+def weigh_f8_paged(q, k_pool, k_exp, weights, workspace, block_tables, starts, positions, *, max_tok, max_ctx, scale,
+                   decay=1.0, weighed=None, window=0, sink=0, stream=None) -> None:
+    """Adds to weights (fp32 [n_pages][num_kv][block_tokens]) what the ragged query rows (as for attn_f8_paged) give each
+    key: softmax weights summed over rows and the heads of a KV group, after decay times what stood for the first
+    weighed[s] keys of each slot (int32 [n_slots], None: positions) and from zero for the others."""
+    dev = _run_device(stream, k_pool)
+    n_pages, bt, kv, hd = k_pool.shape
+    if k_exp.shape != (n_pages, kv):
+        raise ValueError(f"k_exp must be [{n_pages}][{kv}]")
+    if not (k_pool.dtype is k_exp.dtype is _UINT8):
+        raise ValueError("the pool and its exponents must be torch.uint8")
+    _need_weights(weights, k_pool)
+    if not (block_tables.dtype is starts.dtype is positions.dtype is _INT32):
+        raise ValueError("block_tables, starts and positions must be torch.int32")
+    n_slots, mb = block_tables.shape
+    if starts.numel() != n_slots + 1 or positions.numel() != n_slots:
+        raise ValueError(f"starts must hold {n_slots + 1} numbers and positions {n_slots}")
+    rows, nq, qd = q.shape
+    if qd != hd or q.dtype not in FP16:
+        raise ValueError(f"q must be fp16 [rows][num_q][{hd}]")
+    wp = 0
+    if weighed is not None:
+        if weighed.dtype is not _INT32 or weighed.numel() != n_slots:
+            raise ValueError(f"weighed must hold {n_slots} numbers of torch.int32")
+        _on_device(dev, weighed)
+        wp = weighed.data_ptr()
+    _on_device(dev, q, k_pool, k_exp, weights, workspace, block_tables, starts, positions)
+    check(lib().qkv_weigh_f8_paged(
+        q.data_ptr(), k_pool.data_ptr(), k_exp.data_ptr(), weights.data_ptr(), rows, nq, kv, hd, n_slots, max_tok, max_ctx,
+        block_tables.data_ptr(), mb, bt, n_pages, starts.data_ptr(), positions.data_ptr(), wp, float(decay), float(scale),
+        window, sink, workspace.data_ptr(), workspace.nbytes, _raw_stream(stream, dev)), "qkv_weigh_f8_paged")
+
+
 def evict_f8_paged_workspace(n_slots, num_kv, block_tokens, max_ctx, max_keep, device) -> torch.Tensor:
     """Workspace of evict_f8_paged for up to these numbers."""
     n = int(lib().qkv_evict_f8_paged_workspace_bytes(n_slots, num_kv, block_tokens, max_ctx, max_keep))

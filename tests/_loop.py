@@ -198,3 +198,57 @@ def evict(pools, exps, weights, tables, lens, keep, max_ctx, max_keep, sink=0, r
                     pool[page[a], :b - a, h] = np.where((e[a:b] == top)[:, None], codes[a:b], x)
                     exp[page[a], h] = top
     return kept
+
+
+# ---- accumulated weights ---------------------------------------------------------
+
+def weigh(q, kp, ke, weights, tables, starts, positions, scale, weighed=None, decay=1.0, window=0, sink=0,
+          max_ctx=1 << 30, max_tok=1 << 30):
+    """64-bit weights [pages][kv][bt] after a call, and tolerances (0 where nothing is written).
+
+    Each softmax weight is off, relatively, by: its score's fp32 sum (head_dim additions, 2^-24 of sum |q k| each),
+    the scaling, the difference and the exponential (4 of 2^-23 of the largest score), the same in its row's sum,
+    that sum's additions (half the keys in a lane, 40 joining lanes, waves and chunks) and reciprocal, and the sum over
+    rows (half of them in a lane, 40 joining); then the decay's product and sum."""
+    rows, nq, hd = q.shape
+    n_pages, bt, kv, _ = kp.shape
+    g = nq // kv
+    out = weights.astype(np.float64)
+    tol = np.zeros(weights.shape)
+    for s in range(len(positions)):
+        n, p0 = min(int(starts[s + 1] - starts[s]), max_tok), int(positions[s])
+        if n <= 0 or p0 < 0:
+            continue
+        j = np.arange(min(p0 + n, max_ctx))
+        b = j // bt
+        page = np.where(b < tables.shape[1], tables[s][np.minimum(b, tables.shape[1] - 1)], -1)
+        ok = (page >= 0) & (page < n_pages)
+        page = np.where(ok, page, 0)
+        pos = p0 + np.arange(n)[:, None]
+        see = ok & (j <= pos)
+        if window > 0:
+            see &= (j > pos - window) | (j < sink)
+        for h in range(kv):
+            k = R.CODES[kp[page, j % bt, h]] * 2.0 ** (ke[page, h].astype(np.float64) - 127)[:, None]
+            k = np.where(ok[:, None], k, 0.0)
+            a, e = np.zeros(len(j)), np.zeros(len(j))
+            for i in range(g):
+                x = q[starts[s]:starts[s] + n, h * g + i].astype(np.float64)
+                sc = np.where(see, x @ k.T * scale, -np.inf)
+                mag = np.where(see, np.abs(x) @ np.abs(k).T * abs(scale), 0).max(1)
+                top = np.where(see, np.abs(sc), 0).max(1)
+                with np.errstate(invalid="ignore"):
+                    w = np.exp(sc - np.where(see.any(1), sc.max(1), 0)[:, None])
+                w = w / np.maximum(w.sum(1, keepdims=True), 1e-300)
+                d = 2 * ((hd + 2) * 2.0 ** -24 * mag + 4 * (top + 1) * 2.0 ** -23) + (len(j) / 2 + 44) * 2.0 ** -24
+                a += w.sum(0)
+                e += (w * np.expm1(d)[:, None]).sum(0)
+            e += a * (n * g / 2 + 40) * 2.0 ** -24
+            old = np.zeros(len(j))
+            stands = j < (p0 if weighed is None else weighed[s])
+            if decay != 0:
+                old = np.where(stands, decay * weights[page, h, j % bt].astype(np.float64), 0.0)
+            at = page[ok], h, (j % bt)[ok]
+            out[at] = (old + a)[ok]
+            tol[at] = (e + (np.abs(old) * 2 + a) * 2.0 ** -24 + 2.0 ** -120)[ok]
+    return out, tol
