@@ -164,17 +164,22 @@ static int check_weigh(int num_q, int num_kv, int head_dim, int n_slots, int n_r
   if (num_kv <= 0 || num_q <= 0 || num_q % num_kv != 0 || n_slots <= 0 || n_rows <= 0 || max_tok <= 0 || max_ctx <= 0)
     return QKV_ERR_INVALID;
   if (num_q / num_kv > 8 || num_q > 1024 || max_ctx > (1 << 30)) return QKV_ERR_UNSUPPORTED;
-  // workgroups of a launch, and rows of a slot and KV head, counted in 31 bits
-  const double heads = (double)n_slots * num_kv, rows = (double)std::min(max_tok, n_rows) * (num_q / num_kv);
-  const double wgs = heads * std::max({(rows / qkv::kWeighRows + 1) * (max_ctx / (double)qkv::kWeighChunk + 1),
-                                       (rows / qkv::kWeighSpan + 1) * (max_ctx / (double)qkv::kWeighKeys + 1), rows / 16 + 1,
-                                       max_ctx / 128.0 + 1});
-  if (wgs > 2147483000.0 || rows > (double)(1 << 30)) return QKV_ERR_UNSUPPORTED;
+  // workgroups of a launch, rows of a slot and KV head, and steps of the line of all tiles (by rows, then by keys),
+  // counted in 31 bits, a head's steps in 30
+  const double gqa = num_q / num_kv, tok = std::min(max_tok, n_rows), rows = tok * gqa, heads = (double)n_slots * num_kv;
+  const double row_tiles = std::min(n_slots * (rows / 512 + 1), n_rows * gqa / 512 + n_slots);
+  const double by_rows = row_tiles * (max_ctx / 64.0 + 6), by_keys = (max_ctx / 512.0 + 1) * (n_rows * gqa / 64 + 6.0 * n_slots);
+  if (heads * std::max(rows / 16 + 1, max_ctx / 128.0 + 1) > 2147480000.0 || rows > (double)(1 << 30) ||
+      std::max(by_rows, by_keys) * std::max(num_kv, 2) > 2147480000.0)
+    return QKV_ERR_UNSUPPORTED;
   return QKV_OK;
 }
 
 static size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
-static size_t weigh_total(const qkv::WeighPlan& x) { return round256(x.stat_bytes) + round256(x.rec_bytes) + round256(x.sum_bytes); }
+constexpr size_t kWeighCuts = 16 * qkv::kWeighGroups;
+static size_t weigh_total(const qkv::WeighPlan& x) {
+  return kWeighCuts + 2 * round256(4 * x.stat_rows) + round256(x.rec_bytes) + round256(x.sum_bytes);
+}
 
 size_t qkv_weigh_f8_paged_workspace_bytes(int num_q, int num_kv, int head_dim, int n_slots, int n_rows, int max_tok,
                                           int max_ctx) {
@@ -182,13 +187,13 @@ size_t qkv_weigh_f8_paged_workspace_bytes(int num_q, int num_kv, int head_dim, i
   if (max_tok > n_rows) max_tok = n_rows;
   const qkv::WeighPlan x = qkv::weigh_plan(num_q, num_kv, n_slots, n_rows, max_tok, max_ctx);
   // Calls with smaller numbers: their scores need at most kWeighScores bytes and at most those of up to 64 rows a
-  // slot at this context, their records a 64th of it (8 bytes for 128 scores or more) and their rows' statistics
-  // one of 32 bytes; the other sizes grow with each number.
+  // slot at this context, their records a 64th of it (8 bytes for 128 scores or more) and 8 bytes a row; the
+  // other sizes grow with each number.
   const double pitch = (max_ctx + 31.0) / 32 * 32, tokens = std::min(64 / (num_q / num_kv), max_tok);
-  const size_t most = (size_t)std::min((double)qkv::kWeighScores, (double)n_slots * tokens * num_q * pitch * 4);
   const size_t few_rows = (size_t)((double)n_slots * tokens * num_q);
-  return round256(std::max(x.stat_bytes, 8 * few_rows)) + round256(std::max(x.rec_bytes, most / 64 + 8 * few_rows)) +
-         round256(std::max(x.sum_bytes, most)) + 1024;
+  const size_t most = (size_t)std::min((double)qkv::kWeighScores, (double)few_rows * pitch * 4);
+  return kWeighCuts + 2 * round256(4 * std::max(x.stat_rows, few_rows)) + round256(std::max(x.rec_bytes, most / 64 + 8 * few_rows)) +
+         round256(std::max(x.sum_bytes, most));
 }
 
 int qkv_weigh_f8_paged(const uint16_t* q, const uint8_t* k_pool, const uint8_t* k_exp, float* weights, int n_rows,
@@ -220,10 +225,13 @@ int qkv_weigh_f8_paged(const uint16_t* q, const uint8_t* k_pool, const uint8_t* 
   a.starts = starts;
   a.positions = positions;
   a.weighed = weighed;
-  a.stat = reinterpret_cast<float*>(ws);
-  a.rec = reinterpret_cast<float*>(ws + round256(x.stat_bytes));
-  a.scores = reinterpret_cast<float*>(ws + round256(x.stat_bytes) + round256(x.rec_bytes));
-  a.partial = a.scores;   // (the one kind's launches are done before the other's)
+  const size_t stat = round256(4 * x.stat_rows);
+  a.cuts = reinterpret_cast<int*>(ws);
+  a.stat_m = reinterpret_cast<float*>(ws + kWeighCuts);
+  a.stat_il = reinterpret_cast<float*>(ws + kWeighCuts + stat);
+  a.rec = reinterpret_cast<float*>(ws + kWeighCuts + 2 * stat);
+  a.scores = reinterpret_cast<float*>(ws + kWeighCuts + 2 * stat + round256(x.rec_bytes));
+  a.sums = a.scores;   // (the one kind's launches are done before the other's)
   a.rows = n_rows;
   a.score_pitch = x.pitch;
   a.scale_log2 = scale * 1.4426950408889634f;

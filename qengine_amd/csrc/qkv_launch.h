@@ -242,9 +242,8 @@ int f8_attn_apart(int num_q, int num_kv, int head_dim, int n_slots, long rows, i
 hipError_t launch_f8_attn(const F8AttnArgs& a, const F8AttnPlan& plan, int head_dim, hipStream_t stream);
 
 // Attention weights of the keys of the paged 8-bit cache, accumulated (weigh_f8.hip).
-constexpr int kWeighRows = 256, kWeighKeys = 256;   // rows, keys of a workgroup of the kernels for many rows
-constexpr int kWeighChunk = 1024;                   // keys of the one, rows of the other that it passes by
-constexpr int kWeighSpan = 2048;
+constexpr int kWeighGroups = 256;                          // workgroups of the kernels for many rows, one on each CU
+constexpr size_t kWeighRec = 2 * kWeighGroups * 512 * 8;   // bytes of their records of rows, twice those of keys
 constexpr long kWeighScores = 256l << 20;           // bytes of scores that a call may store
 struct WeighArgs {
   const uint16_t* q;         // [rows][num_q][head_dim]
@@ -255,10 +254,12 @@ struct WeighArgs {
   const int32_t* starts;
   const int32_t* positions;
   const int32_t* weighed;    // [n_slots] keys whose weights stand, nullptr: positions
-  float* rec;                // workspace: [rows of the launch][chunks] {m, l}
-  float* stat;               // workspace: [rows of the launch] {m, 1 / l}
+  float* rec;                // workspace: {m, l} [rows of the launch][chunks], or of cut tiles (many rows)
+  float* stat_m;             // workspace: m and 1 / l of the launch's rows
+  float* stat_il;
   float* scores;             // workspace: [rows of the launch][score_pitch] (few rows)
-  float* partial;            // workspace: [rows * gqa / kWeighSpan + n_slots][num_kv][max_ctx] (many rows)
+  float* sums;               // workspace, the same place: of cut tiles (many rows)
+  int* cuts;                 // workspace: [kWeighGroups][4] where each part begins
   long rows, score_pitch;
   float scale_log2, decay;
   int num_q, num_kv, n_slots, max_tok, max_ctx, max_blocks, block_tokens, n_pages, window, sink;
@@ -266,20 +267,18 @@ struct WeighArgs {
   uint32_t bt_magic, gqa_magic;   // as in F8AttnArgs
   // set by the launcher
   int from_tok, to_tok;      // the slots of a launch: those that own so many rows
-  int slot0, slot_end;       // and lie here
+  int slot0, heads;          // from here on, heads = slots * num_kv
   int local_tok;             // tokens of a slot in the workspace; 0: rows lie there as in q
   int chunk_keys, chunks;    // keys of a record, records of a row
-  int tile_rows;             // rows that share their records' number (0: a slot's)
-  int spans;                 // of kWeighSpan rows, of a slot with max_tok tokens
   int per;                   // workgroups of a (slot, KV head)
 };
 struct WeighPlan {
   int few_tok;               // slots of up to so many tokens store their scores,
   int few_slots;             // so many slots at a time
   bool many;                 // whether there may be others
-  int few_keys, few_chunks, many_chunks;
+  int few_keys, few_chunks;
   long pitch;
-  size_t stat_bytes, rec_bytes, sum_bytes;
+  size_t stat_rows, rec_bytes, sum_bytes;
 };
 WeighPlan weigh_plan(int num_q, int num_kv, int n_slots, long rows, int max_tok, int max_ctx);
 hipError_t launch_weigh(WeighArgs a, const WeighPlan& plan, int head_dim, hipStream_t stream);

@@ -17,6 +17,7 @@
 // exponential on and never rounded to fewer bits.  All sums are taken in one order, whatever the timing.
 #include <algorithm>
 
+#include "f8_line.h"
 #include "qkv_device.h"
 #include "qkv_launch.h"
 
@@ -26,6 +27,9 @@ namespace {
 
 typedef float f16x_t __attribute__((ext_vector_type(16)));
 typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(4))) const int32_t const_i32;   // (read by scalar loads)
+typedef __attribute__((address_space(3))) void lds_void;
+typedef __attribute__((address_space(1))) const void glb_void;
 
 __device__ __forceinline__ h2_t cvt2(uint32_t w, float scale, bool hi) {
   return hi ? __builtin_bit_cast(h2_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, true))
@@ -74,15 +78,19 @@ struct Slot {
   int t0, n, pos0, end;
 };
 __device__ __forceinline__ Slot slot_of(const WeighArgs& p, int s) {
+  const const_i32 *starts = (const const_i32*)p.starts + s, *positions = (const const_i32*)p.positions + s;
   Slot x;
-  x.t0 = min(max(p.starts[s], 0), (int)p.rows);
-  x.n = min(min(max(p.starts[s + 1], x.t0), (int)p.rows) - x.t0, p.max_tok);
-  x.pos0 = p.positions[s];
+  x.t0 = min(max(starts[0], 0), (int)p.rows);
+  x.n = min(min(max(starts[1], x.t0), (int)p.rows) - x.t0, p.max_tok);
+  x.pos0 = positions[0];
   if (x.pos0 < 0 || x.pos0 > kMaxPosition || x.n < p.from_tok || x.n > p.to_tok) x.n = 0;
   x.end = (int)min((long)x.pos0 + x.n, (long)p.max_ctx);
   return x;
 }
-__device__ __forceinline__ int page_of(const WeighArgs& p, const int32_t* table, int block) {
+// (T: const_i32 for a block that the whole wave asks for, by a scalar load: a vector load's wait would be for all
+// loads under way)
+template <class T>
+__device__ __forceinline__ int page_of(const WeighArgs& p, const T* table, int block) {
   const int pg = block < p.max_blocks ? table[block] : -1;
   return pg >= 0 && pg < p.n_pages ? pg : -1;
 }
@@ -95,22 +103,29 @@ __device__ __forceinline__ long row_at(const WeighArgs& p, const Slot& x, int h,
   return (long)(x.t0 + tok) * p.num_q + h * p.gqa + (row - tok * p.gqa);
 }
 
-// Workgroup x of `per` for one (slot, KV head)
+// Workgroup x of those for one (slot, KV head).  Workgroups go round the XCDs in order, so the pairs are turned
+// by one with each x: no XCD has the same pair, or the same x, each time.
 struct Work {
   int x, s, h;
 };
 __device__ __forceinline__ bool work_of(const WeighArgs& p, Work& w) {
-  const uint32_t wg = blockIdx.y * kGridX + blockIdx.x, head = wg / (uint32_t)p.per;
-  w.x = (int)(wg - head * (uint32_t)p.per);
+  const uint32_t wg = blockIdx.y * kGridX + blockIdx.x, x = wg / (uint32_t)p.heads, head = (wg + x) % (uint32_t)p.heads;
+  w.x = (int)x;
   w.s = (int)(head / (uint32_t)p.num_kv);
   w.h = (int)(head - (uint32_t)w.s * (uint32_t)p.num_kv);
   w.s += p.slot0;
-  return w.s < p.slot_end;
+  return x < (uint32_t)p.per;
 }
 
 // Whether no row of the slot sees a key of the 32 from k0 on (a multiple of 32) for its window.
 __device__ __forceinline__ bool out_of_window(const WeighArgs& p, const Slot& x, int k0) {
   return p.window > 0 && k0 >= p.sink && k0 + 31 <= x.pos0 - p.window;
+}
+
+// m and 1 / l of a row; (infinity, 0) where it sees no key.
+__device__ __forceinline__ void put_stat(const WeighArgs& p, long at, Stat x) {
+  p.stat_m[at] = x.l == 0.f ? INFINITY : x.m;
+  p.stat_il[at] = x.l == 0.f ? 0.f : 1.f / x.l;
 }
 
 // Where the workspace holds a row's statistics (and scores): by its place in q, or, where a call's slots are taken
@@ -142,7 +157,7 @@ __global__ __launch_bounds__(256, 2) void weigh_scores_kernel(WeighArgs p) {
   const int first = chunk * p.chunk_keys, end = min(sl.end, first + p.chunk_keys);
   if (sl.n <= 0 || first >= sl.end) return;
   const int rows = sl.n * p.gqa;
-  const int32_t* table = p.tables + (long)s * p.max_blocks;
+  const const_i32* table = (const const_i32*)(p.tables + (long)s * p.max_blocks);
   const uint32_t key_bytes = (uint32_t)p.num_kv * HD;
 
   u4_t kr[2][KW];
@@ -245,24 +260,28 @@ __global__ __launch_bounds__(256, 2) void weigh_scores_kernel(WeighArgs p) {
   }
 }
 
-// m and 1 / l of every row from its chunks' statistics, 16 lanes a row; (infinity, 0) where a row sees no key.
-__global__ __launch_bounds__(256) void weigh_merge_kernel(WeighArgs p) {
-  Work wk;
-  if (!work_of(p, wk)) return;
-  const int tid = threadIdx.x, part = tid & 15, s = wk.s, h = wk.h;
-  const Slot sl = slot_of(p, s);
-  const int row = wk.x * 16 + (tid >> 4), rows = sl.n * p.gqa;
-  if (row >= rows) return;
-  // the chunks that the row's tile was formed over
-  const int tile_end = p.tile_rows ? min(sl.pos0 + token_of(p, min(rows, (row / p.tile_rows + 1) * p.tile_rows) - 1) + 1, p.max_ctx) : sl.end;
-  const int n = (tile_end + p.chunk_keys - 1) / p.chunk_keys;
-  const long at = place_of(p, sl, s, h, row);
+// A row's statistics from its chunks', by 16 neighbouring lanes (lane `part` of them), in each of these.
+__device__ __forceinline__ Stat join_chunks(const WeighArgs& p, const Slot& sl, long at, int part) {
+  const int n = (sl.end + p.chunk_keys - 1) / p.chunk_keys;
   const f2_t* rec = reinterpret_cast<const f2_t*>(p.rec) + at * p.chunks;
   Stat x{-INFINITY, 0.f};
   for (int c = part; c < n; c += 16) x = join(x, Stat{rec[c][0], rec[c][1]});
 #pragma unroll
   for (int d = 8; d; d >>= 1) x = join(x, Stat{__shfl_xor(x.m, d), __shfl_xor(x.l, d)});
-  if (part == 0) *reinterpret_cast<f2_t*>(p.stat + 2 * at) = x.l == 0.f ? f2_t{INFINITY, 0.f} : f2_t{x.m, 1.f / x.l};
+  return x;
+}
+
+// The statistics of every row, where the next kernel's workgroups would be long in joining those of a slot each.
+__global__ __launch_bounds__(256) void weigh_merge_kernel(WeighArgs p) {
+  Work wk;
+  if (!work_of(p, wk)) return;
+  const int tid = threadIdx.x, s = wk.s, h = wk.h;
+  const Slot sl = slot_of(p, s);
+  const int row = wk.x * 16 + (tid >> 4);
+  if (row >= sl.n * p.gqa) return;
+  const long at = place_of(p, sl, s, h, row);
+  const Stat x = join_chunks(p, sl, at, tid & 15);
+  if ((tid & 15) == 0) put_stat(p, at, x);
 }
 
 // What a key's weight becomes (a key whose page is absent has none).
@@ -274,7 +293,8 @@ __device__ __forceinline__ void put_weight(const WeighArgs& p, const int32_t* ta
   *w = key < weighed && p.decay != 0.f ? __builtin_fmaf(p.decay, *w, a) : a;
 }
 
-// Few rows: 1,024 keys a workgroup, four of a thread.
+// Few rows: 1,024 keys a workgroup, four of a thread.  MERGED: by the rows' statistics, else by their chunks'.
+template <bool MERGED>
 __global__ __launch_bounds__(256) void weigh_few_kernel(WeighArgs p) {
   constexpr int ROWS = 64;
   __shared__ f2_t stat[ROWS];
@@ -286,10 +306,21 @@ __global__ __launch_bounds__(256) void weigh_few_kernel(WeighArgs p) {
   const int key = wk.x * 1024 + 4 * tid;
   if (sl.n <= 0 || wk.x * 1024 >= sl.end) return;
   const int rows = sl.n * p.gqa;
-  if (tid < rows) {
-    const long x = place_of(p, sl, s, h, tid);
-    at[tid] = x * p.score_pitch;
-    stat[tid] = *reinterpret_cast<const f2_t*>(p.stat + 2 * x);
+  if constexpr (MERGED) {
+    if (tid < rows) {
+      const long x = place_of(p, sl, s, h, tid);
+      at[tid] = x * p.score_pitch;
+      stat[tid] = f2_t{p.stat_m[x], p.stat_il[x]};
+    }
+  } else {
+    for (int r = tid >> 4; r < rows; r += 16) {
+      const long x = place_of(p, sl, s, h, r);
+      const Stat st = join_chunks(p, sl, x, tid & 15);
+      if ((tid & 15) == 0) {
+        at[r] = x * p.score_pitch;
+        stat[r] = st.l == 0.f ? f2_t{INFINITY, 0.f} : f2_t{st.m, 1.f / st.l};
+      }
+    }
   }
   __syncthreads();
   if (key >= sl.end) return;
@@ -310,255 +341,478 @@ __global__ __launch_bounds__(256) void weigh_few_kernel(WeighArgs p) {
 // ---------------------------------------------------------------------------
 // many rows
 // ---------------------------------------------------------------------------
-// Statistics: four waves of 64 rows, whose queries stay in registers, over chunk_keys keys, 32 at a time through
-// LDS as fp16 (converted once for all waves).
-template <int HD>
-__global__ __launch_bounds__(256, 2) void weigh_stats_kernel(WeighArgs p) {
-  constexpr int KT = 32, KP = HD * 2 + 16, NB = HD / 16, LD = HD / 128;   // LD: 16-byte loads of a thread and tile
-  __shared__ __align__(16) uint8_t k_lds[2][KT * KP];
-  __shared__ int page_lds[2][2];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int c = lane & 31, hh = lane >> 5;
-  Work wk;
-  if (!work_of(p, wk)) return;
-  const int tile = wk.x / p.chunks, chunk = wk.x - tile * p.chunks, h = wk.h, s = wk.s;
-  const Slot sl = slot_of(p, s);
-  const int rows = sl.n * p.gqa, r0 = tile * kWeighRows;
-  if (sl.n <= 0 || r0 >= rows) return;
-  const int tile_lo = sl.pos0 + token_of(p, r0), tile_hi = sl.pos0 + token_of(p, min(rows, r0 + kWeighRows) - 1);
-  const int end = min(tile_hi + 1, p.max_ctx), first = chunk * p.chunk_keys;
-  if (first >= end) return;
-  const int32_t* table = p.tables + (long)s * p.max_blocks;
-  const uint32_t key_bytes = (uint32_t)p.num_kv * HD;
+// Both kernels: eight waves of 64 stationary rows (or keys) in registers, the others 64 at a step through a ring of
+// kRing LDS tiles that are loaded past the registers, kRing - 1 steps ahead.  A tile's rows are stored as they are,
+// but for their 16-byte words, which are permuted by the row's number so that 16 rows' same word lies on distinct
+// banks.  Operand dims: lane l's 16-byte word of codes holds the dims of two products.
+//
+// Work: the steps of all stationary tiles, KV heads and slots form one line that is cut into equal parts, a
+// workgroup's each, so ragged and causal lengths balance by themselves (workgroups of 64 to 512 rows by 512 to
+// 1,024 keys as launched: 1.6 to 2 times as long).  A tile that lies in one part is finished there; one that is cut
+// leaves records that a second kernel joins.
+constexpr int kRing = 4, kWaves = 8, kTile = 64 * kWaves, kThreads = 64 * kWaves;
+constexpr int kWeighLead = 3;   // steps that a tile costs beside its own
 
-  const int row_w = r0 + wave * 64;
-  h8_t qf[2][NB];
-  int pos[2];
-  long at[2];
-#pragma unroll
-  for (int b = 0; b < 2; b++) {
-    const int row = min(row_w + 32 * b + c, rows - 1);
-    at[b] = row_at(p, sl, h, row);
-    pos[b] = sl.pos0 + token_of(p, row);
-    const uint16_t* src = p.q + at[b] * HD + 8 * hh;
-#pragma unroll
-    for (int i = 0; i < NB; i++) qf[b][i] = *reinterpret_cast<const h8_t*>(src + 16 * i);
-  }
-  const bool live = row_w < rows;
-  const int pos_lo = sl.pos0 + token_of(p, min(row_w, rows - 1)), pos_hi = sl.pos0 + token_of(p, min(row_w + 64, rows) - 1);
-
-  // tiles of the chunk that some row sees: on to the window past the sinks
-  const int stop = min(end, first + p.chunk_keys);
-  const int w0 = p.window > 0 ? max(0, tile_lo - p.window + 1) / KT * KT : 0;
-  auto skip = [&](int k0) { return k0 >= p.sink && k0 < w0 ? max(w0, first) : k0; };
-
-  u4_t raw[LD];
-  uint32_t ex = 0;
-  int pg = -1;
-  const int ld_key = tid >> 3, ld_part = tid & 7;
-  auto load = [&](int k0) {
-    const BlockAt x = block_at(p, k0 + ld_key);
-    pg = k0 + ld_key < end ? page_of(p, table, x.b) : -1;
-    const long page = max(pg, 0);
-    const uint8_t* src = p.k_pool + (page * p.block_tokens + x.row) * key_bytes + h * HD + ld_part * 16 * LD;
-    ex = p.k_exp[page * p.num_kv + h];
-#pragma unroll
-    for (int i = 0; i < LD; i++) raw[i] = *reinterpret_cast<const u4_t*>(src + 16 * i);
+// The tiles of a slot's rows and their steps over keys: v below n_sink are key steps v, then w0 on.
+struct RowTiles {
+  const WeighArgs& p;
+  struct Tile {
+    int steps, n_sink, w0, end;
+    __device__ __forceinline__ int first(int v) const { return (v < n_sink ? v : v - n_sink + w0) * 64; }
   };
-  auto store = [&](int buf) {
-    const float f = pow2f(ex);
-    uint8_t* dst = k_lds[buf] + ld_key * KP + ld_part * 32 * LD;
-#pragma unroll
-    for (int i = 0; i < LD; i++) {
-      *reinterpret_cast<h8_t*>(dst + 32 * i) = cvt8(raw[i][0], raw[i][1], f);
-      *reinterpret_cast<h8_t*>(dst + 32 * i + 16) = cvt8(raw[i][2], raw[i][3], f);
-    }
-    if ((ld_key & 15) == 0 && ld_part == 0) page_lds[buf][ld_key >> 4] = pg;
+  __device__ __forceinline__ int count(const Slot& x) const { return (x.n * p.gqa + kTile - 1) / kTile; }
+  __device__ __forceinline__ Tile tile(const Slot& x, int i) const {
+    const int lo = x.pos0 + token_of(p, i * kTile), hi = x.pos0 + token_of(p, min(x.n * p.gqa, (i + 1) * kTile) - 1);
+    Tile t;
+    t.end = min(hi + 1, p.max_ctx);
+    t.w0 = p.window > 0 ? max(0, lo - p.window + 1) / 64 : 0;
+    t.n_sink = p.window > 0 ? min((p.sink + 63) / 64, t.w0) : 0;
+    // (the window may lie past max_ctx: then the sinks alone)
+    t.steps = t.n_sink + max(0, (t.end + 63) / 64 - t.w0);
+    return t;
+  }
+};
+
+// The tiles of a slot's keys and their steps over the rows r_lo .. r_hi-1 that see a key of the tile.
+struct KeyTiles {
+  const WeighArgs& p;
+  struct Tile {
+    int steps, r_lo, r_hi;
   };
-  Stat st[2] = {{-INFINITY, 0.f}, {-INFINITY, 0.f}};
-  int k0 = skip(first), buf = 0;
-  if (k0 < stop) {
-    load(k0);
-    store(0);
+  __device__ __forceinline__ int count(const Slot& x) const { return x.n > 0 ? (x.end + kTile - 1) / kTile : 0; }
+  __device__ __forceinline__ Tile tile(const Slot& x, int i) const {
+    const int k0 = i * kTile, k1 = min(k0 + kTile, x.end) - 1;
+    long hi = (long)x.n * p.gqa;
+    if (p.window > 0 && k0 >= p.sink) hi = min(hi, max(0l, (long)k1 + p.window - x.pos0) * p.gqa);
+    Tile t;
+    t.r_hi = (int)hi;
+    t.r_lo = (int)min((long)max(0, k0 - x.pos0) * p.gqa / 64 * 64, hi);
+    t.steps = (t.r_hi - t.r_lo + 63) / 64;
+    return t;
   }
-  while (k0 < stop) {
-    const int next = skip(k0 + KT);
-    if (next < stop) load(next);
-    __syncthreads();   // (this tile is stored; the one before is done with)
-    const int pg0 = page_lds[buf][0], pg1 = page_lds[buf][1];
-    if (live && k0 <= pos_hi) {
-      f16x_t acc[2] = {f16x_t{}, f16x_t{}};
-      const uint8_t* src = k_lds[buf] + c * KP + 16 * hh;
-#pragma unroll
-      for (int i = 0; i < NB; i++) {
-        const h8_t a = *reinterpret_cast<const h8_t*>(src + 32 * i);
-#pragma unroll
-        for (int b = 0; b < 2; b++) acc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qf[b][i], acc[b], 0, 0, 0);
-      }
-      const bool whole = pg0 >= 0 && pg1 >= 0 && k0 + KT - 1 <= pos_lo && k0 + KT <= end &&
-                         (p.window <= 0 || k0 > pos_hi - p.window || k0 + KT <= p.sink);
-#pragma unroll
-      for (int b = 0; b < 2; b++) {
-        // lane c's row, keys 8 (x / 4) + 4 hh + x % 4
-        float top = -INFINITY;
-        uint32_t seen = 0xffffu;
-        if (!whole) {
-          seen = 0;
-#pragma unroll
-          for (int x = 0; x < 16; x++)
-            seen |= (x < 8 ? pg0 : pg1) >= 0 && sees(p, k0 + 8 * (x >> 2) + 4 * hh + (x & 3), pos[b], end) ? 1u << x : 0u;
-#pragma unroll
-          for (int x = 0; x < 16; x++) top = fmaxf(top, seen >> x & 1 ? acc[b][x] * p.scale_log2 : -INFINITY);
-        } else {
-#pragma unroll
-          for (int x = 0; x < 16; x++) top = fmaxf(top, acc[b][x] * p.scale_log2);
+};
+
+struct LineLds {
+  int scan[kWaves], upto[kThreads], found[3];
+};
+
+// The line of one head, walked kThreads slots at a time: their tiles are counted, then taken up by as many threads as
+// there are.
+template <class Tiles>
+struct TileLine {
+  const WeighArgs& p;
+  const Tiles& tiles;
+  LineLds& lds;
+  int s, i, mine, inc;         // this thread's tile of the last step, its units and the line's up to its end
+  bool one = true;             // the line is one step: what the registers hold
+
+  template <class F>
+  __device__ __forceinline__ void walk(F&& done) {   // done(units so far): whether to stop
+    int base = 0;
+    for (int s0 = 0; s0 < p.n_slots; s0 += kThreads) {
+      const int mine_s = s0 + (int)threadIdx.x;
+      int n;
+      const int count = mine_s < p.n_slots ? tiles.count(slot_of(p, mine_s)) : 0;
+      lds.upto[threadIdx.x] = block_scan<kThreads>(count, lds.scan, n);
+      __syncthreads();
+      n = __builtin_amdgcn_readfirstlane(n);
+      for (int x0 = 0; x0 < n; x0 += kThreads) {
+        const int x = x0 + (int)threadIdx.x;
+        mine = 0;
+        if (x < n) {
+          int lo = 0, hi = kThreads - 1;   // the first slot whose tiles end past x
+          for (int w = kThreads / 2; w; w >>= 1) {
+            const int mid = (lo + hi) / 2;
+            if (lds.upto[mid] > x) hi = mid; else lo = mid + 1;
+          }
+          s = s0 + lo;
+          i = x - (lo ? lds.upto[lo - 1] : 0);
+          mine = kWeighLead + tiles.tile(slot_of(p, s), i).steps;
         }
-        const float mn = fmaxf(st[b].m, top), ref = mn == -INFINITY ? 0.f : mn;
-        float l = st[b].l * __builtin_amdgcn_exp2f(st[b].m - ref);
-#pragma unroll
-        for (int x = 0; x < 16; x++) {
-          const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[b][x], p.scale_log2, -ref));
-          l += whole || (seen >> x & 1) ? w : 0.f;
-        }
-        st[b] = {mn, l};
+        int sum;
+        inc = add_units(base, block_scan<kThreads>(mine, lds.scan, sum));
+        base = __builtin_amdgcn_readfirstlane(add_units(base, sum));
+        if (done(base)) return;
       }
+      __syncthreads();   // (upto is written again)
     }
-    buf ^= 1;
-    if (next < stop) store(buf);
-    k0 = next;
   }
-#pragma unroll
-  for (int b = 0; b < 2; b++) {
-    const Stat x = join(st[b], Stat{other32(st[b].m, lane), other32(st[b].l, lane)});
-    if (hh == 0 && row_w + 32 * b + c < rows) *reinterpret_cast<f2_t*>(p.rec + (at[b] * p.chunks + chunk) * 2) = f2_t{x.m, x.l};
+  // units of the line (0: too many, which starts in order cannot make)
+  __device__ __forceinline__ int units() {
+    int total = 0, steps = 0;
+    walk([&](int so_far) {
+      total = so_far;
+      steps++;
+      return false;
+    });
+    one = steps <= 1;
+    return total < kLineMax && (long)total * p.num_kv < (1l << 31) ? total : 0;
+  }
+  // the tile that holds unit u of the line (u < its length), and the unit in it
+  __device__ __forceinline__ void find(int u, int& slot, int& tile, int& at) {
+    auto look = [&](int so_far) {
+      if (u >= inc - mine && u < inc) {
+        lds.found[0] = s;
+        lds.found[1] = i;
+        lds.found[2] = u - (inc - mine);
+      }
+      return so_far > u;
+    };
+    if (one) look(0); else walk(look);
+    __syncthreads();
+    slot = __builtin_amdgcn_readfirstlane(lds.found[0]);
+    tile = __builtin_amdgcn_readfirstlane(lds.found[1]);
+    at = __builtin_amdgcn_readfirstlane(lds.found[2]);
+  }
+};
+
+// This workgroup's part: body(slot, its number, head, tile's number, tile, steps v0 .. v1-1, whether these are all,
+// record) for each tile that it has steps of.  Where a part begins is noted for the second kernel: {slot (-1: no part),
+// tile, head, step}.
+template <class Tiles, class Body>
+__device__ __forceinline__ void run_part(const WeighArgs& p, const Tiles& tiles, LineLds& lds, Body&& body) {
+  TileLine<Tiles> line{p, tiles, lds};
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int total = __builtin_amdgcn_readfirstlane(line.units());
+  const Parts parts(__builtin_amdgcn_readfirstlane(total * p.num_kv), kWeighGroups);
+  // neighbouring parts (the same head's keys and rows) on one XCD, whose L2 holds them
+  const int grp = (int)(blockIdx.x % 8) * (kWeighGroups / 8) + (int)blockIdx.x / 8;
+  int4* cuts = reinterpret_cast<int4*>(p.cuts);
+  if (grp >= parts.n) {
+    if (tid == 0) cuts[grp] = make_int4(-1, 0, 0, 0);
+    return;
+  }
+  int u = parts.begin(grp);
+  const int u_end = parts.begin(grp + 1);
+  int h = u / total, s, i, at;
+  line.find(u - h * total, s, i, at);
+  bool first = true;
+  while (u < u_end) {
+    const Slot sl = slot_of(p, s);
+    if (i >= tiles.count(sl)) {   // on to the next slot with tiles, 64 at a time
+      uint64_t any = 0;
+      int t = s + 1;
+      while (true) {
+        if (t >= p.n_slots) {
+          t = 0;
+          if (++h >= p.num_kv) return;   // (starts or positions that change under the call)
+        }
+        any = __builtin_amdgcn_ballot_w64(t + lane < p.n_slots && tiles.count(slot_of(p, min(t + lane, p.n_slots - 1))) > 0);
+        if (any) break;
+        t += 64;
+      }
+      s = t + (int)__builtin_ctzll(any);
+      i = 0;
+      continue;
+    }
+    const auto t = tiles.tile(sl, i);
+    const int n_u = min(kWeighLead + t.steps - at, u_end - u);
+    if (n_u <= 0) return;
+    const int v0 = max(at - kWeighLead, 0), v1 = at + n_u - kWeighLead;   // (v1 <= v0: the next part's, or no step at all)
+    if (first && tid == 0) cuts[grp] = make_int4(s, i, h, v0);
+    if (v1 > v0 || (t.steps == 0 && v1 == 0)) body(sl, s, h, i, t, v0, v1, v0 == 0 && v1 == t.steps, 2 * grp + (first ? 0 : 1));
+    u += n_u;
+    first = false;
+    at = 0;
+    i++;
   }
 }
 
-// Sums: four waves of 64 keys, which stay in registers as fp16, over kWeighSpan rows, 32 at a time through LDS.
+// The tile that part g continues, if it was begun in part g - 1: its records are `first`, then 2 g, 2 (g + 1) .. of the
+// n - 1 parts that continue it.
+struct CutTile {
+  int s, i, h, first, n, g;
+  __device__ __forceinline__ long record(int x) const { return x == 0 ? first : 2 * (g + x - 1); }
+};
+__device__ __forceinline__ bool cut_tile(const WeighArgs& p, CutTile& c) {
+  __shared__ int4 cuts[kWeighGroups];
+  for (int x = threadIdx.x; x < kWeighGroups; x += kThreads) cuts[x] = reinterpret_cast<const int4*>(p.cuts)[x];
+  __syncthreads();
+  const int g = (int)blockIdx.x + 1;
+  const int4 here = cuts[g], before = cuts[g - 1];
+  auto same = [&](const int4& a) { return a.x == here.x && a.y == here.y && a.z == here.z; };
+  if (here.x < 0 || here.w <= 0 || (same(before) && before.w > 0)) return false;
+  c = {here.x, here.y, here.z, 2 * (g - 1) + (same(before) ? 0 : 1), 2, g};
+  while (g + c.n - 1 < kWeighGroups && same(cuts[g + c.n - 1])) c.n++;
+  return true;
+}
+
+// Statistics of rows.  Codes are converted by each wave as it reads them (16 conversions beside 4 products of 32
+// cycles).  The pages of kLook steps and their exponents are looked up at a time.
 template <int HD>
-__global__ __launch_bounds__(256, 2) void weigh_sums_kernel(WeighArgs p) {
-  constexpr int RT = 32, QP = HD * 2 + 16, NB = HD / 16, LD = HD / 64;   // LD: 16-byte loads of a thread and tile
-  __shared__ __align__(16) uint8_t q_lds[2][RT * QP];
-  __shared__ __align__(16) float m_lds[2][RT], il_lds[2][RT];
-  __shared__ __align__(16) int pos_lds[2][RT];
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void weigh_stats_kernel(WeighArgs p) {
+  constexpr int NB = HD / 32, TB = 64 * HD, LOADS = TB / 1024 / kWaves, RL = 1024 / HD, kLook = 256;
+  __shared__ __align__(16) uint8_t ring[kRing][TB];
+  __shared__ int page_lds[kLook * 4];        // of every 16 keys, -1: none
+  __shared__ float exp_lds[kLook * 4];
+  __shared__ LineLds lds;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 31, hh = lane >> 5;
-  Work wk;
-  if (!work_of(p, wk)) return;
-  const int tile = wk.x / p.spans, span = wk.x - tile * p.spans, h = wk.h, s = wk.s;
-  const Slot sl = slot_of(p, s);
-  const int rows = sl.n * p.gqa, k0 = tile * kWeighKeys;
-  if (sl.n <= 0 || k0 >= sl.end || span * kWeighSpan >= rows) return;
-  const int32_t* table = p.tables + (long)s * p.max_blocks;
   const uint32_t key_bytes = (uint32_t)p.num_kv * HD;
-  const int key_w = k0 + wave * 64;
-
-  // rows of the span that see a key of the tile
-  const int k1 = min(k0 + kWeighKeys, sl.end) - 1;
-  long lo = (long)max(0, k0 - sl.pos0) * p.gqa, hi = rows;
-  if (p.window > 0 && k0 >= p.sink) hi = min(hi, max(0l, (long)k1 + p.window - sl.pos0) * p.gqa);
-  const int r_lo = (int)max(lo, (long)span * kWeighSpan) / RT * RT, r_hi = (int)min(hi, (long)(span + 1) * kWeighSpan);
-
-  h8_t kf[2][NB];
-  float sum[2] = {0.f, 0.f};
-  if (r_lo < r_hi) {
+  run_part(p, RowTiles{p}, lds, [&](const Slot& sl, int s, int h, int i, const RowTiles::Tile& t, int v0, int v1, bool all, int rec)
+                                    __attribute__((always_inline)) {
+    const int rows = sl.n * p.gqa, row_w = i * kTile + wave * 64;
+    h8_t qf[2][NB][2];
+    const bool live = row_w < rows;
+    const int pos_lo = sl.pos0 + token_of(p, min(row_w, rows - 1)), pos_hi = sl.pos0 + token_of(p, min(row_w + 64, rows) - 1);
+    // keys that lane c's rows see: above `from` (or below the sinks), up to `upto`
+    int from[2], upto[2];
 #pragma unroll
     for (int b = 0; b < 2; b++) {
-      const int key = key_w + 32 * b + c;
-      const BlockAt x = block_at(p, min(key, sl.end - 1));
-      const long page = max(page_of(p, table, x.b), 0);
-      const uint8_t* src = p.k_pool + (page * p.block_tokens + x.row) * key_bytes + h * HD + 8 * hh;
-      const float f = pow2f(p.k_exp[page * p.num_kv + h]);
-#pragma unroll
-      for (int i = 0; i < NB; i++) {
-        const u2_t w = *reinterpret_cast<const u2_t*>(src + 16 * i);
-        kf[b][i] = cvt8(w[0], w[1], f);
-      }
+      const int pos = sl.pos0 + token_of(p, min(row_w + 32 * b + c, rows - 1));
+      from[b] = p.window > 0 ? pos - p.window : -1;
+      upto[b] = min(pos, t.end - 1);
     }
-  }
-  u4_t raw[LD];
-  f2_t stat = {0.f, 0.f};
-  int pos = 0;
-  const int ld_row = tid >> 3, ld_part = tid & 7;
-  auto load = [&](int r0) {
-    const int row = min(r0 + ld_row, rows - 1);
-    const long at = row_at(p, sl, h, row);
-    const uint16_t* src = p.q + at * HD + ld_part * 8 * LD;
-#pragma unroll
-    for (int i = 0; i < LD; i++) raw[i] = *reinterpret_cast<const u4_t*>(src + 8 * i);
-    stat = *reinterpret_cast<const f2_t*>(p.stat + 2 * at);
-    pos = r0 + ld_row < r_hi ? sl.pos0 + token_of(p, row) : -1;   // (-1: no row, sees nothing)
-  };
-  auto store = [&](int buf) {
-    uint8_t* dst = q_lds[buf] + ld_row * QP + ld_part * 16 * LD;
-#pragma unroll
-    for (int i = 0; i < LD; i++) *reinterpret_cast<u4_t*>(dst + 16 * i) = raw[i];
-    if (ld_part == 0) {
-      m_lds[buf][ld_row] = stat[0];
-      il_lds[buf][ld_row] = stat[1];
-      pos_lds[buf][ld_row] = pos;
-    }
-  };
-  int buf = 0;
-  if (r_lo < r_hi) {
-    load(r_lo);
-    store(0);
-  }
-  for (int r0 = r_lo; r0 < r_hi; r0 += RT) {
-    if (r0 + RT < r_hi) load(r0 + RT);
-    __syncthreads();
-    const int pos_lo = r0 + RT <= r_hi ? pos_lds[buf][0] : -1, pos_hi = sl.pos0 + token_of(p, min(r0 + RT, rows) - 1);
-    if (key_w <= pos_hi) {
-      f16x_t acc[2] = {f16x_t{}, f16x_t{}};
-      const uint8_t* src = q_lds[buf] + c * QP + 16 * hh;
-#pragma unroll
-      for (int i = 0; i < NB; i++) {
-        const h8_t a = *reinterpret_cast<const h8_t*>(src + 32 * i);
-#pragma unroll
-        for (int b = 0; b < 2; b++) acc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, kf[b][i], acc[b], 0, 0, 0);
+    Stat st[2] = {{-INFINITY, 0.f}, {-INFINITY, 0.f}};
+    for (int va = v0; va < v1; va += kLook) {
+      const int vb = min(va + kLook, v1);
+      __syncthreads();   // (the ring and the pages are written again)
+      for (int x = tid; x < 4 * (vb - va); x += kThreads) {
+        const int key = t.first(va + (x >> 2)) + 16 * (x & 3);
+        const int pg = key < t.end ? page_of(p, p.tables + (long)s * p.max_blocks, block_at(p, key).b) : -1;
+        page_lds[x] = pg;
+        exp_lds[x] = pow2f(p.k_exp[(long)max(pg, 0) * p.num_kv + h]);
       }
-      const bool whole = key_w + 63 <= pos_lo && (p.window <= 0 || key_w > pos_hi - p.window || key_w + 64 <= p.sink);
-      // lane c's key, rows 8 (x / 4) + 4 hh + x % 4
+      __syncthreads();
+      // the wave's part of a step: LOADS times RL keys (past the last step it is loaded again, so that as many loads
+      // are under way as are counted)
+      auto load = [&](int v, int buf) {
+        v = min(v, vb - 1);
+        const int k0 = t.first(v);
 #pragma unroll
-      for (int x4 = 0; x4 < 4; x4++) {
-        const f4_t mr = *reinterpret_cast<const f4_t*>(&m_lds[buf][8 * x4 + 4 * hh]);
-        const f4_t il = *reinterpret_cast<const f4_t*>(&il_lds[buf][8 * x4 + 4 * hh]);
-        const int4 pr = *reinterpret_cast<const int4*>(&pos_lds[buf][8 * x4 + 4 * hh]);
-        const int pos_r[4] = {pr.x, pr.y, pr.z, pr.w};
+        for (int j = 0; j < LOADS; j++) {
+          const int x = (wave * LOADS + j) * RL + lane / (HD / 16), word = (lane % (HD / 16)) ^ (x & (HD / 16 - 1));
+          const long page = max(page_lds[4 * (v - va) + (x >> 4)], 0);
+          const uint8_t* src = p.k_pool + (page * p.block_tokens + block_at(p, k0 + x).row) * key_bytes + h * HD + 16 * word;
+          __builtin_amdgcn_global_load_lds((glb_void*)src, (lds_void*)(ring[buf] + (wave * LOADS + j) * 1024), 16, 0, 0);
+        }
+      };
 #pragma unroll
-        for (int b = 0; b < 2; b++)
+      for (int j = 0; j < kRing - 1; j++) load(va + j, j);
+      if (va == v0) {
 #pragma unroll
-          for (int x = 0; x < 4; x++) {
-            float w = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[b][4 * x4 + x], p.scale_log2, -mr[x])) * il[x];
-            if (!whole && !sees(p, key_w + 32 * b + c, pos_r[x], sl.end)) w = 0.f;
-            sum[b] += w;
+        for (int b = 0; b < 2; b++) {
+          const uint16_t* src = p.q + row_at(p, sl, h, min(row_w + 32 * b + c, rows - 1)) * HD + 16 * hh;
+#pragma unroll
+          for (int j = 0; j < NB; j++)
+#pragma unroll
+            for (int x = 0; x < 2; x++) qf[b][j][x] = *reinterpret_cast<const h8_t*>(src + 32 * j + 8 * x);
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // (from here on only steps are under way)
+      }
+      for (int v = va; v < vb; v++) {
+        const int buf = (v - va) % kRing;
+        // this step has landed, for every wave, and every wave has read the one before
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((kRing - 2) * LOADS) : "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        load(v + kRing - 1, (v - va + kRing - 1) % kRing);
+        const int k0 = t.first(v);
+#pragma unroll
+        for (int half = 0; half < 2; half++) {
+          const int kh = k0 + 32 * half;
+          if (!live || kh > pos_hi || kh >= t.end) continue;
+          const int pi = 4 * (v - va) + 2 * half, pg0 = page_lds[pi], pg1 = page_lds[pi + 1];
+          const float f = exp_lds[pi + (c >> 4)];
+          f16x_t acc[2] = {f16x_t{}, f16x_t{}};
+          // (ahead of the other wave's exponentials: 101 -> 90 us for 8.6 million pairs of 16 heads of 256)
+          __builtin_amdgcn_s_setprio(1);
+          const uint8_t* src = ring[buf] + (32 * half + c) * HD;
+#pragma unroll
+          for (int j = 0; j < NB; j++) {
+            const u4_t w = *reinterpret_cast<const u4_t*>(src + (((2 * j + hh) ^ ((32 * half + c) & (HD / 16 - 1))) * 16));
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+              const h8_t a = cvt8(w[2 * x], w[2 * x + 1], f);
+#pragma unroll
+              for (int b = 0; b < 2; b++) acc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qf[b][j][x], acc[b], 0, 0, 0);
+            }
           }
+          __builtin_amdgcn_s_setprio(0);
+          const bool whole = pg0 >= 0 && pg1 >= 0 && kh + 31 <= pos_lo && kh + 32 <= t.end &&
+                             (p.window <= 0 || kh > pos_hi - p.window || kh + 32 <= p.sink);
+#pragma unroll
+          for (int b = 0; b < 2; b++) {
+            // lane c's row, keys 8 (x / 4) + 4 hh + x % 4
+            auto add = [&](auto&& seen) __attribute__((always_inline)) {
+              float top = -INFINITY;
+#pragma unroll
+              for (int x = 0; x < 16; x++) top = fmaxf(top, seen(x) ? acc[b][x] * p.scale_log2 : -INFINITY);
+              const float mn = fmaxf(st[b].m, top), ref = mn == -INFINITY ? 0.f : mn;
+              float l = st[b].l * __builtin_amdgcn_exp2f(st[b].m - ref);
+#pragma unroll
+              for (int x = 0; x < 16; x++) {
+                const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[b][x], p.scale_log2, -ref));
+                l += seen(x) ? w : 0.f;
+              }
+              st[b] = {mn, l};
+            };
+            if (whole) {
+              add([](int) { return true; });
+            } else {
+              // (no key of an absent page: a bound past every key of it)
+              const int k = kh + 4 * hh, hi = upto[b] - k, lo = from[b] - k, sink = p.sink - k;
+              const int hi0 = pg0 >= 0 ? hi : -64, hi1 = pg1 >= 0 ? hi : -64;
+              add([&](int x) {
+                const int d = 8 * (x >> 2) + (x & 3);
+                return (d <= (x < 8 ? hi0 : hi1)) & ((d > lo) | (d < sink));
+              });
+            }
+          }
+        }
+      }
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // (no load into the ring is under way past here)
+    }
+#pragma unroll
+    for (int b = 0; b < 2; b++) {
+      const Stat x = join(st[b], Stat{other32(st[b].m, lane), other32(st[b].l, lane)});
+      const int r = wave * 64 + 32 * b + c, row = i * kTile + r;
+      if (hh == 0 && row < rows) {
+        if (all) put_stat(p, row_at(p, sl, h, row), x);
+        else *reinterpret_cast<f2_t*>(p.rec + ((long)rec * kTile + r) * 2) = f2_t{x.m, x.l};
       }
     }
-    buf ^= 1;
-    if (r0 + RT < r_hi) store(buf);
-  }
-  // (both halves of the lanes have the same keys, other rows)
-  float* out = p.partial + ((long)(sl.t0 * (long)p.gqa / kWeighSpan + s + span) * p.num_kv + h) * p.max_ctx;
-#pragma unroll
-  for (int b = 0; b < 2; b++) {
-    const float a = sum[b] + other32(sum[b], lane);
-    if (hh == 0 && key_w + 32 * b + c < sl.end) out[key_w + 32 * b + c] = a;
-  }
+  });
 }
 
-// Many rows: the spans' sums into the weights.
-__global__ __launch_bounds__(256) void weigh_many_kernel(WeighArgs p) {
-  Work wk;
-  if (!work_of(p, wk)) return;
-  const int h = wk.h, s = wk.s, key = wk.x * 256 + (int)threadIdx.x;
-  const Slot sl = slot_of(p, s);
-  if (sl.n <= 0 || key >= sl.end) return;
-  const int spans = (sl.n * p.gqa + kWeighSpan - 1) / kWeighSpan;
-  const float* in = p.partial + ((long)(sl.t0 * (long)p.gqa / kWeighSpan + s) * p.num_kv + h) * p.max_ctx + key;
+__global__ __launch_bounds__(kThreads) void weigh_stats_join_kernel(WeighArgs p) {
+  CutTile c;
+  if (!cut_tile(p, c)) return;
+  Stat x{-INFINITY, 0.f};
+#pragma unroll 8
+  for (int j = 0; j < c.n; j++) {
+    const f2_t v = *reinterpret_cast<const f2_t*>(p.rec + (c.record(j) * kTile + threadIdx.x) * 2);
+    x = join(x, Stat{v[0], v[1]});
+  }
+  const Slot sl = slot_of(p, c.s);
+  const int row = c.i * kTile + (int)threadIdx.x;
+  if (row < sl.n * p.gqa) put_stat(p, row_at(p, sl, c.h, row), x);
+}
+
+// Sums of keys.  A step brings its rows' statistics along.
+template <int HD>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void weigh_sums_kernel(WeighArgs p) {
+  constexpr int NB = HD / 32, RB = HD * 2, TB = 64 * RB, LOADS = TB / 1024 / kWaves, WORDS = RB / 16;
+  __shared__ __align__(16) uint8_t ring[kRing][TB];
+  __shared__ __align__(16) float stat_lds[kRing][3][64];   // m, 1 / l, and what the other waves load beside them
+  __shared__ LineLds lds;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c = lane & 31, hh = lane >> 5;
+  const uint32_t key_bytes = (uint32_t)p.num_kv * HD;
+  run_part(p, KeyTiles{p}, lds, [&](const Slot& sl, int s, int h, int i, const KeyTiles::Tile& t, int v0, int v1, bool all, int rec)
+                                    __attribute__((always_inline)) {
+    const int rows = sl.n * p.gqa, key_w = i * kTile + wave * 64;
+    const int32_t* table = p.tables + (long)s * p.max_blocks;
+    float sum[2] = {0.f, 0.f};
+    if (v0 < v1) {
+      // the wave's part of a step, and a number for each of its rows: every wave as many loads
+      auto load = [&](int v, int buf) {
+        const int r0 = t.r_lo + 64 * min(v, v1 - 1);
+#pragma unroll
+        for (int j = 0; j < LOADS; j++) {
+          const int x = (wave * LOADS + j) * (1024 / RB) + lane / WORDS, word = (lane % WORDS) ^ (x & 15);
+          const uint16_t* src = p.q + row_at(p, sl, h, min(r0 + x, rows - 1)) * HD + 8 * word;
+          __builtin_amdgcn_global_load_lds((glb_void*)src, (lds_void*)(ring[buf] + (wave * LOADS + j) * 1024), 16, 0, 0);
+        }
+        const float* src = (wave == 1 ? p.stat_il : p.stat_m) + row_at(p, sl, h, min(r0 + lane, rows - 1));
+        __builtin_amdgcn_global_load_lds((glb_void*)src, (lds_void*)stat_lds[buf][min(wave, 2)], 4, 0, 0);
+      };
+      __syncthreads();   // (the ring is written again)
+#pragma unroll
+      for (int j = 0; j < kRing - 1; j++) load(v0 + j, j);
+      h8_t kf[2][NB][2];
+      int from[2], upto[2];   // rows that see lane c's keys: from .. upto-1
+#pragma unroll
+      for (int b = 0; b < 2; b++) {
+        const int key = min(key_w + 32 * b + c, sl.end - 1);
+        from[b] = (int)min((long)max(0, key - sl.pos0) * p.gqa, (long)t.r_hi);
+        upto[b] = p.window > 0 && key >= p.sink ? (int)min(max(0l, (long)key + p.window - sl.pos0) * p.gqa, (long)t.r_hi) : t.r_hi;
+        const BlockAt x = block_at(p, key);
+        const long page = max(page_of(p, table, x.b), 0);
+        const uint8_t* src = p.k_pool + (page * p.block_tokens + x.row) * key_bytes + h * HD + 16 * hh;
+        const float f = pow2f(p.k_exp[page * p.num_kv + h]);
+#pragma unroll
+        for (int j = 0; j < NB; j++) {
+          const u4_t w = *reinterpret_cast<const u4_t*>(src + 32 * j);
+          kf[b][j][0] = cvt8(w[0], w[1], f);
+          kf[b][j][1] = cvt8(w[2], w[3], f);
+        }
+      }
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // (from here on only steps are under way)
+      for (int v = v0; v < v1; v++) {
+        const int buf = (v - v0) % kRing, r0 = t.r_lo + 64 * v;
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((kRing - 2) * (LOADS + 1)) : "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        load(v + kRing - 1, (v - v0 + kRing - 1) % kRing);
+#pragma unroll
+        for (int half = 0; half < 2; half++) {
+          const int rh = r0 + 32 * half;
+          if (rh >= t.r_hi) continue;
+          const int pos_lo = sl.pos0 + token_of(p, rh), pos_hi = sl.pos0 + token_of(p, min(rh + 32, rows) - 1);
+          if (key_w > pos_hi) continue;
+          f16x_t acc[2] = {f16x_t{}, f16x_t{}};
+          const uint8_t* src = ring[buf] + (32 * half + c) * RB;
+#pragma unroll
+          for (int j = 0; j < NB; j++)
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+              const h8_t a = *reinterpret_cast<const h8_t*>(src + (((4 * j + 2 * hh + x) ^ (c & 15)) * 16));
+#pragma unroll
+              for (int b = 0; b < 2; b++) acc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, kf[b][j][x], acc[b], 0, 0, 0);
+            }
+          const bool whole = rh + 32 <= t.r_hi && key_w + 63 <= pos_lo &&
+                             (p.window <= 0 || key_w > pos_hi - p.window || key_w + 64 <= p.sink);
+          // lane c's key, rows 8 (x / 4) + 4 hh + x % 4
+#pragma unroll
+          for (int x4 = 0; x4 < 4; x4++) {
+            const int at = 32 * half + 8 * x4 + 4 * hh;
+            const f4_t mr = *reinterpret_cast<const f4_t*>(&stat_lds[buf][0][at]), il = *reinterpret_cast<const f4_t*>(&stat_lds[buf][1][at]);
+            float w[2][4];
+#pragma unroll
+            for (int b = 0; b < 2; b++)
+#pragma unroll
+              for (int x = 0; x < 4; x++) w[b][x] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[b][4 * x4 + x], p.scale_log2, -mr[x]));
+            if (whole) {
+#pragma unroll
+              for (int b = 0; b < 2; b++)
+#pragma unroll
+                for (int x = 0; x < 4; x++) sum[b] = __builtin_fmaf(w[b][x], il[x], sum[b]);
+            } else {
+#pragma unroll
+              for (int b = 0; b < 2; b++) {
+                const int lo = from[b] - r0 - at, hi = upto[b] - r0 - at;
+#pragma unroll
+                for (int x = 0; x < 4; x++) sum[b] += x >= lo && x < hi ? w[b][x] * il[x] : 0.f;
+              }
+            }
+          }
+        }
+      }
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // (no load into the ring is under way past here)
+    }
+    // (both halves of the lanes have the same keys, other rows)
+#pragma unroll
+    for (int b = 0; b < 2; b++) {
+      const float a = sum[b] + other32(sum[b], lane);
+      const int x = wave * 64 + 32 * b + c, key = i * kTile + x;
+      if (hh == 0 && key < sl.end) {
+        if (all) put_weight(p, table, h, key, p.weighed ? p.weighed[s] : sl.pos0, a);
+        else p.sums[(long)rec * kTile + x] = a;
+      }
+    }
+  });
+}
+
+__global__ __launch_bounds__(kThreads) void weigh_sums_join_kernel(WeighArgs p) {
+  CutTile c;
+  if (!cut_tile(p, c)) return;
   float a = 0.f;
-  for (int i = 0; i < spans; i++) a += in[(long)i * p.num_kv * p.max_ctx];
-  put_weight(p, p.tables + (long)s * p.max_blocks, h, key, p.weighed ? p.weighed[s] : sl.pos0, a);
+#pragma unroll 8
+  for (int j = 0; j < c.n; j++) a += p.sums[c.record(j) * kTile + threadIdx.x];
+  const Slot sl = slot_of(p, c.s);
+  const int key = c.i * kTile + (int)threadIdx.x;
+  if (key < sl.end) put_weight(p, p.tables + (long)c.s * p.max_blocks, c.h, key, p.weighed ? p.weighed[c.s] : sl.pos0, a);
 }
 
 WeighPlan weigh_plan(int num_q, int num_kv, int n_slots, long rows, int max_tok, int max_ctx) {
@@ -569,35 +823,35 @@ WeighPlan weigh_plan(int num_q, int num_kv, int n_slots, long rows, int max_tok,
   const double token = (double)num_q * x.pitch * 4;
   x.few_tok = (int)std::min((double)std::min(64 / gqa, max_tok), kWeighScores / token);
   x.many = max_tok > x.few_tok;
-  if (x.many && n_slots == 1) x.few_tok = 0;
+  // (beside many rows only where the numbers say that slots differ: three launches more, 13 us)
+  if (x.many && 2 * rows >= (long)n_slots * max_tok) x.few_tok = 0;
   if (x.few_tok > 0) x.few_slots = (int)std::min((double)n_slots, kWeighScores / (token * x.few_tok));
   // of these, workgroups enough for the CUs also where the slots are few, of 128 keys at least
   const long target = std::min(256l, std::max(16l, 8192l / std::max(1l, (long)x.few_slots * num_kv)));
   x.few_keys = (int)(128 * ((max_ctx + 128 * target - 1) / (128 * target)));
   x.few_chunks = (max_ctx + x.few_keys - 1) / x.few_keys;
-  x.many_chunks = (max_ctx + kWeighChunk - 1) / kWeighChunk;
   const size_t few_rows = (size_t)x.few_slots * x.few_tok * num_q, all = (size_t)rows * num_q;
-  const size_t many_sums = ((size_t)rows * gqa / kWeighSpan + n_slots) * num_kv * max_ctx;
-  x.stat_bytes = 8 * std::max(few_rows, x.many ? all : 0);
-  x.rec_bytes = 8 * std::max(few_rows * x.few_chunks, x.many ? all * x.many_chunks : 0);
-  x.sum_bytes = 4 * std::max(few_rows * x.pitch, x.many ? many_sums : 0);
+  x.stat_rows = std::max(few_rows, x.many ? all : 0);
+  x.rec_bytes = std::max(few_rows * x.few_chunks * 8, kWeighRec);
+  x.sum_bytes = std::max(few_rows * x.pitch * 4, kWeighRec / 2);
   return x;
 }
 
 hipError_t launch_weigh(WeighArgs a, const WeighPlan& x, int head_dim, hipStream_t stream) {
   const dim3 block(256);
+  int slots = 0;
   auto launch = [&](auto kernel, long per) {
     a.per = (int)per;
-    hipLaunchKernelGGL(kernel, grid_xy(per * (a.slot_end - a.slot0) * a.num_kv), block, 0, stream, a);
+    a.heads = slots * a.num_kv;
+    hipLaunchKernelGGL(kernel, grid_xy(per * a.heads), block, 0, stream, a);
   };
   if (x.few_tok > 0) for (a.slot0 = 0; a.slot0 < a.n_slots; a.slot0 += x.few_slots) {
-    a.slot_end = std::min(a.n_slots, a.slot0 + x.few_slots);
+    slots = std::min(a.n_slots - a.slot0, x.few_slots);
     a.local_tok = x.few_tok;
     a.from_tok = 1;
     a.to_tok = x.few_tok;
     a.chunk_keys = x.few_keys;
     a.chunks = x.few_chunks;
-    a.tile_rows = 0;
     const int rows = x.few_tok * a.gqa;
     if (head_dim == 128) {
       if (rows <= 16) launch(weigh_scores_kernel<128, 1>, a.chunks);
@@ -608,27 +862,25 @@ hipError_t launch_weigh(WeighArgs a, const WeighPlan& x, int head_dim, hipStream
       else if (rows <= 32) launch(weigh_scores_kernel<256, 2>, a.chunks);
       else launch(weigh_scores_kernel<256, 4>, a.chunks);
     }
-    launch(weigh_merge_kernel, (rows + 15) / 16);
-    launch(weigh_few_kernel, (a.max_ctx + 1023l) / 1024);
+    if (rows * a.chunks <= 2048) {
+      launch(weigh_few_kernel<false>, (a.max_ctx + 1023l) / 1024);
+    } else {
+      launch(weigh_merge_kernel, (rows + 15) / 16);
+      launch(weigh_few_kernel<true>, (a.max_ctx + 1023l) / 1024);
+    }
   }
   if (x.many) {
     a.slot0 = 0;
-    a.slot_end = a.n_slots;
     a.local_tok = 0;
     a.from_tok = x.few_tok + 1;
     a.to_tok = 0x7fffffff;
-    a.chunk_keys = kWeighChunk;
-    a.chunks = x.many_chunks;
-    a.tile_rows = kWeighRows;
-    const long rows = (long)a.max_tok * a.gqa;
-    a.spans = (int)((rows + kWeighSpan - 1) / kWeighSpan);
-    const long tiles = (rows + kWeighRows - 1) / kWeighRows, keys = (a.max_ctx + kWeighKeys - 1l) / kWeighKeys;
-    if (head_dim == 128) launch(weigh_stats_kernel<128>, tiles * a.chunks);
-    else launch(weigh_stats_kernel<256>, tiles * a.chunks);
-    launch(weigh_merge_kernel, (rows + 15) / 16);
-    if (head_dim == 128) launch(weigh_sums_kernel<128>, keys * a.spans);
-    else launch(weigh_sums_kernel<256>, keys * a.spans);
-    launch(weigh_many_kernel, (a.max_ctx + 255l) / 256);
+    const dim3 groups(kWeighGroups), wide(kThreads), joins(kWeighGroups - 1);
+    if (head_dim == 128) hipLaunchKernelGGL(weigh_stats_kernel<128>, groups, wide, 0, stream, a);
+    else hipLaunchKernelGGL(weigh_stats_kernel<256>, groups, wide, 0, stream, a);
+    hipLaunchKernelGGL(weigh_stats_join_kernel, joins, wide, 0, stream, a);
+    if (head_dim == 128) hipLaunchKernelGGL(weigh_sums_kernel<128>, groups, wide, 0, stream, a);
+    else hipLaunchKernelGGL(weigh_sums_kernel<256>, groups, wide, 0, stream, a);
+    hipLaunchKernelGGL(weigh_sums_join_kernel, joins, wide, 0, stream, a);
   }
   return hipGetLastError();
 }
