@@ -674,8 +674,8 @@ int qkv_weigh_f8_paged(const uint16_t* q, const uint8_t* k_pool, const uint8_t* 
  * No page that is written (those from the first row on that moves or that a raised exponent reaches) may
  * belong to two slots, nor twice to one.  After an eviction a row's number is not its position: new rows are turned at
  * their positions by qkv_rope or qkv_norm_rope and appended without a rotation, and windows count rows.
- * max_ctx, max_keep <= 2^30, n_slots * num_kv < 2^22 and n_slots * num_kv * (max_keep / 64 + 1) < 2^24
- * (QKV_ERR_UNSUPPORTED).  workspace: qkv_evict_f8_paged_workspace_bytes of these numbers or larger ones (no
+ * max_ctx, max_keep <= 2^30, n_slots * num_kv * (max_ctx / 4096 + 1) < 2^22 and n_slots * num_kv * (max_keep / 64 + 1)
+ * < 2^24 (QKV_ERR_UNSUPPORTED).  workspace: qkv_evict_f8_paged_workspace_bytes of these numbers or larger ones (no
  * initialisation needed).  Calls sharing one must be ordered. */
 size_t qkv_evict_f8_paged_workspace_bytes(int n_slots, int num_kv, int block_tokens, int max_ctx, int max_keep);
 int qkv_evict_f8_paged(uint8_t* k_pool, uint8_t* v_pool, uint8_t* k_exp, uint8_t* v_exp, float* weights, int n_slots,

@@ -254,16 +254,24 @@ int qkv_weigh_f8_paged(const uint16_t* q, const uint8_t* k_pool, const uint8_t* 
 
 static int check_evict(int n_slots, int num_kv, int block_tokens, int max_ctx, int max_keep) {
   if (n_slots < 0 || num_kv <= 0 || block_tokens <= 0 || max_ctx < 0 || max_keep < 0) return QKV_ERR_INVALID;
-  // chunks of all slots and heads are workgroups of 256 threads of one launch, slots and heads of 1,024
-  if (max_ctx > (1 << 30) || max_keep > (1 << 30) || (double)n_slots * num_kv >= (double)(1 << 22) ||
-      (double)n_slots * num_kv * (max_keep / 64 + 1.0) >= (double)(1 << 24))
+  // chunks of all slots and heads are workgroups of 256 threads of one launch, stretches of 1,024
+  const double chains = (double)n_slots * num_kv;
+  if (max_ctx > (1 << 30) || max_keep > (1 << 30) || chains * (max_ctx / (double)qkv::kEvictStretch + 1) >= (double)(1 << 22) ||
+      chains * (max_keep / 64 + 1.0) >= (double)(1 << 24))
     return QKV_ERR_UNSUPPORTED;
   return QKV_OK;
 }
 
+static int evict_stretches(int max_ctx) {
+  return max_ctx <= qkv::kEvictHeld ? 0 : (max_ctx + qkv::kEvictStretch - 1) / qkv::kEvictStretch;
+}
+
 size_t qkv_evict_f8_paged_workspace_bytes(int n_slots, int num_kv, int block_tokens, int max_ctx, int max_keep) {
   if (n_slots == 0 || check_evict(n_slots, num_kv, block_tokens, max_ctx, max_keep) != QKV_OK) return 0;
-  return 256 + 4 * ((size_t)n_slots * num_kv * (max_keep / 64 + 2));
+  // by slot and KV head: chunks taken and rows to move, flags, and for long slots the digits found, counts above and
+  // two of a digit
+  const size_t each = 4 * qkv::kEvictChain + 4 * (size_t)(max_keep / 64 + 1) + 16, stretch = 4 + 2 * 2 * qkv::kEvictBins;
+  return (size_t)n_slots * num_kv * (each + evict_stretches(max_ctx) * stretch);
 }
 
 int qkv_evict_f8_paged(uint8_t* k_pool, uint8_t* v_pool, uint8_t* k_exp, uint8_t* v_exp, float* weights, int n_slots,
@@ -293,9 +301,13 @@ int qkv_evict_f8_paged(uint8_t* k_pool, uint8_t* v_pool, uint8_t* k_exp, uint8_t
   a.lens = lens;
   a.keep = keep;
   a.kept = kept;
-  a.ticket = static_cast<int*>(workspace);
-  a.moves = a.ticket + 64;
-  a.flags = a.moves + (size_t)n_slots * num_kv;
+  a.chains = static_cast<int*>(workspace);
+  const size_t chains = (size_t)n_slots * num_kv;
+  a.stretches = evict_stretches(max_ctx);
+  a.counts = reinterpret_cast<uint16_t*>(a.chains + qkv::kEvictChain * chains);
+  a.found = reinterpret_cast<uint32_t*>(a.counts + 2 * chains * a.stretches * qkv::kEvictBins);
+  a.above = reinterpret_cast<int*>(a.found + 4 * chains);
+  a.flags = a.above + chains * a.stretches;
   a.n_slots = n_slots;
   a.num_kv = num_kv;
   a.max_ctx = max_ctx;

@@ -285,6 +285,9 @@ hipError_t launch_weigh(WeighArgs a, const WeighPlan& plan, int head_dim, hipStr
 
 // Eviction from the paged 8-bit cache (evict_f8.hip).
 constexpr int kEvictBytes = 16384;   // codes of a chunk of rows, of each pool
+constexpr int kEvictChain = 32;      // ints apart, on lines of their own
+constexpr int kEvictHeld = 16384;    // rows of a slot that one workgroup chooses from
+constexpr int kEvictStretch = 4096, kEvictBins = 2048;   // rows, digits of a workgroup of those for longer slots
 struct EvictArgs {
   uint8_t* k_pool;
   uint8_t* v_pool;
@@ -295,9 +298,12 @@ struct EvictArgs {
   const int32_t* lens;       // [n_slots] rows of a slot
   const int32_t* keep;       // [n_slots] rows that stay
   int32_t* kept;             // [n_slots][num_kv][max_keep]
-  int* ticket;               // workspace: chunks taken; set to 0 by the first launch
-  int* moves;                // workspace: [n_slots * num_kv] rows to write (0: none)
+  int* chains;               // workspace: [n_slots * num_kv][kEvictChain] chunks taken, rows to write (0: none)
   int* flags;                // workspace: [n_slots * num_kv][chunks] 1: read, 2: all before too
+  uint32_t* found;           // workspace: [n_slots * num_kv][4] digits and what is needed, after the first and second
+  int* above;                // workspace: [n_slots * num_kv][stretches] rows above the first two digits
+  uint16_t* counts;          // workspace: [2][n_slots * num_kv][stretches][kEvictBins] of the digits, in turn
+  int stretches;             // of max_ctx rows; 0: one workgroup a slot and KV head
   int n_slots, num_kv, max_ctx, max_keep, max_blocks, block_tokens, n_pages, sink, recent;
   int chunks;                // of max_keep rows
   uint32_t bt_magic;         // floor(2^32 / block_tokens)

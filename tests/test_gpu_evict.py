@@ -83,6 +83,21 @@ def test_long_slots(hd):
     _check(*c, lens, [15000, 19990, 3], 40000, 20000, 4, 100)
 
 
+def test_long_slots_ties_and_kinds():
+    """More equal weights than a stretch of rows holds, NaN and infinities among them; every number kept."""
+    rng = np.random.default_rng(11)
+    lens = [30000, 17000, 4096 + 30, 4097, 100, 0]
+    for sink, recent in ((0, 0), (30, 1)):
+        c = _cache(rng, lens, 256, 1, 128, ties=True)
+        kinds = np.array([0.0, -0.0, np.inf, -np.inf, np.nan, 1e-45, 3.4e38, -1.0], np.float32)
+        c[3][:c[3].shape[0] // 2] = kinds[rng.integers(0, len(kinds), c[3][:c[3].shape[0] // 2].shape)]
+        _check(*c, lens, [29000, 1, 4096, 2000, 99, 5], 30000, 29000, sink, recent)
+    c = _cache(rng, lens, 256, 1, 128)
+    c[3][:] = 1
+    _, kept = _check(*c, lens, [12345, 16999, 10, 4096, 0, 0], 30000, 17000)
+    assert (kept[0, 0, :12345] == np.arange(12345)).all()
+
+
 def test_almost_all_stays_and_next_to_nothing():
     rng = np.random.default_rng(5)
     lens = [5000, 5000, 5000]
