@@ -167,8 +167,8 @@ static int check_weigh(int num_q, int num_kv, int head_dim, int n_slots, int n_r
   // workgroups of a launch, rows of a slot and KV head, and steps of the line of all tiles (by rows, then by keys),
   // counted in 31 bits, a head's steps in 30
   const double gqa = num_q / num_kv, tok = std::min(max_tok, n_rows), rows = tok * gqa, heads = (double)n_slots * num_kv;
-  const double row_tiles = std::min(n_slots * (rows / 512 + 1), n_rows * gqa / 512 + n_slots);
-  const double by_rows = row_tiles * (max_ctx / 64.0 + 6), by_keys = (max_ctx / 512.0 + 1) * (n_rows * gqa / 64 + 6.0 * n_slots);
+  const double row_tiles = std::min(n_slots * (rows / 256 + 1), n_rows * gqa / 256 + n_slots);
+  const double by_rows = row_tiles * (max_ctx / 64.0 + 6), by_keys = (max_ctx / 256.0 + 1) * (n_rows * gqa / 32 + 6.0 * n_slots);
   if (heads * std::max(rows / 16 + 1, max_ctx / 128.0 + 1) > 2147480000.0 || rows > (double)(1 << 30) ||
       std::max(by_rows, by_keys) * std::max(num_kv, 2) > 2147480000.0)
     return QKV_ERR_UNSUPPORTED;

@@ -242,8 +242,8 @@ int f8_attn_apart(int num_q, int num_kv, int head_dim, int n_slots, long rows, i
 hipError_t launch_f8_attn(const F8AttnArgs& a, const F8AttnPlan& plan, int head_dim, hipStream_t stream);
 
 // Attention weights of the keys of the paged 8-bit cache, accumulated (weigh_f8.hip).
-constexpr int kWeighGroups = 256;                          // workgroups of the kernels for many rows, one on each CU
-constexpr size_t kWeighRec = 2 * kWeighGroups * 512 * 8;   // bytes of their records of rows, twice those of keys
+constexpr int kWeighGroups = 768;                          // workgroups of the kernels for many rows, at most
+constexpr size_t kWeighRec = 2 * kWeighGroups * 256 * 8;   // bytes of their records of rows, twice those of keys
 constexpr long kWeighScores = 256l << 20;           // bytes of scores that a call may store
 struct WeighArgs {
   const uint16_t* q;         // [rows][num_q][head_dim]
@@ -259,6 +259,7 @@ struct WeighArgs {
   float* stat_il;
   float* scores;             // workspace: [rows of the launch][score_pitch] (few rows)
   float* sums;               // workspace, the same place: of cut tiles (many rows)
+  int groups;                // workgroups of the kernels for many rows
   int* cuts;                 // workspace: [kWeighGroups][4] where each part begins
   long rows, score_pitch;
   float scale_log2, decay;

@@ -341,16 +341,23 @@ __global__ __launch_bounds__(256) void weigh_few_kernel(WeighArgs p) {
 // ---------------------------------------------------------------------------
 // many rows
 // ---------------------------------------------------------------------------
-// Both kernels: eight waves of 64 stationary rows (or keys) in registers, the others 64 at a step through a ring of
-// kRing LDS tiles that are loaded past the registers, kRing - 1 steps ahead.  A tile's rows are stored as they are,
+// Both kernels: four waves of 64 stationary rows (or keys) in registers, the others 64 (or 32) at a step through a ring
+// of kRing LDS tiles that are loaded past the registers, kRing - 1 steps ahead.  A tile's rows are stored as they are,
 // but for their 16-byte words, which are permuted by the row's number so that 16 rows' same word lies on distinct
 // banks.  Operand dims: lane l's 16-byte word of codes holds the dims of two products.
 //
+// What bounds them is that exponentials, sums and conversions fill the vector unit as long as products do the
+// matrix cores (a score of 64 lanes: fma 4 cycles, exponential 8, sum 4, conversion 2 to 4; its products 16 of
+// 128 dims), and that a wave does them in turn.  So there are as many workgroups on a CU as registers allow, 3 of
+// 128 dims and 2 of 256, none of which waits for another's barrier (one of eight waves instead: 66 and 78 us for 164
+// million scores of 128 dims, now 56 and 70; 90 and 107 for 138 million of 256 dims, now 88 and 97).  Adding up the
+// scores before beside the next ones' products, written into one stream of instructions, needs registers
+// for both: 60 us, and 87.
+//
 // Work: the steps of all stationary tiles, KV heads and slots form one line that is cut into equal parts, a
-// workgroup's each, so ragged and causal lengths balance by themselves (workgroups of 64 to 512 rows by 512 to
-// 1,024 keys as launched: 1.6 to 2 times as long).  A tile that lies in one part is finished there; one that is cut
-// leaves records that a second kernel joins.
-constexpr int kRing = 4, kWaves = 8, kTile = 64 * kWaves, kThreads = 64 * kWaves;
+// workgroup's each, so ragged and causal lengths balance by themselves.  A tile that lies in one part is finished there;
+// one that is cut leaves records that a second kernel joins.
+constexpr int kRing = 4, kWaves = 4, kTile = 64 * kWaves, kThreads = 64 * kWaves;
 constexpr int kWeighLead = 3;   // steps that a tile costs beside its own
 
 // The tiles of a slot's rows and their steps over keys: v below n_sink are key steps v, then w0 on.
@@ -374,6 +381,7 @@ struct RowTiles {
 };
 
 // The tiles of a slot's keys and their steps over the rows r_lo .. r_hi-1 that see a key of the tile.
+template <int STEP>
 struct KeyTiles {
   const WeighArgs& p;
   struct Tile {
@@ -386,8 +394,8 @@ struct KeyTiles {
     if (p.window > 0 && k0 >= p.sink) hi = min(hi, max(0l, (long)k1 + p.window - x.pos0) * p.gqa);
     Tile t;
     t.r_hi = (int)hi;
-    t.r_lo = (int)min((long)max(0, k0 - x.pos0) * p.gqa / 64 * 64, hi);
-    t.steps = (t.r_hi - t.r_lo + 63) / 64;
+    t.r_lo = (int)min((long)max(0, k0 - x.pos0) * p.gqa / STEP * STEP, hi);
+    t.steps = (t.r_hi - t.r_lo + STEP - 1) / STEP;
     return t;
   }
 };
@@ -474,9 +482,9 @@ __device__ __forceinline__ void run_part(const WeighArgs& p, const Tiles& tiles,
   TileLine<Tiles> line{p, tiles, lds};
   const int tid = threadIdx.x, lane = tid & 63;
   const int total = __builtin_amdgcn_readfirstlane(line.units());
-  const Parts parts(__builtin_amdgcn_readfirstlane(total * p.num_kv), kWeighGroups);
+  const Parts parts(__builtin_amdgcn_readfirstlane(total * p.num_kv), p.groups);
   // neighbouring parts (the same head's keys and rows) on one XCD, whose L2 holds them
-  const int grp = (int)(blockIdx.x % 8) * (kWeighGroups / 8) + (int)blockIdx.x / 8;
+  const int grp = (int)(blockIdx.x % 8) * (p.groups / 8) + (int)blockIdx.x / 8;
   int4* cuts = reinterpret_cast<int4*>(p.cuts);
   if (grp >= parts.n) {
     if (tid == 0) cuts[grp] = make_int4(-1, 0, 0, 0);
@@ -526,69 +534,157 @@ struct CutTile {
 };
 __device__ __forceinline__ bool cut_tile(const WeighArgs& p, CutTile& c) {
   __shared__ int4 cuts[kWeighGroups];
-  for (int x = threadIdx.x; x < kWeighGroups; x += kThreads) cuts[x] = reinterpret_cast<const int4*>(p.cuts)[x];
+  for (int x = threadIdx.x; x < p.groups; x += kThreads) cuts[x] = reinterpret_cast<const int4*>(p.cuts)[x];
   __syncthreads();
   const int g = (int)blockIdx.x + 1;
   const int4 here = cuts[g], before = cuts[g - 1];
   auto same = [&](const int4& a) { return a.x == here.x && a.y == here.y && a.z == here.z; };
   if (here.x < 0 || here.w <= 0 || (same(before) && before.w > 0)) return false;
   c = {here.x, here.y, here.z, 2 * (g - 1) + (same(before) ? 0 : 1), 2, g};
-  while (g + c.n - 1 < kWeighGroups && same(cuts[g + c.n - 1])) c.n++;
+  // (the parts that continue it are neighbours: to the first of another tile, 64 at a time)
+  const int lane = (int)threadIdx.x & 63;
+  for (int x = g + 1;; x += 64) {
+    const uint64_t other = __builtin_amdgcn_ballot_w64(x + lane >= p.groups || !same(cuts[min(x + lane, p.groups - 1)]));
+    c.n = x - g + 1 + (other ? (int)__builtin_ctzll(other) : 64);
+    if (other) break;
+  }
   return true;
 }
 
-// Statistics of rows.  Codes are converted by each wave as it reads them (16 conversions beside 4 products of 32
-// cycles).  The pages of kLook steps and their exponents are looked up at a time.
+// Reads of LDS beside loads into LDS.  (For a read that it knows of the compiler waits until every load into LDS has
+// ended, those of later steps too.)
+__device__ __forceinline__ uint32_t lds_at(const void* p) {
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)p;
+}
+__device__ __forceinline__ void lds_read(u4_t (&x)[4], uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("ds_read_b128 %0, %4\n\tds_read_b128 %1, %5\n\tds_read_b128 %2, %6\n\tds_read_b128 %3, %7\n\ts_waitcnt lgkmcnt(0)"
+               : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]) : "v"(a), "v"(b), "v"(c), "v"(d) : "memory");
+}
+// (four rows' numbers of each eight from a on, and those 256 bytes past them)
+__device__ __forceinline__ void lds_read(f4_t (&x)[4], f4_t (&y)[4], uint32_t a) {
+  asm volatile("ds_read_b128 %0, %8\n\tds_read_b128 %1, %8 offset:32\n\tds_read_b128 %2, %8 offset:64\n\t"
+               "ds_read_b128 %3, %8 offset:96\n\tds_read_b128 %4, %8 offset:256\n\tds_read_b128 %5, %8 offset:288\n\t"
+               "ds_read_b128 %6, %8 offset:320\n\tds_read_b128 %7, %8 offset:352\n\ts_waitcnt lgkmcnt(0)"
+               : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]), "=&v"(y[0]), "=&v"(y[1]), "=&v"(y[2]), "=&v"(y[3])
+               : "v"(a) : "memory");
+}
+
+// Scores to be added: of 32 keys from k on, the pages of each 16, whether every row sees all.
+struct Half {
+  int k, pg0, pg1;
+  bool whole;
+};
+
+// Statistics of rows.  Codes are converted by each wave as it reads them.  The pages of kLook steps and their exponents
+// are looked up at a time.  The reference of a row's sum need not be its maximum: it stands until the sum grows past
+// 2^32 (what is lost then lies below 2^-94 of it), which saves the maximum of each score (66 -> 61 us).
 template <int HD>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void weigh_stats_kernel(WeighArgs p) {
-  constexpr int NB = HD / 32, TB = 64 * HD, LOADS = TB / 1024 / kWaves, RL = 1024 / HD, kLook = 256;
-  __shared__ __align__(16) uint8_t ring[kRing][TB];
-  __shared__ int page_lds[kLook * 4];        // of every 16 keys, -1: none
-  __shared__ float exp_lds[kLook * 4];
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(HD == 128 ? 3 : 2, HD == 128 ? 3 : 2))) void weigh_stats_kernel(WeighArgs p) {
+  constexpr int NB = HD / 32, TB = 64 * HD, LOADS = TB / 1024 / kWaves, RL = 1024 / HD, kLook = 128;
+  __shared__ __align__(256) uint8_t ring[kRing][TB];
+  // of every 16 keys: their first row's offset in the pool (absent: 0), their page (-1: none) and its exponent's power
+  __shared__ __align__(16) long at_lds[kLook * 4];
+  __shared__ __align__(16) int page_lds[kLook * 4];
+  __shared__ __align__(16) float exp_lds[kLook * 4];
   __shared__ LineLds lds;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 31, hh = lane >> 5;
   const uint32_t key_bytes = (uint32_t)p.num_kv * HD;
+  // A wave loads 16 keys of a step, RL at a time: this lane's word of the first, and key
+  static_assert(LOADS * RL == 16);
+  const uint32_t my_word = 16 * ((lane % (HD / 16)) ^ (lane / (HD / 16))), my_key = lane / (HD / 16) * key_bytes;
+  const uint32_t page_at = lds_at(page_lds), exp_at = lds_at(exp_lds) + 4 * (c >> 4), at_at = lds_at(at_lds);
+  const uint32_t ring_at = lds_at(ring) + c * HD + ((hh ^ (c & (HD / 16 - 1))) * 16);   // key c's word of the first products
   run_part(p, RowTiles{p}, lds, [&](const Slot& sl, int s, int h, int i, const RowTiles::Tile& t, int v0, int v1, bool all, int rec)
                                     __attribute__((always_inline)) {
     const int rows = sl.n * p.gqa, row_w = i * kTile + wave * 64;
     h8_t qf[2][NB][2];
     const bool live = row_w < rows;
     const int pos_lo = sl.pos0 + token_of(p, min(row_w, rows - 1)), pos_hi = sl.pos0 + token_of(p, min(row_w + 64, rows) - 1);
-    // keys that lane c's rows see: above `from` (or below the sinks), up to `upto`
-    int from[2], upto[2];
-#pragma unroll
-    for (int b = 0; b < 2; b++) {
-      const int pos = sl.pos0 + token_of(p, min(row_w + 32 * b + c, rows - 1));
-      from[b] = p.window > 0 ? pos - p.window : -1;
-      upto[b] = min(pos, t.end - 1);
-    }
     Stat st[2] = {{-INFINITY, 0.f}, {-INFINITY, 0.f}};
+    // Sums by the reference that stands ..
+    auto sums_of = [&](const f16x_t (&x)[2], float (&l)[2]) __attribute__((always_inline)) {
+#pragma unroll
+      for (int b = 0; b < 2; b++) {
+        l[b] = st[b].l;
+#pragma unroll
+        for (int i = 0; i < 16; i++) l[b] += __builtin_amdgcn_exp2f(__builtin_fmaf(x[b][i], p.scale_log2, -st[b].m));
+      }
+    };
+    // .. by the maximum (lane c's row, keys 8 (i / 4) + 4 hh + i % 4) ..
+    auto exact = [&](const f16x_t& x, Stat& st, auto&& seen) __attribute__((always_inline)) {
+      float top = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 16; i++) top = fmaxf(top, seen(i) ? x[i] * p.scale_log2 : -INFINITY);
+      const float mn = fmaxf(st.m, top), ref = mn == -INFINITY ? 0.f : mn;
+      float l = st.l * __builtin_amdgcn_exp2f(st.m - ref);
+#pragma unroll
+      for (int i = 0; i < 16; i++) {
+        const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], p.scale_log2, -ref));
+        l += seen(i) ? w : 0.f;
+      }
+      st = {mn, l};
+    };
+    // .. where that makes large numbers (or there is none yet).
+    auto take = [&](const f16x_t (&x)[2], const float (&l)[2]) __attribute__((always_inline)) {
+      if (__builtin_amdgcn_ballot_w64(!(l[0] < 0x1p32f && l[1] < 0x1p32f))) {
+#pragma unroll
+        for (int b = 0; b < 2; b++) exact(x[b], st[b], [](int) { return true; });
+      } else {
+        st[0].l = l[0];
+        st[1].l = l[1];
+      }
+    };
+    auto add = [&](const f16x_t (&x)[2], const Half& had) __attribute__((always_inline)) {
+      if (had.whole) {
+        float l[2];
+        sums_of(x, l);
+        take(x, l);
+      } else {
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+          // the row sees the keys above `from` (or below the sinks) and up to `upto`, and none of an absent page: a bound
+          // past every key of it
+          const int pos = sl.pos0 + token_of(p, min(row_w + 32 * b + c, rows - 1));
+          const int from = p.window > 0 ? pos - p.window : -1, upto = min(pos, t.end - 1);
+          const int k = had.k + 4 * hh, hi = upto - k, lo = from - k, sink = p.sink - k;
+          const int hi0 = had.pg0 >= 0 ? hi : -64, hi1 = had.pg1 >= 0 ? hi : -64;
+          exact(x[b], st[b], [&](int i) {
+            const int d = 8 * (i >> 2) + (i & 3);
+            return (d <= (i < 8 ? hi0 : hi1)) & ((d > lo) | (d < sink));
+          });
+        }
+      }
+    };
     for (int va = v0; va < v1; va += kLook) {
       const int vb = min(va + kLook, v1);
       __syncthreads();   // (the ring and the pages are written again)
       for (int x = tid; x < 4 * (vb - va); x += kThreads) {
         const int key = t.first(va + (x >> 2)) + 16 * (x & 3);
-        const int pg = key < t.end ? page_of(p, p.tables + (long)s * p.max_blocks, block_at(p, key).b) : -1;
+        const BlockAt y = block_at(p, key);
+        const int pg = key < t.end ? page_of(p, p.tables + (long)s * p.max_blocks, y.b) : -1;
+        at_lds[x] = pg < 0 ? 0 : ((long)pg * p.block_tokens + y.row) * key_bytes;
         page_lds[x] = pg;
         exp_lds[x] = pow2f(p.k_exp[(long)max(pg, 0) * p.num_kv + h]);
       }
       __syncthreads();
       // the wave's part of a step: LOADS times RL keys (past the last step it is loaded again, so that as many loads
       // are under way as are counted)
-      auto load = [&](int v, int buf) {
-        v = min(v, vb - 1);
-        const int k0 = t.first(v);
+      auto load = [&](int buf, long at) __attribute__((always_inline)) {
+        uint32_t word = my_word, key = my_key;
+        asm volatile("" : "+v"(word), "+v"(key));   // (no LOADS offsets held in registers)
 #pragma unroll
         for (int j = 0; j < LOADS; j++) {
-          const int x = (wave * LOADS + j) * RL + lane / (HD / 16), word = (lane % (HD / 16)) ^ (x & (HD / 16 - 1));
-          const long page = max(page_lds[4 * (v - va) + (x >> 4)], 0);
-          const uint8_t* src = p.k_pool + (page * p.block_tokens + block_at(p, k0 + x).row) * key_bytes + h * HD + 16 * word;
+          const uint8_t* src = p.k_pool + h * HD + at + (word ^ (j * RL * 16 & (HD - 1))) + (key + j * RL * key_bytes);
           __builtin_amdgcn_global_load_lds((glb_void*)src, (lds_void*)(ring[buf] + (wave * LOADS + j) * 1024), 16, 0, 0);
         }
       };
+      auto entry = [&](int v) { return 4 * (min(v, vb - 1) - va) + wave; };
+      long at[kRing - 1];
 #pragma unroll
-      for (int j = 0; j < kRing - 1; j++) load(va + j, j);
+      for (int j = 0; j < kRing - 1; j++) at[j] = at_lds[entry(va + j)];
+#pragma unroll
+      for (int j = 0; j < kRing - 1; j++) load(j, at[j]);
       if (va == v0) {
 #pragma unroll
         for (int b = 0; b < 2; b++) {
@@ -606,59 +702,42 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
         asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((kRing - 2) * LOADS) : "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        load(v + kRing - 1, (v - va + kRing - 1) % kRing);
+        u4_t pages;
+        f2_t pow;
+        u2_t from;
+        asm volatile("ds_read_b128 %0, %3\n\tds_read2_b32 %1, %4 offset1:2\n\tds_read_b64 %2, %5\n\ts_waitcnt lgkmcnt(0)"
+                     : "=&v"(pages), "=&v"(pow), "=&v"(from)
+                     : "v"(page_at + 16 * (v - va)), "v"(exp_at + 16 * (v - va)), "v"(at_at + 8 * entry(v + kRing - 1))
+                     : "memory");
+        const long next = (long)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)from[1]) << 32 |
+                                 (uint32_t)__builtin_amdgcn_readfirstlane((int)from[0]));
+        load((v - va + kRing - 1) % kRing, next);
         const int k0 = t.first(v);
 #pragma unroll
         for (int half = 0; half < 2; half++) {
           const int kh = k0 + 32 * half;
           if (!live || kh > pos_hi || kh >= t.end) continue;
-          const int pi = 4 * (v - va) + 2 * half, pg0 = page_lds[pi], pg1 = page_lds[pi + 1];
-          const float f = exp_lds[pi + (c >> 4)];
           f16x_t acc[2] = {f16x_t{}, f16x_t{}};
-          // (ahead of the other wave's exponentials: 101 -> 90 us for 8.6 million pairs of 16 heads of 256)
-          __builtin_amdgcn_s_setprio(1);
-          const uint8_t* src = ring[buf] + (32 * half + c) * HD;
+          const uint32_t src = ring_at + buf * TB + 32 * half * HD;
 #pragma unroll
-          for (int j = 0; j < NB; j++) {
-            const u4_t w = *reinterpret_cast<const u4_t*>(src + (((2 * j + hh) ^ ((32 * half + c) & (HD / 16 - 1))) * 16));
+          for (int j4 = 0; j4 < NB; j4 += 4) {
+            u4_t w[4];
+            lds_read(w, src ^ (32 * j4), src ^ (32 * j4 + 32), src ^ (32 * j4 + 64), src ^ (32 * j4 + 96));
+            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-            for (int x = 0; x < 2; x++) {
-              const h8_t a = cvt8(w[2 * x], w[2 * x + 1], f);
+            for (int j = 0; j < 4; j++)
 #pragma unroll
-              for (int b = 0; b < 2; b++) acc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qf[b][j][x], acc[b], 0, 0, 0);
-            }
+              for (int x = 0; x < 2; x++) {
+                const h8_t a = cvt8(w[j][2 * x], w[j][2 * x + 1], pow[half]);
+#pragma unroll
+                for (int b = 0; b < 2; b++) acc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qf[b][j4 + j][x], acc[b], 0, 0, 0);
+              }
+            __builtin_amdgcn_s_setprio(0);
           }
-          __builtin_amdgcn_s_setprio(0);
+          const int pg0 = __builtin_amdgcn_readfirstlane((int)pages[2 * half]), pg1 = __builtin_amdgcn_readfirstlane((int)pages[2 * half + 1]);
           const bool whole = pg0 >= 0 && pg1 >= 0 && kh + 31 <= pos_lo && kh + 32 <= t.end &&
                              (p.window <= 0 || kh > pos_hi - p.window || kh + 32 <= p.sink);
-#pragma unroll
-          for (int b = 0; b < 2; b++) {
-            // lane c's row, keys 8 (x / 4) + 4 hh + x % 4
-            auto add = [&](auto&& seen) __attribute__((always_inline)) {
-              float top = -INFINITY;
-#pragma unroll
-              for (int x = 0; x < 16; x++) top = fmaxf(top, seen(x) ? acc[b][x] * p.scale_log2 : -INFINITY);
-              const float mn = fmaxf(st[b].m, top), ref = mn == -INFINITY ? 0.f : mn;
-              float l = st[b].l * __builtin_amdgcn_exp2f(st[b].m - ref);
-#pragma unroll
-              for (int x = 0; x < 16; x++) {
-                const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[b][x], p.scale_log2, -ref));
-                l += seen(x) ? w : 0.f;
-              }
-              st[b] = {mn, l};
-            };
-            if (whole) {
-              add([](int) { return true; });
-            } else {
-              // (no key of an absent page: a bound past every key of it)
-              const int k = kh + 4 * hh, hi = upto[b] - k, lo = from[b] - k, sink = p.sink - k;
-              const int hi0 = pg0 >= 0 ? hi : -64, hi1 = pg1 >= 0 ? hi : -64;
-              add([&](int x) {
-                const int d = 8 * (x >> 2) + (x & 3);
-                return (d <= (x < 8 ? hi0 : hi1)) & ((d > lo) | (d < sink));
-              });
-            }
-          }
+          add(acc, Half{kh, pg0, pg1, whole});
         }
       }
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // (no load into the ring is under way past here)
@@ -691,15 +770,33 @@ __global__ __launch_bounds__(kThreads) void weigh_stats_join_kernel(WeighArgs p)
 
 // Sums of keys.  A step brings its rows' statistics along.
 template <int HD>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void weigh_sums_kernel(WeighArgs p) {
-  constexpr int NB = HD / 32, RB = HD * 2, TB = 64 * RB, LOADS = TB / 1024 / kWaves, WORDS = RB / 16;
-  __shared__ __align__(16) uint8_t ring[kRing][TB];
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(HD == 128 ? 3 : 2, HD == 128 ? 3 : 2))) void weigh_sums_kernel(WeighArgs p) {
+  constexpr int STEP = 32, NB = HD / 32, RB = HD * 2, TB = STEP * RB, LOADS = TB / 1024 / kWaves, WORDS = RB / 16;
+  __shared__ __align__(512) uint8_t ring[kRing][TB];
   __shared__ __align__(16) float stat_lds[kRing][3][64];   // m, 1 / l, and what the other waves load beside them
   __shared__ LineLds lds;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 31, hh = lane >> 5;
   const uint32_t key_bytes = (uint32_t)p.num_kv * HD;
-  run_part(p, KeyTiles{p}, lds, [&](const Slot& sl, int s, int h, int i, const KeyTiles::Tile& t, int v0, int v1, bool all, int rec)
+  // row c's word of the first product
+  const uint32_t ring_at = lds_at(ring) + c * RB + (((2 * hh) ^ (c & 15)) * 16), stat_at = lds_at(stat_lds) + 16 * hh;
+  // Bytes of this lane's words (and of a row's number) past the first token's rows of a step that begins with its row
+  // `rem` and has `left` rows
+  auto places = [&](int rem, int left, uint32_t (&at)[LOADS + 1]) {
+    auto place = [&](int x) {
+      const int y = rem + min(x, left - 1);
+      return (uint32_t)(token_of(p, y) * (p.num_q - p.gqa) + y);
+    };
+#pragma unroll
+    for (int j = 0; j < LOADS; j++) {
+      const int x = (wave * LOADS + j) * (1024 / RB) + lane / WORDS;
+      at[j] = place(x) * RB + 16 * ((lane % WORDS) ^ (x & 15));
+    }
+    at[LOADS] = 4 * place(lane);
+  };
+  uint32_t mine[LOADS + 1];   // (the same in most steps, all where groups divide them)
+  places(0, 64, mine);
+  run_part(p, KeyTiles<STEP>{p}, lds, [&](const Slot& sl, int s, int h, int i, const typename KeyTiles<STEP>::Tile& t, int v0, int v1, bool all, int rec)
                                     __attribute__((always_inline)) {
     const int rows = sl.n * p.gqa, key_w = i * kTile + wave * 64;
     const int32_t* table = p.tables + (long)s * p.max_blocks;
@@ -707,15 +804,21 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
     if (v0 < v1) {
       // the wave's part of a step, and a number for each of its rows: every wave as many loads
       auto load = [&](int v, int buf) {
-        const int r0 = t.r_lo + 64 * min(v, v1 - 1);
+        const int r0 = t.r_lo + STEP * min(v, v1 - 1), tok = token_of(p, r0), rem = r0 - tok * p.gqa;
+        const long row = (long)(sl.t0 + tok) * p.num_q + h * p.gqa;
+        uint32_t at[LOADS + 1];
+        if (rem != 0 || rows - r0 < 64) {
+          places(rem, rows - r0, at);
+        } else {
 #pragma unroll
-        for (int j = 0; j < LOADS; j++) {
-          const int x = (wave * LOADS + j) * (1024 / RB) + lane / WORDS, word = (lane % WORDS) ^ (x & 15);
-          const uint16_t* src = p.q + row_at(p, sl, h, min(r0 + x, rows - 1)) * HD + 8 * word;
-          __builtin_amdgcn_global_load_lds((glb_void*)src, (lds_void*)(ring[buf] + (wave * LOADS + j) * 1024), 16, 0, 0);
+          for (int j = 0; j <= LOADS; j++) at[j] = mine[j];
         }
-        const float* src = (wave == 1 ? p.stat_il : p.stat_m) + row_at(p, sl, h, min(r0 + lane, rows - 1));
-        __builtin_amdgcn_global_load_lds((glb_void*)src, (lds_void*)stat_lds[buf][min(wave, 2)], 4, 0, 0);
+#pragma unroll
+        for (int j = 0; j < LOADS; j++)
+          __builtin_amdgcn_global_load_lds((glb_void*)((const uint8_t*)(p.q + row * HD) + at[j]),
+                                           (lds_void*)(ring[buf] + (wave * LOADS + j) * 1024), 16, 0, 0);
+        const float* src = (wave == 1 ? p.stat_il : p.stat_m) + row;
+        __builtin_amdgcn_global_load_lds((glb_void*)((const uint8_t*)src + at[LOADS]), (lds_void*)stat_lds[buf][min(wave, 2)], 4, 0, 0);
       };
       __syncthreads();   // (the ring is written again)
 #pragma unroll
@@ -740,50 +843,55 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
       }
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // (from here on only steps are under way)
       for (int v = v0; v < v1; v++) {
-        const int buf = (v - v0) % kRing, r0 = t.r_lo + 64 * v;
+        const int buf = (v - v0) % kRing, r0 = t.r_lo + STEP * v;
         asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((kRing - 2) * (LOADS + 1)) : "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
         load(v + kRing - 1, (v - v0 + kRing - 1) % kRing);
 #pragma unroll
-        for (int half = 0; half < 2; half++) {
+        for (int half = 0; half < STEP / 32; half++) {
           const int rh = r0 + 32 * half;
           if (rh >= t.r_hi) continue;
           const int pos_lo = sl.pos0 + token_of(p, rh), pos_hi = sl.pos0 + token_of(p, min(rh + 32, rows) - 1);
           if (key_w > pos_hi) continue;
           f16x_t acc[2] = {f16x_t{}, f16x_t{}};
-          const uint8_t* src = ring[buf] + (32 * half + c) * RB;
+          const uint32_t src = ring_at + buf * TB + 32 * half * RB;
 #pragma unroll
-          for (int j = 0; j < NB; j++)
+          for (int j = 0; j < NB; j += 2) {
+            u4_t a[4];
+            lds_read(a, src ^ (64 * j), src ^ (64 * j + 16), src ^ (64 * j + 64), src ^ (64 * j + 80));
+            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-            for (int x = 0; x < 2; x++) {
-              const h8_t a = *reinterpret_cast<const h8_t*>(src + (((4 * j + 2 * hh + x) ^ (c & 15)) * 16));
+            for (int x = 0; x < 4; x++)
 #pragma unroll
-              for (int b = 0; b < 2; b++) acc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, kf[b][j][x], acc[b], 0, 0, 0);
-            }
+              for (int b = 0; b < 2; b++)
+                acc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8_t, a[x]), kf[b][j + x / 2][x % 2], acc[b], 0, 0, 0);
+            __builtin_amdgcn_s_setprio(0);
+          }
+          f4_t mr[4], il[4];
+          lds_read(mr, il, stat_at + buf * (4 * 3 * 64) + 128 * half);
           const bool whole = rh + 32 <= t.r_hi && key_w + 63 <= pos_lo &&
                              (p.window <= 0 || key_w > pos_hi - p.window || key_w + 64 <= p.sink);
           // lane c's key, rows 8 (x / 4) + 4 hh + x % 4
 #pragma unroll
           for (int x4 = 0; x4 < 4; x4++) {
             const int at = 32 * half + 8 * x4 + 4 * hh;
-            const f4_t mr = *reinterpret_cast<const f4_t*>(&stat_lds[buf][0][at]), il = *reinterpret_cast<const f4_t*>(&stat_lds[buf][1][at]);
             float w[2][4];
 #pragma unroll
             for (int b = 0; b < 2; b++)
 #pragma unroll
-              for (int x = 0; x < 4; x++) w[b][x] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[b][4 * x4 + x], p.scale_log2, -mr[x]));
+              for (int x = 0; x < 4; x++) w[b][x] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[b][4 * x4 + x], p.scale_log2, -mr[x4][x]));
             if (whole) {
 #pragma unroll
               for (int b = 0; b < 2; b++)
 #pragma unroll
-                for (int x = 0; x < 4; x++) sum[b] = __builtin_fmaf(w[b][x], il[x], sum[b]);
+                for (int x = 0; x < 4; x++) sum[b] = __builtin_fmaf(w[b][x], il[x4][x], sum[b]);
             } else {
 #pragma unroll
               for (int b = 0; b < 2; b++) {
                 const int lo = from[b] - r0 - at, hi = upto[b] - r0 - at;
 #pragma unroll
-                for (int x = 0; x < 4; x++) sum[b] += x >= lo && x < hi ? w[b][x] * il[x] : 0.f;
+                for (int x = 0; x < 4; x++) sum[b] += x >= lo && x < hi ? w[b][x] * il[x4][x] : 0.f;
               }
             }
           }
@@ -874,7 +982,8 @@ hipError_t launch_weigh(WeighArgs a, const WeighPlan& x, int head_dim, hipStream
     a.local_tok = 0;
     a.from_tok = x.few_tok + 1;
     a.to_tok = 0x7fffffff;
-    const dim3 groups(kWeighGroups), wide(kThreads), joins(kWeighGroups - 1);
+    a.groups = head_dim == 128 ? 768 : 512;
+    const dim3 groups(a.groups), wide(kThreads), joins(a.groups - 1);
     if (head_dim == 128) hipLaunchKernelGGL(weigh_stats_kernel<128>, groups, wide, 0, stream, a);
     else hipLaunchKernelGGL(weigh_stats_kernel<256>, groups, wide, 0, stream, a);
     hipLaunchKernelGGL(weigh_stats_join_kernel, joins, wide, 0, stream, a);
