@@ -560,7 +560,7 @@ int qkv_norm_rope(const uint16_t* q, long q_stride, uint16_t* q_out, long q_out_
  * k_dw (device fp32 [head_dim], NULL: not wanted) the gradients of the weights, summed over tokens and heads
  * in fp32, in an order that does not change from call to call.  With num_q or num_k 0 that side's
  * pointers are neither read nor written.  workspace: qkv_norm_rope_grad_workspace_bytes of these numbers or
- * larger ones where a weight's gradient is wanted (no initialisation needed). */
+ * larger ones where a weight's gradient is wanted (no initialisation needed).  Calls sharing one must be ordered. */
 size_t qkv_norm_rope_grad_workspace_bytes(int n_tok, int num_q, int num_k, int head_dim);
 int qkv_norm_rope_grad(const uint16_t* q, long q_stride, const uint16_t* q_dy, long q_dy_stride, uint16_t* q_dx,
                        long q_dx_stride, const float* q_weight, float* q_dw, const uint16_t* k, long k_stride,
@@ -771,7 +771,7 @@ typedef enum qkv_logits_type { QKV_LOGITS_F16 = 0, QKV_LOGITS_F32 = 1, QKV_LOGIT
  * logits row of the beam (request * beams + b), the token and S as fp32; -1, -1 and -infinity where there are
  * fewer candidates.  S is compared in 64 bits.  beams, take <= 64, beams * vocab < 2^31, n * beams <= 2^24
  * (QKV_ERR_UNSUPPORTED).  workspace: qkv_beam_select_workspace_bytes of these numbers or larger ones, aligned to 8
- * bytes (no initialisation needed). */
+ * bytes (no initialisation needed).  Calls sharing one must be ordered. */
 size_t qkv_beam_select_workspace_bytes(int n, int beams, int vocab, int take);
 int qkv_beam_select(const void* logits, int logits_type, long stride, const float* scores, const int32_t* done,
                     int end_token, int n, int beams, int vocab, int take, int32_t* parents, int32_t* tokens,

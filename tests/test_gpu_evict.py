@@ -180,3 +180,20 @@ def test_captured_and_on_a_stream_with_a_larger_workspace():
         torch.cuda.synchronize()
         for a, b in zip((*d, kept), (*pools, *exps, w, want)):
             assert np.array_equal(a.cpu().numpy(), b)
+
+
+@pytest.mark.parametrize("max_ctx", [16384, 16385])
+def test_lengths_around_what_one_workgroup_holds(max_ctx):
+    """The longest slots of the one kind of selection and the shortest of the other, and whole stretches of rows."""
+    rng = np.random.default_rng(max_ctx)
+    lens = [16384, min(16385, max_ctx), 8192, 4096, 4095, 1]
+    for sink, recent in ((0, 0), (1, 1)):
+        _check(*_cache(rng, lens, 128, 1, 128), lens, [16383, 8000, 4096, 1, 4094, 1], max_ctx, 16384, sink, recent)
+
+
+def test_many_slots_of_many_heads():
+    """More chunks than workgroups are at work at a time, whole and partial, of heads that keep other rows."""
+    rng = np.random.default_rng(17)
+    lens = [int(x) for x in rng.integers(0, 900, 64)]
+    keep = [int(x) for x in rng.integers(0, 900, 64)]
+    _check(*_cache(rng, lens, 32, 16, 256), lens, keep, 900, 900, 4, 30)

@@ -215,3 +215,28 @@ def test_a_workspace_of_larger_numbers_a_stream_and_a_graph():
             g.replay()
             torch.cuda.synchronize()
             assert torch.equal(args[3], want)
+
+
+@pytest.mark.parametrize("hd", [128, 256])
+@pytest.mark.parametrize("nq,kv", [(12, 4), (14, 2), (7, 1)])
+def test_groups_that_do_not_divide_a_tile(hd, nq, kv):
+    rng = np.random.default_rng(hd + nq)
+    _check(_batch(rng, [60, 700, 0], [301, 45, 90], 16, kv, hd, nq), decay=0.5)
+    _check(_batch(rng, [60, 700, 0], [301, 45, 90], 16, kv, hd, nq), window=100, sink=9)
+
+
+@pytest.mark.parametrize("hd", [128, 256])
+@pytest.mark.parametrize("new", [[1], [12], [300]])
+@pytest.mark.parametrize("step", [0.5, 7.0, 28.0, -28.0])
+def test_scores_that_rise_and_fall(hd, new, step):
+    """Scores that change by `step` every 64 keys: what has been summed so far becomes next to nothing, many times, or what
+    follows does."""
+    rng = np.random.default_rng(13)
+    b = _batch(rng, [900], new, 16, 1, hd, 4)
+    j = np.arange(900 + new[0])
+    level = j // 64 + 1 if step > 0 else 15 - j // 64
+    page = b["tables"][0][j // 16]
+    b["kp"][page, j % 16] = R.e4m3_encode(level.astype(np.float64))[:, None, None]   # (exact up to 16)
+    b["ke"][:] = 127
+    b["q"][:] = 1 + rng.integers(-3, 4, b["q"].shape) / 64
+    _check(b, scale=abs(step) / hd)
