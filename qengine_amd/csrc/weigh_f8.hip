@@ -284,13 +284,17 @@ __global__ __launch_bounds__(256) void weigh_merge_kernel(WeighArgs p) {
   if ((tid & 15) == 0) put_stat(p, at, x);
 }
 
-// What a key's weight becomes (a key whose page is absent has none).
+// What a key's weight becomes.
+__device__ __forceinline__ float weight_of(const WeighArgs& p, int key, int weighed, float old, float a) {
+  return key < weighed && p.decay != 0.f ? __builtin_fmaf(p.decay, old, a) : a;
+}
+// (a key whose page is absent has none)
 __device__ __forceinline__ void put_weight(const WeighArgs& p, const int32_t* table, int h, int key, int weighed, float a) {
   const BlockAt x = block_at(p, key);
   const int pg = page_of(p, table, x.b);
   if (pg < 0) return;
   float* w = p.weights + ((long)pg * p.num_kv + h) * p.block_tokens + x.row;
-  *w = key < weighed && p.decay != 0.f ? __builtin_fmaf(p.decay, *w, a) : a;
+  *w = weight_of(p, key, weighed, *w, a);
 }
 
 // Few rows: 1,024 keys a workgroup, four of a thread.  MERGED: by the rows' statistics, else by their chunks'.
@@ -306,6 +310,22 @@ __global__ __launch_bounds__(256) void weigh_few_kernel(WeighArgs p) {
   const int key = wk.x * 1024 + 4 * tid;
   if (sl.n <= 0 || wk.x * 1024 >= sl.end) return;
   const int rows = sl.n * p.gqa;
+  // What does not wait for the statistics, ahead of them: the keys' page (4 keys lie in one), their weights, and the
+  // scores of the first rows.
+  constexpr int AHEAD = 4;
+  const bool live = key < sl.end;
+  const int key_l = live ? key : 0;
+  const BlockAt bl = block_at(p, key_l);
+  const int pg = page_of(p, p.tables + (long)s * p.max_blocks, bl.b);
+  const int weighed = p.weighed ? p.weighed[s] : sl.pos0;
+  float* w = p.weights + ((long)max(pg, 0) * p.num_kv + h) * p.block_tokens + bl.row;
+  const bool out = out_of_window(p, sl, key & ~31);   // (its scores were not stored)
+  f4_t old, ahead[AHEAD];
+#pragma unroll
+  for (int i = 0; i < 4; i++) old[i] = w[i];
+#pragma unroll
+  for (int r = 0; r < AHEAD; r++)
+    ahead[r] = *reinterpret_cast<const f4_t*>(p.scores + place_of(p, sl, s, h, min(r, rows - 1)) * p.score_pitch + key_l);
   if constexpr (MERGED) {
     if (tid < rows) {
       const long x = place_of(p, sl, s, h, tid);
@@ -323,19 +343,21 @@ __global__ __launch_bounds__(256) void weigh_few_kernel(WeighArgs p) {
     }
   }
   __syncthreads();
-  if (key >= sl.end) return;
+  if (!live || pg < 0) return;   // (a key whose page is absent has no weight)
   f4_t a = {0.f, 0.f, 0.f, 0.f};
-  const bool out = out_of_window(p, sl, key & ~31);   // (its scores were not stored)
-  for (int r = 0; r < rows && !out; r++) {
-    const f4_t v = *reinterpret_cast<const f4_t*>(p.scores + at[r] + key);
+  auto add = [&](const f4_t& v, int r) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < 4; i++) a[i] += v[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(v[i] - stat[r][0]) * stat[r][1];
+  };
+  if (!out) {
+#pragma unroll
+    for (int r = 0; r < AHEAD; r++)
+      if (r < rows) add(ahead[r], r);
+    for (int r = AHEAD; r < rows; r++) add(*reinterpret_cast<const f4_t*>(p.scores + at[r] + key), r);
   }
-  const int32_t* table = p.tables + (long)s * p.max_blocks;
-  const int weighed = p.weighed ? p.weighed[s] : sl.pos0;
 #pragma unroll
   for (int i = 0; i < 4; i++)
-    if (key + i < sl.end) put_weight(p, table, h, key + i, weighed, a[i]);
+    if (key + i < sl.end) w[i] = weight_of(p, key + i, weighed, old[i], a[i]);
 }
 
 // ---------------------------------------------------------------------------
