@@ -130,12 +130,14 @@ __global__ __launch_bounds__(1024) void evict_select_kernel(EvictArgs p) {
   int need = c.need;
   if (bad || need == 0) return;
   const int steps = ((c.rows + 15) / 16 + 63) / 64, lo = min(wave * steps * 64, c.rows), hi = min(lo + steps * 64, c.rows);
+  // (all pages' loads, then all weights', under way together; past the wave's rows the last one again)
   uint32_t held[STEPS];
+  int page[STEPS];
+  auto row = [&](int t) { return block_at(p.bt_magic, p.block_tokens, c.first + min(lo + 64 * t + lane, max(hi - 1, 0))); };
 #pragma unroll
-  for (int t = 0; t < STEPS; t++) {
-    const int i = lo + 64 * t + lane;
-    held[t] = i < hi ? weight_at(p, table, h, c.first + i) : 0u;
-  }
+  for (int t = 0; t < STEPS; t++) page[t] = table[row(t).b];
+#pragma unroll
+  for (int t = 0; t < STEPS; t++) held[t] = order_of(p.weights[((long)page[t] * p.num_kv + h) * p.block_tokens + row(t).row]);
   // f(row, key, whether it is one) over the wave's rows in order
   auto each = [&](auto&& f) {
 #pragma unroll
@@ -168,6 +170,11 @@ __global__ __launch_bounds__(1024) void evict_select_kernel(EvictArgs p) {
     __syncthreads();
     prefix = prefix << 8 | (uint32_t)(255 - found[0]);
     need = found[1];
+    if (need == count[255 - found[0]]) {   // (all that begin so stay: the digits below do not matter)
+      prefix <<= shift;
+      need = 0x7fffffff;
+      break;
+    }
   }
   // rows above the threshold stay, and the first `need` of those at it
   int gt = 0, eq = 0;
