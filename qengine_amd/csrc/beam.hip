@@ -5,6 +5,9 @@
 // The logits are read once: a workgroup takes a segment of one row, holds it in registers, sums its
 // exponentials and keeps its `take` largest logits; a second launch joins a request's segments.  Inside a
 // row the order of S is that of x, so segments compare the logits themselves, without a rounding.
+// 512 rows of 131,072 fp16 logits take 31 + 12 us (21 at 6.4 TB/s); the vector unit bounds the first launch, busy
+// 0.8 of its time: 6 instructions a logit for its exponential, 1 for the maximum, and the selection's threshold,
+// maxima of the lanes in turn, a fifth.  Eight workgroups are on a CU, so that others load while one selects.
 //
 // The exponentials are taken in base 2 of the distance to the segment's maximum (exact for 16-bit logits),
 // times log2(e) as two floats: their error stays near their own rounding, where a product of the logit and one
@@ -22,7 +25,7 @@ namespace {
 
 constexpr float kLog2eHi = 1.44269502162933349609375f;   // log2(e) to 24 bits, and what is left of it
 constexpr float kLog2eLo = 1.925963033500011e-8f;
-constexpr int kCap = 512;                                // candidates of a workgroup in LDS
+constexpr int kCap = 512, kWordCap = 128;                // candidates, and words that hold some, of a workgroup in LDS
 
 // v of the lane that steps 1, 2, 7, 15 (mirrored in its quad, half row and row), 16 and 32 pair this one with
 template <int STEP>
@@ -44,10 +47,27 @@ __device__ __forceinline__ double pair_of(double v) {
   const uint64_t hi = __float_as_uint(pair_of<STEP>(__uint_as_float((uint32_t)(b >> 32))));
   return __builtin_bit_cast(double, hi << 32 | lo);
 }
-template <class V>
-__device__ __forceinline__ V larger(V a, V b) { return b > a ? b : a; }
-template <class V>
-__device__ __forceinline__ V wave_max(V v) {   // (no NaN)
+// Values as the selection's maxima compare them: floats by whole numbers in the same order (of which a maximum over lanes
+// is one instruction a step), doubles as they are.
+__device__ __forceinline__ int key_of(float v) {
+  const int b = __float_as_int(v);
+  return b ^ (b >> 31 & 0x7fffffff);
+}
+__device__ __forceinline__ float of_key(int k) { return __int_as_float(k ^ (k >> 31 & 0x7fffffff)); }
+__device__ __forceinline__ double key_of(double v) { return v; }
+__device__ __forceinline__ double of_key(double v) { return v; }
+__device__ __forceinline__ int wave_max(int v) {
+  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0xb1, 0xf, 0xf, true));
+  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x4e, 0xf, 0xf, true));
+  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x141, 0xf, 0xf, true));
+  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x140, 0xf, 0xf, true));
+  const auto a = __builtin_amdgcn_permlane16_swap((uint32_t)v, (uint32_t)v, false, false);
+  v = max((int)a[0], (int)a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap((uint32_t)v, (uint32_t)v, false, false);
+  return max((int)b[0], (int)b[1]);
+}
+__device__ __forceinline__ double wave_max(double v) {   // (no NaN)
+  auto larger = [](double a, double b) { return b > a ? b : a; };
   v = larger(v, pair_of<1>(v));
   v = larger(v, pair_of<2>(v));
   v = larger(v, pair_of<7>(v));
@@ -77,47 +97,53 @@ __device__ __forceinline__ bool better(V a, int ia, V b, int ib) { return a > b 
 
 // The k <= 64 largest of what the 256 threads hold, ties to the lowest index, as put(rank, value, index) by
 // any thread; returns how many there are (at most k).  `top` is this thread's largest, each(f, low) calls
-// f(value, index) for at least those of its values that are >= low; -infinity is no value.
+// f(value, index) for at least those of its values that are >= low; -infinity is no value.  gather(f, low) does so
+// for all threads' together, in any of them.
 //
 // At least k threads hold a value >= the smallest, over the four waves, of the (k + 3) / 4-th largest of the
 // lanes' maxima (and >= the k-th largest of any one wave's, which counts where another wave has too few).  What
 // is at or above that goes to LDS, usually a few times k, and is ranked there by counting.  Where more values
-// tie than LDS holds, they are found one after the other.
-template <class V, class Each, class Put>
-__device__ __forceinline__ int top_of_group(Found<V>& found, int k, V top, Each&& each, Put&& put) {
+// tie than LDS holds, they are found one after the other.  (The smallest maximum of k groups of lanes is found sooner, but
+// more values lie above it: 35 -> 44 us for 512 rows of 131,072.)
+template <class V, class Each, class Gather, class Put>
+__device__ __forceinline__ int top_of_group(Found<V>& found, int k, V top, Each&& each, Gather&& gather, Put&& put) {
   const V none = -INFINITY;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  V mine = top, low = none;
-  auto next = [&](int from, int to) {   // the to-th largest, after `from` of them
-    for (int i = from; i < to; i++) {
-      low = wave_max(mine);
-      const uint64_t m = __builtin_amdgcn_ballot_w64(mine == low);
-      if (m && lane == (int)__builtin_ctzll(m)) mine = none;
+  V low;
+  auto mine = key_of(top);
+  auto next = [&](int n) {   // the wave's n-th largest
+    auto best = mine;
+    for (int i = 0; i < n; i++) {
+      best = wave_max(mine);
+      const uint64_t m = __builtin_amdgcn_ballot_w64(mine == best);
+      if (lane == (int)__builtin_ctzll(m)) mine = key_of(none);
     }
-    if (lane == 0) found.low[wave] = low;
+    if (lane == 0) found.low[wave] = of_key(best);
   };
-  next(0, (k + 3) / 4);
+  next((k + 3) / 4);
   if (tid == 0) found.n = 0;
   __syncthreads();
+  low = found.low[0];
 #pragma unroll
-  for (int w = 0; w < 4; w++) low = found.low[w] < low ? found.low[w] : low;
+  for (int w = 1; w < 4; w++) low = found.low[w] < low ? found.low[w] : low;
   if (low == none) {   // (the same in every wave)
     __syncthreads();
-    next((k + 3) / 4, k);
+    mine = key_of(top);
+    next(k);
     __syncthreads();
+    low = found.low[0];
 #pragma unroll
-    for (int w = 0; w < 4; w++) low = found.low[w] > low ? found.low[w] : low;
+    for (int w = 1; w < 4; w++) low = found.low[w] > low ? found.low[w] : low;
   }
-  if (top >= low)
-    each([&](V v, int at) __attribute__((always_inline)) {
-      if (v >= low && v > none) {
-        const int i = atomicAdd(&found.n, 1);
-        if (i < kCap) {
-          found.v[i] = v;
-          found.at[i] = at;
-        }
+  gather([&](V v, int at) __attribute__((always_inline)) {
+    if (v >= low && v > none) {
+      const int i = atomicAdd(&found.n, 1);
+      if (i < kCap) {
+        found.v[i] = v;
+        found.at[i] = at;
       }
-    }, low);
+    }
+  }, low);
   __syncthreads();
   const int n = found.n;
   if (n <= kCap) {
@@ -125,6 +151,7 @@ __device__ __forceinline__ int top_of_group(Found<V>& found, int k, V top, Each&
       const V v = found.v[i];
       const int at = found.at[i];
       int rank = 0;
+#pragma unroll 8
       for (int j = 0; j < n; j++) rank += better(found.v[j], found.at[j], v, at);
       if (rank < k) put(rank, v, at);
     }
@@ -170,6 +197,13 @@ __device__ __forceinline__ int top_of_group(Found<V>& found, int k, V top, Each&
   return k;
 }
 
+// The largest, or NaN
+__device__ __forceinline__ float maximum(float a, float b, float c) {
+  asm("v_maximum3_f32 %0, %1, %2, %3" : "=v"(a) : "v"(a), "v"(b), "v"(c));
+  return a;
+}
+__device__ __forceinline__ float maximum(float a, float b) { return maximum(a, b, b); }
+
 // Logits of one 16-byte word
 template <int TYPE>
 struct Word;
@@ -178,12 +212,23 @@ struct Word<0> {   // fp16
   static constexpr int N = 8;
   static constexpr uint32_t kNone = 0xfc00u;
   __device__ static __forceinline__ float at(u4_t w, int i) { return h2f(i & 1 ? w[i >> 1] >> 16 : w[i >> 1] & 0xffffu); }
+  // the largest, NaN where one is (pairs at a time: 6 instructions for 8 logits)
+  __device__ static __forceinline__ float top(u4_t w) {
+    uint32_t m;
+    asm("v_pk_maximum3_f16 %0, %1, %2, %3" : "=v"(m) : "v"(w[0]), "v"(w[1]), "v"(w[2]));
+    asm("v_pk_maximum3_f16 %0, %1, %2, %2" : "=v"(m) : "v"(m), "v"(w[3]));
+    return maximum(h2f(m & 0xffffu), h2f(m >> 16));
+  }
+  // x - ref in one instruction
+  __device__ static __forceinline__ float less(u4_t w, int i, float ref, float one) { return __builtin_fmaf(at(w, i), one, -ref); }
 };
 template <>
 struct Word<1> {   // fp32
   static constexpr int N = 4;
   static constexpr uint32_t kNone = 0xff800000u;
   __device__ static __forceinline__ float at(u4_t w, int i) { return __uint_as_float(w[i]); }
+  __device__ static __forceinline__ float top(u4_t w) { return maximum(maximum(at(w, 0), at(w, 1), at(w, 2)), at(w, 3)); }
+  __device__ static __forceinline__ float less(u4_t w, int i, float ref, float) { return at(w, i) - ref; }
 };
 template <>
 struct Word<2> {   // bf16
@@ -192,6 +237,16 @@ struct Word<2> {   // bf16
   __device__ static __forceinline__ float at(u4_t w, int i) {
     return __uint_as_float(i & 1 ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16);
   }
+  __device__ static __forceinline__ float top(u4_t w) {
+    float m = maximum(at(w, 0), at(w, 1));
+#pragma unroll
+    for (int i = 2; i < N; i += 2) {
+      m = maximum(m, at(w, i), at(w, i + 1));
+      asm volatile("" : "+v"(m));   // (in turn: the numbers of many words would fill the registers)
+    }
+    return m;
+  }
+  __device__ static __forceinline__ float less(u4_t w, int i, float ref, float) { return at(w, i) - ref; }
 };
 // NaN and +infinity to -infinity
 template <int TYPE>
@@ -218,6 +273,8 @@ __global__ __launch_bounds__(256, 4) void beam_rows_kernel(BeamArgs p) {
   using W = Word<TYPE>;
   constexpr int SIZE = 16 / W::N;
   __shared__ Found<float> found;
+  __shared__ u4_t word_s[kWordCap];   // words that hold a candidate, and their first element's token
+  __shared__ int word_at[kWordCap], n_words;
   __shared__ float part[4], sums[4];
   const long wg = (long)blockIdx.y * kGridX + blockIdx.x;
   if (wg >= (long)p.rows * p.segments) return;
@@ -255,51 +312,43 @@ __global__ __launch_bounds__(256, 4) void beam_rows_kernel(BeamArgs p) {
         }
     }
   }
-  // Logits that are left out show in the maximum (+infinity) or in the sum (NaN): only then are all looked at.
+  // Logits that are left out show in the maximum (+infinity or NaN): only then are all looked at.
   float tops[NV], top;
   auto look = [&]() __attribute__((always_inline)) {
     top = -INFINITY;
 #pragma unroll
     for (int j = 0; j < NV; j++) {
-      tops[j] = -INFINITY;   // (fmaxf leaves a NaN out)
-#pragma unroll
-      for (int i = 0; i < W::N; i += 2) tops[j] = fmaxf(fmaxf(tops[j], W::at(raw[j], i)), W::at(raw[j], i + 1));
-      top = fmaxf(top, tops[j]);
+      tops[j] = W::top(raw[j]);
+      top = maximum(top, tops[j]);
     }
-    return wave_max(top);
   };
-  auto clean = [&]() __attribute__((always_inline)) {
+  look();
+  if (__builtin_amdgcn_ballot_w64(!(top < INFINITY))) {
 #pragma unroll
     for (int j = 0; j < NV; j++) leave_out<TYPE>(raw[j]);
-    return look();
-  };
-  float wmax = look();
-  if (wmax == INFINITY) wmax = clean();
+    look();
+  }
+  const float wmax = of_key(wave_max(key_of(top)));
   if (lane == 0) part[wave] = wmax;
+  if (tid == 0) n_words = 0;
   __syncthreads();
   const float m = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])), ref = m == -INFINITY ? 0.f : m;
-  auto add = [&]() __attribute__((always_inline)) {
-    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+  float sum[4] = {0.f, 0.f, 0.f, 0.f}, one = 1.f;
+  asm("" : "+v"(one));
 #pragma unroll
-    for (int j = 0; j < NV; j++) {
-      asm("" : "+v"(raw[j]));   // (converted again, not held as floats)
+  for (int j = 0; j < NV; j++) {
+    asm("" : "+v"(raw[j]));   // (converted again, not held as floats)
 #pragma unroll
-      for (int i = 0; i < W::N; i++) {
-        const float t = W::at(raw[j], i) - ref;
-        sum[i & 3] += __builtin_amdgcn_exp2f(__builtin_fmaf(t, kLog2eLo, t * kLog2eHi));
-      }
+    for (int i = 0; i < W::N; i++) {
+      const float t = W::less(raw[j], i, ref, one);
+      sum[i & 3] += __builtin_amdgcn_exp2f(__builtin_fmaf(t, kLog2eLo, t * kLog2eHi));
     }
-    return wave_sum((sum[0] + sum[1]) + (sum[2] + sum[3]));
-  };
-  float l = add();
-  if (l != l) {
-    clean();
-    l = add();
   }
+  const float l = wave_sum((sum[0] + sum[1]) + (sum[2] + sum[3]));
   if (lane == 0) sums[wave] = l;
   const long rec = wg * p.take;
   const int token0 = (int)(w0 * W::N - skip);
-  const int n = top_of_group<float>(found, p.take, top, [&](auto&& f, float low) __attribute__((always_inline)) {
+  auto each = [&](auto&& f, float low) __attribute__((always_inline)) {
 #pragma unroll
     for (int j = 0; j < NV; j++)
       if (tops[j] >= low) {
@@ -309,7 +358,36 @@ __global__ __launch_bounds__(256, 4) void beam_rows_kernel(BeamArgs p) {
 #pragma unroll
         for (int i = 0; i < W::N; i++) f(W::at(w, i), at + i);
       }
-  }, [&](int rank, float v, int at) {
+  };
+  // Words go to LDS whole and are looked at by all threads: a wave of which one lane holds a candidate would look at
+  // all 64 lanes' (35 -> 32 us for 512 rows of 131,072).
+  auto gather = [&](auto&& f, float low) __attribute__((always_inline)) {
+    if (top >= low) {
+#pragma unroll
+      for (int j = 0; j < NV; j++)
+        if (tops[j] >= low) {
+          const int i = atomicAdd(&n_words, 1);
+          if (i < kWordCap) {
+            word_s[i] = raw[j];
+            word_at[i] = token0 + (256 * j + tid) * W::N;
+          }
+        }
+    }
+    __syncthreads();
+    const int n = n_words;
+    if (n > kWordCap) {
+      if (top >= low) each(f, low);
+      return;
+    }
+    for (int x = tid; x < n * W::N; x += 256) {
+      const u4_t w = word_s[x / W::N];
+      float v = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < W::N; i++) v = x % W::N == i ? W::at(w, i) : v;
+      f(v, word_at[x / W::N] + x % W::N);
+    }
+  };
+  const int n = top_of_group<float>(found, p.take, top, each, gather, [&](int rank, float v, int at) {
     p.rec_x[rec + rank] = v;
     p.rec_at[rec + rank] = at;
   });
@@ -399,12 +477,15 @@ __global__ __launch_bounds__(256) void beam_join_kernel(BeamArgs p) {
       }
     }
 #pragma unroll
-    for (int i = 0; i <= RPT; i++) top = larger(top, v[i]);
+    for (int i = 0; i <= RPT; i++) top = v[i] > top ? v[i] : top;
     auto each = [&](auto&& f, double) __attribute__((always_inline)) {
 #pragma unroll
       for (int i = 0; i <= RPT; i++) f(v[i], id[i]);
     };
-    n = top_of_group<double>(found, k, top, each, [&](int rank, double value, int what) {
+    auto gather = [&](auto&& f, double low) __attribute__((always_inline)) {
+      if (top >= low) each(f, low);
+    };
+    n = top_of_group<double>(found, k, top, each, gather, [&](int rank, double value, int what) {
       best[rank] = value;
       best_at[rank] = what;
     });

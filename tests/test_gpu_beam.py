@@ -223,3 +223,23 @@ def test_reorder_large_states_captured():
         g.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip((state, odd, tables, refs), before))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+def test_numbers_that_are_none_of_every_kind(dtype):
+    """Quiet and signalling NaN and infinities beside the largest logits of their words, in rows of every length up to
+    some words of a wave: none is selected, none is summed."""
+    rng = np.random.default_rng(21)
+    bits = {torch.float16: ([0x7e00, 0x7d01, 0xfe00, 0xfd55, 0x7c00, 0xfc00], torch.int16),
+            torch.bfloat16: ([0x7fc0, 0x7f81, 0xffc0, 0xff95, 0x7f80, 0xff80], torch.int16),
+            torch.float32: ([0x7fc00000, 0x7f800001, 0xffc00000, 0xff955555, 0x7f800000, 0xff800000], torch.int32)}[dtype]
+    kinds = torch.tensor(np.array(bits[0], np.uint32).astype(np.int64)).to(torch.int64)
+    kinds = (kinds - (kinds >= 2 ** (31 if dtype is torch.float32 else 15)) * 2 ** (32 if dtype is torch.float32 else 16)).to(bits[1])
+    for vocab in (1, 7, 8, 9, 33, 500, 5000, 40000):
+        for k in (1, 3, 8):
+            x = torch.from_numpy(rng.standard_normal((6, vocab)) * 3).to(dtype)
+            at = torch.from_numpy(rng.random((6, vocab)) < 0.2)
+            pick = torch.from_numpy(rng.integers(0, 6, (6, vocab)))
+            x.view(bits[1])[at] = kinds[pick][at]
+            scores = torch.from_numpy(rng.standard_normal((3, 2)).astype(np.float32))
+            _check(x.to(DEV), scores.to(DEV), k)
