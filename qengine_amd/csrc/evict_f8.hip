@@ -13,7 +13,7 @@
 // for all costs 11 ns a chunk: 106 of 130 us for 9,216 of them.)
 //
 // Bound by latency where slots are few (one of 131,072 rows to 16,384: the selection's four launches 34 us, the rows' 30,
-// of 14 at 4.8 TB/s) and by HBM where they are many (24 slots, 322 MB read and written: 20 and 93 us, 3.5 TB/s; rows of
+// of 14 at 4.8 TB/s) and by HBM where they are many (24 slots, 322 MB read and written: 20 and 85 us, 3.8 TB/s; rows of
 // 128 to 256 bytes, each with the table's and the list's entries ahead of it).
 //
 // A page's exponent becomes the largest of those its rows had; codes of the others are requantized by a power of
@@ -466,7 +466,8 @@ __global__ __launch_bounds__(256) void evict_move_kernel(EvictArgs p) {
 #pragma unroll
         for (int e = 0; e < 4; e++) v[e] = rescale4(v[e], f);
       }
-      if (d > 0 || src[i] != r0 + x) *reinterpret_cast<u4_t*>((j ? p.v_pool : p.k_pool) + o) = v;
+      // (past the caches, which the rows still to be read go through: 93 -> 85 us for 24 slots)
+      if (d > 0 || src[i] != r0 + x) __builtin_nontemporal_store(v, reinterpret_cast<u4_t*>((j ? p.v_pool : p.k_pool) + o));
     }
   }
   if (tid < rows && w_src != r0 + tid) p.weights[((long)w_page * p.num_kv + h) * bt + w_row] = w;
