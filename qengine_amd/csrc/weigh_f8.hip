@@ -794,12 +794,13 @@ __global__ __launch_bounds__(kThreads) void weigh_stats_join_kernel(WeighArgs p)
   if (row < sl.n * p.gqa) put_stat(p, row_at(p, sl, c.h, row), x);
 }
 
-// Sums of keys.  A step brings its rows' statistics along.
+// Sums of keys.  A step brings its rows' statistics along.  (The ring leaves room for as many workgroups as registers do:
+// 128 dims by steps of 32 rows and four of them 70 us, 66 by 64 and three.)
 template <int HD>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(HD == 128 ? 3 : 2, HD == 128 ? 3 : 2))) void weigh_sums_kernel(WeighArgs p) {
-  constexpr int STEP = 32, NB = HD / 32, RB = HD * 2, TB = STEP * RB, LOADS = TB / 1024 / kWaves, WORDS = RB / 16;
-  __shared__ __align__(512) uint8_t ring[kRing][TB];
-  __shared__ __align__(16) float stat_lds[kRing][3][64];   // m, 1 / l, and what the other waves load beside them
+  constexpr int STEP = HD == 128 ? 64 : 32, RING = HD == 128 ? 3 : 4, NB = HD / 32, RB = HD * 2, TB = STEP * RB, LOADS = TB / 1024 / kWaves, WORDS = RB / 16;
+  __shared__ __align__(512) uint8_t ring[RING][TB];
+  __shared__ __align__(16) float stat_lds[RING][3][64];   // m, 1 / l, and what the other waves load beside them
   __shared__ LineLds lds;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 31, hh = lane >> 5;
@@ -848,7 +849,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(HD == 
       };
       __syncthreads();   // (the ring is written again)
 #pragma unroll
-      for (int j = 0; j < kRing - 1; j++) load(v0 + j, j);
+      for (int j = 0; j < RING - 1; j++) load(v0 + j, j);
       h8_t kf[2][NB][2];
       int from[2], upto[2];   // rows that see lane c's keys: from .. upto-1
 #pragma unroll
@@ -869,11 +870,11 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(HD == 
       }
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // (from here on only steps are under way)
       for (int v = v0; v < v1; v++) {
-        const int buf = (v - v0) % kRing, r0 = t.r_lo + STEP * v;
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((kRing - 2) * (LOADS + 1)) : "memory");
+        const int buf = (v - v0) % RING, r0 = t.r_lo + STEP * v;
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((RING - 2) * (LOADS + 1)) : "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        load(v + kRing - 1, (v - v0 + kRing - 1) % kRing);
+        load(v + RING - 1, (v - v0 + RING - 1) % RING);
 #pragma unroll
         for (int half = 0; half < STEP / 32; half++) {
           const int rh = r0 + 32 * half;
