@@ -887,13 +887,11 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(HD == 
           for (int j = 0; j < NB; j += 2) {
             u4_t a[4];
             lds_read(a, src ^ (64 * j), src ^ (64 * j + 16), src ^ (64 * j + 64), src ^ (64 * j + 80));
-            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int x = 0; x < 4; x++)
 #pragma unroll
               for (int b = 0; b < 2; b++)
                 acc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8_t, a[x]), kf[b][j + x / 2][x % 2], acc[b], 0, 0, 0);
-            __builtin_amdgcn_s_setprio(0);
           }
           f4_t mr[4], il[4];
           lds_read(mr, il, stat_at + buf * (4 * 3 * 64) + 128 * half);
