@@ -14,8 +14,8 @@
 // Many rows: both passes form the scores by the matrix cores, 2 head_dim operations a row and key each; the first
 // holds rows in registers and passes keys by (a lane's scores are one row's, so maximum and sum stay in it), the
 // second holds keys and passes rows by (a lane's are one key's).  Bound by the vector unit and the matrix cores together:
-// 164 million scores of 128 dims take 56 + 70 us (34 each at a large library product's rate), 138 million of 256 dims 87 +
-// 95 (60 each).
+// 164 million scores of 128 dims take 55 + 65 us (34 each at a large library product's rate), 138 million of 256 dims 84 +
+// 93 (60 each).
 //
 // Codes are converted to fp16 with their exponent (exact), products summed in fp32; weights are fp32 from the
 // exponential on and never rounded to fewer bits.  All sums are taken in one order, whatever the timing.
@@ -376,7 +376,7 @@ __global__ __launch_bounds__(256) void weigh_few_kernel(WeighArgs p) {
 // matrix cores (a score of 64 lanes: fma 4 cycles, exponential 8, sum 4, conversion 2 to 4; its products 16 of
 // 128 dims), and that a wave does them in turn.  So there are as many workgroups on a CU as registers allow, 3 of
 // 128 dims and 2 of 256, none of which waits for another's barrier (one of eight waves instead: 66 and 78 us for 164
-// million scores of 128 dims, now 56 and 70; 90 and 107 for 138 million of 256 dims, now 88 and 97).  Adding up the
+// million scores of 128 dims, now 55 and 65; 90 and 107 for 138 million of 256 dims, now 84 and 93).  Adding up the
 // scores before beside the next ones' products, written into one stream of instructions, needs registers
 // for both: 60 us, and 87.
 //
