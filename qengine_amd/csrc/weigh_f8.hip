@@ -554,13 +554,14 @@ __device__ __forceinline__ void run_part(const WeighArgs& p, const Tiles& tiles,
 
 // The tile that part g continues, if it was begun in part g - 1: its records are `first`, then 2 g, 2 (g + 1) .. of the
 // n - 1 parts that continue it.
+constexpr int kJoin = 4;   // threads a row or key, each every fourth record (one: 13 us where a tile has 100, now 8)
 struct CutTile {
   int s, i, h, first, n, g;
   __device__ __forceinline__ long record(int x) const { return x == 0 ? first : 2 * (g + x - 1); }
 };
 __device__ __forceinline__ bool cut_tile(const WeighArgs& p, CutTile& c) {
   __shared__ int4 cuts[kWeighGroups];
-  for (int x = threadIdx.x; x < p.groups; x += kThreads) cuts[x] = reinterpret_cast<const int4*>(p.cuts)[x];
+  for (int x = threadIdx.x; x < p.groups; x += kJoin * kThreads) cuts[x] = reinterpret_cast<const int4*>(p.cuts)[x];
   __syncthreads();
   const int g = (int)blockIdx.x + 1;
   const int4 here = cuts[g], before = cuts[g - 1];
@@ -780,17 +781,24 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(HD == 
   });
 }
 
-__global__ __launch_bounds__(kThreads) void weigh_stats_join_kernel(WeighArgs p) {
+__global__ __launch_bounds__(kJoin * kThreads) void weigh_stats_join_kernel(WeighArgs p) {
+  __shared__ f2_t part[kJoin][kThreads];
   CutTile c;
   if (!cut_tile(p, c)) return;
+  const int t = (int)threadIdx.x % kThreads, w = (int)threadIdx.x / kThreads;
   Stat x{-INFINITY, 0.f};
-#pragma unroll 8
-  for (int j = 0; j < c.n; j++) {
-    const f2_t v = *reinterpret_cast<const f2_t*>(p.rec + (c.record(j) * kTile + threadIdx.x) * 2);
+#pragma unroll 4
+  for (int j = w; j < c.n; j += kJoin) {
+    const f2_t v = *reinterpret_cast<const f2_t*>(p.rec + (c.record(j) * kTile + t) * 2);
     x = join(x, Stat{v[0], v[1]});
   }
+  part[w][t] = f2_t{x.m, x.l};
+  __syncthreads();
+  if (w > 0) return;
+#pragma unroll
+  for (int i = 1; i < kJoin; i++) x = join(x, Stat{part[i][t][0], part[i][t][1]});
   const Slot sl = slot_of(p, c.s);
-  const int row = c.i * kTile + (int)threadIdx.x;
+  const int row = c.i * kTile + t;
   if (row < sl.n * p.gqa) put_stat(p, row_at(p, sl, c.h, row), x);
 }
 
@@ -937,14 +945,21 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(HD == 
   });
 }
 
-__global__ __launch_bounds__(kThreads) void weigh_sums_join_kernel(WeighArgs p) {
+__global__ __launch_bounds__(kJoin * kThreads) void weigh_sums_join_kernel(WeighArgs p) {
+  __shared__ float part[kJoin][kThreads];
   CutTile c;
   if (!cut_tile(p, c)) return;
+  const int t = (int)threadIdx.x % kThreads, w = (int)threadIdx.x / kThreads;
   float a = 0.f;
-#pragma unroll 8
-  for (int j = 0; j < c.n; j++) a += p.sums[c.record(j) * kTile + threadIdx.x];
+#pragma unroll 4
+  for (int j = w; j < c.n; j += kJoin) a += p.sums[c.record(j) * kTile + t];
+  part[w][t] = a;
+  __syncthreads();
+  if (w > 0) return;
+#pragma unroll
+  for (int i = 1; i < kJoin; i++) a += part[i][t];
   const Slot sl = slot_of(p, c.s);
-  const int key = c.i * kTile + (int)threadIdx.x;
+  const int key = c.i * kTile + t;
   if (key < sl.end) put_weight(p, p.tables + (long)c.s * p.max_blocks, c.h, key, p.weighed ? p.weighed[c.s] : sl.pos0, a);
 }
 
@@ -1008,13 +1023,13 @@ hipError_t launch_weigh(WeighArgs a, const WeighPlan& x, int head_dim, hipStream
     a.from_tok = x.few_tok + 1;
     a.to_tok = 0x7fffffff;
     a.groups = head_dim == 128 ? 768 : 512;
-    const dim3 groups(a.groups), wide(kThreads), joins(a.groups - 1);
+    const dim3 groups(a.groups), wide(kThreads), joins(a.groups - 1), join_wide(kJoin * kThreads);
     if (head_dim == 128) hipLaunchKernelGGL(weigh_stats_kernel<128>, groups, wide, 0, stream, a);
     else hipLaunchKernelGGL(weigh_stats_kernel<256>, groups, wide, 0, stream, a);
-    hipLaunchKernelGGL(weigh_stats_join_kernel, joins, wide, 0, stream, a);
+    hipLaunchKernelGGL(weigh_stats_join_kernel, joins, join_wide, 0, stream, a);
     if (head_dim == 128) hipLaunchKernelGGL(weigh_sums_kernel<128>, groups, wide, 0, stream, a);
     else hipLaunchKernelGGL(weigh_sums_kernel<256>, groups, wide, 0, stream, a);
-    hipLaunchKernelGGL(weigh_sums_join_kernel, joins, wide, 0, stream, a);
+    hipLaunchKernelGGL(weigh_sums_join_kernel, joins, join_wide, 0, stream, a);
   }
   return hipGetLastError();
 }
