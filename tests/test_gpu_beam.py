@@ -243,3 +243,22 @@ def test_numbers_that_are_none_of_every_kind(dtype):
             x.view(bits[1])[at] = kinds[pick][at]
             scores = torch.from_numpy(rng.standard_normal((3, 2)).astype(np.float32))
             _check(x.to(DEV), scores.to(DEV), k)
+
+
+def test_rows_and_states_past_four_billion_bytes():
+    g = torch.Generator(device=DEV).manual_seed(3)
+    wide = torch.zeros(4, 1 << 30, dtype=torch.float16, device=DEV)
+    x = wide[:, :33333]
+    x.copy_(3 * torch.randn(4, 33333, device=DEV, generator=g))
+    assert _check(x, torch.randn(2, 2, device=DEV, generator=g), 5) == 10
+    del wide, x
+    states = torch.zeros(260, 17 << 20, dtype=torch.uint8, device=DEV)
+    rows = torch.randint(0, 256, (2, 17 << 20), dtype=torch.uint8, device=DEV, generator=g)
+    states[0], states[259] = rows[0], rows[1]
+    tables = torch.full((260, 2), -1, dtype=torch.int32, device=DEV)
+    refs = torch.zeros(4, dtype=torch.int32, device=DEV)
+    slots = torch.tensor([0, 259, 130], dtype=torch.int32, device=DEV)
+    parents = torch.tensor([259, 0, 259], dtype=torch.int32, device=DEV)
+    kvcache.pages_reorder(tables, refs, slots, parents, torch.zeros_like(slots), None, kvcache.page_planes([states]), block_tokens=16)
+    assert torch.equal(states[0], rows[1]) and torch.equal(states[259], rows[0]) and torch.equal(states[130], rows[1])
+    assert not states[1:130].any() and not states[131:259].any()

@@ -259,3 +259,72 @@ def test_a_beam_search(dtype):
         used = c.tables[c.tables >= 0]
         assert np.array_equal(np.bincount(used, minlength=len(c.refs)), c.refs)
     assert done.any()
+
+
+@pytest.mark.parametrize("new", [[1, 1, 1], [90, 5, 1]])
+def test_pages_past_four_billion_bytes(new):
+    """The same pages at the front of a small pool and past 2^32 bytes of a large one: the same bits, and nothing else is
+    touched of the large one's first pages."""
+    rng = np.random.default_rng(23)
+    bt, kv, hd, nq, far, lens = 64, 4, 256, 16, 70000, [700, 64, 1500]
+    tables, starts, positions, n = R.layout(rng, lens, new, bt, kv, hd)
+    pools = [R.random_pool(rng, n, bt, kv, hd) for _ in range(2)]
+    w = rng.random((n, kv, bt)).astype(np.float32)
+    q = _t(rng.standard_normal((int(starts[-1]), nq, hd)).astype(np.float16))
+    keep, rows = [300, 10, 900], [a + b for a, b in zip(lens, new)]
+    out = []
+    for at in (0, far):
+        big = []
+        for x in (pools[0][0], pools[1][0], pools[0][1], pools[1][1], w):
+            y = torch.zeros((at + n, *x.shape[1:]), dtype=torch.float32 if x.dtype == np.float32 else torch.uint8, device=DEV)
+            y[at:].copy_(_t(x))
+            big.append(y)
+        kp, vp, ke, ve, wt = big
+        t = _t(np.where(tables >= 0, tables + at, -1).astype(np.int32))
+        ws = kvcache.weigh_f8_paged_workspace(nq, kv, 3, q.shape[0], max(new), 1700, DEV, head_dim=hd)
+        kvcache.weigh_f8_paged(q, kp, ke, wt, ws, t, _t(starts), _t(positions), max_tok=max(new), max_ctx=1700, scale=hd ** -0.5)
+        weighed = wt[at:].clone()
+        kept = torch.zeros(3, kv, 900, dtype=torch.int32, device=DEV)
+        ews = kvcache.evict_f8_paged_workspace(3, kv, bt, 1700, 900, DEV)
+        kvcache.evict_f8_paged(kp, vp, ke, ve, wt, t, i32(rows), i32(keep), kept, ews, max_ctx=1700, sink=2, recent=9)
+        if at:
+            assert not any(x[:n].any() for x in big)
+        out.append([weighed, kept] + [x[at:] for x in big])
+    for a, b in zip(*out):
+        assert torch.equal(a, b)
+    assert (out[0][1] >= 0).any()
+
+
+def test_two_streams_at_once():
+    """Weighing and eviction of two caches on two streams, with a workspace each: as one after the other."""
+    rng = np.random.default_rng(29)
+    bt, kv, hd, nq, lens = 16, 8, 128, 16, [3000, 17, 1200, 2500]
+    tables, starts, positions, n = R.layout(rng, lens, [1] * 4, bt, kv, hd)
+    rows, keep = [a + 1 for a in lens], [1000, 17, 1100, 2000]
+    pools = [R.random_pool(rng, n, bt, kv, hd) for _ in range(2)]
+    w = rng.random((n, kv, bt)).astype(np.float32)
+    q = [_t(rng.standard_normal((4, nq, hd)).astype(np.float16)) for _ in range(2)]
+    t, st, pos, r, k = _t(tables), _t(starts), _t(positions), i32(rows), i32(keep)
+
+    def state():
+        return [_t(x) for x in (pools[0][0], pools[1][0], pools[0][1], pools[1][1], w)] + \
+               [torch.zeros(4, kv, 2000, dtype=torch.int32, device=DEV), kvcache.weigh_f8_paged_workspace(nq, kv, 4, 4, 1, 3100, DEV, head_dim=hd),
+                kvcache.evict_f8_paged_workspace(4, kv, bt, 3100, 2000, DEV)]
+
+    def run(s, q, stream):
+        kvcache.weigh_f8_paged(q, s[0], s[2], s[4], s[6], t, st, pos, max_tok=1, max_ctx=3100, scale=0.1, stream=stream)
+        kvcache.evict_f8_paged(*s[:5], t, r, k, s[5], s[7], max_ctx=3100, sink=4, recent=30, stream=stream)
+
+    want = [state(), state()]
+    for s, x in zip(want, q):
+        run(s, x, None)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(5):
+        got = [state(), state()]
+        torch.cuda.synchronize()
+        for s, x, stream in zip(got, q, streams):
+            run(s, x, stream)
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert all(torch.equal(x, y) for x, y in zip(a[:6], b[:6]))
