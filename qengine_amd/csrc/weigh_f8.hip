@@ -8,9 +8,9 @@
 // keys that it sees.  A row's m and l must be known before any sum over rows, so there are two passes over the scores.
 //
 // Few rows: keys are read once, the first pass stores the scores (4 bytes a row and key, beside head_dim bytes of
-// codes), the second reads those.  Bound by HBM: 32 single tokens over 333 MB of codes take 87 + 11 us, 4.4 TB/s (without
-// the scores' stores 77; two tiles of a wave under way, the keys of all slots as one line of equal parts, stores past
-// the caches: 88 to 93).
+// codes), the second reads those.  Bound by HBM: 32 single tokens over 333 MB of codes take 77 + 10 us, 5.0 TB/s (without
+// the scores' 23 MB of stores 60; past the caches 79).  Two tiles of a wave under way, or the keys of all slots as one line
+// of equal parts, were slower by 4 to 7.
 // Many rows: both passes form the scores by the matrix cores, 2 head_dim operations a row and key each; the first
 // holds rows in registers and passes keys by (a lane's scores are one row's, so maximum and sum stay in it), the
 // second holds keys and passes rows by (a lane's are one key's).  Bound by the vector unit and the matrix cores together:
@@ -140,18 +140,26 @@ __device__ __forceinline__ long place_of(const WeighArgs& p, const Slot& x, int 
   return ((long)(s - p.slot0) * p.local_tok + tok) * p.num_q + h * p.gqa + (row - tok * p.gqa);
 }
 
+// Where the workspace holds the scores of a (slot, KV head): 32 keys of all its rows, then the next 32.
+__device__ __forceinline__ long scores_of(const WeighArgs& p, int s, int h) {
+  return ((long)(s - p.slot0) * p.num_kv + h) * (p.local_tok * p.gqa) * p.score_pitch;
+}
+
 }  // namespace
 
 // ---------------------------------------------------------------------------
 // few rows: up to 16 RT (token, head) rows of a slot and KV head
 // ---------------------------------------------------------------------------
-// A workgroup takes chunk_keys keys of a (slot, KV head), its four waves every fourth tile of 32: K rows are the A
-// operand as loaded (lane l % 16 the key, group l / 16 the same dims of K and Q), so lane l has the scores of
-// row l % 16 and keys 4 (l / 16) ..  Nothing is shared until the waves' statistics are joined at the end.
+// A workgroup takes chunk_keys keys of a (slot, KV head), its four waves every fourth tile of 32.  A tile's rows are
+// loaded whole lines at a time, past the caches (each byte is used once; as the operand asks for them, 64 bytes of 16
+// rows at a time, 87 us, now 77), and pass through LDS of the wave's own, their 16-byte words permuted by the row's
+// number.  K rows are the A operand (lane l % 16 the key, group l / 16 the same dims of K and Q), so lane l has the
+// scores of row l % 16 and keys 4 (l / 16) ..  Nothing is shared until the waves' statistics are joined at the end.
 template <int HD, int RT>
 __global__ __launch_bounds__(256, 2) void weigh_scores_kernel(WeighArgs p) {
-  constexpr int KT = 32, W = 4, KW = HD / 64;
+  constexpr int KT = 32, W = 4, KW = HD / 64, LPR = HD / 16, RL = 64 / LPR;
   __shared__ float ml[W][16 * RT][2];
+  __shared__ __align__(16) uint8_t tile_s[W][KT * HD];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int m = lane & 15, g = lane >> 4;
   Work wk;
@@ -164,20 +172,30 @@ __global__ __launch_bounds__(256, 2) void weigh_scores_kernel(WeighArgs p) {
   const const_i32* table = (const const_i32*)(p.tables + (long)s * p.max_blocks);
   const uint32_t key_bytes = (uint32_t)p.num_kv * HD;
 
-  u4_t kr[2][KW];
-  uint32_t ke[2];
+  u4_t kr[2][KW];   // RL rows each, a row's words by LPR lanes
+  uint8_t ke[2];   // (widened where it is used: a wait)
   int pg[2];
+  uint8_t* tile = tile_s[wave];
+  auto word_at = [&](int row, int word) {   // (no two of 16 rows' same words on one bank)
+    return reinterpret_cast<u4_t*>(tile + row * HD + (word ^ ((HD == 256 ? row : row >> 1) & (LPR - 1))) * 16);
+  };
   auto load = [&](int key0) {
 #pragma unroll
     for (int hf = 0; hf < 2; hf++) {
       const BlockAt x = block_at(p, key0 + 16 * hf);
       pg[hf] = key0 + 16 * hf < end ? page_of(p, table, x.b) : -1;
       const long page = max(pg[hf], 0);
-      const uint8_t* src = p.k_pool + (page * p.block_tokens + x.row + m) * key_bytes + h * HD + 16 * g;
+      const uint8_t* src = p.k_pool + (page * p.block_tokens + x.row + lane / LPR) * key_bytes + h * HD + 16 * (lane % LPR);
       ke[hf] = p.k_exp[page * p.num_kv + h];
 #pragma unroll
-      for (int i = 0; i < KW; i++) kr[hf][i] = *reinterpret_cast<const u4_t*>(src + 64 * i);
+      for (int i = 0; i < KW; i++) kr[hf][i] = __builtin_nontemporal_load(reinterpret_cast<const u4_t*>(src + i * RL * key_bytes));
     }
+  };
+  // (a wave's accesses to LDS are in order, also of different lanes: so the compiler has to leave them)
+  auto in_order = [&]() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
   };
   auto next = [&](int k) {   // the wave's next tile from k on that some row sees
     while (k < end && out_of_window(p, sl, k)) k += KT * W;
@@ -199,31 +217,46 @@ __global__ __launch_bounds__(256, 2) void weigh_scores_kernel(WeighArgs p) {
 #pragma unroll
       for (int x = 0; x < 2; x++) qf[t][i][x] = *reinterpret_cast<const h8_t*>(src + 64 * i + 8 * x);
     pos[t] = sl.pos0 + token_of(p, row);
-    out[t] = p.scores + place_of(p, sl, s, h, row) * p.score_pitch + 4 * g;
+    out[t] = p.scores + scores_of(p, s, h) + 32 * row + 4 * g;
     st[t] = {-INFINITY, 0.f};
   }
+  // (the queries are here: in the loop the wait for them would be one for the next tile's loads)
+#pragma unroll
+  for (int t = 0; t < RT; t++)
+#pragma unroll
+    for (int i = 0; i < KW; i++)
+#pragma unroll
+      for (int x = 0; x < 2; x++) asm volatile("" : "+v"(qf[t][i][x]));
   const int pos_hi = sl.pos0 + sl.n - 1;
   while (key0 < end) {
     const int key1 = next(key0 + KT * W);
+    const float pow[2] = {pow2f(ke[0]), pow2f(ke[1])};
+    in_order();
+#pragma unroll
+    for (int hf = 0; hf < 2; hf++)
+#pragma unroll
+      for (int i = 0; i < KW; i++) *word_at(16 * hf + i * RL + lane / LPR, lane % LPR) = kr[hf][i];
+    const bool whole = pg[0] >= 0 && pg[1] >= 0 && key0 + KT - 1 <= sl.pos0 && key0 + KT <= end &&
+                       (p.window <= 0 || key0 > pos_hi - p.window || key0 + KT <= p.sink);
+    const int here[2] = {pg[0], pg[1]};
+    if (key1 < end) load(key1);
+    in_order();
     f4_t sc[RT][2];
 #pragma unroll
     for (int t = 0; t < RT; t++) sc[t][0] = sc[t][1] = f4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int hf = 0; hf < 2; hf++) {
-      const float f = pow2f(ke[hf]);
 #pragma unroll
-      for (int i = 0; i < KW; i++)
+      for (int i = 0; i < KW; i++) {
+        const u4_t w = *word_at(16 * hf + m, 4 * i + g);
 #pragma unroll
         for (int x = 0; x < 2; x++) {
-          const h8_t a = cvt8(kr[hf][i][2 * x], kr[hf][i][2 * x + 1], f);
+          const h8_t a = cvt8(w[2 * x], w[2 * x + 1], pow[hf]);
 #pragma unroll
           for (int t = 0; t < RT; t++) sc[t][hf] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qf[t][i][x], sc[t][hf], 0, 0, 0);
         }
+      }
     }
-    const bool whole = pg[0] >= 0 && pg[1] >= 0 && key0 + KT - 1 <= sl.pos0 && key0 + KT <= end &&
-                       (p.window <= 0 || key0 > pos_hi - p.window || key0 + KT <= p.sink);
-    const int here[2] = {pg[0], pg[1]};
-    if (key1 < end) load(key1);
 #pragma unroll
     for (int t = 0; t < RT; t++) {
       float top = -INFINITY;
@@ -240,8 +273,8 @@ __global__ __launch_bounds__(256, 2) void weigh_scores_kernel(WeighArgs p) {
       for (int x = 0; x < 8; x++) l += __builtin_amdgcn_exp2f(sc[t][x >> 2][x & 3] - ref);
       st[t] = {mn, l};
       if (16 * t + m < rows) {
-        *reinterpret_cast<f4_t*>(out[t] + key0) = sc[t][0];
-        if (key0 + 16 < end) *reinterpret_cast<f4_t*>(out[t] + key0 + 16) = sc[t][1];
+        *reinterpret_cast<f4_t*>(out[t] + (long)key0 * rows) = sc[t][0];
+        if (key0 + 16 < end) *reinterpret_cast<f4_t*>(out[t] + (long)key0 * rows + 16) = sc[t][1];
       }
     }
     key0 = key1;
@@ -306,7 +339,6 @@ template <bool MERGED>
 __global__ __launch_bounds__(256) void weigh_few_kernel(WeighArgs p) {
   constexpr int ROWS = 64;
   __shared__ f2_t stat[ROWS];
-  __shared__ long at[ROWS];
   Work wk;
   if (!work_of(p, wk)) return;
   const int tid = threadIdx.x, h = wk.h, s = wk.s;
@@ -324,16 +356,16 @@ __global__ __launch_bounds__(256) void weigh_few_kernel(WeighArgs p) {
   const int weighed = p.weighed ? p.weighed[s] : sl.pos0;
   float* w = p.weights + ((long)max(pg, 0) * p.num_kv + h) * p.block_tokens + bl.row;
   const bool out = out_of_window(p, sl, key & ~31);   // (its scores were not stored)
+  const float* score = p.scores + scores_of(p, s, h) + (long)(key_l & ~31) * rows + (key_l & 31);
   f4_t old, ahead[AHEAD];
 #pragma unroll
   for (int i = 0; i < 4; i++) old[i] = w[i];
 #pragma unroll
   for (int r = 0; r < AHEAD; r++)
-    ahead[r] = *reinterpret_cast<const f4_t*>(p.scores + place_of(p, sl, s, h, min(r, rows - 1)) * p.score_pitch + key_l);
+    ahead[r] = *reinterpret_cast<const f4_t*>(score + 32 * min(r, rows - 1));
   if constexpr (MERGED) {
     if (tid < rows) {
       const long x = place_of(p, sl, s, h, tid);
-      at[tid] = x * p.score_pitch;
       stat[tid] = f2_t{p.stat_m[x], p.stat_il[x]};
     }
   } else {
@@ -341,7 +373,6 @@ __global__ __launch_bounds__(256) void weigh_few_kernel(WeighArgs p) {
       const long x = place_of(p, sl, s, h, r);
       const Stat st = join_chunks(p, sl, x, tid & 15);
       if ((tid & 15) == 0) {
-        at[r] = x * p.score_pitch;
         stat[r] = st.l == 0.f ? f2_t{INFINITY, 0.f} : f2_t{st.m, 1.f / st.l};
       }
     }
@@ -357,7 +388,7 @@ __global__ __launch_bounds__(256) void weigh_few_kernel(WeighArgs p) {
 #pragma unroll
     for (int r = 0; r < AHEAD; r++)
       if (r < rows) add(ahead[r], r);
-    for (int r = AHEAD; r < rows; r++) add(*reinterpret_cast<const f4_t*>(p.scores + at[r] + key), r);
+    for (int r = AHEAD; r < rows; r++) add(*reinterpret_cast<const f4_t*>(score + 32 * r), r);
   }
 #pragma unroll
   for (int i = 0; i < 4; i++)
