@@ -106,8 +106,9 @@ def test_weighing_refusals(L, p):
     assert w(8, 3, 128, 2, 4, 2, 100) == w(8, 2, 64, 2, 4, 2, 100) == w(8, 2, 128, 0, 4, 2, 100) == 0
     assert w(8, 2, 128, 2, 4, 100, 100) == w(8, 2, 128, 2, 4, 4, 100)   # no slot has more rows than the call
     # the stated limit suffices, and far past it nothing is taken
-    for slots, kv, tok, ctx in ((1, 4, 1 << 20, 1 << 15), (64, 8, 4096, 1 << 16), (1 << 12, 8, 1, 1 << 20), (1, 8, 1, 1 << 30)):
-        assert slots * kv * (tok * 4 / 256 + 1) * (ctx / 128 + 1) < 2.0 ** 31
+    for slots, kv, tok, ctx in ((1, 4, 1 << 20, 1 << 15), (64, 8, 4096, 1 << 16), (1 << 12, 8, 1, 1 << 20), (1, 8, 1, 1 << 30),
+                                (40, 1, 1, 1 << 30), (1, 1, 1 << 20, 2000000), (10600, 8, 1, 1 << 20), (1, 8, 4096, 130000000)):
+        assert slots * max(kv, 2) * (tok * 4 / 32 + 6) * (ctx / 256 + 6) < 2.0 ** 31
         assert w(4 * kv, kv, 256, slots, slots * tok if slots * tok < 2**31 else 2**31 - 1, tok, ctx) > 0
     assert w(32, 8, 256, 1 << 16, 1 << 16, 1, 1 << 30) == w(32, 8, 256, 1, 1 << 24, 1 << 24, 1 << 26) == 0
 
