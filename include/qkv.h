@@ -762,9 +762,9 @@ typedef enum qkv_logits_type { QKV_LOGITS_F16 = 0, QKV_LOGITS_F32 = 1, QKV_LOGIT
 
 /* The `take` best continuations of each of n requests over its `beams` beams and the vocabulary:
  *   S(b, v) = scores[b] + logits[b][v] - log(sum_u exp(logits[b][u])),
- * largest first, ties to the lowest beam, then token.  logits: [n * beams][vocab] with `stride` elements between
- * rows, of any alignment (read by whole 16-byte words: up to 15 bytes before and past a row must be there to
- * read, as any allocation's are).  A logit of NaN or +infinity counts as -infinity, which is no candidate.
+ * largest first, ties to the lowest beam, then token (rows of equal logits have equal sums, wherever they lie).
+ * logits: [n * beams][vocab] with `stride` elements between rows, of any alignment; nothing outside the rows is
+ * read.  A logit of NaN or +infinity counts as -infinity, which is no candidate.
  * scores: device fp32 [n * beams]; a beam of -infinity or NaN offers nothing (before the first step all beams of
  * a request but one).  done (device int32 [n * beams], NULL: none): a beam with a nonzero entry has ended, its
  * logits are not read, and it offers end_token at its own score.  parents, tokens, top_scores [n][take]: the

@@ -204,6 +204,10 @@ __device__ __forceinline__ float maximum(float a, float b, float c) {
 }
 __device__ __forceinline__ float maximum(float a, float b) { return maximum(a, b, b); }
 
+// A word at the address of a logit of 2 or 4 bytes
+typedef u4_t __attribute__((aligned(2))) word2_t;
+typedef u4_t __attribute__((aligned(4))) word4_t;
+
 // Logits of one 16-byte word
 template <int TYPE>
 struct Word;
@@ -266,8 +270,9 @@ __device__ __forceinline__ bool searched(const BeamArgs& p, long row) {   // a b
 
 }  // namespace
 
-// A workgroup takes NV words a thread of a row.  Rows need not be aligned: words are, and what they hold
-// outside the row is left out.
+// A workgroup takes NV words a thread of a row.  Words are counted from the row's first logit, whatever its address, so
+// that equal rows are cut and summed in the same order and beams of equal scores tie; the last word of a row is read by
+// the logit, none past its end.
 template <int TYPE, int NV>
 __global__ __launch_bounds__(256, 4) void beam_rows_kernel(BeamArgs p) {
   using W = Word<TYPE>;
@@ -281,36 +286,33 @@ __global__ __launch_bounds__(256, 4) void beam_rows_kernel(BeamArgs p) {
   const long row = wg / p.segments;
   const int seg = (int)(wg - row * p.segments), tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   if (!searched(p, row)) return;
-  const uintptr_t addr = reinterpret_cast<uintptr_t>(p.logits) + (uintptr_t)(row * p.stride) * SIZE;
-  const u4_t* words = reinterpret_cast<const u4_t*>(addr & ~(uintptr_t)15);
-  const int skip = (int)(addr & 15) / SIZE;   // elements of the first word ahead of the row
-  const long w0 = (long)seg * (256 * NV), end = (long)p.vocab + skip;
-  u4_t raw[NV];
+  typedef typename std::conditional<SIZE == 2, uint16_t, uint32_t>::type Logit;
+  typedef typename std::conditional<SIZE == 2, word2_t, word4_t>::type Loaded;
+  const Logit* logits = reinterpret_cast<const Logit*>(p.logits) + row * p.stride;
+  const int w0 = seg * (256 * NV), whole = p.vocab / W::N, rest = p.vocab % W::N;
+  u4_t raw[NV], none;
+#pragma unroll
+  for (int i = 0; i < 4; i++) none[i] = SIZE == 2 ? W::kNone * 0x10001u : W::kNone;
 #pragma unroll
   for (int j = 0; j < NV; j++) {
-    const long e = (w0 + 256 * j + tid) * W::N;
-    if (e < end) {
-      raw[j] = __builtin_nontemporal_load(words + w0 + 256 * j + tid);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; i++) raw[j][i] = SIZE == 2 ? W::kNone * 0x10001u : W::kNone;
-    }
+    const int w = w0 + 256 * j + tid;
+    raw[j] = none;
+    if (w < whole) raw[j] = __builtin_nontemporal_load(reinterpret_cast<const Loaded*>(logits + (long)w * W::N));
   }
+  if (rest != 0 && whole - w0 < 256 * NV) {   // (the same in every thread; whole >= w0)
+    uint32_t v[W::N - 1];
 #pragma unroll
-  for (int j = 0; j < NV; j++) {
-    const long e = (w0 + 256 * j + tid) * W::N;
-    if (e < skip || (e < end && e + W::N > end)) {
+    for (int i = 0; i < W::N - 1; i++) v[i] = logits[(long)whole * W::N + min(i, rest - 1)];
+    u4_t last = none;
 #pragma unroll
-      for (int i = 0; i < W::N; i++)
-        if (e + i < skip || e + i >= end) {
-          if constexpr (SIZE == 2) {
-            const uint32_t keep = i & 1 ? 0xffffu : 0xffff0000u;
-            raw[j][i >> 1] = (raw[j][i >> 1] & keep) | (i & 1 ? W::kNone << 16 : W::kNone);
-          } else {
-            raw[j][i] = W::kNone;
-          }
-        }
+    for (int i = 0; i < W::N - 1; i++) {
+      if (i >= rest) continue;
+      if constexpr (SIZE == 2) last[i >> 1] = i & 1 ? (last[i >> 1] & 0xffffu) | v[i] << 16 : (last[i >> 1] & 0xffff0000u) | v[i];
+      else last[i] = v[i];
     }
+#pragma unroll
+    for (int j = 0; j < NV; j++)
+      if (w0 + 256 * j + tid == whole) raw[j] = last;
   }
   // Logits that are left out show in the maximum (+infinity or NaN): only then are all looked at.
   float tops[NV], top;
@@ -347,7 +349,7 @@ __global__ __launch_bounds__(256, 4) void beam_rows_kernel(BeamArgs p) {
   const float l = wave_sum((sum[0] + sum[1]) + (sum[2] + sum[3]));
   if (lane == 0) sums[wave] = l;
   const long rec = wg * p.take;
-  const int token0 = (int)(w0 * W::N - skip);
+  const int token0 = w0 * W::N;
   auto each = [&](auto&& f, float low) __attribute__((always_inline)) {
 #pragma unroll
     for (int j = 0; j < NV; j++)
@@ -501,13 +503,12 @@ __global__ __launch_bounds__(256) void beam_join_kernel(BeamArgs p) {
 
 // 16-byte words of a thread: few where few rows leave workgroups idle, unless a request's records then
 // outgrow what its join holds at a time.
-BeamPlan beam_plan(long rows, int beams, int vocab, int take, int type, bool whole) {
+BeamPlan beam_plan(long rows, int beams, int vocab, int take, int type) {
   const int n = type == 1 ? 4 : 8;
   BeamPlan x{8, 0};
   for (int nv : {1, 4, 8}) {
     x.words = nv;
-    // (a row that does not begin with a word holds up to n - 1 elements of another)
-    x.segments = (int)(((long)vocab + (whole ? 0 : n - 1) + 256L * nv * n - 1) / (256L * nv * n));
+    x.segments = (int)((vocab + 256L * nv * n - 1) / (256L * nv * n));
     if (rows * x.segments <= kBeamGroups && (long)beams * x.segments * take <= kBeamRecords) break;
   }
   return x;

@@ -367,8 +367,7 @@ int qkv_beam_select(const void* logits, int logits_type, long stride, const floa
   a.vocab = vocab;
   a.take = take;
   a.end_token = end_token;
-  const bool whole = aligned(logits, 16) && (a.rows == 1 || stride * (logits_type == QKV_LOGITS_F32 ? 4 : 2) % 16 == 0);
-  const qkv::BeamPlan plan = qkv::beam_plan(a.rows, beams, vocab, take, logits_type, whole);
+  const qkv::BeamPlan plan = qkv::beam_plan(a.rows, beams, vocab, take, logits_type);
   const size_t segments = (size_t)a.rows * plan.segments;
   a.rec_sum = static_cast<float*>(workspace);
   a.rec_x = a.rec_sum + 2 * segments;

@@ -333,8 +333,8 @@ struct BeamPlan {
   int words;                 // 16-byte words a thread holds
   int segments;              // workgroups of a row
 };
-// type 0: fp16, 1: fp32, 2: bf16; whole: every row begins with a 16-byte word
-BeamPlan beam_plan(long rows, int beams, int vocab, int take, int type, bool whole);
+// type 0: fp16, 1: fp32, 2: bf16
+BeamPlan beam_plan(long rows, int beams, int vocab, int take, int type);
 hipError_t launch_beam(BeamArgs a, const BeamPlan& plan, int type, hipStream_t stream);
 
 // Pages of a cache (kv_pages.hip): tables [n_slots][max_blocks] with a negative

@@ -127,6 +127,29 @@ def test_rows_apart_and_unaligned():
             _check(buf[:, off:off + 1000 + off], s, 9)
 
 
+@pytest.mark.parametrize("dtype,vocab", [("f16", 50257), ("bf16", 50257), ("f32", 32003), ("f16", 1001), ("bf16", 999), ("f32", 133),
+                                         ("f16", 200003), ("f32", 70001), ("f16", 5), ("f32", 3)])
+def test_equal_beams_tie_at_every_alignment(dtype, vocab):
+    """Rows of equal logits and scores that begin at other offsets of a 16-byte word: each token from the lowest beam on, and
+    the same bits from any address."""
+    beams, take = 5, 12
+    row = _inputs(1, 1, vocab, dtype, vocab)[0][0]
+    x, s = row.repeat(2 * beams, 1), torch.full((2, beams), -3.25, device=DEV)
+    p, t, top = (o.cpu().numpy() for o in _select(x, s, take))
+    r = row.float().cpu().numpy()
+    want = np.lexsort((np.arange(beams * vocab), -np.tile(r, beams)))[:take]
+    k = min(take, beams * int((r > -np.inf).sum()))
+    for i in range(2):
+        assert np.array_equal(t[i, :k], want[:k] % vocab) and np.array_equal(p[i, :k], i * beams + want[:k] // vocab)
+    buf = torch.zeros(vocab + 16, dtype=row.dtype, device=DEV)
+    first = None
+    for off in range(9):
+        buf[off:off + vocab] = row
+        got = _select(buf[off:off + vocab].view(1, vocab), s[:1, :1].contiguous(), take)
+        first = got if first is None else first
+        assert all(torch.equal(a, b) for a, b in zip(got, first))
+
+
 def test_a_workspace_of_larger_numbers_and_a_stream_and_a_graph():
     ws = kvcache.beam_select_workspace(64, 8, 60000, 32, DEV)
     cases = [(_inputs(3, 4, 5000, "f16", i), 8) for i in range(3)] + [(_inputs(1, 8, 60000, "f32", 5), 16)]
