@@ -409,7 +409,8 @@ __global__ __launch_bounds__(256) void beam_join_kernel(BeamArgs p) {
   __shared__ int best_at[kMaxTake];
   __shared__ float score[kMaxBeams];
   __shared__ int state[kMaxBeams];   // 0: not alive, 1: searched, 2: done
-  const long req = blockIdx.x, row0 = req * p.beams;
+  const long req = (long)blockIdx.y * kGridX + blockIdx.x, row0 = req * p.beams;
+  if (row0 >= p.rows) return;
   const int tid = threadIdx.x, S = p.segments, k = p.take;
   const int per = S * k, total = p.beams * per;
   const float* rec_x = p.rec_x + row0 * per;
@@ -516,7 +517,7 @@ BeamPlan beam_plan(long rows, int beams, int vocab, int take, int type) {
 
 hipError_t launch_beam(BeamArgs a, const BeamPlan& plan, int type, hipStream_t stream) {
   a.segments = plan.segments;
-  const dim3 grid = grid_xy((long)a.rows * a.segments), block(256), requests((unsigned)(a.rows / a.beams));
+  const dim3 grid = grid_xy((long)a.rows * a.segments), block(256), requests = grid_xy(a.rows / a.beams);
   auto launch = [&](auto t) {
     constexpr int T = decltype(t)::value;
     switch (plan.words) {

@@ -268,6 +268,23 @@ def test_numbers_that_are_none_of_every_kind(dtype):
             _check(x.to(DEV), scores.to(DEV), k)
 
 
+def test_the_most_rows_of_a_call():
+    """2^24 requests of a beam, three tokens each, checked on the device.  A score is off by
+    its sum's rounding (L.beam_scores: at most 3 / e * 5 + 42 of 2^-24) and its own."""
+    n = 1 << 24
+    g = torch.Generator(device=DEV).manual_seed(24)
+    x = torch.randn(n, 3, device=DEV, generator=g).half()
+    s = -torch.rand(n, 1, device=DEV, generator=g)
+    p, t, top = _select(x, s, 2)
+    assert torch.equal(p, torch.arange(n, dtype=torch.int32, device=DEV)[:, None].expand(n, 2))
+    for i in range(0, n, n // 8):
+        a = slice(i, i + n // 8)
+        value, token = x[a].float().sort(stable=True, dim=-1, descending=True)
+        ref = (value[:, :2].double() - x[a].double().logsumexp(-1, keepdim=True)) + s[a].double()
+        assert torch.equal(t[a], token[:, :2].int())
+        assert ((top[a].double() - ref).abs() <= (3 / np.e * 5 + 42 + ref.abs()) * 2.0 ** -24).all()
+
+
 def test_rows_and_states_past_four_billion_bytes():
     g = torch.Generator(device=DEV).manual_seed(3)
     wide = torch.zeros(4, 1 << 30, dtype=torch.float16, device=DEV)
