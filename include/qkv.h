@@ -549,7 +549,8 @@ int qkv_rope(const uint16_t* q, long q_stride, uint16_t* q_out, long q_out_strid
  * 1 + w passes 1 + w).  rot_dim 0: no rotation (positions and turns are not read, amplitude does not
  * count).  Rows, strides, positions and places as for qkv_rope.  eps > 0; head_dim <= 1024
  * (QKV_ERR_UNSUPPORTED); any head_dim, alignment to 2 bytes; fast with head_dim 64, 128, 256, 512 or 1024,
- * rot_dim a multiple of 16, rows and weights aligned to 16 bytes. */
+ * rot_dim a multiple of 16, rows and weights aligned to 16 bytes; others at most 2^34 rows (tokens times heads,
+ * QKV_ERR_UNSUPPORTED). */
 int qkv_norm_rope(const uint16_t* q, long q_stride, uint16_t* q_out, long q_out_stride, const float* q_weight,
                   const uint16_t* k, long k_stride, uint16_t* k_out, long k_out_stride, const float* k_weight,
                   float eps, const int32_t* positions, const uint64_t* turns, float amplitude, int n_tok, int num_q,

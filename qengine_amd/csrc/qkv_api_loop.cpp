@@ -81,6 +81,7 @@ int qkv_norm_rope(const uint16_t* q, long q_stride, uint16_t* q_out, long q_out_
   bool wide = norm_wide(head_dim, rot_dim);
   if (num_q) wide = wide && wide_rows(q, q_stride) && wide_rows(q_out, q_out_stride) && aligned(q_weight, 16);
   if (num_k) wide = wide && wide_rows(k, k_stride) && wide_rows(k_out, k_out_stride) && aligned(k_weight, 16);
+  if (!wide && (double)n_tok * (num_q + num_k) > qkv::kNormRows) return QKV_ERR_UNSUPPORTED;
   return launch_status(qkv::launch_norm_rope(a, wide, stream));
 }
 

@@ -149,6 +149,7 @@ hipError_t launch_rope(RopeArgs a, bool wide, bool in_place, hipStream_t stream)
 // Norms of heads with the rotation, and the gradient (norm_rope.hip).  dq, dk and their strides, the
 // sums of the weights' gradients (q_dw, k_dw) and the partial sums are the gradient's alone.
 constexpr int kNormMaxHead = 1024;
+constexpr double kNormRows = 17179869184.0;   // of a call by a wave a row, four a workgroup, whose number is one of 32 bits
 constexpr int kNormGradGroups = 768;   // workgroups of a gradient: the 3 that fit each CU
 struct NormRopeArgs {
   const uint16_t* q;
