@@ -240,3 +240,35 @@ def test_scores_that_rise_and_fall(hd, new, step):
     b["ke"][:] = 127
     b["q"][:] = 1 + rng.integers(-3, 4, b["q"].shape) / 64
     _check(b, scale=abs(step) / hd)
+
+
+@pytest.mark.parametrize("hd", [128, 256])
+@pytest.mark.parametrize("few", [True, False])
+def test_many_rows_of_many_slots(hd, few):
+    """More slots than a workgroup walks at a time, with runs of more than 64 that have no rows, beside single tokens (taken
+    by the kernels for few rows) or where the call's rows say that all slots are alike."""
+    rng = np.random.default_rng(hd + few)
+    n, tok = 620, 40 if few else 20
+    new = [0] * n
+    for s in (0, 1, 75, 76, 160, 255, 256, 257, 400, 511, 512, 619):
+        new[s] = int(rng.integers(17, tok + 1))
+    if few:
+        new[3] = new[80] = new[300] = new[618] = 1
+    lens = [int(x) for x in rng.integers(0, 300, n)]
+    b = _batch(rng, lens, new, 16, 2, hd, 8)
+    if not few:   # rows behind the last slot's
+        b["q"] = np.concatenate([b["q"], rng.standard_normal((n * tok // 2, 8, hd)).astype(np.float16)])
+    _check(b, max_tok=tok, decay=0.5)
+    _check(b, max_tok=tok, window=70, sink=20)
+
+
+@pytest.mark.parametrize("hd", [128, 256])
+def test_more_tiles_than_a_workgroup_walks_at_a_time(hd):
+    """More than 256 tiles of 256 keys of one slot, of several, and more than 256 tiles of rows."""
+    rng = np.random.default_rng(hd)
+    _check(_batch(rng, [65700], [70], 64, 1, hd, 4), decay=0.5)
+    _check(_batch(rng, [40000, 0, 30000, 5], [40, 0, 70, 90], 64, 1, hd, 4), decay=0.0)
+    _check(_batch(rng, [66000, 100], [33, 40], 64, 1, hd, 4), window=3000, sink=70)
+    b = _batch(rng, [10, 7], [8300, 9], 64, 1, hd, 8)
+    _check(b, max_ctx=300)
+    _check(b, max_ctx=300, window=150, sink=33)
