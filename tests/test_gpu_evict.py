@@ -197,3 +197,12 @@ def test_many_slots_of_many_heads():
     lens = [int(x) for x in rng.integers(0, 900, 64)]
     keep = [int(x) for x in rng.integers(0, 900, 64)]
     _check(*_cache(rng, lens, 32, 16, 256), lens, keep, 900, 900, 4, 30)
+
+
+@pytest.mark.parametrize("hd,bt", [(128, 4096), (256, 8192), (128, 2064)])
+def test_pages_of_thousands_of_rows(hd, bt):
+    """Many chunks of rows a page, each of which needs the exponents of all of the page's rows; slots of one page too."""
+    rng = np.random.default_rng(bt)
+    lens = [20000, 9000, 300, bt]
+    _check(*_cache(rng, lens, bt, 1, hd), lens, [12000, 8999, 299, bt - 1], 20000, 12000, 4, 50)
+    _check(*_cache(rng, lens, bt, 1, hd, ties=True), lens, [bt, 100, 300, 1], 20000, 12000)
