@@ -648,7 +648,8 @@ int qkv_attn_f8_paged(const uint16_t* q, const uint8_t* k_pool, const uint8_t* v
  * the slot's first keys have a weight that stands; others hold anything before.  decay finite; with 0 nothing that
  * stood is read.  Slots without rows, keys past the last and keys without a page are left alone, and of two slots
  * that share a page only one may be named with rows in a call (the other's weights would take its place).  A row
- * that sees no key adds nothing; one whose query is not finite makes weights that are not.  Limits as for
+ * that sees no key adds nothing, nor does one whose products are all -infinity; another whose query is not finite makes
+ * weights that are not.  Limits as for
  * qkv_attn_f8_paged, and n_slots * max(num_kv, 2) * (max_tok * num_q / num_kv / 32 + 6) * (max_ctx / 256 + 6) < 2^31 suffices
  * (QKV_ERR_UNSUPPORTED past what the launches count, and 0 from the workspace query).  workspace:
  * qkv_weigh_f8_paged_workspace_bytes of these numbers or larger ones (n_slots, n_rows, max_tok, max_ctx), 256-byte

@@ -272,3 +272,17 @@ def test_more_tiles_than_a_workgroup_walks_at_a_time(hd):
     b = _batch(rng, [10, 7], [8300, 9], 64, 1, hd, 8)
     _check(b, max_ctx=300)
     _check(b, max_ctx=300, window=150, sink=33)
+
+
+def test_a_query_of_minus_infinity():
+    """Products that are all -infinity are those of keys that are not seen: the row adds nothing."""
+    rng = np.random.default_rng(15)
+    for new in (1, 90):
+        b = _batch(rng, [50], [new], 16, 1, 128, 1)
+        b["kp"][:] = np.abs(rng.integers(1, 120, b["kp"].shape)).astype(np.uint8)   # (positive codes)
+        b["ke"][:] = 127
+        b["q"][:, :, 7] = -np.inf
+        got = _run(b, new, 200, 0.1)
+        page, at = b["tables"][0][np.arange(50 + new) // 16], np.arange(50 + new) % 16
+        want = np.where(np.arange(50 + new) < 50, b["w"][page, 0, at], 0)
+        assert np.array_equal(got[page, 0, at].astype(np.float32), want)
