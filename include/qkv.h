@@ -774,9 +774,10 @@ typedef enum qkv_logits_type { QKV_LOGITS_F16 = 0, QKV_LOGITS_F32 = 1, QKV_LOGIT
  * a request but one).  done (device int32 [n * beams], NULL: none): a beam with a nonzero entry has ended, its
  * logits are not read, and it offers end_token at its own score.  parents, tokens, top_scores [n][take]: the
  * logits row of the beam (request * beams + b), the token and S as fp32; -1, -1 and -infinity where there are
- * fewer candidates.  S is compared in 64 bits.  beams, take <= 64, beams * vocab < 2^31, n * beams <= 2^24
- * (QKV_ERR_UNSUPPORTED).  workspace: qkv_beam_select_workspace_bytes of these numbers or larger ones, aligned to 8
- * bytes (no initialisation needed).  Calls sharing one must be ordered. */
+ * fewer candidates.  S is compared in 64 bits (of a beam's unequal logits that make the same S any may come first).
+ * beams, take <= 64, beams * vocab < 2^31, n * beams <= 2^24 (QKV_ERR_UNSUPPORTED).  workspace:
+ * qkv_beam_select_workspace_bytes of these numbers or larger ones, aligned to 8 bytes (no initialisation needed).
+ * Calls sharing one must be ordered. */
 size_t qkv_beam_select_workspace_bytes(int n, int beams, int vocab, int take);
 int qkv_beam_select(const void* logits, int logits_type, long stride, const float* scores, const int32_t* done,
                     int end_token, int n, int beams, int vocab, int take, int32_t* parents, int32_t* tokens,
