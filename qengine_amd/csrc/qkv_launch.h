@@ -258,7 +258,7 @@ struct WeighArgs {
   float* rec;                // workspace: {m, l} [rows of the launch][chunks], or of cut tiles (many rows)
   float* stat_m;             // workspace: m and 1 / l of the launch's rows
   float* stat_il;
-  float* scores;             // workspace: [rows of the launch][score_pitch] (few rows)
+  float* scores;             // workspace: [(slot, KV head) of the launch][score_pitch / 32][rows][32] (few rows)
   float* sums;               // workspace, the same place: of cut tiles (many rows)
   int groups;                // workgroups of the kernels for many rows
   int* cuts;                 // workspace: [kWeighGroups][4] where each part begins

@@ -908,7 +908,8 @@ def weigh_f8_paged(q, k_pool, k_exp, weights, workspace, block_tables, starts, p
                    decay=1.0, weighed=None, window=0, sink=0, stream=None) -> None:
     """Adds to weights (fp32 [n_pages][num_kv][block_tokens]) what the ragged query rows (as for attn_f8_paged) give each
     key: softmax weights summed over rows and the heads of a KV group, after decay times what stood for the first
-    weighed[s] keys of each slot (int32 [n_slots], None: positions) and from zero for the others."""
+    weighed[s] keys of each slot (int32 [n_slots], None: positions) and from zero for the others.  Of slots that share a page
+    only one may have rows in a call."""
     dev = _run_device(stream, k_pool)
     n_pages, bt, kv, hd = k_pool.shape
     if k_exp.shape != (n_pages, kv):
