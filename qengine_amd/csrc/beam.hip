@@ -5,9 +5,10 @@
 // The logits are read once: a workgroup takes a segment of one row, holds it in registers, sums its
 // exponentials and keeps its `take` largest logits; a second launch joins a request's segments.  Inside a
 // row the order of S is that of x, so segments compare the logits themselves, without a rounding.
-// 512 rows of 131,072 fp16 logits take 31 + 12 us (21 at 6.4 TB/s); the vector unit bounds the first launch, busy
-// 0.8 of its time: 6 instructions a logit for its exponential, 1 for the maximum, and the selection's threshold,
-// maxima of the lanes in turn, a fifth.  Eight workgroups are on a CU, so that others load while one selects.
+// 512 rows of 131,072 fp16 logits take 31 + 11 us (21 at 6.4 TB/s), bf16 32 + 11, fp32 46 + 12 (42); the vector unit bounds the
+// first launch of fp16, busy 0.71 of its time: 6 instructions a logit for its exponential, 1 for the maximum, and the
+// selection's threshold, maxima of the lanes in turn, a fifth.  Eight workgroups are on a CU (five of bf16, by its registers),
+// so that others load while one selects.
 //
 // The exponentials are taken in base 2 of the distance to the segment's maximum (exact for 16-bit logits),
 // times log2(e) as two floats: their error stays near their own rounding, where a product of the logit and one

@@ -155,7 +155,9 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeArgs p) {
   }
 }
 
-// Any even rot, head size, stride and alignment: a wave per row, which it reads twice.
+// Any even rot, head size, stride and alignment: a wave per row, which it reads twice, 2 bytes a lane, and for which it forms
+// the angles again.  Bound by its instructions: 32,768 tokens of 36 heads of 96 take 353 us, of 192 with 64 turned 640 (94 and
+// 189 at the copy's rate).
 __global__ __launch_bounds__(256) void norm_rope_any_kernel(NormRopeArgs p) {
   const long row = (long)(blockIdx.y * kGridX + blockIdx.x) * 4 + (threadIdx.x >> 6);
   const int lane = threadIdx.x & 63, heads = p.num_q + p.num_k;
@@ -262,7 +264,8 @@ __global__ __launch_bounds__(256, 3) void norm_rope_grad_kernel(NormRopeArgs p) 
   }
 }
 
-// Any size and alignment: a wave per row, its part of dw in LDS (each element one lane's).
+// Any size and alignment: a wave per row, its part of dw in LDS (each element one lane's).  8,192 tokens of 20 heads of 96 take
+// 137 us, of 192 308 (20 and 39 at the copy's rate).
 __global__ __launch_bounds__(256) void norm_rope_grad_any_kernel(NormRopeArgs p) {
   __shared__ float part[4][kNormMaxHead];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hd = p.head_dim;
