@@ -52,11 +52,14 @@ def test_norm_refusals(L, p):
     _each(f, NULL, q=[None], qo=[None], k=[None], ko=[None], pos=[None], t=[None])
     _each(f, ALIGN, qw=[p + 2], kw=[p + 1], pos=[p + 2], t=[p + 4])
     assert f(q=p + 1, qo=p + 1) == ALIGN
-    # 2^34 rows and 2,048 more of the kernel for any size
-    most = dict(n=8388609, nq=1024, nk=1024, hd=2, rot=2, qs=2048, qos=2048, ks=2048, kos=2048)
-    assert f(**most) == UNSUPPORTED
     # a side without heads is not looked at, nor are a rotation's tables without one
     assert f(n=0, nq=0, q=None, qo=None) == f(n=0, rot=0, pos=None, t=None) == OK
+
+
+def test_norm_refuses_more_rows_than_workgroups_are_counted(L, p):
+    """2^34 rows and 2,048 more, of a size that takes a wave a row."""
+    assert L.qkv_norm_rope(p, 2048, p, 2048, None, p + 64, 2048, p + 64, 2048, None, 1e-6, p, p, 1.0, 8388609, 1024, 1024, 2, 2,
+                           0, None) == UNSUPPORTED
 
 
 def test_norm_gradient_refusals(L, p):
